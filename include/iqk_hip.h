@@ -36,11 +36,23 @@
 extern "C" {
 #endif
 
-#define IQK_HIP_ABI_VERSION 6
+#define IQK_HIP_ABI_VERSION 7
 
 #define IQK_MEMBER_IQ2_KS 0
 #define IQK_MEMBER_IQ2_K 1
 #define IQK_MEMBER_IQ1_S_R4 2
+
+// Element types of the entry points that take several.
+#define IQK_F32 0
+#define IQK_F16 1
+#define IQK_BF16 2
+
+// Activations of the 4-bit weights' products, and their outputs' type: fp16 or
+// bf16 rows, or 4-bit microscaled rows with fp16 or bf16 outputs.
+#define IQK_ACT_F16 0
+#define IQK_ACT_BF16 1
+#define IQK_ACT_MX_F16 2
+#define IQK_ACT_MX_BF16 3
 
 #define IQK_OK 0
 #define IQK_ERR_MEMBER 1
@@ -256,6 +268,97 @@ int iqk_prefill(int member, int64_t in_features, int64_t out_features, int64_t n
 // of 4 (its four-row groups).
 int iqk_pack(int member, int64_t in_features, int64_t rows, const void *wire,
              void *const *streams, int n_streams, void *stream);
+
+// -- 4-bit microscaled weights and activations, the router -------------------
+//
+// No counterparts in the reference, whose experts are IQ_K members only and
+// whose indices its caller brings (src/mlx_iqk/nn.py:221-238).
+//
+// The format: 32 consecutive values share a scale byte s, 2^(s - 127) (255: the
+// block is NaN), and hold four bits each: bit 3 the sign, bits 0-2 an index into
+// {0, 1/2, 1, 3/2, 2, 3, 4, 6}.  A byte holds two, the even column's in its low
+// half.  codes: u8 [rows, cols / 2] contiguous; scales: u8, scale_stride bytes
+// from row to row, cols / 32 of them used.
+
+// Quantise rows (dtype IQK_F32 / F16 / BF16; row_stride elements apart, 16-byte
+// aligned): the block's scale is 2^(floor(log2 of its largest magnitude) - 2),
+// at least 2^-127; values round to nearest, ties to the even code, to at most 6
+// scales.  A block with a NaN or an infinity gets the NaN scale and codes 0.
+// cols % 32 == 0.
+int iqk_mx_quantize(int dtype, const void *x, int64_t rows, int64_t cols, int64_t row_stride, uint8_t *codes,
+                    uint8_t *scales, int64_t scale_stride, void *stream);
+
+// The values codes and scales stand for, rounded once to dtype: y [rows, cols].
+int iqk_mx_dequantize(int dtype, const uint8_t *codes, const uint8_t *scales, int64_t rows, int64_t cols,
+                      int64_t scale_stride, void *y, void *stream);
+
+// Lay an expert stack's codes and scales (rows = num_experts * out_features)
+// out for the products, with R = out_features up to a multiple of 16 and S =
+// in_features / 128 rounded up:
+//   tiles u8 [E][R / 16][S][64][16], tile_scales u32 [E][S][R], row_exps i32 [E][R].
+// A block more than 2^140 below its row's largest is taken as zero.
+int iqk_mx_pack(int64_t in_features, int64_t out_features, int64_t num_experts, const uint8_t *codes,
+                const uint8_t *scales, int64_t scale_stride, void *tiles, uint32_t *tile_scales, int32_t *row_exps,
+                void *stream);
+
+// The laid-out weights' values, rounded once to dtype: y [E, out_features, in_features].
+int iqk_mx_unpack(int dtype, int64_t in_features, int64_t out_features, int64_t num_experts, const void *tiles,
+                  const uint32_t *tile_scales, const int32_t *row_exps, void *y, void *stream);
+
+// Products of token-expert pairs, each on its own (few pairs):
+//   y[p, r] = sum_k W[ids[p]][r][k] * x[p / pairs_per_x_row][k],
+// exact products, f32 sums, one rounding.  act names x's type: 16-bit rows
+// [n_x_rows, in_features], or 4-bit codes [n_x_rows, in_features / 2] with
+// x_scales (4-byte aligned, x_scale_stride a multiple of 4 and at least 4 S).
+// ids: u32 or (wide_ids) i64 [n_pairs], or NULL: all expert 0 of one.  An id
+// outside [0, num_experts) gives a NaN row.  y: [n_pairs, out_features].
+// With IQK_ACT_F16, weights below 2^-36 of their row's largest scale are rounded
+// to multiples of 2^-37 of it.  num_experts <= 4096, in_features % 32 == 0.
+int iqk_mx_pairs(int act, int64_t in_features, int64_t out_features, int64_t num_experts, const void *x,
+                 int64_t n_x_rows, const uint8_t *x_scales, int64_t x_scale_stride, const void *tiles,
+                 const uint32_t *tile_scales, const int32_t *row_exps, const void *ids, int wide_ids,
+                 int64_t pairs_per_x_row, int64_t n_pairs, void *y, void *stream);
+
+// The same for slots sorted by expert (iqk_route's lists; x_rows, y_rows and
+// out-of-range entries as iqk_fused_gemm):
+//   y[y_rows[s], r] = sum_k W[e][r][k] * x[x_rows[s]][k], s in expert e's slots.
+// group_offsets NULL: one expert with every slot; x_rows, y_rows NULL: the slots'.
+int iqk_mx_groups(int act, int64_t in_features, int64_t out_features, int64_t num_experts, const void *x,
+                  int64_t n_x_rows, const uint8_t *x_scales, int64_t x_scale_stride, const void *tiles,
+                  const uint32_t *tile_scales, const int32_t *row_exps, const uint32_t *group_offsets,
+                  const uint32_t *x_rows, const uint32_t *y_rows, int64_t n_slots, void *y, void *stream);
+
+// The router's choice: ids[t] the k highest logits of row t in falling order,
+// ties to the lowest expert, NaN above all; weights[t] their softmax, taken over
+// the chosen (normalize) or over the whole row.  A row of -inf gives weights 0.
+// logits: dtype [rows, experts]; weights f32, ids i32 [rows, k].  experts <= 1024,
+// k <= 64.
+int iqk_router_topk(int dtype, const void *logits, int64_t rows, int64_t experts, int64_t k, int normalize,
+                    float *weights, int32_t *ids, void *stream);
+
+// Its gradient, from the outputs and d loss / d weights: dlogits dtype [rows,
+// experts].  logits may be NULL with normalize.
+int iqk_router_topk_grad(int dtype, const void *logits, const float *weights, const int32_t *ids,
+                         const float *dweights, int64_t rows, int64_t experts, int64_t k, int normalize, void *dlogits,
+                         void *stream);
+
+// The balance loss of each group of tokens: over its n kept tokens (mask u8
+// [groups, tokens], NULL: all), with c_e the pairs that name expert e and S_e
+// the sum of its softmax probabilities,
+//   loss[g] = experts / (k n^2) * sum_e c_e S_e      (0 where n is 0).
+// Ids outside [0, experts) count for none.  logits dtype [groups, tokens,
+// experts]; ids i32 [groups, tokens, k]; counts i32 [groups, experts]; kept i32
+// [groups]; work: iqk_balance_work words.  The same inputs give the same bits.
+int64_t iqk_balance_work(int64_t groups, int64_t tokens, int64_t experts);
+int iqk_balance(int dtype, const void *logits, const int32_t *ids, const uint8_t *mask, int64_t groups,
+                int64_t tokens, int64_t experts, int64_t k, uint32_t *work, float *loss, int32_t *counts,
+                int32_t *kept, void *stream);
+
+// Its gradient: dlogits dtype [groups, tokens, experts] from dloss f32 [groups],
+//   dloss experts / (k n^2) p_e (c_e - sum_j c_j p_j), 0 for tokens left out.
+int iqk_balance_grad(int dtype, const void *logits, const uint8_t *mask, const int32_t *counts, const int32_t *kept,
+                     const float *dloss, int64_t groups, int64_t tokens, int64_t experts, int64_t k, void *dlogits,
+                     void *stream);
 
 #ifdef __cplusplus
 }

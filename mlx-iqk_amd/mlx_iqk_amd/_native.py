@@ -13,7 +13,7 @@ from pathlib import Path
 from . import build
 from .build import HIP_LIB, LAUNCH_EXT
 
-ABI_VERSION = 6
+ABI_VERSION = 7
 
 OK, ERR_MEMBER, ERR_GEOMETRY, ERR_ARGUMENT, ERR_LAUNCH = 0, 1, 2, 3, 4
 _CODES = {ERR_MEMBER: "unknown member", ERR_GEOMETRY: "unsized geometry",
@@ -63,6 +63,23 @@ SIGNATURES = {
     "iqk_prefill": (c_int, [c_int, c_int64, c_int64, c_int64, c_void_p, c_int64, ctypes.POINTER(c_void_p), c_int,
                             c_int64, c_int64, c_void_p, c_int, c_int64, c_int64, c_int64, c_void_p, c_void_p,
                             c_void_p]),
+    "iqk_mx_quantize": (c_int, [c_int, c_void_p, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_int64, c_void_p]),
+    "iqk_mx_dequantize": (c_int, [c_int, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_void_p, c_void_p]),
+    "iqk_mx_pack": (c_int, [c_int64, c_int64, c_int64, c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_void_p,
+                            c_void_p]),
+    "iqk_mx_unpack": (c_int, [c_int, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
+    "iqk_mx_pairs": (c_int, [c_int, c_int64, c_int64, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p,
+                             c_void_p, c_void_p, c_void_p, c_int, c_int64, c_int64, c_void_p, c_void_p]),
+    "iqk_mx_groups": (c_int, [c_int, c_int64, c_int64, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p,
+                              c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_void_p]),
+    "iqk_router_topk": (c_int, [c_int, c_void_p, c_int64, c_int64, c_int64, c_int, c_void_p, c_void_p, c_void_p]),
+    "iqk_router_topk_grad": (c_int, [c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int,
+                                     c_void_p, c_void_p]),
+    "iqk_balance_work": (c_int64, [c_int64, c_int64, c_int64]),
+    "iqk_balance": (c_int, [c_int, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int64, c_void_p,
+                            c_void_p, c_void_p, c_void_p, c_void_p]),
+    "iqk_balance_grad": (c_int, [c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64,
+                                 c_int64, c_void_p, c_void_p]),
 }
 
 

@@ -41,6 +41,9 @@ HIP_SOURCES = {
     "iqk_pack.hip": (),
     "iqk_floor.hip": (),
     "iqk_route.hip": (),
+    "iqk_mx.hip": (),
+    "iqk_mx_gemm.hip": (),
+    "iqk_router.hip": (),
 }
 OFFLOAD_ARCH = "gfx950"
 

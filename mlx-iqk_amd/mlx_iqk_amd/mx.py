@@ -1,0 +1,374 @@
+"""4-bit microscaled floats: quantisation, and projections whose weights are in them.
+
+The format (the OCP microscaling MXFP4): 32 consecutive values along the last
+axis share a scale ``2**(byte - 127)`` (byte 255: the block is NaN) and hold four
+bits each, a sign and an index into 0, 0.5, 1, 1.5, 2, 3, 4, 6; 4.25 bits a
+value.  A byte holds two codes, the even position's in its low half.
+
+* :func:`quantize` / :func:`dequantize` convert tensors on the GPU;
+* :class:`MxSwitchLinear` is the routed projection of
+  :class:`~mlx_iqk_amd.nn.IqkSwitchLinear` over experts in this format: the same
+  ``(x, indices, sorted_indices)`` call, shapes and treatment of ids out of range;
+* :class:`MxLinear` is one such matrix.
+
+Both projections take 16-bit activations, whose products with the weights are
+exact and summed in f32, or an :class:`MxTensor`, quantised activations, which the
+matrix cores multiply with the weights as they are, at four times the rate.
+Outputs are rounded once.  The weights are frozen: no gradient flows through.
+
+Like every launch of this package, these run asynchronously on torch's current
+stream, and raise where no GPU library is built; nothing falls back to the CPU.
+"""
+
+from __future__ import annotations
+
+import math
+
+import torch
+
+from . import _native
+from .kernels import ROUTE_MAX_EXPERTS, IqkKernelError, _require_cuda, _stream_ptr, route_ids
+from .nn import _KERNEL_IDS, IqkRuntimeError, _pairs_per_x_row
+
+BLOCK = 32
+"""Values that share a scale."""
+_STEP = 128
+_DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+_ACTS = {(torch.float16, False): 0, (torch.bfloat16, False): 1, (torch.float16, True): 2, (torch.bfloat16, True): 3}
+
+PAIR_LIMIT = 63
+"""Token-expert pairs up to which each pair is computed on its own."""
+
+
+def _check_width(n: int) -> int:
+    if n <= 0 or n % BLOCK:
+        raise IqkKernelError(f"a row of {n} values is not whole blocks of {BLOCK}")
+    return n
+
+
+class MxTensor:
+    """Codes ``u8 [..., n/2]`` and scales ``u8 [..., n/32]`` of a tensor ``[..., n]``.
+
+    ``dtype`` is the type of the tensor that was quantised: what
+    :meth:`dequantize` returns, and a projection of these values.
+    """
+
+    __slots__ = ("codes", "scales", "dtype")
+
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor, dtype: torch.dtype = torch.float16):
+        for name, t in (("codes", codes), ("scales", scales)):
+            if not isinstance(t, torch.Tensor) or t.dtype != torch.uint8 or t.dim() < 1:
+                raise IqkKernelError(f"{name} must be a uint8 tensor of at least one dimension")
+        if dtype not in _DTYPES:
+            raise IqkKernelError(f"dtype must be one of {tuple(_DTYPES)}, got {dtype}")
+        if codes.device != scales.device:
+            raise IqkKernelError(f"codes are on {codes.device}, scales on {scales.device}")
+        if codes.shape[:-1] != scales.shape[:-1] or codes.shape[-1] != scales.shape[-1] * (BLOCK // 2) \
+                or not scales.shape[-1]:
+            raise IqkKernelError(f"codes {tuple(codes.shape)} and scales {tuple(scales.shape)} do not describe blocks "
+                                 f"of {BLOCK} values (16 bytes and one scale each)")
+        self.codes, self.scales, self.dtype = codes, scales, dtype
+
+    @property
+    def shape(self) -> torch.Size:
+        return torch.Size((*self.codes.shape[:-1], 2 * self.codes.shape[-1]))
+
+    @property
+    def device(self) -> torch.device:
+        return self.codes.device
+
+    def dequantize(self, dtype: torch.dtype | None = None) -> torch.Tensor:
+        """The values the codes stand for (:func:`dequantize`)."""
+        return dequantize(self, dtype)
+
+    def __repr__(self) -> str:
+        return f"MxTensor({tuple(self.shape)}, {self.dtype}, {self.device})"
+
+
+def _new_scales(lead: tuple, n: int, device) -> tuple[torch.Tensor, int]:
+    """Room for the scales of rows of n values, and the bytes from row to row: a
+    multiple of four, as the products read activations' scales."""
+    stride = 4 * ((n + _STEP - 1) // _STEP)
+    room = torch.empty((*lead, stride), dtype=torch.uint8, device=device)
+    return room[..., :n // BLOCK] if stride != n // BLOCK else room, stride
+
+
+def _row_stride(t: torch.Tensor) -> int | None:
+    """Elements from row to row of t taken as [rows, n], the last axis dense;
+    None where rows are not evenly spaced."""
+    if t.stride(-1) != 1 and t.shape[-1] > 1:
+        return None
+    stride = span = None
+    for size, step in zip(reversed(t.shape[:-1]), reversed(t.stride()[:-1])):
+        if size == 1:
+            continue
+        if span is None:
+            stride, span = step, size * step
+        elif step == span:
+            span = size * step
+        else:
+            return None
+    return t.shape[-1] if stride is None else stride
+
+
+def _aligned_codes(q: MxTensor) -> torch.Tensor:
+    """Contiguous codes at a 16-byte boundary."""
+    codes = q.codes.contiguous()
+    return codes if codes.data_ptr() % 16 == 0 else codes.clone()
+
+
+def _product_scales(q: MxTensor) -> tuple[torch.Tensor, int]:
+    """Scales as the products read an activation row's, four at a time: rows at
+    multiples of four bytes with room for whole groups of four."""
+    n, rows = q.scales.shape[-1], math.prod(q.scales.shape[:-1])
+    need = 4 * ((n + 3) // 4)
+    stride = _row_stride(q.scales)
+    if rows == 1 and stride is not None:
+        stride = max(stride, need) // 4 * 4
+    if stride is not None and stride % 4 == 0 and stride >= need and q.scales.data_ptr() % 4 == 0:
+        left = q.scales.untyped_storage().nbytes() - q.scales.storage_offset()
+        if (rows - 1) * stride + need <= left:
+            return q.scales, stride
+    room = torch.empty((rows, need), dtype=torch.uint8, device=q.scales.device)
+    room[:, :n] = q.scales.reshape(rows, n)
+    return room, need
+
+
+def quantize(x: torch.Tensor) -> MxTensor:
+    """``x`` (f32, f16 or bf16 ``[..., n]`` on a GPU, ``n`` a multiple of 32) in 4 bits.
+
+    A block's scale is ``2**(floor(log2(largest magnitude)) - 2)``, at least
+    2**-127; values round to nearest, ties to the even code, and saturate at 6
+    scales.  A block that holds a NaN or an infinity becomes NaN.
+    """
+    if not isinstance(x, torch.Tensor) or x.dim() < 1:
+        raise IqkKernelError("x must be a tensor of at least one dimension")
+    if x.device.type != "cuda":
+        raise IqkKernelError(f"x must live on a GPU, got {x.device}")
+    if x.dtype not in _DTYPES:
+        raise IqkKernelError(f"x must be one of {tuple(_DTYPES)}, got {x.dtype}")
+    n, lead = _check_width(x.shape[-1]), tuple(x.shape[:-1])
+    rows = math.prod(lead)
+    x = x.detach()
+    per16 = 16 // x.element_size()
+    stride = _row_stride(x)
+    if stride is None or stride < n and rows > 1 or stride % per16 or x.data_ptr() % 16:
+        x, stride = x.contiguous(), n
+        if x.data_ptr() % 16:
+            x = x.clone()
+    codes = torch.empty((*lead, n // 2), dtype=torch.uint8, device=x.device)
+    scales, scale_stride = _new_scales(lead, n, x.device)
+    if rows:
+        rc = _native.load().iqk_mx_quantize(_DTYPES[x.dtype], x.data_ptr(), rows, n, stride, codes.data_ptr(),
+                                            scales.data_ptr(), scale_stride, _stream_ptr(x.device))
+        _native.check(rc, f"iqk_mx_quantize({rows}x{n})")
+    return MxTensor(codes, scales, x.dtype)
+
+
+def dequantize(q: MxTensor, dtype: torch.dtype | None = None) -> torch.Tensor:
+    """The values of ``q``, rounded once to ``dtype`` (its own by default; a
+    value is exact in f32 and, but for the smallest scales, in bf16)."""
+    dtype = q.dtype if dtype is None else dtype
+    if dtype not in _DTYPES:
+        raise IqkKernelError(f"dtype must be one of {tuple(_DTYPES)}, got {dtype}")
+    if q.device.type != "cuda":
+        raise IqkKernelError(f"codes must live on a GPU, got {q.device}")
+    n, rows = q.shape[-1], math.prod(q.shape[:-1])
+    codes, scales, stride = _aligned_codes(q), q.scales, _row_stride(q.scales)
+    if stride is None or stride < n // BLOCK:
+        scales, stride = scales.contiguous(), n // BLOCK
+    y = torch.empty(q.shape, dtype=dtype, device=q.device)
+    if rows:
+        rc = _native.load().iqk_mx_dequantize(_DTYPES[dtype], codes.data_ptr(), scales.data_ptr(), rows, n, stride,
+                                              y.data_ptr(), _stream_ptr(q.device))
+        _native.check(rc, f"iqk_mx_dequantize({rows}x{n})")
+    return y
+
+
+class _MxStack(torch.nn.Module):
+    """``num_experts`` matrices ``[out, in]`` in the products' layout, as buffers:
+
+    * ``tiles`` u8 ``[E, out/16, in/128, 64, 16]``, the codes in the order that a
+      wavefront loads them;
+    * ``tile_scales`` i32 ``[E, in/128, out]``, the scales of four blocks a word,
+      relative to their row's;
+    * ``row_exps`` i32 ``[E, out]``, each row's power of two.
+
+    ``out`` and ``in`` round up to whole tiles; 4.27 bits a weight.
+    """
+
+    def __init__(self, num_experts: int, out_features: int, in_features: int, device=None):
+        super().__init__()
+        self.num_experts, self.out_features = int(num_experts), int(out_features)
+        self.in_features = _check_width(int(in_features))
+        if not 0 < self.num_experts <= ROUTE_MAX_EXPERTS:
+            raise IqkRuntimeError(f"a stack holds 1 .. {ROUTE_MAX_EXPERTS} experts (num_experts={num_experts})")
+        if self.out_features <= 0:
+            raise IqkRuntimeError(f"out_features must be positive, got {out_features}")
+        rows, steps = (self.out_features + 15) // 16 * 16, (self.in_features + _STEP - 1) // _STEP
+        E = self.num_experts
+        self.register_buffer("tiles", torch.zeros((E, rows // 16, steps, 64, 16), dtype=torch.uint8, device=device))
+        self.register_buffer("tile_scales", torch.zeros((E, steps, rows), dtype=torch.int32, device=device))
+        self.register_buffer("row_exps", torch.zeros((E, rows), dtype=torch.int32, device=device))
+
+    def _load(self, codes: torch.Tensor, scales: torch.Tensor) -> None:
+        device = self.tiles.device
+        if device.type != "cuda":
+            raise IqkKernelError(f"the module must live on a GPU to load weights, got {device}")
+        q = MxTensor(codes.to(device), scales.to(device))
+        codes, scales, stride = _aligned_codes(q), q.scales, _row_stride(q.scales)
+        if stride is None or stride < self.in_features // BLOCK:
+            scales, stride = scales.contiguous(), self.in_features // BLOCK
+        rc = _native.load().iqk_mx_pack(self.in_features, self.out_features, self.num_experts, codes.data_ptr(),
+                                        scales.data_ptr(), stride, self.tiles.data_ptr(), self.tile_scales.data_ptr(),
+                                        self.row_exps.data_ptr(), _stream_ptr(device))
+        _native.check(rc, f"iqk_mx_pack({self.num_experts}x{self.out_features}x{self.in_features})")
+
+    def _dequantized(self, dtype: torch.dtype) -> torch.Tensor:
+        if dtype not in _DTYPES:
+            raise IqkKernelError(f"dtype must be one of {tuple(_DTYPES)}, got {dtype}")
+        _require_cuda(self.tiles, "the module", torch.uint8)
+        y = torch.empty((self.num_experts, self.out_features, self.in_features), dtype=dtype, device=self.tiles.device)
+        rc = _native.load().iqk_mx_unpack(_DTYPES[dtype], self.in_features, self.out_features, self.num_experts,
+                                          self.tiles.data_ptr(), self.tile_scales.data_ptr(), self.row_exps.data_ptr(),
+                                          y.data_ptr(), _stream_ptr(y.device))
+        _native.check(rc, f"iqk_mx_unpack({self.num_experts}x{self.out_features}x{self.in_features})")
+        return y
+
+    def _activations(self, x) -> tuple:
+        """x's rows as the kernels take them: (act, rows, scales, scale stride, dtype)."""
+        mx = isinstance(x, MxTensor)
+        device = self.tiles.device
+        if not mx and not isinstance(x, torch.Tensor):
+            raise IqkKernelError("x must be a tensor or an MxTensor")
+        if x.device != device or device.type != "cuda":
+            raise IqkKernelError(f"x is on {x.device}, the module on {device}; both must be on one GPU")
+        act = _ACTS.get((x.dtype, mx))
+        if act is None:
+            raise IqkKernelError(f"activations are float16 or bfloat16, or quantised from them; got {x.dtype}")
+        if x.shape[-1] != self.in_features:
+            raise IqkRuntimeError(f"x has rows of {x.shape[-1]} values, the weights take {self.in_features}")
+        if mx:
+            scales, stride = _product_scales(x)
+            return act, _aligned_codes(x), scales, stride, x.dtype
+        if x.requires_grad and torch.is_grad_enabled():
+            raise IqkRuntimeError("the weights are frozen and no gradient flows through them: detach x, or call "
+                                  "under torch.no_grad()")
+        rows = x.detach().contiguous()
+        return act, rows if rows.data_ptr() % 16 == 0 else rows.clone(), None, 0, x.dtype
+
+    def _launch(self, entry: str, act, rows, scales, stride, n_x_rows, *args) -> None:
+        rc = getattr(_native.load(), entry)(
+            act, self.in_features, self.out_features, self.num_experts, rows.data_ptr(), n_x_rows,
+            None if scales is None else scales.data_ptr(), stride, self.tiles.data_ptr(),
+            self.tile_scales.data_ptr(), self.row_exps.data_ptr(), *args, _stream_ptr(rows.device))
+        if rc:
+            _native.check(rc, f"{entry}({self.num_experts}x{self.out_features}x{self.in_features})")
+
+    def extra_repr(self) -> str:
+        return f"{self.num_experts}, {self.out_features}, {self.in_features}"
+
+
+class MxSwitchLinear(_MxStack):
+    """One routed projection: ``num_experts`` 4-bit ``[out, in]`` matrices, called
+    with ``(x, indices)`` as :class:`~mlx_iqk_amd.nn.IqkSwitchLinear` is: x
+    ``[..., M, in]`` whose leading shape broadcasts with indices ``[..., top_k]``,
+    outputs ``[..., top_k, M, out]`` in x's type.  An id outside the stack gives
+    rows of NaN."""
+
+    mode = "mx"
+
+    def load(self, weights: MxTensor) -> None:
+        """Take the codes and scales of ``weights`` ``[num_experts, out, in]``."""
+        want = (self.num_experts, self.out_features, self.in_features)
+        if not isinstance(weights, MxTensor) or tuple(weights.shape) != want:
+            raise IqkRuntimeError(f"weights must be an MxTensor {want}, got "
+                                  f"{tuple(weights.shape) if hasattr(weights, 'shape') else type(weights).__name__}")
+        self._load(weights.codes, weights.scales)
+
+    def dequantized(self, dtype: torch.dtype = torch.float16) -> torch.Tensor:
+        """The weights' values ``[num_experts, out, in]``, rounded once to ``dtype``."""
+        return self._dequantized(dtype)
+
+    def forward(self, x, indices: torch.Tensor, sorted_indices: bool = False) -> torch.Tensor:
+        """Project ``x`` through the experts named by ``indices``: up to
+        :data:`PAIR_LIMIT` pairs each on its own, else (or with
+        ``sorted_indices``) grouped by expert on the device."""
+        if len(x.shape) < 2:
+            raise IqkRuntimeError(f"x must be [..., M, {self.in_features}], got {tuple(x.shape)}")
+        act, rows, scales, stride, dtype = self._activations(x)
+        xbatch, M = tuple(x.shape[:-2]), int(x.shape[-2])
+        batch = torch.broadcast_shapes(xbatch, tuple(indices.shape))
+        pairs = math.prod(batch)
+        y = torch.empty((*batch, M, self.out_features), dtype=dtype, device=rows.device)
+        if y.numel() == 0:
+            return y
+        per_row = _pairs_per_x_row(xbatch, batch)
+        if per_row is None:  # x broadcasts over leading dimensions: a row of its own for each pair
+            rows = rows.expand(*batch, M, rows.shape[-1]).contiguous()
+            if scales is not None:
+                n = self.in_features // BLOCK
+                scales, stride = _product_scales(MxTensor(rows, x.scales.expand(*batch, M, n).contiguous()))
+            per_row = 1
+        n_x_rows = rows.numel() // rows.shape[-1]
+        ids = self._ids(indices, batch)
+        wide = _KERNEL_IDS[ids.dtype]
+        if pairs <= PAIR_LIMIT and M == 1 and not sorted_indices:
+            self._launch("iqk_mx_pairs", act, rows, scales, stride, n_x_rows, ids.data_ptr(), wide, per_row, pairs,
+                         y.data_ptr())
+            return y
+        offsets, x_rows, y_rows = route_ids(ids, self.num_experts, M, per_row, n_x_rows)
+        self._launch("iqk_mx_groups", act, rows, scales, stride, n_x_rows, offsets.data_ptr(), x_rows.data_ptr(),
+                     y_rows.data_ptr(), pairs * M, y.data_ptr())
+        return y
+
+    def _ids(self, indices: torch.Tensor, batch) -> torch.Tensor:
+        """Expert ids of the pairs in order, of a type the kernels read.  Other
+        integers are clamped so that none wraps into the stack."""
+        if indices.is_floating_point() or indices.is_complex() or indices.dtype == torch.bool:
+            raise IqkKernelError(f"indices must be integers, got {indices.dtype}")
+        ids = indices if indices.device == self.tiles.device else indices.to(self.tiles.device)
+        if tuple(ids.shape) != tuple(batch):
+            ids = ids.broadcast_to(batch)
+        if ids.dtype not in _KERNEL_IDS:
+            ids = torch.clamp(ids.to(torch.int64), -1, self.num_experts)
+        return ids.reshape(-1).contiguous()
+
+
+class MxLinear(_MxStack):
+    """One 4-bit ``[out, in]`` matrix: x ``[..., in]`` to ``[..., out]`` in x's type."""
+
+    mode = "mx"
+
+    def __init__(self, out_features: int, in_features: int, device=None):
+        super().__init__(1, out_features, in_features, device)
+
+    def load(self, weights: MxTensor) -> None:
+        """Take the codes and scales of ``weights`` ``[out, in]``."""
+        want = (self.out_features, self.in_features)
+        if not isinstance(weights, MxTensor) or tuple(weights.shape) != want:
+            raise IqkRuntimeError(f"weights must be an MxTensor {want}, got "
+                                  f"{tuple(weights.shape) if hasattr(weights, 'shape') else type(weights).__name__}")
+        self._load(weights.codes, weights.scales)
+
+    def dequantized(self, dtype: torch.dtype = torch.float16) -> torch.Tensor:
+        """The weights' values ``[out, in]``, rounded once to ``dtype``."""
+        return self._dequantized(dtype)[0]
+
+    def forward(self, x) -> torch.Tensor:
+        act, rows, scales, stride, dtype = self._activations(x)
+        n = rows.numel() // rows.shape[-1]
+        y = torch.empty((*x.shape[:-1], self.out_features), dtype=dtype, device=rows.device)
+        if n == 0:
+            return y
+        if n <= 4:
+            self._launch("iqk_mx_pairs", act, rows, scales, stride, n, None, 0, 1, n, y.data_ptr())
+        else:
+            self._launch("iqk_mx_groups", act, rows, scales, stride, n, None, None, None, n, y.data_ptr())
+        return y
+
+    def extra_repr(self) -> str:
+        return f"{self.out_features}, {self.in_features}"
+
+
+__all__ = ["BLOCK", "PAIR_LIMIT", "MxLinear", "MxSwitchLinear", "MxTensor", "dequantize", "quantize"]

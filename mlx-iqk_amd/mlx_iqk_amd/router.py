@@ -1,0 +1,179 @@
+"""The router of a layer of experts: which experts a token goes to, with what
+weights, and the loss that keeps the experts evenly loaded; with gradients.
+
+:func:`topk`'s ids are the ``indices`` of the switch modules
+(:class:`~mlx_iqk_amd.nn.IqkSwitchLinear`, :class:`~mlx_iqk_amd.mx.MxSwitchLinear`),
+its weights scale their outputs.  Logits are f32, f16 or bf16 on a GPU, for up to
+1024 experts; sums, probabilities, weights and losses are f32.
+"""
+
+from __future__ import annotations
+
+import math
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _native
+from .kernels import IqkKernelError, _stream_ptr
+from .mx import _DTYPES
+
+MAX_EXPERTS = 1024
+MAX_K = 64
+
+
+def _check_logits(logits: torch.Tensor, dims: int) -> int:
+    if not isinstance(logits, torch.Tensor) or logits.dim() < dims:
+        raise IqkKernelError(f"logits must be a tensor of at least {dims} dimensions")
+    if logits.device.type != "cuda":
+        raise IqkKernelError(f"logits must live on a GPU, got {logits.device}")
+    if logits.dtype not in _DTYPES:
+        raise IqkKernelError(f"logits must be one of {tuple(_DTYPES)}, got {logits.dtype}")
+    experts = int(logits.shape[-1])
+    if not 0 < experts <= MAX_EXPERTS:
+        raise IqkKernelError(f"a router takes 1 .. {MAX_EXPERTS} experts, got {experts}")
+    return experts
+
+
+def _topk(logits: torch.Tensor, k: int, normalize: bool) -> tuple[torch.Tensor, torch.Tensor]:
+    shape, device = (*logits.shape[:-1], k), logits.device
+    weights = torch.empty(shape, dtype=torch.float32, device=device)
+    ids = torch.empty(shape, dtype=torch.int32, device=device)
+    rc = _native.load().iqk_router_topk(_DTYPES[logits.dtype], logits.data_ptr(), weights.numel() // k,
+                                        logits.shape[-1], k, normalize, weights.data_ptr(), ids.data_ptr(),
+                                        _stream_ptr(device))
+    if rc:
+        _native.check(rc, f"iqk_router_topk({tuple(logits.shape)}, {k})")
+    return weights, ids
+
+
+class _TopK(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, k, normalize):
+        weights, ids = _topk(logits, k, normalize)
+        ctx.mark_non_differentiable(ids)
+        ctx.set_materialize_grads(False)
+        ctx.normalize, ctx.dtype, ctx.shape = normalize, logits.dtype, logits.shape
+        ctx.save_for_backward(weights, ids, *(() if normalize else (logits,)))
+        return weights, ids
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dweights, _):
+        if dweights is None:
+            return None, None, None
+        weights, ids, *rest = ctx.saved_tensors
+        dweights = dweights.to(torch.float32).contiguous()
+        dlogits = torch.empty(ctx.shape, dtype=ctx.dtype, device=weights.device)
+        k = weights.shape[-1]
+        rc = _native.load().iqk_router_topk_grad(
+            _DTYPES[ctx.dtype], rest[0].data_ptr() if rest else None, weights.data_ptr(), ids.data_ptr(),
+            dweights.data_ptr(), weights.numel() // k, ctx.shape[-1], k, ctx.normalize, dlogits.data_ptr(),
+            _stream_ptr(weights.device))
+        if rc:
+            _native.check(rc, f"iqk_router_topk_grad({tuple(ctx.shape)}, {k})")
+        return dlogits, None, None
+
+
+def topk(logits: torch.Tensor, k: int, *, normalize: bool = True) -> tuple[torch.Tensor, torch.Tensor]:
+    """The ``k`` experts of each token: ``(weights f32 [..., k], ids i32 [..., k])``.
+
+    ``logits`` is ``[..., experts]``.  Ids are in falling order of their logits,
+    ties to the lowest expert, NaN above all.  Weights are the softmax over the
+    chosen (``normalize``), or over all experts.  Experts with -inf are
+    masked: weight 0, chosen only where fewer than ``k`` others are left; a
+    token with nothing else gets weights 0.  Differentiable in the logits.
+    """
+    experts = _check_logits(logits, 1)
+    k = int(k)
+    if not 0 < k <= min(MAX_K, experts):
+        raise IqkKernelError(f"k must be 1 .. {min(MAX_K, experts)} of {experts} experts, got {k}")
+    if not logits.is_contiguous():
+        logits = logits.contiguous()
+    if logits.requires_grad and torch.is_grad_enabled():
+        return _TopK.apply(logits, k, bool(normalize))
+    return _topk(logits, k, bool(normalize))
+
+
+def _balance(logits, ids, mask):
+    *lead, tokens, experts = logits.shape
+    groups, device = math.prod(lead), logits.device
+    lib = _native.load()
+    loss = torch.empty(lead, dtype=torch.float32, device=device)
+    counts = torch.empty((*lead, experts), dtype=torch.int32, device=device)
+    kept = torch.empty(lead, dtype=torch.int32, device=device)
+    if groups:
+        work = torch.empty(lib.iqk_balance_work(groups, tokens, experts), dtype=torch.int32, device=device)
+        rc = lib.iqk_balance(_DTYPES[logits.dtype], logits.data_ptr(), ids.data_ptr(),
+                             None if mask is None else mask.data_ptr(), groups, tokens, experts, ids.shape[-1],
+                             work.data_ptr(), loss.data_ptr(), counts.data_ptr(), kept.data_ptr(),
+                             _stream_ptr(device))
+        if rc:
+            _native.check(rc, f"iqk_balance({tuple(logits.shape)}, {ids.shape[-1]})")
+    return loss, counts, kept
+
+
+class _Balance(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, ids, mask):
+        loss, counts, kept = _balance(logits, ids, mask)
+        ctx.mark_non_differentiable(counts)
+        ctx.set_materialize_grads(False)
+        ctx.k = ids.shape[-1]
+        ctx.save_for_backward(logits, counts, kept, mask)
+        return loss, counts
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dloss, _):
+        if dloss is None:
+            return None, None, None
+        logits, counts, kept, mask = ctx.saved_tensors
+        dloss = dloss.to(torch.float32).contiguous()
+        dlogits = torch.empty_like(logits)
+        *lead, tokens, experts = logits.shape
+        rc = _native.load().iqk_balance_grad(
+            _DTYPES[logits.dtype], logits.data_ptr(), None if mask is None else mask.data_ptr(), counts.data_ptr(),
+            kept.data_ptr(), dloss.data_ptr(), math.prod(lead), tokens, experts, ctx.k, dlogits.data_ptr(),
+            _stream_ptr(logits.device))
+        if rc:
+            _native.check(rc, f"iqk_balance_grad({tuple(logits.shape)}, {ctx.k})")
+        return dlogits, None, None
+
+
+def balance_loss(logits: torch.Tensor, ids: torch.Tensor, *,
+                 mask: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """How unevenly tokens fall on experts: ``(loss f32 [...], counts i32 [..., experts])``.
+
+    ``logits`` is ``[..., tokens, experts]``, ``ids`` the chosen experts ``[..., tokens,
+    k]``; each leading index (a sequence, say) has a loss of its own.  With n
+    tokens, ``f_e = counts_e / (k n)`` the share of the pairs that name expert e
+    and ``P_e`` the mean of its softmax probability, ``loss = experts * sum_e f_e
+    P_e``: 1 where either is even, up to ``experts / k`` where the same k experts
+    take all.  Tokens whose ``mask`` (bool ``[..., tokens]``) is false are left out;
+    with none left the loss is 0.  Ids outside the stack count for none.
+    Differentiable in the logits (through ``P``; counts are constants).
+    """
+    experts = _check_logits(logits, 2)
+    if not isinstance(ids, torch.Tensor) or ids.is_floating_point() or ids.dtype == torch.bool:
+        raise IqkKernelError("ids must be an integer tensor")
+    if ids.device != logits.device or tuple(ids.shape[:-1]) != tuple(logits.shape[:-1]):
+        raise IqkKernelError(f"ids {tuple(ids.shape)} on {ids.device} do not belong to logits {tuple(logits.shape)} "
+                             f"on {logits.device}")
+    k = int(ids.shape[-1])
+    if not 0 < k <= min(MAX_K, experts):
+        raise IqkKernelError(f"a token has 1 .. {min(MAX_K, experts)} of {experts} experts, got {k}")
+    if mask is not None:
+        if mask.dtype != torch.bool or mask.device != logits.device or tuple(mask.shape) != tuple(logits.shape[:-1]):
+            raise IqkKernelError(f"mask must be bool {tuple(logits.shape[:-1])} on {logits.device}, got {mask.dtype} "
+                                 f"{tuple(mask.shape)} on {mask.device}")
+        mask = mask.contiguous()
+    if ids.dtype != torch.int32:
+        ids = torch.clamp(ids.to(torch.int64), -1, experts).to(torch.int32)
+    logits, ids = logits.contiguous(), ids.contiguous()
+    if logits.requires_grad and torch.is_grad_enabled():
+        return _Balance.apply(logits, ids, mask)
+    return _balance(logits, ids, mask)[:2]
+
+
+__all__ = ["MAX_EXPERTS", "MAX_K", "balance_loss", "topk"]

@@ -1,0 +1,318 @@
+"""The router's choice of experts and its balance loss, with their gradients,
+against plain 64-bit forms."""
+
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+
+import mxref
+from mlx_iqk_amd import router
+from mlx_iqk_amd.kernels import IqkKernelError
+
+pytestmark = pytest.mark.gpu
+F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
+DTYPES = (F32, F16, BF16)
+ULP = 2.0 ** -23
+FLOOR = 2.0 ** -126  # f32's smallest normal: exponentials below it flush
+
+
+def _f64(t: torch.Tensor) -> np.ndarray:
+    return t.detach().cpu().to(torch.float64).numpy()
+
+
+def _logits(rng, *shape, dtype, device) -> torch.Tensor:
+    return torch.from_numpy(rng.standard_normal(shape) * 2).to(dtype).to(device)
+
+
+def _rel(experts: int) -> float:
+    """Relative error of a probability: exponentials to 4 ulp, a sum of experts /
+    16 in a lane and 4 over lanes, a division."""
+    return (experts / 16 + 16) * ULP
+
+
+def _rounded(dtype) -> float:
+    return 0.0 if dtype == F32 else mxref.HALF_ULP[dtype]
+
+
+# experts at both sides of each register count, odd ones; k from one to all
+SHAPES = ((1, 1, 1), (1, 8, 8), (5, 60, 4), (33, 64, 6), (17, 65, 64), (100, 128, 17), (7, 161, 8), (64, 256, 6),
+          (3, 257, 33), (9, 512, 16), (2, 1023, 10), (4, 1024, 64), (1000, 160, 6))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("normalize", (True, False))
+@pytest.mark.parametrize("tokens,experts,k", SHAPES)
+def test_topk(device, dtype, normalize, tokens, experts, k):
+    print(f"topk {dtype} {normalize} {tokens} {experts} {k}", flush=True)
+    rng = np.random.default_rng(experts + k)
+    logits = _logits(rng, tokens, experts, dtype=dtype, device=device)
+    weights, ids = router.topk(logits, k, normalize=normalize)
+    want_w, want_ids = mxref.topk(_f64(logits), k, normalize)
+    assert weights.dtype == F32 and ids.dtype == torch.int32
+    np.testing.assert_array_equal(ids.cpu().numpy(), want_ids)
+    assert (np.abs(_f64(weights) - want_w) <= (_rel(experts) + k * ULP) * want_w + FLOOR).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("normalize", (True, False))
+@pytest.mark.parametrize("tokens,experts,k", SHAPES)
+def test_topk_gradient(device, dtype, normalize, tokens, experts, k):
+    print(f"topk gradient {dtype} {normalize} {tokens} {experts} {k}", flush=True)
+    rng = np.random.default_rng(experts + k + 1)
+    logits = _logits(rng, tokens, experts, dtype=dtype, device=device).requires_grad_()
+    dw = rng.standard_normal((tokens, k)).astype(np.float32)
+    weights, ids = router.topk(logits, k, normalize=normalize)
+    (got,) = torch.autograd.grad(weights, logits, torch.from_numpy(dw).to(device))
+    assert got.dtype == dtype and got.shape == logits.shape
+    x = _f64(logits)
+    want = mxref.topk_grad(x, k, normalize, dw.astype(np.float64))
+    w, at = mxref.topk(x, k, normalize)
+    # |w| (|dw| + sum |w dw|), each of them as exact as a probability
+    q = np.zeros_like(x)
+    np.put_along_axis(q, at, w, -1)
+    size = np.zeros_like(x)
+    np.put_along_axis(size, at, w * np.abs(dw), -1)
+    p = q if normalize else mxref.softmax(x)
+    size += p * (w * np.abs(dw)).sum(-1, keepdims=True)
+    bound = 3 * (_rel(experts) + k * ULP) * size + _rounded(dtype) * np.abs(want) + mxref.TINY[dtype] + 64 * FLOOR
+    assert (np.abs(_f64(got) - want) <= bound).all()
+
+
+@pytest.mark.parametrize("normalize", (True, False))
+def test_topk_gradient_against_differences(device, normalize):
+    """Central differences of the plain 64-bit weights along random directions
+    (logits far enough apart that no choice changes)."""
+    print(f"topk differences {normalize}", flush=True)
+    rng = np.random.default_rng(11)
+    x = (rng.permuted(np.tile(np.arange(24.0), (6, 1)), axis=1) * 0.25).astype(np.float32)
+    logits = torch.from_numpy(x).to(device).requires_grad_()
+    dw = rng.standard_normal((6, 5))
+    weights, _ = router.topk(logits, 5, normalize=normalize)
+    (got,) = torch.autograd.grad(weights, logits, torch.from_numpy(dw).to(device, F32))
+    step = 1e-5
+    for _ in range(4):
+        d = rng.standard_normal(x.shape)
+        hi, lo = (mxref.topk(x + s * step * d, 5, normalize)[0] for s in (1, -1))
+        slope = ((hi - lo) / (2 * step) * dw).sum()
+        # differences: step^2 and 1e-16 / step; the gradient: 24 x 6 terms to 1e-6
+        assert abs((_f64(got) * d).sum() - slope) <= 1e-6 * np.abs(_f64(got) * d).sum() + 1e-8 + 40 * 2e-6 * 1e-2
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_topk_ties_masks_and_bad_values(device, dtype):
+    print(f"topk ties {dtype}", flush=True)
+    inf, nan = float("inf"), float("nan")
+    rows = [[1.0] * 20, [0.0, -0.0] * 10, [-inf] * 20, [-inf] * 18 + [2.0, 3.0], [2.0, -inf, 2.0] + [-inf] * 17,
+            list(range(20)), [5.0, 5.0, 7.0, 7.0] * 5, [-60000.0] * 10 + [60000.0] * 10, [60000.0] + [-60000.0] * 19]
+    logits = torch.tensor(rows, dtype=torch.float64).to(dtype).to(device).requires_grad_()
+    for normalize in (True, False):
+        for k in (1, 3, 20):
+            weights, ids = router.topk(logits, k, normalize=normalize)
+            want_w, want_ids = mxref.topk(_f64(logits), k, normalize)
+            np.testing.assert_array_equal(ids.cpu().numpy(), want_ids)
+            assert (np.abs(_f64(weights) - want_w) <= (_rel(20) + k * ULP) * want_w + FLOOR).all()
+            (grad,) = torch.autograd.grad(weights, logits, torch.ones_like(weights))
+            assert bool(torch.isfinite(grad).all())
+            assert not bool(grad[2].any())  # nothing to choose from
+    bad = torch.tensor([[1.0, nan, 2.0, nan, inf], [1.0, inf, 2.0, 0.0, inf], [0.0, 1.0, 2.0, 3.0, 4.0]]).to(dtype)
+    weights, ids = router.topk(bad.to(device), 3)
+    assert ids.tolist() == [[1, 3, 4], [1, 4, 2], [4, 3, 2]]
+    assert bool(torch.isnan(weights[:2]).all()) and bool(torch.isfinite(weights[2]).all())
+
+
+def test_topk_shapes_and_strides(device):
+    print("topk shapes", flush=True)
+    base = torch.randn((6, 50, 80), device=device)
+    for logits in (base[0, 0], base[:, 0], base[:, ::3, 1:61], base.transpose(0, 2)[:, :, 0][:, :50].T.contiguous().T,
+                   base[:0], base.to(BF16)[..., 1:78]):
+        weights, ids = router.topk(logits, 3)
+        flat = logits.reshape(-1, logits.shape[-1])
+        want_w, want_ids = mxref.topk(_f64(flat), 3, True)
+        assert weights.shape == ids.shape == (*logits.shape[:-1], 3)
+        np.testing.assert_array_equal(ids.cpu().numpy().reshape(-1, 3), want_ids.reshape(-1, 3))
+    # gradients of strided logits and of a broadcast gradient
+    x = torch.randn((40, 30), device=device).requires_grad_()
+    weights, _ = router.topk(x.T, 4, normalize=False)
+    weights.sum().backward()
+    y = x.detach().T.contiguous().requires_grad_()
+    router.topk(y, 4, normalize=False)[0].sum().backward()
+    assert torch.equal(x.grad, y.grad.T)
+
+
+# ------------------------------------------------------------- balance loss ---
+
+BALANCE = ((1, 1, 1, 1), (1, 7, 60, 4), (1, 33, 64, 2), (2, 100, 65, 6), (3, 31, 128, 8), (1, 500, 161, 6),
+           (5, 64, 256, 6), (2, 70, 512, 3), (2, 40, 1023, 10), (1, 3000, 16, 2), (300, 5, 8, 2))
+
+
+def _balance_case(rng, groups, tokens, experts, k, dtype, device, masked):
+    logits = _logits(rng, groups, tokens, experts, dtype=dtype, device=device)
+    ids = np.stack([mxref.topk(x, k, True)[1] for x in _f64(logits)])
+    mask = rng.random((groups, tokens)) < 0.7 if masked else np.ones((groups, tokens), bool)
+    return logits, ids, mask
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("masked", (False, True))
+@pytest.mark.parametrize("groups,tokens,experts,k", BALANCE)
+def test_balance_loss_and_gradient(device, dtype, masked, groups, tokens, experts, k):
+    print(f"balance {dtype} {masked} {groups} {tokens} {experts} {k}", flush=True)
+    rng = np.random.default_rng(tokens + experts)
+    logits, ids, mask = _balance_case(rng, groups, tokens, experts, k, dtype, device, masked)
+    if masked and groups > 1:
+        mask[1] = False  # a sequence that is all padding
+    logits.requires_grad_()
+    loss, counts = router.balance_loss(logits, torch.from_numpy(ids).to(device, torch.int32),
+                                       mask=torch.from_numpy(mask).to(device) if masked else None)
+    dloss = rng.standard_normal(groups).astype(np.float32)
+    (got,) = torch.autograd.grad(loss, logits, torch.from_numpy(dloss).to(device))
+    assert loss.shape == (groups,) and counts.shape == (groups, experts) and got.dtype == dtype
+    # sums of positive terms: a lane's tokens, the wavefronts, the shares
+    steps = tokens / 32 + 8 + min(256, tokens / 32 + 1) + experts / 64 + 8
+    x = _f64(logits)
+    for g in range(groups):
+        want, want_counts = mxref.balance(x[g], ids[g], mask[g])
+        np.testing.assert_array_equal(counts[g].cpu().numpy(), want_counts)
+        assert abs(_f64(loss)[g] - want) <= (_rel(experts) + steps * ULP) * want
+        grad = dloss[g] * mxref.balance_grad(x[g], ids[g], mask[g])
+        n = max(int(mask[g].sum()), 1)
+        p = mxref.softmax(x[g]) * mask[g][:, None]
+        size = abs(dloss[g]) * experts / (k * n * n) * p * (want_counts + (p * want_counts).sum(-1, keepdims=True))
+        bound = 3 * _rel(experts) * size + _rounded(dtype) * np.abs(grad) + mxref.TINY[dtype] + 64 * FLOOR
+        assert (np.abs(_f64(got)[g] - grad) <= bound).all()
+
+
+def test_balance_gradient_against_differences(device):
+    print("balance differences", flush=True)
+    rng = np.random.default_rng(12)
+    logits, ids, mask = _balance_case(rng, 1, 40, 20, 3, F32, device, True)
+    flat = logits[0].clone().requires_grad_()
+    loss, _ = router.balance_loss(flat, torch.from_numpy(ids[0]).to(device), mask=torch.from_numpy(mask[0]).to(device))
+    assert loss.shape == ()
+    loss.backward()
+    x, step = _f64(flat), 1e-5
+    for _ in range(4):
+        d = rng.standard_normal(x.shape)
+        hi, lo = (mxref.balance(x + s * step * d, ids[0], mask[0])[0] for s in (1, -1))
+        terms = np.abs(_f64(flat.grad) * d).sum()
+        assert abs((_f64(flat.grad) * d).sum() - (hi - lo) / (2 * step)) <= 1e-5 * terms + 1e-8
+
+
+def test_balance_even_and_uneven_loads(device):
+    """1 where every expert gets its share, experts / k where k experts take all."""
+    print("balance loads", flush=True)
+    even = torch.zeros((64, 16), device=device)
+    ids = (torch.arange(64, device=device)[:, None] * 2 + torch.arange(2, device=device)) % 16
+    assert float(router.balance_loss(even, ids)[0]) == pytest.approx(1.0, rel=_rel(16) + 16 * ULP)
+    worst = torch.full((64, 16), -float("inf"), device=device)
+    worst[:, :2] = 3.0
+    loss, counts = router.balance_loss(worst, torch.tensor([[0, 1]], device=device).expand(64, 2))
+    assert float(loss) == pytest.approx(8.0, rel=_rel(16) + 16 * ULP)
+    assert counts.tolist() == [64, 64] + [0] * 14
+
+
+def test_balance_ids_outside_the_stack_and_empty_rows(device):
+    print("balance outside", flush=True)
+    rng = np.random.default_rng(13)
+    logits = _logits(rng, 30, 12, dtype=F32, device=device)
+    logits[4] = -float("inf")
+    logits.requires_grad_()
+    ids = rng.integers(0, 12, (30, 3))
+    ids[3], ids[9, 1], ids[10, 0] = (-1, 12, 2 ** 31), -2 ** 40, 2 ** 32 + 1
+    named = torch.from_numpy(ids).to(device)
+    loss, counts = router.balance_loss(logits, named)
+    (grad,) = torch.autograd.grad(loss, logits)
+    want, want_counts = mxref.balance(_f64(logits), ids, np.ones(30, bool))
+    np.testing.assert_array_equal(counts.cpu().numpy(), want_counts)
+    assert float(loss.detach()) == pytest.approx(want, rel=1e-5)
+    assert bool(torch.isfinite(grad).all()) and not bool(grad[4].any())
+    none = torch.zeros((30,), dtype=torch.bool, device=device)
+    loss, counts = router.balance_loss(logits, named, mask=none)
+    (grad,) = torch.autograd.grad(loss, logits)
+    assert float(loss.detach()) == 0.0 and not bool(counts.any()) and not bool(grad.any())
+    empty = torch.zeros((3, 0, 12), device=device)
+    loss, counts = router.balance_loss(empty, torch.zeros((3, 0, 2), dtype=torch.int32, device=device))
+    assert loss.tolist() == [0.0] * 3 and not bool(counts.any())
+    assert router.balance_loss(torch.zeros((0, 4, 12), device=device),
+                               torch.zeros((0, 4, 2), dtype=torch.int32, device=device))[0].shape == (0,)
+
+
+def test_masked_tokens_may_hold_anything(device):
+    print("masked tokens", flush=True)
+    rng = np.random.default_rng(14)
+    logits, ids, mask = _balance_case(rng, 1, 90, 40, 4, F32, device, True)
+    named, keep = torch.from_numpy(ids).to(device), torch.from_numpy(mask).to(device)
+    clean = logits.clone().requires_grad_()
+    want = router.balance_loss(clean, named, mask=keep)
+    spoiled = torch.where(keep[..., None], logits, torch.tensor(float("nan"), device=device)).requires_grad_()
+    got = router.balance_loss(spoiled, named, mask=keep)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    one = torch.ones(1, device=device)
+    a, b = torch.autograd.grad(want[0], clean, one)[0], torch.autograd.grad(got[0], spoiled, one)[0]
+    assert torch.equal(a, b)
+
+
+def test_repeats_and_streams(device):
+    """The same bits on every call and on another stream."""
+    print("repeats", flush=True)
+    rng = np.random.default_rng(15)
+    logits = _logits(rng, 2, 5000, 64, dtype=BF16, device=device).requires_grad_()
+    dw = torch.randn((2, 5000, 4), device=device)
+
+    def step():
+        weights, ids = router.topk(logits, 4)
+        loss, counts = router.balance_loss(logits, ids)
+        (grad,) = torch.autograd.grad((weights, loss), logits, (dw, torch.ones_like(loss)))
+        return weights, ids, loss, counts, grad
+
+    want = step()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    for _ in range(3):
+        with torch.cuda.stream(side):
+            got = step()
+        torch.cuda.synchronize()
+        assert all(torch.equal(g, w) for g, w in zip(got, want))
+
+
+def test_graph_replays(device):
+    """The forward passes from a captured graph, as a serving step holds them."""
+    print("router graph", flush=True)
+    logits = torch.randn((2, 5000, 64), device=device).to(BF16)
+
+    def step():
+        weights, ids = router.topk(logits, 4)
+        return weights, ids, *router.balance_loss(logits, ids)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step()
+    for _ in range(4):
+        logits.copy_(torch.randn(logits.shape, device=device))
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [h.clone() for h in held]
+        assert all(torch.equal(g, w) for g, w in zip(got, step()))
+
+
+def test_refusals(device):
+    print("router refusals", flush=True)
+    z = lambda *s, dtype=F32: torch.zeros(s, dtype=dtype, device=device)  # noqa: E731
+    for logits, k in ((torch.zeros(3, 8), 2), (z(3, 8), 0), (z(3, 8), 9), (z(3, 1025), 2), (z(3, 100), 65), (z(3, 0), 1),
+                      (z(3, 8, dtype=torch.float64), 2), (z(3, 8, dtype=torch.int32), 2), (None, 1)):
+        with pytest.raises(IqkKernelError):
+            router.topk(logits, k)
+    ids = z(3, 2, dtype=torch.int32)
+    for logits, named, mask in ((z(8), ids, None), (z(4, 8), ids, None), (z(3, 8), z(3, 2), None),
+                                (z(3, 8), ids.cpu(), None), (z(3, 8), z(3, 9, dtype=torch.int32), None),
+                                (z(3, 8), ids, z(3)), (z(3, 8), ids, z(4, dtype=torch.bool)),
+                                (z(3, 8), ids, torch.zeros(3, dtype=torch.bool)), (torch.zeros(3, 8), ids, None)):
+        with pytest.raises(IqkKernelError):
+            router.balance_loss(logits, named, mask=mask)
