@@ -293,17 +293,17 @@ int iqk_mx_dequantize(int dtype, const uint8_t *codes, const uint8_t *scales, in
                       int64_t scale_stride, void *y, void *stream);
 
 // Lay an expert stack's codes and scales (rows = num_experts * out_features)
-// out for the products, with R = out_features up to a multiple of 16 and S =
-// in_features / 128 rounded up:
-//   tiles u8 [E][R / 16][S][64][16], tile_scales u32 [E][S][R], row_exps i32 [E][R].
+// out for the products, with R = out_features up to a multiple of 16, Q =
+// out_features / 64 and S = in_features / 128, both rounded up:
+//   tiles u8 [E][R / 16][S][64][16], tile_scales u8 [E][S][Q][64][4], row_exps i32 [E][R].
 // A block more than 2^140 below its row's largest is taken as zero.
 int iqk_mx_pack(int64_t in_features, int64_t out_features, int64_t num_experts, const uint8_t *codes,
-                const uint8_t *scales, int64_t scale_stride, void *tiles, uint32_t *tile_scales, int32_t *row_exps,
+                const uint8_t *scales, int64_t scale_stride, void *tiles, uint8_t *tile_scales, int32_t *row_exps,
                 void *stream);
 
 // The laid-out weights' values, rounded once to dtype: y [E, out_features, in_features].
 int iqk_mx_unpack(int dtype, int64_t in_features, int64_t out_features, int64_t num_experts, const void *tiles,
-                  const uint32_t *tile_scales, const int32_t *row_exps, void *y, void *stream);
+                  const uint8_t *tile_scales, const int32_t *row_exps, void *y, void *stream);
 
 // Products of token-expert pairs, each on its own (few pairs):
 //   y[p, r] = sum_k W[ids[p]][r][k] * x[p / pairs_per_x_row][k],
@@ -316,7 +316,7 @@ int iqk_mx_unpack(int dtype, int64_t in_features, int64_t out_features, int64_t 
 // to multiples of 2^-37 of it.  num_experts <= 4096, in_features % 32 == 0.
 int iqk_mx_pairs(int act, int64_t in_features, int64_t out_features, int64_t num_experts, const void *x,
                  int64_t n_x_rows, const uint8_t *x_scales, int64_t x_scale_stride, const void *tiles,
-                 const uint32_t *tile_scales, const int32_t *row_exps, const void *ids, int wide_ids,
+                 const uint8_t *tile_scales, const int32_t *row_exps, const void *ids, int wide_ids,
                  int64_t pairs_per_x_row, int64_t n_pairs, void *y, void *stream);
 
 // The same for slots sorted by expert (iqk_route's lists; x_rows, y_rows and
@@ -325,7 +325,7 @@ int iqk_mx_pairs(int act, int64_t in_features, int64_t out_features, int64_t num
 // group_offsets NULL: one expert with every slot; x_rows, y_rows NULL: the slots'.
 int iqk_mx_groups(int act, int64_t in_features, int64_t out_features, int64_t num_experts, const void *x,
                   int64_t n_x_rows, const uint8_t *x_scales, int64_t x_scale_stride, const void *tiles,
-                  const uint32_t *tile_scales, const int32_t *row_exps, const uint32_t *group_offsets,
+                  const uint8_t *tile_scales, const int32_t *row_exps, const uint32_t *group_offsets,
                   const uint32_t *x_rows, const uint32_t *y_rows, int64_t n_slots, void *y, void *stream);
 
 // The router's choice: ids[t] the k highest logits of row t in falling order,

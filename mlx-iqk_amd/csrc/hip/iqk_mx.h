@@ -10,9 +10,11 @@
 // holds the 16 code bytes of row r, block g, and a tile is those 64 x 16
 // bytes in lane order, so that a wavefront's load is 1 KiB in one piece.
 //   tiles  u8  [E][rows / 16][steps][64][16]   (steps = columns / 128)
-//   tscale u32 [E][steps][rows]                byte g: block g's scale
+//   tscale u8  [E][steps][rows / 64][64][4]    byte i of lane 16 g + r: row 16 i + r, block g
 //   rexp   i32 [E][rows]
-// rows and columns round up to 16 and 128 (codes 0, scale 1).  A row's scales
+// so a lane's word of scales serves a wavefront's 64 rows, the MFMA selecting
+// the byte.  rows and columns round up to 16 (of tscale to 64) and 128 (codes 0,
+// scale 1).  A row's scales
 // are kept relative to its largest: byte + 140 - largest, and the row's
 // products are multiplied by 2^rexp, rexp = largest - 140, at the end.  So the
 // largest weight in a row is between 2^13 and 6 x 2^13, inside fp16, where

@@ -122,9 +122,9 @@ struct PackArgs {
     const uint8_t *codes;
     const uint8_t *scales;
     uint4_t *tiles;
-    uint32_t *tscale;
+    uint8_t *tscale;
     int32_t *rexp;
-    uint32_t out, rows, blocks, steps;  // rows: out up to 16; blocks: in / 32; steps: in / 128 up
+    uint32_t out, rows, blocks, steps, quads;  // rows: out up to 16; blocks: in / 32; steps: in / 128 up; quads: out / 64 up
     int64_t scale_stride;
 };
 
@@ -174,19 +174,16 @@ __global__ __launch_bounds__(256) void mx_pack_kernel(PackArgs a) {
                 byte = raw + kMxTop - top[rr];
         }
         a.tiles[((size_t(e) * trows + t) * a.steps + s) * 64 + lane] = c;
-        uint32_t word = byte << (8 * g);
-        word |= uint32_t(__shfl_xor(int(word), 16, 64));
-        word |= uint32_t(__shfl_xor(int(word), 32, 64));
-        if (lane < kMxRows) a.tscale[(size_t(e) * a.steps + s) * a.rows + kMxRows * t + lane] = word;
+        a.tscale[(((size_t(e) * a.steps + s) * a.quads + t / 4) * 64 + lane) * 4 + t % 4] = uint8_t(byte);
     }
 }
 
 struct UnpackArgs {
     const uint4_t *tiles;
-    const uint32_t *tscale;
+    const uint8_t *tscale;
     const int32_t *rexp;
     void *y;
-    uint32_t out, rows, blocks, steps;
+    uint32_t out, rows, blocks, steps, quads;
     uint64_t total;  // num_experts * out * blocks * 4
 };
 
@@ -202,7 +199,8 @@ __global__ __launch_bounds__(kCastThreads) void mx_unpack_kernel(UnpackArgs a) {
         const uint4_t *const tile =
             a.tiles + ((size_t(e) * (a.rows / kMxRows) + row / kMxRows) * a.steps + s) * 64 + 16 * g + row % kMxRows;
         const uint32_t c = reinterpret_cast<const uint32_t *>(tile)[q];
-        const uint32_t rel = (a.tscale[(size_t(e) * a.steps + s) * a.rows + row] >> (8 * g)) & 255u;
+        const uint32_t rel =
+            a.tscale[(((size_t(e) * a.steps + s) * a.quads + row / 64) * 64 + 16 * g + row % 16) * 4 + row / 16 % 4];
         // back to the format's byte: rel was byte + kMxTop - largest
         const int byte = rel == 255u ? 255 : int(rel) + a.rexp[size_t(e) * a.rows + row];
         store_eight<DT>(a.y, 8u * size_t(i), c, scale_float(uint32_t(min(max(byte, 0), 255))));
@@ -271,7 +269,7 @@ int iqk_mx_dequantize(int dtype, const uint8_t *codes, const uint8_t *scales, in
 }
 
 int iqk_mx_pack(int64_t in_features, int64_t out_features, int64_t num_experts, const uint8_t *codes,
-                const uint8_t *scales, int64_t scale_stride, void *tiles, uint32_t *tile_scales, int32_t *row_exps,
+                const uint8_t *scales, int64_t scale_stride, void *tiles, uint8_t *tile_scales, int32_t *row_exps,
                 void *stream) {
     using namespace iqk;
     if (!mx_shape_ok(in_features, out_features, num_experts)) return IQK_ERR_GEOMETRY;
@@ -280,21 +278,22 @@ int iqk_mx_pack(int64_t in_features, int64_t out_features, int64_t num_experts, 
         return IQK_ERR_ARGUMENT;
     const uint32_t rows = uint32_t((out_features + 15) / 16 * 16);
     PackArgs a{codes, scales, static_cast<uint4_t *>(tiles), tile_scales, row_exps, uint32_t(out_features), rows,
-               uint32_t(in_features / kMxBlock), uint32_t((in_features + kMxStep - 1) / kMxStep), scale_stride};
+               uint32_t(in_features / kMxBlock), uint32_t((in_features + kMxStep - 1) / kMxStep),
+               uint32_t((out_features + 63) / 64), scale_stride};
     hipLaunchKernelGGL(mx_pack_kernel, dim3{uint32_t(num_experts * (rows / kMxRows))}, dim3{256}, 0, as_stream(stream),
                        a);
     return record_launch(hipGetLastError());
 }
 
 int iqk_mx_unpack(int dtype, int64_t in_features, int64_t out_features, int64_t num_experts, const void *tiles,
-                  const uint32_t *tile_scales, const int32_t *row_exps, void *y, void *stream) {
+                  const uint8_t *tile_scales, const int32_t *row_exps, void *y, void *stream) {
     using namespace iqk;
     if (dtype < MX_F32 || dtype > MX_BF16) return IQK_ERR_ARGUMENT;
     if (!mx_shape_ok(in_features, out_features, num_experts)) return IQK_ERR_GEOMETRY;
     if (!tiles || !tile_scales || !row_exps || !y || !aligned16(tiles) || !aligned16(y)) return IQK_ERR_ARGUMENT;
     const uint32_t rows = uint32_t((out_features + 15) / 16 * 16), blocks = uint32_t(in_features / kMxBlock);
     UnpackArgs a{static_cast<const uint4_t *>(tiles), tile_scales, row_exps, y, uint32_t(out_features), rows, blocks,
-                 uint32_t((in_features + kMxStep - 1) / kMxStep),
+                 uint32_t((in_features + kMxStep - 1) / kMxStep), uint32_t((out_features + 63) / 64),
                  uint64_t(num_experts) * uint64_t(out_features) * blocks * 4};
     const dim3 grid{cast_blocks(a.total)}, block{kCastThreads};
     if (dtype == MX_F32)

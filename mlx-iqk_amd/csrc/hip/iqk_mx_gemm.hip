@@ -31,14 +31,14 @@ struct MxArgs {
     const uint8_t *xscale;   // 4-bit rows' scales
     int64_t xscale_stride;
     const uint4_t *tiles;
-    const uint32_t *tscale;
+    const uint32_t *tscale;  // words of a lane
     const int32_t *rexp;
     const uint32_t *ids;     // pairs: expert ids, or null: all expert 0
     const uint32_t *offs;    // groups: first slots, or null: one group
     const uint32_t *xr;      // groups: activation rows, or null: the slots'
     const uint32_t *yr;      // groups: output rows, or null: the slots'
     uint16_t *y;
-    uint32_t K, N, rows, steps, E, n_slots, n_x_rows, per_row, wide;
+    uint32_t K, N, rows, steps, quads, E, n_slots, n_x_rows, per_row, wide, set;
 };
 
 template <int ACT>
@@ -69,127 +69,6 @@ __device__ __forceinline__ float4_t mfma4(uint4_t a, uint32_t sa, uint4_t b, uin
     return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(av, bv, c, 4, 4, 0, int(sa), 0, int(sb));
 }
 
-// ------------------------------------------------------------- single pairs ---
-//
-// A workgroup computes 16 outputs of one token-expert pair.  Its wavefronts
-// split the reduction axis, four tiles of 128 columns each (all loads of the
-// four issued before the first is used), and their sums meet in LDS.  Only
-// column 0 of the activations' operand is real, so only its four lanes load.
-constexpr int kPairSteps = 4;
-
-template <int ACT, int WAVES>
-__global__ __launch_bounds__(64 * WAVES) void mx_pair_kernel(MxArgs a) {
-    __shared__ float part[WAVES][kMxRows];
-    const uint32_t trows = a.rows / kMxRows;
-    const uint32_t p = blockIdx.x / trows, t = blockIdx.x % trows;
-    const uint32_t lane = threadIdx.x & 63u, g = lane >> 4, r = lane & 15u;
-    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const uint32_t e = a.ids ? expert_id(a.ids, p, a.wide) : 0u;
-    if (e >= a.E) {
-        const uint32_t row = kMxRows * t + threadIdx.x;
-        if (threadIdx.x < kMxRows && row < a.N) a.y[size_t(p) * a.N + row] = kOutNaN<ACT>;
-        return;
-    }
-    const uint4_t *const tile = a.tiles + (size_t(e) * trows + t) * a.steps * 64 + lane;
-    const uint32_t *const ts = a.tscale + size_t(e) * a.steps * a.rows + kMxRows * t + r;
-    const size_t xrow = p / a.per_row;
-    const uint32_t blocks = a.K / kMxBlock;
-    float4_t acc[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
-    for (uint32_t s0 = wave * kPairSteps; s0 < a.steps; s0 += WAVES * kPairSteps) {
-        uint4_t w[kPairSteps];
-        uint32_t sc[kPairSteps];
-        constexpr int XN = act_mx(ACT) ? 1 : 4;
-        uint4_t x[kPairSteps][XN];
-        uint32_t xs[kPairSteps];
-#pragma unroll
-        for (int i = 0; i < kPairSteps; ++i) {
-            const uint32_t s = min(s0 + i, a.steps - 1u);  // past the last: its weights again, against zeros
-            w[i] = tile[size_t(s) * 64];
-            sc[i] = ts[size_t(s) * a.rows];
-        }
-#pragma unroll
-        for (int i = 0; i < kPairSteps; ++i) {
-            const uint32_t b = 4 * (s0 + i) + g;
-            xs[i] = 127u;
-#pragma unroll
-            for (int j = 0; j < XN; ++j) x[i][j] = uint4_t{0, 0, 0, 0};
-            if (r == 0 && b < blocks) {
-                if constexpr (act_mx(ACT)) {
-                    x[i][0] = load_u4(a.x + xrow * (a.K / 2) + 16 * size_t(b));
-                    xs[i] = a.xscale[xrow * a.xscale_stride + b];
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) x[i][j] = load_u4(a.x + xrow * a.K * 2 + 64 * size_t(b) + 16 * j);
-                }
-            }
-        }
-#pragma unroll
-        for (int i = 0; i < kPairSteps; ++i) {
-            const uint32_t byte = (sc[i] >> (8 * g)) & 255u;
-            if constexpr (act_mx(ACT)) {
-                acc[i & 1] = mfma4(w[i], byte, x[i][0], xs[i], acc[i & 1]);
-            } else {
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    acc[j & 1] = mfma16<ACT>(eight16<act_bf16(ACT)>(w[i][j], scale_float(byte)), x[i][j], acc[j & 1]);
-            }
-        }
-    }
-    if (r == 0) *reinterpret_cast<float4_t *>(&part[wave][4 * g]) = acc[0] + acc[1];
-    __syncthreads();
-    const uint32_t row = kMxRows * t + threadIdx.x;
-    if (threadIdx.x < kMxRows && row < a.N) {
-        float v = 0.f;
-#pragma unroll
-        for (int k = 0; k < WAVES; ++k) v += part[k][threadIdx.x];
-        a.y[size_t(p) * a.N + row] = uint16_t(out16<ACT>(ldexpf(v, a.rexp[size_t(e) * a.rows + row])));
-    }
-}
-
-// ------------------------------------------------------------------- groups ---
-//
-// Slots sorted by expert; a workgroup of eight wavefronts computes 256 outputs
-// of up to 128 slots of one expert.  Both operands go from memory straight
-// into LDS, in three stages of which two are in flight while one is
-// contracted; nothing is held in registers on the way.
-//
-// A stage is 128 columns (16-bit activations: 256 bytes a slot) or 256 (4-bit:
-// 128 bytes a slot).  The slots' 16-byte chunks are stored at positions
-// chunk ^ f(slot), so that the 16 lanes of an operand read, one chunk of 16
-// slots, cover all 64 banks once; the weights' tiles are in lane order already.
-//
-// Wavefronts stand 4 x 2 (64 outputs, 64 slots each) in a tile of more than 64
-// slots, else 8 x 1 (32 outputs, all the slots), and run only the 16-slot
-// columns that the tile has.
-//
-// Work list: group e's M-tiles take the numbers from offs[e] / BM + e on, at
-// least as many as it has: a workgroup finds its group from the offsets by
-// two ballots, with no scan and no list, and those in the gaps leave.  The
-// output blocks of a tile are consecutive workgroups, so with eight of them
-// each XCD keeps one slice of an expert's weights in its L2 over the
-// expert's tiles.
-constexpr int kMxBM = 128, kMxBN = 256, kMxWaves = 8, kMxStages = 3;
-constexpr uint32_t kMxMaxExperts = 4096;  // 64 x 64, the two ballots
-
-template <int ACT>
-struct Stage {
-    static constexpr int STEPS = act_mx(ACT) ? 2 : 1;                // tiles of 128 columns
-    static constexpr int XROW = act_mx(ACT) ? 128 : 256;             // bytes of a slot
-    static constexpr int CHUNKS = XROW / 16;
-    static constexpr int XROWS = 64 / CHUNKS;                        // slots of a load instruction
-    static constexpr int W = 0;                                      // [16 tile rows][STEPS][1024]
-    static constexpr int X = W + 16 * STEPS * kMxTileBytes;          // [128 slots][XROW]
-    static constexpr int WS = X + kMxBM * XROW;                      // [STEPS][256 rows] u32
-    static constexpr int XS = WS + STEPS * kMxBN * 4;                // 4-bit: [STEPS][128 slots] u32
-    static constexpr int BYTES = XS + (act_mx(ACT) ? STEPS * kMxBM * 4 : 0);
-    static constexpr int WLOADS = 16 * STEPS / kMxWaves;             // of a wavefront
-    static __device__ __forceinline__ uint32_t swizzle(uint32_t slot) {
-        return act_mx(ACT) ? (slot >> 1) & 7u : slot & 15u;
-    }
-};
-
-__device__ uint4_t mx_zeros;
-
 // One 16-byte (4-byte) load per lane from global memory into LDS at lds + 16
 // (4) lane, M0 holding the wavefront's base.  Inline asm, so that the compiler
 // sees no load to wait for: the waits are written out below.  An LDS DMA right
@@ -206,11 +85,138 @@ __device__ __forceinline__ void to_lds4(uint32_t lds, const void *src) {
 }
 #pragma clang diagnostic pop
 
-// All but the N loads issued last have landed, this wavefront's LDS reads have
-// returned, and every wavefront is here.
-template <int N>
-__device__ __forceinline__ void wait_stage() {
-    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
+__device__ __forceinline__ uint32_t lds_address(const void *p) {
+    return uint32_t(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) const uint8_t *)(p)));
+}
+
+__device__ uint4_t mx_zeros;
+
+typedef const __attribute__((address_space(1))) uint8_t *global_ptr;
+
+__device__ __forceinline__ uint4_t load_u4(global_ptr p) {
+    return *reinterpret_cast<const __attribute__((address_space(1))) uint4_t *>(p);
+}
+
+// Sixteen bytes of zeros, as an address of which the compiler knows nothing: a
+// load from there or from a row stays one load.
+__device__ __forceinline__ global_ptr zero_chunk() {
+    uint64_t p = reinterpret_cast<uint64_t>(&mx_zeros);
+    asm("" : "+v"(p));
+    return reinterpret_cast<global_ptr>(p);
+}
+
+// ------------------------------------------------------------- single pairs ---
+//
+// A workgroup computes 16 outputs of one token-expert pair.  Its wavefronts
+// split the reduction axis, four tiles of 128 columns each, whose loads are all
+// in flight before the first is used, and their sums meet in LDS.  The
+// activations of a wavefront's 512 columns go straight into LDS (one load of 1 KiB,
+// 256 bytes of 4-bit codes) and are read by all lanes of a block of 32, so every
+// column of the MFMA holds the same slot.
+constexpr int kPairSteps = 4;
+
+template <int ACT, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void mx_pair_kernel(MxArgs a) {
+    constexpr int XBYTES = act_mx(ACT) ? 256 : 1024;
+    __shared__ float part[WAVES][kMxRows];
+    __shared__ __attribute__((aligned(16))) uint8_t xlds[WAVES][XBYTES];
+    const uint32_t trows = a.rows / kMxRows;
+    const uint32_t p = blockIdx.x / trows;
+    uint32_t t = blockIdx.x % trows;
+    // the four tile rows that share words of scales run on one XCD (workgroups
+    // eight apart), so that HBM is read once for them
+    if (trows % 32 == 0) t = (t & ~31u) | (t & 7u) << 2 | (t >> 3 & 3u);
+    const uint32_t lane = threadIdx.x & 63u, g = lane >> 4;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t e = a.ids ? expert_id(a.ids, p, a.wide) : 0u;
+    if (e >= a.E) {
+        const uint32_t row = kMxRows * t + threadIdx.x;
+        if (threadIdx.x < kMxRows && row < a.N) a.y[size_t(p) * a.N + row] = kOutNaN<ACT>;
+        return;
+    }
+    const uint4_t *const tile = a.tiles + (size_t(e) * trows + t) * a.steps * 64 + lane;
+    const uint32_t *const ts = a.tscale + (size_t(e) * a.steps * a.quads + t / 4) * 64 + lane;
+    const size_t xrow = p / a.per_row;
+    const uint32_t xat = lds_address(xlds[wave]), blocks = a.K / kMxBlock;
+    float4_t acc[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+    for (uint32_t s0 = wave * kPairSteps; s0 < a.steps; s0 += WAVES * kPairSteps) {
+        if constexpr (act_mx(ACT)) {  // lane: 8 columns
+            const uint32_t c = 64 * s0 + lane * 4;
+            to_lds4(xat, c < a.K / 2 ? static_cast<const void *>(a.x + xrow * (a.K / 2) + c) : &mx_zeros);
+        } else {
+            const uint32_t c = 128 * s0 + lane * 8;
+            to_lds16(xat, c < a.K ? static_cast<const void *>(a.x + 2 * (xrow * a.K + c)) : &mx_zeros);
+        }
+        uint4_t w[kPairSteps];
+        uint32_t sc[kPairSteps], xs[kPairSteps];
+#pragma unroll
+        for (int i = 0; i < kPairSteps; ++i) {
+            const uint32_t s = min(s0 + i, a.steps - 1u);  // past the last: its weights again, against zeros
+            w[i] = tile[size_t(s) * 64];
+            sc[i] = ts[size_t(s) * a.quads * 64];
+            if constexpr (act_mx(ACT))
+                xs[i] = *reinterpret_cast<const uint32_t *>(a.xscale + xrow * a.xscale_stride + 4 * s);
+        }
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+#pragma unroll
+        for (int i = 0; i < kPairSteps; ++i) {
+            const uint32_t byte = (sc[i] >> (8 * (t & 3u))) & 255u;
+            if constexpr (act_mx(ACT)) {
+                const uint32_t sx = 4 * (s0 + i) + g < blocks ? xs[i] >> (8 * g) : 127u;
+                acc[i & 1] = mfma4(w[i], byte, load_u4(xlds[wave] + 64 * i + 16 * g), sx, acc[i & 1]);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    acc[j & 1] = mfma16<ACT>(eight16<act_bf16(ACT)>(w[i][j], scale_float(byte)),
+                                             load_u4(xlds[wave] + 256 * i + 64 * g + 16 * j), acc[j & 1]);
+            }
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // before the next turn's load into the same place
+    }
+    if ((lane & 15u) == 0) *reinterpret_cast<float4_t *>(&part[wave][4 * g]) = acc[0] + acc[1];
+    __syncthreads();
+    const uint32_t row = kMxRows * t + threadIdx.x;
+    if (threadIdx.x < kMxRows && row < a.N) {
+        float v = 0.f;
+#pragma unroll
+        for (int k = 0; k < WAVES; ++k) v += part[k][threadIdx.x];
+        a.y[size_t(p) * a.N + row] = uint16_t(out16<ACT>(ldexpf(v, a.rexp[size_t(e) * a.rows + row])));
+    }
+}
+
+// ------------------------------------------------------------------- groups ---
+//
+// Slots sorted by expert; a workgroup of four wavefronts computes 256 outputs
+// of up to 64 slots of one expert, a wavefront 64 of the outputs for all the
+// slots, so that each weight is loaded and scaled by one wavefront only.  The
+// weights go from memory into registers in the MFMA's layout, two steps of 128
+// columns (4-bit activations: four) ahead; the slots' rows go through LDS, 256
+// bytes a slot and turn (128 columns, or 512 of 4 bits), two buffers.  Two
+// workgroups fit a CU, so that one's start, end and waits run under the other's
+// products: with one workgroup of 128 slots a CU and both operands in an LDS
+// ring, finding the tile, the first loads and the stores took 8 us a tile in
+// which the CU did nothing else.
+//
+// The slots' 16-byte chunks are stored at positions chunk ^ swizzle(slot), so
+// that an operand read (16 slots, one chunk each) meets no bank twice in any of
+// its four parts of 16 lanes, which are {0-3, 12-15, 20-23, 24-27} and alike.
+//
+// Work list: the experts' M-tiles in order, an expert's ceil(slots / 64) of them.  A
+// wavefront finds its tile from the offsets with two scans in registers: no
+// list, and no workgroup without work but past the end.  (Numbers with gaps,
+// offs[e] / 64 + e on for expert e, need no scan, but their empty workgroups cost
+// more than their run: 256 experts of 64 slots took 451 us, and 286 without.)
+// The workgroups of an M-tile's outputs run on one XCD, four M-tiles together, so
+// that it reads a slot's activations once for all outputs and a slice of the weights
+// once for the four.
+constexpr int kMxBM = 64, kMxBN = 256, kMxWaves = 4;
+constexpr int kMxRowBytes = 256;          // of a slot and turn in LDS
+constexpr uint32_t kMxMaxExperts = 4096;  // 64 x 64, the two scans
+
+template <int ACT>
+__device__ __forceinline__ uint32_t swizzle(uint32_t slot) {
+    // chunks read together: 4 g + j (16-bit), 4 j + g
+    return act_mx(ACT) ? 2u * (slot & 3u) + (slot & 8u) : (slot & 3u) | ((slot & 8u) ? 12u : 0u);
 }
 
 struct MxTile {
@@ -219,212 +225,354 @@ struct MxTile {
 
 // The workgroup's tile; false (uniformly) in a gap of the list.
 __device__ __forceinline__ bool find_tile(const MxArgs &a, MxTile &t) {
-    const uint32_t nblocks = (a.N + kMxBN - 1) / kMxBN;
-    const uint32_t u = blockIdx.x / nblocks, lane = threadIdx.x & 63u;
-    t.n0 = blockIdx.x % nblocks * kMxBN;
+    const uint32_t nblocks = (a.N + kMxBN - 1) / kMxBN, lane = threadIdx.x & 63u;
+    // a set of 8 a.set M-tiles: a.set on each XCD, and there, for each block of
+    // outputs, one after another
+    uint32_t u = blockIdx.x / nblocks, nb = blockIdx.x % nblocks;
+    if (a.set) {
+        const uint32_t span = 8u * a.set * nblocks, v = blockIdx.x / span, i = blockIdx.x % span, k = i >> 3;
+        u = (8u * v + (i & 7u)) * a.set + k % a.set;
+        nb = k / a.set;
+    }
+    t.n0 = nb * kMxBN;
     if (!a.offs) {
         t.e = 0;
+        if (u >= (a.n_slots + kMxBM - 1) / kMxBM) return false;
         t.m0 = u * kMxBM;
         t.n = min(a.n_slots - t.m0, uint32_t(kMxBM));
         return true;
     }
-    const uint32_t stride = (a.E + 63u) / 64u;
-    uint32_t at = lane * stride;
-    const bool first = at < a.E && a.offs[at < a.E ? at : 0u] / kMxBM + at <= u;
-    const uint32_t base = (max(uint32_t(__popcll(__ballot(first))), 1u) - 1u) * stride;
-    at = base + lane;
-    const bool second = lane < stride && at < a.E && a.offs[at < a.E ? at : 0u] / kMxBM + at <= u;
-    t.e = base + max(uint32_t(__popcll(__ballot(second))), 1u) - 1u;
-    t.e = __builtin_amdgcn_readfirstlane(t.e);
+    // lane l counts the M-tiles of `per` experts from l per on; the lane whose
+    // count holds u is then taken apart, a lane an expert
+    const uint32_t per = (a.E + 63u) / 64u;
+    const auto tiles_of = [&](uint32_t from, uint32_t n) {
+        uint32_t count = 0, lo = a.offs[min(from, a.E)];
+        for (uint32_t i = 1; i <= n; ++i) {
+            const uint32_t hi = a.offs[min(from + i, a.E)];
+            count += (hi - lo + kMxBM - 1u) / kMxBM;
+            lo = hi;
+        }
+        return count;
+    };
+    // the first lane whose running total exceeds u; u becomes its place in that lane
+    const auto find = [&](uint32_t count) {
+        uint32_t total = count;
+#pragma unroll
+        for (int off = 1; off < 64; off <<= 1) {
+            const uint32_t before = uint32_t(__shfl_up(int(total), off, 64));
+            if (lane >= uint32_t(off)) total += before;
+        }
+        const uint64_t past = __ballot(total > u);
+        if (past == 0) return 64u;
+        const int at = __ffsll((unsigned long long)past) - 1;
+        u -= uint32_t(__builtin_amdgcn_readlane(int(total - count), at));
+        return uint32_t(at);
+    };
+    uint32_t at = find(tiles_of(lane * per, per));
+    if (at == 64u) return false;  // past the last tile
+    if (per == 1) {
+        t.e = at;
+    } else {
+        const uint32_t first = at * per;
+        at = find(lane < per ? tiles_of(first + lane, 1) : 0u);
+        t.e = first + at;
+    }
+    if (t.e >= a.E) return false;
     const uint32_t lo = a.offs[t.e], hi = min(a.offs[t.e + 1], a.n_slots);
-    const uint64_t m0 = uint64_t(lo) + uint64_t(u - (lo / kMxBM + t.e)) * kMxBM;
+    const uint64_t m0 = uint64_t(lo) + uint64_t(u) * kMxBM;
     if (m0 >= hi) return false;
     t.m0 = uint32_t(m0);
     t.n = min(hi - t.m0, uint32_t(kMxBM));
     return true;
 }
 
-template <int ACT>
-struct MxBlock {
-    using S = Stage<ACT>;
-    const MxArgs &a;
-    const MxTile &t;
-    uint8_t *lds;
-    const uint32_t *dst;  // per slot: output row, bit 31 where its activations are real
-    uint32_t lane, g, r, wave, stages;
+struct MxShared {
+    __attribute__((aligned(16))) uint8_t x[2][kMxBM * kMxRowBytes];
+    uint32_t xs[2][256];  // 4-bit slots' scales, a word a step
+    uint32_t dst[kMxBM];  // output row, bit 31 where the slot's activations are real
+};
 
-    // XL activation loads a wavefront and stage, RT tile rows and NC columns
-    // of 16 slots a wavefront.  EXTRA: the wavefront loads scales too.
-    template <int XL, int RT, int NC, bool EXTRA>
-    __device__ __forceinline__ void run() {
-        const uint32_t base = uint32_t(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) uint8_t *)(lds)));
-        const uint32_t trows = a.rows / kMxRows, blocks = a.K / kMxBlock;
-        // activation sources: instruction i of the wavefront moves XROWS slots
-        const uint8_t *xsrc[XL];
-        uint32_t xchunk[XL];
-        const size_t xbytes = act_mx(ACT) ? a.K / 2 : 2 * size_t(a.K);
-        const auto xrow_of = [&](uint32_t slot) {
-            uint32_t row = 0;
-            if (slot < t.n) row = a.xr ? a.xr[t.m0 + slot] : t.m0 + slot;
-            return row < a.n_x_rows ? row : 0u;
-        };
-#pragma unroll
-        for (int i = 0; i < XL; ++i) {
-            const uint32_t slot = (wave * XL + i) * S::XROWS + lane / S::CHUNKS;
-            xchunk[i] = (lane % S::CHUNKS) ^ S::swizzle(slot);
-            xsrc[i] = a.x + xrow_of(slot) * xbytes + 16 * xchunk[i];
-        }
-        // weight sources: tile rows 2 wave, 2 wave + 1
-        const uint4_t *wsrc[2];
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const uint32_t tr = min(t.n0 / kMxRows + 2 * wave + i, trows - 1u);
-            wsrc[i] = a.tiles + (size_t(t.e) * trows + tr) * a.steps * 64 + lane;
-        }
-        const uint32_t *const wscale = a.tscale + size_t(t.e) * a.steps * a.rows + min(t.n0 + 4 * lane, a.rows - 4u);
-        const uint32_t xs_q = (wave - uint32_t(S::STEPS)) & 3u;  // 4-bit: of the four wavefronts with slots' scales
-        const uint8_t *xscale = nullptr;
-        if constexpr (act_mx(ACT) && EXTRA)
-            xscale = a.xscale + size_t(xrow_of(64 * (xs_q & 1u) + lane)) * a.xscale_stride;
+// A word of scales (a step's four blocks) with those of blocks past the row's end made 1.
+__device__ __forceinline__ uint32_t clip_scales(uint32_t word, uint32_t step, uint32_t blocks) {
+    const int n = int(blocks) - int(4 * step);  // blocks of this step
+    const uint32_t keep = n >= 4 ? 0xffffffffu : n <= 0 ? 0u : (1u << (8 * n)) - 1u;
+    return (word & keep) | (0x7f7f7f7fu & ~keep);
+}
 
-        const auto issue = [&](uint32_t s) {  // stage s; past the last: the last again
-            const uint32_t at = base + s % kMxStages * S::BYTES;
-            const uint32_t sc = min(s, stages - 1u);
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-#pragma unroll
-                for (int q = 0; q < S::STEPS; ++q)
-                    to_lds16(at + S::W + ((2 * wave + i) * S::STEPS + q) * kMxTileBytes,
-                             wsrc[i] + size_t(min(sc * S::STEPS + q, a.steps - 1u)) * 64);
-#pragma unroll
-            for (int i = 0; i < XL; ++i) {
-                // 16-byte chunks hold 8 or 32 columns: those past K read zeros
-                const uint32_t per = act_mx(ACT) ? 32u : 8u;
-                const bool in = (sc * S::CHUNKS + xchunk[i]) * per < a.K;
-                to_lds16(at + S::X + (wave * XL + i) * 1024,
-                         in ? static_cast<const void *>(xsrc[i] + size_t(sc) * S::XROW) : &mx_zeros);
-            }
-            if constexpr (EXTRA) {
-                if (wave < uint32_t(S::STEPS))
-                    to_lds16(at + S::WS + wave * (kMxBN * 4),
-                             wscale + size_t(min(sc * S::STEPS + wave, a.steps - 1u)) * a.rows);
-                else
-                    to_lds4(at + S::XS + ((xs_q >> 1) * kMxBM + 64 * (xs_q & 1u)) * 4,
-                            xscale + 4 * size_t(min(sc * S::STEPS + (xs_q >> 1), a.steps - 1u)));
-            }
-        };
-        constexpr int LOADS = S::WLOADS + XL + (EXTRA ? 1 : 0);
-        issue(0);
-        issue(1);
+// The weights of a wavefront's 64 outputs: AHEAD steps of four tile rows in
+// registers, and their words of scales.
+template <int ACT, int AHEAD>
+struct MxWeights {
+    const uint4_t *src[4];
+    const uint32_t *ssrc;
+    uint32_t steps, sstep;
+    uint4_t w[AHEAD][4];
+    uint32_t sw[AHEAD];
 
-        const uint32_t wr = RT == 4 ? wave >> 1 : wave, wc = RT == 4 ? wave & 1u : 0u;
-        float4_t acc[RT][NC];
+    __device__ __forceinline__ void init(const MxArgs &a, uint32_t e, uint32_t row, uint32_t lane) {
+        const uint32_t trows = a.rows / kMxRows;
+        steps = a.steps;
+        sstep = a.quads * 64;
 #pragma unroll
-        for (int i = 0; i < RT; ++i)
-#pragma unroll
-            for (int c = 0; c < NC; ++c) acc[i][c] = float4_t{0, 0, 0, 0};
-
-        for (uint32_t s = 0; s < stages; ++s) {
-            wait_stage<LOADS>();  // stage s is whole; stage s - 1's place is free
-            issue(s + 2);
-            const uint8_t *const st = lds + s % kMxStages * S::BYTES;
-            const uint8_t *const wt = st + S::W + wr * RT * S::STEPS * kMxTileBytes + 16 * lane;
-            const uint8_t *const ws = st + S::WS + 4 * (wr * RT * kMxRows + r);
-            const uint8_t *const xt = st + S::X + (64 * wc + r) * S::XROW;
-            const uint32_t swz = S::swizzle(r);  // slots 16 c + r of the tile have the same
-            if constexpr (act_mx(ACT)) {
-#pragma unroll
-                for (int q = 0; q < 2; ++q) {
-                    const uint32_t step = 2 * s + q;
-                    if (step >= a.steps) break;  // uniform
-                    uint4_t w[RT];
-                    uint32_t sw[RT];
-#pragma unroll
-                    for (int i = 0; i < RT; ++i) {
-                        w[i] = load_u4(wt + (i * 2 + q) * kMxTileBytes);
-                        sw[i] = *reinterpret_cast<const uint32_t *>(ws + q * kMxBN * 4 + i * kMxRows * 4) >> (8 * g);
-                    }
-                    const bool in = 4 * step + g < blocks;
-#pragma unroll
-                    for (int c = 0; c < NC; ++c) {
-                        const uint4_t b = load_u4(xt + c * 16 * S::XROW + 16 * ((4 * q + g) ^ swz));
-                        const uint32_t raw = *reinterpret_cast<const uint32_t *>(
-                            st + S::XS + (q * kMxBM + 64 * wc + 16 * c + r) * 4) >> (8 * g);
-                        const uint32_t sx = in ? raw : 127u;
-#pragma unroll
-                        for (int i = 0; i < RT; ++i) acc[i][c] = mfma4(w[i], sw[i], b, sx, acc[i][c]);
-                    }
-                }
-            } else {
-                uint4_t w[RT];
-                float sw[RT];
-#pragma unroll
-                for (int i = 0; i < RT; ++i) {
-                    w[i] = load_u4(wt + i * kMxTileBytes);
-                    sw[i] = scale_float(
-                        (*reinterpret_cast<const uint32_t *>(ws + i * kMxRows * 4) >> (8 * g)) & 255u);
-                }
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    uint4_t wv[RT];
-#pragma unroll
-                    for (int i = 0; i < RT; ++i) wv[i] = eight16<act_bf16(ACT)>(w[i][j], sw[i]);
-#pragma unroll
-                    for (int c = 0; c < NC; ++c) {
-                        const uint4_t b = load_u4(xt + c * 16 * S::XROW + 16 * ((4 * g + j) ^ swz));
-#pragma unroll
-                        for (int i = 0; i < RT; ++i) acc[i][c] = mfma16<ACT>(wv[i], b, acc[i][c]);
-                    }
-                }
-            }
-        }
-        // no load into LDS may be in flight when the workgroup's LDS is released
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-
-        const bool whole = a.N % 4 == 0 && (reinterpret_cast<uintptr_t>(a.y) & 7u) == 0;
-#pragma unroll
-        for (int i = 0; i < RT; ++i) {
-            const uint32_t row = t.n0 + (wr * RT + i) * kMxRows + 4 * g;
-            if (row >= a.N) continue;
-            const int32_t *const re = a.rexp + size_t(t.e) * a.rows + row;
-            const int32_t ex[4] = {re[0], re[1], re[2], re[3]};  // rows is a multiple of 16
-#pragma unroll
-            for (int c = 0; c < NC; ++c) {
-                const uint32_t slot = 64 * wc + 16 * c + r;
-                const uint32_t d = dst[slot];
-                if (d == 0xffffffffu) continue;
-                uint32_t v[4];
-#pragma unroll
-                for (int k = 0; k < 4; ++k)
-                    v[k] = d >> 31 ? out16<ACT>(ldexpf(acc[i][c][k], ex[k])) : uint32_t(kOutNaN<ACT>);
-                uint16_t *const y = a.y + size_t(d & 0x7fffffffu) * a.N + row;
-                if (whole) {
-                    *reinterpret_cast<uint2_t *>(y) = uint2_t{v[0] | v[1] << 16, v[2] | v[3] << 16};
-                } else {
-#pragma unroll
-                    for (int k = 0; k < 4; ++k)
-                        if (row + k < a.N) y[k] = uint16_t(v[k]);
-                }
-            }
-        }
+        for (int i = 0; i < 4; ++i)  // outputs past the last: its tile row, never stored
+            src[i] = a.tiles + (size_t(e) * trows + min(row / kMxRows + i, trows - 1u)) * steps * 64 + lane;
+        ssrc = a.tscale + (size_t(e) * steps * a.quads + min(row / 64, a.quads - 1u)) * 64 + lane;
     }
-
-    template <int XL, int RT, int NC>
-    __device__ __forceinline__ void go() {
-        // scales: 16-bit, wavefront 0; 4-bit, wavefronts 0, 1 and 2 .. 5
-        if (wave < (act_mx(ACT) ? 6u : 1u))
-            run<XL, RT, NC, true>();
-        else
-            run<XL, RT, NC, false>();
+    __device__ __forceinline__ void load(int slot, uint32_t step) {  // past the last: the last again
+        const size_t s = min(step, steps - 1u);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[slot][i] = src[i][s * 64];
+        sw[slot] = ssrc[s * sstep];
+    }
+    // four MFMAs of 4-bit operands: the weights' scale is byte i of the word
+    __device__ __forceinline__ void multiply4(int slot, uint4_t b, uint32_t sb, float4_t &c0, float4_t &c1,
+                                              float4_t &c2, float4_t &c3) const {
+        const int8v_t bv = {int(b.x), int(b.y), int(b.z), int(b.w), 0, 0, 0, 0};
+        const auto av = [&](int i) {
+            const uint4_t v = w[slot][i];
+            return int8v_t{int(v.x), int(v.y), int(v.z), int(v.w), 0, 0, 0, 0};
+        };
+        const int sa = int(sw[slot]);
+        c0 = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(av(0), bv, c0, 4, 4, 0, sa, 0, int(sb));
+        c1 = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(av(1), bv, c1, 4, 4, 1, sa, 0, int(sb));
+        c2 = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(av(2), bv, c2, 4, 4, 2, sa, 0, int(sb));
+        c3 = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(av(3), bv, c3, 4, 4, 3, sa, 0, int(sb));
+    }
+    // the j-th eight of each block's values in 16 bits
+    __device__ __forceinline__ void scaled(int slot, int j, uint4_t (&wv)[4]) const {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            wv[i] = eight16<act_bf16(ACT)>(w[slot][i][j], scale_float((sw[slot] >> (8 * i)) & 255u));
     }
 };
+
+// The activation row of a slot of the tile; of one without activations, any row.
+__device__ __forceinline__ uint32_t slot_row(const MxArgs &a, const MxTile &t, uint32_t slot) {
+    uint32_t row = 0;
+    if (slot < t.n) row = a.xr ? a.xr[t.m0 + slot] : t.m0 + slot;
+    return row < a.n_x_rows ? row : 0u;
+}
+
+// The wavefront's outputs: row0 its first, acc[i][c] tile row i, slots 16 c ...
+template <int ACT, int NC>
+__device__ __forceinline__ void store_outputs(const MxArgs &a, uint32_t e, uint32_t row0, const uint32_t *dst,
+                                              const float4_t (&acc)[4][NC], uint32_t lane) {
+    const uint32_t g = lane >> 4, r = lane & 15u;
+    const bool whole = a.N % 4 == 0 && (reinterpret_cast<uintptr_t>(a.y) & 7u) == 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t row = row0 + i * kMxRows + 4 * g;
+        if (row >= a.N) continue;
+        const int32_t *const re = a.rexp + size_t(e) * a.rows + row;
+        const int32_t ex[4] = {re[0], re[1], re[2], re[3]};  // rows is a multiple of 16
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            const uint32_t d = dst[16 * c + r];
+            if (d == 0xffffffffu) continue;
+            uint32_t v[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                v[k] = d >> 31 ? out16<ACT>(ldexpf(acc[i][c][k], ex[k])) : uint32_t(kOutNaN<ACT>);
+            uint16_t *const y = a.y + size_t(d & 0x7fffffffu) * a.N + row;
+            if (whole) {
+                *reinterpret_cast<uint2_t *>(y) = uint2_t{v[0] | v[1] << 16, v[2] | v[3] << 16};
+            } else {
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    if (row + k < a.N) y[k] = uint16_t(v[k]);
+            }
+        }
+    }
+}
+
+// The loops below run whole rounds of AHEAD steps without a way out in between,
+// and no loaded value is touched before its use: a branch or a select there
+// makes the compiler copy the registers that a load in flight will fill, and
+// wait for it.  So what lies past the end is read from a zero (activations) or is
+// the last step again (weights), and adds nothing.
+
+// A tile of at most 16 slots: the slots' rows come straight from memory in
+// the MFMA's layout too, so the wavefronts run on their own, with AHEAD steps of
+// both operands in flight, and HBM is kept busy.  (Eight steps of weights for
+// 16-bit slots too: 220 us against 203 over 256 experts of eight slots.)
+template <int ACT>
+__device__ __forceinline__ void few_tile(const MxArgs &a, const MxTile &t, const MxShared &sh) {
+    constexpr bool MX = act_mx(ACT);
+    constexpr int AHEAD = MX ? 8 : 4, XN = MX ? 1 : 4, STEP = MX ? 64 : 256;
+    const uint32_t lane = threadIdx.x & 63u, g = lane >> 4, r = lane & 15u;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t row0 = t.n0 + 64 * wave, steps = row0 < a.N ? a.steps : 0u;
+    MxWeights<ACT, AHEAD> w;
+    w.init(a, t.e, row0, lane);
+    // the lane's bytes of a step stand at [STEP step + STEP / 4 g, ..)
+    const size_t row = slot_row(a, t, r);
+    const uint32_t xbytes = MX ? a.K / 2 : 2 * a.K, end = r < t.n ? xbytes - STEP / 4 * g : 0u;
+    const global_ptr xsrc = global_ptr(a.x) + row * xbytes + STEP / 4 * g;
+    const uint8_t *const xscale = MX ? a.xscale + row * a.xscale_stride : nullptr;
+    const global_ptr zeros = zero_chunk();
+    uint4_t x[AHEAD][XN];
+    uint32_t xs[AHEAD];
+    const auto load_x = [&](int slot, uint32_t step) {
+        const uint32_t at = step * STEP;
+        const bool in = int(at) < int(end);
+#pragma unroll
+        for (int j = 0; j < XN; ++j)
+            x[slot][j] = load_u4(in ? xsrc + at + 16 * j : zeros);
+        if constexpr (MX) xs[slot] = *reinterpret_cast<const uint32_t *>(xscale + 4 * min(step, a.steps - 1u));
+    };
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) {
+        w.load(i, i);
+        load_x(i, i);
+    }
+    float4_t acc[4][1];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc[i][0] = float4_t{0, 0, 0, 0};
+    for (uint32_t s0 = 0; s0 < steps; s0 += AHEAD) {
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) {
+            if constexpr (MX) {
+                const uint32_t sx = clip_scales(xs[i], s0 + i, a.K / kMxBlock) >> (8 * g);
+                w.multiply4(i, x[i][0], sx, acc[0][0], acc[1][0], acc[2][0], acc[3][0]);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    uint4_t wv[4];
+                    w.scaled(i, j, wv);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) acc[k][0] = mfma16<ACT>(wv[k], x[i][j], acc[k][0]);
+                }
+            }
+            w.load(i, s0 + i + AHEAD);
+            load_x(i, s0 + i + AHEAD);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    }
+    __syncthreads();  // the slots' outputs
+    store_outputs<ACT, 1>(a, t.e, row0, sh.dst, acc, lane);
+}
+
+// A tile of at most 16 NC slots (NC > 1), T steps a turn: 16 KiB of slots, which
+// are loaded XR turns before they go into LDS.
+template <int ACT, int NC, int T, int AHEAD, int XR>
+__device__ __forceinline__ void group_tile(const MxArgs &a, const MxTile &t, MxShared &sh) {
+    constexpr bool MX = act_mx(ACT);
+    constexpr int STEP = MX ? 64 : 256;             // bytes of a slot and step
+    constexpr int ROW = T * STEP, CHUNKS = ROW / 16;  // of a slot and turn
+    constexpr int XL = NC * CHUNKS / 16;            // 16-byte loads of a thread and turn
+    static_assert(16 * NC * ROW <= kMxBM * kMxRowBytes && (!MX || 16 * NC * T <= 256) && AHEAD % T == 0, "");
+    const uint32_t tid = threadIdx.x, lane = tid & 63u, g = lane >> 4, r = lane & 15u;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const uint32_t row0 = t.n0 + 64 * wave, steps = a.steps;
+    MxWeights<ACT, AHEAD> w;
+    w.init(a, t.e, row0, lane);
+
+    // activations: chunk tid % CHUNKS of slots tid / CHUNKS + (256 / CHUNKS) i
+    constexpr int PER = 256 / CHUNKS;
+    const uint32_t xbytes = MX ? a.K / 2 : 2 * a.K, chunk = tid % CHUNKS, slot0 = tid / CHUNKS;
+    global_ptr xsrc[XL];
+    uint32_t put[XL];
+#pragma unroll
+    for (int i = 0; i < XL; ++i) {
+        const uint32_t slot = slot0 + PER * i;
+        xsrc[i] = global_ptr(a.x) + size_t(slot_row(a, t, slot)) * xbytes + 16 * chunk;
+        put[i] = slot * ROW + 16 * ((chunk & ~15u) | ((chunk & 15u) ^ swizzle<ACT>(slot)));
+    }
+    // 4-bit slots' scales: word tid % T of slot tid / T
+    const uint8_t *const xscale =
+        MX ? a.xscale + size_t(slot_row(a, t, min(tid / T, uint32_t(16 * NC - 1)))) * a.xscale_stride : nullptr;
+    const global_ptr zeros = zero_chunk();
+    uint4_t xv[XR][XL];
+    uint32_t xsv[XR];
+    const auto load_x = [&](int reg, uint32_t turn) {
+        const bool in = turn * ROW + 16 * chunk < xbytes;
+#pragma unroll
+        for (int i = 0; i < XL; ++i) xv[reg][i] = load_u4(in ? xsrc[i] + turn * ROW : zeros);
+        if constexpr (MX)
+            xsv[reg] = *reinterpret_cast<const uint32_t *>(xscale + 4 * min(T * turn + tid % T, steps - 1u));
+    };
+    const auto store_x = [&](int reg, uint32_t turn, uint32_t buf) {
+#pragma unroll
+        for (int i = 0; i < XL; ++i) *reinterpret_cast<uint4_t *>(&sh.x[buf][put[i]]) = xv[reg][i];
+        if constexpr (MX) sh.xs[buf][tid] = clip_scales(xsv[reg], T * turn + tid % T, a.K / kMxBlock);
+    };
+
+    load_x(0, 0);
+    if constexpr (XR == 2) load_x(1, 1);
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) w.load(i, i);
+    float4_t acc[4][NC];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int c = 0; c < NC; ++c) acc[i][c] = float4_t{0, 0, 0, 0};
+    store_x(0, 0, 0);
+    load_x(0, XR);
+    __syncthreads();
+
+    const uint32_t swz = swizzle<ACT>(r);  // slots 16 c + r have the same
+    // Turn s contracts buffer s % 2; turn s + 1's rows, loaded XR turns ago, go into
+    // the other one, which every wavefront left before the last barrier.
+    constexpr int ROUND = AHEAD < 2 * T ? 2 * T : AHEAD;  // steps of two turns at least
+    for (uint32_t s0 = 0; s0 < steps; s0 += ROUND) {
+#pragma unroll
+        for (int u = 0; u < ROUND / T; ++u) {
+            const uint32_t first = s0 + u * T, turn = first / T;
+            const int buf = u & 1;
+            const int reg = XR == 2 ? buf ^ 1 : 0;
+            store_x(reg, turn + 1, buf ^ 1);
+            load_x(reg, turn + 1 + XR);
+            const uint8_t *const xt = sh.x[buf] + r * ROW;
+            const uint32_t *const xs = sh.xs[buf] + r * T;
+            // a quarter's (4-bit: a step's) operands are read while the one
+            // before is multiplied, and no earlier: the scheduler would read
+            // the whole turn's and spill
+            constexpr int PARTS = MX ? T : 4 * T;
+            uint4_t b[2][NC];
+            uint32_t bs[2][NC];
+            const auto read = [&](int q) {
+                const uint32_t at = MX ? 256 * (q / 4) + 16 * ((4 * (q % 4) + g) ^ swz)
+                                       : 256 * (q / 4) + 16 * ((4 * g + q % 4) ^ swz);
+#pragma unroll
+                for (int c = 0; c < NC; ++c) {
+                    b[q & 1][c] = load_u4(xt + 16 * c * ROW + at);
+                    if constexpr (MX) bs[q & 1][c] = xs[16 * c * T + q];
+                }
+            };
+            read(0);
+#pragma unroll
+            for (int q = 0; q < PARTS; ++q) {
+                const int i = (u * T + (MX ? q : q / 4)) % AHEAD;  // the step's registers
+                if (q + 1 < PARTS) {
+                    read(q + 1);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+                if constexpr (MX) {
+#pragma unroll
+                    for (int c = 0; c < NC; ++c)
+                        w.multiply4(i, b[q & 1][c], bs[q & 1][c] >> (8 * g), acc[0][c], acc[1][c], acc[2][c],
+                                    acc[3][c]);
+                } else {
+                    uint4_t wv[4];
+                    w.scaled(i, q % 4, wv);
+#pragma unroll
+                    for (int c = 0; c < NC; ++c)
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) acc[k][c] = mfma16<ACT>(wv[k], b[q & 1][c], acc[k][c]);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+                if (MX || q % 4 == 3) w.load(i, first + (MX ? q : q / 4) + AHEAD);
+            }
+            __syncthreads();
+        }
+    }
+    if (row0 < a.N) store_outputs<ACT, NC>(a, t.e, row0, sh.dst, acc, lane);
+}
 
 template <int ACT>
 __global__ __launch_bounds__(64 * kMxWaves) __attribute__((amdgpu_waves_per_eu(2)))
 void mx_group_kernel(MxArgs a) {
-    using S = Stage<ACT>;
-    __shared__ __attribute__((aligned(16))) uint8_t lds[kMxStages * S::BYTES];
-    __shared__ uint32_t dst[kMxBM];
+    __shared__ MxShared sh;
     MxTile t;
     if (!find_tile(a, t)) return;
     if (threadIdx.x < kMxBM) {
@@ -434,25 +582,17 @@ void mx_group_kernel(MxArgs a) {
             const uint32_t yrow = a.yr ? a.yr[slot] : slot, xrow = a.xr ? a.xr[slot] : slot;
             if (yrow < a.n_slots) d = yrow | (xrow < a.n_x_rows ? 0x80000000u : 0u);
         }
-        dst[threadIdx.x] = d;
+        sh.dst[threadIdx.x] = d;
     }
-    __syncthreads();
-    const uint32_t lane = threadIdx.x & 63u;
-    MxBlock<ACT> b{a, t, lds, dst, lane, lane >> 4, lane & 15u,
-                   uint32_t(__builtin_amdgcn_readfirstlane(threadIdx.x >> 6)),
-                   (a.steps + S::STEPS - 1) / S::STEPS};
-    // slots of a wavefront's XL loads: 8 XL XROWS
-    constexpr int X32 = act_mx(ACT) ? 1 : 1, X64 = act_mx(ACT) ? 1 : 2, X128 = act_mx(ACT) ? 2 : 4;
+    constexpr bool MX = act_mx(ACT);
     if (t.n <= 16)
-        b.template go<X32, 2, 1>();
+        few_tile<ACT>(a, t, sh);
     else if (t.n <= 32)
-        b.template go<X32, 2, 2>();
+        group_tile<ACT, 2, MX ? 4 : 2, MX ? 8 : 4, MX ? 1 : 2>(a, t, sh);
     else if (t.n <= 48)
-        b.template go<X64, 2, 3>();
-    else if (t.n <= 64)
-        b.template go<X64, 2, 4>();
+        group_tile<ACT, 3, MX ? 4 : 1, MX ? 4 : 2, MX ? 1 : 2>(a, t, sh);
     else
-        b.template go<X128, 4, 4>();
+        group_tile<ACT, 4, MX ? 4 : 1, MX ? 4 : 2, MX ? 1 : 2>(a, t, sh);
 }
 
 template <int ACT>
@@ -465,9 +605,14 @@ void launch_pairs(const MxArgs &a, hipStream_t stream) {
 }
 
 template <int ACT>
-void launch_groups(const MxArgs &a, hipStream_t stream) {
+void launch_groups(MxArgs a, hipStream_t stream) {
     const uint32_t nblocks = (a.N + kMxBN - 1) / kMxBN;
-    const uint32_t mtiles = a.offs ? a.n_slots / kMxBM + a.E : (a.n_slots + kMxBM - 1) / kMxBM;
+    uint32_t mtiles = a.offs ? a.n_slots / kMxBM + min(a.E, a.n_slots) : (a.n_slots + kMxBM - 1) / kMxBM;
+    a.set = mtiles >= 64 ? 4 : mtiles >= 8 ? 1 : 0;
+    // one matrix, fewer bytes of slots than of weights: the weights stay, a
+    // block of outputs on one XCD
+    if (!a.offs && uint64_t(a.n_slots) * (act_mx(ACT) ? 1 : 4) <= a.N) a.set = 0;
+    if (a.set) mtiles = (mtiles + 8 * a.set - 1) / (8 * a.set) * (8 * a.set);
     hipLaunchKernelGGL((mx_group_kernel<ACT>), dim3{mtiles * nblocks}, dim3{64 * kMxWaves}, 0, stream, a);
 }
 
@@ -475,7 +620,7 @@ bool at16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 // What both entry points refuse, and the arguments they share.
 int product_args(MxArgs &a, int act, int64_t in, int64_t out, int64_t experts, const void *x, int64_t n_x_rows,
-                 const uint8_t *x_scales, int64_t x_scale_stride, const void *tiles, const uint32_t *tile_scales,
+                 const uint8_t *x_scales, int64_t x_scale_stride, const void *tiles, const uint8_t *tile_scales,
                  const int32_t *row_exps, int64_t n_slots, void *y) {
     constexpr int64_t kLim = int64_t(1) << 31;
     if (act < ACT_F16 || act > ACT_MX_BF16) return IQK_ERR_ARGUMENT;
@@ -495,13 +640,14 @@ int product_args(MxArgs &a, int act, int64_t in, int64_t out, int64_t experts, c
     a.xscale = x_scales;
     a.xscale_stride = x_scale_stride;
     a.tiles = static_cast<const uint4_t *>(tiles);
-    a.tscale = tile_scales;
+    a.tscale = reinterpret_cast<const uint32_t *>(tile_scales);
     a.rexp = row_exps;
     a.y = static_cast<uint16_t *>(y);
     a.K = uint32_t(in);
     a.N = uint32_t(out);
     a.rows = uint32_t((out + kMxRows - 1) / kMxRows * kMxRows);
     a.steps = uint32_t((in + kMxStep - 1) / kMxStep);
+    a.quads = uint32_t((out + 63) / 64);
     a.E = uint32_t(experts);
     a.n_slots = uint32_t(n_slots);
     a.n_x_rows = uint32_t(n_x_rows);
@@ -514,7 +660,7 @@ extern "C" {
 
 int iqk_mx_pairs(int act, int64_t in_features, int64_t out_features, int64_t num_experts, const void *x,
                  int64_t n_x_rows, const uint8_t *x_scales, int64_t x_scale_stride, const void *tiles,
-                 const uint32_t *tile_scales, const int32_t *row_exps, const void *ids, int wide_ids,
+                 const uint8_t *tile_scales, const int32_t *row_exps, const void *ids, int wide_ids,
                  int64_t pairs_per_x_row, int64_t n_pairs, void *y, void *stream) {
     using namespace iqk;
     MxArgs a;
@@ -538,7 +684,7 @@ int iqk_mx_pairs(int act, int64_t in_features, int64_t out_features, int64_t num
 
 int iqk_mx_groups(int act, int64_t in_features, int64_t out_features, int64_t num_experts, const void *x,
                   int64_t n_x_rows, const uint8_t *x_scales, int64_t x_scale_stride, const void *tiles,
-                  const uint32_t *tile_scales, const int32_t *row_exps, const uint32_t *group_offsets,
+                  const uint8_t *tile_scales, const int32_t *row_exps, const uint32_t *group_offsets,
                   const uint32_t *x_rows, const uint32_t *y_rows, int64_t n_slots, void *y, void *stream) {
     using namespace iqk;
     MxArgs a;

@@ -190,8 +190,8 @@ class _MxStack(torch.nn.Module):
 
     * ``tiles`` u8 ``[E, out/16, in/128, 64, 16]``, the codes in the order that a
       wavefront loads them;
-    * ``tile_scales`` i32 ``[E, in/128, out]``, the scales of four blocks a word,
-      relative to their row's;
+    * ``tile_scales`` u8 ``[E, in/128, out/64, 64, 4]``, the blocks' scales relative to
+      their row's;
     * ``row_exps`` i32 ``[E, out]``, each row's power of two.
 
     ``out`` and ``in`` round up to whole tiles; 4.27 bits a weight.
@@ -208,7 +208,8 @@ class _MxStack(torch.nn.Module):
         rows, steps = (self.out_features + 15) // 16 * 16, (self.in_features + _STEP - 1) // _STEP
         E = self.num_experts
         self.register_buffer("tiles", torch.zeros((E, rows // 16, steps, 64, 16), dtype=torch.uint8, device=device))
-        self.register_buffer("tile_scales", torch.zeros((E, steps, rows), dtype=torch.int32, device=device))
+        self.register_buffer("tile_scales", torch.zeros((E, steps, (rows + 63) // 64, 64, 4), dtype=torch.uint8,
+                                                        device=device))
         self.register_buffer("row_exps", torch.zeros((E, rows), dtype=torch.int32, device=device))
 
     def _load(self, codes: torch.Tensor, scales: torch.Tensor) -> None:
