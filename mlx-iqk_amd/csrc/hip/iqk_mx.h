@@ -42,6 +42,7 @@ typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
 typedef _Float16 half8_t __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
 typedef int int8v_t __attribute__((ext_vector_type(8)));
+typedef int int4v_t __attribute__((ext_vector_type(4)));
 typedef float float2v_t __attribute__((ext_vector_type(2)));
 
 __device__ __forceinline__ float scale_float(uint32_t byte) { return __builtin_bit_cast(float, byte << 23); }

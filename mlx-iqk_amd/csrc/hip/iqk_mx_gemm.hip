@@ -139,6 +139,8 @@ __global__ __launch_bounds__(64 * WAVES) void mx_pair_kernel(MxArgs a) {
     const size_t xrow = p / a.per_row;
     const uint32_t xat = lds_address(xlds[wave]), blocks = a.K / kMxBlock;
     float4_t acc[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+    // the row's exponent, needed last, is on its way from the start (rows past N: up to 16, they exist)
+    const int32_t ex = a.rexp[size_t(e) * a.rows + kMxRows * t + (threadIdx.x & 15u)];
     for (uint32_t s0 = wave * kPairSteps; s0 < a.steps; s0 += WAVES * kPairSteps) {
         if constexpr (act_mx(ACT)) {  // lane: 8 columns
             const uint32_t c = 64 * s0 + lane * 4;
@@ -180,7 +182,7 @@ __global__ __launch_bounds__(64 * WAVES) void mx_pair_kernel(MxArgs a) {
         float v = 0.f;
 #pragma unroll
         for (int k = 0; k < WAVES; ++k) v += part[k][threadIdx.x];
-        a.y[size_t(p) * a.N + row] = uint16_t(out16<ACT>(ldexpf(v, a.rexp[size_t(e) * a.rows + row])));
+        a.y[size_t(p) * a.N + row] = uint16_t(out16<ACT>(ldexpf(v, ex)));
     }
 }
 
@@ -223,7 +225,8 @@ struct MxTile {
     uint32_t e, m0, n, n0;  // expert, first slot, slots, first output
 };
 
-// The workgroup's tile; false (uniformly) in a gap of the list.
+// The workgroup's tile of at most BM slots; false (uniformly) past the last.
+template <int BM>
 __device__ __forceinline__ bool find_tile(const MxArgs &a, MxTile &t) {
     const uint32_t nblocks = (a.N + kMxBN - 1) / kMxBN, lane = threadIdx.x & 63u;
     // a set of 8 a.set M-tiles: a.set on each XCD, and there, for each block of
@@ -237,9 +240,9 @@ __device__ __forceinline__ bool find_tile(const MxArgs &a, MxTile &t) {
     t.n0 = nb * kMxBN;
     if (!a.offs) {
         t.e = 0;
-        if (u >= (a.n_slots + kMxBM - 1) / kMxBM) return false;
-        t.m0 = u * kMxBM;
-        t.n = min(a.n_slots - t.m0, uint32_t(kMxBM));
+        if (u >= (a.n_slots + BM - 1) / BM) return false;
+        t.m0 = u * BM;
+        t.n = min(a.n_slots - t.m0, uint32_t(BM));
         return true;
     }
     // lane l counts the M-tiles of `per` experts from l per on; the lane whose
@@ -249,7 +252,7 @@ __device__ __forceinline__ bool find_tile(const MxArgs &a, MxTile &t) {
         uint32_t count = 0, lo = a.offs[min(from, a.E)];
         for (uint32_t i = 1; i <= n; ++i) {
             const uint32_t hi = a.offs[min(from + i, a.E)];
-            count += (hi - lo + kMxBM - 1u) / kMxBM;
+            count += (hi - lo + BM - 1u) / BM;
             lo = hi;
         }
         return count;
@@ -279,10 +282,10 @@ __device__ __forceinline__ bool find_tile(const MxArgs &a, MxTile &t) {
     }
     if (t.e >= a.E) return false;
     const uint32_t lo = a.offs[t.e], hi = min(a.offs[t.e + 1], a.n_slots);
-    const uint64_t m0 = uint64_t(lo) + uint64_t(u) * kMxBM;
+    const uint64_t m0 = uint64_t(lo) + uint64_t(u) * BM;
     if (m0 >= hi) return false;
     t.m0 = uint32_t(m0);
-    t.n = min(hi - t.m0, uint32_t(kMxBM));
+    t.n = min(hi - t.m0, uint32_t(BM));
     return true;
 }
 
@@ -353,34 +356,56 @@ __device__ __forceinline__ uint32_t slot_row(const MxArgs &a, const MxTile &t, u
     return row < a.n_x_rows ? row : 0u;
 }
 
+// A slot's output row, bit 31 set where its activations are real (else it is NaN); ~0: not stored.
+__device__ __forceinline__ uint32_t slot_output(const MxArgs &a, const MxTile &t, uint32_t in_tile) {
+    if (in_tile >= t.n) return 0xffffffffu;
+    const uint32_t slot = t.m0 + in_tile, yrow = a.yr ? a.yr[slot] : slot, xrow = a.xr ? a.xr[slot] : slot;
+    return yrow < a.n_slots ? yrow | (xrow < a.n_x_rows ? 0x80000000u : 0u) : 0xffffffffu;
+}
+
+// The exponents of rows row .. row + 3 (or, past the last, of any).
+__device__ __forceinline__ int4v_t row_exps(const MxArgs &a, uint32_t e, uint32_t row) {
+    return *reinterpret_cast<const int4v_t *>(a.rexp + size_t(e) * a.rows + min(row, a.rows - 4u));
+}
+
+// Outputs row .. row + 3 of a slot; d: its output row, bit 31 set where its activations are real.
+template <int ACT>
+__device__ __forceinline__ void store_four(const MxArgs &a, uint32_t d, uint32_t row, float4_t acc, int4v_t ex,
+                                           bool whole) {
+    uint32_t v[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) v[k] = d >> 31 ? out16<ACT>(ldexpf(acc[k], ex[k])) : uint32_t(kOutNaN<ACT>);
+    uint16_t *const y = a.y + size_t(d & 0x7fffffffu) * a.N + row;
+    if (whole) {
+        *reinterpret_cast<uint2_t *>(y) = uint2_t{v[0] | v[1] << 16, v[2] | v[3] << 16};
+    } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            if (row + k < a.N) y[k] = uint16_t(v[k]);
+    }
+}
+
 // The wavefront's outputs: row0 its first, acc[i][c] tile row i, slots 16 c ...
-template <int ACT, int NC>
+// The exponents are read before the first store: the compiler must take each store
+// for one that may change them, and would read them again after it.
+template <int ACT, int RT, int NC>
 __device__ __forceinline__ void store_outputs(const MxArgs &a, uint32_t e, uint32_t row0, const uint32_t *dst,
-                                              const float4_t (&acc)[4][NC], uint32_t lane) {
+                                              const float4_t (&acc)[RT][NC], uint32_t lane) {
     const uint32_t g = lane >> 4, r = lane & 15u;
     const bool whole = a.N % 4 == 0 && (reinterpret_cast<uintptr_t>(a.y) & 7u) == 0;
+    int4v_t ex[RT];
+    uint32_t d[NC];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const uint32_t row = row0 + i * kMxRows + 4 * g;
-        if (row >= a.N) continue;
-        const int32_t *const re = a.rexp + size_t(e) * a.rows + row;
-        const int32_t ex[4] = {re[0], re[1], re[2], re[3]};  // rows is a multiple of 16
+    for (int i = 0; i < RT; ++i) ex[i] = row_exps(a, e, row0 + i * kMxRows + 4 * g);
 #pragma unroll
-        for (int c = 0; c < NC; ++c) {
-            const uint32_t d = dst[16 * c + r];
-            if (d == 0xffffffffu) continue;
-            uint32_t v[4];
+    for (int c = 0; c < NC; ++c) d[c] = dst[16 * c + r];
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
-                v[k] = d >> 31 ? out16<ACT>(ldexpf(acc[i][c][k], ex[k])) : uint32_t(kOutNaN<ACT>);
-            uint16_t *const y = a.y + size_t(d & 0x7fffffffu) * a.N + row;
-            if (whole) {
-                *reinterpret_cast<uint2_t *>(y) = uint2_t{v[0] | v[1] << 16, v[2] | v[3] << 16};
-            } else {
+    for (int c = 0; c < NC; ++c) {
+        if (d[c] == 0xffffffffu) continue;
 #pragma unroll
-                for (int k = 0; k < 4; ++k)
-                    if (row + k < a.N) y[k] = uint16_t(v[k]);
-            }
+        for (int i = 0; i < RT; ++i) {
+            const uint32_t row = row0 + i * kMxRows + 4 * g;
+            if (row < a.N) store_four<ACT>(a, d[c], row, acc[i][c], ex[i], whole);
         }
     }
 }
@@ -449,7 +474,7 @@ __device__ __forceinline__ void few_tile(const MxArgs &a, const MxTile &t, const
         }
     }
     __syncthreads();  // the slots' outputs
-    store_outputs<ACT, 1>(a, t.e, row0, sh.dst, acc, lane);
+    store_outputs<ACT, 4, 1>(a, t.e, row0, sh.dst, acc, lane);
 }
 
 // A tile of at most 16 NC slots (NC > 1), T steps a turn: 16 KiB of slots, which
@@ -566,7 +591,7 @@ __device__ __forceinline__ void group_tile(const MxArgs &a, const MxTile &t, MxS
             __syncthreads();
         }
     }
-    if (row0 < a.N) store_outputs<ACT, NC>(a, t.e, row0, sh.dst, acc, lane);
+    if (row0 < a.N) store_outputs<ACT, 4, NC>(a, t.e, row0, sh.dst, acc, lane);
 }
 
 template <int ACT>
@@ -574,16 +599,8 @@ __global__ __launch_bounds__(64 * kMxWaves) __attribute__((amdgpu_waves_per_eu(2
 void mx_group_kernel(MxArgs a) {
     __shared__ MxShared sh;
     MxTile t;
-    if (!find_tile(a, t)) return;
-    if (threadIdx.x < kMxBM) {
-        uint32_t d = 0xffffffffu;  // not stored
-        if (threadIdx.x < t.n) {
-            const uint32_t slot = t.m0 + threadIdx.x;
-            const uint32_t yrow = a.yr ? a.yr[slot] : slot, xrow = a.xr ? a.xr[slot] : slot;
-            if (yrow < a.n_slots) d = yrow | (xrow < a.n_x_rows ? 0x80000000u : 0u);
-        }
-        sh.dst[threadIdx.x] = d;
-    }
+    if (!find_tile<kMxBM>(a, t)) return;
+    if (threadIdx.x < kMxBM) sh.dst[threadIdx.x] = slot_output(a, t, threadIdx.x);
     constexpr bool MX = act_mx(ACT);
     if (t.n <= 16)
         few_tile<ACT>(a, t, sh);
@@ -593,6 +610,157 @@ void mx_group_kernel(MxArgs a) {
         group_tile<ACT, 3, MX ? 4 : 1, MX ? 4 : 2, MX ? 1 : 2>(a, t, sh);
     else
         group_tile<ACT, 4, MX ? 4 : 1, MX ? 4 : 2, MX ? 1 : 2>(a, t, sh);
+}
+
+// ------------------------------------------------------- many 4-bit slots ---
+//
+// Both operands in 4 bits are bound by what feeds the matrix cores: a 64 x 256
+// tile moves 69 bytes a clock and CU at their full rate.  Where there are many
+// slots, a workgroup computes 256 slots by 256 outputs (34 bytes a clock), eight
+// wavefronts of 64 outputs by 128 slots, two a SIMD.  Both operands go straight into
+// LDS, a step of 128 columns at a time, four steps in a ring; a step's weights are
+// read into registers while the step before is multiplied, the slots' three
+// columns of 16 ahead.  (Four wavefronts of 128 x 128 read a third less from LDS but
+// keep their sums in accumulation registers, where the MFMA took 27 clocks
+// against 20.)
+// Its start and end take 10 us in which the CU does nothing else, so it is used
+// where every CU has a tile: 2048 x 8192 (256 tiles), 4096 columns, 46.6 us
+// against 51.9 with tiles of 64; 1000 x 8192 (128 tiles) 40.8 against 27.6.
+constexpr int kBigBM = 256, kBigBN = 256, kBigWaves = 8, kBigRing = 4;
+constexpr uint32_t kBigTiles = 256;
+constexpr int kBigX = 16 * kMxTileBytes;        // [256 slots][64 bytes], chunks at chunk ^ big_swizzle(slot)
+constexpr int kBigWS = kBigX + kBigBM * 64;     // the outputs' words of scales: [4][64]
+constexpr int kBigXS = kBigWS + kBigBN * 4;     // the slots': [256]
+constexpr int kBigStage = kBigXS + kBigBM * 4;
+
+__device__ __forceinline__ uint32_t big_swizzle(uint32_t slot) { return (slot >> 2) & 2u; }
+
+// All but the N loads issued last have landed, this wavefront's LDS reads have
+// returned, and every wavefront is here.
+template <int N>
+__device__ __forceinline__ void wait_stage() {
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
+}
+
+template <int ACT>
+__global__ __launch_bounds__(64 * kBigWaves) __attribute__((amdgpu_waves_per_eu(2)))
+void mx_big_kernel(MxArgs a) {
+    __shared__ __attribute__((aligned(16))) uint8_t lds[kBigRing * kBigStage];
+    __shared__ uint32_t dst[kBigBM];
+    MxTile t;
+    if (!find_tile<kBigBM>(a, t)) return;
+    const uint32_t tid = threadIdx.x, lane = tid & 63u, g = lane >> 4, r = lane & 15u;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6), wr = wave >> 1, wc = wave & 1u;
+    if (tid < kBigBM) dst[tid] = slot_output(a, t, tid);
+    const uint32_t trows = a.rows / kMxRows, steps = a.steps, base = lds_address(lds), blocks = a.K / kMxBlock;
+
+    // this wavefront's loads of a step: two tile rows, 32 slots, and a quarter of
+    // the outputs' scales (wavefronts 0 .. 3) or of the slots'
+    constexpr int LOADS = 5;
+    const uint4_t *wsrc[2];
+    global_ptr xsrc[2];
+    uint32_t chunk[2];
+    const global_ptr zeros = zero_chunk();
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        wsrc[i] = a.tiles + (size_t(t.e) * trows + min(t.n0 / kMxRows + 2 * wave + i, trows - 1u)) * steps * 64 + lane;
+        const uint32_t slot = 32 * wave + 16 * i + lane / 4;
+        chunk[i] = (lane & 3u) ^ big_swizzle(slot);
+        xsrc[i] = global_ptr(a.x) + size_t(slot_row(a, t, slot)) * (a.K / 2) + 16 * chunk[i];
+    }
+    const uint32_t quarter = wave & 3u;
+    const uint8_t *scales;
+    size_t scales_step;
+    if (wave < 4) {
+        scales = reinterpret_cast<const uint8_t *>(
+            a.tscale + (size_t(t.e) * steps * a.quads + min(t.n0 / 64 + quarter, a.quads - 1u)) * 64 + lane);
+        scales_step = size_t(a.quads) * 256;
+    } else {
+        scales = a.xscale + size_t(slot_row(a, t, 64 * quarter + lane)) * a.xscale_stride;
+        scales_step = 4;
+    }
+    const uint32_t scales_at = (wave < 4 ? kBigWS : kBigXS) + quarter * 256;
+    uint32_t issued = 0, to = base;
+    const auto issue = [&]() {  // past the last step: zeros for slots, the last step again for the rest
+#pragma unroll
+        for (int i = 0; i < 2; ++i) to_lds16(to + (2 * wave + i) * kMxTileBytes, wsrc[i]);
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+            to_lds16(to + kBigX + (2 * wave + i) * 1024,
+                     (const void *)(4 * issued + chunk[i] < blocks ? xsrc[i] + size_t(issued) * 64 : zeros));
+        to_lds4(to + scales_at, scales);
+        to = to == base + (kBigRing - 1) * kBigStage ? base : to + kBigStage;
+        if (++issued < steps) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) wsrc[i] += 64;
+            scales += scales_step;
+        }
+    };
+#pragma unroll
+    for (int i = 0; i < kBigRing; ++i) issue();
+
+    float4_t acc[4][8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int c = 0; c < 8; ++c) acc[i][c] = float4_t{0, 0, 0, 0};
+    uint4_t w[2][4], x[4];
+    uint32_t sw[2], sx[4];
+    const uint32_t wat = 4 * wr * kMxTileBytes + 16 * lane, swat = kBigWS + wr * 256 + 4 * lane;
+    const uint32_t xat = kBigX + (128 * wc + r) * 64 + 16 * (g ^ big_swizzle(r)), sxat = kBigXS + (128 * wc + r) * 4;
+    const auto read_w = [&](int buf, int i, const uint8_t *st) {
+        w[buf][i] = load_u4(st + wat + i * kMxTileBytes);
+        if (i == 0) sw[buf] = *reinterpret_cast<const uint32_t *>(st + swat);
+    };
+    const auto read_x = [&](int place, int c, const uint8_t *st) {
+        x[place] = load_u4(st + xat + c * 1024);
+        sx[place] = *reinterpret_cast<const uint32_t *>(st + sxat + c * 64);
+    };
+    wait_stage<(kBigRing - 1) * LOADS>();
+    const uint8_t *st = lds;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) read_w(0, i, st);
+#pragma unroll
+    for (int c = 0; c < 3; ++c) read_x(c, c, st);
+    // Step s: step s + 1 has landed once only the loads of s + 2 and s + 3 are
+    // outstanding.  Step s + 3 goes where s - 1 stood, which all have read by the
+    // barrier at the start of s.
+    for (uint32_t s0 = 0; s0 < steps; s0 += 2) {
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+            if (s0 + b == 0)
+                wait_stage<(kBigRing - 2) * LOADS>();
+            else {
+                wait_stage<(kBigRing - 3) * LOADS>();
+                issue();
+            }
+            const uint8_t *const next = st == lds + (kBigRing - 1) * kBigStage ? lds : st + kBigStage;
+            const bool in = 4 * (s0 + b) + g < blocks;
+#pragma unroll
+            for (int c = 0; c < 8; ++c) {
+                if (c < 4) read_w(b ^ 1, c, next);
+                read_x((c + 3) & 3, (c + 3) & 7, c < 5 ? st : next);
+                __builtin_amdgcn_sched_barrier(0);
+                const uint4_t bx = x[c & 3];
+                const int8v_t bv = {int(bx.x), int(bx.y), int(bx.z), int(bx.w), 0, 0, 0, 0};
+                const uint32_t raw = sx[c & 3] >> (8 * g);
+                const int sb = int(in ? raw : 127u), sa = int(sw[b]);
+                const auto av = [&](int i) {
+                    const uint4_t v = w[b][i];
+                    return int8v_t{int(v.x), int(v.y), int(v.z), int(v.w), 0, 0, 0, 0};
+                };
+                acc[0][c] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(av(0), bv, acc[0][c], 4, 4, 0, sa, 0, sb);
+                acc[1][c] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(av(1), bv, acc[1][c], 4, 4, 1, sa, 0, sb);
+                acc[2][c] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(av(2), bv, acc[2][c], 4, 4, 2, sa, 0, sb);
+                acc[3][c] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(av(3), bv, acc[3][c], 4, 4, 3, sa, 0, sb);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            st = next;
+        }
+    }
+    // no load into LDS may be in flight when the workgroup's LDS is released
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    store_outputs<ACT, 4, 8>(a, t.e, t.n0 + 64 * wr, dst + 128 * wc, acc, lane);
 }
 
 template <int ACT>
@@ -607,6 +775,13 @@ void launch_pairs(const MxArgs &a, hipStream_t stream) {
 template <int ACT>
 void launch_groups(MxArgs a, hipStream_t stream) {
     const uint32_t nblocks = (a.N + kMxBN - 1) / kMxBN;
+    if constexpr (act_mx(ACT)) {
+        const uint32_t tiles = (a.n_slots + kBigBM - 1) / kBigBM;
+        if (!a.offs && tiles * nblocks >= kBigTiles) {
+            hipLaunchKernelGGL((mx_big_kernel<ACT>), dim3{tiles * nblocks}, dim3{64 * kBigWaves}, 0, stream, a);
+            return;
+        }
+    }
     uint32_t mtiles = a.offs ? a.n_slots / kMxBM + min(a.E, a.n_slots) : (a.n_slots + kMxBM - 1) / kMxBM;
     a.set = mtiles >= 64 ? 4 : mtiles >= 8 ? 1 : 0;
     // one matrix, fewer bytes of slots than of weights: the weights stay, a

@@ -345,6 +345,18 @@ def test_linear(device, quantized, rows, out, n):
     assert torch.equal(line.dequantized(F32).cpu(), torch.from_numpy(mxref.values(codes, s)).to(F32))
 
 
+@pytest.mark.parametrize("rows,out,n", ((4096, 4096, 64), (4100, 4097, 160), (8200, 2050, 416)))
+def test_linear_of_many_quantised_rows(device, rows, out, n):
+    """Enough 4-bit rows and outputs for the tiles of 256 x 256, the last ones not whole."""
+    print(f"linear of many rows {rows} {out} {n}", flush=True)
+    rng = np.random.default_rng(rows)
+    codes, s = mxref.random_codes(rng, (out, n))
+    line = mx.MxLinear(out, n, device=device)
+    line.load(mx.MxTensor(_dev(codes, device), _dev(s, device)))
+    x, xv = _operand(rng, rows, n, BF16, True, device)
+    _check(line(x), xv, mxref.values(codes, s)[None], np.zeros(rows, int), BF16)
+
+
 def test_scales_and_codes_of_other_layouts(device):
     """Activations whose scales are contiguous, strided, or a slice with NaN
     scales behind the row; codes at an odd address."""
