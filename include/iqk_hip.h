@@ -328,6 +328,15 @@ int iqk_mx_groups(int act, int64_t in_features, int64_t out_features, int64_t nu
                   const uint8_t *tile_scales, const int32_t *row_exps, const uint32_t *group_offsets,
                   const uint32_t *x_rows, const uint32_t *y_rows, int64_t n_slots, void *y, void *stream);
 
+// A switch module's grouped call in one: iqk_route (wide_ids: iqk_route_ids64)
+// over n_pairs ids, then iqk_mx_groups on its lists, with the outputs and
+// refusals of the two.  work: u32 [2 n_pairs rows_per_pair + num_experts + 1].
+int iqk_mx_prefill(int act, int64_t in_features, int64_t out_features, int64_t num_experts, const void *x,
+                   int64_t n_x_rows, const uint8_t *x_scales, int64_t x_scale_stride, const void *tiles,
+                   const uint8_t *tile_scales, const int32_t *row_exps, const void *ids, int wide_ids,
+                   int64_t n_pairs, int64_t rows_per_pair, int64_t pairs_per_x_row, uint32_t *work, void *y,
+                   void *stream);
+
 // The router's choice: ids[t] the k highest logits of row t in falling order,
 // ties to the lowest expert, NaN above all; weights[t] their softmax, taken over
 // the chosen (normalize) or over the whole row.  A row of -inf gives weights 0.

@@ -881,4 +881,31 @@ int iqk_mx_groups(int act, int64_t in_features, int64_t out_features, int64_t nu
     return record_launch(hipGetLastError());
 }
 
+int iqk_mx_prefill(int act, int64_t in_features, int64_t out_features, int64_t num_experts, const void *x,
+                   int64_t n_x_rows, const uint8_t *x_scales, int64_t x_scale_stride, const void *tiles,
+                   const uint8_t *tile_scales, const int32_t *row_exps, const void *ids, int wide_ids,
+                   int64_t n_pairs, int64_t rows_per_pair, int64_t pairs_per_x_row, uint32_t *work, void *y,
+                   void *stream) {
+    using namespace iqk;
+    constexpr int64_t kLim = int64_t(1) << 31;
+    if (n_pairs < 0 || n_pairs >= kLim || rows_per_pair <= 0 || rows_per_pair >= kLim ||
+        n_pairs * rows_per_pair >= kLim)
+        return IQK_ERR_ARGUMENT;
+    const int64_t slots = n_pairs * rows_per_pair;
+    MxArgs a;  // what the product refuses is refused before the route runs
+    if (const int rc = product_args(a, act, in_features, out_features, num_experts, x, n_x_rows, x_scales,
+                                    x_scale_stride, tiles, tile_scales, row_exps, slots, y);
+        rc != IQK_OK || slots == 0)
+        return rc;
+    if (!ids || !work) return IQK_ERR_ARGUMENT;
+    uint32_t *const x_rows = work, *const y_rows = work + slots, *const offsets = work + 2 * slots;
+    const int rc = wide_ids ? iqk_route_ids64(static_cast<const int64_t *>(ids), n_pairs, num_experts, rows_per_pair,
+                                              pairs_per_x_row, n_x_rows, offsets, x_rows, y_rows, stream)
+                            : iqk_route(static_cast<const uint32_t *>(ids), n_pairs, num_experts, rows_per_pair,
+                                        pairs_per_x_row, n_x_rows, offsets, x_rows, y_rows, stream);
+    if (rc != IQK_OK) return rc;
+    return iqk_mx_groups(act, in_features, out_features, num_experts, x, n_x_rows, x_scales, x_scale_stride, tiles,
+                         tile_scales, row_exps, offsets, x_rows, y_rows, slots, y, stream);
+}
+
 }  // extern "C"

@@ -72,6 +72,9 @@ SIGNATURES = {
                              c_void_p, c_void_p, c_void_p, c_int, c_int64, c_int64, c_void_p, c_void_p]),
     "iqk_mx_groups": (c_int, [c_int, c_int64, c_int64, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p,
                               c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_void_p]),
+    "iqk_mx_prefill": (c_int, [c_int, c_int64, c_int64, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p,
+                               c_void_p, c_void_p, c_void_p, c_int, c_int64, c_int64, c_int64, c_void_p, c_void_p,
+                               c_void_p]),
     "iqk_router_topk": (c_int, [c_int, c_void_p, c_int64, c_int64, c_int64, c_int, c_void_p, c_void_p, c_void_p]),
     "iqk_router_topk_grad": (c_int, [c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int,
                                      c_void_p, c_void_p]),
@@ -142,6 +145,20 @@ def _load_launch(digest: str) -> None:
 def launcher():
     """The CPython launch binding, or None (after :func:`load`)."""
     return _LAUNCH
+
+
+_ENTRIES: dict = {}
+
+
+def entry(name: str):
+    """``iqk_<name>`` as a function of plain integers (addresses, 0 for none),
+    through the CPython binding where it has it, else through ctypes."""
+    fn = _ENTRIES.get(name)
+    if fn is None:
+        lib = load()
+        fn = getattr(_LAUNCH, name, None) or getattr(lib, f"iqk_{name}")
+        _ENTRIES[name] = fn
+    return fn
 
 
 def check(rc: int, what: str) -> None:

@@ -27,7 +27,7 @@ import math
 import torch
 
 from . import _native
-from .kernels import ROUTE_MAX_EXPERTS, IqkKernelError, _require_cuda, _stream_ptr, route_ids
+from .kernels import ROUTE_MAX_EXPERTS, IqkKernelError, _require_cuda, _stream_ptr
 from .nn import _KERNEL_IDS, IqkRuntimeError, _pairs_per_x_row
 
 BLOCK = 32
@@ -69,6 +69,13 @@ class MxTensor:
                                  f"of {BLOCK} values (16 bytes and one scale each)")
         self.codes, self.scales, self.dtype = codes, scales, dtype
 
+    @classmethod
+    def _of(cls, codes: torch.Tensor, scales: torch.Tensor, dtype: torch.dtype) -> "MxTensor":
+        """One of tensors known to belong together."""
+        q = cls.__new__(cls)
+        q.codes, q.scales, q.dtype = codes, scales, dtype
+        return q
+
     @property
     def shape(self) -> torch.Size:
         return torch.Size((*self.codes.shape[:-1], 2 * self.codes.shape[-1]))
@@ -90,12 +97,14 @@ def _new_scales(lead: tuple, n: int, device) -> tuple[torch.Tensor, int]:
     multiple of four, as the products read activations' scales."""
     stride = 4 * ((n + _STEP - 1) // _STEP)
     room = torch.empty((*lead, stride), dtype=torch.uint8, device=device)
-    return room[..., :n // BLOCK] if stride != n // BLOCK else room, stride
+    return (room if stride * BLOCK == n else room[..., :n // BLOCK]), stride
 
 
 def _row_stride(t: torch.Tensor) -> int | None:
     """Elements from row to row of t taken as [rows, n], the last axis dense;
     None where rows are not evenly spaced."""
+    if t.is_contiguous():
+        return t.shape[-1]
     if t.stride(-1) != 1 and t.shape[-1] > 1:
         return None
     stride = span = None
@@ -111,17 +120,19 @@ def _row_stride(t: torch.Tensor) -> int | None:
     return t.shape[-1] if stride is None else stride
 
 
-def _aligned_codes(q: MxTensor) -> torch.Tensor:
-    """Contiguous codes at a 16-byte boundary."""
-    codes = q.codes.contiguous()
+def _aligned_codes(codes: torch.Tensor) -> torch.Tensor:
+    """Codes, contiguous and at a 16-byte boundary."""
+    codes = codes.contiguous()
     return codes if codes.data_ptr() % 16 == 0 else codes.clone()
 
 
 def _product_scales(q: MxTensor) -> tuple[torch.Tensor, int]:
     """Scales as the products read an activation row's, four at a time: rows at
     multiples of four bytes with room for whole groups of four."""
-    n, rows = q.scales.shape[-1], math.prod(q.scales.shape[:-1])
-    need = 4 * ((n + 3) // 4)
+    n = q.scales.shape[-1]
+    if n % 4 == 0 and q.scales.is_contiguous() and q.scales.data_ptr() % 4 == 0:
+        return q.scales, n
+    rows, need = math.prod(q.scales.shape[:-1]), 4 * ((n + 3) // 4)
     stride = _row_stride(q.scales)
     if rows == 1 and stride is not None:
         stride = max(stride, need) // 4 * 4
@@ -143,45 +154,54 @@ def quantize(x: torch.Tensor) -> MxTensor:
     """
     if not isinstance(x, torch.Tensor) or x.dim() < 1:
         raise IqkKernelError("x must be a tensor of at least one dimension")
-    if x.device.type != "cuda":
+    if not x.is_cuda:
         raise IqkKernelError(f"x must live on a GPU, got {x.device}")
-    if x.dtype not in _DTYPES:
-        raise IqkKernelError(f"x must be one of {tuple(_DTYPES)}, got {x.dtype}")
-    n, lead = _check_width(x.shape[-1]), tuple(x.shape[:-1])
+    dtype = x.dtype
+    code = _DTYPES.get(dtype)
+    if code is None:
+        raise IqkKernelError(f"x must be one of {tuple(_DTYPES)}, got {dtype}")
+    *lead, n = x.shape
+    _check_width(n)
+    device, stride, at = x.device, n, x.data_ptr()
+    if not x.is_contiguous() or at % 16:
+        stride = _row_stride(x)
+        if stride is None or stride < n or stride % (16 // x.element_size()) or at % 16:
+            x, stride = x.contiguous(), n
+            if x.data_ptr() % 16:
+                x = x.clone()
+            at = x.data_ptr()
+    codes = torch.empty((*lead, n // 2), dtype=torch.uint8, device=device)
+    scales, scale_stride = _new_scales(lead, n, device)
     rows = math.prod(lead)
-    x = x.detach()
-    per16 = 16 // x.element_size()
-    stride = _row_stride(x)
-    if stride is None or stride < n and rows > 1 or stride % per16 or x.data_ptr() % 16:
-        x, stride = x.contiguous(), n
-        if x.data_ptr() % 16:
-            x = x.clone()
-    codes = torch.empty((*lead, n // 2), dtype=torch.uint8, device=x.device)
-    scales, scale_stride = _new_scales(lead, n, x.device)
     if rows:
-        rc = _native.load().iqk_mx_quantize(_DTYPES[x.dtype], x.data_ptr(), rows, n, stride, codes.data_ptr(),
-                                            scales.data_ptr(), scale_stride, _stream_ptr(x.device))
-        _native.check(rc, f"iqk_mx_quantize({rows}x{n})")
-    return MxTensor(codes, scales, x.dtype)
+        rc = _native.entry("mx_quantize")(code, at, rows, n, stride, codes.data_ptr(), scales.data_ptr(), scale_stride,
+                                          _stream_ptr(device))
+        if rc:
+            _native.check(rc, f"iqk_mx_quantize({rows}x{n})")
+    return MxTensor._of(codes, scales, dtype)
 
 
 def dequantize(q: MxTensor, dtype: torch.dtype | None = None) -> torch.Tensor:
     """The values of ``q``, rounded once to ``dtype`` (its own by default; a
     value is exact in f32 and, but for the smallest scales, in bf16)."""
     dtype = q.dtype if dtype is None else dtype
-    if dtype not in _DTYPES:
+    code = _DTYPES.get(dtype)
+    if code is None:
         raise IqkKernelError(f"dtype must be one of {tuple(_DTYPES)}, got {dtype}")
-    if q.device.type != "cuda":
-        raise IqkKernelError(f"codes must live on a GPU, got {q.device}")
-    n, rows = q.shape[-1], math.prod(q.shape[:-1])
-    codes, scales, stride = _aligned_codes(q), q.scales, _row_stride(q.scales)
+    codes, scales = q.codes, q.scales
+    if not codes.is_cuda:
+        raise IqkKernelError(f"codes must live on a GPU, got {codes.device}")
+    *lead, half = codes.shape
+    n, rows = 2 * half, math.prod(lead)
+    codes, stride = _aligned_codes(codes), _row_stride(scales)
     if stride is None or stride < n // BLOCK:
         scales, stride = scales.contiguous(), n // BLOCK
-    y = torch.empty(q.shape, dtype=dtype, device=q.device)
+    y = torch.empty((*lead, n), dtype=dtype, device=codes.device)
     if rows:
-        rc = _native.load().iqk_mx_dequantize(_DTYPES[dtype], codes.data_ptr(), scales.data_ptr(), rows, n, stride,
-                                              y.data_ptr(), _stream_ptr(q.device))
-        _native.check(rc, f"iqk_mx_dequantize({rows}x{n})")
+        rc = _native.entry("mx_dequantize")(code, codes.data_ptr(), scales.data_ptr(), rows, n, stride, y.data_ptr(),
+                                            _stream_ptr(codes.device))
+        if rc:
+            _native.check(rc, f"iqk_mx_dequantize({rows}x{n})")
     return y
 
 
@@ -217,7 +237,7 @@ class _MxStack(torch.nn.Module):
         if device.type != "cuda":
             raise IqkKernelError(f"the module must live on a GPU to load weights, got {device}")
         q = MxTensor(codes.to(device), scales.to(device))
-        codes, scales, stride = _aligned_codes(q), q.scales, _row_stride(q.scales)
+        codes, scales, stride = _aligned_codes(q.codes), q.scales, _row_stride(q.scales)
         if stride is None or stride < self.in_features // BLOCK:
             scales, stride = scales.contiguous(), self.in_features // BLOCK
         rc = _native.load().iqk_mx_pack(self.in_features, self.out_features, self.num_experts, codes.data_ptr(),
@@ -236,35 +256,38 @@ class _MxStack(torch.nn.Module):
         _native.check(rc, f"iqk_mx_unpack({self.num_experts}x{self.out_features}x{self.in_features})")
         return y
 
-    def _activations(self, x) -> tuple:
+    def _activations(self, x, tiles: torch.Tensor) -> tuple:
         """x's rows as the kernels take them: (act, rows, scales, scale stride, dtype)."""
         mx = isinstance(x, MxTensor)
-        device = self.tiles.device
         if not mx and not isinstance(x, torch.Tensor):
             raise IqkKernelError("x must be a tensor or an MxTensor")
-        if x.device != device or device.type != "cuda":
-            raise IqkKernelError(f"x is on {x.device}, the module on {device}; both must be on one GPU")
+        rows = x.codes if mx else x
+        if not rows.is_cuda or rows.get_device() != tiles.get_device():
+            raise IqkKernelError(f"x is on {x.device}, the module on {tiles.device}; both must be on one GPU")
         act = _ACTS.get((x.dtype, mx))
         if act is None:
             raise IqkKernelError(f"activations are float16 or bfloat16, or quantised from them; got {x.dtype}")
-        if x.shape[-1] != self.in_features:
-            raise IqkRuntimeError(f"x has rows of {x.shape[-1]} values, the weights take {self.in_features}")
+        width = 2 * rows.shape[-1] if mx else rows.shape[-1]
+        if width != self.in_features:
+            raise IqkRuntimeError(f"x has rows of {width} values, the weights take {self.in_features}")
         if mx:
-            scales, stride = _product_scales(x)
-            return act, _aligned_codes(x), scales, stride, x.dtype
-        if x.requires_grad and torch.is_grad_enabled():
+            return (act, _aligned_codes(rows), *_product_scales(x), x.dtype)
+        if rows.requires_grad and torch.is_grad_enabled():
             raise IqkRuntimeError("the weights are frozen and no gradient flows through them: detach x, or call "
                                   "under torch.no_grad()")
-        rows = x.detach().contiguous()
-        return act, rows if rows.data_ptr() % 16 == 0 else rows.clone(), None, 0, x.dtype
+        if not rows.is_contiguous() or rows.data_ptr() % 16:
+            rows = rows.detach().contiguous()
+            rows = rows if rows.data_ptr() % 16 == 0 else rows.clone()
+        return act, rows, None, 0, x.dtype
 
     def _launch(self, entry: str, act, rows, scales, stride, n_x_rows, *args) -> None:
-        rc = getattr(_native.load(), entry)(
+        buffers = self._buffers  # without Module.__getattr__'s lookups
+        rc = _native.entry(entry)(
             act, self.in_features, self.out_features, self.num_experts, rows.data_ptr(), n_x_rows,
-            None if scales is None else scales.data_ptr(), stride, self.tiles.data_ptr(),
-            self.tile_scales.data_ptr(), self.row_exps.data_ptr(), *args, _stream_ptr(rows.device))
+            0 if scales is None else scales.data_ptr(), stride, buffers["tiles"].data_ptr(),
+            buffers["tile_scales"].data_ptr(), buffers["row_exps"].data_ptr(), *args, _stream_ptr(rows.device))
         if rc:
-            _native.check(rc, f"{entry}({self.num_experts}x{self.out_features}x{self.in_features})")
+            _native.check(rc, f"iqk_{entry}({self.num_experts}x{self.out_features}x{self.in_features})")
 
     def extra_repr(self) -> str:
         return f"{self.num_experts}, {self.out_features}, {self.in_features}"
@@ -297,14 +320,18 @@ class MxSwitchLinear(_MxStack):
         ``sorted_indices``) grouped by expert on the device."""
         if len(x.shape) < 2:
             raise IqkRuntimeError(f"x must be [..., M, {self.in_features}], got {tuple(x.shape)}")
-        act, rows, scales, stride, dtype = self._activations(x)
-        xbatch, M = tuple(x.shape[:-2]), int(x.shape[-2])
-        batch = torch.broadcast_shapes(xbatch, tuple(indices.shape))
-        pairs = math.prod(batch)
-        y = torch.empty((*batch, M, self.out_features), dtype=dtype, device=rows.device)
-        if y.numel() == 0:
-            return y
+        tiles = self._buffers["tiles"]
+        act, rows, scales, stride, dtype = self._activations(x, tiles)
+        *xbatch, M, _ = rows.shape
+        batch = indices.shape
         per_row = _pairs_per_x_row(xbatch, batch)
+        if per_row is None:
+            batch = torch.broadcast_shapes(xbatch, batch)
+            per_row = _pairs_per_x_row(xbatch, batch)
+        pairs = math.prod(batch)
+        y = torch.empty((*batch, M, self.out_features), dtype=dtype, device=tiles.device)
+        if not pairs * M:
+            return y
         if per_row is None:  # x broadcasts over leading dimensions: a row of its own for each pair
             rows = rows.expand(*batch, M, rows.shape[-1]).contiguous()
             if scales is not None:
@@ -312,15 +339,18 @@ class MxSwitchLinear(_MxStack):
                 scales, stride = _product_scales(MxTensor(rows, x.scales.expand(*batch, M, n).contiguous()))
             per_row = 1
         n_x_rows = rows.numel() // rows.shape[-1]
-        ids = self._ids(indices, batch)
-        wide = _KERNEL_IDS[ids.dtype]
+        ids = indices
+        wide = _KERNEL_IDS.get(ids.dtype)
+        if wide is None or ids.shape != batch or not ids.is_contiguous() or ids.get_device() != tiles.get_device():
+            ids = self._ids(indices, batch)
+            wide = _KERNEL_IDS[ids.dtype]
         if pairs <= PAIR_LIMIT and M == 1 and not sorted_indices:
-            self._launch("iqk_mx_pairs", act, rows, scales, stride, n_x_rows, ids.data_ptr(), wide, per_row, pairs,
+            self._launch("mx_pairs", act, rows, scales, stride, n_x_rows, ids.data_ptr(), wide, per_row, pairs,
                          y.data_ptr())
             return y
-        offsets, x_rows, y_rows = route_ids(ids, self.num_experts, M, per_row, n_x_rows)
-        self._launch("iqk_mx_groups", act, rows, scales, stride, n_x_rows, offsets.data_ptr(), x_rows.data_ptr(),
-                     y_rows.data_ptr(), pairs * M, y.data_ptr())
+        work = torch.empty(2 * pairs * M + self.num_experts + 1, dtype=torch.int32, device=tiles.device)
+        self._launch("mx_prefill", act, rows, scales, stride, n_x_rows, ids.data_ptr(), wide, pairs, M, per_row,
+                     work.data_ptr(), y.data_ptr())
         return y
 
     def _ids(self, indices: torch.Tensor, batch) -> torch.Tensor:
@@ -357,15 +387,17 @@ class MxLinear(_MxStack):
         return self._dequantized(dtype)[0]
 
     def forward(self, x) -> torch.Tensor:
-        act, rows, scales, stride, dtype = self._activations(x)
-        n = rows.numel() // rows.shape[-1]
-        y = torch.empty((*x.shape[:-1], self.out_features), dtype=dtype, device=rows.device)
+        tiles = self._buffers["tiles"]
+        act, rows, scales, stride, dtype = self._activations(x, tiles)
+        *lead, width = rows.shape
+        n = math.prod(lead)
+        y = torch.empty((*lead, self.out_features), dtype=dtype, device=tiles.device)
         if n == 0:
             return y
         if n <= 4:
-            self._launch("iqk_mx_pairs", act, rows, scales, stride, n, None, 0, 1, n, y.data_ptr())
+            self._launch("mx_pairs", act, rows, scales, stride, n, 0, 0, 1, n, y.data_ptr())
         else:
-            self._launch("iqk_mx_groups", act, rows, scales, stride, n, None, None, None, n, y.data_ptr())
+            self._launch("mx_groups", act, rows, scales, stride, n, 0, 0, 0, n, y.data_ptr())
         return y
 
     def extra_repr(self) -> str:

@@ -25,7 +25,7 @@ MAX_K = 64
 def _check_logits(logits: torch.Tensor, dims: int) -> int:
     if not isinstance(logits, torch.Tensor) or logits.dim() < dims:
         raise IqkKernelError(f"logits must be a tensor of at least {dims} dimensions")
-    if logits.device.type != "cuda":
+    if not logits.is_cuda:
         raise IqkKernelError(f"logits must live on a GPU, got {logits.device}")
     if logits.dtype not in _DTYPES:
         raise IqkKernelError(f"logits must be one of {tuple(_DTYPES)}, got {logits.dtype}")
@@ -39,9 +39,9 @@ def _topk(logits: torch.Tensor, k: int, normalize: bool) -> tuple[torch.Tensor, 
     shape, device = (*logits.shape[:-1], k), logits.device
     weights = torch.empty(shape, dtype=torch.float32, device=device)
     ids = torch.empty(shape, dtype=torch.int32, device=device)
-    rc = _native.load().iqk_router_topk(_DTYPES[logits.dtype], logits.data_ptr(), weights.numel() // k,
-                                        logits.shape[-1], k, normalize, weights.data_ptr(), ids.data_ptr(),
-                                        _stream_ptr(device))
+    rc = _native.entry("router_topk")(_DTYPES[logits.dtype], logits.data_ptr(), weights.numel() // k,
+                                      logits.shape[-1], k, normalize, weights.data_ptr(), ids.data_ptr(),
+                                      _stream_ptr(device))
     if rc:
         _native.check(rc, f"iqk_router_topk({tuple(logits.shape)}, {k})")
     return weights, ids
@@ -66,8 +66,8 @@ class _TopK(torch.autograd.Function):
         dweights = dweights.to(torch.float32).contiguous()
         dlogits = torch.empty(ctx.shape, dtype=ctx.dtype, device=weights.device)
         k = weights.shape[-1]
-        rc = _native.load().iqk_router_topk_grad(
-            _DTYPES[ctx.dtype], rest[0].data_ptr() if rest else None, weights.data_ptr(), ids.data_ptr(),
+        rc = _native.entry("router_topk_grad")(
+            _DTYPES[ctx.dtype], rest[0].data_ptr() if rest else 0, weights.data_ptr(), ids.data_ptr(),
             dweights.data_ptr(), weights.numel() // k, ctx.shape[-1], k, ctx.normalize, dlogits.data_ptr(),
             _stream_ptr(weights.device))
         if rc:
@@ -98,16 +98,15 @@ def topk(logits: torch.Tensor, k: int, *, normalize: bool = True) -> tuple[torch
 def _balance(logits, ids, mask):
     *lead, tokens, experts = logits.shape
     groups, device = math.prod(lead), logits.device
-    lib = _native.load()
     loss = torch.empty(lead, dtype=torch.float32, device=device)
     counts = torch.empty((*lead, experts), dtype=torch.int32, device=device)
     kept = torch.empty(lead, dtype=torch.int32, device=device)
     if groups:
-        work = torch.empty(lib.iqk_balance_work(groups, tokens, experts), dtype=torch.int32, device=device)
-        rc = lib.iqk_balance(_DTYPES[logits.dtype], logits.data_ptr(), ids.data_ptr(),
-                             None if mask is None else mask.data_ptr(), groups, tokens, experts, ids.shape[-1],
-                             work.data_ptr(), loss.data_ptr(), counts.data_ptr(), kept.data_ptr(),
-                             _stream_ptr(device))
+        work = torch.empty(_native.entry("balance_work")(groups, tokens, experts), dtype=torch.int32, device=device)
+        rc = _native.entry("balance")(_DTYPES[logits.dtype], logits.data_ptr(), ids.data_ptr(),
+                                      0 if mask is None else mask.data_ptr(), groups, tokens, experts,
+                                      ids.shape[-1], work.data_ptr(), loss.data_ptr(), counts.data_ptr(),
+                                      kept.data_ptr(), _stream_ptr(device))
         if rc:
             _native.check(rc, f"iqk_balance({tuple(logits.shape)}, {ids.shape[-1]})")
     return loss, counts, kept
@@ -132,8 +131,8 @@ class _Balance(torch.autograd.Function):
         dloss = dloss.to(torch.float32).contiguous()
         dlogits = torch.empty_like(logits)
         *lead, tokens, experts = logits.shape
-        rc = _native.load().iqk_balance_grad(
-            _DTYPES[logits.dtype], logits.data_ptr(), None if mask is None else mask.data_ptr(), counts.data_ptr(),
+        rc = _native.entry("balance_grad")(
+            _DTYPES[logits.dtype], logits.data_ptr(), 0 if mask is None else mask.data_ptr(), counts.data_ptr(),
             kept.data_ptr(), dloss.data_ptr(), math.prod(lead), tokens, experts, ctx.k, dlogits.data_ptr(),
             _stream_ptr(logits.device))
         if rc:

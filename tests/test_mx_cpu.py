@@ -79,6 +79,43 @@ def test_product_entry_points_refuse_bad_arguments(lib):
     assert pairs(pairs=0) == OK and groups(slots=0) == OK
 
 
+def test_grouped_call_refuses_bad_arguments(lib):
+    def prefill(act=0, n=64, out=16, experts=2, x=P, rows=4, ids=P, pairs=4, per_pair=1, per_row=1, work=P, y=P):
+        return lib.iqk_mx_prefill(act, n, out, experts, x, rows, None, 0, P, P, P, ids, 0, pairs, per_pair, per_row,
+                                  work, y, None)
+
+    for bad in (dict(act=4), dict(experts=4097), dict(x=None), dict(y=None), dict(ids=None), dict(work=None),
+                dict(per_pair=0), dict(per_row=0), dict(pairs=-1), dict(pairs=1 << 20, per_pair=1 << 20),
+                dict(rows=3), dict(act=2)):
+        assert prefill(**bad) == ARGUMENT, bad
+    assert prefill(n=48) == GEOMETRY and prefill(pairs=0) == OK
+
+
+def test_launch_binding_reaches_the_same_entry_points(lib):
+    """The binding's functions give the entry points' refusals, and refuse
+    arguments that a C int would cut."""
+    fast = _native.launcher()
+    assert fast is not None, "the launch binding is built beside the library by build()"
+    for name in ("mx_quantize", "mx_dequantize", "mx_pairs", "mx_groups", "mx_prefill", "router_topk",
+                 "router_topk_grad", "balance_work", "balance", "balance_grad"):
+        assert _native.entry(name) is getattr(fast, name)
+        with pytest.raises(TypeError):
+            getattr(fast, name)(0)
+    assert fast.mx_quantize(0, P, 4, 33, 33, P, P, 8, 0) == GEOMETRY
+    assert fast.mx_dequantize(0, P, P, 4, 33, 8, P, 0) == GEOMETRY
+    assert fast.mx_pairs(4, 64, 16, 2, P, 4, 0, 0, P, P, P, P, 0, 1, 4, P, 0) == ARGUMENT
+    assert fast.mx_groups(0, 48, 16, 2, P, 4, 0, 0, P, P, P, P, P, P, 4, P, 0) == GEOMETRY
+    assert fast.mx_prefill(0, 64, 16, 2, P, 4, 0, 0, P, P, P, P, 0, 4, 1, 1, 0, P, 0) == ARGUMENT
+    assert fast.router_topk(0, P, 4, 8, 9, 1, P, P, 0) == GEOMETRY
+    assert fast.router_topk_grad(0, 0, P, P, P, 4, 8, 2, 0, P, 0) == ARGUMENT
+    assert fast.balance_work(2, 33, 8) == lib.iqk_balance_work(2, 33, 8)
+    assert fast.balance(0, P, 0, 0, 1, 4, 8, 2, P, P, P, P, 0) == ARGUMENT
+    assert fast.balance_grad(0, P, 0, P, 0, P, 1, 4, 8, 2, P, 0) == ARGUMENT
+    for bad in ((1 << 32, P, 4, 64, 64, P, P, 2, 0), (-1 << 40, P, 4, 64, 64, P, P, 2, 0)):
+        with pytest.raises(OverflowError):
+            fast.mx_quantize(*bad)
+
+
 def test_router_entry_points_refuse_bad_arguments(lib):
     topk, grad = lib.iqk_router_topk, lib.iqk_router_topk_grad
     for rows, experts, k in ((4, 0, 1), (4, 1025, 1), (4, 8, 0), (4, 8, 9), (4, 100, 65), (-1, 8, 1), (1 << 31, 8, 1)):
