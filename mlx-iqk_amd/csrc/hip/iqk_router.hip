@@ -2,8 +2,9 @@
 // balance loss and its gradient.  Logits are [tokens, experts], experts <= 1024.
 //
 // Every kernel reads a token's logits once, 16 lanes a token (four tokens a
-// wavefront), a lane VPT consecutive ones in registers, and reduces over the 16
-// lanes by row rotations.  All arithmetic is f32.
+// wavefront), and reduces over the 16 lanes by row rotations, which cost an
+// instruction each; a lane holds VPT logits in registers, four consecutive ones at
+// every 64th, so that 16 lanes read 64 in one piece.  All arithmetic is f32.
 
 #include <type_traits>
 
@@ -28,19 +29,24 @@ __device__ __forceinline__ float rotate(float x) {
     return __builtin_bit_cast(float, rotate<N>(__builtin_bit_cast(uint32_t, x)));
 }
 
-__device__ __forceinline__ uint32_t row_max(uint32_t v) {
-    v = max(v, rotate<8>(v));
-    v = max(v, rotate<4>(v));
-    v = max(v, rotate<2>(v));
-    return max(v, rotate<1>(v));
+template <typename T, typename F>
+__device__ __forceinline__ T row_reduce(T v, F f) {
+    v = f(v, rotate<8>(v));
+    v = f(v, rotate<4>(v));
+    v = f(v, rotate<2>(v));
+    return f(v, rotate<1>(v));
 }
-
-// The same value in all 16 lanes: each step adds the two halves of a ring.
+__device__ __forceinline__ uint32_t row_max(uint32_t v) {
+    return row_reduce(v, [](uint32_t a, uint32_t b) { return max(a, b); });
+}
+__device__ __forceinline__ uint32_t row_min(uint32_t v) {
+    return row_reduce(v, [](uint32_t a, uint32_t b) { return min(a, b); });
+}
+__device__ __forceinline__ float row_max(float v) {
+    return row_reduce(v, [](float a, float b) { return fmaxf(a, b); });
+}
 __device__ __forceinline__ float row_sum(float v) {
-    v += rotate<8>(v);
-    v += rotate<4>(v);
-    v += rotate<2>(v);
-    return v + rotate<1>(v);
+    return row_reduce(v, [](float a, float b) { return a + b; });
 }
 
 // exp(x) for x <= 0 or NaN: 2^(x log2 e) with the product's rounding error put back.
@@ -53,13 +59,6 @@ __device__ __forceinline__ float exp_neg(float x) {
 }
 
 template <int DT>
-__device__ __forceinline__ float value_at(const void *p, size_t i) {
-    if constexpr (DT == MX_F32) return static_cast<const float *>(p)[i];
-    const uint32_t u = static_cast<const uint16_t *>(p)[i];
-    return DT == MX_F16 ? half_bits_to_float(u) : __builtin_bit_cast(float, u << 16);
-}
-
-template <int DT>
 __device__ __forceinline__ void put_at(void *p, size_t i, float v) {
     if constexpr (DT == MX_F32)
         static_cast<float *>(p)[i] = v;
@@ -67,49 +66,82 @@ __device__ __forceinline__ void put_at(void *p, size_t i, float v) {
         static_cast<uint16_t *>(p)[i] = uint16_t(DT == MX_F16 ? float_to_half_bits(v) : bf16_bits(v));
 }
 
-// The lane's VPT logits of a row, `none` past E.  quads: E is a multiple of
-// four and rows are aligned to four elements.
+// The expert at place i of lane j.  QUADS: experts are a multiple of four and
+// rows aligned to four of them; else a lane holds every 16th.
+template <bool QUADS>
+__device__ __forceinline__ constexpr uint32_t expert_of(uint32_t i, uint32_t j) {
+    return QUADS ? (i / 4 * kRowLanes + j) * 4 + i % 4 : i * kRowLanes + j;
+}
+
+// The lane's VPT logits of a row as they stand (16-bit ones two a word).
 template <int DT, int VPT>
-__device__ __forceinline__ void load_row(const void *x, size_t row, uint32_t E, uint32_t j, bool quads, float none,
-                                         float (&v)[VPT]) {
+using RowWords = uint32_t[DT == MX_F32 ? VPT : VPT / 2];
+
+template <int DT, int VPT, bool QUADS>
+__device__ __forceinline__ void load_words(const void *x, size_t row, uint32_t E, uint32_t j,
+                                           RowWords<DT, VPT> &v) {
     const size_t base = row * E;
-    if (quads) {
+    if constexpr (QUADS) {
 #pragma unroll
-        for (int q = 0; q < VPT; q += 4) {
-            const uint32_t e = j * VPT + q;
-            const bool in = e < E;
-            const size_t at = base + (in ? e : 0u);
+        for (int q = 0; q < VPT / 4; ++q) {
+            const uint32_t e = expert_of<true>(4 * q, j);
+            const size_t at = base + (e < E ? e : 0u);  // past the end: any, masked at use
             if constexpr (DT == MX_F32) {
-                const float4_t f = *reinterpret_cast<const float4_t *>(static_cast<const float *>(x) + at);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) v[q + i] = in ? f[i] : none;
+                const uint4_t w = load_u4(static_cast<const float *>(x) + at);
+                v[4 * q] = w.x, v[4 * q + 1] = w.y, v[4 * q + 2] = w.z, v[4 * q + 3] = w.w;
             } else {
-                const uint2_t u = *reinterpret_cast<const uint2_t *>(static_cast<const uint16_t *>(x) + at);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const uint32_t w = i < 2 ? u.x : u.y, h = i & 1 ? w >> 16 : w & 0xffffu;
-                    const float f = DT == MX_F16 ? half_bits_to_float(h) : __builtin_bit_cast(float, h << 16);
-                    v[q + i] = in ? f : none;
-                }
+                const uint2_t w = *reinterpret_cast<const uint2_t *>(static_cast<const uint16_t *>(x) + at);
+                v[2 * q] = w.x, v[2 * q + 1] = w.y;
             }
         }
     } else {
 #pragma unroll
         for (int i = 0; i < VPT; ++i) {
-            const uint32_t e = j * VPT + i;
-            v[i] = e < E ? value_at<DT>(x, base + (e < E ? e : 0u)) : none;
+            const uint32_t e = expert_of<false>(i, j);
+            const size_t at = base + (e < E ? e : 0u);
+            if constexpr (DT == MX_F32) {
+                v[i] = static_cast<const uint32_t *>(x)[at];
+            } else {
+                const uint32_t h = static_cast<const uint16_t *>(x)[at];
+                v[i / 2] = i & 1 ? v[i / 2] | h << 16 : h;
+            }
         }
     }
 }
 
-template <int DT, int VPT>
-__device__ __forceinline__ void store_row(void *y, size_t row, uint32_t E, uint32_t j, bool quads,
-                                          const float (&v)[VPT]) {
+// A 16-bit logit's bits.
+template <int VPT>
+__device__ __forceinline__ uint32_t half_of(const uint32_t (&v)[VPT], int i) {
+    return i & 1 ? v[i / 2] >> 16 : v[i / 2] & 0xffffu;
+}
+
+template <int DT>
+__device__ __forceinline__ float float_of(uint32_t bits) {
+    return DT == MX_F32 ? __builtin_bit_cast(float, bits)
+           : DT == MX_F16 ? half_bits_to_float(bits) : __builtin_bit_cast(float, bits << 16);
+}
+
+// As floats, -inf past E.
+template <int DT, int VPT, bool QUADS>
+__device__ __forceinline__ void to_floats(const RowWords<DT, VPT> &w, uint32_t E, uint32_t j, float (&v)[VPT]) {
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+        uint32_t bits;
+        if constexpr (DT == MX_F32)
+            bits = w[i];
+        else
+            bits = half_of(w, i);
+        v[i] = expert_of<QUADS>(i, j) < E ? float_of<DT>(bits) : -__builtin_inff();
+    }
+}
+
+template <int DT, int VPT, bool QUADS>
+__device__ __forceinline__ void store_row(void *y, size_t row, uint32_t E, uint32_t j, const float (&v)[VPT]) {
     const size_t base = row * E;
-    if (quads) {
+    if constexpr (QUADS) {
 #pragma unroll
         for (int q = 0; q < VPT; q += 4) {
-            const uint32_t e = j * VPT + q;
+            const uint32_t e = expert_of<true>(q, j);
             if (e >= E) continue;
             if constexpr (DT == MX_F32) {
                 *reinterpret_cast<float4_t *>(static_cast<float *>(y) + base + e) =
@@ -125,7 +157,7 @@ __device__ __forceinline__ void store_row(void *y, size_t row, uint32_t E, uint3
     } else {
 #pragma unroll
         for (int i = 0; i < VPT; ++i)
-            if (j * VPT + i < E) put_at<DT>(y, base + j * VPT + i, v[i]);
+            if (expert_of<false>(i, j) < E) put_at<DT>(y, base + expert_of<false>(i, j), v[i]);
     }
 }
 
@@ -139,14 +171,29 @@ __device__ __forceinline__ float key_value(uint32_t k) {
     return __builtin_bit_cast(float, k >> 31 ? k == 0xffffffffu ? 0x7fc00000u : k & 0x7fffffffu : ~k);
 }
 
+// The same of a 16-bit float's bits, in the high half; the low half orders
+// experts, the lowest highest, so that no two keys are equal.
+template <int DT>
+__device__ __forceinline__ uint32_t order_key16(uint32_t h, uint32_t e) {
+    constexpr uint32_t kInf = DT == MX_F16 ? 0x7c00u : 0x7f80u;
+    const uint32_t m = h & 0x7fffu;
+    const uint32_t k = m > kInf ? 0xffffu : (h >> 15) ? 0x8000u - m : 0x8000u + m;  // -0 is +0
+    return k << 16 | (0xffffu - e);
+}
+template <int DT>
+__device__ __forceinline__ float key16_value(uint32_t key) {
+    const uint32_t k = key >> 16;
+    return float_of<DT>(k == 0xffffu ? 0x7fffu : k >= 0x8000u ? k - 0x8000u : (0x8000u - k) | 0x8000u);
+}
+
 // v -> softmax over the row's 16 lanes, in place (none of it where every
-// logit is -inf: zeros).  Lanes' places past E hold -inf.
+// logit is -inf: zeros).  A NaN makes the sum, and so the row, NaN.
 template <int VPT>
 __device__ __forceinline__ void row_softmax(float (&v)[VPT]) {
-    uint32_t m = 0;
+    float top = v[0];
 #pragma unroll
-    for (int i = 0; i < VPT; ++i) m = max(m, order_key(v[i]));
-    const float top = key_value(row_max(m));
+    for (int i = 1; i < VPT; ++i) top = fmaxf(top, v[i]);
+    top = row_max(top);
     float s = 0.f;
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
@@ -154,10 +201,10 @@ __device__ __forceinline__ void row_softmax(float (&v)[VPT]) {
         s += v[i];
     }
     s = row_sum(s);
+    const bool none = top == -__builtin_inff();
     const float inv = 1.0f / s;
-    const bool empty = top == -__builtin_inff();
 #pragma unroll
-    for (int i = 0; i < VPT; ++i) v[i] = empty ? 0.f : v[i] * inv;
+    for (int i = 0; i < VPT; ++i) v[i] = none ? 0.f : v[i] * inv;
 }
 
 // -------------------------------------------------------------------- top k ---
@@ -169,23 +216,31 @@ struct TopkArgs {
     const float *dweights;
     void *dlogits;
     uint32_t rows, E, k;
-    uint32_t quads;
 };
 
 // The k highest logits, ties to the lowest expert, and their softmax weights:
-// over the chosen (NORM) or over all.  k rounds of a maximum over the row;
-// lanes hold consecutive experts, so of the lanes that hold the maximum the
-// lowest has the lowest expert.
-template <int DT, int VPT, bool NORM>
+// over the chosen (NORM) or over all.  k rounds of a maximum over the row.
+// 16-bit logits and their expert make one key, so that a round compares,
+// removes and finds the expert with three instructions a logit; f32 logits
+// need five, the lowest of the experts that hold the maximum being a second
+// reduction.
+template <int DT, int VPT, bool NORM, bool QUADS>
 __global__ __launch_bounds__(256) void topk_kernel(TopkArgs a) {
+    constexpr bool WIDE = DT == MX_F32;
     const uint32_t lane = threadIdx.x & 63u, j = lane & 15u;
     const uint32_t row = (blockIdx.x * 256 + threadIdx.x) / kRowLanes;
     const bool live = row < a.rows;
-    float v[VPT];
-    load_row<DT, VPT>(a.logits, live ? row : 0u, a.E, j, a.quads, -__builtin_inff(), v);
+    RowWords<DT, VPT> words;
+    load_words<DT, VPT, QUADS>(a.logits, live ? row : 0u, a.E, j, words);
     uint32_t key[VPT];
 #pragma unroll
-    for (int i = 0; i < VPT; ++i) key[i] = j * VPT + i < a.E ? order_key(v[i]) : 0u;
+    for (int i = 0; i < VPT; ++i) {
+        const uint32_t e = expert_of<QUADS>(i, j);
+        if constexpr (WIDE)
+            key[i] = e < a.E ? order_key(float_of<DT>(words[i])) : 0u;
+        else
+            key[i] = e < a.E ? order_key16<DT>(half_of(words, i), e) : 0u;
+    }
     float chosen[4];  // lane j: choices j, 16 + j, ..
     int32_t id[4];
     float top = 0.f, sum = 0.f;
@@ -198,24 +253,33 @@ __global__ __launch_bounds__(256) void topk_kernel(TopkArgs a) {
 #pragma unroll
             for (int i = 1; i < VPT; ++i) m = max(m, key[i]);
             const uint32_t best = row_max(m);
-            const uint32_t has = uint32_t(__ballot(m == best) >> (lane & 48u)) & 0xffffu;
-            const uint32_t win = uint32_t(__ffs(int(has))) - 1u;
-            int32_t at = 0;
+            uint32_t e;
+            float value;
+            if constexpr (WIDE) {
+                uint32_t at = 0xffffu;
 #pragma unroll
-            for (int i = VPT - 1; i >= 0; --i) at = key[i] == best ? i : at;
-            const int32_t e = __shfl(int32_t(j) * VPT + at, int(win), kRowLanes);
+                for (int i = VPT - 1; i >= 0; --i) at = key[i] == best ? uint32_t(expert_of<QUADS>(i, j)) : at;
+                e = row_min(at);
 #pragma unroll
-            for (int i = 0; i < VPT; ++i) key[i] = j == win && i == at ? 0u : key[i];
-            const float value = key_value(best);
+                for (int i = 0; i < VPT; ++i) key[i] = expert_of<QUADS>(i, j) == e ? 0u : key[i];
+                value = key_value(best);
+            } else {
+#pragma unroll
+                for (int i = 0; i < VPT; ++i) key[i] = key[i] == best ? 0u : key[i];
+                e = 0xffffu - (best & 0xffffu);
+                value = key16_value<DT>(best);
+            }
             if (q == 0 && c == 0) top = value;
             if constexpr (NORM) sum += exp_neg(value - top);
             if (j == c) {
                 chosen[q] = value;
-                id[q] = e;
+                id[q] = int32_t(e);
             }
         }
     }
     if constexpr (!NORM) {
+        float v[VPT];
+        to_floats<DT, VPT, QUADS>(words, a.E, j, v);
 #pragma unroll
         for (int i = 0; i < VPT; ++i) sum += exp_neg(v[i] - top);
         sum = row_sum(sum);
@@ -235,7 +299,7 @@ __global__ __launch_bounds__(256) void topk_kernel(TopkArgs a) {
 //   NORM      w_i (dw_i - D) at the chosen, 0 elsewhere
 //   otherwise p_e (dw_e - D), dw_e = 0 where e was not chosen.
 // The chosen's values meet their place in the row through LDS.
-template <int DT, int VPT, bool NORM>
+template <int DT, int VPT, bool NORM, bool QUADS>
 __global__ __launch_bounds__(256) void topk_grad_kernel(TopkArgs a) {
     constexpr int PLACES = kRowLanes * VPT;
     __shared__ __attribute__((aligned(16))) float place[16][PLACES];
@@ -256,24 +320,38 @@ __global__ __launch_bounds__(256) void topk_grad_kernel(TopkArgs a) {
         if (in) dot += w[q] * dw[q];
     }
     dot = row_sum(dot);
+    // a row's places are written and read by the 16 lanes of one wavefront
+    // only, whose LDS operations stay in order
 #pragma unroll
-    for (int i = 0; i < VPT; ++i) place[r][j * VPT + i] = 0.f;
-    __syncthreads();
+    for (int q = 0; q < VPT / 4; ++q)
+        *reinterpret_cast<float4_t *>(&place[r][(q * kRowLanes + j) * 4]) = float4_t{0, 0, 0, 0};
+    __builtin_amdgcn_wave_barrier();
 #pragma unroll
     for (int q = 0; q < 4; ++q)
         if (uint32_t(id[q]) < a.E) place[r][id[q]] = NORM ? w[q] * (dw[q] - dot) : dw[q];
-    __syncthreads();
+    __builtin_amdgcn_wave_barrier();
     float d[VPT];
+    if constexpr (QUADS) {
 #pragma unroll
-    for (int i = 0; i < VPT; ++i) d[i] = place[r][j * VPT + i];
+        for (int q = 0; q < VPT / 4; ++q) {
+            const float4_t v = *reinterpret_cast<const float4_t *>(&place[r][(q * kRowLanes + j) * 4]);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) d[4 * q + i] = v[i];
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < VPT; ++i) d[i] = place[r][expert_of<false>(i, j)];
+    }
     if constexpr (!NORM) {
+        RowWords<DT, VPT> words;
+        load_words<DT, VPT, QUADS>(a.logits, live ? row : 0u, a.E, j, words);
         float p[VPT];
-        load_row<DT, VPT>(a.logits, live ? row : 0u, a.E, j, a.quads, -__builtin_inff(), p);
+        to_floats<DT, VPT, QUADS>(words, a.E, j, p);
         row_softmax<VPT>(p);
 #pragma unroll
         for (int i = 0; i < VPT; ++i) d[i] = p[i] * (d[i] - dot);
     }
-    if (live) store_row<DT, VPT>(a.dlogits, row, a.E, j, a.quads, d);
+    if (live) store_row<DT, VPT, QUADS>(a.dlogits, row, a.E, j, d);
 }
 
 // ------------------------------------------------------------- balance loss ---
@@ -298,10 +376,11 @@ struct BalanceArgs {
     int32_t *kept;
     const float *dloss;
     void *dlogits;
-    uint32_t T, E, k, shares, share, quads;  // share: tokens of one
+    uint32_t T, E, k, shares, share;  // share: tokens of one
 };
 
-template <int DT, int VPT>
+// A wavefront loads its next four tokens before it works on the ones it has.
+template <int DT, int VPT, bool QUADS>
 __global__ __launch_bounds__(kBalanceThreads) void balance_sums_kernel(BalanceArgs a) {
     constexpr int PLACES = kRowLanes * VPT;
     __shared__ float sums[kBalanceThreads / 64][PLACES];
@@ -316,17 +395,17 @@ __global__ __launch_bounds__(kBalanceThreads) void balance_sums_kernel(BalanceAr
     float s[VPT];
 #pragma unroll
     for (int i = 0; i < VPT; ++i) s[i] = 0.f;
+    const auto row_of = [&](uint32_t t) { return size_t(group) * a.T + (t < hi ? t : lo); };
+    RowWords<DT, VPT> words;
+    uint32_t t = lo + tid / kRowLanes;
+    if (lo < hi) load_words<DT, VPT, QUADS>(a.logits, row_of(t), a.E, j, words);
     uint32_t mine = 0;
-    for (uint32_t t0 = lo; t0 < hi; t0 += kBalanceRows) {
-        const uint32_t t = t0 + tid / kRowLanes;
-        const bool in = t < hi;
-        const size_t row = size_t(group) * a.T + (in ? t : lo);
-        const bool keep = in && (!a.mask || a.mask[row]);
+    for (uint32_t t0 = lo; t0 < hi; t0 += kBalanceRows, t += kBalanceRows) {
         float p[VPT];
-        load_row<DT, VPT>(a.logits, row, a.E, j, a.quads, -__builtin_inff(), p);
-        row_softmax<VPT>(p);
-#pragma unroll
-        for (int i = 0; i < VPT; ++i) s[i] += keep ? p[i] : 0.f;
+        to_floats<DT, VPT, QUADS>(words, a.E, j, p);
+        load_words<DT, VPT, QUADS>(a.logits, row_of(t + kBalanceRows), a.E, j, words);
+        const size_t row = row_of(t);
+        const bool keep = t < hi && (!a.mask || a.mask[row]);
         if (keep) {
             for (uint32_t c = j; c < a.k; c += kRowLanes) {
                 const uint32_t e = uint32_t(a.ids[row * a.k + c]);
@@ -334,6 +413,9 @@ __global__ __launch_bounds__(kBalanceThreads) void balance_sums_kernel(BalanceAr
             }
             mine += j == 0;
         }
+        row_softmax<VPT>(p);
+#pragma unroll
+        for (int i = 0; i < VPT; ++i) s[i] += keep ? p[i] : 0.f;
     }
     if (mine) atomicAdd(&kept, int32_t(mine));
     // the four rows of a wavefront, then the wavefronts
@@ -341,7 +423,7 @@ __global__ __launch_bounds__(kBalanceThreads) void balance_sums_kernel(BalanceAr
     for (int i = 0; i < VPT; ++i) {
         s[i] += __shfl_xor(s[i], 16, 64);
         s[i] += __shfl_xor(s[i], 32, 64);
-        if (lane < 16) sums[wave][j * VPT + i] = s[i];
+        if (lane < 16) sums[wave][expert_of<QUADS>(i, j)] = s[i];
     }
     __syncthreads();
     const size_t at = size_t(group) * a.shares + share;
@@ -355,82 +437,139 @@ __global__ __launch_bounds__(kBalanceThreads) void balance_sums_kernel(BalanceAr
     if (tid == 0) a.pkept[at] = kept;
 }
 
-__global__ __launch_bounds__(1024) void balance_join_kernel(BalanceArgs a) {
-    __shared__ float part[16];
-    const uint32_t tid = threadIdx.x, group = blockIdx.x;
+// One workgroup a group: `slices` threads an expert, each over every slices-th
+// share, four loads of both sums in flight.
+constexpr int kJoinThreads = 1024;
+
+__global__ __launch_bounds__(kJoinThreads) void balance_join_kernel(BalanceArgs a) {
+    __shared__ float vsum[kJoinThreads];
+    __shared__ int32_t csum[kJoinThreads];
+    __shared__ float part[kJoinThreads / 64];
+    __shared__ int32_t npart[kJoinThreads / 64];
+    const uint32_t tid = threadIdx.x, lane = tid & 63u, group = blockIdx.x;
     const size_t base = size_t(group) * a.shares;
     int32_t n = 0;
-    for (uint32_t s = 0; s < a.shares; ++s) n += a.pkept[base + s];
-    float dot = 0.f;
-    for (uint32_t e = tid; e < a.E; e += 1024) {
-        float v = 0.f;
-        int32_t c = 0;
-        for (uint32_t s = 0; s < a.shares; ++s) {
-            v += a.psum[(base + s) * a.E + e];
-            c += a.pcount[(base + s) * a.E + e];
+    for (uint32_t s = tid; s < a.shares; s += kJoinThreads) n += a.pkept[base + s];
+    const uint32_t wide = (a.E + 63u) & ~63u, slices = kJoinThreads / wide;
+    const uint32_t slice = tid / wide, e = tid % wide;
+    float v = 0.f;
+    int32_t c = 0;
+    if (slice < slices && e < a.E) {
+        for (uint32_t s0 = slice; s0 < a.shares; s0 += 4 * slices) {
+            float lv[4];
+            int32_t lc[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint32_t s = s0 + i * slices;
+                const size_t at = (base + (s < a.shares ? s : slice)) * a.E + e;
+                lv[i] = a.psum[at];
+                lc[i] = a.pcount[at];
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const bool in = s0 + i * slices < a.shares;
+                v += in ? lv[i] : 0.f;
+                c += in ? lc[i] : 0;
+            }
         }
-        a.counts[size_t(group) * a.E + e] = c;
-        dot += float(c) * v;
+    }
+    vsum[tid] = v;
+    csum[tid] = c;
+    __syncthreads();
+    float dot = 0.f;
+    if (tid < a.E) {
+        for (uint32_t i = 1; i < slices; ++i) {
+            v += vsum[i * wide + tid];
+            c += csum[i * wide + tid];
+        }
+        a.counts[size_t(group) * a.E + tid] = c;
+        dot = float(c) * v;
     }
 #pragma unroll
-    for (int off = 32; off > 0; off >>= 1) dot += __shfl_xor(dot, off, 64);
-    if ((tid & 63u) == 0) part[tid >> 6] = dot;
+    for (int off = 32; off > 0; off >>= 1) {
+        dot += __shfl_xor(dot, off, 64);
+        n += __shfl_xor(n, off, 64);
+    }
+    if (lane == 0) {
+        part[tid >> 6] = dot;
+        npart[tid >> 6] = n;
+    }
     __syncthreads();
     if (tid == 0) {
-        float v = 0.f;
-        for (int w = 0; w < 16; ++w) v += part[w];
+        v = 0.f;
+        n = 0;
+        for (int w = 0; w < kJoinThreads / 64; ++w) {
+            v += part[w];
+            n += npart[w];
+        }
         const float fn = float(n);
         a.loss[group] = n ? v / fn * (float(a.E) / (float(a.k) * fn)) : 0.f;
         a.kept[group] = n;
     }
 }
 
-template <int DT, int VPT>
+// A workgroup walks over every gridDim.x-th 16 tokens of its group, the experts'
+// counts in registers.
+template <int DT, int VPT, bool QUADS>
 __global__ __launch_bounds__(256) void balance_grad_kernel(BalanceArgs a) {
-    const uint32_t lane = threadIdx.x & 63u, j = lane & 15u;
-    const uint32_t group = blockIdx.y, t = (blockIdx.x * 256 + threadIdx.x) / kRowLanes;
-    const bool live = t < a.T;
-    const size_t row = size_t(group) * a.T + (live ? t : 0u);
+    const uint32_t j = threadIdx.x & 15u, group = blockIdx.y, step = gridDim.x * 16;
     const int32_t n = a.kept[group];
-    const bool keep = live && n > 0 && (!a.mask || a.mask[row]);
-    float p[VPT];
-    load_row<DT, VPT>(a.logits, row, a.E, j, a.quads, -__builtin_inff(), p);
-    row_softmax<VPT>(p);
-    float c[VPT], dot = 0.f;
+    const float fn = float(n), scale = n > 0 ? a.dloss[group] / fn * (float(a.E) / (float(a.k) * fn)) : 0.f;
+    float c[VPT];
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
-        const uint32_t e = j * VPT + i;
+        const uint32_t e = expert_of<QUADS>(i, j);
         c[i] = e < a.E ? float(a.counts[size_t(group) * a.E + (e < a.E ? e : 0u)]) : 0.f;
-        dot += c[i] * p[i];
     }
-    dot = row_sum(dot);
-    const float fn = float(n), scale = a.dloss[group] / fn * (float(a.E) / (float(a.k) * fn));
+    const auto row_of = [&](uint32_t t) { return size_t(group) * a.T + (t < a.T ? t : 0u); };
+    uint32_t t = blockIdx.x * 16 + threadIdx.x / kRowLanes;
+    RowWords<DT, VPT> words;
+    load_words<DT, VPT, QUADS>(a.logits, row_of(t), a.E, j, words);
+    for (uint32_t t0 = blockIdx.x * 16; t0 < a.T; t0 += step, t += step) {
+        float p[VPT];
+        to_floats<DT, VPT, QUADS>(words, a.E, j, p);
+        load_words<DT, VPT, QUADS>(a.logits, row_of(t + step < t ? a.T : t + step), a.E, j, words);
+        row_softmax<VPT>(p);
+        float dot = 0.f;
 #pragma unroll
-    for (int i = 0; i < VPT; ++i) p[i] = keep ? scale * p[i] * (c[i] - dot) : 0.f;
-    if (live) store_row<DT, VPT>(a.dlogits, row, a.E, j, a.quads, p);
+        for (int i = 0; i < VPT; ++i) dot += c[i] * p[i];
+        dot = row_sum(dot);
+        const bool live = t < a.T;
+        const size_t row = row_of(t);
+        const bool keep = live && n > 0 && (!a.mask || a.mask[row]);
+#pragma unroll
+        for (int i = 0; i < VPT; ++i) p[i] = keep ? scale * p[i] * (c[i] - dot) : 0.f;
+        if (live) store_row<DT, VPT, QUADS>(a.dlogits, row, a.E, j, p);
+    }
 }
 
-// f(dtype, places a lane) as compile-time constants.
+// f(dtype, places a lane, quads) as compile-time constants.
 template <typename F>
-void by_shape(int dtype, int64_t experts, F &&f) {
-    const auto with = [&](auto dt) {
-        if (experts <= 64)
-            f(dt, std::integral_constant<int, 4>{});
-        else if (experts <= 128)
-            f(dt, std::integral_constant<int, 8>{});
-        else if (experts <= 256)
-            f(dt, std::integral_constant<int, 16>{});
-        else if (experts <= 512)
-            f(dt, std::integral_constant<int, 32>{});
+void by_shape(int dtype, int64_t experts, bool quads, F &&f) {
+    const auto with = [&](auto dt, auto vpt) {
+        if (quads)
+            f(dt, vpt, std::true_type{});
         else
-            f(dt, std::integral_constant<int, 64>{});
+            f(dt, vpt, std::false_type{});
+    };
+    const auto sized = [&](auto dt) {
+        if (experts <= 64)
+            with(dt, std::integral_constant<int, 4>{});
+        else if (experts <= 128)
+            with(dt, std::integral_constant<int, 8>{});
+        else if (experts <= 256)
+            with(dt, std::integral_constant<int, 16>{});
+        else if (experts <= 512)
+            with(dt, std::integral_constant<int, 32>{});
+        else
+            with(dt, std::integral_constant<int, 64>{});
     };
     if (dtype == MX_F32)
-        with(std::integral_constant<int, MX_F32>{});
+        sized(std::integral_constant<int, MX_F32>{});
     else if (dtype == MX_F16)
-        with(std::integral_constant<int, MX_F16>{});
+        sized(std::integral_constant<int, MX_F16>{});
     else
-        with(std::integral_constant<int, MX_BF16>{});
+        sized(std::integral_constant<int, MX_BF16>{});
 }
 
 bool router_shape_ok(int64_t rows, int64_t experts, int64_t k) {
@@ -468,14 +607,15 @@ int iqk_router_topk(int dtype, const void *logits, int64_t rows, int64_t experts
     a.rows = uint32_t(rows);
     a.E = uint32_t(experts);
     a.k = uint32_t(k);
-    a.quads = quads_ok(dtype, experts, logits, nullptr);
+    const bool quads = quads_ok(dtype, experts, logits, nullptr);
     const dim3 grid{uint32_t((rows + 15) / 16)};
-    by_shape(dtype, experts, [&](auto dt, auto vpt) {
+    by_shape(dtype, experts, quads, [&](auto dt, auto vpt, auto qd) {
         constexpr int DT = decltype(dt)::value, VPT = decltype(vpt)::value;
+        constexpr bool Q = decltype(qd)::value;
         if (normalize)
-            hipLaunchKernelGGL((topk_kernel<DT, VPT, true>), grid, dim3{256}, 0, as_stream(stream), a);
+            hipLaunchKernelGGL((topk_kernel<DT, VPT, true, Q>), grid, dim3{256}, 0, as_stream(stream), a);
         else
-            hipLaunchKernelGGL((topk_kernel<DT, VPT, false>), grid, dim3{256}, 0, as_stream(stream), a);
+            hipLaunchKernelGGL((topk_kernel<DT, VPT, false, Q>), grid, dim3{256}, 0, as_stream(stream), a);
     });
     return record_launch(hipGetLastError());
 }
@@ -497,14 +637,15 @@ int iqk_router_topk_grad(int dtype, const void *logits, const float *weights, co
     a.rows = uint32_t(rows);
     a.E = uint32_t(experts);
     a.k = uint32_t(k);
-    a.quads = quads_ok(dtype, experts, normalize ? nullptr : logits, dlogits);
+    const bool quads = quads_ok(dtype, experts, normalize ? nullptr : logits, dlogits);
     const dim3 grid{uint32_t((rows + 15) / 16)};
-    by_shape(dtype, experts, [&](auto dt, auto vpt) {
+    by_shape(dtype, experts, quads, [&](auto dt, auto vpt, auto qd) {
         constexpr int DT = decltype(dt)::value, VPT = decltype(vpt)::value;
+        constexpr bool Q = decltype(qd)::value;
         if (normalize)
-            hipLaunchKernelGGL((topk_grad_kernel<DT, VPT, true>), grid, dim3{256}, 0, as_stream(stream), a);
+            hipLaunchKernelGGL((topk_grad_kernel<DT, VPT, true, Q>), grid, dim3{256}, 0, as_stream(stream), a);
         else
-            hipLaunchKernelGGL((topk_grad_kernel<DT, VPT, false>), grid, dim3{256}, 0, as_stream(stream), a);
+            hipLaunchKernelGGL((topk_grad_kernel<DT, VPT, false, Q>), grid, dim3{256}, 0, as_stream(stream), a);
     });
     return record_launch(hipGetLastError());
 }
@@ -540,13 +681,13 @@ int iqk_balance(int dtype, const void *logits, const int32_t *ids, const uint8_t
     a.shares = uint32_t(shares);
     const int64_t turns = (tokens + kBalanceRows - 1) / kBalanceRows;
     a.share = uint32_t((turns + shares - 1) / shares * kBalanceRows);
-    a.quads = quads_ok(dtype, experts, logits, nullptr);
-    by_shape(dtype, experts, [&](auto dt, auto vpt) {
-        hipLaunchKernelGGL((balance_sums_kernel<decltype(dt)::value, decltype(vpt)::value>),
+    const bool quads = quads_ok(dtype, experts, logits, nullptr);
+    by_shape(dtype, experts, quads, [&](auto dt, auto vpt, auto qd) {
+        hipLaunchKernelGGL((balance_sums_kernel<decltype(dt)::value, decltype(vpt)::value, decltype(qd)::value>),
                            dim3(uint32_t(shares), uint32_t(groups)), dim3{kBalanceThreads}, 0, as_stream(stream), a);
     });
     if (const hipError_t err = hipGetLastError(); err != hipSuccess) return record_launch(err);
-    hipLaunchKernelGGL(balance_join_kernel, dim3{uint32_t(groups)}, dim3{1024}, 0, as_stream(stream), a);
+    hipLaunchKernelGGL(balance_join_kernel, dim3{uint32_t(groups)}, dim3{kJoinThreads}, 0, as_stream(stream), a);
     return record_launch(hipGetLastError());
 }
 
@@ -568,10 +709,13 @@ int iqk_balance_grad(int dtype, const void *logits, const uint8_t *mask, const i
     a.T = uint32_t(tokens);
     a.E = uint32_t(experts);
     a.k = uint32_t(k);
-    a.quads = quads_ok(dtype, experts, logits, dlogits);
-    by_shape(dtype, experts, [&](auto dt, auto vpt) {
-        hipLaunchKernelGGL((balance_grad_kernel<decltype(dt)::value, decltype(vpt)::value>),
-                           dim3(uint32_t((tokens + 15) / 16), uint32_t(groups)), dim3{256}, 0, as_stream(stream), a);
+    const bool quads = quads_ok(dtype, experts, logits, dlogits);
+    // 16 tokens a turn, about eight workgroups a CU
+    const int64_t turns = (tokens + 15) / 16, most = (256 * 8 + groups - 1) / groups;
+    by_shape(dtype, experts, quads, [&](auto dt, auto vpt, auto qd) {
+        hipLaunchKernelGGL((balance_grad_kernel<decltype(dt)::value, decltype(vpt)::value, decltype(qd)::value>),
+                           dim3(uint32_t(turns < most ? turns : most), uint32_t(groups)), dim3{256}, 0,
+                           as_stream(stream), a);
     });
     return record_launch(hipGetLastError());
 }
