@@ -219,11 +219,12 @@ struct TopkArgs {
 };
 
 // The k highest logits, ties to the lowest expert, and their softmax weights:
-// over the chosen (NORM) or over all.  k rounds of a maximum over the row.
-// 16-bit logits and their expert make one key, so that a round compares,
-// removes and finds the expert with three instructions a logit; f32 logits
-// need five, the lowest of the experts that hold the maximum being a second
-// reduction.
+// over the chosen (NORM) or over all.  k rounds of a maximum over the row, bound
+// by their instructions.  16-bit logits and their expert make one key, and of
+// the keys below the last choice the highest has the highest unsigned key -
+// choice (those at or above it wrap to less), so that a round needs a
+// subtraction and half a maximum a logit.  f32 logits need five instructions: the
+// lowest of the experts that hold the maximum is a second reduction.
 template <int DT, int VPT, bool NORM, bool QUADS>
 __global__ __launch_bounds__(256) void topk_kernel(TopkArgs a) {
     constexpr bool WIDE = DT == MX_F32;
@@ -241,57 +242,63 @@ __global__ __launch_bounds__(256) void topk_kernel(TopkArgs a) {
         else
             key[i] = e < a.E ? order_key16<DT>(half_of(words, i), e) : 0u;
     }
-    float chosen[4];  // lane j: choices j, 16 + j, ..
-    int32_t id[4];
-    float top = 0.f, sum = 0.f;
+    // lane j: choices j, 16 + j, ..
+    uint32_t chosen[4], id[4];
+    uint32_t best = 0, first = 0;
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
+        chosen[q] = id[q] = 0;
         if (16u * q >= a.k) break;  // uniform
         const uint32_t n = min(a.k - 16u * q, 16u);
         for (uint32_t c = 0; c < n; ++c) {
-            uint32_t m = key[0];
-#pragma unroll
-            for (int i = 1; i < VPT; ++i) m = max(m, key[i]);
-            const uint32_t best = row_max(m);
-            uint32_t e;
-            float value;
+            uint32_t e = 0;
             if constexpr (WIDE) {
+                uint32_t m = key[0];
+#pragma unroll
+                for (int i = 1; i < VPT; ++i) m = max(m, key[i]);
+                best = row_max(m);
                 uint32_t at = 0xffffu;
 #pragma unroll
                 for (int i = VPT - 1; i >= 0; --i) at = key[i] == best ? uint32_t(expert_of<QUADS>(i, j)) : at;
                 e = row_min(at);
 #pragma unroll
                 for (int i = 0; i < VPT; ++i) key[i] = expert_of<QUADS>(i, j) == e ? 0u : key[i];
-                value = key_value(best);
             } else {
+                uint32_t m = key[0] - best;
 #pragma unroll
-                for (int i = 0; i < VPT; ++i) key[i] = key[i] == best ? 0u : key[i];
-                e = 0xffffu - (best & 0xffffu);
-                value = key16_value<DT>(best);
+                for (int i = 1; i < VPT; ++i) m = max(m, key[i] - best);
+                best += row_max(m);
             }
-            if (q == 0 && c == 0) top = value;
-            if constexpr (NORM) sum += exp_neg(value - top);
+            if (q == 0 && c == 0) first = best;
             if (j == c) {
-                chosen[q] = value;
-                id[q] = int32_t(e);
+                chosen[q] = best;
+                id[q] = WIDE ? e : 0xffffu - (best & 0xffffu);
             }
         }
+    }
+    const auto value = [](uint32_t k) { return WIDE ? key_value(k) : key16_value<DT>(k); };
+    const float top = value(first);
+    float ex[4], sum = 0.f;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        ex[q] = 16u * q + j < a.k ? exp_neg(value(chosen[q]) - top) : 0.f;
+        if constexpr (NORM) sum += ex[q];
     }
     if constexpr (!NORM) {
         float v[VPT];
         to_floats<DT, VPT, QUADS>(words, a.E, j, v);
 #pragma unroll
         for (int i = 0; i < VPT; ++i) sum += exp_neg(v[i] - top);
-        sum = row_sum(sum);
     }
+    sum = row_sum(sum);
     const bool empty = top == -__builtin_inff();
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
         const uint32_t c = 16u * q + j;
         if (!live || c >= a.k) continue;
         const size_t at = size_t(row) * a.k + c;
-        a.weights[at] = empty ? 0.f : exp_neg(chosen[q] - top) / sum;
-        a.ids[at] = id[q];
+        a.weights[at] = empty ? 0.f : ex[q] / sum;
+        a.ids[at] = int32_t(id[q]);
     }
 }
 
@@ -583,9 +590,9 @@ bool quads_ok(int dtype, int64_t experts, const void *a, const void *b) {
 }
 
 int64_t balance_shares(int64_t groups, int64_t tokens) {
-    // a share is whole turns of the workgroup's rows; about one workgroup a CU
+    // a share is whole turns of the workgroup's rows; about two workgroups a CU
     const int64_t most = (tokens + kBalanceRows - 1) / kBalanceRows;
-    const int64_t want = (256 + groups - 1) / groups;
+    const int64_t want = (512 + groups - 1) / groups;
     return most < want ? (most > 0 ? most : 1) : want;
 }
 
