@@ -1,5 +1,5 @@
 /* A CPython binding of the decode, verify and prefill entry points of
- * libiqk_hip.so, and of the 4-bit and router ones: the launch paths an eager call of a switch module takes (a
+ * libiqk_hip.so: the launch paths an eager call of the switch module takes (a
  * 1-token dispatch's kernel runs for ~6 us, and a ctypes call with twelve
  * converted arguments costs ~4 us of host time).  Each function takes the C ABI's arguments as Python integers
  * (device pointers as addresses, the stream as its handle) and returns the
@@ -104,53 +104,6 @@ static PyObject *prefill(PyObject *self, PyObject *const *args, Py_ssize_t nargs
     return PyLong_FromLong(rc);
 }
 
-/* The 4-bit and router entry points, each a function of the entry point's
- * arguments in order.  Those in the mask are C ints and are range-checked. */
-static int integers(PyObject *const *args, Py_ssize_t nargs, int want, unsigned narrow, long long *v) {
-    if (nargs != want) {
-        PyErr_Format(PyExc_TypeError, "this entry point takes %d integer arguments, got %zd", want, nargs);
-        return 0;
-    }
-    for (int i = 0; i < want; ++i) {
-        if (!as_i64(args[i], &v[i])) return 0;
-        if ((narrow >> i & 1u) && (v[i] < INT_MIN || v[i] > INT_MAX)) {
-            PyErr_Format(PyExc_OverflowError, "argument %d is out of range", i);
-            return 0;
-        }
-    }
-    return 1;
-}
-
-#define AT(i) ((void *)(uintptr_t)v[i])
-#define ENTRY(name, count, narrow, call)                                                  \
-    static PyObject *name(PyObject *self, PyObject *const *args, Py_ssize_t nargs) {      \
-        (void)self;                                                                       \
-        long long v[count];                                                               \
-        if (!integers(args, nargs, count, narrow, v)) return NULL;                        \
-        return PyLong_FromLongLong(call);                                                 \
-    }
-
-ENTRY(mx_quantize, 9, 1u << 0, iqk_mx_quantize((int)v[0], AT(1), v[2], v[3], v[4], AT(5), AT(6), v[7], AT(8)))
-ENTRY(mx_dequantize, 8, 1u << 0, iqk_mx_dequantize((int)v[0], AT(1), AT(2), v[3], v[4], v[5], AT(6), AT(7)))
-ENTRY(mx_pairs, 17, 1u << 0 | 1u << 12,
-      iqk_mx_pairs((int)v[0], v[1], v[2], v[3], AT(4), v[5], AT(6), v[7], AT(8), AT(9), AT(10), AT(11), (int)v[12],
-                   v[13], v[14], AT(15), AT(16)))
-ENTRY(mx_groups, 17, 1u << 0,
-      iqk_mx_groups((int)v[0], v[1], v[2], v[3], AT(4), v[5], AT(6), v[7], AT(8), AT(9), AT(10), AT(11), AT(12), AT(13),
-                    v[14], AT(15), AT(16)))
-ENTRY(mx_prefill, 19, 1u << 0 | 1u << 12,
-      iqk_mx_prefill((int)v[0], v[1], v[2], v[3], AT(4), v[5], AT(6), v[7], AT(8), AT(9), AT(10), AT(11), (int)v[12],
-                     v[13], v[14], v[15], AT(16), AT(17), AT(18)))
-ENTRY(router_topk, 9, 1u << 0 | 1u << 5,
-      iqk_router_topk((int)v[0], AT(1), v[2], v[3], v[4], (int)v[5], AT(6), AT(7), AT(8)))
-ENTRY(router_topk_grad, 11, 1u << 0 | 1u << 8,
-      iqk_router_topk_grad((int)v[0], AT(1), AT(2), AT(3), AT(4), v[5], v[6], v[7], (int)v[8], AT(9), AT(10)))
-ENTRY(balance_work, 3, 0, iqk_balance_work(v[0], v[1], v[2]))
-ENTRY(balance, 13, 1u << 0,
-      iqk_balance((int)v[0], AT(1), AT(2), AT(3), v[4], v[5], v[6], v[7], AT(8), AT(9), AT(10), AT(11), AT(12)))
-ENTRY(balance_grad, 12, 1u << 0,
-      iqk_balance_grad((int)v[0], AT(1), AT(2), AT(3), AT(4), AT(5), v[6], v[7], v[8], v[9], AT(10), AT(11)))
-
 static PyObject *source_hash(PyObject *self, PyObject *unused) {
     (void)self;
     (void)unused;
@@ -161,9 +114,6 @@ static PyMethodDef methods[] = {
     {"gemv", (PyCFunction)(void (*)(void))gemv, METH_FASTCALL, "iqk_gemv / _floor / _floor_grid / _ids64"},
     {"sorted", (PyCFunction)(void (*)(void))sorted, METH_FASTCALL, "iqk_gemv_sorted / _union"},
     {"prefill", (PyCFunction)(void (*)(void))prefill, METH_FASTCALL, "iqk_prefill"},
-#define METHOD(name) {#name, (PyCFunction)(void (*)(void))name, METH_FASTCALL, "iqk_" #name}
-    METHOD(mx_quantize), METHOD(mx_dequantize), METHOD(mx_pairs), METHOD(mx_groups), METHOD(mx_prefill),
-    METHOD(router_topk), METHOD(router_topk_grad), METHOD(balance_work), METHOD(balance), METHOD(balance_grad),
     {"source_hash", source_hash, METH_NOARGS, "digest of the kernel sources this binding was built with"},
     {NULL, NULL, 0, NULL},
 };

@@ -11,7 +11,7 @@ from ctypes import c_char_p, c_int, c_int64, c_uint32, c_void_p
 from pathlib import Path
 
 from . import build
-from .build import HIP_LIB, LAUNCH_EXT
+from .build import HIP_LIB, LAUNCH_EXT, TORCH_EXT
 
 ABI_VERSION = 7
 
@@ -92,6 +92,7 @@ class IqkNativeError(RuntimeError):
 
 _LIB = None
 _LAUNCH = None
+_TORCH = None
 
 
 def library_path() -> Path:
@@ -132,14 +133,19 @@ def _load_launch(digest: str) -> None:
     global _LAUNCH
     if not LAUNCH_EXT.is_file():
         return
-    import importlib.util
-    spec = importlib.util.spec_from_file_location("_iqk_launch", LAUNCH_EXT)
-    mod = importlib.util.module_from_spec(spec)
-    spec.loader.exec_module(mod)
+    mod = _import("_iqk_launch", LAUNCH_EXT)
     if mod.source_hash() != digest:
         raise IqkNativeError(f"{LAUNCH_EXT} was built with other sources than {HIP_LIB}; rebuild both with "
                              "`python -m mlx_iqk_amd.build`")
     _LAUNCH = mod
+
+
+def _import(name: str, path: Path):
+    import importlib.util
+    spec = importlib.util.spec_from_file_location(name, path)
+    mod = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(mod)
+    return mod
 
 
 def launcher():
@@ -147,18 +153,21 @@ def launcher():
     return _LAUNCH
 
 
-_ENTRIES: dict = {}
-
-
-def entry(name: str):
-    """``iqk_<name>`` as a function of plain integers (addresses, 0 for none),
-    through the CPython binding where it has it, else through ctypes."""
-    fn = _ENTRIES.get(name)
-    if fn is None:
-        lib = load()
-        fn = getattr(_LAUNCH, name, None) or getattr(lib, f"iqk_{name}")
-        _ENTRIES[name] = fn
-    return fn
+def torch_binding():
+    """The torch binding of the 4-bit and router calls (``_iqk_torch``); raises
+    where it is not built, or was built with other sources than the library."""
+    global _TORCH
+    if _TORCH is None:
+        digest = load().iqk_hip_source_hash().decode()
+        if not TORCH_EXT.is_file():
+            raise IqkNativeError(f"{TORCH_EXT} is not built; run `python -m mlx_iqk_amd.build`")
+        import torch  # noqa: F401  (its libraries, which the binding links against)
+        mod = _import("_iqk_torch", TORCH_EXT)
+        if mod.source_hash() != digest:
+            raise IqkNativeError(f"{TORCH_EXT} was built with other sources than {HIP_LIB}; rebuild both with "
+                                 "`python -m mlx_iqk_amd.build`")
+        _TORCH = mod
+    return _TORCH
 
 
 def check(rc: int, what: str) -> None:

@@ -1,11 +1,13 @@
-"""Build recipes for the two native libraries of this package.
+"""Build recipes for the native libraries of this package.
 
 * ``libiqk_codec.so`` -- the CPU codec (quantizers and dequantizers), g++.
 * ``libiqk_hip.so``   -- the gfx950 kernels behind the C ABI, hipcc.
+* ``_iqk_launch``     -- the CPython binding of the IQ_K calls, gcc.
+* ``_iqk_torch``      -- the torch binding of the 4-bit and router calls, g++.
 
-Both land in ``mlx_iqk_amd/_lib/`` beside the Python sources, so the built
+All land in ``mlx_iqk_amd/_lib/`` beside the Python sources, so the built
 files travel with the source tree.  ``python -m mlx_iqk_amd.build`` builds
-both.
+them.
 """
 
 from __future__ import annotations
@@ -28,6 +30,7 @@ LIBDIR = PACKAGE / "_lib"
 CODEC_LIB = LIBDIR / "libiqk_codec.so"
 HIP_LIB = LIBDIR / "libiqk_hip.so"
 LAUNCH_EXT = LIBDIR / ("_iqk_launch" + (sysconfig.get_config_var("EXT_SUFFIX") or ".so"))
+TORCH_EXT = LIBDIR / ("_iqk_torch" + (sysconfig.get_config_var("EXT_SUFFIX") or ".so"))
 
 # Source -> extra hipcc flags.  The MFMA decode GEMV folds each accumulator
 # right after its MFMA chain, so its MFMA results go straight to VGPRs.
@@ -143,10 +146,34 @@ def build_launch() -> Path:
     return LAUNCH_EXT
 
 
+def torch_command(out: Path = TORCH_EXT, source_hash: str = "") -> list[str]:
+    """The torch binding, against torch's own headers and libraries and the
+    kernel library beside it."""
+    import torch
+    home = Path(torch.__file__).resolve().parent
+    include = home / "include"
+    return ["g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-D__HIP_PLATFORM_AMD__", "-DUSE_ROCM",
+            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+            f"-I{include}", f"-I{include / 'torch' / 'csrc' / 'api' / 'include'}",
+            f"-I{Path(_hipcc()).resolve().parents[1] / 'include'}", f"-I{sysconfig.get_paths()['include']}",
+            f"-I{INCLUDE}", f'-DIQK_SOURCE_HASH="{source_hash or hip_source_hash()}"', "-o", str(out),
+            str(CSRC / "torch" / "iqk_torch.cpp"), f"-L{home / 'lib'}", "-ltorch", "-ltorch_cpu", "-lc10",
+            "-lc10_hip", "-ltorch_python", f"-L{LIBDIR}", "-liqk_hip", "-Wl,-rpath,$ORIGIN"]
+
+
+def build_torch() -> Path:
+    LIBDIR.mkdir(parents=True, exist_ok=True)
+    tmp = TORCH_EXT.with_suffix(".so.tmp")
+    _run(torch_command(tmp))
+    tmp.replace(TORCH_EXT)
+    return TORCH_EXT
+
+
 def build_all() -> None:
     build_codec()
     build_hip()
     build_launch()
+    build_torch()
 
 
 if __name__ == "__main__":

@@ -92,14 +92,6 @@ class MxTensor:
         return f"MxTensor({tuple(self.shape)}, {self.dtype}, {self.device})"
 
 
-def _new_scales(lead: tuple, n: int, device) -> tuple[torch.Tensor, int]:
-    """Room for the scales of rows of n values, and the bytes from row to row: a
-    multiple of four, as the products read activations' scales."""
-    stride = 4 * ((n + _STEP - 1) // _STEP)
-    room = torch.empty((*lead, stride), dtype=torch.uint8, device=device)
-    return (room if stride * BLOCK == n else room[..., :n // BLOCK]), stride
-
-
 def _row_stride(t: torch.Tensor) -> int | None:
     """Elements from row to row of t taken as [rows, n], the last axis dense;
     None where rows are not evenly spaced."""
@@ -157,28 +149,17 @@ def quantize(x: torch.Tensor) -> MxTensor:
     if not x.is_cuda:
         raise IqkKernelError(f"x must live on a GPU, got {x.device}")
     dtype = x.dtype
-    code = _DTYPES.get(dtype)
-    if code is None:
+    if dtype not in _DTYPES:
         raise IqkKernelError(f"x must be one of {tuple(_DTYPES)}, got {dtype}")
-    *lead, n = x.shape
-    _check_width(n)
-    device, stride, at = x.device, n, x.data_ptr()
+    n = _check_width(x.shape[-1])
+    stride, at = n, x.data_ptr()
     if not x.is_contiguous() or at % 16:
         stride = _row_stride(x)
         if stride is None or stride < n or stride % (16 // x.element_size()) or at % 16:
             x, stride = x.contiguous(), n
             if x.data_ptr() % 16:
                 x = x.clone()
-            at = x.data_ptr()
-    codes = torch.empty((*lead, n // 2), dtype=torch.uint8, device=device)
-    scales, scale_stride = _new_scales(lead, n, device)
-    rows = math.prod(lead)
-    if rows:
-        rc = _native.entry("mx_quantize")(code, at, rows, n, stride, codes.data_ptr(), scales.data_ptr(), scale_stride,
-                                          _stream_ptr(device))
-        if rc:
-            _native.check(rc, f"iqk_mx_quantize({rows}x{n})")
-    return MxTensor._of(codes, scales, dtype)
+    return MxTensor._of(*_native.torch_binding().mx_quantize(x, stride), dtype)
 
 
 def dequantize(q: MxTensor, dtype: torch.dtype | None = None) -> torch.Tensor:
@@ -191,18 +172,10 @@ def dequantize(q: MxTensor, dtype: torch.dtype | None = None) -> torch.Tensor:
     codes, scales = q.codes, q.scales
     if not codes.is_cuda:
         raise IqkKernelError(f"codes must live on a GPU, got {codes.device}")
-    *lead, half = codes.shape
-    n, rows = 2 * half, math.prod(lead)
     codes, stride = _aligned_codes(codes), _row_stride(scales)
-    if stride is None or stride < n // BLOCK:
-        scales, stride = scales.contiguous(), n // BLOCK
-    y = torch.empty((*lead, n), dtype=dtype, device=codes.device)
-    if rows:
-        rc = _native.entry("mx_dequantize")(code, codes.data_ptr(), scales.data_ptr(), rows, n, stride, y.data_ptr(),
-                                            _stream_ptr(codes.device))
-        if rc:
-            _native.check(rc, f"iqk_mx_dequantize({rows}x{n})")
-    return y
+    if stride is None or stride < scales.shape[-1]:
+        scales, stride = scales.contiguous(), scales.shape[-1]
+    return _native.torch_binding().mx_dequantize(codes, scales, stride, code)
 
 
 class _MxStack(torch.nn.Module):
@@ -257,7 +230,7 @@ class _MxStack(torch.nn.Module):
         return y
 
     def _activations(self, x, tiles: torch.Tensor) -> tuple:
-        """x's rows as the kernels take them: (act, rows, scales, scale stride, dtype)."""
+        """x's rows as the kernels take them: (act, rows, scales, scale stride)."""
         mx = isinstance(x, MxTensor)
         if not mx and not isinstance(x, torch.Tensor):
             raise IqkKernelError("x must be a tensor or an MxTensor")
@@ -271,23 +244,22 @@ class _MxStack(torch.nn.Module):
         if width != self.in_features:
             raise IqkRuntimeError(f"x has rows of {width} values, the weights take {self.in_features}")
         if mx:
-            return (act, _aligned_codes(rows), *_product_scales(x), x.dtype)
+            return (act, _aligned_codes(rows), *_product_scales(x))
         if rows.requires_grad and torch.is_grad_enabled():
             raise IqkRuntimeError("the weights are frozen and no gradient flows through them: detach x, or call "
                                   "under torch.no_grad()")
         if not rows.is_contiguous() or rows.data_ptr() % 16:
             rows = rows.detach().contiguous()
             rows = rows if rows.data_ptr() % 16 == 0 else rows.clone()
-        return act, rows, None, 0, x.dtype
+        return act, rows, None, 0
 
-    def _launch(self, entry: str, act, rows, scales, stride, n_x_rows, *args) -> None:
+    def _project(self, x: tuple, ids, shape: tuple, pairs: int, M: int, per_row: int, grouped: bool) -> torch.Tensor:
+        """Outputs ``shape`` of the activations ``x`` (:meth:`_activations`' first four)."""
+        act, rows, scales, stride = x
         buffers = self._buffers  # without Module.__getattr__'s lookups
-        rc = _native.entry(entry)(
-            act, self.in_features, self.out_features, self.num_experts, rows.data_ptr(), n_x_rows,
-            0 if scales is None else scales.data_ptr(), stride, buffers["tiles"].data_ptr(),
-            buffers["tile_scales"].data_ptr(), buffers["row_exps"].data_ptr(), *args, _stream_ptr(rows.device))
-        if rc:
-            _native.check(rc, f"iqk_{entry}({self.num_experts}x{self.out_features}x{self.in_features})")
+        return _native.torch_binding().mx_project(
+            act, rows, scales, stride, buffers["tiles"], buffers["tile_scales"], buffers["row_exps"], ids, shape,
+            self.in_features, pairs, M, per_row, grouped)
 
     def extra_repr(self) -> str:
         return f"{self.num_experts}, {self.out_features}, {self.in_features}"
@@ -321,37 +293,27 @@ class MxSwitchLinear(_MxStack):
         if len(x.shape) < 2:
             raise IqkRuntimeError(f"x must be [..., M, {self.in_features}], got {tuple(x.shape)}")
         tiles = self._buffers["tiles"]
-        act, rows, scales, stride, dtype = self._activations(x, tiles)
+        act, rows, scales, stride = self._activations(x, tiles)
         *xbatch, M, _ = rows.shape
         batch = indices.shape
         per_row = _pairs_per_x_row(xbatch, batch)
         if per_row is None:
             batch = torch.broadcast_shapes(xbatch, batch)
             per_row = _pairs_per_x_row(xbatch, batch)
-        pairs = math.prod(batch)
-        y = torch.empty((*batch, M, self.out_features), dtype=dtype, device=tiles.device)
-        if not pairs * M:
-            return y
         if per_row is None:  # x broadcasts over leading dimensions: a row of its own for each pair
             rows = rows.expand(*batch, M, rows.shape[-1]).contiguous()
             if scales is not None:
                 n = self.in_features // BLOCK
                 scales, stride = _product_scales(MxTensor(rows, x.scales.expand(*batch, M, n).contiguous()))
             per_row = 1
-        n_x_rows = rows.numel() // rows.shape[-1]
         ids = indices
-        wide = _KERNEL_IDS.get(ids.dtype)
-        if wide is None or ids.shape != batch or not ids.is_contiguous() or ids.get_device() != tiles.get_device():
+        if ids.dtype not in _KERNEL_IDS or ids.shape != batch or not ids.is_contiguous() \
+                or ids.get_device() != tiles.get_device():
             ids = self._ids(indices, batch)
-            wide = _KERNEL_IDS[ids.dtype]
-        if pairs <= PAIR_LIMIT and M == 1 and not sorted_indices:
-            self._launch("mx_pairs", act, rows, scales, stride, n_x_rows, ids.data_ptr(), wide, per_row, pairs,
-                         y.data_ptr())
-            return y
-        work = torch.empty(2 * pairs * M + self.num_experts + 1, dtype=torch.int32, device=tiles.device)
-        self._launch("mx_prefill", act, rows, scales, stride, n_x_rows, ids.data_ptr(), wide, pairs, M, per_row,
-                     work.data_ptr(), y.data_ptr())
-        return y
+        pairs = math.prod(batch)
+        grouped = sorted_indices or M != 1 or pairs > PAIR_LIMIT
+        return self._project((act, rows, scales, stride), ids, (*batch, M, self.out_features), pairs, M, per_row,
+                             grouped)
 
     def _ids(self, indices: torch.Tensor, batch) -> torch.Tensor:
         """Expert ids of the pairs in order, of a type the kernels read.  Other
@@ -388,17 +350,10 @@ class MxLinear(_MxStack):
 
     def forward(self, x) -> torch.Tensor:
         tiles = self._buffers["tiles"]
-        act, rows, scales, stride, dtype = self._activations(x, tiles)
-        *lead, width = rows.shape
+        x = self._activations(x, tiles)
+        lead = x[1].shape[:-1]
         n = math.prod(lead)
-        y = torch.empty((*lead, self.out_features), dtype=dtype, device=tiles.device)
-        if n == 0:
-            return y
-        if n <= 4:
-            self._launch("mx_pairs", act, rows, scales, stride, n, 0, 0, 1, n, y.data_ptr())
-        else:
-            self._launch("mx_groups", act, rows, scales, stride, n, 0, 0, 0, n, y.data_ptr())
-        return y
+        return self._project(x, None, (*lead, self.out_features), n, 1, 1, n > 4)
 
     def extra_repr(self) -> str:
         return f"{self.out_features}, {self.in_features}"

@@ -4,18 +4,16 @@ weights, and the loss that keeps the experts evenly loaded; with gradients.
 :func:`topk`'s ids are the ``indices`` of the switch modules
 (:class:`~mlx_iqk_amd.nn.IqkSwitchLinear`, :class:`~mlx_iqk_amd.mx.MxSwitchLinear`),
 its weights scale their outputs.  Logits are f32, f16 or bf16 on a GPU, for up to
-1024 experts; sums, probabilities, weights and losses are f32.
+1024 experts; sums, probabilities, weights and losses are f32.  Gradients are
+differentiable once.
 """
 
 from __future__ import annotations
 
-import math
-
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _native
-from .kernels import IqkKernelError, _stream_ptr
+from .kernels import IqkKernelError
 from .mx import _DTYPES
 
 MAX_EXPERTS = 1024
@@ -35,46 +33,6 @@ def _check_logits(logits: torch.Tensor, dims: int) -> int:
     return experts
 
 
-def _topk(logits: torch.Tensor, k: int, normalize: bool) -> tuple[torch.Tensor, torch.Tensor]:
-    shape, device = (*logits.shape[:-1], k), logits.device
-    weights = torch.empty(shape, dtype=torch.float32, device=device)
-    ids = torch.empty(shape, dtype=torch.int32, device=device)
-    rc = _native.entry("router_topk")(_DTYPES[logits.dtype], logits.data_ptr(), weights.numel() // k,
-                                      logits.shape[-1], k, normalize, weights.data_ptr(), ids.data_ptr(),
-                                      _stream_ptr(device))
-    if rc:
-        _native.check(rc, f"iqk_router_topk({tuple(logits.shape)}, {k})")
-    return weights, ids
-
-
-class _TopK(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, k, normalize):
-        weights, ids = _topk(logits, k, normalize)
-        ctx.mark_non_differentiable(ids)
-        ctx.set_materialize_grads(False)
-        ctx.normalize, ctx.dtype, ctx.shape = normalize, logits.dtype, logits.shape
-        ctx.save_for_backward(weights, ids, *(() if normalize else (logits,)))
-        return weights, ids
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dweights, _):
-        if dweights is None:
-            return None, None, None
-        weights, ids, *rest = ctx.saved_tensors
-        dweights = dweights.to(torch.float32).contiguous()
-        dlogits = torch.empty(ctx.shape, dtype=ctx.dtype, device=weights.device)
-        k = weights.shape[-1]
-        rc = _native.entry("router_topk_grad")(
-            _DTYPES[ctx.dtype], rest[0].data_ptr() if rest else 0, weights.data_ptr(), ids.data_ptr(),
-            dweights.data_ptr(), weights.numel() // k, ctx.shape[-1], k, ctx.normalize, dlogits.data_ptr(),
-            _stream_ptr(weights.device))
-        if rc:
-            _native.check(rc, f"iqk_router_topk_grad({tuple(ctx.shape)}, {k})")
-        return dlogits, None, None
-
-
 def topk(logits: torch.Tensor, k: int, *, normalize: bool = True) -> tuple[torch.Tensor, torch.Tensor]:
     """The ``k`` experts of each token: ``(weights f32 [..., k], ids i32 [..., k])``.
 
@@ -90,54 +48,7 @@ def topk(logits: torch.Tensor, k: int, *, normalize: bool = True) -> tuple[torch
         raise IqkKernelError(f"k must be 1 .. {min(MAX_K, experts)} of {experts} experts, got {k}")
     if not logits.is_contiguous():
         logits = logits.contiguous()
-    if logits.requires_grad and torch.is_grad_enabled():
-        return _TopK.apply(logits, k, bool(normalize))
-    return _topk(logits, k, bool(normalize))
-
-
-def _balance(logits, ids, mask):
-    *lead, tokens, experts = logits.shape
-    groups, device = math.prod(lead), logits.device
-    loss = torch.empty(lead, dtype=torch.float32, device=device)
-    counts = torch.empty((*lead, experts), dtype=torch.int32, device=device)
-    kept = torch.empty(lead, dtype=torch.int32, device=device)
-    if groups:
-        work = torch.empty(_native.entry("balance_work")(groups, tokens, experts), dtype=torch.int32, device=device)
-        rc = _native.entry("balance")(_DTYPES[logits.dtype], logits.data_ptr(), ids.data_ptr(),
-                                      0 if mask is None else mask.data_ptr(), groups, tokens, experts,
-                                      ids.shape[-1], work.data_ptr(), loss.data_ptr(), counts.data_ptr(),
-                                      kept.data_ptr(), _stream_ptr(device))
-        if rc:
-            _native.check(rc, f"iqk_balance({tuple(logits.shape)}, {ids.shape[-1]})")
-    return loss, counts, kept
-
-
-class _Balance(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, ids, mask):
-        loss, counts, kept = _balance(logits, ids, mask)
-        ctx.mark_non_differentiable(counts)
-        ctx.set_materialize_grads(False)
-        ctx.k = ids.shape[-1]
-        ctx.save_for_backward(logits, counts, kept, mask)
-        return loss, counts
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dloss, _):
-        if dloss is None:
-            return None, None, None
-        logits, counts, kept, mask = ctx.saved_tensors
-        dloss = dloss.to(torch.float32).contiguous()
-        dlogits = torch.empty_like(logits)
-        *lead, tokens, experts = logits.shape
-        rc = _native.entry("balance_grad")(
-            _DTYPES[logits.dtype], logits.data_ptr(), 0 if mask is None else mask.data_ptr(), counts.data_ptr(),
-            kept.data_ptr(), dloss.data_ptr(), math.prod(lead), tokens, experts, ctx.k, dlogits.data_ptr(),
-            _stream_ptr(logits.device))
-        if rc:
-            _native.check(rc, f"iqk_balance_grad({tuple(logits.shape)}, {ctx.k})")
-        return dlogits, None, None
+    return _native.torch_binding().topk(logits, k, normalize)
 
 
 def balance_loss(logits: torch.Tensor, ids: torch.Tensor, *,
@@ -169,10 +80,7 @@ def balance_loss(logits: torch.Tensor, ids: torch.Tensor, *,
         mask = mask.contiguous()
     if ids.dtype != torch.int32:
         ids = torch.clamp(ids.to(torch.int64), -1, experts).to(torch.int32)
-    logits, ids = logits.contiguous(), ids.contiguous()
-    if logits.requires_grad and torch.is_grad_enabled():
-        return _Balance.apply(logits, ids, mask)
-    return _balance(logits, ids, mask)[:2]
+    return _native.torch_binding().balance(logits.contiguous(), ids.contiguous(), mask)
 
 
 __all__ = ["MAX_EXPERTS", "MAX_K", "balance_loss", "topk"]

@@ -91,29 +91,21 @@ def test_grouped_call_refuses_bad_arguments(lib):
     assert prefill(n=48) == GEOMETRY and prefill(pairs=0) == OK
 
 
-def test_launch_binding_reaches_the_same_entry_points(lib):
-    """The binding's functions give the entry points' refusals, and refuse
-    arguments that a C int would cut."""
-    fast = _native.launcher()
-    assert fast is not None, "the launch binding is built beside the library by build()"
-    for name in ("mx_quantize", "mx_dequantize", "mx_pairs", "mx_groups", "mx_prefill", "router_topk",
-                 "router_topk_grad", "balance_work", "balance", "balance_grad"):
-        assert _native.entry(name) is getattr(fast, name)
+def test_torch_binding_is_built_from_the_same_sources(lib):
+    binding = _native.torch_binding()
+    assert binding.source_hash() == lib.iqk_hip_source_hash().decode()
+    for name, args in (("topk", 3), ("balance", 3), ("mx_quantize", 2), ("mx_dequantize", 4), ("mx_project", 14)):
         with pytest.raises(TypeError):
-            getattr(fast, name)(0)
-    assert fast.mx_quantize(0, P, 4, 33, 33, P, P, 8, 0) == GEOMETRY
-    assert fast.mx_dequantize(0, P, P, 4, 33, 8, P, 0) == GEOMETRY
-    assert fast.mx_pairs(4, 64, 16, 2, P, 4, 0, 0, P, P, P, P, 0, 1, 4, P, 0) == ARGUMENT
-    assert fast.mx_groups(0, 48, 16, 2, P, 4, 0, 0, P, P, P, P, P, P, 4, P, 0) == GEOMETRY
-    assert fast.mx_prefill(0, 64, 16, 2, P, 4, 0, 0, P, P, P, P, 0, 4, 1, 1, 0, P, 0) == ARGUMENT
-    assert fast.router_topk(0, P, 4, 8, 9, 1, P, P, 0) == GEOMETRY
-    assert fast.router_topk_grad(0, 0, P, P, P, 4, 8, 2, 0, P, 0) == ARGUMENT
-    assert fast.balance_work(2, 33, 8) == lib.iqk_balance_work(2, 33, 8)
-    assert fast.balance(0, P, 0, 0, 1, 4, 8, 2, P, P, P, P, 0) == ARGUMENT
-    assert fast.balance_grad(0, P, 0, P, 0, P, 1, 4, 8, 2, P, 0) == ARGUMENT
-    for bad in ((1 << 32, P, 4, 64, 64, P, P, 2, 0), (-1 << 40, P, 4, 64, 64, P, P, 2, 0)):
-        with pytest.raises(OverflowError):
-            fast.mx_quantize(*bad)
+            getattr(binding, name)()
+        with pytest.raises(TypeError):
+            getattr(binding, name)(*[0] * args)  # not tensors
+
+
+def test_a_missing_or_stale_torch_binding_is_refused(monkeypatch, tmp_path, lib):
+    monkeypatch.setattr(_native, "_TORCH", None)
+    monkeypatch.setattr(_native, "TORCH_EXT", tmp_path / "absent.so")
+    with pytest.raises(_native.IqkNativeError, match="not built"):
+        _native.torch_binding()
 
 
 def test_router_entry_points_refuse_bad_arguments(lib):

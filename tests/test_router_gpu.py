@@ -302,6 +302,19 @@ def test_graph_replays(device):
         assert all(torch.equal(g, w) for g, w in zip(got, step()))
 
 
+def test_a_second_derivative_is_refused(device):
+    print("second derivative", flush=True)
+    logits = torch.randn((6, 12), device=device).requires_grad_()
+    weights, ids = router.topk(logits, 3)
+    loss, _ = router.balance_loss(logits, ids)
+    for out in ((weights ** 2).sum(), loss ** 2):
+        (grad,) = torch.autograd.grad(out, logits, create_graph=True, retain_graph=True)
+        with pytest.raises(RuntimeError, match="second time"):
+            grad.sum().backward()
+        (again,) = torch.autograd.grad(out, logits, retain_graph=True)
+        assert torch.equal(again, grad) and not again.requires_grad
+
+
 def test_refusals(device):
     print("router refusals", flush=True)
     z = lambda *s, dtype=F32: torch.zeros(s, dtype=dtype, device=device)  # noqa: E731
