@@ -38,7 +38,7 @@ struct MxArgs {
     const uint32_t *xr;      // groups: activation rows, or null: the slots'
     const uint32_t *yr;      // groups: output rows, or null: the slots'
     uint16_t *y;
-    uint32_t K, N, rows, steps, quads, E, n_slots, n_x_rows, per_row, wide, set;
+    uint32_t K, N, rows, steps, quads, E, n_slots, n_x_rows, per_row, wide, set, run;
 };
 
 template <int ACT>
@@ -208,9 +208,13 @@ __global__ __launch_bounds__(64 * WAVES) void mx_pair_kernel(MxArgs a) {
 // list, and no workgroup without work but past the end.  (Numbers with gaps,
 // offs[e] / 64 + e on for expert e, need no scan, but their empty workgroups cost
 // more than their run: 256 experts of 64 slots took 451 us, and 286 without.)
-// The workgroups of an M-tile's outputs run on one XCD, four M-tiles together, so
-// that it reads a slot's activations once for all outputs and a slice of the weights
-// once for the four.
+// The workgroups of an M-tile's outputs run on one XCD, with those of the next
+// few M-tiles, so that it reads a slot's activations once for all outputs and a slice
+// of the weights once for an expert's M-tiles.  An XCD's workgroups go to its shader
+// engines in turn, whatever these still have to do, so consecutive ones are alike:
+// eight blocks of outputs of one M-tile.  (One M-tile a shader engine, as heavy as it
+// happens to be, left 27% of the wavefronts' places empty: 334 us against 317
+// on the 2048-token Zipf prefill.)
 constexpr int kMxBM = 64, kMxBN = 256, kMxWaves = 4;
 constexpr int kMxRowBytes = 256;          // of a slot and turn in LDS
 constexpr uint32_t kMxMaxExperts = 4096;  // 64 x 64, the two scans
@@ -229,13 +233,13 @@ struct MxTile {
 template <int BM>
 __device__ __forceinline__ bool find_tile(const MxArgs &a, MxTile &t) {
     const uint32_t nblocks = (a.N + kMxBN - 1) / kMxBN, lane = threadIdx.x & 63u;
-    // a set of 8 a.set M-tiles: a.set on each XCD, and there, for each block of
-    // outputs, one after another
+    // 8 a.set M-tiles at a time, a.set on each XCD; there a.run blocks of outputs of
+    // each of them, then the next a.run
     uint32_t u = blockIdx.x / nblocks, nb = blockIdx.x % nblocks;
     if (a.set) {
         const uint32_t span = 8u * a.set * nblocks, v = blockIdx.x / span, i = blockIdx.x % span, k = i >> 3;
-        u = (8u * v + (i & 7u)) * a.set + k % a.set;
-        nb = k / a.set;
+        u = (8u * v + (i & 7u)) * a.set + k / a.run % a.set;
+        nb = k / (a.run * a.set) * a.run + k % a.run;
     }
     t.n0 = nb * kMxBN;
     if (!a.offs) {
@@ -427,8 +431,10 @@ __device__ __forceinline__ void few_tile(const MxArgs &a, const MxTile &t, const
     const uint32_t lane = threadIdx.x & 63u, g = lane >> 4, r = lane & 15u;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t row0 = t.n0 + 64 * wave, steps = row0 < a.N ? a.steps : 0u;
-    MxWeights<ACT, AHEAD> w;
+    MxWeights<ACT, AHEAD> w;  // on their way before the slots' rows are known
     w.init(a, t.e, row0, lane);
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) w.load(i, i);
     // the lane's bytes of a step stand at [STEP step + STEP / 4 g, ..)
     const size_t row = slot_row(a, t, r);
     const uint32_t xbytes = MX ? a.K / 2 : 2 * a.K, end = r < t.n ? xbytes - STEP / 4 * g : 0u;
@@ -446,10 +452,7 @@ __device__ __forceinline__ void few_tile(const MxArgs &a, const MxTile &t, const
         if constexpr (MX) xs[slot] = *reinterpret_cast<const uint32_t *>(xscale + 4 * min(step, a.steps - 1u));
     };
 #pragma unroll
-    for (int i = 0; i < AHEAD; ++i) {
-        w.load(i, i);
-        load_x(i, i);
-    }
+    for (int i = 0; i < AHEAD; ++i) load_x(i, i);
     float4_t acc[4][1];
 #pragma unroll
     for (int i = 0; i < 4; ++i) acc[i][0] = float4_t{0, 0, 0, 0};
@@ -489,8 +492,10 @@ __device__ __forceinline__ void group_tile(const MxArgs &a, const MxTile &t, MxS
     const uint32_t tid = threadIdx.x, lane = tid & 63u, g = lane >> 4, r = lane & 15u;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const uint32_t row0 = t.n0 + 64 * wave, steps = a.steps;
-    MxWeights<ACT, AHEAD> w;
+    MxWeights<ACT, AHEAD> w;  // on their way before the slots' rows are known
     w.init(a, t.e, row0, lane);
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) w.load(i, i);
 
     // activations: chunk tid % CHUNKS of slots tid / CHUNKS + (256 / CHUNKS) i
     constexpr int PER = 256 / CHUNKS;
@@ -524,8 +529,6 @@ __device__ __forceinline__ void group_tile(const MxArgs &a, const MxTile &t, MxS
 
     load_x(0, 0);
     if constexpr (XR == 2) load_x(1, 1);
-#pragma unroll
-    for (int i = 0; i < AHEAD; ++i) w.load(i, i);
     float4_t acc[4][NC];
 #pragma unroll
     for (int i = 0; i < 4; ++i)
@@ -783,7 +786,10 @@ void launch_groups(MxArgs a, hipStream_t stream) {
         }
     }
     uint32_t mtiles = a.offs ? a.n_slots / kMxBM + min(a.E, a.n_slots) : (a.n_slots + kMxBM - 1) / kMxBM;
-    a.set = mtiles >= 64 ? 4 : mtiles >= 8 ? 1 : 0;
+    // an XCD takes as many M-tiles together as an expert has of them on average
+    const uint64_t even = a.offs ? uint64_t(kMxBM) * a.E : 1;
+    a.set = mtiles < 8 ? 0 : mtiles < 64 || a.n_slots <= even ? 1 : a.n_slots <= 3 * even ? 2 : 4;
+    a.run = nblocks % 8 == 0 ? 8 : nblocks % 4 == 0 ? 4 : nblocks < 16 ? nblocks : 1;
     // one matrix, fewer bytes of slots than of weights: the weights stay, a
     // block of outputs on one XCD
     if (!a.offs && uint64_t(a.n_slots) * (act_mx(ACT) ? 1 : 4) <= a.N) a.set = 0;
