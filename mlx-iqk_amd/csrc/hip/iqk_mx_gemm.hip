@@ -229,10 +229,10 @@ struct MxTile {
     uint32_t e, m0, n, n0;  // expert, first slot, slots, first output
 };
 
-// The workgroup's tile of at most BM slots; false (uniformly) past the last.
-template <int BM>
+// The workgroup's tile of at most BM slots by BN outputs; false (uniformly) past the last.
+template <int BM, int BN>
 __device__ __forceinline__ bool find_tile(const MxArgs &a, MxTile &t) {
-    const uint32_t nblocks = (a.N + kMxBN - 1) / kMxBN, lane = threadIdx.x & 63u;
+    const uint32_t nblocks = (a.N + BN - 1) / BN, lane = threadIdx.x & 63u;
     // 8 a.set M-tiles at a time, a.set on each XCD; there a.run blocks of outputs of
     // each of them, then the next a.run
     uint32_t u = blockIdx.x / nblocks, nb = blockIdx.x % nblocks;
@@ -241,7 +241,7 @@ __device__ __forceinline__ bool find_tile(const MxArgs &a, MxTile &t) {
         u = (8u * v + (i & 7u)) * a.set + k / a.run % a.set;
         nb = k / (a.run * a.set) * a.run + k % a.run;
     }
-    t.n0 = nb * kMxBN;
+    t.n0 = nb * BN;
     if (!a.offs) {
         t.e = 0;
         if (u >= (a.n_slots + BM - 1) / BM) return false;
@@ -420,21 +420,22 @@ __device__ __forceinline__ void store_outputs(const MxArgs &a, uint32_t e, uint3
 // wait for it.  So what lies past the end is read from a zero (activations) or is
 // the last step again (weights), and adds nothing.
 
-// A tile of at most 16 slots: the slots' rows come straight from memory in
-// the MFMA's layout too, so the wavefronts run on their own, with AHEAD steps of
-// both operands in flight, and HBM is kept busy.  (Eight steps of weights for
-// 16-bit slots too: 220 us against 203 over 256 experts of eight slots.)
+// Up to 16 slots by a wavefront's 64 outputs, over the steps first, first + stride, ..:
+// the slots' rows come straight from memory in the MFMA's layout too, so the
+// wavefronts run on their own, with AHEAD steps of both operands in flight, and HBM
+// is kept busy.  (Eight steps of weights for 16-bit slots too: 220 us against
+// 203 over 256 experts of eight slots.)
 template <int ACT>
-__device__ __forceinline__ void few_tile(const MxArgs &a, const MxTile &t, const MxShared &sh) {
+__device__ __forceinline__ void few_slots(const MxArgs &a, const MxTile &t, uint32_t row0, uint32_t first,
+                                          uint32_t stride, float4_t (&acc)[4][1]) {
     constexpr bool MX = act_mx(ACT);
     constexpr int AHEAD = MX ? 8 : 4, XN = MX ? 1 : 4, STEP = MX ? 64 : 256;
     const uint32_t lane = threadIdx.x & 63u, g = lane >> 4, r = lane & 15u;
-    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const uint32_t row0 = t.n0 + 64 * wave, steps = row0 < a.N ? a.steps : 0u;
+    const uint32_t steps = row0 < a.N ? a.steps : 0u;
     MxWeights<ACT, AHEAD> w;  // on their way before the slots' rows are known
     w.init(a, t.e, row0, lane);
 #pragma unroll
-    for (int i = 0; i < AHEAD; ++i) w.load(i, i);
+    for (int i = 0; i < AHEAD; ++i) w.load(i, first + i * stride);
     // the lane's bytes of a step stand at [STEP step + STEP / 4 g, ..)
     const size_t row = slot_row(a, t, r);
     const uint32_t xbytes = MX ? a.K / 2 : 2 * a.K, end = r < t.n ? xbytes - STEP / 4 * g : 0u;
@@ -447,20 +448,19 @@ __device__ __forceinline__ void few_tile(const MxArgs &a, const MxTile &t, const
         const uint32_t at = step * STEP;
         const bool in = int(at) < int(end);
 #pragma unroll
-        for (int j = 0; j < XN; ++j)
-            x[slot][j] = load_u4(in ? xsrc + at + 16 * j : zeros);
+        for (int j = 0; j < XN; ++j) x[slot][j] = load_u4(in ? xsrc + at + 16 * j : zeros);
         if constexpr (MX) xs[slot] = *reinterpret_cast<const uint32_t *>(xscale + 4 * min(step, a.steps - 1u));
     };
 #pragma unroll
-    for (int i = 0; i < AHEAD; ++i) load_x(i, i);
-    float4_t acc[4][1];
+    for (int i = 0; i < AHEAD; ++i) load_x(i, first + i * stride);
 #pragma unroll
     for (int i = 0; i < 4; ++i) acc[i][0] = float4_t{0, 0, 0, 0};
-    for (uint32_t s0 = 0; s0 < steps; s0 += AHEAD) {
+    for (uint32_t s0 = first; s0 < steps; s0 += AHEAD * stride) {
 #pragma unroll
         for (int i = 0; i < AHEAD; ++i) {
+            const uint32_t s = s0 + i * stride;
             if constexpr (MX) {
-                const uint32_t sx = clip_scales(xs[i], s0 + i, a.K / kMxBlock) >> (8 * g);
+                const uint32_t sx = clip_scales(xs[i], s, a.K / kMxBlock) >> (8 * g);
                 w.multiply4(i, x[i][0], sx, acc[0][0], acc[1][0], acc[2][0], acc[3][0]);
             } else {
 #pragma unroll
@@ -471,13 +471,57 @@ __device__ __forceinline__ void few_tile(const MxArgs &a, const MxTile &t, const
                     for (int k = 0; k < 4; ++k) acc[k][0] = mfma16<ACT>(wv[k], x[i][j], acc[k][0]);
                 }
             }
-            w.load(i, s0 + i + AHEAD);
-            load_x(i, s0 + i + AHEAD);
+            w.load(i, s + AHEAD * stride);
+            load_x(i, s + AHEAD * stride);
             __builtin_amdgcn_sched_barrier(0);
         }
     }
+}
+
+template <int ACT>
+__device__ __forceinline__ void few_tile(const MxArgs &a, const MxTile &t, const MxShared &sh) {
+    const uint32_t row0 = t.n0 + 64 * __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    float4_t acc[4][1];
+    few_slots<ACT>(a, t, row0, 0, 1, acc);
     __syncthreads();  // the slots' outputs
-    store_outputs<ACT, 4, 1>(a, t.e, row0, sh.dst, acc, lane);
+    store_outputs<ACT, 4, 1>(a, t.e, row0, sh.dst, acc, threadIdx.x & 63u);
+}
+
+// Where the tiles above would leave CUs without work: tiles of 16 slots by 64
+// outputs, whose four wavefronts split the reduction axis and add up in LDS, in
+// their order.  Two of them fit a CU, and a round of 512 takes 8 us with 4096
+// columns, hardly less with 2048; a round of 64 x 256 tiles up to 33 (4-bit slots:
+// 14) however few they are.  So split tiles serve while one round holds them, half
+// of one under 24 steps or for 4-bit slots: one matrix of 2048 outputs and 64 slots
+// 8.5 us against 32.6 (4-bit 8.8, 13.4), 8 experts of 8 slots 10.7 against 18.6;
+// past the limit 60 experts [1000 x 1440] of 10 slots (960 tiles) 20.1 against 14.8.
+constexpr int kSplitBM = 16, kSplitBN = 64;
+
+// About how many a call has: an expert one, or its share of the slots.
+inline uint64_t split_tiles(const MxArgs &a) {
+    const uint32_t experts = min(a.E, a.n_slots), all = (a.n_slots + kSplitBM - 1) / kSplitBM;
+    return uint64_t(max(experts, all)) * ((a.N + kSplitBN - 1) / kSplitBN);
+}
+
+template <int ACT>
+__global__ __launch_bounds__(64 * kMxWaves) __attribute__((amdgpu_waves_per_eu(2)))
+void mx_split_kernel(MxArgs a) {
+    __shared__ __attribute__((aligned(16))) float4_t part[kMxWaves][4][64];
+    __shared__ uint32_t dst[kSplitBM];
+    MxTile t;
+    if (!find_tile<kSplitBM, kSplitBN>(a, t)) return;
+    if (threadIdx.x < kSplitBM) dst[threadIdx.x] = slot_output(a, t, threadIdx.x);
+    const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    float4_t acc[4][1];
+    few_slots<ACT>(a, t, t.n0, wave, kMxWaves, acc);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) part[wave][i][lane] = acc[i][0];
+    __syncthreads();
+    // wavefront i adds up and stores tile row i
+    float4_t sum[1][1] = {{part[0][wave][lane]}};
+#pragma unroll
+    for (int i = 1; i < kMxWaves; ++i) sum[0][0] += part[i][wave][lane];
+    store_outputs<ACT, 1, 1>(a, t.e, t.n0 + kMxRows * wave, dst, sum, lane);
 }
 
 // A tile of at most 16 NC slots (NC > 1), T steps a turn: 16 KiB of slots, which
@@ -602,7 +646,7 @@ __global__ __launch_bounds__(64 * kMxWaves) __attribute__((amdgpu_waves_per_eu(2
 void mx_group_kernel(MxArgs a) {
     __shared__ MxShared sh;
     MxTile t;
-    if (!find_tile<kMxBM>(a, t)) return;
+    if (!find_tile<kMxBM, kMxBN>(a, t)) return;
     if (threadIdx.x < kMxBM) sh.dst[threadIdx.x] = slot_output(a, t, threadIdx.x);
     constexpr bool MX = act_mx(ACT);
     if (t.n <= 16)
@@ -633,7 +677,7 @@ constexpr int kBigBM = 256, kBigBN = 256, kBigWaves = 8, kBigRing = 4;
 constexpr uint32_t kBigTiles = 256;
 constexpr int kBigX = 16 * kMxTileBytes;        // [256 slots][64 bytes], chunks at chunk ^ big_swizzle(slot)
 constexpr int kBigWS = kBigX + kBigBM * 64;     // the outputs' words of scales: [4][64]
-constexpr int kBigXS = kBigWS + kBigBN * 4;     // the slots': [256]
+constexpr int kBigXS = kBigWS + kBigBN * 4;     // the slots': [2][16][8], slot 128 i + 16 k + j at [i][j][k]
 constexpr int kBigStage = kBigXS + kBigBM * 4;
 
 __device__ __forceinline__ uint32_t big_swizzle(uint32_t slot) { return (slot >> 2) & 2u; }
@@ -651,7 +695,7 @@ void mx_big_kernel(MxArgs a) {
     __shared__ __attribute__((aligned(16))) uint8_t lds[kBigRing * kBigStage];
     __shared__ uint32_t dst[kBigBM];
     MxTile t;
-    if (!find_tile<kBigBM>(a, t)) return;
+    if (!find_tile<kBigBM, kBigBN>(a, t)) return;
     const uint32_t tid = threadIdx.x, lane = tid & 63u, g = lane >> 4, r = lane & 15u;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6), wr = wave >> 1, wc = wave & 1u;
     if (tid < kBigBM) dst[tid] = slot_output(a, t, tid);
@@ -679,7 +723,9 @@ void mx_big_kernel(MxArgs a) {
             a.tscale + (size_t(t.e) * steps * a.quads + min(t.n0 / 64 + quarter, a.quads - 1u)) * 64 + lane);
         scales_step = size_t(a.quads) * 256;
     } else {
-        scales = a.xscale + size_t(slot_row(a, t, 64 * quarter + lane)) * a.xscale_stride;
+        const uint32_t at = 64 * quarter + lane;  // a lane's eight columns together
+        const uint32_t slot = (at & 128u) + 16 * (at & 7u) + (at >> 3 & 15u);
+        scales = a.xscale + size_t(slot_row(a, t, slot)) * a.xscale_stride;
         scales_step = 4;
     }
     const uint32_t scales_at = (wave < 4 ? kBigWS : kBigXS) + quarter * 256;
@@ -708,16 +754,17 @@ void mx_big_kernel(MxArgs a) {
 #pragma unroll
         for (int c = 0; c < 8; ++c) acc[i][c] = float4_t{0, 0, 0, 0};
     uint4_t w[2][4], x[4];
-    uint32_t sw[2], sx[4];
+    uint32_t sw[2];
+    uint4_t sx[2][2];
     const uint32_t wat = 4 * wr * kMxTileBytes + 16 * lane, swat = kBigWS + wr * 256 + 4 * lane;
-    const uint32_t xat = kBigX + (128 * wc + r) * 64 + 16 * (g ^ big_swizzle(r)), sxat = kBigXS + (128 * wc + r) * 4;
+    const uint32_t xat = kBigX + (128 * wc + r) * 64 + 16 * (g ^ big_swizzle(r)), sxat = kBigXS + (128 * wc + 8 * r) * 4;
     const auto read_w = [&](int buf, int i, const uint8_t *st) {
         w[buf][i] = load_u4(st + wat + i * kMxTileBytes);
         if (i == 0) sw[buf] = *reinterpret_cast<const uint32_t *>(st + swat);
+        if (i >= 2) sx[buf][i - 2] = load_u4(st + sxat + 16 * (i - 2));
     };
     const auto read_x = [&](int place, int c, const uint8_t *st) {
         x[place] = load_u4(st + xat + c * 1024);
-        sx[place] = *reinterpret_cast<const uint32_t *>(st + sxat + c * 64);
     };
     wait_stage<(kBigRing - 1) * LOADS>();
     const uint8_t *st = lds;
@@ -725,28 +772,29 @@ void mx_big_kernel(MxArgs a) {
     for (int i = 0; i < 4; ++i) read_w(0, i, st);
 #pragma unroll
     for (int c = 0; c < 3; ++c) read_x(c, c, st);
-    // Step s: step s + 1 has landed once only the loads of s + 2 and s + 3 are
-    // outstanding.  Step s + 3 goes where s - 1 stood, which all have read by the
-    // barrier at the start of s.
+    // In the middle of step s, with its slots' last columns read, the wavefronts
+    // meet: step s + 1 has landed once only the loads of s + 2 and s + 3 are
+    // outstanding, and s + 4 goes where s stood, three steps ahead.  (Meeting at the
+    // start of a step, with two ahead, takes as long: 172 us against 171 for 8192
+    // slots [8192 x 4096]; the step is LDS bandwidth, not the loads' latency.)
     for (uint32_t s0 = 0; s0 < steps; s0 += 2) {
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
-            if (s0 + b == 0)
-                wait_stage<(kBigRing - 2) * LOADS>();
-            else {
-                wait_stage<(kBigRing - 3) * LOADS>();
-                issue();
-            }
             const uint8_t *const next = st == lds + (kBigRing - 1) * kBigStage ? lds : st + kBigStage;
             const bool in = 4 * (s0 + b) + g < blocks;
 #pragma unroll
             for (int c = 0; c < 8; ++c) {
-                if (c < 4) read_w(b ^ 1, c, next);
+                if (c == 5) {
+                    wait_stage<(kBigRing - 2) * LOADS>();
+                    issue();
+                    read_w(b ^ 1, 0, next);
+                }
+                if (c >= 5) read_w(b ^ 1, c - 4, next);
                 read_x((c + 3) & 3, (c + 3) & 7, c < 5 ? st : next);
                 __builtin_amdgcn_sched_barrier(0);
                 const uint4_t bx = x[c & 3];
                 const int8v_t bv = {int(bx.x), int(bx.y), int(bx.z), int(bx.w), 0, 0, 0, 0};
-                const uint32_t raw = sx[c & 3] >> (8 * g);
+                const uint32_t raw = sx[b][c / 4][c % 4] >> (8 * g);
                 const int sb = int(in ? raw : 127u), sa = int(sw[b]);
                 const auto av = [&](int i) {
                     const uint4_t v = w[b][i];
@@ -775,6 +823,22 @@ void launch_pairs(const MxArgs &a, hipStream_t stream) {
         hipLaunchKernelGGL((mx_pair_kernel<ACT, 4>), grid, dim3{256}, 0, stream, a);
 }
 
+// The grid of tiles BM x BN, and how they go to the XCDs (find_tile).
+template <int ACT, int BM, int BN>
+dim3 tile_grid(MxArgs &a) {
+    const uint32_t nblocks = (a.N + BN - 1) / BN;
+    uint32_t mtiles = a.offs ? a.n_slots / BM + min(a.E, a.n_slots) : (a.n_slots + BM - 1) / BM;
+    // an XCD takes as many M-tiles together as an expert has of them on average
+    const uint64_t even = a.offs ? uint64_t(BM) * a.E : 1;
+    a.set = mtiles < 8 ? 0 : mtiles < 64 || a.n_slots <= even ? 1 : a.n_slots <= 3 * even ? 2 : 4;
+    a.run = nblocks % 8 == 0 ? 8 : nblocks % 4 == 0 ? 4 : nblocks < 16 ? nblocks : 1;
+    // one matrix, fewer bytes of slots than of weights: the weights stay, a
+    // block of outputs on one XCD
+    if (!a.offs && uint64_t(a.n_slots) * (act_mx(ACT) ? 1 : 4) <= a.N) a.set = 0;
+    if (a.set) mtiles = (mtiles + 8 * a.set - 1) / (8 * a.set) * (8 * a.set);
+    return dim3{mtiles * nblocks};
+}
+
 template <int ACT>
 void launch_groups(MxArgs a, hipStream_t stream) {
     const uint32_t nblocks = (a.N + kMxBN - 1) / kMxBN;
@@ -785,16 +849,13 @@ void launch_groups(MxArgs a, hipStream_t stream) {
             return;
         }
     }
-    uint32_t mtiles = a.offs ? a.n_slots / kMxBM + min(a.E, a.n_slots) : (a.n_slots + kMxBM - 1) / kMxBM;
-    // an XCD takes as many M-tiles together as an expert has of them on average
-    const uint64_t even = a.offs ? uint64_t(kMxBM) * a.E : 1;
-    a.set = mtiles < 8 ? 0 : mtiles < 64 || a.n_slots <= even ? 1 : a.n_slots <= 3 * even ? 2 : 4;
-    a.run = nblocks % 8 == 0 ? 8 : nblocks % 4 == 0 ? 4 : nblocks < 16 ? nblocks : 1;
-    // one matrix, fewer bytes of slots than of weights: the weights stay, a
-    // block of outputs on one XCD
-    if (!a.offs && uint64_t(a.n_slots) * (act_mx(ACT) ? 1 : 4) <= a.N) a.set = 0;
-    if (a.set) mtiles = (mtiles + 8 * a.set - 1) / (8 * a.set) * (8 * a.set);
-    hipLaunchKernelGGL((mx_group_kernel<ACT>), dim3{mtiles * nblocks}, dim3{64 * kMxWaves}, 0, stream, a);
+    if (split_tiles(a) <= (a.steps >= 24 ? 512u : 256u) / (act_mx(ACT) ? 2 : 1)) {
+        const dim3 grid = tile_grid<ACT, kSplitBM, kSplitBN>(a);
+        hipLaunchKernelGGL((mx_split_kernel<ACT>), grid, dim3{64 * kMxWaves}, 0, stream, a);
+        return;
+    }
+    const dim3 grid = tile_grid<ACT, kMxBM, kMxBN>(a);
+    hipLaunchKernelGGL((mx_group_kernel<ACT>), grid, dim3{64 * kMxWaves}, 0, stream, a);
 }
 
 bool at16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }

@@ -37,7 +37,14 @@ _DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 _ACTS = {(torch.float16, False): 0, (torch.bfloat16, False): 1, (torch.float16, True): 2, (torch.bfloat16, True): 3}
 
 PAIR_LIMIT = 63
-"""Token-expert pairs up to which each pair is computed on its own."""
+"""Token-expert pairs up to which each pair is computed on its own, where they
+are at most eight more than the experts; beyond, experts are named again and again
+and their weights better read once (eight experts: 16 pairs 11.2 us against
+10.7 and 5 for the grouping, 64 pairs 29 against 11)."""
+ROW_LIMIT = 16384
+"""Outputs in all up to which the rows of an :class:`MxLinear` are computed on their
+own (2048 outputs: 8 rows 5.6 us against 7.8, 16 rows 8.9 against 8.4; 8192
+outputs: 4 rows 10.1 against 8.5)."""
 
 
 def _check_width(n: int) -> int:
@@ -287,9 +294,9 @@ class MxSwitchLinear(_MxStack):
         return self._dequantized(dtype)
 
     def forward(self, x, indices: torch.Tensor, sorted_indices: bool = False) -> torch.Tensor:
-        """Project ``x`` through the experts named by ``indices``: up to
-        :data:`PAIR_LIMIT` pairs each on its own, else (or with
-        ``sorted_indices``) grouped by expert on the device."""
+        """Project ``x`` through the experts named by ``indices``: few pairs
+        each on its own (:data:`PAIR_LIMIT`), else (or with ``sorted_indices``) grouped
+        by expert on the device."""
         if len(x.shape) < 2:
             raise IqkRuntimeError(f"x must be [..., M, {self.in_features}], got {tuple(x.shape)}")
         tiles = self._buffers["tiles"]
@@ -311,7 +318,7 @@ class MxSwitchLinear(_MxStack):
                 or ids.get_device() != tiles.get_device():
             ids = self._ids(indices, batch)
         pairs = math.prod(batch)
-        grouped = sorted_indices or M != 1 or pairs > PAIR_LIMIT
+        grouped = sorted_indices or M != 1 or pairs > min(PAIR_LIMIT, self.num_experts + 8)
         return self._project((act, rows, scales, stride), ids, (*batch, M, self.out_features), pairs, M, per_row,
                              grouped)
 
@@ -353,7 +360,7 @@ class MxLinear(_MxStack):
         x = self._activations(x, tiles)
         lead = x[1].shape[:-1]
         n = math.prod(lead)
-        return self._project(x, None, (*lead, self.out_features), n, 1, 1, n > 4)
+        return self._project(x, None, (*lead, self.out_features), n, 1, 1, n > 1 and n * self.out_features > ROW_LIMIT)
 
     def extra_repr(self) -> str:
         return f"{self.out_features}, {self.in_features}"

@@ -181,8 +181,8 @@ def test_few_pairs(device, quantized, dtype, E, out, n):
     print(f"pairs {quantized} {dtype} {E} {out} {n}", flush=True)
     rng = np.random.default_rng(out + n)
     module, w = _switch(rng, E, out, n, device)
-    for tokens, k, per_pair, wide in ((1, 1, False, False), (1, 2, False, True), (5, 2, False, False),
-                                      (7, 2, True, True)):
+    for tokens, k, per_pair, wide in ((1, 1, False, False), (1, 2, False, True), (4, 2, False, False),
+                                      (5, 2, True, True)):
         ids = rng.integers(0, E, (tokens, k))
         x, xv = _operand(rng, tokens * k if per_pair else tokens, n, dtype, quantized, device)
         y = module(_shape(x, tokens, k, 1) if per_pair else _shape(x, tokens, 1, 1),
@@ -193,14 +193,15 @@ def test_few_pairs(device, quantized, dtype, E, out, n):
 
 
 # pairs of each expert: none, one, the tile's quarters and both sides of them,
-# a tile, one more, several
+# a tile, one more, several; few outputs go to the tiles that split the reduction
+# axis, thousands to the others
 COUNTS = ([0, 1, 15, 16, 17, 0], [32, 33, 48, 49], [64, 65, 128, 129, 3], [300, 0, 0, 7, 81, 97, 113])
 
 
 @pytest.mark.parametrize("quantized", (False, True))
 @pytest.mark.parametrize("dtype", HALF)
 @pytest.mark.parametrize("counts", COUNTS, ids=lambda c: "-".join(map(str, c)))
-@pytest.mark.parametrize("out,n", ((48, 128), (257, 160), (300, 1440), (512, 768)))
+@pytest.mark.parametrize("out,n", ((48, 128), (257, 160), (300, 1440), (100, 3360), (4100, 160), (4352, 1440)))
 def test_groups(device, quantized, dtype, counts, out, n):
     print(f"groups {quantized} {dtype} {counts} {out} {n}", flush=True)
     rng = np.random.default_rng(out + n + len(counts))
@@ -303,9 +304,9 @@ def test_bad_rows_stay_where_they_are(device, quantized, n, pairs):
 
 
 @pytest.mark.parametrize("dtype", HALF)
-@pytest.mark.parametrize("pairs", (5, 100))
+@pytest.mark.parametrize("pairs", (5, 100, 1500))
 def test_rows_of_very_different_scales(device, dtype, pairs):
-    """Rows from 2^-100 to 2^100, blocks 36 powers of two apart in a row."""
+    """Rows from 2^-100 to 2^100, blocks 36 powers of two apart in a row, by every route."""
     print(f"scales apart {dtype} {pairs}", flush=True)
     rng = np.random.default_rng(21)
     E, out, n = 2, 48, 256
@@ -329,7 +330,8 @@ def test_rows_of_very_different_scales(device, dtype, pairs):
 
 
 @pytest.mark.parametrize("quantized", (False, True))
-@pytest.mark.parametrize("rows,out,n", ((1, 33, 96), (4, 64, 1440), (5, 300, 160), (128, 256, 512), (200, 700, 1056)))
+@pytest.mark.parametrize("rows,out,n", ((1, 33, 96), (4, 64, 1440), (5, 300, 160), (5, 4000, 160), (17, 1100, 3168),
+                                        (128, 256, 512), (200, 700, 1056), (300, 2100, 1056)))
 def test_linear(device, quantized, rows, out, n):
     print(f"linear {quantized} {rows} {out} {n}", flush=True)
     rng = np.random.default_rng(rows)
