@@ -330,7 +330,8 @@ int iqk_mx_groups(int act, int64_t in_features, int64_t out_features, int64_t nu
 
 // A switch module's grouped call in one: iqk_route (wide_ids: iqk_route_ids64)
 // over n_pairs ids, then iqk_mx_groups on its lists, with the outputs and
-// refusals of the two.  work: u32 [2 n_pairs rows_per_pair + num_experts + 1].
+// refusals of the two.  Few pairs are sorted by the products themselves, in the
+// same order.  work: u32 [2 n_pairs rows_per_pair + num_experts + 1].
 int iqk_mx_prefill(int act, int64_t in_features, int64_t out_features, int64_t num_experts, const void *x,
                    int64_t n_x_rows, const uint8_t *x_scales, int64_t x_scale_stride, const void *tiles,
                    const uint8_t *tile_scales, const int32_t *row_exps, const void *ids, int wide_ids,

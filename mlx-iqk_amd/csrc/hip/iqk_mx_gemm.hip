@@ -229,38 +229,28 @@ struct MxTile {
     uint32_t e, m0, n, n0;  // expert, first slot, slots, first output
 };
 
-// The workgroup's tile of at most BM slots by BN outputs; false (uniformly) past the last.
-template <int BM, int BN>
-__device__ __forceinline__ bool find_tile(const MxArgs &a, MxTile &t) {
-    const uint32_t nblocks = (a.N + BN - 1) / BN, lane = threadIdx.x & 63u;
-    // 8 a.set M-tiles at a time, a.set on each XCD; there a.run blocks of outputs of
-    // each of them, then the next a.run
+// The M-tile and the block of outputs of the workgroup: 8 a.set M-tiles at a time,
+// a.set on each XCD; there a.run blocks of outputs of each of them, then the next a.run.
+template <int BN>
+__device__ __forceinline__ uint32_t tile_place(const MxArgs &a, uint32_t &n0) {
+    const uint32_t nblocks = (a.N + BN - 1) / BN;
     uint32_t u = blockIdx.x / nblocks, nb = blockIdx.x % nblocks;
     if (a.set) {
         const uint32_t span = 8u * a.set * nblocks, v = blockIdx.x / span, i = blockIdx.x % span, k = i >> 3;
         u = (8u * v + (i & 7u)) * a.set + k / a.run % a.set;
         nb = k / (a.run * a.set) * a.run + k % a.run;
     }
-    t.n0 = nb * BN;
-    if (!a.offs) {
-        t.e = 0;
-        if (u >= (a.n_slots + BM - 1) / BM) return false;
-        t.m0 = u * BM;
-        t.n = min(a.n_slots - t.m0, uint32_t(BM));
-        return true;
-    }
-    // lane l counts the M-tiles of `per` experts from l per on; the lane whose
-    // count holds u is then taken apart, a lane an expert
-    const uint32_t per = (a.E + 63u) / 64u;
-    const auto tiles_of = [&](uint32_t from, uint32_t n) {
-        uint32_t count = 0, lo = a.offs[min(from, a.E)];
-        for (uint32_t i = 1; i <= n; ++i) {
-            const uint32_t hi = a.offs[min(from + i, a.E)];
-            count += (hi - lo + BM - 1u) / BM;
-            lo = hi;
-        }
-        return count;
-    };
+    n0 = nb * BN;
+    return u;
+}
+
+// The expert that holds M-tile u of all, or a.E past the last; u becomes its place in
+// the expert.  tiles_of(from, n): the M-tiles of experts from .. from + n - 1.  Lane l
+// counts those of `per` experts from l per on; the lane whose count holds u is
+// then taken apart, a lane an expert.
+template <class F>
+__device__ __forceinline__ uint32_t find_expert(const MxArgs &a, uint32_t &u, F tiles_of) {
+    const uint32_t lane = threadIdx.x & 63u, per = (a.E + 63u) / 64u;
     // the first lane whose running total exceeds u; u becomes its place in that lane
     const auto find = [&](uint32_t count) {
         uint32_t total = count;
@@ -275,15 +265,33 @@ __device__ __forceinline__ bool find_tile(const MxArgs &a, MxTile &t) {
         u -= uint32_t(__builtin_amdgcn_readlane(int(total - count), at));
         return uint32_t(at);
     };
-    uint32_t at = find(tiles_of(lane * per, per));
-    if (at == 64u) return false;  // past the last tile
-    if (per == 1) {
-        t.e = at;
-    } else {
-        const uint32_t first = at * per;
-        at = find(lane < per ? tiles_of(first + lane, 1) : 0u);
-        t.e = first + at;
+    const uint32_t at = find(tiles_of(lane * per, per));
+    if (at == 64u) return a.E;  // past the last tile
+    if (per == 1) return at;
+    const uint32_t first = at * per;
+    return first + find(lane < per ? tiles_of(first + lane, 1) : 0u);
+}
+
+// The workgroup's tile of at most BM slots by BN outputs; false (uniformly) past the last.
+template <int BM, int BN>
+__device__ __forceinline__ bool find_tile(const MxArgs &a, MxTile &t) {
+    uint32_t u = tile_place<BN>(a, t.n0);
+    if (!a.offs) {
+        t.e = 0;
+        if (u >= (a.n_slots + BM - 1) / BM) return false;
+        t.m0 = u * BM;
+        t.n = min(a.n_slots - t.m0, uint32_t(BM));
+        return true;
     }
+    t.e = find_expert(a, u, [&](uint32_t from, uint32_t n) {
+        uint32_t count = 0, lo = a.offs[min(from, a.E)];
+        for (uint32_t i = 1; i <= n; ++i) {
+            const uint32_t hi = a.offs[min(from + i, a.E)];
+            count += (hi - lo + BM - 1u) / BM;
+            lo = hi;
+        }
+        return count;
+    });
     if (t.e >= a.E) return false;
     const uint32_t lo = a.offs[t.e], hi = min(a.offs[t.e + 1], a.n_slots);
     const uint64_t m0 = uint64_t(lo) + uint64_t(u) * BM;
@@ -293,10 +301,98 @@ __device__ __forceinline__ bool find_tile(const MxArgs &a, MxTile &t) {
     return true;
 }
 
+// Few pairs are grouped by the workgroups themselves, which spares the launch
+// that sorts them: each counts the experts' pairs in LDS, finds its tile and the pairs
+// of its expert that are in it, in their order.
+// The sorting takes 3.5 us; this up to 1 us a workgroup at 1024 pairs, so it has to
+// be spared where workgroups are many (ids_pay: a round of 256 ids for 4096 of
+// them): 60 experts [1000 x 1440], 596 pairs 14.7 us against 18.3 (0.25 of a
+// limit), 256 experts [2048 x 4096], 400 pairs 152 against 157 (1), but 256 of
+// [4096 x 2048], 1000 pairs 207 against 205 (4).
+constexpr uint32_t kIdsPairs = 1024, kIdsExperts = 512;
+constexpr int kIdsRounds = kIdsPairs / 256;
+
+inline bool ids_pay(const MxArgs &a) {
+    const uint64_t tiles = uint64_t(min(a.E, a.n_slots)) * ((a.N + kMxBN - 1) / kMxBN);
+    return a.n_slots <= kIdsPairs && a.E <= kIdsExperts && tiles * ((a.n_slots + 255) / 256) <= 4096;
+}
+
+struct MxIds {
+    uint32_t count[kIdsExperts];
+    uint32_t hits[kIdsRounds][kMxWaves];
+};
+
+// A tile's slots: activation row, and output row, bit 31 where the slot's activations
+// are real (~0: no slot).
+template <int BM>
+struct MxSlots {
+    uint32_t row[BM], dst[BM];
+};
+
+// find_tile for the pairs a.ids, with the tile's slots.
+template <int BM, int BN>
+__device__ __forceinline__ bool find_ids(const MxArgs &a, MxTile &t, MxIds &sh, MxSlots<BM> &slots) {
+    const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    uint32_t id[kIdsRounds];
+#pragma unroll
+    for (int i = 0; i < kIdsRounds; ++i) {
+        const uint32_t p = tid + 256 * i;
+        if (256u * i < a.n_slots) id[i] = expert_id(a.ids, min(p, a.n_slots - 1u), a.wide);
+    }
+    for (uint32_t e = tid; e < a.E; e += 256) sh.count[e] = 0;
+    if (tid < BM) {
+        slots.row[tid] = 0;
+        slots.dst[tid] = 0xffffffffu;
+    }
+    __syncthreads();
+    // an id out of range counts as the last expert's
+#pragma unroll
+    for (int i = 0; i < kIdsRounds; ++i)
+        if (tid + 256 * i < a.n_slots) atomicAdd(&sh.count[min(id[i], a.E - 1u)], 1u);
+    __syncthreads();
+    uint32_t u = tile_place<BN>(a, t.n0);
+    t.e = find_expert(a, u, [&](uint32_t from, uint32_t n) {
+        uint32_t tiles = 0;
+        for (uint32_t e = from; e < min(from + n, a.E); ++e) tiles += (sh.count[e] + BM - 1u) / BM;
+        return tiles;
+    });
+    if (t.e >= a.E) return false;
+    t.m0 = u * BM;  // of the expert's pairs
+    t.n = min(sh.count[t.e] - t.m0, uint32_t(BM));
+    uint64_t hit[kIdsRounds];
+#pragma unroll
+    for (int i = 0; i < kIdsRounds; ++i) {
+        hit[i] = __ballot(tid + 256 * i < a.n_slots && min(id[i], a.E - 1u) == t.e);
+        if (lane == 0) sh.hits[i][wave] = uint32_t(__popcll(hit[i]));
+    }
+    __syncthreads();
+    uint32_t before = 0;
+#pragma unroll
+    for (int i = 0; i < kIdsRounds; ++i) {
+        if (256u * i >= a.n_slots) break;
+        uint32_t all = 0, mine = 0;
+#pragma unroll
+        for (uint32_t w = 0; w < kMxWaves; ++w) {
+            const uint32_t n = sh.hits[i][w];
+            mine += w < wave ? n : 0u;
+            all += n;
+        }
+        const uint32_t at = before + mine + uint32_t(__popcll(hit[i] & ((uint64_t(1) << lane) - 1u))) - t.m0;
+        if ((hit[i] >> lane & 1u) && at < BM) {
+            const uint32_t p = tid + 256 * i, row = p / a.per_row;
+            const bool real = id[i] < a.E && row < a.n_x_rows;
+            slots.row[at] = real ? row : 0u;
+            slots.dst[at] = p | (real ? 0x80000000u : 0u);
+        }
+        before += all;
+    }
+    __syncthreads();
+    return true;
+}
+
 struct MxShared {
     __attribute__((aligned(16))) uint8_t x[2][kMxBM * kMxRowBytes];
     uint32_t xs[2][256];  // 4-bit slots' scales, a word a step
-    uint32_t dst[kMxBM];  // output row, bit 31 where the slot's activations are real
 };
 
 // A word of scales (a step's four blocks) with those of blocks past the row's end made 1.
@@ -359,6 +455,10 @@ __device__ __forceinline__ uint32_t slot_row(const MxArgs &a, const MxTile &t, u
     if (slot < t.n) row = a.xr ? a.xr[t.m0 + slot] : t.m0 + slot;
     return row < a.n_x_rows ? row : 0u;
 }
+template <bool IDS, int BM>
+__device__ __forceinline__ uint32_t slot_row(const MxArgs &a, const MxTile &t, const MxSlots<BM> &slots, uint32_t slot) {
+    return IDS ? slots.row[slot] : slot_row(a, t, slot);
+}
 
 // A slot's output row, bit 31 set where its activations are real (else it is NaN); ~0: not stored.
 __device__ __forceinline__ uint32_t slot_output(const MxArgs &a, const MxTile &t, uint32_t in_tile) {
@@ -418,26 +518,28 @@ __device__ __forceinline__ void store_outputs(const MxArgs &a, uint32_t e, uint3
 // and no loaded value is touched before its use: a branch or a select there
 // makes the compiler copy the registers that a load in flight will fill, and
 // wait for it.  So what lies past the end is read from a zero (activations) or is
-// the last step again (weights), and adds nothing.
+// the last step again (weights), and adds nothing.  The loads before a loop are in
+// the order in which its rounds leave them: the waits inside count the loads
+// behind the awaited one, and take the fewest of the two ways in.  (All weights
+// first, then all slots: the loops waited for everything once a round; 8 experts [2048
+// x 4096] of 32 slots took 27.0 us against 23.3, 32 of 32 40.3 against 34.3.)
 
 // Up to 16 slots by a wavefront's 64 outputs, over the steps first, first + stride, ..:
 // the slots' rows come straight from memory in the MFMA's layout too, so the
 // wavefronts run on their own, with AHEAD steps of both operands in flight, and HBM
 // is kept busy.  (Eight steps of weights for 16-bit slots too: 220 us against
 // 203 over 256 experts of eight slots.)
-template <int ACT>
-__device__ __forceinline__ void few_slots(const MxArgs &a, const MxTile &t, uint32_t row0, uint32_t first,
-                                          uint32_t stride, float4_t (&acc)[4][1]) {
+template <int ACT, bool IDS, int BM>
+__device__ __forceinline__ void few_slots(const MxArgs &a, const MxTile &t, const MxSlots<BM> &slots, uint32_t row0,
+                                          uint32_t first, uint32_t stride, float4_t (&acc)[4][1]) {
     constexpr bool MX = act_mx(ACT);
     constexpr int AHEAD = MX ? 8 : 4, XN = MX ? 1 : 4, STEP = MX ? 64 : 256;
     const uint32_t lane = threadIdx.x & 63u, g = lane >> 4, r = lane & 15u;
     const uint32_t steps = row0 < a.N ? a.steps : 0u;
-    MxWeights<ACT, AHEAD> w;  // on their way before the slots' rows are known
+    MxWeights<ACT, AHEAD> w;
     w.init(a, t.e, row0, lane);
-#pragma unroll
-    for (int i = 0; i < AHEAD; ++i) w.load(i, first + i * stride);
     // the lane's bytes of a step stand at [STEP step + STEP / 4 g, ..)
-    const size_t row = slot_row(a, t, r);
+    const size_t row = slot_row<IDS>(a, t, slots, r);
     const uint32_t xbytes = MX ? a.K / 2 : 2 * a.K, end = r < t.n ? xbytes - STEP / 4 * g : 0u;
     const global_ptr xsrc = global_ptr(a.x) + row * xbytes + STEP / 4 * g;
     const uint8_t *const xscale = MX ? a.xscale + row * a.xscale_stride : nullptr;
@@ -452,7 +554,11 @@ __device__ __forceinline__ void few_slots(const MxArgs &a, const MxTile &t, uint
         if constexpr (MX) xs[slot] = *reinterpret_cast<const uint32_t *>(xscale + 4 * min(step, a.steps - 1u));
     };
 #pragma unroll
-    for (int i = 0; i < AHEAD; ++i) load_x(i, first + i * stride);
+    for (int i = 0; i < AHEAD; ++i) {
+        w.load(i, first + i * stride);
+        load_x(i, first + i * stride);
+        __builtin_amdgcn_sched_barrier(0);
+    }
 #pragma unroll
     for (int i = 0; i < 4; ++i) acc[i][0] = float4_t{0, 0, 0, 0};
     for (uint32_t s0 = first; s0 < steps; s0 += AHEAD * stride) {
@@ -478,23 +584,24 @@ __device__ __forceinline__ void few_slots(const MxArgs &a, const MxTile &t, uint
     }
 }
 
-template <int ACT>
-__device__ __forceinline__ void few_tile(const MxArgs &a, const MxTile &t, const MxShared &sh) {
+template <int ACT, bool IDS>
+__device__ __forceinline__ void few_tile(const MxArgs &a, const MxTile &t, const MxSlots<kMxBM> &slots) {
     const uint32_t row0 = t.n0 + 64 * __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     float4_t acc[4][1];
-    few_slots<ACT>(a, t, row0, 0, 1, acc);
+    few_slots<ACT, IDS>(a, t, slots, row0, 0, 1, acc);
     __syncthreads();  // the slots' outputs
-    store_outputs<ACT, 4, 1>(a, t.e, row0, sh.dst, acc, threadIdx.x & 63u);
+    store_outputs<ACT, 4, 1>(a, t.e, row0, slots.dst, acc, threadIdx.x & 63u);
 }
 
 // Where the tiles above would leave CUs without work: tiles of 16 slots by 64
 // outputs, whose four wavefronts split the reduction axis and add up in LDS, in
-// their order.  Two of them fit a CU, and a round of 512 takes 8 us with 4096
-// columns, hardly less with 2048; a round of 64 x 256 tiles up to 33 (4-bit slots:
-// 14) however few they are.  So split tiles serve while one round holds them, half
-// of one under 24 steps or for 4-bit slots: one matrix of 2048 outputs and 64 slots
-// 8.5 us against 32.6 (4-bit 8.8, 13.4), 8 experts of 8 slots 10.7 against 18.6;
-// past the limit 60 experts [1000 x 1440] of 10 slots (960 tiles) 20.1 against 14.8.
+// their order.  Two of them fit a CU, and a round of 512 takes 10 us with 4096
+// columns and 8 with 1440 (4-bit slots: as long); one of 64 x 256 tiles as long as
+// its slots: 14 us for a few, 23 for 16, 35 for 64 (4-bit: 12, 17, 16).  So split
+// tiles serve while one round holds them, half of one for 4-bit slots or under 24
+// steps: 8 experts [2048 x 4096] of 8 slots 10.0 us against 17.8 (4-bit 10.6,
+// 14.7), of 32 slots 17.2 against 22.3 (4-bit, past the limit: 17.2, 12.8); 16 of 24
+// slots, past it, 32.5 against 24.7, 60 experts [1000 x 1440] of 10 22.5 against 14.3.
 constexpr int kSplitBM = 16, kSplitBN = 64;
 
 // About how many a call has: an expert one, or its share of the slots.
@@ -503,17 +610,30 @@ inline uint64_t split_tiles(const MxArgs &a) {
     return uint64_t(max(experts, all)) * ((a.N + kSplitBN - 1) / kSplitBN);
 }
 
-template <int ACT>
+// The workgroup's tile and its slots, from the lists or the pairs' ids; without IDS,
+// slots.dst is there after the next barrier.
+template <bool IDS, int BM, int BN>
+__device__ __forceinline__ bool find(const MxArgs &a, MxTile &t, MxSlots<BM> &slots) {
+    if constexpr (IDS) {
+        __shared__ MxIds ids;
+        return find_ids<BM, BN>(a, t, ids, slots);
+    } else {
+        if (!find_tile<BM, BN>(a, t)) return false;
+        if (threadIdx.x < BM) slots.dst[threadIdx.x] = slot_output(a, t, threadIdx.x);
+        return true;
+    }
+}
+
+template <int ACT, bool IDS>
 __global__ __launch_bounds__(64 * kMxWaves) __attribute__((amdgpu_waves_per_eu(2)))
 void mx_split_kernel(MxArgs a) {
     __shared__ __attribute__((aligned(16))) float4_t part[kMxWaves][4][64];
-    __shared__ uint32_t dst[kSplitBM];
+    __shared__ MxSlots<kSplitBM> slots;
     MxTile t;
-    if (!find_tile<kSplitBM, kSplitBN>(a, t)) return;
-    if (threadIdx.x < kSplitBM) dst[threadIdx.x] = slot_output(a, t, threadIdx.x);
+    if (!find<IDS, kSplitBM, kSplitBN>(a, t, slots)) return;
     const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     float4_t acc[4][1];
-    few_slots<ACT>(a, t, t.n0, wave, kMxWaves, acc);
+    few_slots<ACT, IDS>(a, t, slots, t.n0, wave, kMxWaves, acc);
 #pragma unroll
     for (int i = 0; i < 4; ++i) part[wave][i][lane] = acc[i][0];
     __syncthreads();
@@ -521,13 +641,14 @@ void mx_split_kernel(MxArgs a) {
     float4_t sum[1][1] = {{part[0][wave][lane]}};
 #pragma unroll
     for (int i = 1; i < kMxWaves; ++i) sum[0][0] += part[i][wave][lane];
-    store_outputs<ACT, 1, 1>(a, t.e, t.n0 + kMxRows * wave, dst, sum, lane);
+    store_outputs<ACT, 1, 1>(a, t.e, t.n0 + kMxRows * wave, slots.dst, sum, lane);
 }
 
 // A tile of at most 16 NC slots (NC > 1), T steps a turn: 16 KiB of slots, which
 // are loaded XR turns before they go into LDS.
-template <int ACT, int NC, int T, int AHEAD, int XR>
-__device__ __forceinline__ void group_tile(const MxArgs &a, const MxTile &t, MxShared &sh) {
+template <int ACT, bool IDS, int NC, int T, int AHEAD, int XR>
+__device__ __forceinline__ void group_tile(const MxArgs &a, const MxTile &t, const MxSlots<kMxBM> &slots,
+                                           MxShared &sh) {
     constexpr bool MX = act_mx(ACT);
     constexpr int STEP = MX ? 64 : 256;             // bytes of a slot and step
     constexpr int ROW = T * STEP, CHUNKS = ROW / 16;  // of a slot and turn
@@ -536,10 +657,8 @@ __device__ __forceinline__ void group_tile(const MxArgs &a, const MxTile &t, MxS
     const uint32_t tid = threadIdx.x, lane = tid & 63u, g = lane >> 4, r = lane & 15u;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const uint32_t row0 = t.n0 + 64 * wave, steps = a.steps;
-    MxWeights<ACT, AHEAD> w;  // on their way before the slots' rows are known
+    MxWeights<ACT, AHEAD> w;
     w.init(a, t.e, row0, lane);
-#pragma unroll
-    for (int i = 0; i < AHEAD; ++i) w.load(i, i);
 
     // activations: chunk tid % CHUNKS of slots tid / CHUNKS + (256 / CHUNKS) i
     constexpr int PER = 256 / CHUNKS;
@@ -549,15 +668,16 @@ __device__ __forceinline__ void group_tile(const MxArgs &a, const MxTile &t, MxS
 #pragma unroll
     for (int i = 0; i < XL; ++i) {
         const uint32_t slot = slot0 + PER * i;
-        xsrc[i] = global_ptr(a.x) + size_t(slot_row(a, t, slot)) * xbytes + 16 * chunk;
+        xsrc[i] = global_ptr(a.x) + size_t(slot_row<IDS>(a, t, slots, slot)) * xbytes + 16 * chunk;
         put[i] = slot * ROW + 16 * ((chunk & ~15u) | ((chunk & 15u) ^ swizzle<ACT>(slot)));
     }
     // 4-bit slots' scales: word tid % T of slot tid / T
     const uint8_t *const xscale =
-        MX ? a.xscale + size_t(slot_row(a, t, min(tid / T, uint32_t(16 * NC - 1)))) * a.xscale_stride : nullptr;
+        MX ? a.xscale + size_t(slot_row<IDS>(a, t, slots, min(tid / T, uint32_t(16 * NC - 1)))) * a.xscale_stride
+           : nullptr;
     const global_ptr zeros = zero_chunk();
-    uint4_t xv[XR][XL];
-    uint32_t xsv[XR];
+    uint4_t xv[XR + 1][XL];  // the last for the first turn's
+    uint32_t xsv[XR + 1];
     const auto load_x = [&](int reg, uint32_t turn) {
         const bool in = turn * ROW + 16 * chunk < xbytes;
 #pragma unroll
@@ -571,15 +691,23 @@ __device__ __forceinline__ void group_tile(const MxArgs &a, const MxTile &t, MxS
         if constexpr (MX) sh.xs[buf][tid] = clip_scales(xsv[reg], T * turn + tid % T, a.K / kMxBlock);
     };
 
-    load_x(0, 0);
+    load_x(XR, 0);
     if constexpr (XR == 2) load_x(1, 1);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int i = 0; i < AHEAD - T; ++i) w.load(i, i);
+    __builtin_amdgcn_sched_barrier(0);
+    load_x(0, XR);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int i = AHEAD - T; i < AHEAD; ++i) w.load(i, i);
+    __builtin_amdgcn_sched_barrier(0);
     float4_t acc[4][NC];
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
         for (int c = 0; c < NC; ++c) acc[i][c] = float4_t{0, 0, 0, 0};
-    store_x(0, 0, 0);
-    load_x(0, XR);
+    store_x(XR, 0, 0);
     __syncthreads();
 
     const uint32_t swz = swizzle<ACT>(r);  // slots 16 c + r have the same
@@ -638,25 +766,25 @@ __device__ __forceinline__ void group_tile(const MxArgs &a, const MxTile &t, MxS
             __syncthreads();
         }
     }
-    if (row0 < a.N) store_outputs<ACT, 4, NC>(a, t.e, row0, sh.dst, acc, lane);
+    if (row0 < a.N) store_outputs<ACT, 4, NC>(a, t.e, row0, slots.dst, acc, lane);
 }
 
-template <int ACT>
+template <int ACT, bool IDS>
 __global__ __launch_bounds__(64 * kMxWaves) __attribute__((amdgpu_waves_per_eu(2)))
 void mx_group_kernel(MxArgs a) {
     __shared__ MxShared sh;
+    __shared__ MxSlots<kMxBM> slots;
     MxTile t;
-    if (!find_tile<kMxBM, kMxBN>(a, t)) return;
-    if (threadIdx.x < kMxBM) sh.dst[threadIdx.x] = slot_output(a, t, threadIdx.x);
+    if (!find<IDS, kMxBM, kMxBN>(a, t, slots)) return;
     constexpr bool MX = act_mx(ACT);
     if (t.n <= 16)
-        few_tile<ACT>(a, t, sh);
+        few_tile<ACT, IDS>(a, t, slots);
     else if (t.n <= 32)
-        group_tile<ACT, 2, MX ? 4 : 2, MX ? 8 : 4, MX ? 1 : 2>(a, t, sh);
+        group_tile<ACT, IDS, 2, MX ? 4 : 2, MX ? 8 : 4, MX ? 1 : 2>(a, t, slots, sh);
     else if (t.n <= 48)
-        group_tile<ACT, 3, MX ? 4 : 1, MX ? 4 : 2, MX ? 1 : 2>(a, t, sh);
+        group_tile<ACT, IDS, 3, MX ? 4 : 1, MX ? 4 : 2, MX ? 1 : 2>(a, t, slots, sh);
     else
-        group_tile<ACT, 4, MX ? 4 : 1, MX ? 4 : 2, MX ? 1 : 2>(a, t, sh);
+        group_tile<ACT, IDS, 4, MX ? 4 : 1, MX ? 4 : 2, MX ? 1 : 2>(a, t, slots, sh);
 }
 
 // ------------------------------------------------------- many 4-bit slots ---
@@ -827,35 +955,47 @@ void launch_pairs(const MxArgs &a, hipStream_t stream) {
 template <int ACT, int BM, int BN>
 dim3 tile_grid(MxArgs &a) {
     const uint32_t nblocks = (a.N + BN - 1) / BN;
-    uint32_t mtiles = a.offs ? a.n_slots / BM + min(a.E, a.n_slots) : (a.n_slots + BM - 1) / BM;
+    const bool groups = a.offs || a.ids;
+    uint32_t mtiles = groups ? a.n_slots / BM + min(a.E, a.n_slots) : (a.n_slots + BM - 1) / BM;
     // an XCD takes as many M-tiles together as an expert has of them on average
-    const uint64_t even = a.offs ? uint64_t(BM) * a.E : 1;
+    const uint64_t even = groups ? uint64_t(BM) * a.E : 1;
     a.set = mtiles < 8 ? 0 : mtiles < 64 || a.n_slots <= even ? 1 : a.n_slots <= 3 * even ? 2 : 4;
     a.run = nblocks % 8 == 0 ? 8 : nblocks % 4 == 0 ? 4 : nblocks < 16 ? nblocks : 1;
     // one matrix, fewer bytes of slots than of weights: the weights stay, a
     // block of outputs on one XCD
-    if (!a.offs && uint64_t(a.n_slots) * (act_mx(ACT) ? 1 : 4) <= a.N) a.set = 0;
+    if (!groups && uint64_t(a.n_slots) * (act_mx(ACT) ? 1 : 4) <= a.N) a.set = 0;
     if (a.set) mtiles = (mtiles + 8 * a.set - 1) / (8 * a.set) * (8 * a.set);
     return dim3{mtiles * nblocks};
 }
 
-template <int ACT>
-void launch_groups(MxArgs a, hipStream_t stream) {
+template <int ACT, bool IDS>
+void launch_tiles(MxArgs a, hipStream_t stream) {
     const uint32_t nblocks = (a.N + kMxBN - 1) / kMxBN;
     if constexpr (act_mx(ACT)) {
         const uint32_t tiles = (a.n_slots + kBigBM - 1) / kBigBM;
-        if (!a.offs && tiles * nblocks >= kBigTiles) {
+        if (!IDS && !a.offs && tiles * nblocks >= kBigTiles) {
             hipLaunchKernelGGL((mx_big_kernel<ACT>), dim3{tiles * nblocks}, dim3{64 * kBigWaves}, 0, stream, a);
             return;
         }
     }
-    if (split_tiles(a) <= (a.steps >= 24 ? 512u : 256u) / (act_mx(ACT) ? 2 : 1)) {
+    if (split_tiles(a) <= (!act_mx(ACT) && a.steps >= 24 ? 512u : 256u)) {
         const dim3 grid = tile_grid<ACT, kSplitBM, kSplitBN>(a);
-        hipLaunchKernelGGL((mx_split_kernel<ACT>), grid, dim3{64 * kMxWaves}, 0, stream, a);
+        hipLaunchKernelGGL((mx_split_kernel<ACT, IDS>), grid, dim3{64 * kMxWaves}, 0, stream, a);
         return;
     }
     const dim3 grid = tile_grid<ACT, kMxBM, kMxBN>(a);
-    hipLaunchKernelGGL((mx_group_kernel<ACT>), grid, dim3{64 * kMxWaves}, 0, stream, a);
+    hipLaunchKernelGGL((mx_group_kernel<ACT, IDS>), grid, dim3{64 * kMxWaves}, 0, stream, a);
+}
+
+template <bool IDS>
+int launch_groups(int act, const MxArgs &a, void *stream) {
+    switch (act) {
+        case ACT_F16: launch_tiles<ACT_F16, IDS>(a, as_stream(stream)); break;
+        case ACT_BF16: launch_tiles<ACT_BF16, IDS>(a, as_stream(stream)); break;
+        case ACT_MX_F16: launch_tiles<ACT_MX_F16, IDS>(a, as_stream(stream)); break;
+        default: launch_tiles<ACT_MX_BF16, IDS>(a, as_stream(stream)); break;
+    }
+    return record_launch(hipGetLastError());
 }
 
 bool at16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
@@ -939,13 +1079,7 @@ int iqk_mx_groups(int act, int64_t in_features, int64_t out_features, int64_t nu
     a.offs = group_offsets;
     a.xr = x_rows;
     a.yr = y_rows;
-    switch (act) {
-        case ACT_F16: launch_groups<ACT_F16>(a, as_stream(stream)); break;
-        case ACT_BF16: launch_groups<ACT_BF16>(a, as_stream(stream)); break;
-        case ACT_MX_F16: launch_groups<ACT_MX_F16>(a, as_stream(stream)); break;
-        default: launch_groups<ACT_MX_BF16>(a, as_stream(stream)); break;
-    }
-    return record_launch(hipGetLastError());
+    return launch_groups<false>(act, a, stream);
 }
 
 int iqk_mx_prefill(int act, int64_t in_features, int64_t out_features, int64_t num_experts, const void *x,
@@ -965,6 +1099,16 @@ int iqk_mx_prefill(int act, int64_t in_features, int64_t out_features, int64_t n
         rc != IQK_OK || slots == 0)
         return rc;
     if (!ids || !work) return IQK_ERR_ARGUMENT;
+    if (rows_per_pair == 1 && ids_pay(a)) {
+        if (pairs_per_x_row <= 0 || pairs_per_x_row >= kLim || (n_pairs - 1) / pairs_per_x_row >= n_x_rows)
+            return IQK_ERR_ARGUMENT;
+        const int64_t mtiles = n_pairs / kSplitBM + num_experts;
+        if (mtiles * ((out_features + kSplitBN - 1) / kSplitBN) >= kLim) return IQK_ERR_ARGUMENT;
+        a.ids = static_cast<const uint32_t *>(ids);
+        a.wide = wide_ids != 0;
+        a.per_row = uint32_t(pairs_per_x_row);
+        return launch_groups<true>(act, a, stream);
+    }
     uint32_t *const x_rows = work, *const y_rows = work + slots, *const offsets = work + 2 * slots;
     const int rc = wide_ids ? iqk_route_ids64(static_cast<const int64_t *>(ids), n_pairs, num_experts, rows_per_pair,
                                               pairs_per_x_row, n_x_rows, offsets, x_rows, y_rows, stream)

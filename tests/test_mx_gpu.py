@@ -279,6 +279,30 @@ def test_ids_outside_the_stack_give_nan(device, quantized, many):
 
 
 @pytest.mark.parametrize("quantized", (False, True))
+@pytest.mark.parametrize("E,out", ((1, 40), (8, 32), (8, 2100), (100, 300), (512, 33), (513, 33)))
+@pytest.mark.parametrize("pairs", (255, 257, 768, 1023, 1024, 1025))
+def test_pairs_that_the_products_group(device, quantized, E, out, pairs):
+    """Both sides of where the workgroups sort the pairs themselves: pairs in rounds of
+    256, an expert with most of them, ids outside the stack, rows of one pair or of three."""
+    print(f"group {quantized} {E} {out} {pairs}", flush=True)
+    rng = np.random.default_rng(E + out + pairs)
+    n, k = 96, 3 if pairs % 3 == 0 else 1
+    module, w = _switch(rng, E, out, n, device)
+    ids = np.where(rng.random(pairs) < 0.3, rng.integers(0, E), rng.integers(0, E, pairs))
+    bad = rng.permutation(pairs)[:5]
+    for dtype, values in ((torch.int32, (-1, E, E + 7, 2 ** 31 - 1, -2 ** 31)),
+                          (torch.int64, (-1, E, 2 ** 32, 2 ** 32 + E - 1, -2 ** 62))):
+        named = ids.copy()
+        named[bad] = values
+        x, xv = _operand(rng, pairs // k, n, BF16, quantized, device)
+        y = module(_shape(x, pairs // k, 1, 1), _dev(named.reshape(-1, k), device, dtype), sorted_indices=True)
+        y = y.view(pairs, out)
+        assert bool(torch.isnan(y[torch.from_numpy(bad)]).all())
+        good = np.setdiff1d(np.arange(pairs), bad)
+        _check(y[torch.from_numpy(good)], np.repeat(xv, k, 0)[good], w, ids[good], BF16)
+
+
+@pytest.mark.parametrize("quantized", (False, True))
 @pytest.mark.parametrize("n", (96, 128, 1440))
 @pytest.mark.parametrize("pairs", (5, 100))
 def test_bad_rows_stay_where_they_are(device, quantized, n, pairs):
