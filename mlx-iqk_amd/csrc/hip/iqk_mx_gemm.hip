@@ -708,6 +708,8 @@ __device__ __forceinline__ void group_tile(const MxArgs &a, const MxTile &t, con
 #pragma unroll
         for (int c = 0; c < NC; ++c) acc[i][c] = float4_t{0, 0, 0, 0};
     store_x(XR, 0, 0);
+    uint4_t wv[2][4];  // 16-bit: a quarter's weights, made while the one before is multiplied
+    if constexpr (!MX) w.scaled(0, 0, wv[0]);
     __syncthreads();
 
     const uint32_t swz = swizzle<ACT>(r);  // slots 16 c + r have the same
@@ -753,12 +755,16 @@ __device__ __forceinline__ void group_tile(const MxArgs &a, const MxTile &t, con
                         w.multiply4(i, b[q & 1][c], bs[q & 1][c] >> (8 * g), acc[0][c], acc[1][c], acc[2][c],
                                     acc[3][c]);
                 } else {
-                    uint4_t wv[4];
-                    w.scaled(i, q % 4, wv);
+                    w.scaled((u * T + (q + 1) / 4) % AHEAD, (q + 1) % 4, wv[(q + 1) & 1]);
 #pragma unroll
                     for (int c = 0; c < NC; ++c)
 #pragma unroll
-                        for (int k = 0; k < 4; ++k) acc[k][c] = mfma16<ACT>(wv[k], b[q & 1][c], acc[k][c]);
+                        for (int k = 0; k < 4; ++k) acc[k][c] = mfma16<ACT>(wv[q & 1][k], b[q & 1][c], acc[k][c]);
+#pragma unroll
+                    for (int k = 0; k < 4 * NC; ++k) {
+                        __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+                        __builtin_amdgcn_sched_group_barrier(0x2, 2, 0);
+                    }
                 }
                 __builtin_amdgcn_sched_barrier(0);
                 if (MX || q % 4 == 3) w.load(i, first + (MX ? q : q / 4) + AHEAD);
@@ -799,8 +805,12 @@ void mx_group_kernel(MxArgs a) {
 // keep their sums in accumulation registers, where the MFMA took 27 clocks
 // against 20.)
 // Its start and end take 10 us in which the CU does nothing else, so it is used
-// where every CU has a tile: 2048 x 8192 (256 tiles), 4096 columns, 46.6 us
-// against 51.9 with tiles of 64; 1000 x 8192 (128 tiles) 40.8 against 27.6.
+// where every CU has a tile: 2048 x 8192 (256 tiles), 4096 columns, 45.9 us
+// against 51.9 with tiles of 64; 1000 x 8192 (128 tiles) 40.8 against 28.1.  8192
+// slots [8192 x 4096], four tiles a CU, take 175 us (3.1 PFLOP/s) at 2.0 GHz, the
+// matrix cores busy for 37% of it; random codes hold a loop of nothing but their
+// MFMA to 4.8.  Staying in a workgroup for all of a CU's tiles, with the next one's
+// loads under the stores, needs more registers than there are (84 spilled: 350 us).
 constexpr int kBigBM = 256, kBigBN = 256, kBigWaves = 8, kBigRing = 4;
 constexpr uint32_t kBigTiles = 256;
 constexpr int kBigX = 16 * kMxTileBytes;        // [256 slots][64 bytes], chunks at chunk ^ big_swizzle(slot)
@@ -810,11 +820,10 @@ constexpr int kBigStage = kBigXS + kBigBM * 4;
 
 __device__ __forceinline__ uint32_t big_swizzle(uint32_t slot) { return (slot >> 2) & 2u; }
 
-// All but the N loads issued last have landed, this wavefront's LDS reads have
-// returned, and every wavefront is here.
+// All but the N loads issued last have landed, and every wavefront is here.
 template <int N>
 __device__ __forceinline__ void wait_stage() {
-    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
+    asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(N) : "memory");
 }
 
 template <int ACT>
@@ -874,7 +883,7 @@ void mx_big_kernel(MxArgs a) {
         }
     };
 #pragma unroll
-    for (int i = 0; i < kBigRing; ++i) issue();
+    for (int i = 0; i < kBigRing - 1; ++i) issue();
 
     float4_t acc[4][8];
 #pragma unroll
@@ -894,17 +903,16 @@ void mx_big_kernel(MxArgs a) {
     const auto read_x = [&](int place, int c, const uint8_t *st) {
         x[place] = load_u4(st + xat + c * 1024);
     };
-    wait_stage<(kBigRing - 1) * LOADS>();
+    wait_stage<(kBigRing - 2) * LOADS>();
     const uint8_t *st = lds;
 #pragma unroll
     for (int i = 0; i < 4; ++i) read_w(0, i, st);
 #pragma unroll
     for (int c = 0; c < 3; ++c) read_x(c, c, st);
-    // In the middle of step s, with its slots' last columns read, the wavefronts
-    // meet: step s + 1 has landed once only the loads of s + 2 and s + 3 are
-    // outstanding, and s + 4 goes where s stood, three steps ahead.  (Meeting at the
-    // start of a step, with two ahead, takes as long: 172 us against 171 for 8192
-    // slots [8192 x 4096]; the step is LDS bandwidth, not the loads' latency.)
+    // In the middle of step s the wavefronts meet: step s + 1 has landed once only the
+    // loads of s + 2 are outstanding, and s + 3 goes where s - 1 stood, whose values
+    // every wavefront has multiplied.  (s + 4 into the place of s, whose last reads
+    // then have to return first: 94.1 us against 92.2, 8192 slots [8192 x 1440].)
     for (uint32_t s0 = 0; s0 < steps; s0 += 2) {
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
@@ -913,7 +921,7 @@ void mx_big_kernel(MxArgs a) {
 #pragma unroll
             for (int c = 0; c < 8; ++c) {
                 if (c == 5) {
-                    wait_stage<(kBigRing - 2) * LOADS>();
+                    wait_stage<(kBigRing - 3) * LOADS>();
                     issue();
                     read_w(b ^ 1, 0, next);
                 }

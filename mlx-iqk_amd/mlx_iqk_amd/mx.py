@@ -36,11 +36,21 @@ _STEP = 128
 _DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 _ACTS = {(torch.float16, False): 0, (torch.bfloat16, False): 1, (torch.float16, True): 2, (torch.bfloat16, True): 3}
 
-PAIR_LIMIT = 63
-"""Token-expert pairs up to which each pair is computed on its own, where they
-are at most eight more than the experts; beyond, experts are named again and again
-and their weights better read once (eight experts: 16 pairs 11.2 us against
-10.7 and 5 for the grouping, 64 pairs 29 against 11)."""
+
+
+def pair_limit(num_experts: int) -> int:
+    """Token-expert pairs up to which each is computed on its own; beyond, experts are
+    named so often that their weights are better read once for all their pairs.
+
+    A token's experts distinct, else uniform, us alone and grouped: [2048 x 4096], 8
+    experts: 12 pairs 8.6, 9.7, 16 pairs 10.3, 9.8; 16 experts: 16 pairs 12.5, 14.7, 24
+    pairs 17.1, 16.5; 128 experts: 48 pairs 31.4, 35.8, 72 pairs 45.2, 40.5; 256 experts:
+    72 pairs 46.9, 54.3, 96 pairs 65.0, 66.0; [1000 x 1440], 60 experts: 42 pairs 8.4,
+    9.2, 66 pairs 11.1, 10.6.
+    """
+    return min(num_experts + 6, 48 + num_experts // 6)
+
+
 ROW_LIMIT = 16384
 """Outputs in all up to which the rows of an :class:`MxLinear` are computed on their
 own (2048 outputs: 8 rows 5.6 us against 7.8, 16 rows 8.9 against 8.4; 8192
@@ -207,6 +217,7 @@ class _MxStack(torch.nn.Module):
             raise IqkRuntimeError(f"out_features must be positive, got {out_features}")
         rows, steps = (self.out_features + 15) // 16 * 16, (self.in_features + _STEP - 1) // _STEP
         E = self.num_experts
+        self._pair_limit = pair_limit(E)
         self.register_buffer("tiles", torch.zeros((E, rows // 16, steps, 64, 16), dtype=torch.uint8, device=device))
         self.register_buffer("tile_scales", torch.zeros((E, steps, (rows + 63) // 64, 64, 4), dtype=torch.uint8,
                                                         device=device))
@@ -295,7 +306,7 @@ class MxSwitchLinear(_MxStack):
 
     def forward(self, x, indices: torch.Tensor, sorted_indices: bool = False) -> torch.Tensor:
         """Project ``x`` through the experts named by ``indices``: few pairs
-        each on its own (:data:`PAIR_LIMIT`), else (or with ``sorted_indices``) grouped
+        each on its own (:func:`pair_limit`), else (or with ``sorted_indices``) grouped
         by expert on the device."""
         if len(x.shape) < 2:
             raise IqkRuntimeError(f"x must be [..., M, {self.in_features}], got {tuple(x.shape)}")
@@ -318,7 +329,7 @@ class MxSwitchLinear(_MxStack):
                 or ids.get_device() != tiles.get_device():
             ids = self._ids(indices, batch)
         pairs = math.prod(batch)
-        grouped = sorted_indices or M != 1 or pairs > min(PAIR_LIMIT, self.num_experts + 8)
+        grouped = sorted_indices or M != 1 or pairs > self._pair_limit
         return self._project((act, rows, scales, stride), ids, (*batch, M, self.out_features), pairs, M, per_row,
                              grouped)
 
