@@ -502,3 +502,49 @@ def test_refusals(device):
         module(grad, ids)
     with torch.no_grad():
         assert module(grad, ids).shape == (3, 2, 1, 20)
+
+
+def test_weights_past_32_bits(device):
+    """The last expert of a stack whose tiles take more than 4 GiB, by each route."""
+    print("weights past 4 GiB", flush=True)
+    E, out, n = 1030, 2048, 4096
+    g = torch.Generator(device=device).manual_seed(4)
+    codes = torch.randint(0, 256, (E, out, n // 2), dtype=torch.uint8, device=device, generator=g)
+    scales = torch.randint(110, 126, (E, out, n // 32), dtype=torch.uint8, device=device, generator=g)
+    module = mx.MxSwitchLinear(E, out, n, device=device)
+    module.load(mx.MxTensor(codes, scales))
+    assert module.tiles.numel() > 2 ** 32
+    w = mxref.values(codes[-1:].cpu().numpy(), scales[-1:].cpu().numpy())
+    del codes, scales
+    rng = np.random.default_rng(3)
+    for quantized in (False, True):
+        for pairs in (3, 40, 2100):
+            x, xv = _operand(rng, pairs, n, BF16, quantized, device)
+            ids = torch.full((pairs,), E - 1, dtype=torch.int32, device=device)
+            y = module(_shape(x, pairs, 1), ids, sorted_indices=pairs > 3).view(pairs, out)
+            rows = np.r_[:2, pairs - 1]
+            _check(y[torch.from_numpy(rows)], xv[rows], w, np.zeros(3, dtype=np.int64), BF16)
+
+
+def test_rows_past_32_bits(device):
+    """Activations and outputs of more than 4 GiB; quantised, codes of more than 2."""
+    print("rows past 4 GiB", flush=True)
+    rows, n, out = 1_060_000, 2080, 2096
+    rng = np.random.default_rng(9)
+    codes, s = mxref.random_codes(rng, (out, n))
+    line = mx.MxLinear(out, n, device=device)
+    line.load(mx.MxTensor(_dev(codes, device), _dev(s, device)))
+    w = mxref.values(codes, s)[None]
+    x = torch.randn((rows, n), dtype=BF16, device=device, generator=torch.Generator(device=device).manual_seed(5))
+    at = np.r_[0, 1, 530_000, rows - 2, rows - 1]
+    index = torch.from_numpy(at).to(device)
+    y = line(x)
+    assert x.numel() * 2 > 2 ** 32 and y.numel() * 2 > 2 ** 32
+    _check(y[index], _f64(x[index]), w, np.zeros(5, dtype=np.int64), BF16)
+    del y
+    q = mx.quantize(x)
+    part = mx.MxTensor(q.codes[index], q.scales[index], BF16)
+    _same_codes(part, x[index])
+    assert torch.equal(q.dequantize()[index], part.dequantize())
+    y = line(q)
+    _check(y[index], _f64(part.dequantize(F32)), w, np.zeros(5, dtype=np.int64), BF16)
