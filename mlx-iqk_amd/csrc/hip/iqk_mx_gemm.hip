@@ -601,21 +601,33 @@ __device__ __forceinline__ void few_tile(const MxArgs &a, const MxTile &t, const
     store_outputs<ACT, 4, 1>(a, t.e, row0, slots.dst, acc, threadIdx.x & 63u);
 }
 
-// Where the tiles above would leave CUs without work: tiles of 16 slots by 64
-// outputs, whose four wavefronts split the reduction axis and add up in LDS, in
-// their order.  Two of them fit a CU, and a round of 512 takes 10 us with 4096
-// columns and 8 with 1440 (4-bit slots: as long); one of 64 x 256 tiles as long as
-// its slots: 14 us for a few, 23 for 16, 35 for 64 (4-bit: 12, 17, 16).  So split
-// tiles serve while one round holds them, half of one for 4-bit slots or under 24
-// steps: 8 experts [2048 x 4096] of 8 slots 10.0 us against 17.8 (4-bit 10.6,
-// 14.7), of 32 slots 17.2 against 22.3 (4-bit, past the limit: 17.2, 12.8); 16 of 24
-// slots, past it, 32.5 against 24.7, 60 experts [1000 x 1440] of 10 22.5 against 14.3.
-constexpr int kSplitBM = 16, kSplitBN = 64;
+// Where the tiles above would leave CUs without work: tiles of 16 slots, whose
+// wavefronts split the reduction axis, in four for 64 outputs or in two for 128, and
+// add up in LDS, in their order.  A round of them takes 10 us with 4096 columns and
+// 8 with 1440, 4-bit slots as long; one of 64 x 256 tiles as long as its slots: 14
+// us for a few, 23 for 16, 30 for 64 (4-bit: 12, 17, 16).  So they serve while every
+// CU has one at most, first of 64, then of 128 outputs: 8 experts [2048 x 4096] of 8
+// slots 10.0, 11.6 and 17.7 us by 64, 128 and 256 outputs (4-bit 10.6, 10.7, 14.7);
+// of 32 slots (past the first limit) 17.1, 15.9 and 19.5; 16 of 24 (past both)
+// 31.9, 28.6 and 22.5; 60 [1000 x 1440] of 10 22.4, 17.0 and 14.3.  4-bit slots under
+// 24 steps leave four ways out: 8192 outputs, 1440 columns, 16 slots 7.7, 6.2 and
+// 8.0; and two where an expert has several such tiles: 8 experts of 32 slots 16.9, 16.2
+// and 12.7, but 16 of 16 19.3, 18.1 and 22.3.
+constexpr int kSplitBM = 16;
 
-// About how many a call has: an expert one, or its share of the slots.
-inline uint64_t split_tiles(const MxArgs &a) {
-    const uint32_t experts = min(a.E, a.n_slots), all = (a.n_slots + kSplitBM - 1) / kSplitBM;
-    return uint64_t(max(experts, all)) * ((a.N + kSplitBN - 1) / kSplitBN);
+// About how many M-tiles of bm slots a call has: an expert one, or its share of the slots.
+inline uint32_t likely_tiles(const MxArgs &a, uint32_t bm) {
+    return max(min(a.E, a.n_slots), (a.n_slots + bm - 1) / bm);
+}
+
+// Into how many ways its tiles split the reduction axis; 1: 64 x 256 tiles.
+template <int ACT>
+int split_ways(const MxArgs &a) {
+    const uint64_t tiles = likely_tiles(a, kSplitBM);
+    const bool mx = act_mx(ACT), once = a.E == 1 || tiles == min(a.E, a.n_slots);
+    if (tiles * ((a.N + 63) / 64) <= 256 && (!mx || a.steps >= 24)) return 4;
+    if (tiles * ((a.N + 127) / 128) <= 256 && (!mx || once)) return 2;
+    return 1;
 }
 
 // The workgroup's tile and its slots, from the lists or the pairs' ids; without IDS,
@@ -632,24 +644,30 @@ __device__ __forceinline__ bool find(const MxArgs &a, MxTile &t, MxSlots<BM> &sl
     }
 }
 
-template <int ACT, bool IDS>
+// WAYS: the wavefronts that share a block of 64 outputs.
+template <int ACT, bool IDS, int WAYS>
 __global__ __launch_bounds__(64 * kMxWaves) __attribute__((amdgpu_waves_per_eu(2)))
 void mx_split_kernel(MxArgs a) {
+    constexpr int ROWS = 4 / WAYS;  // tile rows that a wavefront adds up and stores
     __shared__ __attribute__((aligned(16))) float4_t part[kMxWaves][4][64];
     __shared__ MxSlots<kSplitBM> slots;
     MxTile t;
-    if (!find<IDS, kSplitBM, kSplitBN>(a, t, slots)) return;
+    if (!find<IDS, kSplitBM, 64 * kMxWaves / WAYS>(a, t, slots)) return;
     const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t way = wave % WAYS, row0 = t.n0 + 64 * (wave / WAYS);
     float4_t acc[4][1];
-    few_slots<ACT, IDS>(a, t, slots, t.n0, wave, kMxWaves, acc);
+    few_slots<ACT, IDS>(a, t, slots, row0, way, WAYS, acc);
 #pragma unroll
     for (int i = 0; i < 4; ++i) part[wave][i][lane] = acc[i][0];
     __syncthreads();
-    // wavefront i adds up and stores tile row i
-    float4_t sum[1][1] = {{part[0][wave][lane]}};
+    float4_t sum[ROWS][1];
 #pragma unroll
-    for (int i = 1; i < kMxWaves; ++i) sum[0][0] += part[i][wave][lane];
-    store_outputs<ACT, 1, 1>(a, t.e, t.n0 + kMxRows * wave, slots.dst, sum, lane);
+    for (int i = 0; i < ROWS; ++i) {
+        sum[i][0] = part[wave - way][ROWS * way + i][lane];
+#pragma unroll
+        for (int k = 1; k < WAYS; ++k) sum[i][0] += part[wave - way + k][ROWS * way + i][lane];
+    }
+    store_outputs<ACT, ROWS, 1>(a, t.e, row0 + kMxRows * ROWS * way, slots.dst, sum, lane);
 }
 
 // A tile of at most 16 NC slots (NC > 1), T steps a turn: 16 KiB of slots, which
@@ -975,7 +993,7 @@ dim3 tile_grid(MxArgs &a) {
     uint32_t mtiles = groups ? a.n_slots / BM + min(a.E, a.n_slots) : (a.n_slots + BM - 1) / BM;
     // an XCD takes as many M-tiles together as an expert has of them on average
     const uint64_t even = groups ? uint64_t(BM) * a.E : 1;
-    a.set = mtiles < 8 ? 0 : mtiles < 64 || a.n_slots <= even ? 1 : a.n_slots <= 3 * even ? 2 : 4;
+    a.set = likely_tiles(a, BM) < 8 ? 0 : mtiles < 64 || a.n_slots <= even ? 1 : a.n_slots <= 3 * even ? 2 : 4;
     a.run = nblocks % 8 == 0 ? 8 : nblocks % 4 == 0 ? 4 : nblocks < 16 ? nblocks : 1;
     // one matrix, fewer bytes of slots than of weights: the weights stay, a
     // block of outputs on one XCD
@@ -994,9 +1012,15 @@ void launch_tiles(MxArgs a, hipStream_t stream) {
             return;
         }
     }
-    if (split_tiles(a) <= (!act_mx(ACT) && a.steps >= 24 ? 512u : 256u)) {
-        const dim3 grid = tile_grid<ACT, kSplitBM, kSplitBN>(a);
-        hipLaunchKernelGGL((mx_split_kernel<ACT, IDS>), grid, dim3{64 * kMxWaves}, 0, stream, a);
+    const int ways = split_ways<ACT>(a);
+    if (ways == 4) {
+        const dim3 grid = tile_grid<ACT, kSplitBM, 64>(a);
+        hipLaunchKernelGGL((mx_split_kernel<ACT, IDS, 4>), grid, dim3{64 * kMxWaves}, 0, stream, a);
+        return;
+    }
+    if (ways == 2) {
+        const dim3 grid = tile_grid<ACT, kSplitBM, 128>(a);
+        hipLaunchKernelGGL((mx_split_kernel<ACT, IDS, 2>), grid, dim3{64 * kMxWaves}, 0, stream, a);
         return;
     }
     const dim3 grid = tile_grid<ACT, kMxBM, kMxBN>(a);
@@ -1119,7 +1143,7 @@ int iqk_mx_prefill(int act, int64_t in_features, int64_t out_features, int64_t n
         if (pairs_per_x_row <= 0 || pairs_per_x_row >= kLim || (n_pairs - 1) / pairs_per_x_row >= n_x_rows)
             return IQK_ERR_ARGUMENT;
         const int64_t mtiles = n_pairs / kSplitBM + num_experts;
-        if (mtiles * ((out_features + kSplitBN - 1) / kSplitBN) >= kLim) return IQK_ERR_ARGUMENT;
+        if (mtiles * ((out_features + 63) / 64) >= kLim) return IQK_ERR_ARGUMENT;
         a.ids = static_cast<const uint32_t *>(ids);
         a.wide = wide_ids != 0;
         a.per_row = uint32_t(pairs_per_x_row);

@@ -355,7 +355,8 @@ def test_rows_of_very_different_scales(device, dtype, pairs):
 
 @pytest.mark.parametrize("quantized", (False, True))
 @pytest.mark.parametrize("rows,out,n", ((1, 33, 96), (4, 64, 1440), (5, 300, 160), (5, 4000, 160), (17, 1100, 3168),
-                                        (128, 256, 512), (200, 700, 1056), (300, 2100, 1056)))
+                                        (128, 256, 512), (200, 700, 1056), (300, 1500, 1056),
+                                        (300, 2100, 1056)))
 def test_linear(device, quantized, rows, out, n):
     print(f"linear {quantized} {rows} {out} {n}", flush=True)
     rng = np.random.default_rng(rows)
