@@ -246,12 +246,26 @@ PyObject *py_balance(PyObject *, PyObject *const *args, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
-// mx_quantize(x, row_stride) -> (codes, scales)
+// Whether the kernels take t as it is: on a GPU, dense, at a 16-byte boundary, not empty.
+bool ready(const Tensor &t) {
+    return t.is_cuda() && t.is_contiguous() && t.dim() && t.numel() &&
+           (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15u) == 0;
+}
+
+// mx_quantize(x, row_stride) -> (codes, scales); with a row_stride of 0 x is looked
+// at first, and the answer is None where it is no such tensor
 PyObject *py_mx_quantize(PyObject *, PyObject *const *args, Py_ssize_t n) {
     HANDLE_TH_ERRORS
     arguments(n, 2);
     const Tensor &x = tensor(args[0]);
-    const int64_t row_stride = integer(args[1]), cols = x.size(-1), stride = mx_scale_stride(cols);
+    int64_t row_stride = integer(args[1]);
+    if (row_stride == 0) {
+        const auto type = x.scalar_type();
+        if ((type != at::kFloat && type != at::kHalf && type != at::kBFloat16) || !ready(x) || x.size(-1) % 32)
+            Py_RETURN_NONE;
+        row_stride = x.size(-1);
+    }
+    const int64_t cols = x.size(-1), stride = mx_scale_stride(cols);
     auto shape = x.sizes().vec();
     shape.back() = cols / 2;
     const Tensor codes = empty(shape, at::kByte, x);
@@ -267,12 +281,22 @@ PyObject *py_mx_quantize(PyObject *, PyObject *const *args, Py_ssize_t n) {
 }
 
 // mx_dequantize(codes, scales, scale_stride, like) -> values of the type of
-// IQK_* code `like`
+// IQK_* code `like`; with a scale_stride of 0 codes and scales are looked at first, and
+// the answer is None where they are not ready or scales' rows not evenly spaced
 PyObject *py_mx_dequantize(PyObject *, PyObject *const *args, Py_ssize_t n) {
     HANDLE_TH_ERRORS
     arguments(n, 4);
     const Tensor &codes = tensor(args[0]), &scales = tensor(args[1]);
-    const int64_t stride = integer(args[2]), type = integer(args[3]);
+    int64_t stride = integer(args[2]);
+    const int64_t type = integer(args[3]);
+    if (stride == 0) {
+        const int64_t dim = scales.dim();
+        if (!ready(codes) || scales.stride(-1) != 1) Py_RETURN_NONE;
+        stride = dim > 1 ? scales.stride(-2) : scales.size(-1);
+        for (int64_t i = dim - 3; i >= 0; --i)
+            if (scales.stride(i) != scales.stride(i + 1) * scales.size(i + 1)) Py_RETURN_NONE;
+        if (stride < scales.size(-1)) Py_RETURN_NONE;
+    }
     auto shape = codes.sizes().vec();
     const int64_t cols = shape.back() *= 2;
     const Tensor y = empty(shape, type == IQK_F32 ? at::kFloat : type == IQK_F16 ? at::kHalf : at::kBFloat16, codes);

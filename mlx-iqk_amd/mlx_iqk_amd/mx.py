@@ -161,11 +161,16 @@ def quantize(x: torch.Tensor) -> MxTensor:
     2**-127; values round to nearest, ties to the even code, and saturate at 6
     scales.  A block that holds a NaN or an infinity becomes NaN.
     """
-    if not isinstance(x, torch.Tensor) or x.dim() < 1:
+    if not isinstance(x, torch.Tensor):
+        raise IqkKernelError("x must be a tensor of at least one dimension")
+    binding, dtype = _native.torch_binding(), x.dtype
+    if (got := binding.mx_quantize(x, 0)) is not None:
+        return MxTensor._of(*got, dtype)
+    # what the binding does not take as it is
+    if x.dim() < 1:
         raise IqkKernelError("x must be a tensor of at least one dimension")
     if not x.is_cuda:
         raise IqkKernelError(f"x must live on a GPU, got {x.device}")
-    dtype = x.dtype
     if dtype not in _DTYPES:
         raise IqkKernelError(f"x must be one of {tuple(_DTYPES)}, got {dtype}")
     n = _check_width(x.shape[-1])
@@ -176,7 +181,7 @@ def quantize(x: torch.Tensor) -> MxTensor:
             x, stride = x.contiguous(), n
             if x.data_ptr() % 16:
                 x = x.clone()
-    return MxTensor._of(*_native.torch_binding().mx_quantize(x, stride), dtype)
+    return MxTensor._of(*binding.mx_quantize(x, stride), dtype)
 
 
 def dequantize(q: MxTensor, dtype: torch.dtype | None = None) -> torch.Tensor:
@@ -186,13 +191,15 @@ def dequantize(q: MxTensor, dtype: torch.dtype | None = None) -> torch.Tensor:
     code = _DTYPES.get(dtype)
     if code is None:
         raise IqkKernelError(f"dtype must be one of {tuple(_DTYPES)}, got {dtype}")
-    codes, scales = q.codes, q.scales
+    codes, scales, binding = q.codes, q.scales, _native.torch_binding()
+    if (values := binding.mx_dequantize(codes, scales, 0, code)) is not None:
+        return values
     if not codes.is_cuda:
         raise IqkKernelError(f"codes must live on a GPU, got {codes.device}")
     codes, stride = _aligned_codes(codes), _row_stride(scales)
     if stride is None or stride < scales.shape[-1]:
         scales, stride = scales.contiguous(), scales.shape[-1]
-    return _native.torch_binding().mx_dequantize(codes, scales, stride, code)
+    return binding.mx_dequantize(codes, scales, stride, code)
 
 
 class _MxStack(torch.nn.Module):
