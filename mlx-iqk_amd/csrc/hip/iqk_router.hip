@@ -187,13 +187,15 @@ __device__ __forceinline__ float key16_value(uint32_t key) {
 }
 
 // v -> softmax over the row's 16 lanes, in place (none of it where every
-// logit is -inf: zeros).  A NaN makes the sum, and so the row, NaN.
+// logit is -inf: zeros).  A NaN makes the sum, and so the row, NaN, also where all
+// else is -inf (places past E are) and the maximum, which skips NaN, is too.
 template <int VPT>
 __device__ __forceinline__ void row_softmax(float (&v)[VPT]) {
     float top = v[0];
 #pragma unroll
     for (int i = 1; i < VPT; ++i) top = fmaxf(top, v[i]);
     top = row_max(top);
+    if (top == -__builtin_inff()) top = 0.f;  // no logit but -inf, whose exponentials are 0, and NaN
     float s = 0.f;
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
@@ -201,10 +203,9 @@ __device__ __forceinline__ void row_softmax(float (&v)[VPT]) {
         s += v[i];
     }
     s = row_sum(s);
-    const bool none = top == -__builtin_inff();
-    const float inv = 1.0f / s;
+    const float inv = s == 0.f ? 0.f : 1.0f / s;
 #pragma unroll
-    for (int i = 0; i < VPT; ++i) v[i] = none ? 0.f : v[i] * inv;
+    for (int i = 0; i < VPT; ++i) v[i] *= inv;
 }
 
 // -------------------------------------------------------------------- top k ---

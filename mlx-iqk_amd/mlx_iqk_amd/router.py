@@ -61,7 +61,8 @@ def balance_loss(logits: torch.Tensor, ids: torch.Tensor, *,
     and ``P_e`` the mean of its softmax probability, ``loss = experts * sum_e f_e
     P_e``: 1 where either is even, up to ``experts / k`` where the same k experts
     take all.  Tokens whose ``mask`` (bool ``[..., tokens]``) is false are left out;
-    with none left the loss is 0.  Ids outside the stack count for none.
+    with none left the loss is 0.  Ids outside the stack count for none.  A NaN in
+    a token that is kept makes its loss and its own gradient NaN.
     Differentiable in the logits (through ``P``; counts are constants).
     """
     experts = _check_logits(logits, 2)

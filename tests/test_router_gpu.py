@@ -329,3 +329,44 @@ def test_refusals(device):
                                 (z(3, 8), ids, torch.zeros(3, dtype=torch.bool)), (torch.zeros(3, 8), ids, None)):
         with pytest.raises(IqkKernelError):
             router.balance_loss(logits, named, mask=mask)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("experts", (20, 60, 64, 161, 256, 1000))
+def test_kept_tokens_without_numbers_show(device, dtype, experts):
+    """A kept token whose logits are NaN, or NaN and -inf, makes its group's loss and its own
+    gradient NaN; the other tokens' gradients stay as they are."""
+    print(f"balance NaN {dtype} {experts}", flush=True)
+    rng = np.random.default_rng(experts)
+    logits, ids, mask = _balance_case(rng, 4, 40, experts, 2, dtype, device, False)
+    clean = logits.clone()
+    inf, nan = float("inf"), float("nan")
+    logits[0, 3] = nan
+    logits[1, 5] = -inf
+    logits[1, 5, experts // 2] = nan
+    logits[2, 7, :-1] = nan
+    logits[2, 7, -1] = -inf
+    named, one = torch.from_numpy(ids).to(device), torch.ones(4, device=device)
+    grads = []
+    for x in (logits, clean):
+        x.requires_grad_()
+        loss, _ = router.balance_loss(x, named)
+        grads.append(_f64(torch.autograd.grad(loss, x, one)[0]))
+        np.testing.assert_array_equal(np.isnan(_f64(loss)),
+                                      [np.isnan(mxref.balance(_f64(x)[g], ids[g], mask[g])[0]) for g in range(4)])
+    assert not np.isnan(grads[1]).any()
+    bad = np.zeros((4, 40), bool)
+    bad[[0, 1, 2], [3, 5, 7]] = True
+    assert np.isnan(grads[0][bad]).all()
+    np.testing.assert_array_equal(grads[0][~bad], grads[1][~bad])
+    # the choice's weights and gradient
+    for normalize in (True, False):
+        weights, _ = router.topk(logits, 2, normalize=normalize)
+        (grad,) = torch.autograd.grad(weights, logits, torch.ones_like(weights))
+        want_w, want_ids = mxref.topk(_f64(logits).reshape(160, experts), 2, normalize)
+        np.testing.assert_array_equal(np.isnan(_f64(weights)).reshape(160, 2), np.isnan(want_w))
+        hit = np.zeros((160, experts), bool)
+        np.put_along_axis(hit, want_ids, True, -1)
+        hit = hit.reshape(4, 40, experts) if normalize else np.ones((4, 40, experts), bool)
+        got = np.isnan(_f64(grad))
+        assert got[bad][hit[bad]].all() and not got[~bad].any()
