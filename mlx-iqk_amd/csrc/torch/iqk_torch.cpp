@@ -49,12 +49,17 @@ T *ptr(const Tensor &t) {
     return t.defined() ? static_cast<T *>(t.data_ptr()) : nullptr;
 }
 
-// A gradient that is not differentiable again says so when asked.
-variable_list once(Tensor grad, const variable_list &from) {
-    if (!at::GradMode::is_enabled() || !torch::autograd::any_variable_requires_grad(from)) return {grad};
+// A gradient that is not differentiable again says so when asked.  It depends on what
+// comes from above and on `saved`, the forward's tensor that the formula is of: the
+// node that raises stands between it and them, so that a derivative in either meets it.
+variable_list once(Tensor grad, const variable_list &above, const Tensor &saved) {
+    if (!at::GradMode::is_enabled() || !(saved.requires_grad() || torch::autograd::any_variable_requires_grad(above)))
+        return {grad};
+    variable_list inputs{grad, saved};
+    inputs.insert(inputs.end(), above.begin(), above.end());
     auto error = std::make_shared<torch::autograd::DelayedError>(
-        "the router's gradients are not differentiable a second time", 1);
-    return (*error)({grad.detach().requires_grad_(true)});
+        "the router's gradients are not differentiable a second time", int64_t(inputs.size()));
+    return {(*error)(std::move(inputs))[0]};
 }
 
 // ------------------------------------------------------------------- top k ---
@@ -95,7 +100,7 @@ struct TopK : torch::autograd::Function<TopK> {
                                    ptr<float>(dweights), weights.numel() / k, experts, k, normalize,
                                    dlogits.data_ptr(), stream_of(weights)),
               "iqk_router_topk_grad");
-        auto out = once(dlogits, grads);
+        auto out = once(dlogits, grads, normalize ? weights : logits);
         out.resize(3);
         return out;
     }
@@ -151,7 +156,7 @@ struct Balance : torch::autograd::Function<Balance> {
                                ptr<int32_t>(kept), ptr<float>(dloss), groups, tokens, experts,
                                ctx->saved_data["k"].toInt(), dlogits.data_ptr(), stream_of(logits)),
               "iqk_balance_grad");
-        auto out = once(dlogits, grads);
+        auto out = once(dlogits, grads, logits);
         out.resize(3);
         return out;
     }

@@ -370,3 +370,24 @@ def test_kept_tokens_without_numbers_show(device, dtype, experts):
         hit = hit.reshape(4, 40, experts) if normalize else np.ones((4, 40, experts), bool)
         got = np.isnan(_f64(grad))
         assert got[bad][hit[bad]].all() and not got[~bad].any()
+
+
+def test_a_second_derivative_is_refused_under_constant_gradients(device):
+    """The gradients depend on the logits also where what comes from above is a constant."""
+    print("second derivative, constant gradients", flush=True)
+    logits = torch.randn((6, 12), device=device).requires_grad_()
+    dw = torch.randn((6, 3), device=device)
+    weights, ids = router.topk(logits, 3)
+    full, _ = router.topk(logits, 3, normalize=False)
+    loss, _ = router.balance_loss(logits, ids)
+    for out in (loss, (weights * dw).sum(), (full * dw).sum(), weights[0, 0] + 2 * loss):
+        (plain,) = torch.autograd.grad(out, logits, retain_graph=True)
+        assert not plain.requires_grad
+        (grad,) = torch.autograd.grad(out, logits, create_graph=True)
+        assert torch.equal(grad, plain)
+        with pytest.raises(RuntimeError, match="second time"):
+            grad.sum().backward(retain_graph=True)
+        # beside a term that has a second derivative
+        (both,) = torch.autograd.grad(out + (logits ** 2).sum(), logits, create_graph=True)
+        with pytest.raises(RuntimeError, match="second time"):
+            torch.autograd.grad(both.sum(), logits, retain_graph=True)
