@@ -220,6 +220,11 @@ PyObject *pair(const Tensor &a, const Tensor &b) {
 }
 bool wants_grad(const Tensor &t) { return at::GradMode::is_enabled() && t.requires_grad(); }
 
+// The kernels carry no tangents, and a tensor that has one need not require a gradient.
+void refuse_tangent(const Tensor &t, const char *name) {
+    TORCH_CHECK(!t._fw_grad(0).defined(), name, " has a forward-mode derivative, which the kernels do not carry");
+}
+
 // topk(logits, k, normalize) -> (weights, ids); logits contiguous
 PyObject *py_topk(PyObject *, PyObject *const *args, Py_ssize_t n) {
     HANDLE_TH_ERRORS
@@ -227,6 +232,7 @@ PyObject *py_topk(PyObject *, PyObject *const *args, Py_ssize_t n) {
     const Tensor &logits = tensor(args[0]);
     const int64_t k = integer(args[1]);
     const bool normalize = integer(args[2]) != 0;
+    refuse_tangent(logits, "logits");
     if (wants_grad(logits)) {
         const auto out = TopK::apply(logits, k, normalize);
         return pair(out[0], out[1]);
@@ -242,6 +248,7 @@ PyObject *py_balance(PyObject *, PyObject *const *args, Py_ssize_t n) {
     arguments(n, 3);
     const Tensor &logits = tensor(args[0]), &ids = tensor(args[1]);
     const Tensor mask = tensor_or_none(args[2]);
+    refuse_tangent(logits, "logits");
     if (wants_grad(logits)) {
         const auto out = Balance::apply(logits, ids, mask.defined() ? std::optional<Tensor>(mask) : std::nullopt);
         return pair(out[0], out[1]);
@@ -270,6 +277,7 @@ PyObject *py_mx_quantize(PyObject *, PyObject *const *args, Py_ssize_t n) {
             Py_RETURN_NONE;
         row_stride = x.size(-1);
     }
+    refuse_tangent(x, "x");
     const int64_t cols = x.size(-1), stride = mx_scale_stride(cols);
     auto shape = x.sizes().vec();
     shape.back() = cols / 2;
@@ -318,6 +326,7 @@ PyObject *py_mx_dequantize(PyObject *, PyObject *const *args, Py_ssize_t n) {
 PyObject *py_mx_project(PyObject *, PyObject *const *args, Py_ssize_t n) {
     HANDLE_TH_ERRORS
     arguments(n, 14);
+    refuse_tangent(tensor(args[1]), "x");
     c10::SmallVector<int64_t, 8> shape;
     TORCH_CHECK_TYPE(PyTuple_Check(args[8]), "the shape is a tuple");
     for (Py_ssize_t i = 0; i < PyTuple_GET_SIZE(args[8]); ++i) shape.push_back(integer(PyTuple_GET_ITEM(args[8], i)));

@@ -14,7 +14,8 @@ value.  A byte holds two codes, the even position's in its low half.
 Both projections take 16-bit activations, whose products with the weights are
 exact and summed in f32, or an :class:`MxTensor`, quantised activations, which the
 matrix cores multiply with the weights as they are, at four times the rate.
-Outputs are rounded once.  The weights are frozen: no gradient flows through.
+Outputs are rounded once.  The weights are frozen: no gradient flows through, and an
+x that wants one, or has a forward-mode derivative, is refused.
 
 Like every launch of this package, these run asynchronously on torch's current
 stream, and raise where no GPU library is built; nothing falls back to the CPU.
@@ -274,7 +275,7 @@ class _MxStack(torch.nn.Module):
             raise IqkRuntimeError("the weights are frozen and no gradient flows through them: detach x, or call "
                                   "under torch.no_grad()")
         if not rows.is_contiguous() or rows.data_ptr() % 16:
-            rows = rows.detach().contiguous()
+            rows = rows.contiguous()
             rows = rows if rows.data_ptr() % 16 == 0 else rows.clone()
         return act, rows, None, 0
 

@@ -5,7 +5,7 @@ weights, and the loss that keeps the experts evenly loaded; with gradients.
 (:class:`~mlx_iqk_amd.nn.IqkSwitchLinear`, :class:`~mlx_iqk_amd.mx.MxSwitchLinear`),
 its weights scale their outputs.  Logits are f32, f16 or bf16 on a GPU, for up to
 1024 experts; sums, probabilities, weights and losses are f32.  Gradients are
-differentiable once.
+not differentiable again, and logits with a forward-mode derivative are refused.
 """
 
 from __future__ import annotations

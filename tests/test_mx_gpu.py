@@ -549,3 +549,20 @@ def test_rows_past_32_bits(device):
     assert torch.equal(q.dequantize()[index], part.dequantize())
     y = line(q)
     _check(y[index], _f64(part.dequantize(F32)), w, np.zeros(5, dtype=np.int64), BF16)
+
+
+def test_forward_mode_derivatives_are_refused(device):
+    print("mx forward mode", flush=True)
+    fwd = torch.autograd.forward_ad
+    module, line = mx.MxSwitchLinear(2, 20, 64, device=device), mx.MxLinear(20, 64, device=device)
+    ids = torch.zeros((3, 2), dtype=torch.int32, device=device)
+    base = torch.randn((3, 1, 1, 64), device=device).to(F16)
+    wide = torch.randn((3, 1, 1, 128), device=device).to(F16)[..., ::2]  # copied before the call
+    with fwd.dual_level():
+        for t in (base, wide):
+            x = fwd.make_dual(t, torch.ones_like(t))
+            for call in (lambda: mx.quantize(x), lambda: module(x, ids), lambda: module(x, ids, sorted_indices=True),
+                         lambda: line(x)):
+                with pytest.raises(RuntimeError, match="forward-mode"):
+                    call()
+        assert line(base).shape == (3, 1, 1, 20) and line(wide).shape == (3, 1, 1, 20)

@@ -391,3 +391,19 @@ def test_a_second_derivative_is_refused_under_constant_gradients(device):
         (both,) = torch.autograd.grad(out + (logits ** 2).sum(), logits, create_graph=True)
         with pytest.raises(RuntimeError, match="second time"):
             torch.autograd.grad(both.sum(), logits, retain_graph=True)
+
+
+def test_forward_mode_derivatives_are_refused(device):
+    print("router forward mode", flush=True)
+    fwd = torch.autograd.forward_ad
+    logits, ids = torch.randn((6, 12), device=device), torch.zeros((6, 2), dtype=torch.int32, device=device)
+    want = router.topk(logits, 2)
+    for base in (logits, logits.clone().requires_grad_(), logits.T.contiguous().T):
+        with fwd.dual_level():
+            x = fwd.make_dual(base, torch.ones_like(base))
+            for call in (lambda: router.topk(x, 2), lambda: router.topk(x, 2, normalize=False),
+                         lambda: router.balance_loss(x, ids)):
+                with pytest.raises(RuntimeError, match="forward-mode"):
+                    call()
+            # what carries no tangent is computed as before
+            assert all(torch.equal(a, b) for a, b in zip(router.topk(logits, 2), want))
