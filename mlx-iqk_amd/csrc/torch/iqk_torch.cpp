@@ -273,7 +273,8 @@ PyObject *py_mx_quantize(PyObject *, PyObject *const *args, Py_ssize_t n) {
     int64_t row_stride = integer(args[1]);
     if (row_stride == 0) {
         const auto type = x.scalar_type();
-        if ((type != at::kFloat && type != at::kHalf && type != at::kBFloat16) || !ready(x) || x.size(-1) % 32)
+        if ((type != at::kFloat && type != at::kHalf && type != at::kBFloat16) || !ready(x) || x.size(-1) % 32 ||
+            wants_grad(x))
             Py_RETURN_NONE;
         row_stride = x.size(-1);
     }

@@ -58,6 +58,12 @@ own (2048 outputs: 8 rows 5.6 us against 7.8, 16 rows 8.9 against 8.4; 8192
 outputs: 4 rows 10.1 against 8.5)."""
 
 
+def _refuse_gradient(x: torch.Tensor) -> None:
+    if x.requires_grad and torch.is_grad_enabled():
+        raise IqkRuntimeError("no gradient flows back to x through 4-bit codes or the projections: detach x, or call "
+                              "under torch.no_grad()")
+
+
 def _check_width(n: int) -> int:
     if n <= 0 or n % BLOCK:
         raise IqkKernelError(f"a row of {n} values is not whole blocks of {BLOCK}")
@@ -160,7 +166,8 @@ def quantize(x: torch.Tensor) -> MxTensor:
 
     A block's scale is ``2**(floor(log2(largest magnitude)) - 2)``, at least
     2**-127; values round to nearest, ties to the even code, and saturate at 6
-    scales.  A block that holds a NaN or an infinity becomes NaN.
+    scales.  A block that holds a NaN or an infinity becomes NaN.  Codes carry no
+    gradient: an ``x`` that wants one is refused, as the projections refuse it.
     """
     if not isinstance(x, torch.Tensor):
         raise IqkKernelError("x must be a tensor of at least one dimension")
@@ -175,6 +182,7 @@ def quantize(x: torch.Tensor) -> MxTensor:
     if dtype not in _DTYPES:
         raise IqkKernelError(f"x must be one of {tuple(_DTYPES)}, got {dtype}")
     n = _check_width(x.shape[-1])
+    _refuse_gradient(x)
     stride, at = n, x.data_ptr()
     if not x.is_contiguous() or at % 16:
         stride = _row_stride(x)
@@ -271,9 +279,7 @@ class _MxStack(torch.nn.Module):
             raise IqkRuntimeError(f"x has rows of {width} values, the weights take {self.in_features}")
         if mx:
             return (act, _aligned_codes(rows), *_product_scales(x))
-        if rows.requires_grad and torch.is_grad_enabled():
-            raise IqkRuntimeError("the weights are frozen and no gradient flows through them: detach x, or call "
-                                  "under torch.no_grad()")
+        _refuse_gradient(rows)
         if not rows.is_contiguous() or rows.data_ptr() % 16:
             rows = rows.contiguous()
             rows = rows if rows.data_ptr() % 16 == 0 else rows.clone()

@@ -566,3 +566,17 @@ def test_forward_mode_derivatives_are_refused(device):
                 with pytest.raises(RuntimeError, match="forward-mode"):
                     call()
         assert line(base).shape == (3, 1, 1, 20) and line(wide).shape == (3, 1, 1, 20)
+
+
+def test_quantising_what_wants_a_gradient_is_refused(device):
+    """As a product of it is: codes carry no gradient."""
+    print("quantise with gradient", flush=True)
+    for dtype in (F32, F16, BF16):
+        x = torch.randn((4, 256), device=device).to(dtype).requires_grad_()
+        for t in (x, x[:, ::2], x[:, 8:72], x * 2, x[0], x[:0]):
+            with pytest.raises(IqkRuntimeError, match="detach"):
+                mx.quantize(t)
+            want = mx.quantize(t.detach())
+            with torch.no_grad():
+                got = mx.quantize(t)
+            assert torch.equal(got.codes, want.codes) and torch.equal(got.scales, want.scales)
