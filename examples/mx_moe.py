@@ -40,12 +40,13 @@ class MoE(torch.nn.Module):
     def forward(self, x: torch.Tensor, quantized: bool = False):
         """``x`` 16-bit ``[tokens, hidden]`` -> (y ``[tokens, hidden]``, logits, ids).
 
-        ``quantized``: the experts' activations in 4 bits too.
+        ``quantized``: the experts' activations in 4 bits too.  The experts have no
+        gradient in ``x``: one that wants it is refused.
         """
         logits = self.score(x.float())
         weights, ids = router.topk(logits, self.k)
         cast = mx.quantize if quantized else (lambda t: t)
-        rows = cast(x.detach()[:, None, None])  # [tokens, 1, 1, hidden]: a row for all its pairs
+        rows = cast(x[:, None, None])  # [tokens, 1, 1, hidden]: a row for all its pairs
         hidden = torch.nn.functional.silu(self.gate(rows, ids)) * self.up(rows, ids)
         y = self.down(cast(hidden), ids)[:, :, 0]  # [tokens, k, hidden]: a row a pair
         return (weights[..., None] * y).sum(1).to(x.dtype), logits, ids

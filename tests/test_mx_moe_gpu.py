@@ -80,3 +80,15 @@ def test_served_from_a_graph(mx_moe):
 def test_training_balances_the_router(mx_moe):
     balances = mx_moe.main("--experts 16 --hidden 160 --inner 96 --top-k 2 --sequences 3 --tokens 70 --steps 30".split())
     assert balances[-1] < balances[0]
+
+
+@pytest.mark.parametrize("quantized", (False, True))
+def test_a_gradient_in_x_is_refused(mx_moe, quantized):
+    """The layer's experts have no gradient in x, so a part of it (the router's) is not offered."""
+    moe = mx_moe.random_layer(12, 160, 96, 3)
+    x = torch.randn(5, 160, device="cuda", dtype=torch.bfloat16)
+    want = moe(x, quantized=quantized)[0]
+    with pytest.raises(RuntimeError, match="detach"):
+        moe(x.clone().requires_grad_(), quantized=quantized)
+    with torch.no_grad():
+        assert torch.equal(moe(x.clone().requires_grad_(), quantized=quantized)[0], want)
