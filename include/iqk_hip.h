@@ -296,6 +296,8 @@ int iqk_mx_dequantize(int dtype, const uint8_t *codes, const uint8_t *scales, in
 // out for the products, with R = out_features up to a multiple of 16, Q =
 // out_features / 64 and S = in_features / 128, both rounded up:
 //   tiles u8 [E][R / 16][S][64][16], tile_scales u8 [E][S][Q][64][4], row_exps i32 [E][R].
+// A row is kept over 2^row_exps, the power nearest to 1 that brings its scales within
+// 2^-13 .. 2^13, or where they are more than 2^26 apart the largest to 2^13.
 // A block more than 2^140 below its row's largest is taken as zero.
 int iqk_mx_pack(int64_t in_features, int64_t out_features, int64_t num_experts, const uint8_t *codes,
                 const uint8_t *scales, int64_t scale_stride, void *tiles, uint8_t *tile_scales, int32_t *row_exps,
@@ -307,13 +309,14 @@ int iqk_mx_unpack(int dtype, int64_t in_features, int64_t out_features, int64_t 
 
 // Products of token-expert pairs, each on its own (few pairs):
 //   y[p, r] = sum_k W[ids[p]][r][k] * x[p / pairs_per_x_row][k],
-// exact products, f32 sums, one rounding.  act names x's type: 16-bit rows
+// exact products, f32 sums (of the row over 2^row_exps), one rounding.  act names x's type: 16-bit rows
 // [n_x_rows, in_features], or 4-bit codes [n_x_rows, in_features / 2] with
 // x_scales (4-byte aligned, x_scale_stride a multiple of 4 and at least 4 S).
 // ids: u32 or (wide_ids) i64 [n_pairs], or NULL: all expert 0 of one.  An id
 // outside [0, num_experts) gives a NaN row.  y: [n_pairs, out_features].
 // With IQK_ACT_F16, weights below 2^-36 of their row's largest scale are rounded
-// to multiples of 2^-37 of it.  num_experts <= 4096, in_features % 32 == 0.
+// to multiples of 2^-37 of it where the row's scales are more than 2^26 apart, and
+// those below 2^-27 summed as exactly as values of 2^-27.  num_experts <= 4096, in_features % 32 == 0.
 int iqk_mx_pairs(int act, int64_t in_features, int64_t out_features, int64_t num_experts, const void *x,
                  int64_t n_x_rows, const uint8_t *x_scales, int64_t x_scale_stride, const void *tiles,
                  const uint8_t *tile_scales, const int32_t *row_exps, const void *ids, int wide_ids,

@@ -14,14 +14,17 @@
 //   rexp   i32 [E][rows]
 // so a lane's word of scales serves a wavefront's 64 rows, the MFMA selecting
 // the byte.  rows and columns round up to 16 (of tscale to 64) and 128 (codes 0,
-// scale 1).  A row's scales
-// are kept relative to its largest: byte + 140 - largest, and the row's
-// products are multiplied by 2^rexp, rexp = largest - 140, at the end.  So the
-// largest weight in a row is between 2^13 and 6 x 2^13, inside fp16, where
+// scale 1).  A row's scales are kept as byte - rexp, and its products' f32 sums are
+// multiplied by 2^rexp at the end.  rexp brings the row into fp16: it is 0 where every
+// block with a value has a scale of 2^-13 .. 2^13, whose weights are normal numbers
+// there, and otherwise the one nearest to 0 with which that holds.  So the sums are
+// those of the values themselves, and reach as far as f32 does, in every row but
+// those.  Where the row's scales are more than 2^26 apart its largest becomes 2^13:
 // weights down to 2^-36 of the largest scale are exact (fp16's smallest value
-// is 2^-24); a block below that rounds to multiples of 2^-24, under 2^-38 of the
-// row's largest weight.  bf16 and the scaled MFMA hold all of them; a block
-// more than 2^140 below its row's largest counts as zero.
+// is 2^-24), and a block below that rounds to multiples of 2^-24, under 2^-38 of the
+// row's largest weight; below 2^-27 of it they are subnormal, and the matrix cores
+// add them as exactly as values of 2^-27.  bf16 and the scaled MFMA hold all of them; a
+// block more than 2^140 below its row's largest counts as zero.
 #ifndef IQK_MX_H
 #define IQK_MX_H
 
@@ -33,7 +36,8 @@ constexpr int kMxBlock = 32;          // values of one scale
 constexpr int kMxStep = 128;          // columns of a tile
 constexpr int kMxRows = 16;           // rows of a tile
 constexpr int kMxTileBytes = 1024;
-constexpr int kMxTop = 140;           // the relative scale of a row's largest block
+constexpr int kMxTop = 140;           // the stored scale of a row's largest block, at most
+constexpr int kMxLow = 114;           // of its smallest, at least, where kMxTop leaves room
 
 enum MxDtype : int { MX_F32 = 0, MX_F16 = 1, MX_BF16 = 2 };
 

@@ -130,30 +130,43 @@ struct PackArgs {
     int64_t scale_stride;
 };
 
+// The power of two that is taken out of a row whose blocks with a value have scale
+// bytes least .. most.
+__device__ __forceinline__ int row_exponent(int least, int most) {
+    return most - min(max(most, kMxLow + most - least), kMxTop);
+}
+
 // One block of 256 threads a tile row (16 rows of one expert), thread (r, j):
-// first the row's largest scale among blocks with a value, then the tiles.
+// first the row's smallest and largest scale among blocks with a value, then the tiles.
 __global__ __launch_bounds__(256) void mx_pack_kernel(PackArgs a) {
-    __shared__ uint32_t part[kMxRows][16];
-    __shared__ uint32_t top[kMxRows];
+    __shared__ int least_of[kMxRows][16], most_of[kMxRows][16];
+    __shared__ int taken[kMxRows];
     const uint32_t trows = a.rows / kMxRows, e = blockIdx.x / trows, t = blockIdx.x % trows;
     const uint32_t tid = threadIdx.x, r = tid >> 4, j = tid & 15u, row = kMxRows * t + r;
     const size_t src = size_t(e) * a.out + row;
     const uint4_t *const codes = reinterpret_cast<const uint4_t *>(a.codes) + src * a.blocks;
     const uint8_t *const scales = a.scales + src * a.scale_stride;
-    uint32_t most = 0;
+    int least = 255, most = -1;
     if (row < a.out)
         for (uint32_t b = j; b < a.blocks; b += 16) {
-            const uint32_t s = scales[b];
+            const int s = scales[b];
             const uint4_t c = codes[b];
-            if (s != 255u && ((c.x | c.y | c.z | c.w) & 0x77777777u)) most = max(most, s + 1u);
+            if (s != 255 && ((c.x | c.y | c.z | c.w) & 0x77777777u)) {
+                least = min(least, s);
+                most = max(most, s);
+            }
         }
-    part[r][j] = most;
+    least_of[r][j] = least;
+    most_of[r][j] = most;
     __syncthreads();
     if (tid < kMxRows) {
-        uint32_t m = 0;
-        for (int k = 0; k < 16; ++k) m = max(m, part[tid][k]);
-        top[tid] = m ? m - 1u : 127u;
-        a.rexp[size_t(e) * a.rows + kMxRows * t + tid] = int32_t(top[tid]) - kMxTop;
+        least = 255, most = -1;
+        for (int k = 0; k < 16; ++k) {
+            least = min(least, least_of[tid][k]);
+            most = max(most, most_of[tid][k]);
+        }
+        taken[tid] = most < 0 ? 0 : row_exponent(least, most);
+        a.rexp[size_t(e) * a.rows + kMxRows * t + tid] = taken[tid];
     }
     __syncthreads();
     // thread -> lane 16 g + rr of step s
@@ -166,14 +179,14 @@ __global__ __launch_bounds__(256) void mx_pack_kernel(PackArgs a) {
         uint32_t byte = 127u;
         if (row2 < a.out && b < a.blocks) {
             c = reinterpret_cast<const uint4_t *>(a.codes)[src2 * a.blocks + b];
-            const uint32_t raw = a.scales[src2 * a.scale_stride + b];
+            const int raw = a.scales[src2 * a.scale_stride + b], kept = raw - taken[rr];
             // a block of zeros may have any scale, also one above the largest
-            if (raw == 255u)
+            if (raw == 255)
                 byte = 255u;
-            else if (raw + kMxTop < top[rr] || !((c.x | c.y | c.z | c.w) & 0x77777777u))
+            else if (kept < 0 || !((c.x | c.y | c.z | c.w) & 0x77777777u))
                 c = uint4_t{0, 0, 0, 0};
             else
-                byte = raw + kMxTop - top[rr];
+                byte = uint32_t(kept);
         }
         a.tiles[((size_t(e) * trows + t) * a.steps + s) * 64 + lane] = c;
         a.tscale[(((size_t(e) * a.steps + s) * a.quads + t / 4) * 64 + lane) * 4 + t % 4] = uint8_t(byte);
@@ -203,7 +216,7 @@ __global__ __launch_bounds__(kCastThreads) void mx_unpack_kernel(UnpackArgs a) {
         const uint32_t c = reinterpret_cast<const uint32_t *>(tile)[q];
         const uint32_t rel =
             a.tscale[(((size_t(e) * a.steps + s) * a.quads + row / 64) * 64 + 16 * g + row % 16) * 4 + row / 16 % 4];
-        // back to the format's byte: rel was byte + kMxTop - largest
+        // back to the format's byte
         const int byte = rel == 255u ? 255 : int(rel) + a.rexp[size_t(e) * a.rows + row];
         store_eight<DT>(a.y, 8u * size_t(i), c, scale_float(uint32_t(min(max(byte, 0), 255))));
     }

@@ -14,6 +14,14 @@ value.  A byte holds two codes, the even position's in its low half.
 Both projections take 16-bit activations, whose products with the weights are
 exact and summed in f32, or an :class:`MxTensor`, quantised activations, which the
 matrix cores multiply with the weights as they are, at four times the rate.
+
+A row of weights whose scales do not lie within 2**-13 .. 2**13 is brought there by a power
+of two before the products, which the sums get back.  What that costs: where the row's
+scales are more than 2**26 apart, float16 activations meet weights under 2**-27 of the
+largest scale in fewer bits, under 2**-36 as multiples of 2**-37 of it; and a block more than
+2**140 below the row's largest is zero, in :meth:`~MxSwitchLinear.dequantized` too.  Sums of
+such a row overflow where the scaled ones do, those of other rows where f32 does.
+
 Outputs are rounded once.  The weights are frozen: no gradient flows through, and an
 x that wants one, or has a forward-mode derivative, is refused.
 
@@ -216,9 +224,10 @@ class _MxStack(torch.nn.Module):
 
     * ``tiles`` u8 ``[E, out/16, in/128, 64, 16]``, the codes in the order that a
       wavefront loads them;
-    * ``tile_scales`` u8 ``[E, in/128, out/64, 64, 4]``, the blocks' scales relative to
-      their row's;
-    * ``row_exps`` i32 ``[E, out]``, each row's power of two.
+    * ``tile_scales`` u8 ``[E, in/128, out/64, 64, 4]``, the blocks' scales over their
+      row's power of two;
+    * ``row_exps`` i32 ``[E, out]``, that power: 0 for a row whose scales lie within
+      2**-13 .. 2**13.
 
     ``out`` and ``in`` round up to whole tiles; 4.27 bits a weight.
     """

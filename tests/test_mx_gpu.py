@@ -580,3 +580,47 @@ def test_quantising_what_wants_a_gradient_is_refused(device):
             with torch.no_grad():
                 got = mx.quantize(t)
             assert torch.equal(got.codes, want.codes) and torch.equal(got.scales, want.scales)
+
+
+@pytest.mark.parametrize("quantized", (False, True))
+@pytest.mark.parametrize("pairs", (5, 100, 1500))
+@pytest.mark.parametrize("exponent", (-112, 0, 118))
+def test_small_and_large_bfloat16_rows(device, quantized, pairs, exponent):
+    """Activations near both ends of f32, weights of ordinary size (scales of 2^-16 to 2^-6), by
+    every route: as exact as between.  The sums stay inside f32."""
+    print(f"range {quantized} {pairs} {exponent}", flush=True)
+    rng = np.random.default_rng(pairs)
+    E, out, n = 2, 48, 256
+    module, w = _switch(rng, E, out, n, device, lo=111, hi=121)
+    ids = rng.integers(0, E, pairs)
+    x = _dev(np.ldexp(np.clip(rng.standard_normal((pairs, n)), -3.9, 3.9), exponent), device, BF16)
+    q = mx.quantize(x) if quantized else x
+    xv = _f64(q.dequantize(F32) if quantized else x)
+    y = module(_shape(q, pairs, 1), _dev(ids, device)).view(pairs, out)
+    _check(y, xv, w, ids, BF16)
+    line = mx.MxLinear(out, n, device=device)
+    one = module.dequantized(F32)[0]
+    line.load(mx.quantize(one))
+    _check(line(q), xv, _f64(line.dequantized(F32))[None], np.zeros(pairs, int), BF16)
+
+
+def test_ordinary_rows_are_kept_as_they_are(device):
+    """Rows with scales of 2^-13 .. 2^13 have no power of two taken out, others the least that
+    brings them there, or their largest to 2^13; blocks without values have no say."""
+    print("row exponents", flush=True)
+    rows = ([127 - 13, 127 + 13], [120, 118], [127 - 14, 120], [127 - 40, 127 - 37], [127 + 14, 127], [127 + 30, 127 + 10],
+            [10, 50], [127 + 60, 127 - 60], [0, 0], [254, 254], [254, 0], [120, 255], [255, 255])
+    want = [0, 0, -1, -27, 1, 17, -90, 47, -114, 114, 114, 0, 0]
+    codes = np.full((1, len(rows) + 2, 64), 0x3f, dtype=np.uint8)
+    s = np.empty((1, len(rows) + 2, 4), dtype=np.uint8)
+    s[0, :-2, :2] = rows
+    s[0, -2:, :2] = [[130, 5], [5, 130]]
+    codes[0, -2, 16:32] = codes[0, -1, :16] = 0x80
+    codes[..., 32:] = 0x08
+    s[..., 2:] = [3, 250]
+    module = mx.MxSwitchLinear(1, len(rows) + 2, 128, device=device)
+    module.load(mx.MxTensor(_dev(codes, device), _dev(s, device)))
+    assert module.row_exps[0].tolist() == want + [0, 0] + [0]
+    values = mxref.values(codes, s)
+    values[0, 10, 32:64] = 0  # 2^254 below
+    np.testing.assert_array_equal(_f64(module.dequantized(F32)), _f64(torch.from_numpy(values).to(F32)))
