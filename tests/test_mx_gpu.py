@@ -624,3 +624,40 @@ def test_ordinary_rows_are_kept_as_they_are(device):
     values = mxref.values(codes, s)
     values[0, 10, 32:64] = 0  # 2^254 below
     np.testing.assert_array_equal(_f64(module.dequantized(F32)), _f64(torch.from_numpy(values).to(F32)))
+
+
+@pytest.mark.parametrize("pairs", (5, 100, 1500))
+def test_blocks_far_below_their_rows_largest(device, pairs):
+    """f16 rows take weights below 2^-36 of the row's largest scale as multiples of 2^-37 of
+    it (one product at a time: sums of those are another matter); bf16 and quantised rows hold
+    2^-140 of it, below which a block is zero."""
+    print(f"blocks apart {pairs}", flush=True)
+    rng = np.random.default_rng(31)
+    out, n = 48, 160
+    codes, s = mxref.random_codes(rng, (1, out, n))
+    below = np.array([0, 36, 38, 100, 141])  # powers of two below the row's first block
+    s[0] = 160 - below[None] - np.arange(out)[:, None] % 3
+    module = mx.MxSwitchLinear(1, out, n, device=device)
+    module.load(mx.MxTensor(_dev(codes, device), _dev(s, device)))
+    w = mxref.values(codes, s)
+    w[..., 128:] = 0
+    np.testing.assert_array_equal(_f64(module.dequantized(F32)), w)
+    ids = _dev(np.zeros(pairs, int), device)
+    for quantized in (False, True):
+        for first in (1, 2, 3, 4):  # only from this block on does the row have values
+            x = rng.standard_normal((pairs, n))
+            x[:, :32 * first] = 0
+            t = _dev(x, device, BF16)
+            q = mx.quantize(t) if quantized else t
+            xv = _f64(q.dequantize(F32) if quantized else t)
+            y = _f64(module(_shape(q, pairs, 1), ids).view(pairs, out))
+            want, bound = mxref.product_bound(xv, w[0], BF16)
+            assert (np.abs(y - want) <= bound).all(), (quantized, first)
+    unit = np.ldexp(1.0, s[0, :, :1].astype(int) - 127 - 37)
+    rounded = np.rint(w[0] / unit) * unit  # to the nearest, ties to even
+    x = np.zeros((pairs, n))
+    x[np.arange(pairs), rng.integers(32, n, pairs)] = rng.standard_normal(pairs)
+    t = _dev(x, device, F16)
+    y = _f64(module(_shape(t, pairs, 1), ids).view(pairs, out))
+    want = _f64(t) @ rounded.T
+    assert (np.abs(y - want) <= mxref.HALF_ULP[F16] * np.abs(want) + mxref.TINY[F16]).all()
