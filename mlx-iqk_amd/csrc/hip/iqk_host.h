@@ -12,6 +12,9 @@ namespace iqk {
 // Remember a launch failure's hipError_t for iqk_hip_last_error().
 int record_launch(hipError_t err);
 
+// Whether a one-dimensional grid can be launched: 2^32 threads cannot.
+inline bool grid_ok(int64_t blocks, int64_t threads) { return blocks < ((int64_t(1) << 32) + threads - 1) / threads; }
+
 inline hipStream_t as_stream(void *s) { return reinterpret_cast<hipStream_t>(s); }
 
 inline int stream_count(int member) {

@@ -130,6 +130,8 @@ struct PackArgs {
     int64_t scale_stride;
 };
 
+constexpr int kPackThreads = 256;
+
 // The power of two that is taken out of a row whose blocks with a value have scale
 // bytes least .. most.
 __device__ __forceinline__ int row_exponent(int least, int most) {
@@ -138,7 +140,7 @@ __device__ __forceinline__ int row_exponent(int least, int most) {
 
 // One block of 256 threads a tile row (16 rows of one expert), thread (r, j):
 // first the row's smallest and largest scale among blocks with a value, then the tiles.
-__global__ __launch_bounds__(256) void mx_pack_kernel(PackArgs a) {
+__global__ __launch_bounds__(kPackThreads) void mx_pack_kernel(PackArgs a) {
     __shared__ int least_of[kMxRows][16], most_of[kMxRows][16];
     __shared__ int taken[kMxRows];
     const uint32_t trows = a.rows / kMxRows, e = blockIdx.x / trows, t = blockIdx.x % trows;
@@ -232,7 +234,7 @@ uint32_t cast_blocks(uint64_t total) {
 bool mx_shape_ok(int64_t in, int64_t out, int64_t experts) {
     return in > 0 && in % kMxBlock == 0 && in < (int64_t(1) << 24) && out > 0 && out < (int64_t(1) << 24) &&
            experts > 0 && experts < (int64_t(1) << 20) &&
-           ((out + 15) / 16) * experts < (int64_t(1) << 31);
+           grid_ok((out + 15) / 16 * experts, kPackThreads);
 }
 
 bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
@@ -295,8 +297,8 @@ int iqk_mx_pack(int64_t in_features, int64_t out_features, int64_t num_experts, 
     PackArgs a{codes, scales, static_cast<uint4_t *>(tiles), tile_scales, row_exps, uint32_t(out_features), rows,
                uint32_t(in_features / kMxBlock), uint32_t((in_features + kMxStep - 1) / kMxStep),
                uint32_t((out_features + 63) / 64), scale_stride};
-    hipLaunchKernelGGL(mx_pack_kernel, dim3{uint32_t(num_experts * (rows / kMxRows))}, dim3{256}, 0, as_stream(stream),
-                       a);
+    hipLaunchKernelGGL(mx_pack_kernel, dim3{uint32_t(num_experts * (rows / kMxRows))}, dim3{kPackThreads}, 0,
+                       as_stream(stream), a);
     return record_launch(hipGetLastError());
 }
 

@@ -976,10 +976,12 @@ void mx_big_kernel(MxArgs a) {
     store_outputs<ACT, 4, 8>(a, t.e, t.n0 + 64 * wr, dst + 128 * wc, acc, lane);
 }
 
+inline int pair_waves(const MxArgs &a) { return a.steps > 4 * kPairSteps ? 8 : 4; }
+
 template <int ACT>
 void launch_pairs(const MxArgs &a, hipStream_t stream) {
     const dim3 grid{a.n_slots * (a.rows / kMxRows)};
-    if (a.steps > 4 * kPairSteps)
+    if (pair_waves(a) == 8)
         hipLaunchKernelGGL((mx_pair_kernel<ACT, 8>), grid, dim3{512}, 0, stream, a);
     else
         hipLaunchKernelGGL((mx_pair_kernel<ACT, 4>), grid, dim3{256}, 0, stream, a);
@@ -1090,7 +1092,7 @@ int iqk_mx_pairs(int act, int64_t in_features, int64_t out_features, int64_t num
                                 tiles, tile_scales, row_exps, n_pairs, y);
     if (rc != IQK_OK || n_pairs == 0) return rc;
     if ((!ids && num_experts != 1) || pairs_per_x_row <= 0 || pairs_per_x_row >= (int64_t(1) << 31) ||
-        (n_pairs - 1) / pairs_per_x_row >= n_x_rows || n_pairs * (a.rows / kMxRows) >= (int64_t(1) << 31))
+        (n_pairs - 1) / pairs_per_x_row >= n_x_rows || !grid_ok(n_pairs * (a.rows / kMxRows), 64 * pair_waves(a)))
         return IQK_ERR_ARGUMENT;
     a.ids = static_cast<const uint32_t *>(ids);
     a.wide = wide_ids != 0;
@@ -1114,8 +1116,9 @@ int iqk_mx_groups(int act, int64_t in_features, int64_t out_features, int64_t nu
                                 tiles, tile_scales, row_exps, n_slots, y);
     if (rc != IQK_OK || n_slots == 0) return rc;
     if (!group_offsets && num_experts != 1) return IQK_ERR_ARGUMENT;
-    const int64_t mtiles = group_offsets ? n_slots / kMxBM + num_experts : (n_slots + kMxBM - 1) / kMxBM;
-    if (mtiles * ((out_features + kMxBN - 1) / kMxBN) >= (int64_t(1) << 31)) return IQK_ERR_ARGUMENT;
+    // with the M-tiles that make whole sets for the XCDs; larger and smaller tiles make smaller grids
+    const int64_t mtiles = (group_offsets ? n_slots / kMxBM + num_experts : (n_slots + kMxBM - 1) / kMxBM) + 31;
+    if (!grid_ok(mtiles * ((out_features + kMxBN - 1) / kMxBN), 64 * kMxWaves)) return IQK_ERR_ARGUMENT;
     a.offs = group_offsets;
     a.xr = x_rows;
     a.yr = y_rows;

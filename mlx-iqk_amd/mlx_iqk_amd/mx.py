@@ -242,7 +242,7 @@ class _MxStack(torch.nn.Module):
             raise IqkRuntimeError(f"out_features must be positive, got {out_features}")
         rows, steps = (self.out_features + 15) // 16 * 16, (self.in_features + _STEP - 1) // _STEP
         E = self.num_experts
-        self._pair_limit = pair_limit(E)
+        self._pair_limit = min(pair_limit(E), 2 ** 27 // rows)  # 2**23 workgroups of 16 outputs can be launched
         self.register_buffer("tiles", torch.zeros((E, rows // 16, steps, 64, 16), dtype=torch.uint8, device=device))
         self.register_buffer("tile_scales", torch.zeros((E, steps, (rows + 63) // 64, 64, 4), dtype=torch.uint8,
                                                         device=device))

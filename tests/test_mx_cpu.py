@@ -173,3 +173,19 @@ def test_plain_quantisation_finds_the_nearest_code():
     assert ((top >= 4) & (top < 8)).all()
     ties = np.array([[0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0, 4.0] * 4])
     np.testing.assert_array_equal(mxref.values(*mxref.quantize(ties))[0, :8], [0, 1, 1, 2, 2, 4, 4, 4])
+
+
+def test_grids_that_cannot_be_launched_are_refused(lib):
+    """2^32 threads are one too many: 256 or 512 a workgroup."""
+    def pairs(n, rows, out=16):
+        return lib.iqk_mx_pairs(0, n, out, 2, P, rows, None, 0, P, P, P, P, 0, 1, rows, P, None)
+
+    assert pairs(64, 1 << 24) == ARGUMENT and pairs(64, 1 << 20, out=256) == ARGUMENT
+    assert pairs(4096, 1 << 23) == ARGUMENT and pairs(4096, 1 << 19, out=256) == ARGUMENT
+    assert lib.iqk_mx_groups(0, 64, 512, 2, P, 4, None, 0, P, P, P, P, P, P, 1 << 30, P, None) == ARGUMENT
+    assert lib.iqk_mx_groups(0, 64, 512, 1, P, 4, None, 0, P, P, P, None, None, None, 1 << 30, P, None) == ARGUMENT
+    assert lib.iqk_mx_pack(64, 272, (1 << 20) - 1, P, P, 2, P, P, P, None) == GEOMETRY
+    assert lib.iqk_hip_last_error() == 0  # none reached a launch
+    # a module groups its pairs before there are so many
+    few = mx.MxSwitchLinear(4096, 1 << 18, 32, device="meta")._pair_limit
+    assert few == 512 < mx.pair_limit(4096)
