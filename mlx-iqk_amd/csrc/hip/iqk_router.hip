@@ -231,7 +231,7 @@ template <int DT, int VPT, bool NORM, bool QUADS>
 __global__ __launch_bounds__(256) void topk_kernel(TopkArgs a) {
     constexpr bool WIDE = DT == MX_F32;
     const uint32_t lane = threadIdx.x & 63u, j = lane & 15u;
-    const uint32_t row = (blockIdx.x * 256 + threadIdx.x) / kRowLanes;
+    const uint32_t row = blockIdx.x * 16 + threadIdx.x / kRowLanes;
     const bool live = row < a.rows;
     RowWords<DT, VPT> words;
     load_words<DT, VPT, QUADS>(a.logits, live ? row : 0u, a.E, j, words);
@@ -556,6 +556,25 @@ __global__ __launch_bounds__(256) void balance_grad_kernel(BalanceArgs a) {
     }
 }
 
+// launch(a, workgroups) for each part of the rows that one launch holds (2^32 threads are
+// too many), a's pointers moved to it; 16 rows, a workgroup's, keep every alignment.
+template <typename F>
+void by_rows(const TopkArgs &all, int64_t rows, int dtype, F &&launch) {
+    constexpr int64_t kPart = int64_t(1) << 27;
+    const int64_t size = dtype == MX_F32 ? 4 : 2;
+    for (int64_t first = 0; first < rows; first += kPart) {
+        TopkArgs a = all;
+        const int64_t n = rows - first < kPart ? rows - first : kPart;
+        a.rows = uint32_t(n);
+        if (a.logits) a.logits = static_cast<const char *>(a.logits) + first * all.E * size;
+        if (a.dlogits) a.dlogits = static_cast<char *>(a.dlogits) + first * all.E * size;
+        a.weights += first * all.k;
+        a.ids += first * all.k;
+        if (a.dweights) a.dweights += first * all.k;
+        launch(a, uint32_t((n + 15) / 16));
+    }
+}
+
 // f(dtype, places a lane, quads) as compile-time constants.
 template <typename F>
 void by_shape(int dtype, int64_t experts, bool quads, F &&f) {
@@ -617,18 +636,18 @@ int iqk_router_topk(int dtype, const void *logits, int64_t rows, int64_t experts
     a.logits = logits;
     a.weights = weights;
     a.ids = ids;
-    a.rows = uint32_t(rows);
     a.E = uint32_t(experts);
     a.k = uint32_t(k);
     const bool quads = quads_ok(dtype, experts, logits, nullptr);
-    const dim3 grid{uint32_t((rows + 15) / 16)};
     by_shape(dtype, experts, quads, [&](auto dt, auto vpt, auto qd) {
         constexpr int DT = decltype(dt)::value, VPT = decltype(vpt)::value;
         constexpr bool Q = decltype(qd)::value;
-        if (normalize)
-            hipLaunchKernelGGL((topk_kernel<DT, VPT, true, Q>), grid, dim3{256}, 0, as_stream(stream), a);
-        else
-            hipLaunchKernelGGL((topk_kernel<DT, VPT, false, Q>), grid, dim3{256}, 0, as_stream(stream), a);
+        by_rows(a, rows, dtype, [&](const TopkArgs &part, uint32_t blocks) {
+            if (normalize)
+                hipLaunchKernelGGL((topk_kernel<DT, VPT, true, Q>), dim3{blocks}, dim3{256}, 0, as_stream(stream), part);
+            else
+                hipLaunchKernelGGL((topk_kernel<DT, VPT, false, Q>), dim3{blocks}, dim3{256}, 0, as_stream(stream), part);
+        });
     });
     return record_launch(hipGetLastError());
 }
@@ -647,18 +666,18 @@ int iqk_router_topk_grad(int dtype, const void *logits, const float *weights, co
     a.ids = const_cast<int32_t *>(ids);
     a.dweights = dweights;
     a.dlogits = dlogits;
-    a.rows = uint32_t(rows);
     a.E = uint32_t(experts);
     a.k = uint32_t(k);
     const bool quads = quads_ok(dtype, experts, normalize ? nullptr : logits, dlogits);
-    const dim3 grid{uint32_t((rows + 15) / 16)};
     by_shape(dtype, experts, quads, [&](auto dt, auto vpt, auto qd) {
         constexpr int DT = decltype(dt)::value, VPT = decltype(vpt)::value;
         constexpr bool Q = decltype(qd)::value;
-        if (normalize)
-            hipLaunchKernelGGL((topk_grad_kernel<DT, VPT, true, Q>), grid, dim3{256}, 0, as_stream(stream), a);
-        else
-            hipLaunchKernelGGL((topk_grad_kernel<DT, VPT, false, Q>), grid, dim3{256}, 0, as_stream(stream), a);
+        by_rows(a, rows, dtype, [&](const TopkArgs &part, uint32_t blocks) {
+            if (normalize)
+                hipLaunchKernelGGL((topk_grad_kernel<DT, VPT, true, Q>), dim3{blocks}, dim3{256}, 0, as_stream(stream), part);
+            else
+                hipLaunchKernelGGL((topk_grad_kernel<DT, VPT, false, Q>), dim3{blocks}, dim3{256}, 0, as_stream(stream), part);
+        });
     });
     return record_launch(hipGetLastError());
 }

@@ -407,3 +407,62 @@ def test_forward_mode_derivatives_are_refused(device):
                     call()
             # what carries no tangent is computed as before
             assert all(torch.equal(a, b) for a, b in zip(router.topk(logits, 2), want))
+
+
+@pytest.mark.parametrize("normalize", (True, False))
+def test_topk_past_32_bits(device, normalize):
+    """More than 2^28 tokens (2^32 threads) and 2^32 logits, with the gradient."""
+    print(f"topk past 2^32 {normalize}", flush=True)
+    rows, experts, k = 2 ** 28 + 37, 17, 2
+    g = torch.Generator(device=device).manual_seed(7)
+    logits = torch.empty((rows, experts), dtype=F16, device=device)
+    for part in logits.split(2 ** 25):
+        part.copy_(torch.randn(part.shape, dtype=F16, device=device, generator=g))
+    assert logits.numel() > 2 ** 32
+    at = np.r_[0, 1, 2 ** 27 - 1, 2 ** 27, 2 ** 28 - 16, 2 ** 28 - 1, 2 ** 28, rows - 1]
+    index = torch.from_numpy(at).to(device)
+    x = _f64(logits[index])
+    weights, ids = router.topk(logits.requires_grad_(), k, normalize=normalize)
+    want_w, want_ids = mxref.topk(x, k, normalize)
+    np.testing.assert_array_equal(ids[index].cpu().numpy(), want_ids)
+    assert (np.abs(_f64(weights[index]) - want_w) <= (_rel(experts) + k * ULP) * want_w + FLOOR).all()
+    few, few_ids = router.topk(logits.detach()[-99:], k, normalize=normalize)
+    assert torch.equal(weights.detach()[-99:], few) and torch.equal(ids[-99:], few_ids)
+    dw = torch.arange(1, k + 1, device=device, dtype=F32).expand(rows, k)
+    (grad,) = torch.autograd.grad(weights, logits, dw)
+    want = mxref.topk_grad(x, k, normalize, np.broadcast_to(np.arange(1.0, k + 1), (len(at), k)))
+    # |p| (|dw| + sum |w dw|) <= 2 k, each as exact as a probability, and the rounding
+    bound = 3 * (_rel(experts) + k * ULP) * 2 * k + _rounded(F16) * np.abs(want) + mxref.TINY[F16]
+    assert (np.abs(_f64(grad[index]) - want) <= bound).all()
+
+
+def test_balance_past_32_bits(device):
+    """A group of more than 2^32 logits, with its gradient."""
+    print("balance past 2^32", flush=True)
+    tokens, experts, k = 2 ** 22 + 5, 1024, 2
+    g = torch.Generator(device=device).manual_seed(8)
+    logits = torch.empty((tokens, experts), dtype=F16, device=device)
+    for part in logits.split(2 ** 19):
+        part.copy_(torch.randn(part.shape, dtype=F16, device=device, generator=g))
+    assert logits.numel() > 2 ** 32
+    ids = torch.randint(0, experts, (tokens, k), dtype=torch.int32, device=device, generator=g)
+    mean = torch.zeros(experts, dtype=torch.float64, device=device)
+    for part in logits.split(2 ** 19):
+        mean += torch.softmax(part.double(), -1).sum(0) / tokens
+    loss, counts = router.balance_loss(logits.requires_grad_(), ids)
+    want_counts = torch.bincount(ids.reshape(-1), minlength=experts)
+    assert torch.equal(counts.long(), want_counts)
+    want = float(experts * (want_counts.double() / (k * tokens) * mean).sum())
+    # a lane adds its share's tokens, then wavefronts, shares and experts
+    steps = tokens / 512 / 32 + 8 + 512 + experts / 64 + 8
+    assert abs(float(loss.detach()) - want) <= (_rel(experts) + steps * ULP) * want
+    # times 2^22, so that fp16 holds it
+    (grad,) = torch.autograd.grad(loss, logits, torch.tensor(2.0 ** 22, device=device))
+    at = np.r_[0, 2 ** 21, 2 ** 22 - 1, tokens - 1]
+    index = torch.from_numpy(at).to(device)
+    p, c = mxref.softmax(_f64(logits[index])), want_counts.double().cpu().numpy()
+    factor = 2.0 ** 22 * experts / (k * float(tokens) ** 2)
+    exact = factor * p * (c - (c * p).sum(-1, keepdims=True))
+    size = factor * p * (c + (c * p).sum(-1, keepdims=True))
+    bound = 3 * _rel(experts) * size + _rounded(F16) * np.abs(exact) + mxref.TINY[F16]
+    assert (np.abs(_f64(grad[index]) - exact) <= bound).all()
