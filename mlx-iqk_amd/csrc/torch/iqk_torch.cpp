@@ -125,7 +125,9 @@ BalanceSums balance_forward(const Tensor &logits, const Tensor &ids, const Tenso
     s.counts = empty(shape, at::kInt, logits);
     s.kept = empty(lead, at::kInt, logits);
     if (groups) {
-        const Tensor work = empty({iqk_balance_work(groups, tokens, experts)}, at::kInt, logits);
+        const int64_t words = iqk_balance_work(groups, tokens, experts);
+        check(words < 0 ? IQK_ERR_GEOMETRY : IQK_OK, "iqk_balance_work");
+        const Tensor work = empty({words}, at::kInt, logits);
         check(iqk_balance(type_code(logits), logits.data_ptr(), ptr<int32_t>(ids), ptr<uint8_t>(mask), groups, tokens,
                           experts, k, ptr<uint32_t>(work), ptr<float>(s.loss), ptr<int32_t>(s.counts),
                           ptr<int32_t>(s.kept), stream_of(logits)),

@@ -10,6 +10,8 @@ not differentiable again, and logits with a forward-mode derivative are refused.
 
 from __future__ import annotations
 
+import math
+
 import torch
 
 from . import _native
@@ -18,6 +20,8 @@ from .mx import _DTYPES
 
 MAX_EXPERTS = 1024
 MAX_K = 64
+MAX_GROUPS = 65535
+"""Losses of one :func:`balance_loss` call."""
 
 
 def _check_logits(logits: torch.Tensor, dims: int) -> int:
@@ -56,7 +60,8 @@ def balance_loss(logits: torch.Tensor, ids: torch.Tensor, *,
     """How unevenly tokens fall on experts: ``(loss f32 [...], counts i32 [..., experts])``.
 
     ``logits`` is ``[..., tokens, experts]``, ``ids`` the chosen experts ``[..., tokens,
-    k]``; each leading index (a sequence, say) has a loss of its own.  With n
+    k]``; each leading index (a sequence, say) has a loss of its own, up to
+    :data:`MAX_GROUPS` of them.  With n
     tokens, ``f_e = counts_e / (k n)`` the share of the pairs that name expert e
     and ``P_e`` the mean of its softmax probability, ``loss = experts * sum_e f_e
     P_e``: 1 where either is even, up to ``experts / k`` where the same k experts
@@ -74,6 +79,9 @@ def balance_loss(logits: torch.Tensor, ids: torch.Tensor, *,
     k = int(ids.shape[-1])
     if not 0 < k <= min(MAX_K, experts):
         raise IqkKernelError(f"a token has 1 .. {min(MAX_K, experts)} of {experts} experts, got {k}")
+    groups = math.prod(logits.shape[:-2])
+    if groups > MAX_GROUPS:
+        raise IqkKernelError(f"a call gives at most {MAX_GROUPS} losses, logits {tuple(logits.shape)} ask for {groups}")
     if mask is not None:
         if mask.dtype != torch.bool or mask.device != logits.device or tuple(mask.shape) != tuple(logits.shape[:-1]):
             raise IqkKernelError(f"mask must be bool {tuple(logits.shape[:-1])} on {logits.device}, got {mask.dtype} "
@@ -84,4 +92,4 @@ def balance_loss(logits: torch.Tensor, ids: torch.Tensor, *,
     return _native.torch_binding().balance(logits.contiguous(), ids.contiguous(), mask)
 
 
-__all__ = ["MAX_EXPERTS", "MAX_K", "balance_loss", "topk"]
+__all__ = ["MAX_EXPERTS", "MAX_GROUPS", "MAX_K", "balance_loss", "topk"]

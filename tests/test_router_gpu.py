@@ -466,3 +466,27 @@ def test_balance_past_32_bits(device):
     size = factor * p * (c + (c * p).sum(-1, keepdims=True))
     bound = 3 * _rel(experts) * size + _rounded(F16) * np.abs(exact) + mxref.TINY[F16]
     assert (np.abs(_f64(grad[index]) - exact) <= bound).all()
+
+
+def test_balance_takes_65535_groups(device):
+    """And says so for one more."""
+    print("balance groups", flush=True)
+    rng = np.random.default_rng(16)
+    logits = _logits(rng, 1, 1, 65536, 1, 8, dtype=F32, device=device)[0]
+    ids = torch.from_numpy(rng.integers(0, 8, (1, 65536, 1, 2))).to(device)
+    with pytest.raises(IqkKernelError, match="65535"):
+        router.balance_loss(logits, ids)
+    with pytest.raises(RuntimeError, match="iqk_balance_work"):  # nor 2^31 tokens
+        router.balance_loss(logits.view(-1)[:1].to(F16).expand(2 ** 31, 1), ids.view(-1)[:1].expand(2 ** 31, 1))
+    logits = logits[:, 1:].clone().requires_grad_()
+    loss, counts = router.balance_loss(logits, ids[:, 1:])
+    (grad,) = torch.autograd.grad(loss, logits, torch.ones_like(loss))
+    assert loss.shape == (1, 65535) and counts.shape == (1, 65535, 8)
+    for g in (0, 32768, 65534):
+        x, named, one = _f64(logits)[0, g], ids[0, 1 + g].cpu().numpy(), np.ones(1, bool)
+        want, want_counts = mxref.balance(x, named, one)
+        np.testing.assert_array_equal(counts[0, g].cpu().numpy(), want_counts)
+        assert abs(_f64(loss)[0, g] - want) <= (_rel(8) + 8 * ULP) * want
+        p = mxref.softmax(x)
+        size = 8 / 2 * p * (want_counts + (p * want_counts).sum(-1, keepdims=True))
+        assert (np.abs(_f64(grad)[0, g] - mxref.balance_grad(x, named, one)) <= 3 * _rel(8) * size + 64 * FLOOR).all()
