@@ -11,6 +11,7 @@
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <ATen/ATen.h>
+#include <c10/hip/HIPException.h>
 #include <c10/hip/HIPStream.h>
 
 #include "iqk_hip.h"
@@ -47,6 +48,15 @@ void check(int rc, const char *what) {
 template <typename T>
 T *ptr(const Tensor &t) {
     return t.defined() ? static_cast<T *>(t.data_ptr()) : nullptr;
+}
+
+// A backward pass under a graph's capture has ended the process when the capture ended, for
+// a reason that is not known; only the forward calls are for a graph.
+void refuse_capture() {
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    C10_HIP_CHECK(hipStreamIsCapturing(c10::hip::getCurrentHIPStream().stream(), &status));
+    TORCH_CHECK(status == hipStreamCaptureStatusNone,
+                "the router's gradients cannot be captured in a graph; run the backward pass eagerly");
 }
 
 // A gradient that is not differentiable again says so when asked.  It depends on what
@@ -87,6 +97,7 @@ struct TopK : torch::autograd::Function<TopK> {
         return {weights, ids};
     }
     static variable_list backward(AutogradContext *ctx, variable_list grads) {
+        refuse_capture();
         if (!grads[0].defined()) return {Tensor(), Tensor(), Tensor()};
         const auto saved = ctx->get_saved_variables();
         const Tensor &weights = saved[0], &ids = saved[1], &logits = saved[2];
@@ -148,6 +159,7 @@ struct Balance : torch::autograd::Function<Balance> {
         return {s.loss, s.counts};
     }
     static variable_list backward(AutogradContext *ctx, variable_list grads) {
+        refuse_capture();
         if (!grads[0].defined()) return {Tensor(), Tensor(), Tensor()};
         const auto saved = ctx->get_saved_variables();
         const Tensor &logits = saved[0], &counts = saved[1], &kept = saved[2], &mask = saved[3];

@@ -6,6 +6,7 @@ weights, and the loss that keeps the experts evenly loaded; with gradients.
 its weights scale their outputs.  Logits are f32, f16 or bf16 on a GPU, for up to
 1024 experts; sums, probabilities, weights and losses are f32.  Gradients are
 not differentiable again, and logits with a forward-mode derivative are refused.
+The calls can be captured in a graph; their gradients cannot, and raise under a capture.
 """
 
 from __future__ import annotations

@@ -490,3 +490,28 @@ def test_balance_takes_65535_groups(device):
         p = mxref.softmax(x)
         size = 8 / 2 * p * (want_counts + (p * want_counts).sum(-1, keepdims=True))
         assert (np.abs(_f64(grad)[0, g] - mxref.balance_grad(x, named, one)) <= 3 * _rel(8) * size + 64 * FLOOR).all()
+
+
+def test_gradients_under_capture_are_refused(device):
+    """The nodes themselves, without the autograd engine: nothing of a backward pass runs under
+    the capture, and the graph of what was captured beside them replays."""
+    print("gradients under capture", flush=True)
+    logits = torch.randn((6, 12), device=device).requires_grad_()
+    weights, ids = router.topk(logits, 3)
+    loss, _ = router.balance_loss(logits, ids)
+    dw, one, x = torch.ones_like(weights), torch.ones_like(loss), torch.zeros(8, device=device)
+    with torch.no_grad():
+        weights.grad_fn(dw, None)  # not captured: as ever
+        loss.grad_fn(one, None)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        x += 1
+        with torch.no_grad():
+            for node, above in ((weights.grad_fn, dw), (loss.grad_fn, one)):
+                with pytest.raises(RuntimeError, match="captured"):
+                    node(above, None)
+    for n in (1, 2):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert x.tolist() == [float(n)] * 8
