@@ -19,6 +19,9 @@
 #ifndef IQK_SOURCE_HASH
 #define IQK_SOURCE_HASH "unset"
 #endif
+#ifndef IQK_BINDING_HASH
+#define IQK_BINDING_HASH "unset"
+#endif
 
 namespace {
 
@@ -353,11 +356,13 @@ PyObject *py_mx_project(PyObject *, PyObject *const *args, Py_ssize_t n) {
 }
 
 PyObject *source_hash(PyObject *, PyObject *) { return PyUnicode_FromString(IQK_SOURCE_HASH); }
+PyObject *binding_hash(PyObject *, PyObject *) { return PyUnicode_FromString(IQK_BINDING_HASH); }
 
 #define METHOD(name) {#name, (PyCFunction)(void (*)(void))py_##name, METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {
     METHOD(topk), METHOD(balance), METHOD(mx_quantize), METHOD(mx_dequantize), METHOD(mx_project),
     {"source_hash", source_hash, METH_NOARGS, "digest of the kernel sources this binding was built with"},
+    {"binding_hash", binding_hash, METH_NOARGS, "digest of this binding's own source and torch's version"},
     {nullptr, nullptr, 0, nullptr},
 };
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_iqk_torch", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

@@ -155,17 +155,21 @@ def launcher():
 
 def torch_binding():
     """The torch binding of the 4-bit and router calls (``_iqk_torch``); raises
-    where it is not built, or was built with other sources than the library."""
+    where it is not built, or was built with other sources than the library or than
+    its own now, or for another torch."""
     global _TORCH
     if _TORCH is None:
         digest = load().iqk_hip_source_hash().decode()
         if not TORCH_EXT.is_file():
             raise IqkNativeError(f"{TORCH_EXT} is not built; run `python -m mlx_iqk_amd.build`")
-        import torch  # noqa: F401  (its libraries, which the binding links against)
+        import torch  # its libraries, which the binding links against
         mod = _import("_iqk_torch", TORCH_EXT)
         if mod.source_hash() != digest:
             raise IqkNativeError(f"{TORCH_EXT} was built with other sources than {HIP_LIB}; rebuild both with "
                                  "`python -m mlx_iqk_amd.build`")
+        if mod.binding_hash() != build.torch_binding_hash():
+            raise IqkNativeError(f"{TORCH_EXT} was built from another {build.TORCH_SOURCE.name} or for another torch than "
+                                 f"{torch.__version__}; rebuild it with `python -m mlx_iqk_amd.build`")
         _TORCH = mod
     return _TORCH
 

@@ -146,6 +146,18 @@ def build_launch() -> Path:
     return LAUNCH_EXT
 
 
+TORCH_SOURCE = CSRC / "torch" / "iqk_torch.cpp"
+
+
+def torch_binding_hash() -> str:
+    """A digest of what the torch binding is compiled from: its source, torch's
+    version, and the kernel library's own digest.  Compiled into the binding
+    (``binding_hash``), as the library's is into it."""
+    import torch
+    h = hashlib.sha256(hip_source_hash().encode() + TORCH_SOURCE.read_bytes() + torch.__version__.encode())
+    return h.hexdigest()[:16]
+
+
 def torch_command(out: Path = TORCH_EXT, source_hash: str = "") -> list[str]:
     """The torch binding, against torch's own headers and libraries and the
     kernel library beside it."""
@@ -156,8 +168,8 @@ def torch_command(out: Path = TORCH_EXT, source_hash: str = "") -> list[str]:
             f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
             f"-I{include}", f"-I{include / 'torch' / 'csrc' / 'api' / 'include'}",
             f"-I{Path(_hipcc()).resolve().parents[1] / 'include'}", f"-I{sysconfig.get_paths()['include']}",
-            f"-I{INCLUDE}", f'-DIQK_SOURCE_HASH="{source_hash or hip_source_hash()}"', "-o", str(out),
-            str(CSRC / "torch" / "iqk_torch.cpp"), f"-L{home / 'lib'}", "-ltorch", "-ltorch_cpu", "-lc10",
+            f"-I{INCLUDE}", f'-DIQK_SOURCE_HASH="{source_hash or hip_source_hash()}"',
+            f'-DIQK_BINDING_HASH="{torch_binding_hash()}"', "-o", str(out), str(TORCH_SOURCE), f"-L{home / 'lib'}", "-ltorch", "-ltorch_cpu", "-lc10",
             "-lc10_hip", "-ltorch_python", f"-L{LIBDIR}", "-liqk_hip", "-Wl,-rpath,$ORIGIN"]
 
 

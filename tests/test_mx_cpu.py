@@ -189,3 +189,21 @@ def test_grids_that_cannot_be_launched_are_refused(lib):
     # a module groups its pairs before there are so many
     few = mx.MxSwitchLinear(4096, 1 << 18, 32, device="meta")._pair_limit
     assert few == 512 < mx.pair_limit(4096)
+
+
+def test_a_torch_binding_of_another_source_or_torch_is_refused(monkeypatch, tmp_path, lib):
+    assert _native.torch_binding().binding_hash() == build.torch_binding_hash()
+    edited = tmp_path / "iqk_torch.cpp"
+    edited.write_bytes(build.TORCH_SOURCE.read_bytes() + b"\n")
+    for at, name, value in ((build, "TORCH_SOURCE", edited), (torch, "__version__", torch.__version__ + "x")):
+        with monkeypatch.context() as m:
+            m.setattr(_native, "_TORCH", None)
+            m.setattr(at, name, value)
+            with pytest.raises(_native.IqkNativeError, match="another"):
+                _native.torch_binding()
+    with monkeypatch.context() as m:  # a library of other sources than the binding's
+        m.setattr(_native, "_TORCH", None)
+        m.setattr(_native, "_import", lambda *_: type("Stale", (), {"source_hash": staticmethod(lambda: "0" * 16)}))
+        with pytest.raises(_native.IqkNativeError, match="other sources"):
+            _native.torch_binding()
+    assert _native.torch_binding() is not None
