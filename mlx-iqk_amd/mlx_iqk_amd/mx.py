@@ -400,4 +400,4 @@ class MxLinear(_MxStack):
         return f"{self.out_features}, {self.in_features}"
 
 
-__all__ = ["BLOCK", "PAIR_LIMIT", "MxLinear", "MxSwitchLinear", "MxTensor", "dequantize", "quantize"]
+__all__ = ["BLOCK", "ROW_LIMIT", "MxLinear", "MxSwitchLinear", "MxTensor", "dequantize", "pair_limit", "quantize"]

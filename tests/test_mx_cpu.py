@@ -207,3 +207,10 @@ def test_a_torch_binding_of_another_source_or_torch_is_refused(monkeypatch, tmp_
         with pytest.raises(_native.IqkNativeError, match="other sources"):
             _native.torch_binding()
     assert _native.torch_binding() is not None
+
+
+def test_every_public_name_is_there():
+    import mlx_iqk_amd
+    for module in (mlx_iqk_amd, mx, router):
+        for name in module.__all__:
+            assert getattr(module, name) is not None, (module.__name__, name)
