@@ -359,8 +359,8 @@ int iqk_router_topk_grad(int dtype, const void *logits, const float *weights, co
 // [groups, tokens], NULL: all), with c_e the pairs that name expert e and S_e
 // the sum of its softmax probabilities,
 //   loss[g] = experts / (k n^2) * sum_e c_e S_e      (0 where n is 0).
-// Ids outside [0, experts) count for none.  logits dtype [groups, tokens,
-// experts]; ids i32 [groups, tokens, k]; counts i32 [groups, experts]; kept i32
+// Ids outside [0, experts) count for none.  groups <= 65535; logits dtype [groups,
+// tokens, experts]; ids i32 [groups, tokens, k]; counts i32 [groups, experts]; kept i32
 // [groups]; work: iqk_balance_work words.  The same inputs give the same bits.
 int64_t iqk_balance_work(int64_t groups, int64_t tokens, int64_t experts);
 int iqk_balance(int dtype, const void *logits, const int32_t *ids, const uint8_t *mask, int64_t groups,

@@ -214,7 +214,7 @@ __global__ __launch_bounds__(64 * WAVES) void mx_pair_kernel(MxArgs a) {
 // Measured, [2048 x 4096]: 144 pairs of 4-bit slots through 256 experts (117
 // named) 86 us (5.7 TB/s: the weights), the 2048-token Zipf prefill (12288
 // slots in bf16, 255 experts) 310 us, where 8192 evenly spread take 233 (4.9 TB/s)
-// and 32768 550 (1.0 PFLOP/s; the matrix cores are busy for 55% of 1.6 GHz).
+// and 32768 530 (1.0 PFLOP/s; the matrix cores are busy for 61% of 1.6 GHz).
 //
 // The workgroups of an M-tile's outputs run on one XCD, with those of the next
 // few M-tiles, so that it reads a slot's activations once for all outputs and a slice
@@ -610,8 +610,9 @@ __device__ __forceinline__ void few_tile(const MxArgs &a, const MxTile &t, const
 // slots 10.0, 11.6 and 17.7 us by 64, 128 and 256 outputs (4-bit 10.6, 10.7, 14.7);
 // of 32 slots (past the first limit) 17.1, 15.9 and 19.5; 16 of 24 (past both)
 // 31.9, 28.6 and 22.5; 60 [1000 x 1440] of 10 22.4, 17.0 and 14.3.  4-bit slots under
-// 24 steps leave four ways out: 8192 outputs, 1440 columns, 16 slots 7.7, 6.2 and
-// 8.0; and two where an expert has several such tiles: 8 experts of 32 slots 16.9, 16.2
+// 24 steps leave four ways out, which are slower below 17 (8 experts x 2048 outputs of 8
+// slots, 16 steps 9.0 by four, 8.2 by two, 10.0 by one; 12 steps 8.3, 7.9 and 9.4) and would
+// be faster from 18 on (8.9, 9.6 and 11.2; 22 steps 9.2, 9.8 and 11.3); and two where an expert has several such tiles: 8 experts of 32 slots 16.9, 16.2
 // and 12.7, but 16 of 16 19.3, 18.1 and 22.3.
 constexpr int kSplitBM = 16;
 
@@ -993,12 +994,21 @@ dim3 tile_grid(MxArgs &a) {
     const uint32_t nblocks = (a.N + BN - 1) / BN;
     const bool groups = a.offs || a.ids;
     uint32_t mtiles = groups ? a.n_slots / BM + min(a.E, a.n_slots) : (a.n_slots + BM - 1) / BM;
-    // an XCD takes as many M-tiles together as an expert has of them on average
+    // An XCD takes as many M-tiles together as an expert has of them on average.  Sets
+    // of 0 (plain order), 1, 2 and 4 with 2048 x 4096: 64 experts of 64 slots 102, 73, 74 and
+    // 72 us (4-bit slots 82, 62, 62 and 61), of 128 153, 128, 126 and 123 (103, 99, 82 and
+    // 82), of 256 251, 244, 237 and 231 (141, 179, 137 and 130).  Under 8 M-tiles sets cannot
+    // fill the XCDs: 4 experts of 64 slots 15, 16, 15 and 25; under 64 larger ones leave some
+    // empty: 8 experts of 64 30, 30, 31 and 32 (17, 17, 17 and 23).
     const uint64_t even = groups ? uint64_t(BM) * a.E : 1;
     a.set = likely_tiles(a, BM) < 8 ? 0 : mtiles < 64 || a.n_slots <= even ? 1 : a.n_slots <= 3 * even ? 2 : 4;
+    // eight blocks in a run where they divide into such: 8 experts [8192 x 4096] of 512 slots
+    // by 8, 16 and 32 219, 224 and 232 us (4-bit 120, 120 and 178), by 1 to 4 as by 8
     a.run = nblocks % 8 == 0 ? 8 : nblocks % 4 == 0 ? 4 : nblocks < 16 ? nblocks : 1;
     // one matrix, fewer bytes of slots than of weights: the weights stay, a
-    // block of outputs on one XCD
+    // block of outputs on one XCD ([8192 x 4096], plain order and sets of 1: 512 slots 32 and
+    // 33 us, 2048 109 and 115, 4-bit 1024 28 and 46; past the limit, with sets of 4, 4096
+    // slots 206 and 208, 8192 410 and 413)
     if (!groups && uint64_t(a.n_slots) * (act_mx(ACT) ? 1 : 4) <= a.N) a.set = 0;
     if (a.set) mtiles = (mtiles + 8 * a.set - 1) / (8 * a.set) * (8 * a.set);
     return dim3{mtiles * nblocks};

@@ -225,8 +225,10 @@ struct TopkArgs {
 // the keys below the last choice the highest has the highest unsigned key -
 // choice (those at or above it wrap to less), so that a round needs a
 // subtraction and half a maximum a logit.  f32 logits need five instructions: the
-// lowest of the experts that hold the maximum is a second reduction.  Top 6 of 256,
-// 65536 tokens in bf16: 15.2 us (2.4 TB/s); one token in f32: 3.8, a launch.
+// lowest of the experts that hold the maximum is a second reduction.  65536 tokens,
+// bf16 and f32: top 4 of 60 6.4 and 7.6 us, 6 of 256 15.4 and 21.3 (2.4 and 3.3 TB/s), 12 of
+// 256 19.9 and 34.9, 8 of 512 26.2 and 44.0; over all experts 4 to 9 more, for their
+// exponentials.  One token in f32: 3.8, a launch.
 template <int DT, int VPT, bool NORM, bool QUADS>
 __global__ __launch_bounds__(256) void topk_kernel(TopkArgs a) {
     constexpr bool WIDE = DT == MX_F32;
@@ -308,7 +310,8 @@ __global__ __launch_bounds__(256) void topk_kernel(TopkArgs a) {
 //   NORM      w_i (dw_i - D) at the chosen, 0 elsewhere
 //   otherwise p_e (dw_e - D), dw_e = 0 where e was not chosen.
 // The chosen's values meet their place in the row through LDS.  Bound by the store of
-// the rows: 65536 tokens of 256, bf16, NORM, 8.5 us (4.3 TB/s).
+// the rows: 65536 tokens of 256, bf16, NORM, 8.5 us (4.3 TB/s); over all experts, which
+// reads the logits too, 15.9 (4.5 TB/s).
 template <int DT, int VPT, bool NORM, bool QUADS>
 __global__ __launch_bounds__(256) void topk_grad_kernel(TopkArgs a) {
     constexpr int PLACES = kRowLanes * VPT;
@@ -373,7 +376,9 @@ __global__ __launch_bounds__(256) void topk_grad_kernel(TopkArgs a) {
 // shares of a group's tokens, then one workgroup a group over the shares.
 // 16 groups of 4096 tokens, 256 experts in f32 (67 MB): sums 18.2 us (3.7 TB/s),
 // join 3.9, gradient 28.6 (4.7 TB/s read and written); one group of 500 tokens, 60
-// experts: 3.6, 3.0 and 3.7, a launch each.
+// experts: 3.6, 3.0 and 3.7, a launch each.  What bounds the sums is not shown: a workgroup
+// has four turns between clearing its LDS and adding up through it.  The join is one
+// workgroup a group: 65536 tokens of 256 in one group take it 18.3, as long as their sums.
 constexpr int kBalanceThreads = 512;
 constexpr int kBalanceRows = kBalanceThreads / kRowLanes;
 

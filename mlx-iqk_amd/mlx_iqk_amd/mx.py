@@ -51,19 +51,23 @@ def pair_limit(num_experts: int) -> int:
     """Token-expert pairs up to which each is computed on its own; beyond, experts are
     named so often that their weights are better read once for all their pairs.
 
-    A token's experts distinct, else uniform, us alone and grouped: [2048 x 4096], 8
-    experts: 12 pairs 8.6, 9.7, 16 pairs 10.3, 9.8; 16 experts: 16 pairs 12.5, 14.7, 24
-    pairs 17.1, 16.5; 128 experts: 48 pairs 31.4, 35.8, 72 pairs 45.2, 40.5; 256 experts:
-    72 pairs 46.9, 54.3, 96 pairs 65.0, 66.0; [1000 x 1440], 60 experts: 42 pairs 8.4,
-    9.2, 66 pairs 11.1, 10.6.
+    A token's experts distinct, else uniform, us alone and grouped, for 16-bit and for
+    4-bit activations, whose pairs are a little cheaper: [2048 x 4096], 8 experts: 12 pairs
+    9.3, 9.9 (8.4, 10.1), 16 pairs 10.2, 9.8 (8.7, 10.1); 16 experts: 16 pairs 12.3, 13.4
+    (11.4, 13.4), 24 pairs 15.9, 15.5 (14.1, 15.5); 128 experts: 48 pairs 31.7, 36.4 (31.8,
+    35.8), 72 pairs 45.0, 40.2 (44.6, 40.2); 256 experts: 72 pairs 47.1, 53.7 (45.1, 53.1),
+    96 pairs 66.3, 65.3 (61.3, 65.9).  Of other sizes: [1000 x 1440], 60 experts: 42 pairs
+    8.4, 9.4 (7.9, 9.9), 66 pairs 11.1, 10.7 (10.5, 11.7); [4096 x 2048], 256 experts: 120
+    pairs 79, 85 (76, 84); [512 x 1024], 64 experts: 66 pairs 5.3, 7.1 (4.7, 8.0).
     """
     return min(num_experts + 6, 48 + num_experts // 6)
 
 
 ROW_LIMIT = 16384
 """Outputs in all up to which the rows of an :class:`MxLinear` are computed on their
-own (2048 outputs: 8 rows 5.6 us against 7.8, 16 rows 8.9 against 8.4; 8192
-outputs: 4 rows 10.1 against 8.5)."""
+own (4096 columns, 16-bit activations and 4-bit ones: 2048 outputs, 8 rows 5.5 us
+against 6.6 and 4.4 against 6.3, 16 rows 8.6 against 7.9 and 6.7 against 7.2; 8192 outputs, 2
+rows 6.7 against 6.4 and 5.9 against 6.5, 4 rows 9.9 against 6.6 and 8.3 against 6.7)."""
 
 
 def _refuse_gradient(x: torch.Tensor) -> None:
