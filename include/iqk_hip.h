@@ -36,7 +36,7 @@
 extern "C" {
 #endif
 
-#define IQK_HIP_ABI_VERSION 7
+#define IQK_HIP_ABI_VERSION 8
 
 #define IQK_MEMBER_IQ2_KS 0
 #define IQK_MEMBER_IQ2_K 1
@@ -372,6 +372,51 @@ int iqk_balance(int dtype, const void *logits, const int32_t *ids, const uint8_t
 int iqk_balance_grad(int dtype, const void *logits, const uint8_t *mask, const int32_t *counts, const int32_t *kept,
                      const float *dloss, int64_t groups, int64_t tokens, int64_t experts, int64_t k, void *dlogits,
                      void *stream);
+
+// -- between the router and the experts ---------------------------------------
+//
+// Token-expert pairs sorted by expert (the reference leaves this to its caller's
+// _gather_sort and the unsorting after it, src/mlx_iqk/nn.py:221-238).  Pair p = t
+// pairs_per_token + j; an id outside [0, num_experts) leaves its pair out, which is
+// sorted behind the last expert.  offsets i32 [num_experts + 1]: the pairs of experts < e,
+// the last all that have an expert.  Per slot: sorted_ids (num_experts where left out) and
+// tokens i32 [n_tokens pairs_per_token]; per pair: slots, its place.  Stable, so the lists are
+// the same on every call.  ids: u32 or (wide_ids) i64.  work: iqk_sort_work words (0: may be
+// NULL).  num_experts <= 1024, pairs_per_token <= 64, fewer than 2^31 pairs.
+int64_t iqk_sort_work(int64_t n_tokens, int64_t pairs_per_token, int64_t num_experts);
+int iqk_sort(const void *ids, int wide_ids, int64_t n_tokens, int64_t pairs_per_token, int64_t num_experts,
+             uint32_t *work, int32_t *offsets, int32_t *sorted_ids, int32_t *tokens, int32_t *slots, void *stream);
+
+// rows[slots[t, j]] = x[t], zeros in slots >= *kept (kept: offsets + num_experts; NULL: none).  x:
+// dtype [n_tokens, cols], rows: [n_tokens pairs_per_token, cols], at any element's address.
+// cols < 2^28.  A slot outside the rows is not written.
+int iqk_dispatch(int dtype, const void *x, const int32_t *slots, const int32_t *kept, int64_t n_tokens,
+                 int64_t pairs_per_token, int64_t cols, void *rows, void *stream);
+
+// out[t] = sum_j weights[t, j] y[slots[t, j]] + add[t], f32 sums in the order of j, one rounding.
+// slots NULL: pair p's row is p; slots >= *kept are skipped; weights NULL: ones (the gradient of
+// iqk_dispatch); add NULL: none.  y: dtype [n_tokens pairs_per_token, cols].
+int iqk_combine(int dtype, const void *y, const int32_t *slots, const int32_t *kept, const float *weights,
+                const void *add, int64_t n_tokens, int64_t pairs_per_token, int64_t cols, void *out, void *stream);
+
+// Its gradients from dout, dtype [n_tokens, cols]: dy[slots[t, j]] = weights[t, j] dout[t] (zeros
+// in slots >= *kept) and dweights[t, j] = dout[t] . y[slots[t, j]] (0 there); either may be NULL,
+// and y where dweights is.
+int iqk_combine_grad(int dtype, const void *dout, const void *y, const int32_t *slots, const int32_t *kept,
+                     const float *weights, int64_t n_tokens, int64_t pairs_per_token, int64_t cols, void *dy,
+                     float *dweights, void *stream);
+
+// -- low-rank adapters ---------------------------------------------------------
+//
+// out[t] = y[t] + scales[a] up[a] (down[a] x[t]) with a = ids[t / rows_per_id]: down dtype (F16
+// or BF16) [num_adapters, rank, in_features], up [num_adapters, out_features, rank], both
+// 16-byte aligned; scales f32.  An id of -1 gives y[t], another outside the bank a row of NaN.
+// f32 sums, one rounding.  out may be y.  ids: i32 or (wide_ids) i64.  work: iqk_adapters_work
+// words.  in_features and rank multiples of 8, rank <= 256, num_adapters <= 1024.
+int64_t iqk_adapters_work(int64_t in_features, int64_t out_features, int64_t rank, int64_t num_adapters, int64_t rows);
+int iqk_adapters(int dtype, int64_t in_features, int64_t out_features, int64_t rank, int64_t num_adapters,
+                 const void *x, int64_t rows, const void *ids, int wide_ids, int64_t rows_per_id, const void *down,
+                 const void *up, const float *scales, uint32_t *work, const void *y, void *out, void *stream);
 
 #ifdef __cplusplus
 }

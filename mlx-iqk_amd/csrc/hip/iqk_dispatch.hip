@@ -1,0 +1,572 @@
+// Token-expert pairs sorted by expert, their rows moved there and back (gfx950).
+//
+// Pair p = (token t, choice j) has the key ids[p], E where that is no expert (the pair
+// is left out), and the slot
+//   slot(p) = #{q: key_q < key_p} + #{q < p: key_q = key_p},
+// a stable counting sort; the left-out pairs' slots come last, so slots are a
+// permutation whose first offsets[E] have an expert.  Rows move by it:
+//   dispatch       rows[slot(t, j)] = x[t], 0 where left out
+//   its gradient   dx[t] = sum_j drows[slot(t, j)]
+//   combine        out[t] = sum_j w[t, j] y[slot(t, j)] (+ add[t])
+//   its gradients  dy[slot(t, j)] = w[t, j] dout[t],  dw[t, j] = dout[t] . y[slot(t, j)]
+// with the left-out pairs skipped in sums.  Sums are f32, in the choices' order; each
+// output is rounded once.  Nothing is added in memory, so results repeat bit for bit.
+//
+// Rows are addressed in 16-byte chunks from their start, at whatever element they start
+// (loads and stores of 16 bytes need no alignment here), the last of them by elements.
+
+#include <type_traits>
+
+#include "iqk_host.h"
+#include "iqk_mx.h"
+
+namespace iqk {
+
+constexpr int64_t kSortMaxExperts = 1024;
+constexpr int64_t kSortMaxK = 64;
+constexpr int kSortWaves = 8, kSortThreads = 64 * kSortWaves;
+constexpr int kSortKeys = int(kSortMaxExperts) + 1;
+// Pairs up to which every workgroup counts all of them itself, in one launch.
+constexpr int64_t kSortOne = 16384;
+constexpr int64_t kSortBlocks = 256;  // workgroups of a sort, at most
+
+struct SortArgs {
+    const uint32_t *ids;
+    uint32_t *hist;  // [blocks][E + 1], or null: every workgroup counts all pairs
+    int32_t *offsets, *sorted_ids, *tokens, *slots;
+    uint32_t P, E, k, share;  // share: pairs of a workgroup, in order
+};
+
+template <bool WIDE>
+__device__ __forceinline__ uint32_t key_of(const uint32_t *ids, uint32_t p, uint32_t E) {
+    return min(expert_id(ids, p, WIDE ? 1u : 0u), E);
+}
+
+// A workgroup's counts of its share of the pairs, by key.
+template <bool WIDE>
+__global__ __launch_bounds__(kSortThreads) void sort_count_kernel(SortArgs a) {
+    __shared__ uint32_t count[kSortKeys];
+    const uint32_t K = a.E + 1;
+    for (uint32_t e = threadIdx.x; e < K; e += kSortThreads) count[e] = 0;
+    __syncthreads();
+    const uint32_t lo = min(a.P, blockIdx.x * a.share), hi = min(a.P, lo + a.share);
+    for (uint32_t p = lo + threadIdx.x; p < hi; p += kSortThreads) atomicAdd(&count[key_of<WIDE>(a.ids, p, a.E)], 1u);
+    __syncthreads();
+    for (uint32_t e = threadIdx.x; e < K; e += kSortThreads) a.hist[size_t(blockIdx.x) * K + e] = count[e];
+}
+
+struct SortShared {
+    uint32_t total[kSortKeys];                // pairs of each key, then those of the keys below
+    uint32_t before[kSortKeys];               // those of the shares before this one
+    uint32_t wave[kSortWaves][kSortKeys];     // those of each wavefront's share, then its next slot
+    uint32_t sums[kSortWaves];
+};
+
+// Exclusive sums of s.total over K keys, in place; a barrier before and after.
+__device__ __forceinline__ void scan_keys(SortShared &s, uint32_t K) {
+    constexpr int PER = (kSortKeys + kSortThreads - 1) / kSortThreads;  // consecutive keys of a thread
+    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, first = threadIdx.x * PER;
+    uint32_t v[PER], sum = 0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+        v[i] = first + i < K ? s.total[first + i] : 0u;
+        sum += v[i];
+    }
+    uint32_t incl = sum;
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+        const uint32_t up = __shfl_up(incl, off, 64);
+        if (lane >= uint32_t(off)) incl += up;
+    }
+    if (lane == 63) s.sums[wave] = incl;
+    __syncthreads();
+    uint32_t at = incl - sum;
+#pragma unroll
+    for (int w = 0; w < kSortWaves; ++w)
+        if (uint32_t(w) < wave) at += s.sums[w];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+        if (first + i < K) s.total[first + i] = at;
+        at += v[i];
+    }
+    __syncthreads();
+}
+
+// A workgroup's share of the pairs to their slots.  Its wavefronts take equal parts of the share
+// in order; a wavefront ranks 64 pairs at a time among those of the same key, which ballots of the
+// key's bits find, and keeps each key's next slot in LDS.
+template <bool WIDE>
+__global__ __launch_bounds__(kSortThreads) void sort_kernel(SortArgs a) {
+    __shared__ SortShared s;
+    const uint32_t K = a.E + 1, lane = threadIdx.x & 63u;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    for (uint32_t e = threadIdx.x; e < K; e += kSortThreads) {
+        s.total[e] = s.before[e] = 0;
+#pragma unroll
+        for (int w = 0; w < kSortWaves; ++w) s.wave[w][e] = 0;
+    }
+    __syncthreads();
+    const uint32_t lo = min(a.P, blockIdx.x * a.share), hi = min(a.P, lo + a.share);
+    const uint32_t part = (a.share / kSortWaves + 63u) & ~63u;
+    const uint32_t from = min(hi, lo + wave * part), to = min(hi, from + part);
+    if (a.hist) {
+        for (uint32_t e = lane; e < K; e += 64) {
+            uint32_t total = 0, before = 0;
+            for (uint32_t b = wave; b < gridDim.x; b += kSortWaves) {
+                const uint32_t n = a.hist[size_t(b) * K + e];
+                total += n;
+                if (b < blockIdx.x) before += n;
+            }
+            atomicAdd(&s.total[e], total);
+            atomicAdd(&s.before[e], before);
+        }
+    } else {
+        for (uint32_t p = threadIdx.x; p < a.P; p += kSortThreads) {
+            const uint32_t e = key_of<WIDE>(a.ids, p, a.E);
+            atomicAdd(&s.total[e], 1u);
+            if (p < lo) atomicAdd(&s.before[e], 1u);
+        }
+    }
+    for (uint32_t p = from + lane; p < to; p += 64) atomicAdd(&s.wave[wave][key_of<WIDE>(a.ids, p, a.E)], 1u);
+    __syncthreads();
+    scan_keys(s, K);
+    for (uint32_t e = threadIdx.x; e < K; e += kSortThreads) {
+        uint32_t at = s.total[e];
+        if (blockIdx.x == 0) a.offsets[e] = int32_t(at);
+        at += s.before[e];
+#pragma unroll
+        for (int w = 0; w < kSortWaves; ++w) {
+            const uint32_t n = s.wave[w][e];
+            s.wave[w][e] = at;
+            at += n;
+        }
+    }
+    __syncthreads();
+    volatile uint32_t *const next = s.wave[wave];
+    const int bits = 32 - __clz(int(a.E));  // of the largest key, E
+    for (uint32_t base = from; base < to; base += 64) {
+        const uint32_t p = base + lane;
+        const bool live = p < to;
+        const uint32_t key = live ? key_of<WIDE>(a.ids, p, a.E) : 0u;
+        uint64_t same = __ballot(live);
+        for (int b = 0; b < bits; ++b) {
+            const bool bit = (key >> b) & 1u;
+            const uint64_t m = __ballot(bit);
+            same &= bit ? m : ~m;
+        }
+        const uint32_t rank = __builtin_amdgcn_mbcnt_hi(uint32_t(same >> 32), __builtin_amdgcn_mbcnt_lo(uint32_t(same), 0));
+        if (live) {
+            const uint32_t slot = next[key] + rank;
+            __builtin_amdgcn_wave_barrier();  // all lanes have read before the last of each key writes
+            if (rank + 1 == uint32_t(__popcll(same))) next[key] = slot + 1;
+            if (slot < a.P) {  // unless another stream changed the ids meanwhile
+                a.slots[p] = int32_t(slot);
+                a.sorted_ids[slot] = int32_t(key);
+                a.tokens[slot] = int32_t(p / a.k);
+            }
+        }
+        __builtin_amdgcn_wave_barrier();
+    }
+}
+
+// --------------------------------------------------------------------- rows ---
+
+// 16 bytes at any element.
+typedef uint32_t chunk_t __attribute__((ext_vector_type(4), aligned(2)));
+typedef uint16_t half16_t __attribute__((aligned(2)));
+
+template <int DT>
+constexpr int kChunk = DT == MX_F32 ? 4 : 8;  // values of a chunk
+
+template <int DT>
+__device__ __forceinline__ void unpack(uint4_t w, float (&v)[kChunk<DT>]) {
+    if constexpr (DT == MX_F32) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t word = w[i];  // a bit cast of the vector's element itself reads element 0
+            v[i] = __builtin_bit_cast(float, word);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if constexpr (DT == MX_F16) {
+                v[2 * i] = half_bits_to_float(w[i] & 0xffffu);
+                v[2 * i + 1] = half_bits_to_float(w[i] >> 16);
+            } else {
+                v[2 * i] = __builtin_bit_cast(float, w[i] << 16);
+                v[2 * i + 1] = __builtin_bit_cast(float, w[i] & 0xffff0000u);
+            }
+        }
+    }
+}
+
+template <int DT>
+__device__ __forceinline__ uint4_t pack(const float (&v)[kChunk<DT>]) {
+    uint4_t w;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if constexpr (DT == MX_F32)
+            w[i] = __builtin_bit_cast(uint32_t, v[i]);
+        else if constexpr (DT == MX_F16)
+            w[i] = float_to_half_bits(v[2 * i]) | float_to_half_bits(v[2 * i + 1]) << 16;
+        else
+            w[i] = bf16_bits(v[2 * i]) | bf16_bits(v[2 * i + 1]) << 16;
+    }
+    return w;
+}
+
+// The first `halves` (1 .. 8) 16-bit halves of a chunk, zeros behind them.
+__device__ __forceinline__ uint4_t load_chunk(const uint8_t *p, uint32_t halves) {
+    if (halves == 8) return *reinterpret_cast<const chunk_t *>(p);
+    uint4_t w = {0, 0, 0, 0};
+#pragma unroll
+    for (uint32_t i = 0; i < 7; ++i)
+        if (i < halves) w[i / 2] |= uint32_t(reinterpret_cast<const half16_t *>(p)[i]) << (16 * (i & 1));
+    return w;
+}
+
+__device__ __forceinline__ void store_chunk(uint8_t *p, uint4_t w, uint32_t halves) {
+    if (halves == 8) {
+        *reinterpret_cast<chunk_t *>(p) = w;
+        return;
+    }
+#pragma unroll
+    for (uint32_t i = 0; i < 7; ++i)
+        if (i < halves) reinterpret_cast<half16_t *>(p)[i] = uint16_t(w[i / 2] >> (16 * (i & 1)));
+}
+
+struct RowArgs {
+    const uint8_t *in;        // a row for each token (dispatch, combine's gradients), or for each slot
+    const uint8_t *y;         // combine's gradients: the slots' rows, or null
+    const uint8_t *add;       // a row for each token, or null
+    const int32_t *slots;     // [T][k], or null: the pairs'
+    const int32_t *kept;      // the slots that have an expert, or null: all
+    const float *weights;     // [T][k], or null: ones
+    uint8_t *out;             // rows of tokens, or of slots, or null
+    float *dweights;          // or null
+    uint32_t T, k, P;
+    uint32_t row, chunks;     // bytes and chunks of a row
+    uint32_t log_width, columns;  // threads of a token (a power of two), and workgroups of a row
+    uint32_t first;           // the launch's first token
+};
+
+// What one thread has of rows: a token and a chunk of them.
+struct Place {
+    uint32_t t, chunk, halves;
+    bool live;
+    __device__ __forceinline__ explicit Place(const RowArgs &a) {
+        const uint32_t width = 1u << a.log_width;
+        t = a.first + (blockIdx.x / a.columns << (8 - a.log_width)) + (threadIdx.x >> a.log_width);
+        chunk = (blockIdx.x % a.columns << a.log_width) + (threadIdx.x & (width - 1u));
+        live = t < a.T && chunk < a.chunks;
+        halves = min(8u, (a.row - 16u * chunk) / 2u);
+    }
+};
+
+__device__ __forceinline__ uint32_t slots_kept(const RowArgs &a) { return a.kept ? min(uint32_t(*a.kept), a.P) : a.P; }
+
+// Each token's row to its slots, zeros to those left out.
+__global__ __launch_bounds__(256) void dispatch_kernel(RowArgs a) {
+    const Place at(a);
+    if (!at.live) return;
+    const uint32_t kept = slots_kept(a);
+    const size_t column = size_t(at.chunk) * 16;
+    const uint4_t w = load_chunk(a.in + size_t(at.t) * a.row + column, at.halves);
+    for (uint32_t j = 0; j < a.k; ++j) {
+        const uint32_t slot = uint32_t(a.slots[size_t(at.t) * a.k + j]);
+        if (slot < a.P) store_chunk(a.out + size_t(slot) * a.row + column, slot < kept ? w : uint4_t{0, 0, 0, 0}, at.halves);
+    }
+}
+
+// A token's rows, weighted and summed.
+template <int DT>
+__global__ __launch_bounds__(256) void combine_kernel(RowArgs a) {
+    constexpr int N = kChunk<DT>, AHEAD = 8;  // rows on their way at once
+    const Place at(a);
+    if (!at.live) return;
+    const uint32_t kept = slots_kept(a);
+    const size_t column = size_t(at.chunk) * 16, pair = size_t(at.t) * a.k;
+    float sum[N] = {};
+    for (uint32_t j0 = 0; j0 < a.k; j0 += AHEAD) {
+        uint4_t w[AHEAD];
+        bool has[AHEAD];
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) {
+            const uint32_t j = min(j0 + i, a.k - 1u);
+            const uint32_t slot = a.slots ? uint32_t(a.slots[pair + j]) : uint32_t(pair) + j;
+            has[i] = j0 + i < a.k && slot < kept;
+            w[i] = uint4_t{0, 0, 0, 0};
+            if (has[i]) w[i] = load_chunk(a.in + size_t(slot) * a.row + column, at.halves);
+        }
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) {
+            if (!has[i]) continue;
+            float v[N];
+            unpack<DT>(w[i], v);
+            const float weight = a.weights ? a.weights[pair + j0 + i] : 1.f;
+#pragma unroll
+            for (int n = 0; n < N; ++n) sum[n] = fmaf(weight, v[n], sum[n]);
+        }
+    }
+    const size_t mine = size_t(at.t) * a.row + column;
+    if (a.add) {
+        float v[N];
+        unpack<DT>(load_chunk(a.add + mine, at.halves), v);
+#pragma unroll
+        for (int n = 0; n < N; ++n) sum[n] += v[n];
+    }
+    store_chunk(a.out + mine, pack<DT>(sum), at.halves);
+}
+
+// Both gradients of a token's sum: WAVES wavefronts a token take its row's chunks in turn.
+template <int DT, int WAVES>
+__global__ __launch_bounds__(256) void combine_grad_kernel(RowArgs a) {
+    constexpr int N = kChunk<DT>, AHEAD = 8;
+    __shared__ float part[4][AHEAD];
+    const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t t = a.first + (WAVES == 1 ? blockIdx.x * 4 + wave : blockIdx.x);
+    if (WAVES == 1 && t >= a.T) return;  // whole wavefronts, and no barrier follows
+    const uint32_t kept = slots_kept(a);
+    const size_t pair = size_t(t) * a.k;
+    for (uint32_t j0 = 0; j0 < a.k; j0 += AHEAD) {
+        uint32_t slot[AHEAD];
+        float weight[AHEAD], dot[AHEAD];
+        bool has[AHEAD];
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) {
+            const uint32_t j = min(j0 + i, a.k - 1u);
+            slot[i] = a.slots ? uint32_t(a.slots[pair + j]) : uint32_t(pair) + j;
+            if (j0 + i >= a.k) slot[i] = a.P;
+            has[i] = slot[i] < kept;
+            weight[i] = has[i] ? a.weights[pair + j] : 0.f;
+            dot[i] = 0.f;
+        }
+        for (uint32_t c = (WAVES == 1 ? 0 : wave * 64) + lane; c < a.chunks; c += WAVES * 64) {
+            const uint32_t halves = min(8u, (a.row - 16u * c) / 2u);
+            const size_t column = size_t(c) * 16;
+            uint4_t w[AHEAD];
+            if (a.dweights) {
+#pragma unroll
+                for (int i = 0; i < AHEAD; ++i) {
+                    w[i] = uint4_t{0, 0, 0, 0};
+                    if (has[i]) w[i] = load_chunk(a.y + size_t(slot[i]) * a.row + column, halves);
+                }
+            }
+            float g[N];
+            unpack<DT>(load_chunk(a.in + size_t(t) * a.row + column, halves), g);
+#pragma unroll
+            for (int i = 0; i < AHEAD; ++i) {
+                if (a.dweights && has[i]) {
+                    float v[N];
+                    unpack<DT>(w[i], v);
+#pragma unroll
+                    for (int n = 0; n < N; ++n) dot[i] = fmaf(g[n], v[n], dot[i]);
+                }
+                if (a.out && slot[i] < a.P) {
+                    float v[N];
+#pragma unroll
+                    for (int n = 0; n < N; ++n) v[n] = weight[i] * g[n];
+                    store_chunk(a.out + size_t(slot[i]) * a.row + column,
+                                has[i] ? pack<DT>(v) : uint4_t{0, 0, 0, 0}, halves);
+                }
+            }
+        }
+        if (!a.dweights) continue;
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) {
+#pragma unroll
+            for (int off = 32; off > 0; off >>= 1) dot[i] += __shfl_xor(dot[i], off, 64);
+        }
+        if constexpr (WAVES == 1) {
+#pragma unroll
+            for (int i = 0; i < AHEAD; ++i)
+                if (lane == uint32_t(i) && j0 + i < a.k) a.dweights[pair + j0 + i] = has[i] ? dot[i] : 0.f;
+        } else {
+            if (lane == 0) {
+#pragma unroll
+                for (int i = 0; i < AHEAD; ++i) part[wave][i] = has[i] ? dot[i] : 0.f;
+            }
+            __syncthreads();
+            if (threadIdx.x < AHEAD && j0 + threadIdx.x < a.k) {
+                float sum = 0.f;
+#pragma unroll
+                for (int w = 0; w < WAVES; ++w) sum += part[w][threadIdx.x];
+                a.dweights[pair + j0 + threadIdx.x] = sum;
+            }
+            __syncthreads();  // before the next choices' parts
+        }
+    }
+}
+
+// --------------------------------------------------------------------- host ---
+
+struct SortPlan {
+    int64_t blocks, share;
+    bool counted;  // a launch before counts the shares
+};
+
+SortPlan sort_plan(int64_t pairs) {
+    const int64_t turns = (pairs + kSortThreads - 1) / kSortThreads;
+    const int64_t per = (turns + kSortBlocks - 1) / kSortBlocks;
+    const int64_t blocks = per ? (turns + per - 1) / per : 1;
+    return {blocks, (per ? per : 1) * kSortThreads, pairs > kSortOne};
+}
+
+bool sort_shape_ok(int64_t tokens, int64_t k, int64_t experts) {
+    return experts > 0 && experts <= kSortMaxExperts && k > 0 && k <= kSortMaxK && tokens >= 0 &&
+           tokens < (int64_t(1) << 31) && tokens * k < (int64_t(1) << 31);
+}
+
+int sort_launch(const void *ids, int wide, int64_t tokens, int64_t k, int64_t experts, uint32_t *work, int32_t *offsets,
+                int32_t *sorted_ids, int32_t *token_of, int32_t *slots, hipStream_t stream) {
+    const SortPlan plan = sort_plan(tokens * k);
+    SortArgs a{};
+    a.ids = static_cast<const uint32_t *>(ids);
+    a.hist = plan.counted ? work : nullptr;
+    a.offsets = offsets;
+    a.sorted_ids = sorted_ids;
+    a.tokens = token_of;
+    a.slots = slots;
+    a.P = uint32_t(tokens * k);
+    a.E = uint32_t(experts);
+    a.k = uint32_t(k);
+    a.share = uint32_t(plan.share);
+    const auto run = [&](auto kernel) {
+        hipLaunchKernelGGL(kernel, dim3{uint32_t(plan.blocks)}, dim3{kSortThreads}, 0, stream, a);
+        return hipGetLastError();
+    };
+    if (plan.counted) {
+        const hipError_t err = wide ? run(sort_count_kernel<true>) : run(sort_count_kernel<false>);
+        if (err != hipSuccess) return record_launch(err);
+    }
+    return record_launch(wide ? run(sort_kernel<true>) : run(sort_kernel<false>));
+}
+
+bool rows_shape_ok(int dtype, int64_t tokens, int64_t k, int64_t cols) {
+    return dtype >= MX_F32 && dtype <= MX_BF16 && k > 0 && k <= kSortMaxK && tokens >= 0 && tokens < (int64_t(1) << 31) &&
+           tokens * k < (int64_t(1) << 31) && cols > 0 && cols < (int64_t(1) << 28);
+}
+
+RowArgs row_args(int dtype, int64_t tokens, int64_t k, int64_t cols) {
+    RowArgs a{};
+    a.T = uint32_t(tokens);
+    a.k = uint32_t(k);
+    a.P = uint32_t(tokens * k);
+    a.row = uint32_t(cols * (dtype == MX_F32 ? 4 : 2));
+    a.chunks = (a.row + 15u) / 16u;
+    while (a.log_width < 8 && (1u << a.log_width) < a.chunks) ++a.log_width;
+    a.columns = (a.chunks + (1u << a.log_width) - 1u) >> a.log_width;
+    return a;
+}
+
+// launch(a, workgroups) for each part of the tokens that a grid of under 2^32 threads holds.
+template <typename F>
+void by_tokens(RowArgs a, int64_t tokens_of_group, int64_t groups_of_tokens, F &&launch) {
+    const int64_t T = a.T, most = (int64_t(1) << 23) / groups_of_tokens * tokens_of_group;
+    for (int64_t first = 0; first < T; first += most) {
+        const int64_t n = T - first < most ? T - first : most;
+        a.first = uint32_t(first);
+        a.T = uint32_t(first + n);
+        launch(a, uint32_t((n + tokens_of_group - 1) / tokens_of_group * groups_of_tokens));
+    }
+}
+
+template <typename F>
+void by_dtype(int dtype, F &&f) {
+    if (dtype == MX_F32)
+        f(std::integral_constant<int, MX_F32>{});
+    else if (dtype == MX_F16)
+        f(std::integral_constant<int, MX_F16>{});
+    else
+        f(std::integral_constant<int, MX_BF16>{});
+}
+
+}  // namespace iqk
+
+extern "C" {
+
+int64_t iqk_sort_work(int64_t n_tokens, int64_t pairs_per_token, int64_t num_experts) {
+    using namespace iqk;
+    if (!sort_shape_ok(n_tokens, pairs_per_token, num_experts)) return -1;
+    const SortPlan plan = sort_plan(n_tokens * pairs_per_token);
+    return plan.counted ? plan.blocks * (num_experts + 1) : 0;
+}
+
+int iqk_sort(const void *ids, int wide_ids, int64_t n_tokens, int64_t pairs_per_token, int64_t num_experts,
+             uint32_t *work, int32_t *offsets, int32_t *sorted_ids, int32_t *tokens, int32_t *slots, void *stream) {
+    using namespace iqk;
+    if (!sort_shape_ok(n_tokens, pairs_per_token, num_experts)) return IQK_ERR_GEOMETRY;
+    if (!offsets || (n_tokens && (!ids || !sorted_ids || !tokens || !slots))) return IQK_ERR_ARGUMENT;
+    if (sort_plan(n_tokens * pairs_per_token).counted && !work) return IQK_ERR_ARGUMENT;
+    return sort_launch(ids, wide_ids, n_tokens, pairs_per_token, num_experts, work, offsets, sorted_ids, tokens, slots,
+                       as_stream(stream));
+}
+
+int iqk_dispatch(int dtype, const void *x, const int32_t *slots, const int32_t *kept, int64_t n_tokens,
+                 int64_t pairs_per_token, int64_t cols, void *rows, void *stream) {
+    using namespace iqk;
+    if (!rows_shape_ok(dtype, n_tokens, pairs_per_token, cols)) return IQK_ERR_GEOMETRY;
+    if (n_tokens == 0) return IQK_OK;
+    if (!x || !slots || !rows) return IQK_ERR_ARGUMENT;
+    RowArgs a = row_args(dtype, n_tokens, pairs_per_token, cols);
+    a.in = static_cast<const uint8_t *>(x);
+    a.slots = slots;
+    a.kept = kept;
+    a.out = static_cast<uint8_t *>(rows);
+    by_tokens(a, 256 >> a.log_width, a.columns, [&](const RowArgs &part, uint32_t blocks) {
+        hipLaunchKernelGGL(dispatch_kernel, dim3{blocks}, dim3{256}, 0, as_stream(stream), part);
+    });
+    return record_launch(hipGetLastError());
+}
+
+int iqk_combine(int dtype, const void *y, const int32_t *slots, const int32_t *kept, const float *weights,
+                const void *add, int64_t n_tokens, int64_t pairs_per_token, int64_t cols, void *out, void *stream) {
+    using namespace iqk;
+    if (!rows_shape_ok(dtype, n_tokens, pairs_per_token, cols)) return IQK_ERR_GEOMETRY;
+    if (n_tokens == 0) return IQK_OK;
+    if (!y || !out) return IQK_ERR_ARGUMENT;
+    RowArgs a = row_args(dtype, n_tokens, pairs_per_token, cols);
+    a.in = static_cast<const uint8_t *>(y);
+    a.add = static_cast<const uint8_t *>(add);
+    a.slots = slots;
+    a.kept = kept;
+    a.weights = weights;
+    a.out = static_cast<uint8_t *>(out);
+    by_dtype(dtype, [&](auto dt) {
+        by_tokens(a, 256 >> a.log_width, a.columns, [&](const RowArgs &part, uint32_t blocks) {
+            hipLaunchKernelGGL((combine_kernel<decltype(dt)::value>), dim3{blocks}, dim3{256}, 0, as_stream(stream), part);
+        });
+    });
+    return record_launch(hipGetLastError());
+}
+
+int iqk_combine_grad(int dtype, const void *dout, const void *y, const int32_t *slots, const int32_t *kept,
+                     const float *weights, int64_t n_tokens, int64_t pairs_per_token, int64_t cols, void *dy,
+                     float *dweights, void *stream) {
+    using namespace iqk;
+    if (!rows_shape_ok(dtype, n_tokens, pairs_per_token, cols)) return IQK_ERR_GEOMETRY;
+    if (n_tokens == 0 || (!dy && !dweights)) return IQK_OK;
+    if (!dout || !weights || (dweights && !y)) return IQK_ERR_ARGUMENT;
+    RowArgs a = row_args(dtype, n_tokens, pairs_per_token, cols);
+    a.in = static_cast<const uint8_t *>(dout);
+    a.y = static_cast<const uint8_t *>(y);
+    a.slots = slots;
+    a.kept = kept;
+    a.weights = weights;
+    a.out = static_cast<uint8_t *>(dy);
+    a.dweights = dweights;
+    by_dtype(dtype, [&](auto dt) {
+        constexpr int DT = decltype(dt)::value;
+        if (a.chunks <= 64)
+            by_tokens(a, 4, 1, [&](const RowArgs &part, uint32_t blocks) {
+                hipLaunchKernelGGL((combine_grad_kernel<DT, 1>), dim3{blocks}, dim3{256}, 0, as_stream(stream), part);
+            });
+        else
+            by_tokens(a, 1, 1, [&](const RowArgs &part, uint32_t blocks) {
+                hipLaunchKernelGGL((combine_grad_kernel<DT, 4>), dim3{blocks}, dim3{256}, 0, as_stream(stream), part);
+            });
+    });
+    return record_launch(hipGetLastError());
+}
+
+}  // extern "C"

@@ -1,4 +1,4 @@
-// The eager calls of the 4-bit modules and of the router on torch tensors: what
+// The eager calls of the 4-bit modules, the router and the adapters on torch tensors: what
 // an operator needs between its argument checks (in Python) and its launches --
 // outputs, workspaces, the stream, and for the router the autograd nodes.  The
 // kernels are libiqk_hip.so's, reached through its C ABI; nothing is computed here.
@@ -63,12 +63,13 @@ void refuse_capture() {
 }
 
 // A gradient that is not differentiable again says so when asked.  It depends on what
-// comes from above and on `saved`, the forward's tensor that the formula is of: the
+// comes from above and on `saved`, the forward's tensor that the formula is of (if any): the
 // node that raises stands between it and them, so that a derivative in either meets it.
 variable_list once(Tensor grad, const variable_list &above, const Tensor &saved) {
-    if (!at::GradMode::is_enabled() || !(saved.requires_grad() || torch::autograd::any_variable_requires_grad(above)))
-        return {grad};
-    variable_list inputs{grad, saved};
+    const bool of_saved = saved.defined() && saved.requires_grad();
+    if (!at::GradMode::is_enabled() || !(of_saved || torch::autograd::any_variable_requires_grad(above))) return {grad};
+    variable_list inputs{grad};
+    if (saved.defined()) inputs.push_back(saved);
     inputs.insert(inputs.end(), above.begin(), above.end());
     auto error = std::make_shared<torch::autograd::DelayedError>(
         "the router's gradients are not differentiable a second time", int64_t(inputs.size()));
@@ -179,6 +180,114 @@ struct Balance : torch::autograd::Function<Balance> {
     }
 };
 
+// ---------------------------------------------------- sort, dispatch, combine ---
+
+struct Sorted {
+    Tensor offsets, ids, tokens, slots;
+};
+
+// ids [..., k], contiguous, i32 or i64
+Sorted sort_pairs(const Tensor &ids, int64_t experts) {
+    const int64_t k = ids.size(-1), pairs = ids.numel(), tokens = pairs / k;
+    Sorted s;
+    s.offsets = empty({experts + 1}, at::kInt, ids);
+    s.ids = empty({pairs}, at::kInt, ids);
+    s.tokens = empty({pairs}, at::kInt, ids);
+    s.slots = empty(ids.sizes(), at::kInt, ids);
+    const int64_t words = iqk_sort_work(tokens, k, experts);
+    check(words < 0 ? IQK_ERR_GEOMETRY : IQK_OK, "iqk_sort_work");
+    const Tensor work = words ? empty({words}, at::kInt, ids) : Tensor();
+    check(iqk_sort(ids.data_ptr(), ids.scalar_type() == at::kLong, tokens, k, experts, ptr<uint32_t>(work),
+                   ptr<int32_t>(s.offsets), ptr<int32_t>(s.ids), ptr<int32_t>(s.tokens), ptr<int32_t>(s.slots),
+                   stream_of(ids)),
+          "iqk_sort");
+    return s;
+}
+
+// The number of slots that have an expert, the last of the offsets.
+const int32_t *kept(const Tensor &offsets) {
+    return offsets.defined() ? ptr<int32_t>(offsets) + offsets.numel() - 1 : nullptr;
+}
+
+Tensor dispatch_forward(const Tensor &x, const Tensor &slots, const Tensor &offsets) {
+    const int64_t k = slots.size(-1), tokens = slots.numel() / k, cols = x.size(-1);
+    Tensor rows = empty({tokens * k, cols}, x.scalar_type(), x);
+    check(iqk_dispatch(type_code(x), x.data_ptr(), ptr<int32_t>(slots), kept(offsets), tokens, k, cols, rows.data_ptr(),
+                       stream_of(x)),
+          "iqk_dispatch");
+    return rows;
+}
+
+// The sum of a token's rows: [..., cols], weights' leading shape (slots' without weights).
+Tensor combine_forward(const Tensor &y, const Tensor &weights, const Tensor &slots, const Tensor &offsets,
+                       const Tensor &add) {
+    const Tensor &pairs = weights.defined() ? weights : slots;
+    auto shape = pairs.sizes().vec();
+    const int64_t k = shape.back(), cols = y.size(-1);
+    shape.back() = cols;
+    Tensor out = empty(shape, y.scalar_type(), y);
+    check(iqk_combine(type_code(y), y.data_ptr(), ptr<int32_t>(slots), kept(offsets), ptr<float>(weights),
+                      ptr<void>(add), pairs.numel() / k, k, cols, out.data_ptr(), stream_of(y)),
+          "iqk_combine");
+    return out;
+}
+
+struct Dispatch : torch::autograd::Function<Dispatch> {
+    static variable_list forward(AutogradContext *ctx, const Tensor &x, const Tensor &slots, const Tensor &offsets) {
+        ctx->set_materialize_grads(false);
+        ctx->save_for_backward({slots, offsets});
+        return {dispatch_forward(x, slots, offsets)};
+    }
+    static variable_list backward(AutogradContext *ctx, variable_list grads) {
+        refuse_capture();
+        if (!grads[0].defined()) return {Tensor(), Tensor(), Tensor()};
+        const auto saved = ctx->get_saved_variables();
+        const Tensor dx = combine_forward(grads[0].detach().contiguous(), Tensor(), saved[0], saved[1], Tensor());
+        auto out = once(dx, grads, Tensor());
+        out.resize(3);
+        return out;
+    }
+};
+
+struct Combine : torch::autograd::Function<Combine> {
+    static variable_list forward(AutogradContext *ctx, const Tensor &y, const Tensor &weights,
+                                 const std::optional<Tensor> &slots, const std::optional<Tensor> &offsets,
+                                 const std::optional<Tensor> &add) {
+        ctx->set_materialize_grads(false);
+        const bool dy = y.requires_grad(), dw = weights.requires_grad();
+        ctx->saved_data["dy"] = dy;
+        ctx->saved_data["dw"] = dw;
+        ctx->saved_data["dadd"] = add && add->requires_grad();
+        ctx->saved_data["shape"] = y.sizes().vec();
+        const Tensor s = slots.value_or(Tensor()), o = offsets.value_or(Tensor());
+        // y for the weights' gradient only, which is the larger by far
+        ctx->save_for_backward({dw ? y : Tensor(), dy || dw ? weights : Tensor(), s, o});
+        return {combine_forward(y, weights, s, o, add.value_or(Tensor()))};
+    }
+    static variable_list backward(AutogradContext *ctx, variable_list grads) {
+        refuse_capture();
+        variable_list out(5);
+        if (!grads[0].defined()) return out;
+        const auto saved = ctx->get_saved_variables();
+        const Tensor &y = saved[0], &weights = saved[1], &slots = saved[2], &offsets = saved[3];
+        const Tensor dout = grads[0].detach().contiguous();
+        Tensor dy, dweights;
+        if (ctx->saved_data["dy"].toBool()) dy = empty(ctx->saved_data["shape"].toIntVector(), dout.scalar_type(), dout);
+        if (ctx->saved_data["dw"].toBool()) dweights = empty(weights.sizes(), at::kFloat, dout);
+        if (dy.defined() || dweights.defined()) {
+            const int64_t k = weights.size(-1);
+            check(iqk_combine_grad(type_code(dout), dout.data_ptr(), ptr<void>(y), ptr<int32_t>(slots), kept(offsets),
+                                   ptr<float>(weights), weights.numel() / k, k, dout.size(-1), ptr<void>(dy),
+                                   ptr<float>(dweights), stream_of(dout)),
+                  "iqk_combine_grad");
+            if (dy.defined()) out[0] = once(dy, grads, weights)[0];
+            if (dweights.defined()) out[1] = once(dweights, grads, y)[0];
+        }
+        if (ctx->saved_data["dadd"].toBool()) out[4] = grads[0];
+        return out;
+    }
+};
+
 // ------------------------------------------------------------ 4-bit modules ---
 
 int64_t mx_scale_stride(int64_t cols) { return (cols + 127) / 128 * 4; }
@@ -275,6 +384,76 @@ PyObject *py_balance(PyObject *, PyObject *const *args, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
+PyObject *tuple(std::initializer_list<Tensor> tensors) {
+    PyObject *const t = PyTuple_New(Py_ssize_t(tensors.size()));
+    Py_ssize_t i = 0;
+    for (const Tensor &x : tensors) PyTuple_SET_ITEM(t, i++, THPVariable_Wrap(x));
+    return t;
+}
+
+// sort(ids, experts) -> (offsets, ids, tokens, slots); ids contiguous, i32 or i64
+PyObject *py_sort(PyObject *, PyObject *const *args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    arguments(n, 2);
+    const Sorted s = sort_pairs(tensor(args[0]), integer(args[1]));
+    return tuple({s.offsets, s.ids, s.tokens, s.slots});
+    END_HANDLE_TH_ERRORS
+}
+
+// dispatch(x, ids, experts) -> (rows, offsets, ids, tokens, slots); x and ids contiguous
+PyObject *py_dispatch(PyObject *, PyObject *const *args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    arguments(n, 3);
+    const Tensor &x = tensor(args[0]);
+    refuse_tangent(x, "x");
+    const Sorted s = sort_pairs(tensor(args[1]), integer(args[2]));
+    const Tensor rows = wants_grad(x) ? Dispatch::apply(x, s.slots, s.offsets)[0] : dispatch_forward(x, s.slots, s.offsets);
+    return tuple({rows, s.offsets, s.ids, s.tokens, s.slots});
+    END_HANDLE_TH_ERRORS
+}
+
+// combine(y, weights, slots | None, offsets | None, add | None) -> out; all contiguous
+PyObject *py_combine(PyObject *, PyObject *const *args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    arguments(n, 5);
+    const Tensor &y = tensor(args[0]), &weights = tensor(args[1]);
+    const Tensor slots = tensor_or_none(args[2]), offsets = tensor_or_none(args[3]), add = tensor_or_none(args[4]);
+    refuse_tangent(y, "y");
+    refuse_tangent(weights, "weights");
+    if (add.defined()) refuse_tangent(add, "add");
+    if (wants_grad(y) || wants_grad(weights) || (add.defined() && wants_grad(add))) {
+        const auto given = [](const Tensor &t) { return t.defined() ? std::optional<Tensor>(t) : std::nullopt; };
+        return THPVariable_Wrap(Combine::apply(y, weights, given(slots), given(offsets), given(add))[0]);
+    }
+    return THPVariable_Wrap(combine_forward(y, weights, slots, offsets, add));
+    END_HANDLE_TH_ERRORS
+}
+
+// adapters(x, ids, rows_per_id, down, up, scales, y, out | None) -> out; all contiguous
+PyObject *py_adapters(PyObject *, PyObject *const *args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    arguments(n, 8);
+    const Tensor &x = tensor(args[0]), &ids = tensor(args[1]), &down = tensor(args[3]), &up = tensor(args[4]),
+                 &scales = tensor(args[5]), &y = tensor(args[6]);
+    refuse_tangent(x, "x");
+    refuse_tangent(y, "y");
+    TORCH_CHECK(down.dim() == 3 && up.dim() == 3 && up.size(0) == down.size(0) && up.size(2) == down.size(1) &&
+                    scales.numel() == down.size(0) && x.size(-1) == down.size(2) && y.size(-1) == up.size(1),
+                "the bank's tensors do not belong together: down ", down.sizes(), ", up ", up.sizes(), ", scales ",
+                scales.sizes());
+    const int64_t adapters = down.size(0), rank = down.size(1), in = down.size(2), out = up.size(1);
+    const int64_t rows = x.numel() / in, words = iqk_adapters_work(in, out, rank, adapters, rows);
+    check(words < 0 ? IQK_ERR_GEOMETRY : IQK_OK, "iqk_adapters_work");
+    const Tensor sum = args[7] == Py_None ? empty(y.sizes(), y.scalar_type(), y) : tensor(args[7]);
+    const Tensor work = empty({words}, at::kInt, x);
+    check(iqk_adapters(type_code(x), in, out, rank, adapters, x.data_ptr(), rows, ids.data_ptr(),
+                       ids.scalar_type() == at::kLong, integer(args[2]), down.data_ptr(), up.data_ptr(),
+                       ptr<float>(scales), ptr<uint32_t>(work), y.data_ptr(), sum.data_ptr(), stream_of(x)),
+          "iqk_adapters");
+    return THPVariable_Wrap(sum);
+    END_HANDLE_TH_ERRORS
+}
+
 // Whether the kernels take t as it is: on a GPU, dense, at a 16-byte boundary, not empty.
 bool ready(const Tensor &t) {
     return t.is_cuda() && t.is_contiguous() && t.dim() && t.numel() &&
@@ -360,7 +539,7 @@ PyObject *binding_hash(PyObject *, PyObject *) { return PyUnicode_FromString(IQK
 
 #define METHOD(name) {#name, (PyCFunction)(void (*)(void))py_##name, METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {
-    METHOD(topk), METHOD(balance), METHOD(mx_quantize), METHOD(mx_dequantize), METHOD(mx_project),
+    METHOD(topk), METHOD(balance), METHOD(sort), METHOD(dispatch), METHOD(combine), METHOD(adapters), METHOD(mx_quantize), METHOD(mx_dequantize), METHOD(mx_project),
     {"source_hash", source_hash, METH_NOARGS, "digest of the kernel sources this binding was built with"},
     {"binding_hash", binding_hash, METH_NOARGS, "digest of this binding's own source and torch's version"},
     {nullptr, nullptr, 0, nullptr},

@@ -9,14 +9,15 @@ Modules, in dependency order:
 - :mod:`mlx_iqk_amd.nn` -- :class:`IqkSwitchLinear`, the drop-in switch module;
 - :mod:`mlx_iqk_amd.mx` -- 4-bit microscaled quantisation, :class:`MxSwitchLinear` and
   :class:`MxLinear`, whose weights are in that format;
-- :mod:`mlx_iqk_amd.router` -- the router's choice of experts and its balance loss,
-  with their gradients;
+- :mod:`mlx_iqk_amd.adapters` -- low-rank adapters of many requests beside a projection;
+- :mod:`mlx_iqk_amd.router` -- the router's choice of experts, its balance loss, and the
+  tokens' rows sorted by expert and combined again, with their gradients;
 - :mod:`mlx_iqk_amd.synth` -- seeded synthetic expert stacks for the routed geometry.
 """
 
 from .format import MEMBERS, bits_per_weight, component_shapes, decode, pack, unpack
 
-__all__ = ["MEMBERS", "IqkSwitchLinear", "MxLinear", "MxSwitchLinear", "MxTensor", "bits_per_weight",
+__all__ = ["MEMBERS", "IqkSwitchLinear", "LowRankAdapters", "MxLinear", "MxSwitchLinear", "MxTensor", "bits_per_weight",
            "component_shapes", "decode", "pack", "unpack"]
 
 
@@ -25,6 +26,9 @@ def __getattr__(name):
     if name == "IqkSwitchLinear":
         from .nn import IqkSwitchLinear
         return IqkSwitchLinear
+    if name == "LowRankAdapters":
+        from .adapters import LowRankAdapters
+        return LowRankAdapters
     if name in ("MxLinear", "MxSwitchLinear", "MxTensor"):
         from . import mx
         return getattr(mx, name)

@@ -13,7 +13,7 @@ from pathlib import Path
 from . import build
 from .build import HIP_LIB, LAUNCH_EXT, TORCH_EXT
 
-ABI_VERSION = 7
+ABI_VERSION = 8
 
 OK, ERR_MEMBER, ERR_GEOMETRY, ERR_ARGUMENT, ERR_LAUNCH = 0, 1, 2, 3, 4
 _CODES = {ERR_MEMBER: "unknown member", ERR_GEOMETRY: "unsized geometry",
@@ -83,6 +83,17 @@ SIGNATURES = {
                             c_void_p, c_void_p, c_void_p, c_void_p]),
     "iqk_balance_grad": (c_int, [c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64,
                                  c_int64, c_void_p, c_void_p]),
+    "iqk_sort_work": (c_int64, [c_int64, c_int64, c_int64]),
+    "iqk_sort": (c_int, [c_void_p, c_int, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+                         c_void_p]),
+    "iqk_dispatch": (c_int, [c_int, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_void_p, c_void_p]),
+    "iqk_combine": (c_int, [c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_void_p,
+                            c_void_p]),
+    "iqk_combine_grad": (c_int, [c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64,
+                                 c_void_p, c_void_p, c_void_p]),
+    "iqk_adapters_work": (c_int64, [c_int64, c_int64, c_int64, c_int64, c_int64]),
+    "iqk_adapters": (c_int, [c_int, c_int64, c_int64, c_int64, c_int64, c_void_p, c_int64, c_void_p, c_int, c_int64,
+                             c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
 }
 
 
@@ -154,7 +165,7 @@ def launcher():
 
 
 def torch_binding():
-    """The torch binding of the 4-bit and router calls (``_iqk_torch``); raises
+    """The torch binding of the 4-bit, router and adapter calls (``_iqk_torch``); raises
     where it is not built, or was built with other sources than the library or than
     its own now, or for another torch."""
     global _TORCH

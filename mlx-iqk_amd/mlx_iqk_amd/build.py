@@ -3,7 +3,7 @@
 * ``libiqk_codec.so`` -- the CPU codec (quantizers and dequantizers), g++.
 * ``libiqk_hip.so``   -- the gfx950 kernels behind the C ABI, hipcc.
 * ``_iqk_launch``     -- the CPython binding of the IQ_K calls, gcc.
-* ``_iqk_torch``      -- the torch binding of the 4-bit and router calls, g++.
+* ``_iqk_torch``      -- the torch binding of the 4-bit, router and adapter calls, g++.
 
 All land in ``mlx_iqk_amd/_lib/`` beside the Python sources, so the built
 files travel with the source tree.  ``python -m mlx_iqk_amd.build`` builds
@@ -47,6 +47,8 @@ HIP_SOURCES = {
     "iqk_mx.hip": (),
     "iqk_mx_gemm.hip": (),
     "iqk_router.hip": (),
+    "iqk_dispatch.hip": (),
+    "iqk_adapters.hip": (),
 }
 OFFLOAD_ARCH = "gfx950"
 

@@ -36,6 +36,7 @@ import math
 import torch
 
 from . import _native
+from .adapters import LowRankAdapters
 from .kernels import ROUTE_MAX_EXPERTS, IqkKernelError, _require_cuda, _stream_ptr
 from .nn import _KERNEL_IDS, IqkRuntimeError, _pairs_per_x_row
 
@@ -393,12 +394,27 @@ class MxLinear(_MxStack):
         """The weights' values ``[out, in]``, rounded once to ``dtype``."""
         return self._dequantized(dtype)[0]
 
-    def forward(self, x) -> torch.Tensor:
+    def forward(self, x, adapters=None, adapter_ids: torch.Tensor | None = None) -> torch.Tensor:
+        """Project ``x``; with ``adapters`` (a :class:`~mlx_iqk_amd.adapters.LowRankAdapters` of
+        this matrix's size, ``x`` in its 16-bit type) each row's own, which ``adapter_ids``
+        names, is added to the rounded product."""
         tiles = self._buffers["tiles"]
-        x = self._activations(x, tiles)
-        lead = x[1].shape[:-1]
+        rows = self._activations(x, tiles)
+        lead = rows[1].shape[:-1]
         n = math.prod(lead)
-        return self._project(x, None, (*lead, self.out_features), n, 1, 1, n > 1 and n * self.out_features > ROW_LIMIT)
+        shape, grouped = (*lead, self.out_features), n > 1 and n * self.out_features > ROW_LIMIT
+        if adapters is None:
+            return self._project(rows, None, shape, n, 1, 1, grouped)
+        if not isinstance(adapters, LowRankAdapters):
+            raise IqkRuntimeError(f"adapters must be LowRankAdapters, got {type(adapters).__name__}")
+        if isinstance(x, MxTensor):
+            raise IqkRuntimeError("adapters take 16-bit activations: add them to the product of quantised ones with "
+                                  "adapters(x, ids, y)")
+        if adapters.out_features != self.out_features or adapters.in_features != self.in_features:
+            raise IqkRuntimeError(f"the adapters are for [{adapters.out_features}, {adapters.in_features}], the weights "
+                                  f"are [{self.out_features}, {self.in_features}]")
+        y = self._project(rows, None, shape, n, 1, 1, grouped)
+        return adapters._add(x, adapter_ids, y, y)
 
     def extra_repr(self) -> str:
         return f"{self.out_features}, {self.in_features}"
