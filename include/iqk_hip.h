@@ -410,7 +410,7 @@ int iqk_combine_grad(int dtype, const void *dout, const void *y, const int32_t *
 //
 // out[t] = y[t] + scales[a] up[a] (down[a] x[t]) with a = ids[t / rows_per_id]: down dtype (F16
 // or BF16) [num_adapters, rank, in_features], up [num_adapters, out_features, rank], both
-// 16-byte aligned; scales f32.  An id of -1 gives y[t], another outside the bank a row of NaN.
+// 16-byte aligned, as work is; scales f32.  An id of -1 gives y[t], another outside the bank a row of NaN.
 // f32 sums, one rounding.  out may be y.  ids: i32 or (wide_ids) i64.  work: iqk_adapters_work
 // words.  in_features and rank multiples of 8, rank <= 256, num_adapters <= 1024.
 int64_t iqk_adapters_work(int64_t in_features, int64_t out_features, int64_t rank, int64_t num_adapters, int64_t rows);

@@ -8,10 +8,11 @@
 
 #include "iqk_host.h"
 #include "iqk_mx.h"
+#include "iqk_sort.h"
 
 namespace iqk {
 
-constexpr int64_t kAdaptersMax = 1024;
+constexpr int64_t kAdaptersMax = kSortMaxExperts;
 constexpr int64_t kRankMax = 256;
 
 typedef uint32_t chunk_t __attribute__((ext_vector_type(4), aligned(2)));
@@ -25,6 +26,13 @@ struct AdapterArgs {
     const uint16_t *y;
     uint16_t *out;
     uint32_t T, in, N, rank, adapters, wide, per_id;
+    // grouped form
+    const uint32_t *offs;     // first slots of each adapter, then of the rows without one
+    const uint32_t *rows;     // [T] each slot's row
+    uint4_t *tiles;           // adapter, first slot, slots
+    uint4_t *pieces;          // A x of a tile's slots, split, as operand B of the second product
+    float *powers;            // [tile][slots] what the pieces are multiplied with
+    uint32_t chunks;          // operands B of a slot: of 32 ranks, a power of two of them
 };
 
 // The adapter of row t: the bank's size for none, more for one that does not exist.
@@ -101,12 +109,381 @@ __global__ __launch_bounds__(256) void adapter_up_kernel(AdapterArgs a) {
     a.out[at] = uint16_t(BF ? bf16_bits(sum) : float_to_half_bits(sum));
 }
 
+// ------------------------------------------------------------- many rows ---
+//
+// Rows sorted by adapter, in tiles of SLOTS = 16 CT slots of one adapter; both products on the
+// 16x16x32 MFMAs, operand A the adapter's (16 ranks, 16 outputs), operand B the slots'.  The
+// first kernel leaves A x split into 16-bit pieces that give f32 back: a bf16 product takes three
+// pieces of eight bits (truncated, so that their sum is exact), an f16 product two of eleven
+// bits over a power of two of the slot's largest, which is multiplied back in f32.
+
+template <bool BF>
+constexpr int kPieces = BF ? 3 : 2;
+
+template <bool BF>
+__device__ __forceinline__ float4_t mfma(uint4_t a, uint4_t b, float4_t c) {
+    if constexpr (BF)
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b),
+                                                       c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8_t, a), __builtin_bit_cast(half8_t, b), c,
+                                                      0, 0, 0);
+}
+
+struct Tile {
+    uint32_t adapter, first, slots;  // slots 0: none
+};
+
+// Tile t of the list in which each adapter's slots, and the rows without one (adapter: the
+// bank's size), take whole tiles in order.  All threads of a workgroup of THREADS call it.
+template <int SLOTS, int THREADS>
+__device__ __forceinline__ Tile find_tile(const AdapterArgs &a, uint32_t t, uint32_t (&sums)[THREADS / 64], uint32_t (&found)[3]) {
+    constexpr int PER = (int(kAdaptersMax) + THREADS) / THREADS;  // consecutive groups of a thread
+    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, g0 = threadIdx.x * PER;
+    uint32_t first[PER + 1], mine = 0;
+#pragma unroll
+    for (int i = 0; i <= PER; ++i) first[i] = g0 + i <= a.adapters ? a.offs[g0 + i] : a.T;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) mine += (first[i + 1] - first[i] + SLOTS - 1) / SLOTS;
+    uint32_t incl = mine;
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+        const uint32_t up = __shfl_up(incl, off, 64);
+        if (lane >= uint32_t(off)) incl += up;
+    }
+    if (lane == 63) sums[wave] = incl;
+    if (threadIdx.x == 0) found[2] = 0;
+    __syncthreads();
+    uint32_t at = incl - mine;
+#pragma unroll
+    for (int w = 0; w < THREADS / 64; ++w)
+        if (uint32_t(w) < wave) at += sums[w];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+        const uint32_t n = first[i + 1] - first[i], tiles = (n + SLOTS - 1) / SLOTS;
+        if (t >= at && t < at + tiles) {
+            const uint32_t begin = (t - at) * SLOTS;
+            found[0] = g0 + i;
+            found[1] = first[i] + begin;
+            found[2] = min(n - begin, uint32_t(SLOTS));
+        }
+        at += tiles;
+    }
+    __syncthreads();
+    return {found[0], found[1], found[2]};
+}
+
+// A x of a tile: WAVES wavefronts take 64 columns in turn, and their sums meet in LDS.
+template <bool BF, int RT, int CT, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void adapter_down_tiles_kernel(AdapterArgs a) {
+    constexpr int SLOTS = 16 * CT, RANKS = 16 * RT, THREADS = 64 * WAVES, KC = (RT + 1) / 2;
+    __shared__ float part[WAVES][SLOTS][RANKS + 4];
+    __shared__ uint32_t sums[WAVES], found[3];
+    const Tile tile = find_tile<SLOTS, THREADS>(a, blockIdx.x, sums, found);
+    if (threadIdx.x == 0) a.tiles[blockIdx.x] = uint4_t{tile.adapter, tile.first, tile.slots, 0};
+    if (tile.slots == 0 || tile.adapter >= a.adapters) return;  // uniform
+    const uint32_t lane = threadIdx.x & 63u, g = lane >> 4, m = lane & 15u;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint16_t *w[RT], *x[CT];
+#pragma unroll
+    for (int r = 0; r < RT; ++r)  // ranks past the last: it again, its sums not used
+        w[r] = a.down + (size_t(tile.adapter) * a.rank + min(16u * r + m, a.rank - 1u)) * a.in;
+#pragma unroll
+    for (int c = 0; c < CT; ++c) x[c] = a.x + size_t(a.rows[tile.first + min(16u * c + m, tile.slots - 1u)]) * a.in;
+    float4_t acc[RT][CT];
+#pragma unroll
+    for (int r = 0; r < RT; ++r)
+#pragma unroll
+        for (int c = 0; c < CT; ++c) acc[r][c] = float4_t{0, 0, 0, 0};
+    for (uint32_t k0 = 64 * wave; k0 < a.in; k0 += 64 * WAVES) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const uint32_t k = k0 + 32 * h + 8 * g;
+            const bool in = k < a.in;
+            const uint32_t at = in ? k : 0u;
+            uint4_t xv[CT], wv[RT];
+#pragma unroll
+            for (int c = 0; c < CT; ++c) xv[c] = *reinterpret_cast<const chunk_t *>(x[c] + at);
+#pragma unroll
+            for (int r = 0; r < RT; ++r) wv[r] = load_u4(w[r] + at);
+            if (!in) {  // past the row: zeros on both sides
+#pragma unroll
+                for (int c = 0; c < CT; ++c) xv[c] = uint4_t{0, 0, 0, 0};
+#pragma unroll
+                for (int r = 0; r < RT; ++r) wv[r] = uint4_t{0, 0, 0, 0};
+            }
+#pragma unroll
+            for (int r = 0; r < RT; ++r)
+#pragma unroll
+                for (int c = 0; c < CT; ++c) acc[r][c] = mfma<BF>(wv[r], xv[c], acc[r][c]);
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < RT; ++r)
+#pragma unroll
+        for (int c = 0; c < CT; ++c) *reinterpret_cast<float4_t *>(&part[wave][16 * c + m][16 * r + 4 * g]) = acc[r][c];
+    __syncthreads();
+    const float scale = a.scales[tile.adapter];
+    constexpr int UNITS = 4 * KC;  // eights of a slot's ranks, rounded up to whole operands
+    for (uint32_t u = threadIdx.x; u < SLOTS * UNITS; u += THREADS) {
+        const uint32_t slot = u / UNITS, unit = u % UNITS, r0 = 8 * unit;
+        float v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = 0.f;
+        if (r0 < a.rank) {  // whole eights
+#pragma unroll
+            for (int k = 0; k < WAVES; ++k)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[i] += part[k][slot][r0 + i];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] *= scale;
+        }
+        // operand B of chunk kc: lane 16 g + n has slot n's ranks 32 kc + 8 g ..
+        const size_t at = ((size_t(blockIdx.x) * CT + slot / 16) * KC + unit / 4) * kPieces<BF> * 64 + 16 * (unit & 3u) +
+                          (slot & 15u);
+        if constexpr (BF) {
+#pragma unroll
+            for (int p = 0; p < 3; ++p) {
+                uint4_t out;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const uint32_t bits = __builtin_bit_cast(uint32_t, v[i]);
+                    const bool finite = (bits & 0x7f800000u) != 0x7f800000u;
+                    uint32_t top = bits >> 16;
+                    if (!finite && (bits & 0x7fffffu)) top |= 0x40u;  // a NaN stays one
+                    v[i] = finite ? v[i] - __builtin_bit_cast(float, bits & 0xffff0000u) : 0.f;
+                    out[i / 2] = i & 1 ? out[i / 2] | top << 16 : top;
+                }
+                a.pieces[at + 64 * p] = out;
+            }
+        } else {
+            float most = 0.f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) most = fmaxf(most, fabsf(v[i]));
+#pragma unroll
+            for (int off = 1; off < UNITS; off <<= 1) most = fmaxf(most, __shfl_xor(most, off, 64));
+            // the largest to 2^14 .. 2^15; with an infinity (or nothing) as it is
+            const int e = most > 0.f && most < __builtin_inff() ? 14 - ilogbf(most) : 0;
+            uint4_t hi, lo;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float t = ldexpf(v[i], e);
+                const uint32_t top = float_to_half_bits(t);
+                const float rest = fabsf(t) < __builtin_inff() ? t - half_bits_to_float(top) : 0.f;
+                const uint32_t low = float_to_half_bits(rest);
+                hi[i / 2] = i & 1 ? hi[i / 2] | top << 16 : top;
+                lo[i / 2] = i & 1 ? lo[i / 2] | low << 16 : low;
+            }
+            a.pieces[at] = hi;
+            a.pieces[at + 64] = lo;
+            if (unit == 0) a.powers[size_t(blockIdx.x) * SLOTS + slot] = ldexpf(1.f, -e);
+        }
+    }
+}
+
+// A tile's outputs: a wavefront takes 64 of them for all slots, lane 16 g + n sixteen
+// consecutive ones (16 g ..) of slot n, so that y is read and written 32 bytes a lane.
+template <bool BF, int CT>
+__global__ __launch_bounds__(256) void adapter_up_tiles_kernel(AdapterArgs a) {
+    constexpr int SLOTS = 16 * CT, P = kPieces<BF>;
+    const uint32_t columns = (a.N + 255) / 256, t = blockIdx.x / columns;
+    const uint32_t lane = threadIdx.x & 63u, g = lane >> 4, m = lane & 15u;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t n0 = blockIdx.x % columns * 256 + 64 * wave;
+    const uint4_t tile = a.tiles[t];
+    const uint32_t adapter = tile.x, first = tile.y, slots = tile.z;
+    if (slots == 0 || n0 >= a.N) return;
+    const uint32_t mine = n0 + 16 * g;  // the lane's first output
+    const uint32_t have = mine < a.N ? min(a.N - mine, 16u) : 0u;
+    if (adapter >= a.adapters) {  // rows without an adapter
+#pragma unroll
+        for (int c = 0; c < CT; ++c) {
+            const uint32_t slot = 16 * c + m;
+            if (slot >= slots) continue;
+            const uint32_t row = a.rows[first + slot];
+            const size_t at = size_t(row) * a.N + mine;
+            const bool bare = adapter_of(a, row) == a.adapters;
+            if (bare && a.out == a.y) continue;
+            for (uint32_t i = 0; i < have; ++i) a.out[at + i] = bare ? a.y[at + i] : BF ? uint16_t(0x7fc0) : kHalfNaN;
+        }
+        return;
+    }
+    // operand A's row m of tile j is output 16 (m / 4) + 4 j + m % 4
+    const uint16_t *w[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+        w[j] = a.up + (size_t(adapter) * a.N + min(n0 + 16 * (m >> 2) + 4 * j + (m & 3u), a.N - 1u)) * a.rank;
+    const uint4_t *const b = a.pieces + size_t(t) * CT * a.chunks * P * 64 + lane;
+    size_t at[CT];
+    uint4_t y[CT][2];
+#pragma unroll
+    for (int c = 0; c < CT; ++c) {
+        at[c] = size_t(a.rows[first + min(16u * c + m, slots - 1u)]) * a.N + mine;
+        y[c][0] = y[c][1] = uint4_t{0, 0, 0, 0};
+        if (have == 16) {
+            y[c][0] = *reinterpret_cast<const chunk_t *>(a.y + at[c]);
+            y[c][1] = *reinterpret_cast<const chunk_t *>(a.y + at[c] + 8);
+        }
+    }
+    float4_t acc[4][CT];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int c = 0; c < CT; ++c) acc[j][c] = float4_t{0, 0, 0, 0};
+    for (uint32_t kc = 0; 32 * kc < a.rank; ++kc) {
+        const uint32_t k = 32 * kc + 8 * g;
+        uint4_t wv[4], bv[CT][P];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            wv[j] = uint4_t{0, 0, 0, 0};
+            if (k < a.rank) wv[j] = load_u4(w[j] + k);
+        }
+#pragma unroll
+        for (int c = 0; c < CT; ++c)
+#pragma unroll
+            for (int p = 0; p < P; ++p) bv[c][p] = b[((size_t(c) * a.chunks + kc) * P + p) * 64];
+#pragma unroll
+        for (int p = P - 1; p >= 0; --p)  // the small pieces first
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+                for (int c = 0; c < CT; ++c) acc[j][c] = mfma<BF>(wv[j], bv[c][p], acc[j][c]);
+    }
+#pragma unroll
+    for (int c = 0; c < CT; ++c) {
+        if (16 * c + m >= slots) continue;
+        const float power = BF ? 1.f : a.powers[size_t(t) * SLOTS + 16 * c + m];
+        float v[16];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[4 * j + i] = BF ? acc[j][c][i] : acc[j][c][i] * power;
+        if (have == 16) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                uint4_t out;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const uint32_t word = y[c][h][i];
+                    const float2v_t old = floats<BF>(word);
+                    const float lo = old.x + v[8 * h + 2 * i], hi = old.y + v[8 * h + 2 * i + 1];
+                    out[i] = BF ? bf16_bits(lo) | bf16_bits(hi) << 16 : float_to_half_bits(lo) | float_to_half_bits(hi) << 16;
+                }
+                *reinterpret_cast<chunk_t *>(a.out + at[c] + 8 * h) = out;
+            }
+        } else {
+#pragma unroll
+            for (uint32_t i = 0; i < 16; ++i) {
+                if (i >= have) continue;
+                const float sum = float_of16<BF>(a.y[at[c] + i]) + v[i];
+                a.out[at[c] + i] = uint16_t(BF ? bf16_bits(sum) : float_to_half_bits(sum));
+            }
+        }
+    }
+}
+
+namespace {
+
 bool adapters_shape_ok(int64_t in, int64_t out, int64_t rank, int64_t adapters, int64_t rows) {
     constexpr int64_t kLim = int64_t(1) << 31;
     return in > 0 && in < kLim && in % 8 == 0 && out > 0 && out < kLim && rank > 0 && rank <= kRankMax && rank % 8 == 0 &&
            adapters > 0 && adapters <= kAdaptersMax && rows >= 0 && rows < kLim;
 }
 
+constexpr int64_t kRowsAlone = 64;  // rows up to which each is computed on its own
+
+// The grouped form's workspace, in words: where each part begins.
+struct GroupPlan {
+    int64_t slots, tiles, chunks, hist, offs, rows, desc, pieces, powers, words;
+};
+
+GroupPlan group_plan(int64_t rank, int64_t adapters, int64_t rows) {
+    GroupPlan p{};
+    p.slots = rank > 128 ? 16 : 32;
+    // every adapter and the rows without one may end in a part of a tile
+    const int64_t most = rows / p.slots + adapters + 1;
+    p.tiles = most < rows ? most : rows;
+    const SortPlan sort = sort_plan(rows);
+    for (p.chunks = 1; 32 * p.chunks < rank;) p.chunks *= 2;
+    const auto take = [&](int64_t words) {
+        const int64_t at = p.words;
+        p.words += (words + 3) / 4 * 4;  // 16-byte steps
+        return at;
+    };
+    p.hist = take(sort.counted ? sort.blocks * (adapters + 1) : 0);
+    p.offs = take(adapters + 1);
+    p.rows = take(rows);
+    p.desc = take(4 * p.tiles);
+    p.pieces = take(p.tiles * (p.slots / 16) * p.chunks * 3 * 64 * 4);
+    p.powers = take(p.tiles * p.slots);
+    return p;
+}
+
+template <typename F>
+void by_ranks(int64_t rank, F &&f) {
+    const auto with = [&](auto rt, auto ct, auto waves) { f(rt, ct, waves); };
+    using std::integral_constant;
+    if (rank <= 16)
+        with(integral_constant<int, 1>{}, integral_constant<int, 2>{}, integral_constant<int, 8>{});
+    else if (rank <= 32)
+        with(integral_constant<int, 2>{}, integral_constant<int, 2>{}, integral_constant<int, 8>{});
+    else if (rank <= 64)
+        with(integral_constant<int, 4>{}, integral_constant<int, 2>{}, integral_constant<int, 4>{});
+    else if (rank <= 128)
+        with(integral_constant<int, 8>{}, integral_constant<int, 2>{}, integral_constant<int, 2>{});
+    else
+        with(integral_constant<int, 16>{}, integral_constant<int, 1>{}, integral_constant<int, 2>{});
+}
+
+int rows_alone(const AdapterArgs &a, bool bf, hipStream_t stream) {
+    const int64_t downs = int64_t(a.T) * ((a.rank + 3) / 4), ups = int64_t(a.T) * ((int64_t(a.N) + 255) / 256);
+    if (!grid_ok(downs, 256) || !grid_ok(ups, 256)) return IQK_ERR_GEOMETRY;
+    const auto run = [&](auto kernel, int64_t blocks) {
+        hipLaunchKernelGGL(kernel, dim3{uint32_t(blocks)}, dim3{256}, 0, stream, a);
+        return hipGetLastError();
+    };
+    if (const hipError_t err = bf ? run(adapter_down_kernel<true>, downs) : run(adapter_down_kernel<false>, downs);
+        err != hipSuccess)
+        return record_launch(err);
+    return record_launch(bf ? run(adapter_up_kernel<true>, ups) : run(adapter_up_kernel<false>, ups));
+}
+
+int rows_grouped(AdapterArgs a, bool bf, uint32_t *work, hipStream_t stream) {
+    const GroupPlan p = group_plan(a.rank, a.adapters, a.T);
+    const int64_t ups = p.tiles * ((int64_t(a.N) + 255) / 256);
+    if (!grid_ok(ups, 256) || !grid_ok(p.tiles, 512)) return IQK_ERR_GEOMETRY;
+    SortCall c{};
+    c.ids = a.ids;
+    c.wide = a.wide;
+    c.pairs = a.T;
+    c.experts = a.adapters;
+    c.per_token = 1;
+    c.per_id = a.per_id;
+    c.work = work + p.hist;
+    c.offsets = reinterpret_cast<int32_t *>(work + p.offs);
+    c.tokens = reinterpret_cast<int32_t *>(work + p.rows);
+    if (const int rc = sort_launch(c, stream); rc != IQK_OK) return rc;
+    a.offs = work + p.offs;
+    a.rows = work + p.rows;
+    a.tiles = reinterpret_cast<uint4_t *>(work + p.desc);
+    a.pieces = reinterpret_cast<uint4_t *>(work + p.pieces);
+    a.powers = reinterpret_cast<float *>(work + p.powers);
+    a.chunks = uint32_t(p.chunks);
+    by_ranks(a.rank, [&](auto rt, auto ct, auto waves) {
+        constexpr int RT = decltype(rt)::value, CT = decltype(ct)::value, WAVES = decltype(waves)::value;
+        const auto run = [&](auto down, auto up) {
+            hipLaunchKernelGGL(down, dim3{uint32_t(p.tiles)}, dim3{64 * WAVES}, 0, stream, a);
+            hipLaunchKernelGGL(up, dim3{uint32_t(ups)}, dim3{256}, 0, stream, a);
+        };
+        if (bf)
+            run(adapter_down_tiles_kernel<true, RT, CT, WAVES>, adapter_up_tiles_kernel<true, CT>);
+        else
+            run(adapter_down_tiles_kernel<false, RT, CT, WAVES>, adapter_up_tiles_kernel<false, CT>);
+    });
+    return record_launch(hipGetLastError());
+}
+
+}  // namespace
 }  // namespace iqk
 
 extern "C" {
@@ -114,7 +491,7 @@ extern "C" {
 int64_t iqk_adapters_work(int64_t in_features, int64_t out_features, int64_t rank, int64_t num_adapters, int64_t rows) {
     using namespace iqk;
     if (!adapters_shape_ok(in_features, out_features, rank, num_adapters, rows)) return -1;
-    return rows * rank;
+    return rows <= kRowsAlone ? rows * rank : group_plan(rank, num_adapters, rows).words;
 }
 
 int iqk_adapters(int dtype, int64_t in_features, int64_t out_features, int64_t rank, int64_t num_adapters,
@@ -127,7 +504,8 @@ int iqk_adapters(int dtype, int64_t in_features, int64_t out_features, int64_t r
     if (!x || !ids || rows_per_id <= 0 || rows_per_id >= (int64_t(1) << 31) || !down || !up || !scales || !work || !y ||
         !out)
         return IQK_ERR_ARGUMENT;
-    if ((reinterpret_cast<uintptr_t>(down) | reinterpret_cast<uintptr_t>(up)) & 15u) return IQK_ERR_ARGUMENT;
+    if ((reinterpret_cast<uintptr_t>(down) | reinterpret_cast<uintptr_t>(up) | reinterpret_cast<uintptr_t>(work)) & 15u)
+        return IQK_ERR_ARGUMENT;
     AdapterArgs a{};
     a.x = static_cast<const uint16_t *>(x);
     a.ids = static_cast<const uint32_t *>(ids);
@@ -144,17 +522,8 @@ int iqk_adapters(int dtype, int64_t in_features, int64_t out_features, int64_t r
     a.adapters = uint32_t(num_adapters);
     a.wide = wide_ids != 0;
     a.per_id = uint32_t(rows_per_id);
-    const int64_t downs = rows * ((rank + 3) / 4), ups = rows * ((out_features + 255) / 256);
-    if (!grid_ok(downs, 256) || !grid_ok(ups, 256)) return IQK_ERR_GEOMETRY;
-    const auto run = [&](auto kernel, int64_t blocks) {
-        hipLaunchKernelGGL(kernel, dim3{uint32_t(blocks)}, dim3{256}, 0, as_stream(stream), a);
-        return hipGetLastError();
-    };
     const bool bf = dtype == MX_BF16;
-    if (const hipError_t err = bf ? run(adapter_down_kernel<true>, downs) : run(adapter_down_kernel<false>, downs);
-        err != hipSuccess)
-        return record_launch(err);
-    return record_launch(bf ? run(adapter_up_kernel<true>, ups) : run(adapter_up_kernel<false>, ups));
+    return rows <= kRowsAlone ? rows_alone(a, bf, as_stream(stream)) : rows_grouped(a, bf, work, as_stream(stream));
 }
 
 }  // extern "C"

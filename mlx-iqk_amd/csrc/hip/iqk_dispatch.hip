@@ -19,10 +19,10 @@
 
 #include "iqk_host.h"
 #include "iqk_mx.h"
+#include "iqk_sort.h"
 
 namespace iqk {
 
-constexpr int64_t kSortMaxExperts = 1024;
 constexpr int64_t kSortMaxK = 64;
 constexpr int kSortWaves = 8, kSortThreads = 64 * kSortWaves;
 constexpr int kSortKeys = int(kSortMaxExperts) + 1;
@@ -33,13 +33,14 @@ constexpr int64_t kSortBlocks = 256;  // workgroups of a sort, at most
 struct SortArgs {
     const uint32_t *ids;
     uint32_t *hist;  // [blocks][E + 1], or null: every workgroup counts all pairs
-    int32_t *offsets, *sorted_ids, *tokens, *slots;
+    int32_t *offsets, *sorted_ids, *tokens, *slots;  // sorted_ids and slots may be null
     uint32_t P, E, k, share;  // share: pairs of a workgroup, in order
+    uint32_t per_id;          // pairs of an id
 };
 
 template <bool WIDE>
-__device__ __forceinline__ uint32_t key_of(const uint32_t *ids, uint32_t p, uint32_t E) {
-    return min(expert_id(ids, p, WIDE ? 1u : 0u), E);
+__device__ __forceinline__ uint32_t key_of(const SortArgs &a, uint32_t p) {
+    return min(expert_id(a.ids, a.per_id == 1 ? p : p / a.per_id, WIDE ? 1u : 0u), a.E);
 }
 
 // A workgroup's counts of its share of the pairs, by key.
@@ -50,7 +51,7 @@ __global__ __launch_bounds__(kSortThreads) void sort_count_kernel(SortArgs a) {
     for (uint32_t e = threadIdx.x; e < K; e += kSortThreads) count[e] = 0;
     __syncthreads();
     const uint32_t lo = min(a.P, blockIdx.x * a.share), hi = min(a.P, lo + a.share);
-    for (uint32_t p = lo + threadIdx.x; p < hi; p += kSortThreads) atomicAdd(&count[key_of<WIDE>(a.ids, p, a.E)], 1u);
+    for (uint32_t p = lo + threadIdx.x; p < hi; p += kSortThreads) atomicAdd(&count[key_of<WIDE>(a, p)], 1u);
     __syncthreads();
     for (uint32_t e = threadIdx.x; e < K; e += kSortThreads) a.hist[size_t(blockIdx.x) * K + e] = count[e];
 }
@@ -122,12 +123,12 @@ __global__ __launch_bounds__(kSortThreads) void sort_kernel(SortArgs a) {
         }
     } else {
         for (uint32_t p = threadIdx.x; p < a.P; p += kSortThreads) {
-            const uint32_t e = key_of<WIDE>(a.ids, p, a.E);
+            const uint32_t e = key_of<WIDE>(a, p);
             atomicAdd(&s.total[e], 1u);
             if (p < lo) atomicAdd(&s.before[e], 1u);
         }
     }
-    for (uint32_t p = from + lane; p < to; p += 64) atomicAdd(&s.wave[wave][key_of<WIDE>(a.ids, p, a.E)], 1u);
+    for (uint32_t p = from + lane; p < to; p += 64) atomicAdd(&s.wave[wave][key_of<WIDE>(a, p)], 1u);
     __syncthreads();
     scan_keys(s, K);
     for (uint32_t e = threadIdx.x; e < K; e += kSortThreads) {
@@ -147,7 +148,7 @@ __global__ __launch_bounds__(kSortThreads) void sort_kernel(SortArgs a) {
     for (uint32_t base = from; base < to; base += 64) {
         const uint32_t p = base + lane;
         const bool live = p < to;
-        const uint32_t key = live ? key_of<WIDE>(a.ids, p, a.E) : 0u;
+        const uint32_t key = live ? key_of<WIDE>(a, p) : 0u;
         uint64_t same = __ballot(live);
         for (int b = 0; b < bits; ++b) {
             const bool bit = (key >> b) & 1u;
@@ -160,8 +161,8 @@ __global__ __launch_bounds__(kSortThreads) void sort_kernel(SortArgs a) {
             __builtin_amdgcn_wave_barrier();  // all lanes have read before the last of each key writes
             if (rank + 1 == uint32_t(__popcll(same))) next[key] = slot + 1;
             if (slot < a.P) {  // unless another stream changed the ids meanwhile
-                a.slots[p] = int32_t(slot);
-                a.sorted_ids[slot] = int32_t(key);
+                if (a.slots) a.slots[p] = int32_t(slot);
+                if (a.sorted_ids) a.sorted_ids[slot] = int32_t(key);
                 a.tokens[slot] = int32_t(p / a.k);
             }
         }
@@ -400,11 +401,6 @@ __global__ __launch_bounds__(256) void combine_grad_kernel(RowArgs a) {
 
 // --------------------------------------------------------------------- host ---
 
-struct SortPlan {
-    int64_t blocks, share;
-    bool counted;  // a launch before counts the shares
-};
-
 SortPlan sort_plan(int64_t pairs) {
     const int64_t turns = (pairs + kSortThreads - 1) / kSortThreads;
     const int64_t per = (turns + kSortBlocks - 1) / kSortBlocks;
@@ -412,35 +408,41 @@ SortPlan sort_plan(int64_t pairs) {
     return {blocks, (per ? per : 1) * kSortThreads, pairs > kSortOne};
 }
 
+namespace {
+
 bool sort_shape_ok(int64_t tokens, int64_t k, int64_t experts) {
     return experts > 0 && experts <= kSortMaxExperts && k > 0 && k <= kSortMaxK && tokens >= 0 &&
            tokens < (int64_t(1) << 31) && tokens * k < (int64_t(1) << 31);
 }
 
-int sort_launch(const void *ids, int wide, int64_t tokens, int64_t k, int64_t experts, uint32_t *work, int32_t *offsets,
-                int32_t *sorted_ids, int32_t *token_of, int32_t *slots, hipStream_t stream) {
-    const SortPlan plan = sort_plan(tokens * k);
+}  // namespace
+
+int sort_launch(const SortCall &c, hipStream_t stream) {
+    const SortPlan plan = sort_plan(c.pairs);
     SortArgs a{};
-    a.ids = static_cast<const uint32_t *>(ids);
-    a.hist = plan.counted ? work : nullptr;
-    a.offsets = offsets;
-    a.sorted_ids = sorted_ids;
-    a.tokens = token_of;
-    a.slots = slots;
-    a.P = uint32_t(tokens * k);
-    a.E = uint32_t(experts);
-    a.k = uint32_t(k);
+    a.ids = static_cast<const uint32_t *>(c.ids);
+    a.hist = plan.counted ? c.work : nullptr;
+    a.offsets = c.offsets;
+    a.sorted_ids = c.sorted_ids;
+    a.tokens = c.tokens;
+    a.slots = c.slots;
+    a.P = uint32_t(c.pairs);
+    a.E = uint32_t(c.experts);
+    a.k = uint32_t(c.per_token);
+    a.per_id = uint32_t(c.per_id);
     a.share = uint32_t(plan.share);
     const auto run = [&](auto kernel) {
         hipLaunchKernelGGL(kernel, dim3{uint32_t(plan.blocks)}, dim3{kSortThreads}, 0, stream, a);
         return hipGetLastError();
     };
     if (plan.counted) {
-        const hipError_t err = wide ? run(sort_count_kernel<true>) : run(sort_count_kernel<false>);
+        const hipError_t err = c.wide ? run(sort_count_kernel<true>) : run(sort_count_kernel<false>);
         if (err != hipSuccess) return record_launch(err);
     }
-    return record_launch(wide ? run(sort_kernel<true>) : run(sort_kernel<false>));
+    return record_launch(c.wide ? run(sort_kernel<true>) : run(sort_kernel<false>));
 }
+
+namespace {
 
 bool rows_shape_ok(int dtype, int64_t tokens, int64_t k, int64_t cols) {
     return dtype >= MX_F32 && dtype <= MX_BF16 && k > 0 && k <= kSortMaxK && tokens >= 0 && tokens < (int64_t(1) << 31) &&
@@ -481,6 +483,7 @@ void by_dtype(int dtype, F &&f) {
         f(std::integral_constant<int, MX_BF16>{});
 }
 
+}  // namespace
 }  // namespace iqk
 
 extern "C" {
@@ -498,8 +501,19 @@ int iqk_sort(const void *ids, int wide_ids, int64_t n_tokens, int64_t pairs_per_
     if (!sort_shape_ok(n_tokens, pairs_per_token, num_experts)) return IQK_ERR_GEOMETRY;
     if (!offsets || (n_tokens && (!ids || !sorted_ids || !tokens || !slots))) return IQK_ERR_ARGUMENT;
     if (sort_plan(n_tokens * pairs_per_token).counted && !work) return IQK_ERR_ARGUMENT;
-    return sort_launch(ids, wide_ids, n_tokens, pairs_per_token, num_experts, work, offsets, sorted_ids, tokens, slots,
-                       as_stream(stream));
+    SortCall c{};
+    c.ids = ids;
+    c.wide = wide_ids != 0;
+    c.pairs = n_tokens * pairs_per_token;
+    c.experts = num_experts;
+    c.per_token = pairs_per_token;
+    c.per_id = 1;
+    c.work = work;
+    c.offsets = offsets;
+    c.sorted_ids = sorted_ids;
+    c.tokens = tokens;
+    c.slots = slots;
+    return sort_launch(c, as_stream(stream));
 }
 
 int iqk_dispatch(int dtype, const void *x, const int32_t *slots, const int32_t *kept, int64_t n_tokens,
