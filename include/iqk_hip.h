@@ -381,8 +381,8 @@ int iqk_balance_grad(int dtype, const void *logits, const uint8_t *mask, const i
 // sorted behind the last expert.  offsets i32 [num_experts + 1]: the pairs of experts < e,
 // the last all that have an expert.  Per slot: sorted_ids (num_experts where left out) and
 // tokens i32 [n_tokens pairs_per_token]; per pair: slots, its place.  Stable, so the lists are
-// the same on every call.  ids: u32 or (wide_ids) i64.  work: iqk_sort_work words (0: may be
-// NULL).  num_experts <= 1024, pairs_per_token <= 64, fewer than 2^31 pairs.
+// the same on every call.  ids: u32 or (wide_ids) i64.  work: iqk_sort_work words, 16-byte
+// aligned (0: may be NULL).  num_experts <= 1024, pairs_per_token <= 64, fewer than 2^31 pairs.
 int64_t iqk_sort_work(int64_t n_tokens, int64_t pairs_per_token, int64_t num_experts);
 int iqk_sort(const void *ids, int wide_ids, int64_t n_tokens, int64_t pairs_per_token, int64_t num_experts,
              uint32_t *work, int32_t *offsets, int32_t *sorted_ids, int32_t *tokens, int32_t *slots, void *stream);

@@ -5,6 +5,7 @@
 // product with s_a stay in f32, and the sum with y is rounded once.
 
 #include <type_traits>
+#include <utility>
 
 #include "iqk_host.h"
 #include "iqk_mx.h"
@@ -111,11 +112,13 @@ __global__ __launch_bounds__(256) void adapter_up_kernel(AdapterArgs a) {
 
 // ------------------------------------------------------------- many rows ---
 //
-// Rows sorted by adapter, in tiles of SLOTS = 16 CT slots of one adapter; both products on the
-// 16x16x32 MFMAs, operand A the adapter's (16 ranks, 16 outputs), operand B the slots'.  The
+// Rows sorted by adapter, in tiles of 64 slots of one adapter; both products on the
+// 16x16x32 MFMAs, operand A the adapter's (16 ranks, 16 outputs), operand B 16 slots'.  The
 // first kernel leaves A x split into 16-bit pieces that give f32 back: a bf16 product takes three
 // pieces of eight bits (truncated, so that their sum is exact), an f16 product two of eleven
 // bits over a power of two of the slot's largest, which is multiplied back in f32.
+
+constexpr int kTileSlots = 64, kTileGroups = kTileSlots / 16;
 
 template <bool BF>
 constexpr int kPieces = BF ? 3 : 2;
@@ -136,7 +139,7 @@ struct Tile {
 
 // Tile t of the list in which each adapter's slots, and the rows without one (adapter: the
 // bank's size), take whole tiles in order.  All threads of a workgroup of THREADS call it.
-template <int SLOTS, int THREADS>
+template <int THREADS>
 __device__ __forceinline__ Tile find_tile(const AdapterArgs &a, uint32_t t, uint32_t (&sums)[THREADS / 64], uint32_t (&found)[3]) {
     constexpr int PER = (int(kAdaptersMax) + THREADS) / THREADS;  // consecutive groups of a thread
     const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, g0 = threadIdx.x * PER;
@@ -144,7 +147,7 @@ __device__ __forceinline__ Tile find_tile(const AdapterArgs &a, uint32_t t, uint
 #pragma unroll
     for (int i = 0; i <= PER; ++i) first[i] = g0 + i <= a.adapters ? a.offs[g0 + i] : a.T;
 #pragma unroll
-    for (int i = 0; i < PER; ++i) mine += (first[i + 1] - first[i] + SLOTS - 1) / SLOTS;
+    for (int i = 0; i < PER; ++i) mine += (first[i + 1] - first[i] + kTileSlots - 1) / kTileSlots;
     uint32_t incl = mine;
 #pragma unroll
     for (int off = 1; off < 64; off <<= 1) {
@@ -160,12 +163,12 @@ __device__ __forceinline__ Tile find_tile(const AdapterArgs &a, uint32_t t, uint
         if (uint32_t(w) < wave) at += sums[w];
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-        const uint32_t n = first[i + 1] - first[i], tiles = (n + SLOTS - 1) / SLOTS;
+        const uint32_t n = first[i + 1] - first[i], tiles = (n + kTileSlots - 1) / kTileSlots;
         if (t >= at && t < at + tiles) {
-            const uint32_t begin = (t - at) * SLOTS;
+            const uint32_t begin = (t - at) * kTileSlots;
             found[0] = g0 + i;
             found[1] = first[i] + begin;
-            found[2] = min(n - begin, uint32_t(SLOTS));
+            found[2] = min(n - begin, uint32_t(kTileSlots));
         }
         at += tiles;
     }
@@ -173,15 +176,19 @@ __device__ __forceinline__ Tile find_tile(const AdapterArgs &a, uint32_t t, uint
     return {found[0], found[1], found[2]};
 }
 
-// A x of a tile: WAVES wavefronts take 64 columns in turn, and their sums meet in LDS.
-template <bool BF, int RT, int CT, int WAVES>
+// A x of 16 CT slots of a tile: WAVES wavefronts take 32 KH columns in turn, DEPTH such steps on
+// their way at once, and their sums meet in LDS.
+template <bool BF, int RT, int CT, int WAVES, int KH, int DEPTH>
 __global__ __launch_bounds__(64 * WAVES) void adapter_down_tiles_kernel(AdapterArgs a) {
-    constexpr int SLOTS = 16 * CT, RANKS = 16 * RT, THREADS = 64 * WAVES, KC = (RT + 1) / 2;
+    constexpr int SLOTS = 16 * CT, RANKS = 16 * RT, THREADS = 64 * WAVES, KC = (RT + 1) / 2, PARTS = kTileGroups / CT;
     __shared__ float part[WAVES][SLOTS][RANKS + 4];
     __shared__ uint32_t sums[WAVES], found[3];
-    const Tile tile = find_tile<SLOTS, THREADS>(a, blockIdx.x, sums, found);
-    if (threadIdx.x == 0) a.tiles[blockIdx.x] = uint4_t{tile.adapter, tile.first, tile.slots, 0};
-    if (tile.slots == 0 || tile.adapter >= a.adapters) return;  // uniform
+    const uint32_t t = blockIdx.x / PARTS, group = blockIdx.x % PARTS * CT;  // the first of its groups of 16
+    Tile tile = find_tile<THREADS>(a, t, sums, found);
+    if (threadIdx.x == 0 && group == 0) a.tiles[t] = uint4_t{tile.adapter, tile.first, tile.slots, 0};
+    if (tile.slots <= 16 * group || tile.adapter >= a.adapters) return;  // uniform
+    tile.first += 16 * group;
+    tile.slots = min(tile.slots - 16 * group, uint32_t(SLOTS));
     const uint32_t lane = threadIdx.x & 63u, g = lane >> 4, m = lane & 15u;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint16_t *w[RT], *x[CT];
@@ -195,27 +202,43 @@ __global__ __launch_bounds__(64 * WAVES) void adapter_down_tiles_kernel(AdapterA
     for (int r = 0; r < RT; ++r)
 #pragma unroll
         for (int c = 0; c < CT; ++c) acc[r][c] = float4_t{0, 0, 0, 0};
-    for (uint32_t k0 = 64 * wave; k0 < a.in; k0 += 64 * WAVES) {
+    uint4_t xv[DEPTH][KH][CT], wv[DEPTH][KH][RT];
+    constexpr uint32_t STEP = 32 * KH * WAVES;
+    const auto load = [&](int d, uint32_t k0) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
+        for (int h = 0; h < KH; ++h) {
             const uint32_t k = k0 + 32 * h + 8 * g;
             const bool in = k < a.in;
             const uint32_t at = in ? k : 0u;
-            uint4_t xv[CT], wv[RT];
 #pragma unroll
-            for (int c = 0; c < CT; ++c) xv[c] = *reinterpret_cast<const chunk_t *>(x[c] + at);
+            for (int c = 0; c < CT; ++c) xv[d][h][c] = *reinterpret_cast<const chunk_t *>(x[c] + at);
 #pragma unroll
-            for (int r = 0; r < RT; ++r) wv[r] = load_u4(w[r] + at);
-            if (!in) {  // past the row: zeros on both sides
+            for (int r = 0; r < RT; ++r) wv[d][h][r] = load_u4(w[r] + at);
+        }
+    };
+    const auto multiply = [&](int d, uint32_t k0) {
 #pragma unroll
-                for (int c = 0; c < CT; ++c) xv[c] = uint4_t{0, 0, 0, 0};
+        for (int h = 0; h < KH; ++h) {
+            if (k0 + 32 * h + 32 > a.in && k0 + 32 * h + 8 * g >= a.in) {  // past the row: zeros on both sides
 #pragma unroll
-                for (int r = 0; r < RT; ++r) wv[r] = uint4_t{0, 0, 0, 0};
+                for (int c = 0; c < CT; ++c) xv[d][h][c] = uint4_t{0, 0, 0, 0};
+#pragma unroll
+                for (int r = 0; r < RT; ++r) wv[d][h][r] = uint4_t{0, 0, 0, 0};
             }
 #pragma unroll
             for (int r = 0; r < RT; ++r)
 #pragma unroll
-                for (int c = 0; c < CT; ++c) acc[r][c] = mfma<BF>(wv[r], xv[c], acc[r][c]);
+                for (int c = 0; c < CT; ++c) acc[r][c] = mfma<BF>(wv[d][h][r], xv[d][h][c], acc[r][c]);
+        }
+    };
+    uint32_t k0 = 32 * KH * wave;
+#pragma unroll
+    for (int d = 0; d < DEPTH - 1; ++d) load(d, k0 + d * STEP);
+    for (; k0 < a.in; k0 += DEPTH * STEP) {
+#pragma unroll
+        for (int d = 0; d < DEPTH; ++d) {
+            load((d + DEPTH - 1) % DEPTH, k0 + (d + DEPTH - 1) * STEP);
+            if (k0 + d * STEP < a.in) multiply(d, k0 + d * STEP);  // uniform
         }
     }
 #pragma unroll
@@ -239,8 +262,8 @@ __global__ __launch_bounds__(64 * WAVES) void adapter_down_tiles_kernel(AdapterA
             for (int i = 0; i < 8; ++i) v[i] *= scale;
         }
         // operand B of chunk kc: lane 16 g + n has slot n's ranks 32 kc + 8 g ..
-        const size_t at = ((size_t(blockIdx.x) * CT + slot / 16) * KC + unit / 4) * kPieces<BF> * 64 + 16 * (unit & 3u) +
-                          (slot & 15u);
+        const size_t at = ((size_t(t) * kTileGroups + group + slot / 16) * KC + unit / 4) * kPieces<BF> * 64 +
+                          16 * (unit & 3u) + (slot & 15u);
         if constexpr (BF) {
 #pragma unroll
             for (int p = 0; p < 3; ++p) {
@@ -267,44 +290,68 @@ __global__ __launch_bounds__(64 * WAVES) void adapter_down_tiles_kernel(AdapterA
             uint4_t hi, lo;
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const float t = ldexpf(v[i], e);
-                const uint32_t top = float_to_half_bits(t);
-                const float rest = fabsf(t) < __builtin_inff() ? t - half_bits_to_float(top) : 0.f;
+                const float scaled = ldexpf(v[i], e);
+                const uint32_t top = float_to_half_bits(scaled);
+                const float rest = fabsf(scaled) < __builtin_inff() ? scaled - half_bits_to_float(top) : 0.f;
                 const uint32_t low = float_to_half_bits(rest);
                 hi[i / 2] = i & 1 ? hi[i / 2] | top << 16 : top;
                 lo[i / 2] = i & 1 ? lo[i / 2] | low << 16 : low;
             }
             a.pieces[at] = hi;
             a.pieces[at + 64] = lo;
-            if (unit == 0) a.powers[size_t(blockIdx.x) * SLOTS + slot] = ldexpf(1.f, -e);
+            if (unit == 0) a.powers[size_t(t) * kTileSlots + 16 * group + slot] = ldexpf(1.f, -e);
         }
     }
 }
 
-// A tile's outputs: a wavefront takes 64 of them for all slots, lane 16 g + n sixteen
-// consecutive ones (16 g ..) of slot n, so that y is read and written 32 bytes a lane.
-template <bool BF, int CT>
+// Two outputs in 16 bits.
+template <bool BF>
+__device__ __forceinline__ uint32_t pair_bits(float lo, float hi) {
+    return BF ? bf16_bits(lo) | bf16_bits(hi) << 16 : float_to_half_bits(lo) | float_to_half_bits(hi) << 16;
+}
+
+// 256 outputs of a tile: a wavefront takes 64 of them for all slots, lane 16 g + n sixteen
+// consecutive ones (16 g ..) of slot n of each group, so that y is read and written 32 bytes a
+// lane.  The slots' operands go through LDS, which all four wavefronts read.
+template <bool BF>
 __global__ __launch_bounds__(256) void adapter_up_tiles_kernel(AdapterArgs a) {
-    constexpr int SLOTS = 16 * CT, P = kPieces<BF>;
+    constexpr int P = kPieces<BF>, CT = kTileGroups, STAGE = 2;  // chunks of 32 ranks in LDS at once
+    __shared__ uint4_t operands[STAGE][CT][P][64];
     const uint32_t columns = (a.N + 255) / 256, t = blockIdx.x / columns;
     const uint32_t lane = threadIdx.x & 63u, g = lane >> 4, m = lane & 15u;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t n0 = blockIdx.x % columns * 256 + 64 * wave;
     const uint4_t tile = a.tiles[t];
     const uint32_t adapter = tile.x, first = tile.y, slots = tile.z;
-    if (slots == 0 || n0 >= a.N) return;
+    if (slots == 0) return;  // uniform
     const uint32_t mine = n0 + 16 * g;  // the lane's first output
     const uint32_t have = mine < a.N ? min(a.N - mine, 16u) : 0u;
-    if (adapter >= a.adapters) {  // rows without an adapter
+    size_t at[CT];
+    uint32_t row[CT];
+    uint4_t y[CT][2];
+#pragma unroll
+    for (int c = 0; c < CT; ++c) {
+        row[c] = a.rows[first + min(16u * c + m, slots - 1u)];
+        at[c] = size_t(row[c]) * a.N + mine;
+        y[c][0] = y[c][1] = uint4_t{0, 0, 0, 0};
+        if (have == 16 && 16u * c < slots) {
+            y[c][0] = *reinterpret_cast<const chunk_t *>(a.y + at[c]);
+            y[c][1] = *reinterpret_cast<const chunk_t *>(a.y + at[c] + 8);
+        }
+    }
+    if (adapter >= a.adapters) {  // rows without an adapter; uniform
 #pragma unroll
         for (int c = 0; c < CT; ++c) {
-            const uint32_t slot = 16 * c + m;
-            if (slot >= slots) continue;
-            const uint32_t row = a.rows[first + slot];
-            const size_t at = size_t(row) * a.N + mine;
-            const bool bare = adapter_of(a, row) == a.adapters;
-            if (bare && a.out == a.y) continue;
-            for (uint32_t i = 0; i < have; ++i) a.out[at + i] = bare ? a.y[at + i] : BF ? uint16_t(0x7fc0) : kHalfNaN;
+            if (16 * c + m >= slots) continue;
+            const bool bare = adapter_of(a, row[c]) == a.adapters;
+            const uint32_t nan = BF ? 0x7fc07fc0u : 0x7e007e00u;
+            if (have == 16) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+                    *reinterpret_cast<chunk_t *>(a.out + at[c] + 8 * h) = bare ? y[c][h] : uint4_t{nan, nan, nan, nan};
+            } else {
+                for (uint32_t i = 0; i < have; ++i) a.out[at[c] + i] = bare ? a.y[at[c] + i] : uint16_t(nan);
+            }
         }
         return;
     }
@@ -313,46 +360,53 @@ __global__ __launch_bounds__(256) void adapter_up_tiles_kernel(AdapterArgs a) {
 #pragma unroll
     for (int j = 0; j < 4; ++j)
         w[j] = a.up + (size_t(adapter) * a.N + min(n0 + 16 * (m >> 2) + 4 * j + (m & 3u), a.N - 1u)) * a.rank;
-    const uint4_t *const b = a.pieces + size_t(t) * CT * a.chunks * P * 64 + lane;
-    size_t at[CT];
-    uint4_t y[CT][2];
-#pragma unroll
-    for (int c = 0; c < CT; ++c) {
-        at[c] = size_t(a.rows[first + min(16u * c + m, slots - 1u)]) * a.N + mine;
-        y[c][0] = y[c][1] = uint4_t{0, 0, 0, 0};
-        if (have == 16) {
-            y[c][0] = *reinterpret_cast<const chunk_t *>(a.y + at[c]);
-            y[c][1] = *reinterpret_cast<const chunk_t *>(a.y + at[c] + 8);
-        }
-    }
     float4_t acc[4][CT];
 #pragma unroll
     for (int j = 0; j < 4; ++j)
 #pragma unroll
         for (int c = 0; c < CT; ++c) acc[j][c] = float4_t{0, 0, 0, 0};
-    for (uint32_t kc = 0; 32 * kc < a.rank; ++kc) {
-        const uint32_t k = 32 * kc + 8 * g;
-        uint4_t wv[4], bv[CT][P];
+    for (uint32_t k0 = 0; k0 < a.rank; k0 += 32 * STAGE) {
+        uint4_t wv[STAGE][4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            wv[j] = uint4_t{0, 0, 0, 0};
-            if (k < a.rank) wv[j] = load_u4(w[j] + k);
+        for (int s = 0; s < STAGE; ++s) {
+            const uint32_t k = k0 + 32 * s + 8 * g;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                wv[s][j] = uint4_t{0, 0, 0, 0};
+                if (k < a.rank) wv[s][j] = load_u4(w[j] + k);
+            }
         }
+        if (k0) __syncthreads();  // the stage before has been read
 #pragma unroll
-        for (int c = 0; c < CT; ++c)
+        for (int s = 0; s < STAGE; ++s) {
+            if (k0 + 32 * s >= a.rank) continue;  // uniform
 #pragma unroll
-            for (int p = 0; p < P; ++p) bv[c][p] = b[((size_t(c) * a.chunks + kc) * P + p) * 64];
+            for (int i = 0; i < (CT * P * 64) / 256; ++i) {  // a group's pieces of a chunk lie together
+                const uint32_t u = 256 * i + threadIdx.x, c = u / (P * 64), rest = u % (P * 64);
+                const size_t from = ((size_t(t) * CT + c) * a.chunks + k0 / 32 + s) * P * 64 + rest;
+                if (16 * c < slots) operands[s][c][rest / 64][rest % 64] = a.pieces[from];
+            }
+        }
+        __syncthreads();
 #pragma unroll
-        for (int p = P - 1; p >= 0; --p)  // the small pieces first
+        for (int s = 0; s < STAGE; ++s) {
+            if (k0 + 32 * s >= a.rank) continue;  // uniform
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
+            for (int c = 0; c < CT; ++c) {
+                if (16u * c >= slots) continue;  // uniform
 #pragma unroll
-                for (int c = 0; c < CT; ++c) acc[j][c] = mfma<BF>(wv[j], bv[c][p], acc[j][c]);
+                for (int p = P - 1; p >= 0; --p) {  // the small pieces first
+                    const uint4_t b = operands[s][c][p][lane];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) acc[j][c] = mfma<BF>(wv[s][j], b, acc[j][c]);
+                }
+            }
+        }
     }
 #pragma unroll
     for (int c = 0; c < CT; ++c) {
         if (16 * c + m >= slots) continue;
-        const float power = BF ? 1.f : a.powers[size_t(t) * SLOTS + 16 * c + m];
+        const float power = BF ? 1.f : a.powers[size_t(t) * kTileSlots + 16 * c + m];
         float v[16];
 #pragma unroll
         for (int j = 0; j < 4; ++j)
@@ -366,8 +420,7 @@ __global__ __launch_bounds__(256) void adapter_up_tiles_kernel(AdapterArgs a) {
                 for (int i = 0; i < 4; ++i) {
                     const uint32_t word = y[c][h][i];
                     const float2v_t old = floats<BF>(word);
-                    const float lo = old.x + v[8 * h + 2 * i], hi = old.y + v[8 * h + 2 * i + 1];
-                    out[i] = BF ? bf16_bits(lo) | bf16_bits(hi) << 16 : float_to_half_bits(lo) | float_to_half_bits(hi) << 16;
+                    out[i] = pair_bits<BF>(old.x + v[8 * h + 2 * i], old.y + v[8 * h + 2 * i + 1]);
                 }
                 *reinterpret_cast<chunk_t *>(a.out + at[c] + 8 * h) = out;
             }
@@ -394,45 +447,49 @@ constexpr int64_t kRowsAlone = 64;  // rows up to which each is computed on its 
 
 // The grouped form's workspace, in words: where each part begins.
 struct GroupPlan {
-    int64_t slots, tiles, chunks, hist, offs, rows, desc, pieces, powers, words;
+    int64_t tiles, chunks, hist, offs, rows, desc, pieces, powers, words;
 };
 
 GroupPlan group_plan(int64_t rank, int64_t adapters, int64_t rows) {
     GroupPlan p{};
-    p.slots = rank > 128 ? 16 : 32;
     // every adapter and the rows without one may end in a part of a tile
-    const int64_t most = rows / p.slots + adapters + 1;
+    const int64_t most = rows / kTileSlots + adapters + 1;
     p.tiles = most < rows ? most : rows;
-    const SortPlan sort = sort_plan(rows);
     for (p.chunks = 1; 32 * p.chunks < rank;) p.chunks *= 2;
     const auto take = [&](int64_t words) {
         const int64_t at = p.words;
         p.words += (words + 3) / 4 * 4;  // 16-byte steps
         return at;
     };
-    p.hist = take(sort.counted ? sort.blocks * (adapters + 1) : 0);
+    p.hist = take(sort_plan(rows, adapters).words);
     p.offs = take(adapters + 1);
     p.rows = take(rows);
     p.desc = take(4 * p.tiles);
-    p.pieces = take(p.tiles * (p.slots / 16) * p.chunks * 3 * 64 * 4);
-    p.powers = take(p.tiles * p.slots);
+    p.pieces = take(p.tiles * kTileGroups * p.chunks * 3 * 64 * 4);
+    p.powers = take(p.tiles * kTileSlots);
     return p;
 }
 
+// f(16s of ranks, groups of slots, wavefronts, 32s of columns a step, steps on their way)
 template <typename F>
 void by_ranks(int64_t rank, F &&f) {
-    const auto with = [&](auto rt, auto ct, auto waves) { f(rt, ct, waves); };
-    using std::integral_constant;
+    using std::integer_sequence;
     if (rank <= 16)
-        with(integral_constant<int, 1>{}, integral_constant<int, 2>{}, integral_constant<int, 8>{});
+        f(integer_sequence<int, 1, 2, 8, 2, 4>{});
     else if (rank <= 32)
-        with(integral_constant<int, 2>{}, integral_constant<int, 2>{}, integral_constant<int, 8>{});
+        f(integer_sequence<int, 2, 2, 8, 2, 4>{});
     else if (rank <= 64)
-        with(integral_constant<int, 4>{}, integral_constant<int, 2>{}, integral_constant<int, 4>{});
+        f(integer_sequence<int, 4, 2, 8, 2, 2>{});
     else if (rank <= 128)
-        with(integral_constant<int, 8>{}, integral_constant<int, 2>{}, integral_constant<int, 2>{});
+        f(integer_sequence<int, 8, 2, 4, 1, 2>{});
     else
-        with(integral_constant<int, 16>{}, integral_constant<int, 1>{}, integral_constant<int, 2>{});
+        f(integer_sequence<int, 16, 1, 4, 1, 2>{});
+}
+
+template <bool BF, int RT, int CT, int WAVES, int KH, int DEPTH>
+void launch_down(const AdapterArgs &a, int64_t tiles, hipStream_t stream, std::integer_sequence<int, RT, CT, WAVES, KH, DEPTH>) {
+    hipLaunchKernelGGL((adapter_down_tiles_kernel<BF, RT, CT, WAVES, KH, DEPTH>), dim3{uint32_t(tiles * (kTileGroups / CT))},
+                       dim3{64 * WAVES}, 0, stream, a);
 }
 
 int rows_alone(const AdapterArgs &a, bool bf, hipStream_t stream) {
@@ -451,7 +508,7 @@ int rows_alone(const AdapterArgs &a, bool bf, hipStream_t stream) {
 int rows_grouped(AdapterArgs a, bool bf, uint32_t *work, hipStream_t stream) {
     const GroupPlan p = group_plan(a.rank, a.adapters, a.T);
     const int64_t ups = p.tiles * ((int64_t(a.N) + 255) / 256);
-    if (!grid_ok(ups, 256) || !grid_ok(p.tiles, 512)) return IQK_ERR_GEOMETRY;
+    if (!grid_ok(ups, 256) || !grid_ok(p.tiles * kTileGroups, 512)) return IQK_ERR_GEOMETRY;
     SortCall c{};
     c.ids = a.ids;
     c.wide = a.wide;
@@ -469,17 +526,17 @@ int rows_grouped(AdapterArgs a, bool bf, uint32_t *work, hipStream_t stream) {
     a.pieces = reinterpret_cast<uint4_t *>(work + p.pieces);
     a.powers = reinterpret_cast<float *>(work + p.powers);
     a.chunks = uint32_t(p.chunks);
-    by_ranks(a.rank, [&](auto rt, auto ct, auto waves) {
-        constexpr int RT = decltype(rt)::value, CT = decltype(ct)::value, WAVES = decltype(waves)::value;
-        const auto run = [&](auto down, auto up) {
-            hipLaunchKernelGGL(down, dim3{uint32_t(p.tiles)}, dim3{64 * WAVES}, 0, stream, a);
-            hipLaunchKernelGGL(up, dim3{uint32_t(ups)}, dim3{256}, 0, stream, a);
-        };
+    by_ranks(a.rank, [&](auto shape) {
         if (bf)
-            run(adapter_down_tiles_kernel<true, RT, CT, WAVES>, adapter_up_tiles_kernel<true, CT>);
+            launch_down<true>(a, p.tiles, stream, shape);
         else
-            run(adapter_down_tiles_kernel<false, RT, CT, WAVES>, adapter_up_tiles_kernel<false, CT>);
+            launch_down<false>(a, p.tiles, stream, shape);
     });
+    if (const hipError_t err = hipGetLastError(); err != hipSuccess) return record_launch(err);
+    if (bf)
+        hipLaunchKernelGGL(adapter_up_tiles_kernel<true>, dim3{uint32_t(ups)}, dim3{256}, 0, stream, a);
+    else
+        hipLaunchKernelGGL(adapter_up_tiles_kernel<false>, dim3{uint32_t(ups)}, dim3{256}, 0, stream, a);
     return record_launch(hipGetLastError());
 }
 

@@ -32,7 +32,7 @@ constexpr int64_t kSortBlocks = 256;  // workgroups of a sort, at most
 
 struct SortArgs {
     const uint32_t *ids;
-    uint32_t *hist;  // [blocks][E + 1], or null: every workgroup counts all pairs
+    uint32_t *hist;  // [blocks][hist_stride(E)], 16-byte aligned, or null: every workgroup counts all pairs
     int32_t *offsets, *sorted_ids, *tokens, *slots;  // sorted_ids and slots may be null
     uint32_t P, E, k, share;  // share: pairs of a workgroup, in order
     uint32_t per_id;          // pairs of an id
@@ -43,17 +43,62 @@ __device__ __forceinline__ uint32_t key_of(const SortArgs &a, uint32_t p) {
     return min(expert_id(a.ids, a.per_id == 1 ? p : p / a.per_id, WIDE ? 1u : 0u), a.E);
 }
 
+// The lanes whose key is this lane's (bits: of the largest key), found by a ballot for each bit.
+__device__ __forceinline__ uint64_t same_key(uint32_t key, bool live, int bits) {
+    uint64_t same = __ballot(live);
+    for (int b = 0; b < bits; ++b) {
+        const bool bit = (key >> b) & 1u;
+        const uint64_t m = __ballot(bit);
+        same &= bit ? m : ~m;
+    }
+    return same;
+}
+
+// How many of a set of lanes come before this one.
+__device__ __forceinline__ uint32_t rank_in(uint64_t lanes) {
+    return __builtin_amdgcn_mbcnt_hi(uint32_t(lanes >> 32), __builtin_amdgcn_mbcnt_lo(uint32_t(lanes), 0));
+}
+
+// add(key, n, p) for the pairs from `base` to `end` that a wavefront takes, 64 from p on at every
+// STRIDE-th: once for each key among them, by one lane, with their number n (LDS adds to one
+// address one after the other).  AHEAD loads of ids are on their way at once.
+template <bool WIDE, uint32_t STRIDE, typename F>
+__device__ __forceinline__ void count_keys(const SortArgs &a, uint32_t base, uint32_t end, int bits, F &&add) {
+    constexpr int AHEAD = 4;
+    const uint32_t lane = threadIdx.x & 63u;
+    for (; base < end; base += AHEAD * STRIDE) {
+        uint32_t key[AHEAD];
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) key[i] = key_of<WIDE>(a, min(base + i * STRIDE + lane, end - 1u));
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) {
+            const uint32_t p = base + i * STRIDE;
+            if (p >= end) continue;  // uniform
+            const bool live = p + lane < end;
+            const uint64_t same = same_key(key[i], live, bits);
+            if (live && rank_in(same) == 0) add(key[i], uint32_t(__popcll(same)), p);
+        }
+    }
+}
+
+__device__ __forceinline__ int key_bits(const SortArgs &a) { return 32 - __clz(int(a.E)); }  // of the largest key, E
+
+// Words from one workgroup's counts to the next one's: whole 16 bytes.
+__host__ __device__ constexpr int64_t hist_stride(int64_t experts) { return (experts + 1 + 3) / 4 * 4; }
+
 // A workgroup's counts of its share of the pairs, by key.
 template <bool WIDE>
 __global__ __launch_bounds__(kSortThreads) void sort_count_kernel(SortArgs a) {
-    __shared__ uint32_t count[kSortKeys];
-    const uint32_t K = a.E + 1;
-    for (uint32_t e = threadIdx.x; e < K; e += kSortThreads) count[e] = 0;
+    __shared__ uint32_t count[kSortKeys + 3];
+    const uint32_t stride = uint32_t(hist_stride(a.E));
+    for (uint32_t e = threadIdx.x; e < stride; e += kSortThreads) count[e] = 0;
     __syncthreads();
     const uint32_t lo = min(a.P, blockIdx.x * a.share), hi = min(a.P, lo + a.share);
-    for (uint32_t p = lo + threadIdx.x; p < hi; p += kSortThreads) atomicAdd(&count[key_of<WIDE>(a, p)], 1u);
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    count_keys<WIDE, kSortThreads>(a, lo + 64 * wave, hi, key_bits(a),
+                                   [&](uint32_t key, uint32_t n, uint32_t) { atomicAdd(&count[key], n); });
     __syncthreads();
-    for (uint32_t e = threadIdx.x; e < K; e += kSortThreads) a.hist[size_t(blockIdx.x) * K + e] = count[e];
+    for (uint32_t e = threadIdx.x; e < stride; e += kSortThreads) a.hist[size_t(blockIdx.x) * stride + e] = count[e];
 }
 
 struct SortShared {
@@ -110,25 +155,41 @@ __global__ __launch_bounds__(kSortThreads) void sort_kernel(SortArgs a) {
     const uint32_t lo = min(a.P, blockIdx.x * a.share), hi = min(a.P, lo + a.share);
     const uint32_t part = (a.share / kSortWaves + 63u) & ~63u;
     const uint32_t from = min(hi, lo + wave * part), to = min(hi, from + part);
+    const int bits = key_bits(a);
     if (a.hist) {
-        for (uint32_t e = lane; e < K; e += 64) {
-            uint32_t total = 0, before = 0;
-            for (uint32_t b = wave; b < gridDim.x; b += kSortWaves) {
-                const uint32_t n = a.hist[size_t(b) * K + e];
-                total += n;
-                if (b < blockIdx.x) before += n;
+        // four keys a lane, a wavefront every kSortWaves-th share's counts, AHEAD of them at once
+        constexpr uint32_t AHEAD = 8;
+        const uint32_t stride = uint32_t(hist_stride(a.E));
+        for (uint32_t e = 4 * lane; e < K; e += 256) {
+            uint4_t total = {0, 0, 0, 0}, before = {0, 0, 0, 0};
+            for (uint32_t b0 = wave; b0 < gridDim.x; b0 += AHEAD * kSortWaves) {
+                uint4_t n[AHEAD];
+#pragma unroll
+                for (uint32_t i = 0; i < AHEAD; ++i)
+                    n[i] = load_u4(a.hist + size_t(min(b0 + i * kSortWaves, gridDim.x - 1u)) * stride + e);
+#pragma unroll
+                for (uint32_t i = 0; i < AHEAD; ++i) {
+                    const uint32_t b = b0 + i * kSortWaves;
+                    if (b < gridDim.x) total += n[i];
+                    if (b < blockIdx.x) before += n[i];
+                }
             }
-            atomicAdd(&s.total[e], total);
-            atomicAdd(&s.before[e], before);
+#pragma unroll
+            for (uint32_t i = 0; i < 4; ++i) {
+                if (e + i < K) {
+                    atomicAdd(&s.total[e + i], total[i]);
+                    atomicAdd(&s.before[e + i], before[i]);
+                }
+            }
         }
     } else {
-        for (uint32_t p = threadIdx.x; p < a.P; p += kSortThreads) {
-            const uint32_t e = key_of<WIDE>(a, p);
-            atomicAdd(&s.total[e], 1u);
-            if (p < lo) atomicAdd(&s.before[e], 1u);
-        }
+        // 64 pairs lie on one side of the share's start
+        count_keys<WIDE, kSortThreads>(a, 64 * wave, a.P, bits, [&](uint32_t key, uint32_t n, uint32_t p) {
+            atomicAdd(&s.total[key], n);
+            if (p < lo) atomicAdd(&s.before[key], n);
+        });
     }
-    for (uint32_t p = from + lane; p < to; p += 64) atomicAdd(&s.wave[wave][key_of<WIDE>(a, p)], 1u);
+    count_keys<WIDE, 64>(a, from, to, bits, [&](uint32_t key, uint32_t n, uint32_t) { atomicAdd(&s.wave[wave][key], n); });
     __syncthreads();
     scan_keys(s, K);
     for (uint32_t e = threadIdx.x; e < K; e += kSortThreads) {
@@ -144,18 +205,12 @@ __global__ __launch_bounds__(kSortThreads) void sort_kernel(SortArgs a) {
     }
     __syncthreads();
     volatile uint32_t *const next = s.wave[wave];
-    const int bits = 32 - __clz(int(a.E));  // of the largest key, E
     for (uint32_t base = from; base < to; base += 64) {
         const uint32_t p = base + lane;
         const bool live = p < to;
         const uint32_t key = live ? key_of<WIDE>(a, p) : 0u;
-        uint64_t same = __ballot(live);
-        for (int b = 0; b < bits; ++b) {
-            const bool bit = (key >> b) & 1u;
-            const uint64_t m = __ballot(bit);
-            same &= bit ? m : ~m;
-        }
-        const uint32_t rank = __builtin_amdgcn_mbcnt_hi(uint32_t(same >> 32), __builtin_amdgcn_mbcnt_lo(uint32_t(same), 0));
+        const uint64_t same = same_key(key, live, bits);
+        const uint32_t rank = rank_in(same);
         if (live) {
             const uint32_t slot = next[key] + rank;
             __builtin_amdgcn_wave_barrier();  // all lanes have read before the last of each key writes
@@ -216,24 +271,29 @@ __device__ __forceinline__ uint4_t pack(const float (&v)[kChunk<DT>]) {
     return w;
 }
 
-// The first `halves` (1 .. 8) 16-bit halves of a chunk, zeros behind them.
+// A chunk, or (not WHOLE) its first `halves` (1 .. 7) 16-bit halves and zeros behind them.
+template <bool WHOLE>
 __device__ __forceinline__ uint4_t load_chunk(const uint8_t *p, uint32_t halves) {
-    if (halves == 8) return *reinterpret_cast<const chunk_t *>(p);
-    uint4_t w = {0, 0, 0, 0};
+    if constexpr (WHOLE) {
+        return *reinterpret_cast<const chunk_t *>(p);
+    } else {
+        uint4_t w = {0, 0, 0, 0};
 #pragma unroll
-    for (uint32_t i = 0; i < 7; ++i)
-        if (i < halves) w[i / 2] |= uint32_t(reinterpret_cast<const half16_t *>(p)[i]) << (16 * (i & 1));
-    return w;
+        for (uint32_t i = 0; i < 7; ++i)
+            if (i < halves) w[i / 2] |= uint32_t(reinterpret_cast<const half16_t *>(p)[i]) << (16 * (i & 1));
+        return w;
+    }
 }
 
+template <bool WHOLE>
 __device__ __forceinline__ void store_chunk(uint8_t *p, uint4_t w, uint32_t halves) {
-    if (halves == 8) {
+    if constexpr (WHOLE) {
         *reinterpret_cast<chunk_t *>(p) = w;
-        return;
-    }
+    } else {
 #pragma unroll
-    for (uint32_t i = 0; i < 7; ++i)
-        if (i < halves) reinterpret_cast<half16_t *>(p)[i] = uint16_t(w[i / 2] >> (16 * (i & 1)));
+        for (uint32_t i = 0; i < 7; ++i)
+            if (i < halves) reinterpret_cast<half16_t *>(p)[i] = uint16_t(w[i / 2] >> (16 * (i & 1)));
+    }
 }
 
 struct RowArgs {
@@ -251,13 +311,16 @@ struct RowArgs {
     uint32_t first;           // the launch's first token
 };
 
-// What one thread has of rows: a token and a chunk of them.
+// What one thread has of rows: a token and a chunk of them.  UNIFORM: a wavefront's threads have
+// one token (at least 64 threads a token), so that its slots and weights are scalars.
+template <bool UNIFORM>
 struct Place {
     uint32_t t, chunk, halves;
     bool live;
     __device__ __forceinline__ explicit Place(const RowArgs &a) {
         const uint32_t width = 1u << a.log_width;
         t = a.first + (blockIdx.x / a.columns << (8 - a.log_width)) + (threadIdx.x >> a.log_width);
+        if constexpr (UNIFORM) t = __builtin_amdgcn_readfirstlane(t);
         chunk = (blockIdx.x % a.columns << a.log_width) + (threadIdx.x & (width - 1u));
         live = t < a.T && chunk < a.chunks;
         halves = min(8u, (a.row - 16u * chunk) / 2u);
@@ -266,129 +329,163 @@ struct Place {
 
 __device__ __forceinline__ uint32_t slots_kept(const RowArgs &a) { return a.kept ? min(uint32_t(*a.kept), a.P) : a.P; }
 
-// Each token's row to its slots, zeros to those left out.
-__global__ __launch_bounds__(256) void dispatch_kernel(RowArgs a) {
-    const Place at(a);
-    if (!at.live) return;
+constexpr int kAhead = 8;  // choices whose rows are on their way at once
+
+template <bool WHOLE, typename PLACE>
+__device__ __forceinline__ void dispatch_chunk(const RowArgs &a, const PLACE &at) {
     const uint32_t kept = slots_kept(a);
     const size_t column = size_t(at.chunk) * 16;
-    const uint4_t w = load_chunk(a.in + size_t(at.t) * a.row + column, at.halves);
+    const uint4_t w = load_chunk<WHOLE>(a.in + size_t(at.t) * a.row + column, at.halves);
     for (uint32_t j = 0; j < a.k; ++j) {
         const uint32_t slot = uint32_t(a.slots[size_t(at.t) * a.k + j]);
-        if (slot < a.P) store_chunk(a.out + size_t(slot) * a.row + column, slot < kept ? w : uint4_t{0, 0, 0, 0}, at.halves);
+        if (slot < a.P)
+            store_chunk<WHOLE>(a.out + size_t(slot) * a.row + column, slot < kept ? w : uint4_t{0, 0, 0, 0}, at.halves);
     }
 }
 
-// A token's rows, weighted and summed.
-template <int DT>
-__global__ __launch_bounds__(256) void combine_kernel(RowArgs a) {
-    constexpr int N = kChunk<DT>, AHEAD = 8;  // rows on their way at once
-    const Place at(a);
+// Each token's row to its slots, zeros to those left out.
+template <bool UNIFORM>
+__global__ __launch_bounds__(256) void dispatch_kernel(RowArgs a) {
+    const Place<UNIFORM> at(a);
     if (!at.live) return;
+    if (at.halves == 8)
+        dispatch_chunk<true>(a, at);
+    else
+        dispatch_chunk<false>(a, at);
+}
+
+template <int DT, bool WHOLE, typename PLACE>
+__device__ __forceinline__ void combine_chunk(const RowArgs &a, const PLACE &at) {
+    constexpr int N = kChunk<DT>;
     const uint32_t kept = slots_kept(a);
     const size_t column = size_t(at.chunk) * 16, pair = size_t(at.t) * a.k;
     float sum[N] = {};
-    for (uint32_t j0 = 0; j0 < a.k; j0 += AHEAD) {
-        uint4_t w[AHEAD];
-        bool has[AHEAD];
+    for (uint32_t j0 = 0; j0 < a.k; j0 += kAhead) {
+        uint32_t slot[kAhead];
+        uint4_t w[kAhead];
+        float weight[kAhead];
 #pragma unroll
-        for (int i = 0; i < AHEAD; ++i) {
+        for (int i = 0; i < kAhead; ++i) {
             const uint32_t j = min(j0 + i, a.k - 1u);
-            const uint32_t slot = a.slots ? uint32_t(a.slots[pair + j]) : uint32_t(pair) + j;
-            has[i] = j0 + i < a.k && slot < kept;
-            w[i] = uint4_t{0, 0, 0, 0};
-            if (has[i]) w[i] = load_chunk(a.in + size_t(slot) * a.row + column, at.halves);
+            slot[i] = a.slots ? uint32_t(a.slots[pair + j]) : uint32_t(pair) + j;
+            weight[i] = a.weights ? a.weights[pair + j] : 1.f;
+            if (j0 + i >= a.k) slot[i] = a.P;
         }
 #pragma unroll
-        for (int i = 0; i < AHEAD; ++i) {
-            if (!has[i]) continue;
+        for (int i = 0; i < kAhead; ++i)
+            if (slot[i] < kept) w[i] = load_chunk<WHOLE>(a.in + size_t(slot[i]) * a.row + column, at.halves);
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+            if (slot[i] >= kept) continue;
             float v[N];
             unpack<DT>(w[i], v);
-            const float weight = a.weights ? a.weights[pair + j0 + i] : 1.f;
 #pragma unroll
-            for (int n = 0; n < N; ++n) sum[n] = fmaf(weight, v[n], sum[n]);
+            for (int n = 0; n < N; ++n) sum[n] = fmaf(weight[i], v[n], sum[n]);
         }
     }
     const size_t mine = size_t(at.t) * a.row + column;
     if (a.add) {
         float v[N];
-        unpack<DT>(load_chunk(a.add + mine, at.halves), v);
+        unpack<DT>(load_chunk<WHOLE>(a.add + mine, at.halves), v);
 #pragma unroll
         for (int n = 0; n < N; ++n) sum[n] += v[n];
     }
-    store_chunk(a.out + mine, pack<DT>(sum), at.halves);
+    store_chunk<WHOLE>(a.out + mine, pack<DT>(sum), at.halves);
+}
+
+// A token's rows, weighted and summed.
+template <int DT, bool UNIFORM>
+__global__ __launch_bounds__(256) void combine_kernel(RowArgs a) {
+    const Place<UNIFORM> at(a);
+    if (!at.live) return;
+    if (at.halves == 8)
+        combine_chunk<DT, true>(a, at);
+    else
+        combine_chunk<DT, false>(a, at);
+}
+
+// What a chunk of a token's dout adds to its choices' dots, and its chunk of their rows' gradients.
+template <int DT, bool WHOLE>
+__device__ __forceinline__ void grad_chunk(const RowArgs &a, uint32_t t, uint32_t chunk, uint32_t halves, uint32_t kept,
+                                           const uint32_t (&slot)[kAhead], const float (&weight)[kAhead], float (&dot)[kAhead]) {
+    constexpr int N = kChunk<DT>;
+    const size_t column = size_t(chunk) * 16;
+    const uint4_t gw = load_chunk<WHOLE>(a.in + size_t(t) * a.row + column, halves);
+    uint4_t w[kAhead];
+    if (a.dweights) {
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i)
+            if (slot[i] < kept) w[i] = load_chunk<WHOLE>(a.y + size_t(slot[i]) * a.row + column, halves);
+    }
+    float g[N];
+    unpack<DT>(gw, g);
+    if (a.out) {
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+            if (slot[i] >= a.P) continue;
+            float v[N];
+#pragma unroll
+            for (int n = 0; n < N; ++n) v[n] = weight[i] * g[n];
+            store_chunk<WHOLE>(a.out + size_t(slot[i]) * a.row + column,
+                               slot[i] < kept ? pack<DT>(v) : uint4_t{0, 0, 0, 0}, halves);
+        }
+    }
+    if (a.dweights) {
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+            if (slot[i] >= kept) continue;
+            float v[N];
+            unpack<DT>(w[i], v);
+#pragma unroll
+            for (int n = 0; n < N; ++n) dot[i] = fmaf(g[n], v[n], dot[i]);
+        }
+    }
 }
 
 // Both gradients of a token's sum: WAVES wavefronts a token take its row's chunks in turn.
 template <int DT, int WAVES>
 __global__ __launch_bounds__(256) void combine_grad_kernel(RowArgs a) {
-    constexpr int N = kChunk<DT>, AHEAD = 8;
-    __shared__ float part[4][AHEAD];
+    __shared__ float part[4][kAhead];
     const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t t = a.first + (WAVES == 1 ? blockIdx.x * 4 + wave : blockIdx.x);
     if (WAVES == 1 && t >= a.T) return;  // whole wavefronts, and no barrier follows
     const uint32_t kept = slots_kept(a);
     const size_t pair = size_t(t) * a.k;
-    for (uint32_t j0 = 0; j0 < a.k; j0 += AHEAD) {
-        uint32_t slot[AHEAD];
-        float weight[AHEAD], dot[AHEAD];
-        bool has[AHEAD];
+    for (uint32_t j0 = 0; j0 < a.k; j0 += kAhead) {
+        uint32_t slot[kAhead];
+        float weight[kAhead], dot[kAhead];
 #pragma unroll
-        for (int i = 0; i < AHEAD; ++i) {
+        for (int i = 0; i < kAhead; ++i) {
             const uint32_t j = min(j0 + i, a.k - 1u);
             slot[i] = a.slots ? uint32_t(a.slots[pair + j]) : uint32_t(pair) + j;
+            weight[i] = a.weights[pair + j];
             if (j0 + i >= a.k) slot[i] = a.P;
-            has[i] = slot[i] < kept;
-            weight[i] = has[i] ? a.weights[pair + j] : 0.f;
             dot[i] = 0.f;
         }
         for (uint32_t c = (WAVES == 1 ? 0 : wave * 64) + lane; c < a.chunks; c += WAVES * 64) {
             const uint32_t halves = min(8u, (a.row - 16u * c) / 2u);
-            const size_t column = size_t(c) * 16;
-            uint4_t w[AHEAD];
-            if (a.dweights) {
-#pragma unroll
-                for (int i = 0; i < AHEAD; ++i) {
-                    w[i] = uint4_t{0, 0, 0, 0};
-                    if (has[i]) w[i] = load_chunk(a.y + size_t(slot[i]) * a.row + column, halves);
-                }
-            }
-            float g[N];
-            unpack<DT>(load_chunk(a.in + size_t(t) * a.row + column, halves), g);
-#pragma unroll
-            for (int i = 0; i < AHEAD; ++i) {
-                if (a.dweights && has[i]) {
-                    float v[N];
-                    unpack<DT>(w[i], v);
-#pragma unroll
-                    for (int n = 0; n < N; ++n) dot[i] = fmaf(g[n], v[n], dot[i]);
-                }
-                if (a.out && slot[i] < a.P) {
-                    float v[N];
-#pragma unroll
-                    for (int n = 0; n < N; ++n) v[n] = weight[i] * g[n];
-                    store_chunk(a.out + size_t(slot[i]) * a.row + column,
-                                has[i] ? pack<DT>(v) : uint4_t{0, 0, 0, 0}, halves);
-                }
-            }
+            if (halves == 8)
+                grad_chunk<DT, true>(a, t, c, halves, kept, slot, weight, dot);
+            else
+                grad_chunk<DT, false>(a, t, c, halves, kept, slot, weight, dot);
         }
         if (!a.dweights) continue;
 #pragma unroll
-        for (int i = 0; i < AHEAD; ++i) {
+        for (int i = 0; i < kAhead; ++i) {
 #pragma unroll
             for (int off = 32; off > 0; off >>= 1) dot[i] += __shfl_xor(dot[i], off, 64);
         }
         if constexpr (WAVES == 1) {
 #pragma unroll
-            for (int i = 0; i < AHEAD; ++i)
-                if (lane == uint32_t(i) && j0 + i < a.k) a.dweights[pair + j0 + i] = has[i] ? dot[i] : 0.f;
+            for (int i = 0; i < kAhead; ++i)
+                if (lane == uint32_t(i) && j0 + i < a.k) a.dweights[pair + j0 + i] = dot[i];
         } else {
             if (lane == 0) {
 #pragma unroll
-                for (int i = 0; i < AHEAD; ++i) part[wave][i] = has[i] ? dot[i] : 0.f;
+                for (int i = 0; i < kAhead; ++i) part[wave][i] = dot[i];
             }
             __syncthreads();
-            if (threadIdx.x < AHEAD && j0 + threadIdx.x < a.k) {
+            if (threadIdx.x < kAhead && j0 + threadIdx.x < a.k) {
                 float sum = 0.f;
 #pragma unroll
                 for (int w = 0; w < WAVES; ++w) sum += part[w][threadIdx.x];
@@ -401,11 +498,11 @@ __global__ __launch_bounds__(256) void combine_grad_kernel(RowArgs a) {
 
 // --------------------------------------------------------------------- host ---
 
-SortPlan sort_plan(int64_t pairs) {
+SortPlan sort_plan(int64_t pairs, int64_t experts) {
     const int64_t turns = (pairs + kSortThreads - 1) / kSortThreads;
-    const int64_t per = (turns + kSortBlocks - 1) / kSortBlocks;
-    const int64_t blocks = per ? (turns + per - 1) / per : 1;
-    return {blocks, (per ? per : 1) * kSortThreads, pairs > kSortOne};
+    const int64_t per = turns ? (turns + kSortBlocks - 1) / kSortBlocks : 1;
+    const int64_t blocks = turns ? (turns + per - 1) / per : 1;
+    return {blocks, per * kSortThreads, pairs > kSortOne ? blocks * hist_stride(experts) : 0};
 }
 
 namespace {
@@ -418,10 +515,10 @@ bool sort_shape_ok(int64_t tokens, int64_t k, int64_t experts) {
 }  // namespace
 
 int sort_launch(const SortCall &c, hipStream_t stream) {
-    const SortPlan plan = sort_plan(c.pairs);
+    const SortPlan plan = sort_plan(c.pairs, c.experts);
     SortArgs a{};
     a.ids = static_cast<const uint32_t *>(c.ids);
-    a.hist = plan.counted ? c.work : nullptr;
+    a.hist = plan.words ? c.work : nullptr;
     a.offsets = c.offsets;
     a.sorted_ids = c.sorted_ids;
     a.tokens = c.tokens;
@@ -435,7 +532,7 @@ int sort_launch(const SortCall &c, hipStream_t stream) {
         hipLaunchKernelGGL(kernel, dim3{uint32_t(plan.blocks)}, dim3{kSortThreads}, 0, stream, a);
         return hipGetLastError();
     };
-    if (plan.counted) {
+    if (plan.words) {
         const hipError_t err = c.wide ? run(sort_count_kernel<true>) : run(sort_count_kernel<false>);
         if (err != hipSuccess) return record_launch(err);
     }
@@ -491,8 +588,7 @@ extern "C" {
 int64_t iqk_sort_work(int64_t n_tokens, int64_t pairs_per_token, int64_t num_experts) {
     using namespace iqk;
     if (!sort_shape_ok(n_tokens, pairs_per_token, num_experts)) return -1;
-    const SortPlan plan = sort_plan(n_tokens * pairs_per_token);
-    return plan.counted ? plan.blocks * (num_experts + 1) : 0;
+    return sort_plan(n_tokens * pairs_per_token, num_experts).words;
 }
 
 int iqk_sort(const void *ids, int wide_ids, int64_t n_tokens, int64_t pairs_per_token, int64_t num_experts,
@@ -500,7 +596,9 @@ int iqk_sort(const void *ids, int wide_ids, int64_t n_tokens, int64_t pairs_per_
     using namespace iqk;
     if (!sort_shape_ok(n_tokens, pairs_per_token, num_experts)) return IQK_ERR_GEOMETRY;
     if (!offsets || (n_tokens && (!ids || !sorted_ids || !tokens || !slots))) return IQK_ERR_ARGUMENT;
-    if (sort_plan(n_tokens * pairs_per_token).counted && !work) return IQK_ERR_ARGUMENT;
+    if (sort_plan(n_tokens * pairs_per_token, num_experts).words &&
+        (!work || (reinterpret_cast<uintptr_t>(work) & 15u)))
+        return IQK_ERR_ARGUMENT;
     SortCall c{};
     c.ids = ids;
     c.wide = wide_ids != 0;
@@ -528,7 +626,10 @@ int iqk_dispatch(int dtype, const void *x, const int32_t *slots, const int32_t *
     a.kept = kept;
     a.out = static_cast<uint8_t *>(rows);
     by_tokens(a, 256 >> a.log_width, a.columns, [&](const RowArgs &part, uint32_t blocks) {
-        hipLaunchKernelGGL(dispatch_kernel, dim3{blocks}, dim3{256}, 0, as_stream(stream), part);
+        if (part.log_width >= 6)
+            hipLaunchKernelGGL(dispatch_kernel<true>, dim3{blocks}, dim3{256}, 0, as_stream(stream), part);
+        else
+            hipLaunchKernelGGL(dispatch_kernel<false>, dim3{blocks}, dim3{256}, 0, as_stream(stream), part);
     });
     return record_launch(hipGetLastError());
 }
@@ -548,7 +649,11 @@ int iqk_combine(int dtype, const void *y, const int32_t *slots, const int32_t *k
     a.out = static_cast<uint8_t *>(out);
     by_dtype(dtype, [&](auto dt) {
         by_tokens(a, 256 >> a.log_width, a.columns, [&](const RowArgs &part, uint32_t blocks) {
-            hipLaunchKernelGGL((combine_kernel<decltype(dt)::value>), dim3{blocks}, dim3{256}, 0, as_stream(stream), part);
+            constexpr int DT = decltype(dt)::value;
+            if (part.log_width >= 6)
+                hipLaunchKernelGGL((combine_kernel<DT, true>), dim3{blocks}, dim3{256}, 0, as_stream(stream), part);
+            else
+                hipLaunchKernelGGL((combine_kernel<DT, false>), dim3{blocks}, dim3{256}, 0, as_stream(stream), part);
         });
     });
     return record_launch(hipGetLastError());

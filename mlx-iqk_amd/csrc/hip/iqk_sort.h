@@ -9,13 +9,12 @@ namespace iqk {
 
 constexpr int64_t kSortMaxExperts = 1024;
 
-// How `pairs` pairs are sorted: by `blocks` workgroups of `share` pairs each, and whether a
-// launch before counts the shares, into a workspace of blocks * (experts + 1) words.
+// How pairs are sorted: by `blocks` workgroups of `share` pairs each; where a launch before
+// counts the shares, into a workspace of `words`, 16-byte aligned.
 struct SortPlan {
-    int64_t blocks, share;
-    bool counted;
+    int64_t blocks, share, words;
 };
-SortPlan sort_plan(int64_t pairs);
+SortPlan sort_plan(int64_t pairs, int64_t experts);
 
 // Pair p has the key ids[p / per_id], experts where that is outside [0, experts).
 struct SortCall {

@@ -48,7 +48,7 @@ HIP_SOURCES = {
     "iqk_mx_gemm.hip": (),
     "iqk_router.hip": (),
     "iqk_dispatch.hip": (),
-    "iqk_adapters.hip": (),
+    "iqk_adapters.hip": ("-mllvm", "-amdgpu-mfma-vgpr-form"),
 }
 OFFLOAD_ARCH = "gfx950"
 
