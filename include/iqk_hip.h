@@ -408,11 +408,12 @@ int iqk_combine_grad(int dtype, const void *dout, const void *y, const int32_t *
 
 // -- low-rank adapters ---------------------------------------------------------
 //
-// out[t] = y[t] + scales[a] up[a] (down[a] x[t]) with a = ids[t / rows_per_id]: down dtype (F16
-// or BF16) [num_adapters, rank, in_features], up [num_adapters, out_features, rank], both
-// 16-byte aligned, as work is; scales f32.  An id of -1 gives y[t], another outside the bank a row of NaN.
+// out[t] = y[t] + scales[a] B_a (A_a x[t]) with a = ids[t / rows_per_id], dtype F16 or BF16:
+// A_a [rank, in_features] in down [num_adapters, in_features / 8, rank, 8] (columns 8 c + i of
+// rank r at [c, r, i]), B_a [out_features, rank] in up [num_adapters, rank / 8, out_features, 8]
+// (rank 8 c + i of output n at [c, n, i]), both 16-byte aligned, as work is; scales f32.  An id of -1 gives y[t], another outside the bank a row of NaN.
 // f32 sums, one rounding.  out may be y.  ids: i32 or (wide_ids) i64.  work: iqk_adapters_work
-// words.  in_features and rank multiples of 8, rank <= 256, num_adapters <= 1024.
+// words (0: may be NULL).  in_features and rank multiples of 8, rank <= 256, num_adapters <= 1024.
 int64_t iqk_adapters_work(int64_t in_features, int64_t out_features, int64_t rank, int64_t num_adapters, int64_t rows);
 int iqk_adapters(int dtype, int64_t in_features, int64_t out_features, int64_t rank, int64_t num_adapters,
                  const void *x, int64_t rows, const void *ids, int wide_ids, int64_t rows_per_id, const void *down,

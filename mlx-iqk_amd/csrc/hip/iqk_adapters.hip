@@ -1,6 +1,8 @@
 // Low-rank adapters of many requests beside a shared projection (gfx950):
 //   out[t] = y[t] + s_a B_a (A_a x[t]),  a = ids[t],
-// A_a [rank, in], B_a [out, rank], 16-bit like x and y; an id of -1 leaves y[t], another one
+// A_a [rank, in], B_a [out, rank], 16-bit like x and y.  Both are kept with eight consecutive
+// values of their reduction axis together, so that lanes that take one rank or output each read
+// consecutive 16 bytes: down [in / 8][rank][8], up [rank / 8][out][8].  An id of -1 leaves y[t], another one
 // outside the bank gives a row of NaN.  Products are exact and summed in f32, A_a x and its
 // product with s_a stay in f32, and the sum with y is rounded once.
 
@@ -23,7 +25,6 @@ struct AdapterArgs {
     const uint32_t *ids;
     const uint16_t *down, *up;
     const float *scales;
-    float *t;                 // [T][rank]
     const uint16_t *y;
     uint16_t *out;
     uint32_t T, in, N, rank, adapters, wide, per_id;
@@ -31,9 +32,10 @@ struct AdapterArgs {
     const uint32_t *offs;     // first slots of each adapter, then of the rows without one
     const uint32_t *rows;     // [T] each slot's row
     uint4_t *tiles;           // adapter, first slot, slots
+    uint32_t *tile_rows;      // [tile][slots] their rows
     uint4_t *pieces;          // A x of a tile's slots, split, as operand B of the second product
     float *powers;            // [tile][slots] what the pieces are multiplied with
-    uint32_t chunks;          // operands B of a slot: of 32 ranks, a power of two of them
+    uint32_t columns;         // 256s of outputs of a workgroup
 };
 
 // The adapter of row t: the bank's size for none, more for one that does not exist.
@@ -61,52 +63,109 @@ __device__ __forceinline__ float float_of16(uint16_t h) {
     return BF ? __builtin_bit_cast(float, uint32_t(h) << 16) : half_bits_to_float(h);
 }
 
-// t[row][j] = s A_a[j] . x[row]: a wavefront each.
+// Two values in 16 bits.
 template <bool BF>
-__global__ __launch_bounds__(256) void adapter_down_kernel(AdapterArgs a) {
-    const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const uint32_t groups = (a.rank + 3) / 4, row = blockIdx.x / groups, j = blockIdx.x % groups * 4 + wave;
-    if (j >= a.rank) return;
-    const uint32_t id = adapter_of(a, row);
-    if (id >= a.adapters) return;
-    const uint16_t *const x = a.x + size_t(row) * a.in, *const w = a.down + (size_t(id) * a.rank + j) * a.in;
-    float sum = 0.f;
-    for (uint32_t c = 8 * lane; c < a.in; c += 512) {
-        const uint4_t xv = *reinterpret_cast<const chunk_t *>(x + c), wv = load_u4(w + c);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float2v_t p = floats<BF>(xv[i]), q = floats<BF>(wv[i]);
-            sum = fmaf(p.y, q.y, fmaf(p.x, q.x, sum));
-        }
-    }
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) sum += __shfl_xor(sum, off, 64);
-    if (lane == 0) a.t[size_t(row) * a.rank + j] = sum * a.scales[id];
+__device__ __forceinline__ uint32_t pair_bits(float lo, float hi) {
+    return BF ? bf16_bits(lo) | bf16_bits(hi) << 16 : float_to_half_bits(lo) | float_to_half_bits(hi) << 16;
 }
 
-// out[row][n] = y[row][n] + B_a[n] . t[row]: a thread each.
 template <bool BF>
-__global__ __launch_bounds__(256) void adapter_up_kernel(AdapterArgs a) {
-    const uint32_t groups = (a.N + 255) / 256, row = blockIdx.x / groups, n = blockIdx.x % groups * 256 + threadIdx.x;
-    if (n >= a.N) return;
-    const uint32_t id = adapter_of(a, row);
-    const size_t at = size_t(row) * a.N + n;
-    if (id >= a.adapters) {
-        a.out[at] = id == a.adapters ? a.y[at] : BF ? uint16_t(0x7fc0) : kHalfNaN;
+constexpr uint16_t kNaN16 = BF ? 0x7fc0 : kHalfNaN;
+
+// ------------------------------------------------------------- rows alone ---
+//
+// A workgroup computes A x of one row, then up to 1024 of its outputs, a thread each; that A x
+// is computed again in every 1024 outputs' workgroup costs less than a second launch (the
+// adapter comes from L2).  Of A's units of eight columns 16 lanes take 16 ranks each and a
+// wavefront four units at a time; B's and y's loads, which wait for nothing, are on their way from the start.
+constexpr int kAloneWaves = 16, kAloneThreads = 64 * kAloneWaves;
+
+// UP: eights of ranks whose B is loaded ahead (0: none).
+template <bool BF, int UP>
+__global__ __launch_bounds__(kAloneThreads) void adapter_row_kernel(AdapterArgs a) {
+    constexpr int GROUPS = 4, AHEAD = 4;  // groups of 16 ranks, and units, at once
+    __shared__ float part[kAloneWaves][kRankMax];
+    __shared__ __attribute__((aligned(16))) float t[kRankMax];
+    const uint32_t columns = (a.N + kAloneThreads - 1) / kAloneThreads, row = blockIdx.x / columns;
+    const uint32_t n = blockIdx.x % columns * kAloneThreads + threadIdx.x;
+    const uint32_t id = __builtin_amdgcn_readfirstlane(adapter_of(a, row));
+    const size_t at = size_t(row) * a.N + min(n, a.N - 1u);
+    const uint16_t old = a.y[at];
+    if (id >= a.adapters) {  // uniform
+        if (n < a.N) a.out[at] = id == a.adapters ? old : kNaN16<BF>;
         return;
     }
-    const uint16_t *const w = a.up + (size_t(id) * a.N + n) * a.rank;
-    const float *const t = a.t + size_t(row) * a.rank;
-    float sum = 0.f;
-    for (uint32_t c = 0; c < a.rank; c += 8) {
-        const uint4_t wv = load_u4(w + c);
+    const uint32_t eights = a.rank / 8, units = a.in / 8;
+    const uint16_t *const up = a.up + (size_t(id) * eights * a.N + min(n, a.N - 1u)) * 8;
+    uint4_t ahead[UP ? UP : 1];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float2v_t q = floats<BF>(wv[i]);
-            sum = fmaf(t[c + 2 * i + 1], q.y, fmaf(t[c + 2 * i], q.x, sum));
+    for (int i = 0; i < UP; ++i) ahead[i] = load_u4(up + size_t(min(uint32_t(i), eights - 1u)) * a.N * 8);
+    const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint16_t *const x = a.x + size_t(row) * a.in, *const down = a.down + size_t(id) * units * a.rank * 8;
+    for (uint32_t r0 = 0; r0 < a.rank; r0 += 16 * GROUPS) {
+        const uint32_t r = r0 + (lane & 15u);
+        float sum[GROUPS] = {};
+        for (uint32_t c0 = 4 * wave + (lane >> 4); c0 < units + (lane >> 4); c0 += 4 * kAloneWaves * AHEAD) {
+            uint4_t xv[AHEAD], wv[AHEAD][GROUPS];
+#pragma unroll
+            for (int i = 0; i < AHEAD; ++i) {
+                const uint32_t c = min(c0 + 4 * kAloneWaves * i, units - 1u);
+                xv[i] = *reinterpret_cast<const chunk_t *>(x + 8 * size_t(c));
+#pragma unroll
+                for (int q = 0; q < GROUPS; ++q)
+                    if (r0 + 16 * q < a.rank)  // uniform
+                        wv[i][q] = load_u4(down + (size_t(c) * a.rank + min(r + 16 * q, a.rank - 1u)) * 8);
+            }
+#pragma unroll
+            for (int i = 0; i < AHEAD; ++i) {
+                if (c0 + 4 * kAloneWaves * i >= units) continue;
+#pragma unroll
+                for (int q = 0; q < GROUPS; ++q) {
+                    if (r0 + 16 * q >= a.rank) continue;
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const float2v_t p = floats<BF>(xv[i][k]), w = floats<BF>(wv[i][q][k]);
+                        sum[q] = fmaf(p.y, w.y, fmaf(p.x, w.x, sum[q]));
+                    }
+                }
+            }
+        }
+#pragma unroll
+        for (int q = 0; q < GROUPS; ++q) {
+            if (r0 + 16 * q >= a.rank) continue;
+            sum[q] += __shfl_xor(sum[q], 16, 64);
+            sum[q] += __shfl_xor(sum[q], 32, 64);
+            if (lane < 16 && r + 16 * q < a.rank) part[wave][r + 16 * q] = sum[q];
         }
     }
-    sum += float_of16<BF>(a.y[at]);
+    __syncthreads();
+    if (threadIdx.x < a.rank) {
+        float sum = 0.f;
+#pragma unroll
+        for (int w = 0; w < kAloneWaves; ++w) sum += part[w][threadIdx.x];
+        t[threadIdx.x] = sum * a.scales[id];
+    }
+    __syncthreads();
+    if (n >= a.N) return;
+    float sum = 0.f;
+    const auto add = [&](uint4_t w, uint32_t i) {
+        const float4_t lo = *reinterpret_cast<const float4_t *>(&t[8 * i]), hi = *reinterpret_cast<const float4_t *>(&t[8 * i + 4]);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const float2v_t b = floats<BF>(w[k]);
+            const float t0 = k < 2 ? lo[2 * k] : hi[2 * k - 4], t1 = k < 2 ? lo[2 * k + 1] : hi[2 * k - 3];
+            sum = fmaf(t1, b.y, fmaf(t0, b.x, sum));
+        }
+    };
+    if constexpr (UP > 0) {
+#pragma unroll
+        for (int i = 0; i < UP; ++i)
+            if (uint32_t(i) < eights) add(ahead[i], i);
+    } else {
+#pragma unroll 8
+        for (uint32_t i = 0; i < eights; ++i) add(load_u4(up + size_t(i) * a.N * 8), i);
+    }
+    sum += float_of16<BF>(old);
     a.out[at] = uint16_t(BF ? bf16_bits(sum) : float_to_half_bits(sum));
 }
 
@@ -176,75 +235,112 @@ __device__ __forceinline__ Tile find_tile(const AdapterArgs &a, uint32_t t, uint
     return {found[0], found[1], found[2]};
 }
 
-// A x of 16 CT slots of a tile: WAVES wavefronts take 32 KH columns in turn, DEPTH such steps on
-// their way at once, and their sums meet in LDS.
-template <bool BF, int RT, int CT, int WAVES, int KH, int DEPTH>
+// Lanes of a wavefront read what others of it wrote to LDS.
+__device__ __forceinline__ void wavefront_fence() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
+// A x of 16 CT slots of a tile.  WAVES wavefronts take 64 columns in turn and their sums meet in
+// LDS.  A wavefront reads 128 bytes of a row together and turns them into operand B in its
+// own part of LDS (rows read as the operand wants them, 16 of them 64 bytes each in an
+// instruction, kept the loads waiting for the cache: 8192 rows of 4096, rank 16, 34 us);
+// XD steps of x and AD of A are on their way at once.
+template <bool BF, int RT, int CT, int WAVES, int XD, int AD>
 __global__ __launch_bounds__(64 * WAVES) void adapter_down_tiles_kernel(AdapterArgs a) {
     constexpr int SLOTS = 16 * CT, RANKS = 16 * RT, THREADS = 64 * WAVES, KC = (RT + 1) / 2, PARTS = kTileGroups / CT;
-    __shared__ float part[WAVES][SLOTS][RANKS + 4];
+    constexpr int SUMS = SLOTS * (RANKS + 4), STAGE = SLOTS * 32;  // floats of a wavefront's sums, of its turned rows
+    __shared__ __attribute__((aligned(16))) float shared[WAVES][SUMS > STAGE ? SUMS : STAGE];
     __shared__ uint32_t sums[WAVES], found[3];
     const uint32_t t = blockIdx.x / PARTS, group = blockIdx.x % PARTS * CT;  // the first of its groups of 16
     Tile tile = find_tile<THREADS>(a, t, sums, found);
     if (threadIdx.x == 0 && group == 0) a.tiles[t] = uint4_t{tile.adapter, tile.first, tile.slots, 0};
-    if (tile.slots <= 16 * group || tile.adapter >= a.adapters) return;  // uniform
+    if (tile.slots <= 16 * group) return;  // uniform
     tile.first += 16 * group;
     tile.slots = min(tile.slots - 16 * group, uint32_t(SLOTS));
-    const uint32_t lane = threadIdx.x & 63u, g = lane >> 4, m = lane & 15u;
+    if (threadIdx.x < SLOTS)
+        a.tile_rows[t * kTileSlots + 16 * group + threadIdx.x] = a.rows[tile.first + min(threadIdx.x, tile.slots - 1u)];
+    if (tile.adapter >= a.adapters) return;  // uniform
+    const uint32_t lane = threadIdx.x & 63u, g = lane >> 4, m = lane & 15u, c8 = lane & 7u, r8 = lane >> 3;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const uint16_t *w[RT], *x[CT];
+    const uint16_t *w[RT], *x[2 * CT];
 #pragma unroll
     for (int r = 0; r < RT; ++r)  // ranks past the last: it again, its sums not used
-        w[r] = a.down + (size_t(tile.adapter) * a.rank + min(16u * r + m, a.rank - 1u)) * a.in;
+        w[r] = a.down + size_t(tile.adapter) * a.rank * a.in + 8 * min(16u * r + m, a.rank - 1u);
 #pragma unroll
-    for (int c = 0; c < CT; ++c) x[c] = a.x + size_t(a.rows[tile.first + min(16u * c + m, tile.slots - 1u)]) * a.in;
+    for (int c = 0; c < 2 * CT; ++c) x[c] = a.x + size_t(a.rows[tile.first + min(8u * c + r8, tile.slots - 1u)]) * a.in;
     float4_t acc[RT][CT];
 #pragma unroll
     for (int r = 0; r < RT; ++r)
 #pragma unroll
         for (int c = 0; c < CT; ++c) acc[r][c] = float4_t{0, 0, 0, 0};
-    uint4_t xv[DEPTH][KH][CT], wv[DEPTH][KH][RT];
-    constexpr uint32_t STEP = 32 * KH * WAVES;
-    const auto load = [&](int d, uint32_t k0) {
+    uint4_t xv[XD][2 * CT], wv[AD][2][RT];
+    constexpr uint32_t STEP = 64 * WAVES;
+    uint4_t *const turned = reinterpret_cast<uint4_t *>(shared[wave]);  // [slot][8 chunks], chunk c at c ^ slot % 8
+    const auto load_x = [&](int d, uint32_t k0) {
+        const uint32_t k = k0 + 8 * c8, at = k < a.in ? k : 0u;
 #pragma unroll
-        for (int h = 0; h < KH; ++h) {
-            const uint32_t k = k0 + 32 * h + 8 * g;
-            const bool in = k < a.in;
-            const uint32_t at = in ? k : 0u;
+        for (int c = 0; c < 2 * CT; ++c) xv[d][c] = *reinterpret_cast<const chunk_t *>(x[c] + at);
+    };
+    const auto load_w = [&](int d, uint32_t k0) {
 #pragma unroll
-            for (int c = 0; c < CT; ++c) xv[d][h][c] = *reinterpret_cast<const chunk_t *>(x[c] + at);
+        for (int h = 0; h < 2; ++h) {
+            const uint32_t k = k0 + 32 * h + 8 * g, at = k < a.in ? k : 0u;
 #pragma unroll
-            for (int r = 0; r < RT; ++r) wv[d][h][r] = load_u4(w[r] + at);
+            for (int r = 0; r < RT; ++r) wv[d][h][r] = load_u4(w[r] + size_t(at) * a.rank);
         }
     };
-    const auto multiply = [&](int d, uint32_t k0) {
+    const auto multiply = [&](int xd, int ad, uint32_t k0) {
+        const bool rest = k0 + 64 > a.in;  // uniform: columns past the row, zeros on both sides
+        wavefront_fence();
 #pragma unroll
-        for (int h = 0; h < KH; ++h) {
-            if (k0 + 32 * h + 32 > a.in && k0 + 32 * h + 8 * g >= a.in) {  // past the row: zeros on both sides
+        for (int c = 0; c < 2 * CT; ++c) {
+            if (rest && k0 + 8 * c8 >= a.in) xv[xd][c] = uint4_t{0, 0, 0, 0};
+            turned[(8 * c + r8) * 8 + (c8 ^ r8)] = xv[xd][c];
+        }
+        wavefront_fence();
 #pragma unroll
-                for (int c = 0; c < CT; ++c) xv[d][h][c] = uint4_t{0, 0, 0, 0};
+        for (int h = 0; h < 2; ++h) {
+            uint4_t b[CT];
 #pragma unroll
-                for (int r = 0; r < RT; ++r) wv[d][h][r] = uint4_t{0, 0, 0, 0};
+            for (int c = 0; c < CT; ++c) b[c] = turned[(16 * c + m) * 8 + ((4 * h + g) ^ (m & 7u))];
+            if (rest && k0 + 32 * h + 8 * g >= a.in) {
+#pragma unroll
+                for (int r = 0; r < RT; ++r) wv[ad][h][r] = uint4_t{0, 0, 0, 0};
             }
 #pragma unroll
             for (int r = 0; r < RT; ++r)
 #pragma unroll
-                for (int c = 0; c < CT; ++c) acc[r][c] = mfma<BF>(wv[d][h][r], xv[d][h][c], acc[r][c]);
+                for (int c = 0; c < CT; ++c) acc[r][c] = mfma<BF>(wv[ad][h][r], b[c], acc[r][c]);
         }
     };
-    uint32_t k0 = 32 * KH * wave;
+    constexpr int UNROLL = XD > AD ? XD : AD;
+    static_assert(UNROLL % XD == 0 && UNROLL % AD == 0, "a turn of the loop is whole turns of both rings");
+    // Each workgroup begins at another step: in step with each other they would all read the same
+    // eighth of rows that lie a power of two apart, from few of the memory's channels.
+    const uint32_t steps = (a.in + STEP - 1) / STEP, turn = blockIdx.x % steps;
+    const auto column = [&](uint32_t i) { return 64 * wave + STEP * (i + turn < steps ? i + turn : i + turn - steps); };
 #pragma unroll
-    for (int d = 0; d < DEPTH - 1; ++d) load(d, k0 + d * STEP);
-    for (; k0 < a.in; k0 += DEPTH * STEP) {
+    for (int d = 0; d < UNROLL - 1; ++d) {  // the oldest step's loads first
+        if (d < XD - 1) load_x(d, column(min(uint32_t(d), steps - 1u)));
+        if (d < AD - 1) load_w(d, column(min(uint32_t(d), steps - 1u)));
+        __builtin_amdgcn_sched_barrier(0);
+    }
+    for (uint32_t i0 = 0; i0 < steps; i0 += UNROLL) {
 #pragma unroll
-        for (int d = 0; d < DEPTH; ++d) {
-            load((d + DEPTH - 1) % DEPTH, k0 + (d + DEPTH - 1) * STEP);
-            if (k0 + d * STEP < a.in) multiply(d, k0 + d * STEP);  // uniform
+        for (int d = 0; d < UNROLL; ++d) {
+            load_x((d + XD - 1) % XD, column(min(i0 + d + XD - 1, steps - 1u)));
+            load_w((d + AD - 1) % AD, column(min(i0 + d + AD - 1, steps - 1u)));
+            __builtin_amdgcn_sched_barrier(0);
+            if (i0 + d < steps && column(i0 + d) < a.in) multiply(d % XD, d % AD, column(i0 + d));  // uniform
         }
     }
+    wavefront_fence();
+    const auto part = [&](uint32_t w, uint32_t slot, uint32_t rank) -> float & { return shared[w][slot * (RANKS + 4) + rank]; };
 #pragma unroll
     for (int r = 0; r < RT; ++r)
 #pragma unroll
-        for (int c = 0; c < CT; ++c) *reinterpret_cast<float4_t *>(&part[wave][16 * c + m][16 * r + 4 * g]) = acc[r][c];
+        for (int c = 0; c < CT; ++c) *reinterpret_cast<float4_t *>(&part(wave, 16 * c + m, 16 * r + 4 * g)) = acc[r][c];
     __syncthreads();
     const float scale = a.scales[tile.adapter];
     constexpr int UNITS = 4 * KC;  // eights of a slot's ranks, rounded up to whole operands
@@ -257,7 +353,7 @@ __global__ __launch_bounds__(64 * WAVES) void adapter_down_tiles_kernel(AdapterA
 #pragma unroll
             for (int k = 0; k < WAVES; ++k)
 #pragma unroll
-                for (int i = 0; i < 8; ++i) v[i] += part[k][slot][r0 + i];
+                for (int i = 0; i < 8; ++i) v[i] += part(k, slot, r0 + i);
 #pragma unroll
             for (int i = 0; i < 8; ++i) v[i] *= scale;
         }
@@ -304,133 +400,162 @@ __global__ __launch_bounds__(64 * WAVES) void adapter_down_tiles_kernel(AdapterA
     }
 }
 
-// Two outputs in 16 bits.
-template <bool BF>
-__device__ __forceinline__ uint32_t pair_bits(float lo, float hi) {
-    return BF ? bf16_bits(lo) | bf16_bits(hi) << 16 : float_to_half_bits(lo) | float_to_half_bits(hi) << 16;
-}
-
-// 256 outputs of a tile: a wavefront takes 64 of them for all slots, lane 16 g + n sixteen
-// consecutive ones (16 g ..) of slot n of each group, so that y is read and written 32 bytes a
-// lane.  The slots' operands go through LDS, which all four wavefronts read.
-template <bool BF>
+// Outputs of a tile: 256 at a time, of which a wavefront takes 64 for all slots, the next 256's
+// y and B on their way meanwhile.  The slots' operands lie in LDS for all of them (KC chunks of
+// 32 ranks), and the sums go through it: the matrix cores leave four outputs of 16 slots to
+// 64 lanes, memory wants 64 outputs of a slot together.
+template <bool BF, int KC>
 __global__ __launch_bounds__(256) void adapter_up_tiles_kernel(AdapterArgs a) {
-    constexpr int P = kPieces<BF>, CT = kTileGroups, STAGE = 2;  // chunks of 32 ranks in LDS at once
-    __shared__ uint4_t operands[STAGE][CT][P][64];
-    const uint32_t columns = (a.N + 255) / 256, t = blockIdx.x / columns;
-    const uint32_t lane = threadIdx.x & 63u, g = lane >> 4, m = lane & 15u;
+    constexpr int P = kPieces<BF>, CT = kTileGroups, STAGE = KC < 2 ? KC : 2;  // chunks of B in registers at once
+    constexpr bool AHEAD = KC <= 2;  // of B; y always is
+    __shared__ uint4_t operands[CT][KC][P][64];
+    __shared__ __attribute__((aligned(16))) float turned[4][16][64 + 4];
+    const uint32_t groups = (a.N + 256 * a.columns - 1) / (256 * a.columns), t = blockIdx.x / groups;
+    const uint32_t lane = threadIdx.x & 63u, g = lane >> 4, m = lane & 15u, s8 = lane >> 3;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const uint32_t n0 = blockIdx.x % columns * 256 + 64 * wave;
+    const uint32_t begin = blockIdx.x % groups * 256 * a.columns, end = min(a.N, begin + 256 * a.columns);
     const uint4_t tile = a.tiles[t];
-    const uint32_t adapter = tile.x, first = tile.y, slots = tile.z;
+    const uint32_t adapter = tile.x, slots = tile.z;
     if (slots == 0) return;  // uniform
-    const uint32_t mine = n0 + 16 * g;  // the lane's first output
-    const uint32_t have = mine < a.N ? min(a.N - mine, 16u) : 0u;
-    size_t at[CT];
-    uint32_t row[CT];
-    uint4_t y[CT][2];
+    uint32_t row[CT][2];  // a lane's outputs are of slots s8 and s8 + 8 of each group
 #pragma unroll
-    for (int c = 0; c < CT; ++c) {
-        row[c] = a.rows[first + min(16u * c + m, slots - 1u)];
-        at[c] = size_t(row[c]) * a.N + mine;
-        y[c][0] = y[c][1] = uint4_t{0, 0, 0, 0};
-        if (have == 16 && 16u * c < slots) {
-            y[c][0] = *reinterpret_cast<const chunk_t *>(a.y + at[c]);
-            y[c][1] = *reinterpret_cast<const chunk_t *>(a.y + at[c] + 8);
-        }
-    }
+    for (int c = 0; c < CT; ++c)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) row[c][h] = a.tile_rows[t * kTileSlots + min(16u * c + 8 * h + s8, slots - 1u)];
+    const uint32_t mine = 8 * (lane & 7u);
     if (adapter >= a.adapters) {  // rows without an adapter; uniform
+        for (uint32_t n0 = begin + 64 * wave; n0 < end; n0 += 256) {
+            const uint32_t n = n0 + mine, have = n < a.N ? min(a.N - n, 8u) : 0u;
 #pragma unroll
-        for (int c = 0; c < CT; ++c) {
-            if (16 * c + m >= slots) continue;
-            const bool bare = adapter_of(a, row[c]) == a.adapters;
-            const uint32_t nan = BF ? 0x7fc07fc0u : 0x7e007e00u;
-            if (have == 16) {
+            for (int c = 0; c < CT; ++c)
 #pragma unroll
-                for (int h = 0; h < 2; ++h)
-                    *reinterpret_cast<chunk_t *>(a.out + at[c] + 8 * h) = bare ? y[c][h] : uint4_t{nan, nan, nan, nan};
-            } else {
-                for (uint32_t i = 0; i < have; ++i) a.out[at[c] + i] = bare ? a.y[at[c] + i] : uint16_t(nan);
-            }
+                for (int h = 0; h < 2; ++h) {
+                    if (16u * c + 8 * h + s8 >= slots) continue;
+                    const size_t at = size_t(row[c][h]) * a.N + n;
+                    const bool bare = adapter_of(a, row[c][h]) == a.adapters;
+                    const uint32_t nan = kNaN16<BF> * 0x10001u;
+                    if (have == 8)
+                        *reinterpret_cast<chunk_t *>(a.out + at) =
+                            bare ? uint4_t(*reinterpret_cast<const chunk_t *>(a.y + at)) : uint4_t{nan, nan, nan, nan};
+                    else
+                        for (uint32_t i = 0; i < have; ++i) a.out[at + i] = bare ? a.y[at + i] : kNaN16<BF>;
+                }
         }
         return;
     }
-    // operand A's row m of tile j is output 16 (m / 4) + 4 j + m % 4
-    const uint16_t *w[4];
+    const uint16_t *const up = a.up + size_t(adapter) * a.rank * a.N;
+    uint4_t y[2][CT][2], w[AHEAD ? 2 : 1][STAGE][4];
+    const auto load_y = [&](int d, uint32_t n0) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-        w[j] = a.up + (size_t(adapter) * a.N + min(n0 + 16 * (m >> 2) + 4 * j + (m & 3u), a.N - 1u)) * a.rank;
-    float4_t acc[4][CT];
+        for (int c = 0; c < CT; ++c) {
+            if (16u * c >= slots) continue;  // uniform
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-#pragma unroll
-        for (int c = 0; c < CT; ++c) acc[j][c] = float4_t{0, 0, 0, 0};
-    for (uint32_t k0 = 0; k0 < a.rank; k0 += 32 * STAGE) {
-        uint4_t wv[STAGE][4];
+            for (int h = 0; h < 2; ++h)
+                if (n0 + mine + 8 <= a.N) y[d][c][h] = *reinterpret_cast<const chunk_t *>(a.y + size_t(row[c][h]) * a.N + n0 + mine);
+        }
+    };
+    const auto load_w = [&](int d, uint32_t n0, uint32_t k0) {
 #pragma unroll
         for (int s = 0; s < STAGE; ++s) {
-            const uint32_t k = k0 + 32 * s + 8 * g;
+            const uint32_t k = k0 + 32 * s + 8 * g, eight = min(k / 8, a.rank / 8 - 1u);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) w[d][s][j] = load_u4(up + (size_t(eight) * a.N + min(n0 + 16 * j + m, a.N - 1u)) * 8);
+        }
+    };
+    // tiles begin at different columns, as their A x does
+    const uint32_t turns = (end - begin + 255) / 256, turn = t % turns;
+    const auto column = [&](uint32_t i) { return begin + 64 * wave + 256 * (i + turn < turns ? i + turn : i + turn - turns); };
+    load_y(0, column(0));
+    if (AHEAD) load_w(0, column(0), 0);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int i = 0; i < CT * KC * P * 64 / 256; ++i) {  // a group's operands lie together
+        const uint32_t u = 256 * i + threadIdx.x;
+        if (16 * (u / (KC * P * 64)) < slots) (&operands[0][0][0][0])[u] = a.pieces[size_t(t) * CT * KC * P * 64 + u];
+    }
+    __syncthreads();
+    float power[CT];
+#pragma unroll
+    for (int c = 0; c < CT; ++c) power[c] = BF || 16u * c >= slots ? 1.f : a.powers[size_t(t) * kTileSlots + 16 * c + m];
+    const auto compute = [&](int d, uint32_t n0) {
+        const uint32_t n = n0 + mine, have = n < a.N ? min(a.N - n, 8u) : 0u;
+        if constexpr (AHEAD) {  // past the ranks: zeros, as in the slots' operands
+#pragma unroll
+            for (int s = 0; s < STAGE; ++s)
+                if (32 * s + 8 * g >= a.rank) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) w[d][s][j] = uint4_t{0, 0, 0, 0};
+                }
+        }
+#pragma unroll
+        for (int c = 0; c < CT; ++c) {
+            if (16u * c >= slots) continue;  // uniform
+            float4_t acc[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) acc[j] = float4_t{0, 0, 0, 0};
+#pragma unroll
+            for (int k0 = 0; k0 < 32 * KC; k0 += 32 * STAGE) {
+                if (k0 && uint32_t(k0) >= a.rank) continue;  // uniform
+                if constexpr (!AHEAD) {
+                    load_w(0, n0, k0);
+#pragma unroll
+                    for (int s = 0; s < STAGE; ++s)
+                        if (k0 + 32 * s + 8 * g >= a.rank) {
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) w[0][s][j] = uint4_t{0, 0, 0, 0};
+                        }
+                }
+#pragma unroll
+                for (int s = 0; s < STAGE; ++s)
+#pragma unroll
+                    for (int p = P - 1; p >= 0; --p) {  // the small pieces first
+                        const uint4_t b = operands[c][k0 / 32 + s][p][lane];
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) acc[j] = mfma<BF>(w[AHEAD ? d : 0][s][j], b, acc[j]);
+                    }
+            }
+            wavefront_fence();
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                wv[s][j] = uint4_t{0, 0, 0, 0};
-                if (k < a.rank) wv[s][j] = load_u4(w[j] + k);
+                float4_t v = acc[j];
+                if constexpr (!BF) v *= power[c];
+                *reinterpret_cast<float4_t *>(&turned[wave][m][16 * j + 4 * g]) = v;
             }
-        }
-        if (k0) __syncthreads();  // the stage before has been read
-#pragma unroll
-        for (int s = 0; s < STAGE; ++s) {
-            if (k0 + 32 * s >= a.rank) continue;  // uniform
-#pragma unroll
-            for (int i = 0; i < (CT * P * 64) / 256; ++i) {  // a group's pieces of a chunk lie together
-                const uint32_t u = 256 * i + threadIdx.x, c = u / (P * 64), rest = u % (P * 64);
-                const size_t from = ((size_t(t) * CT + c) * a.chunks + k0 / 32 + s) * P * 64 + rest;
-                if (16 * c < slots) operands[s][c][rest / 64][rest % 64] = a.pieces[from];
-            }
-        }
-        __syncthreads();
-#pragma unroll
-        for (int s = 0; s < STAGE; ++s) {
-            if (k0 + 32 * s >= a.rank) continue;  // uniform
-#pragma unroll
-            for (int c = 0; c < CT; ++c) {
-                if (16u * c >= slots) continue;  // uniform
-#pragma unroll
-                for (int p = P - 1; p >= 0; --p) {  // the small pieces first
-                    const uint4_t b = operands[s][c][p][lane];
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) acc[j][c] = mfma<BF>(wv[s][j], b, acc[j][c]);
-                }
-            }
-        }
-    }
-#pragma unroll
-    for (int c = 0; c < CT; ++c) {
-        if (16 * c + m >= slots) continue;
-        const float power = BF ? 1.f : a.powers[size_t(t) * kTileSlots + 16 * c + m];
-        float v[16];
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) v[4 * j + i] = BF ? acc[j][c][i] : acc[j][c][i] * power;
-        if (have == 16) {
+            wavefront_fence();
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                uint4_t out;
+                if (16u * c + 8 * h + s8 >= slots) continue;
+                const float *const v = &turned[wave][8 * h + s8][mine];
+                const size_t at = size_t(row[c][h]) * a.N + n;
+                if (have == 8) {
+                    const float4_t lo = *reinterpret_cast<const float4_t *>(v), hi = *reinterpret_cast<const float4_t *>(v + 4);
+                    uint4_t out;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const uint32_t word = y[c][h][i];
-                    const float2v_t old = floats<BF>(word);
-                    out[i] = pair_bits<BF>(old.x + v[8 * h + 2 * i], old.y + v[8 * h + 2 * i + 1]);
+                    for (int i = 0; i < 4; ++i) {
+                        const float2v_t old = floats<BF>(y[d][c][h][i]);
+                        const float v0 = i < 2 ? lo[2 * i] : hi[2 * i - 4], v1 = i < 2 ? lo[2 * i + 1] : hi[2 * i - 3];
+                        out[i] = pair_bits<BF>(old.x + v0, old.y + v1);
+                    }
+                    *reinterpret_cast<chunk_t *>(a.out + at) = out;
+                } else {
+                    for (uint32_t i = 0; i < have; ++i) {
+                        const float sum = float_of16<BF>(a.y[at + i]) + v[i];
+                        a.out[at + i] = uint16_t(BF ? bf16_bits(sum) : float_to_half_bits(sum));
+                    }
                 }
-                *reinterpret_cast<chunk_t *>(a.out + at[c] + 8 * h) = out;
             }
-        } else {
+        }
+    };
+    for (uint32_t i = 0; i < turns; i += 2) {
 #pragma unroll
-            for (uint32_t i = 0; i < 16; ++i) {
-                if (i >= have) continue;
-                const float sum = float_of16<BF>(a.y[at[c] + i]) + v[i];
-                a.out[at[c] + i] = uint16_t(BF ? bf16_bits(sum) : float_to_half_bits(sum));
+        for (int d = 0; d < 2; ++d) {
+            if (i + d >= turns) break;  // uniform
+            if (i + d + 1 < turns) {
+                load_y(1 - d, column(i + d + 1));
+                if (AHEAD) load_w(1 - d, column(i + d + 1), 0);
             }
+            __builtin_amdgcn_sched_barrier(0);
+            compute(d, column(i + d));
         }
     }
 }
@@ -447,7 +572,7 @@ constexpr int64_t kRowsAlone = 64;  // rows up to which each is computed on its 
 
 // The grouped form's workspace, in words: where each part begins.
 struct GroupPlan {
-    int64_t tiles, chunks, hist, offs, rows, desc, pieces, powers, words;
+    int64_t tiles, chunks, hist, offs, rows, desc, tile_rows, pieces, powers, words;
 };
 
 GroupPlan group_plan(int64_t rank, int64_t adapters, int64_t rows) {
@@ -465,50 +590,60 @@ GroupPlan group_plan(int64_t rank, int64_t adapters, int64_t rows) {
     p.offs = take(adapters + 1);
     p.rows = take(rows);
     p.desc = take(4 * p.tiles);
+    p.tile_rows = take(p.tiles * kTileSlots);
     p.pieces = take(p.tiles * kTileGroups * p.chunks * 3 * 64 * 4);
     p.powers = take(p.tiles * kTileSlots);
     return p;
 }
 
-// f(16s of ranks, groups of slots, wavefronts, 32s of columns a step, steps on their way)
+// f(16s of ranks, groups of slots, wavefronts, steps of x and of A on their way)
 template <typename F>
 void by_ranks(int64_t rank, F &&f) {
     using std::integer_sequence;
     if (rank <= 16)
-        f(integer_sequence<int, 1, 2, 8, 2, 4>{});
+        f(integer_sequence<int, 1, 2, 8, 4, 4>{});
     else if (rank <= 32)
-        f(integer_sequence<int, 2, 2, 8, 2, 4>{});
+        f(integer_sequence<int, 2, 2, 8, 4, 2>{});
     else if (rank <= 64)
-        f(integer_sequence<int, 4, 2, 8, 2, 2>{});
+        f(integer_sequence<int, 4, 2, 8, 4, 2>{});
     else if (rank <= 128)
-        f(integer_sequence<int, 8, 2, 4, 1, 2>{});
+        f(integer_sequence<int, 8, 2, 4, 2, 1>{});
     else
-        f(integer_sequence<int, 16, 1, 4, 1, 2>{});
+        f(integer_sequence<int, 16, 1, 4, 2, 1>{});
 }
 
-template <bool BF, int RT, int CT, int WAVES, int KH, int DEPTH>
-void launch_down(const AdapterArgs &a, int64_t tiles, hipStream_t stream, std::integer_sequence<int, RT, CT, WAVES, KH, DEPTH>) {
-    hipLaunchKernelGGL((adapter_down_tiles_kernel<BF, RT, CT, WAVES, KH, DEPTH>), dim3{uint32_t(tiles * (kTileGroups / CT))},
-                       dim3{64 * WAVES}, 0, stream, a);
+template <bool BF, int RT, int CT, int WAVES, int XD, int AD>
+hipError_t launch_tiles(const AdapterArgs &a, int64_t tiles, hipStream_t stream,
+                        std::integer_sequence<int, RT, CT, WAVES, XD, AD>) {
+    const int64_t ups = tiles * ((int64_t(a.N) + 256 * a.columns - 1) / (256 * a.columns));
+    hipLaunchKernelGGL((adapter_down_tiles_kernel<BF, RT, CT, WAVES, XD, AD>),
+                       dim3{uint32_t(tiles * (kTileGroups / CT))}, dim3{64 * WAVES}, 0, stream, a);
+    if (const hipError_t err = hipGetLastError(); err != hipSuccess) return err;
+    hipLaunchKernelGGL((adapter_up_tiles_kernel<BF, (RT + 1) / 2>), dim3{uint32_t(ups)}, dim3{256}, 0, stream, a);
+    return hipGetLastError();
 }
 
 int rows_alone(const AdapterArgs &a, bool bf, hipStream_t stream) {
-    const int64_t downs = int64_t(a.T) * ((a.rank + 3) / 4), ups = int64_t(a.T) * ((int64_t(a.N) + 255) / 256);
-    if (!grid_ok(downs, 256) || !grid_ok(ups, 256)) return IQK_ERR_GEOMETRY;
-    const auto run = [&](auto kernel, int64_t blocks) {
-        hipLaunchKernelGGL(kernel, dim3{uint32_t(blocks)}, dim3{256}, 0, stream, a);
-        return hipGetLastError();
+    const int64_t blocks = int64_t(a.T) * ((int64_t(a.N) + kAloneThreads - 1) / kAloneThreads);
+    if (!grid_ok(blocks, kAloneThreads)) return IQK_ERR_GEOMETRY;
+    const auto run = [&](auto kernel) {
+        hipLaunchKernelGGL(kernel, dim3{uint32_t(blocks)}, dim3{kAloneThreads}, 0, stream, a);
     };
-    if (const hipError_t err = bf ? run(adapter_down_kernel<true>, downs) : run(adapter_down_kernel<false>, downs);
-        err != hipSuccess)
-        return record_launch(err);
-    return record_launch(bf ? run(adapter_up_kernel<true>, ups) : run(adapter_up_kernel<false>, ups));
+    if (a.rank <= 16)
+        bf ? run(adapter_row_kernel<true, 2>) : run(adapter_row_kernel<false, 2>);
+    else if (a.rank <= 32)
+        bf ? run(adapter_row_kernel<true, 4>) : run(adapter_row_kernel<false, 4>);
+    else
+        bf ? run(adapter_row_kernel<true, 0>) : run(adapter_row_kernel<false, 0>);
+    return record_launch(hipGetLastError());
 }
 
 int rows_grouped(AdapterArgs a, bool bf, uint32_t *work, hipStream_t stream) {
     const GroupPlan p = group_plan(a.rank, a.adapters, a.T);
-    const int64_t ups = p.tiles * ((int64_t(a.N) + 255) / 256);
-    if (!grid_ok(ups, 256) || !grid_ok(p.tiles * kTileGroups, 512)) return IQK_ERR_GEOMETRY;
+    // workgroups of up to 8 x 256 outputs, about two a CU
+    const int64_t wide = (int64_t(a.N) + 255) / 256, each = p.tiles * wide / 512;
+    a.columns = uint32_t(each < 1 ? 1 : each > 8 ? 8 : each);
+    if (!grid_ok(p.tiles * wide, 256) || !grid_ok(p.tiles * kTileGroups, 512)) return IQK_ERR_GEOMETRY;
     SortCall c{};
     c.ids = a.ids;
     c.wide = a.wide;
@@ -523,21 +658,14 @@ int rows_grouped(AdapterArgs a, bool bf, uint32_t *work, hipStream_t stream) {
     a.offs = work + p.offs;
     a.rows = work + p.rows;
     a.tiles = reinterpret_cast<uint4_t *>(work + p.desc);
+    a.tile_rows = work + p.tile_rows;
     a.pieces = reinterpret_cast<uint4_t *>(work + p.pieces);
     a.powers = reinterpret_cast<float *>(work + p.powers);
-    a.chunks = uint32_t(p.chunks);
+    hipError_t err = hipSuccess;
     by_ranks(a.rank, [&](auto shape) {
-        if (bf)
-            launch_down<true>(a, p.tiles, stream, shape);
-        else
-            launch_down<false>(a, p.tiles, stream, shape);
+        err = bf ? launch_tiles<true>(a, p.tiles, stream, shape) : launch_tiles<false>(a, p.tiles, stream, shape);
     });
-    if (const hipError_t err = hipGetLastError(); err != hipSuccess) return record_launch(err);
-    if (bf)
-        hipLaunchKernelGGL(adapter_up_tiles_kernel<true>, dim3{uint32_t(ups)}, dim3{256}, 0, stream, a);
-    else
-        hipLaunchKernelGGL(adapter_up_tiles_kernel<false>, dim3{uint32_t(ups)}, dim3{256}, 0, stream, a);
-    return record_launch(hipGetLastError());
+    return record_launch(err);
 }
 
 }  // namespace
@@ -548,7 +676,7 @@ extern "C" {
 int64_t iqk_adapters_work(int64_t in_features, int64_t out_features, int64_t rank, int64_t num_adapters, int64_t rows) {
     using namespace iqk;
     if (!adapters_shape_ok(in_features, out_features, rank, num_adapters, rows)) return -1;
-    return rows <= kRowsAlone ? rows * rank : group_plan(rank, num_adapters, rows).words;
+    return rows <= kRowsAlone ? 0 : group_plan(rank, num_adapters, rows).words;
 }
 
 int iqk_adapters(int dtype, int64_t in_features, int64_t out_features, int64_t rank, int64_t num_adapters,
@@ -558,8 +686,8 @@ int iqk_adapters(int dtype, int64_t in_features, int64_t out_features, int64_t r
     if (dtype != MX_F16 && dtype != MX_BF16) return IQK_ERR_ARGUMENT;
     if (!adapters_shape_ok(in_features, out_features, rank, num_adapters, rows)) return IQK_ERR_GEOMETRY;
     if (rows == 0) return IQK_OK;
-    if (!x || !ids || rows_per_id <= 0 || rows_per_id >= (int64_t(1) << 31) || !down || !up || !scales || !work || !y ||
-        !out)
+    if (!x || !ids || rows_per_id <= 0 || rows_per_id >= (int64_t(1) << 31) || !down || !up || !scales || !y || !out ||
+        (rows > kRowsAlone && !work))
         return IQK_ERR_ARGUMENT;
     if ((reinterpret_cast<uintptr_t>(down) | reinterpret_cast<uintptr_t>(up) | reinterpret_cast<uintptr_t>(work)) & 15u)
         return IQK_ERR_ARGUMENT;
@@ -569,7 +697,6 @@ int iqk_adapters(int dtype, int64_t in_features, int64_t out_features, int64_t r
     a.down = static_cast<const uint16_t *>(down);
     a.up = static_cast<const uint16_t *>(up);
     a.scales = scales;
-    a.t = reinterpret_cast<float *>(work);
     a.y = static_cast<const uint16_t *>(y);
     a.out = static_cast<uint16_t *>(out);
     a.T = uint32_t(rows);

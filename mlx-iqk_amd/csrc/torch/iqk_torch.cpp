@@ -437,15 +437,16 @@ PyObject *py_adapters(PyObject *, PyObject *const *args, Py_ssize_t n) {
                  &scales = tensor(args[5]), &y = tensor(args[6]);
     refuse_tangent(x, "x");
     refuse_tangent(y, "y");
-    TORCH_CHECK(down.dim() == 3 && up.dim() == 3 && up.size(0) == down.size(0) && up.size(2) == down.size(1) &&
-                    scales.numel() == down.size(0) && x.size(-1) == down.size(2) && y.size(-1) == up.size(1),
+    TORCH_CHECK(down.dim() == 4 && up.dim() == 4 && up.size(0) == down.size(0) && 8 * up.size(1) == down.size(2) &&
+                    down.size(3) == 8 && up.size(3) == 8 && scales.numel() == down.size(0) &&
+                    x.size(-1) == 8 * down.size(1) && y.size(-1) == up.size(2),
                 "the bank's tensors do not belong together: down ", down.sizes(), ", up ", up.sizes(), ", scales ",
                 scales.sizes());
-    const int64_t adapters = down.size(0), rank = down.size(1), in = down.size(2), out = up.size(1);
+    const int64_t adapters = down.size(0), rank = down.size(2), in = 8 * down.size(1), out = up.size(2);
     const int64_t rows = x.numel() / in, words = iqk_adapters_work(in, out, rank, adapters, rows);
     check(words < 0 ? IQK_ERR_GEOMETRY : IQK_OK, "iqk_adapters_work");
     const Tensor sum = args[7] == Py_None ? empty(y.sizes(), y.scalar_type(), y) : tensor(args[7]);
-    const Tensor work = empty({words}, at::kInt, x);
+    const Tensor work = words ? empty({words}, at::kInt, x) : Tensor();
     check(iqk_adapters(type_code(x), in, out, rank, adapters, x.data_ptr(), rows, ids.data_ptr(),
                        ids.scalar_type() == at::kLong, integer(args[2]), down.data_ptr(), up.data_ptr(),
                        ptr<float>(scales), ptr<uint32_t>(work), y.data_ptr(), sum.data_ptr(), stream_of(x)),

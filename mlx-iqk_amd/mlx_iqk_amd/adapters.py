@@ -24,13 +24,14 @@ _HALF = (torch.float16, torch.bfloat16)
 
 
 class LowRankAdapters(torch.nn.Module):
-    """``num_adapters`` adapters of up to ``rank`` for a projection ``[out, in]``, as buffers:
+    """``num_adapters`` adapters of up to ``rank`` for a projection ``[out, in]``, as buffers in
+    the kernels' layout, eight values of the reduction axis together (R: the rank rounded
+    up to a multiple of 8):
 
-    * ``down`` 16-bit ``[num_adapters, R, in]`` and ``up`` ``[num_adapters, out, R]``, R the
-      rank rounded up to a multiple of 8;
+    * ``down`` 16-bit ``[num_adapters, in/8, R, 8]`` and ``up`` ``[num_adapters, R/8, out, 8]``;
     * ``scales`` f32 ``[num_adapters]``.
 
-    All zeros, which add nothing, until :meth:`load`.
+    All zeros, which add nothing, until :meth:`load`; :meth:`adapter` gives one back.
     """
 
     def __init__(self, num_adapters: int, out_features: int, in_features: int, rank: int,
@@ -49,8 +50,10 @@ class LowRankAdapters(torch.nn.Module):
         if dtype not in _HALF:
             raise IqkRuntimeError(f"adapters are float16 or bfloat16, got {dtype}")
         ranks = (self.rank + 7) // 8 * 8
-        self.register_buffer("down", torch.zeros((self.num_adapters, ranks, self.in_features), dtype=dtype, device=device))
-        self.register_buffer("up", torch.zeros((self.num_adapters, self.out_features, ranks), dtype=dtype, device=device))
+        self.register_buffer("down", torch.zeros((self.num_adapters, self.in_features // 8, ranks, 8), dtype=dtype,
+                                                 device=device))
+        self.register_buffer("up", torch.zeros((self.num_adapters, ranks // 8, self.out_features, 8), dtype=dtype,
+                                               device=device))
         self.register_buffer("scales", torch.zeros(self.num_adapters, dtype=torch.float32, device=device))
 
     def load(self, index: int, down: torch.Tensor, up: torch.Tensor, scale: float = 1.0) -> None:
@@ -62,13 +65,20 @@ class LowRankAdapters(torch.nn.Module):
                 or down.shape[1] != self.in_features or up.shape[0] != self.out_features:
             raise IqkRuntimeError(f"an adapter is [r, {self.in_features}] and [{self.out_features}, r] with r up to "
                                   f"{self.rank}, got {tuple(down.shape)} and {tuple(up.shape)}")
-        r = down.shape[0]
+        r, ranks = down.shape[0], self.down.shape[2]
         with torch.no_grad():
-            self.down[index, :r].copy_(down)
-            self.down[index, r:].zero_()
-            self.up[index, :, :r].copy_(up)
-            self.up[index, :, r:].zero_()
+            a, b = (t.new_zeros(n, ranks, dtype=self.down.dtype) for t, n in ((down, self.in_features), (up, self.out_features)))
+            a[:, :r], b[:, :r] = down.T, up
+            self.down[index].copy_(a.view(-1, 8, ranks).transpose(1, 2))
+            self.up[index].copy_(b.view(-1, ranks // 8, 8).transpose(0, 1))
             self.scales[index] = float(scale)
+
+    def adapter(self, index: int) -> tuple[torch.Tensor, torch.Tensor, float]:
+        """Adapter ``index`` as :meth:`load` takes it, of rank R: ``(down, up, scale)``."""
+        if not 0 <= index < self.num_adapters:
+            raise IqkRuntimeError(f"the bank holds adapters 0 .. {self.num_adapters - 1}, got {index}")
+        down, up = (blocks[index].transpose(0, 1).flatten(1) for blocks in (self.down, self.up))
+        return down, up, float(self.scales[index])
 
     def forward(self, x: torch.Tensor, ids: torch.Tensor, y: torch.Tensor) -> torch.Tensor:
         """``y + scales[a] up[a] (down[a] x)`` with each row's own ``a``, in y's type.

@@ -33,12 +33,19 @@ def test_banks_are_refused():
 
 def test_load_on_the_host():
     bank = LowRankAdapters(2, 6, 16, 5, dtype=torch.float16)
-    assert bank.down.shape == (2, 8, 16) and bank.up.shape == (2, 6, 8)
+    assert bank.down.shape == (2, 2, 8, 8) and bank.up.shape == (2, 1, 6, 8)
     down, up = torch.randn(3, 16), torch.randn(6, 3)
+    bank.load(1, torch.randn(5, 16), torch.randn(6, 5))
     bank.load(1, down, up, 0.25)
-    assert torch.equal(bank.down[1, :3], down.half()) and torch.equal(bank.up[1, :, :3], up.half())
-    assert not bank.down[1, 3:].any() and not bank.up[1, :, 3:].any() and bank.scales.tolist() == [0.0, 0.25]
+    got_down, got_up, scale = bank.adapter(1)
+    assert torch.equal(got_down[:3], down.half()) and torch.equal(got_up[:, :3], up.half()) and scale == 0.25
+    assert not got_down[3:].any() and not got_up[:, 3:].any() and bank.scales.tolist() == [0.0, 0.25]
+    assert torch.equal(bank.down[1, 1, 2], down[2, 8:].half()) and torch.equal(bank.up[1, 0, 4, :3], up[4].half())
     assert not bank.down[0].any()
+    bank.load(0, down, up.T.contiguous().T)
+    assert torch.equal(bank.adapter(0)[1], got_up)
+    with pytest.raises(IqkRuntimeError):
+        bank.adapter(2)
     for index, a, b in ((2, down, up), (-1, down, up), (0, torch.randn(6, 16), torch.randn(6, 6)),
                         (0, down, torch.randn(6, 2)), (0, torch.randn(3, 8), up), (0, down, torch.randn(5, 3)),
                         (0, down[0], up)):
@@ -95,7 +102,7 @@ def test_sort_and_rows_refuse_bad_arguments(lib):
 def test_adapters_refuse_bad_arguments(lib):
     p, odd = ctypes.c_void_p(16), ctypes.c_void_p(24)  # never dereferenced: every call below is refused first
     f = lib.iqk_adapters
-    assert lib.iqk_adapters_work(64, 48, 8, 4, 3) > 0
+    assert lib.iqk_adapters_work(64, 48, 8, 4, 3) == 0 and lib.iqk_adapters_work(64, 48, 8, 4, 5000) > 0
     for n, out, rank, adapters, rows in ((0, 48, 8, 4, 3), (60, 48, 8, 4, 3), (64, 0, 8, 4, 3), (64, 48, 0, 4, 3),
                                          (64, 48, 12, 4, 3), (64, 48, 264, 4, 3), (64, 48, 8, 0, 3), (64, 48, 8, 1025, 3),
                                          (64, 48, 8, 4, -1), (64, 48, 8, 4, 1 << 31), (1 << 31, 48, 8, 4, 3),
@@ -105,10 +112,11 @@ def test_adapters_refuse_bad_arguments(lib):
     for dtype in (0, 3, -1):
         assert f(dtype, 64, 48, 8, 4, p, 3, p, 0, 1, p, p, p, p, p, p, None) == _native.ERR_ARGUMENT
     good = [2, 64, 48, 8, 4, p, 3, p, 0, 1, p, p, p, p, p, p, None]
-    for place in (5, 7, 10, 11, 12, 13, 14, 15):
-        assert f(*[None if i == place else v for i, v in enumerate(good)]) == _native.ERR_ARGUMENT
-    for place in (10, 11):
-        assert f(*[odd if i == place else v for i, v in enumerate(good)]) == _native.ERR_ARGUMENT
+    for rows, places in ((3, (5, 7, 10, 11, 12, 14, 15)), (5000, (5, 7, 10, 11, 12, 13, 14, 15))):
+        for place in places:
+            assert f(*[None if i == place else rows if i == 6 else v for i, v in enumerate(good)]) == _native.ERR_ARGUMENT
+        for place in (10, 11, 13):
+            assert f(*[odd if i == place else rows if i == 6 else v for i, v in enumerate(good)]) == _native.ERR_ARGUMENT
     for per_id in (0, -1, 1 << 31):
         assert f(*[per_id if i == 9 else v for i, v in enumerate(good)]) == _native.ERR_ARGUMENT
     assert f(2, 64, 48, 8, 4, None, 0, None, 0, 1, None, None, None, None, None, None, None) == _native.OK

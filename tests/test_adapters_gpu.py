@@ -37,7 +37,8 @@ def _rows(rng, rows, n, dtype, device):
 
 def _check(got, bank, x, ids, y, dtype):
     """got against float64, row by row; ids one a row."""
-    down, up, scales = _f64(bank.down), _f64(bank.up), _f64(bank.scales)
+    down, up, scales = (np.stack(parts) for parts in zip(*(
+        (_f64(down), _f64(up), scale) for down, up, scale in map(bank.adapter, range(bank.num_adapters)))))
     x, y, got = _f64(x), _f64(y), _f64(got)
     n, rank = down.shape[2], down.shape[1]
     for a in sorted(set(ids.tolist())):
@@ -92,7 +93,8 @@ def test_adapters_of_several_ranks(device, dtype, rows):
     for a, r in ((1, 1), (2, 39), (4, 8)):
         bank.load(a, torch.from_numpy(rng.standard_normal((r, 80))).to(dtype),
                   torch.from_numpy(rng.standard_normal((120, r))).to(dtype), -0.5)
-        assert not bank.down[a, r:].any() and not bank.up[a, :, r:].any()
+        down, up, scale = bank.adapter(a)
+        assert not down[r:].any() and not up[:, r:].any() and scale == -0.5
     x, y = _rows(rng, rows, 80, dtype, device), _rows(rng, rows, 120, dtype, device)
     ids = rng.integers(0, 6, rows)
     _check(bank(x, torch.from_numpy(ids).to(device), y), bank, x, ids, y, dtype)
@@ -157,8 +159,8 @@ def test_bad_rows_stay_where_they_are(device, dtype, rows):
     got[2, 5] = want[2, 5]
     rest = [r for r in range(rows) if r not in (1, 3)]
     assert torch.equal(got[rest], want[rest])
-    bank.down[3, 0, 0] = nan
-    bank.up[3, 7, 2] = inf
+    bank.down[3, 0, 0, 0] = nan
+    bank.up[3, 1, 7, 2] = inf
     got = bank(x, named, y)
     others = torch.from_numpy(ids != 3).to(device)
     assert torch.equal(got[others], want[others]) and bool(got[~others].isnan().all())
