@@ -29,10 +29,8 @@ struct AdapterArgs {
     uint16_t *out;
     uint32_t T, in, N, rank, adapters, wide, per_id;
     // grouped form
-    const uint32_t *offs;     // first slots of each adapter, then of the rows without one
-    const uint32_t *rows;     // [T] each slot's row
-    uint4_t *tiles;           // adapter, first slot, slots
-    uint32_t *tile_rows;      // [tile][slots] their rows
+    const uint4_t *tiles;      // adapter (the bank's size: none), -, slots (0: no such tile), -
+    const uint32_t *tile_rows; // [tile][slots] their rows
     uint4_t *pieces;          // A x of a tile's slots, split, as operand B of the second product
     float *powers;            // [tile][slots] what the pieces are multiplied with
     uint32_t columns;         // 256s of outputs of a workgroup
@@ -177,7 +175,7 @@ __global__ __launch_bounds__(kAloneThreads) void adapter_row_kernel(AdapterArgs 
 // pieces of eight bits (truncated, so that their sum is exact), an f16 product two of eleven
 // bits over a power of two of the slot's largest, which is multiplied back in f32.
 
-constexpr int kTileSlots = 64, kTileGroups = kTileSlots / 16;
+constexpr int kTileSlots = int(kSortTile), kTileGroups = kTileSlots / 16;
 
 template <bool BF>
 constexpr int kPieces = BF ? 3 : 2;
@@ -190,49 +188,6 @@ __device__ __forceinline__ float4_t mfma(uint4_t a, uint4_t b, float4_t c) {
     else
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8_t, a), __builtin_bit_cast(half8_t, b), c,
                                                       0, 0, 0);
-}
-
-struct Tile {
-    uint32_t adapter, first, slots;  // slots 0: none
-};
-
-// Tile t of the list in which each adapter's slots, and the rows without one (adapter: the
-// bank's size), take whole tiles in order.  All threads of a workgroup of THREADS call it.
-template <int THREADS>
-__device__ __forceinline__ Tile find_tile(const AdapterArgs &a, uint32_t t, uint32_t (&sums)[THREADS / 64], uint32_t (&found)[3]) {
-    constexpr int PER = (int(kAdaptersMax) + THREADS) / THREADS;  // consecutive groups of a thread
-    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, g0 = threadIdx.x * PER;
-    uint32_t first[PER + 1], mine = 0;
-#pragma unroll
-    for (int i = 0; i <= PER; ++i) first[i] = g0 + i <= a.adapters ? a.offs[g0 + i] : a.T;
-#pragma unroll
-    for (int i = 0; i < PER; ++i) mine += (first[i + 1] - first[i] + kTileSlots - 1) / kTileSlots;
-    uint32_t incl = mine;
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-        const uint32_t up = __shfl_up(incl, off, 64);
-        if (lane >= uint32_t(off)) incl += up;
-    }
-    if (lane == 63) sums[wave] = incl;
-    if (threadIdx.x == 0) found[2] = 0;
-    __syncthreads();
-    uint32_t at = incl - mine;
-#pragma unroll
-    for (int w = 0; w < THREADS / 64; ++w)
-        if (uint32_t(w) < wave) at += sums[w];
-#pragma unroll
-    for (int i = 0; i < PER; ++i) {
-        const uint32_t n = first[i + 1] - first[i], tiles = (n + kTileSlots - 1) / kTileSlots;
-        if (t >= at && t < at + tiles) {
-            const uint32_t begin = (t - at) * kTileSlots;
-            found[0] = g0 + i;
-            found[1] = first[i] + begin;
-            found[2] = min(n - begin, uint32_t(kTileSlots));
-        }
-        at += tiles;
-    }
-    __syncthreads();
-    return {found[0], found[1], found[2]};
 }
 
 // Lanes of a wavefront read what others of it wrote to LDS.
@@ -251,24 +206,21 @@ __global__ __launch_bounds__(64 * WAVES) void adapter_down_tiles_kernel(AdapterA
     constexpr int SLOTS = 16 * CT, RANKS = 16 * RT, THREADS = 64 * WAVES, KC = (RT + 1) / 2, PARTS = kTileGroups / CT;
     constexpr int SUMS = SLOTS * (RANKS + 4), STAGE = SLOTS * 32;  // floats of a wavefront's sums, of its turned rows
     __shared__ __attribute__((aligned(16))) float shared[WAVES][SUMS > STAGE ? SUMS : STAGE];
-    __shared__ uint32_t sums[WAVES], found[3];
     const uint32_t t = blockIdx.x / PARTS, group = blockIdx.x % PARTS * CT;  // the first of its groups of 16
-    Tile tile = find_tile<THREADS>(a, t, sums, found);
-    if (threadIdx.x == 0 && group == 0) a.tiles[t] = uint4_t{tile.adapter, tile.first, tile.slots, 0};
-    if (tile.slots <= 16 * group) return;  // uniform
-    tile.first += 16 * group;
-    tile.slots = min(tile.slots - 16 * group, uint32_t(SLOTS));
-    if (threadIdx.x < SLOTS)
-        a.tile_rows[t * kTileSlots + 16 * group + threadIdx.x] = a.rows[tile.first + min(threadIdx.x, tile.slots - 1u)];
-    if (tile.adapter >= a.adapters) return;  // uniform
+    const uint4_t tile = a.tiles[t];
+    const uint32_t adapter = tile.x, slots = tile.z;
+    if (slots <= 16 * group || adapter >= a.adapters) return;  // uniform
     const uint32_t lane = threadIdx.x & 63u, g = lane >> 4, m = lane & 15u, c8 = lane & 7u, r8 = lane >> 3;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint16_t *w[RT], *x[2 * CT];
 #pragma unroll
     for (int r = 0; r < RT; ++r)  // ranks past the last: it again, its sums not used
-        w[r] = a.down + size_t(tile.adapter) * a.rank * a.in + 8 * min(16u * r + m, a.rank - 1u);
+        w[r] = a.down + size_t(adapter) * a.rank * a.in + 8 * min(16u * r + m, a.rank - 1u);
 #pragma unroll
-    for (int c = 0; c < 2 * CT; ++c) x[c] = a.x + size_t(a.rows[tile.first + min(8u * c + r8, tile.slots - 1u)]) * a.in;
+    for (int c = 0; c < 2 * CT; ++c) {
+        const uint32_t slot = 16 * group + 8 * c + r8, row = a.tile_rows[t * kTileSlots + slot];
+        x[c] = a.x + size_t(slot < slots ? row : 0u) * a.in;  // past the tile's: row 0, its sums not used
+    }
     float4_t acc[RT][CT];
 #pragma unroll
     for (int r = 0; r < RT; ++r)
@@ -342,7 +294,7 @@ __global__ __launch_bounds__(64 * WAVES) void adapter_down_tiles_kernel(AdapterA
 #pragma unroll
         for (int c = 0; c < CT; ++c) *reinterpret_cast<float4_t *>(&part(wave, 16 * c + m, 16 * r + 4 * g)) = acc[r][c];
     __syncthreads();
-    const float scale = a.scales[tile.adapter];
+    const float scale = a.scales[adapter];
     constexpr int UNITS = 4 * KC;  // eights of a slot's ranks, rounded up to whole operands
     for (uint32_t u = threadIdx.x; u < SLOTS * UNITS; u += THREADS) {
         const uint32_t slot = u / UNITS, unit = u % UNITS, r0 = 8 * unit;
@@ -421,7 +373,10 @@ __global__ __launch_bounds__(256) void adapter_up_tiles_kernel(AdapterArgs a) {
 #pragma unroll
     for (int c = 0; c < CT; ++c)
 #pragma unroll
-        for (int h = 0; h < 2; ++h) row[c][h] = a.tile_rows[t * kTileSlots + min(16u * c + 8 * h + s8, slots - 1u)];
+        for (int h = 0; h < 2; ++h) {
+            const uint32_t slot = 16 * c + 8 * h + s8, of = a.tile_rows[t * kTileSlots + slot];
+            row[c][h] = slot < slots ? of : 0u;
+        }
     const uint32_t mine = 8 * (lane & 7u);
     if (adapter >= a.adapters) {  // rows without an adapter; uniform
         for (uint32_t n0 = begin + 64 * wave; n0 < end; n0 += 256) {
@@ -572,26 +527,23 @@ constexpr int64_t kRowsAlone = 64;  // rows up to which each is computed on its 
 
 // The grouped form's workspace, in words: where each part begins.
 struct GroupPlan {
-    int64_t tiles, chunks, hist, offs, rows, desc, tile_rows, pieces, powers, words;
+    int64_t tiles, hist, desc, tile_rows, pieces, powers, words;
 };
 
 GroupPlan group_plan(int64_t rank, int64_t adapters, int64_t rows) {
     GroupPlan p{};
-    // every adapter and the rows without one may end in a part of a tile
-    const int64_t most = rows / kTileSlots + adapters + 1;
-    p.tiles = most < rows ? most : rows;
-    for (p.chunks = 1; 32 * p.chunks < rank;) p.chunks *= 2;
+    p.tiles = sort_tiles(rows, adapters);
+    int64_t chunks = 1;  // operands of 32 ranks: a power of two of them
+    while (32 * chunks < rank) chunks *= 2;
     const auto take = [&](int64_t words) {
         const int64_t at = p.words;
         p.words += (words + 3) / 4 * 4;  // 16-byte steps
         return at;
     };
     p.hist = take(sort_plan(rows, adapters).words);
-    p.offs = take(adapters + 1);
-    p.rows = take(rows);
     p.desc = take(4 * p.tiles);
     p.tile_rows = take(p.tiles * kTileSlots);
-    p.pieces = take(p.tiles * kTileGroups * p.chunks * 3 * 64 * 4);
+    p.pieces = take(p.tiles * kTileGroups * chunks * 3 * 64 * 4);
     p.powers = take(p.tiles * kTileSlots);
     return p;
 }
@@ -652,12 +604,11 @@ int rows_grouped(AdapterArgs a, bool bf, uint32_t *work, hipStream_t stream) {
     c.per_token = 1;
     c.per_id = a.per_id;
     c.work = work + p.hist;
-    c.offsets = reinterpret_cast<int32_t *>(work + p.offs);
-    c.tokens = reinterpret_cast<int32_t *>(work + p.rows);
+    c.tiles = work + p.desc;
+    c.tile_pairs = work + p.tile_rows;
+    c.n_tiles = p.tiles;
     if (const int rc = sort_launch(c, stream); rc != IQK_OK) return rc;
-    a.offs = work + p.offs;
-    a.rows = work + p.rows;
-    a.tiles = reinterpret_cast<uint4_t *>(work + p.desc);
+    a.tiles = reinterpret_cast<const uint4_t *>(work + p.desc);
     a.tile_rows = work + p.tile_rows;
     a.pieces = reinterpret_cast<uint4_t *>(work + p.pieces);
     a.powers = reinterpret_cast<float *>(work + p.powers);

@@ -24,18 +24,22 @@
 namespace iqk {
 
 constexpr int64_t kSortMaxK = 64;
-constexpr int kSortWaves = 8, kSortThreads = 64 * kSortWaves;
 constexpr int kSortKeys = int(kSortMaxExperts) + 1;
+constexpr int kSortWaves = 16, kSortThreads = 64 * kSortWaves;
 // Pairs up to which every workgroup counts all of them itself, in one launch.
 constexpr int64_t kSortOne = 16384;
-constexpr int64_t kSortBlocks = 256;  // workgroups of a sort, at most
+constexpr int64_t kSortBlocks = 64;  // workgroups of a sort, at most
 
 struct SortArgs {
     const uint32_t *ids;
     uint32_t *hist;  // [blocks][hist_stride(E)], 16-byte aligned, or null: every workgroup counts all pairs
-    int32_t *offsets, *sorted_ids, *tokens, *slots;  // sorted_ids and slots may be null
+    int32_t *offsets, *sorted_ids, *tokens, *slots;
     uint32_t P, E, k, share;  // share: pairs of a workgroup, in order
     uint32_t per_id;          // pairs of an id
+    // instead of the lists: each key's pairs in tiles of kSortTile
+    uint4_t *tiles;           // key, -, pairs (0: none), -
+    uint32_t *tile_pairs;     // [tile][kSortTile]
+    uint32_t n_tiles;
 };
 
 template <bool WIDE>
@@ -59,11 +63,12 @@ __device__ __forceinline__ uint32_t rank_in(uint64_t lanes) {
     return __builtin_amdgcn_mbcnt_hi(uint32_t(lanes >> 32), __builtin_amdgcn_mbcnt_lo(uint32_t(lanes), 0));
 }
 
-// add(key, n, p) for the pairs from `base` to `end` that a wavefront takes, 64 from p on at every
-// STRIDE-th: once for each key among them, by one lane, with their number n (LDS adds to one
-// address one after the other).  AHEAD loads of ids are on their way at once.
+// add(key, p, n) for the pairs p .. p + n of one key, which together are those from `base` to
+// `end` that a wavefront takes, 64 at every STRIDE-th: a lane each, or where all 64 have one key
+// (a request's rows) lane 0 for them, since LDS adds to one address one after the other.  AHEAD
+// loads of ids are on their way at once.
 template <bool WIDE, uint32_t STRIDE, typename F>
-__device__ __forceinline__ void count_keys(const SortArgs &a, uint32_t base, uint32_t end, int bits, F &&add) {
+__device__ __forceinline__ void count_keys(const SortArgs &a, uint32_t base, uint32_t end, F &&add) {
     constexpr int AHEAD = 4;
     const uint32_t lane = threadIdx.x & 63u;
     for (; base < end; base += AHEAD * STRIDE) {
@@ -74,9 +79,11 @@ __device__ __forceinline__ void count_keys(const SortArgs &a, uint32_t base, uin
         for (int i = 0; i < AHEAD; ++i) {
             const uint32_t p = base + i * STRIDE;
             if (p >= end) continue;  // uniform
-            const bool live = p + lane < end;
-            const uint64_t same = same_key(key[i], live, bits);
-            if (live && rank_in(same) == 0) add(key[i], uint32_t(__popcll(same)), p);
+            if (__ballot(key[i] == uint32_t(__builtin_amdgcn_readfirstlane(key[i]))) == ~uint64_t(0)) {
+                if (lane == 0) add(key[i], p, min(end - p, 64u));
+            } else if (p + lane < end) {
+                add(key[i], p + lane, 1u);
+            }
         }
     }
 }
@@ -95,27 +102,29 @@ __global__ __launch_bounds__(kSortThreads) void sort_count_kernel(SortArgs a) {
     __syncthreads();
     const uint32_t lo = min(a.P, blockIdx.x * a.share), hi = min(a.P, lo + a.share);
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    count_keys<WIDE, kSortThreads>(a, lo + 64 * wave, hi, key_bits(a),
-                                   [&](uint32_t key, uint32_t n, uint32_t) { atomicAdd(&count[key], n); });
+    count_keys<WIDE, kSortThreads>(a, lo + 64 * wave, hi,
+                                   [&](uint32_t key, uint32_t, uint32_t n) { atomicAdd(&count[key], n); });
     __syncthreads();
     for (uint32_t e = threadIdx.x; e < stride; e += kSortThreads) a.hist[size_t(blockIdx.x) * stride + e] = count[e];
 }
 
+template <int WAVES>
 struct SortShared {
     uint32_t total[kSortKeys];                // pairs of each key, then those of the keys below
-    uint32_t before[kSortKeys];               // those of the shares before this one
-    uint32_t wave[kSortWaves][kSortKeys];     // those of each wavefront's share, then its next slot
-    uint32_t sums[kSortWaves];
+    uint32_t before[kSortKeys];               // those of the shares before this one, then (tiles) the key's end
+    uint32_t wave[WAVES][kSortKeys];          // those of each wavefront's share, then its next slot
+    uint32_t sums[WAVES];
 };
 
-// Exclusive sums of s.total over K keys, in place; a barrier before and after.
-__device__ __forceinline__ void scan_keys(SortShared &s, uint32_t K) {
-    constexpr int PER = (kSortKeys + kSortThreads - 1) / kSortThreads;  // consecutive keys of a thread
+// Exclusive sums over K keys of f(key): given to g(key, sum).  A barrier before and after.
+template <int WAVES, typename F, typename G>
+__device__ __forceinline__ void scan_keys(SortShared<WAVES> &s, uint32_t K, F &&f, G &&g) {
+    constexpr int THREADS = 64 * WAVES, PER = (kSortKeys + THREADS - 1) / THREADS;  // consecutive keys of a thread
     const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, first = threadIdx.x * PER;
     uint32_t v[PER], sum = 0;
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-        v[i] = first + i < K ? s.total[first + i] : 0u;
+        v[i] = first + i < K ? f(first + i) : 0u;
         sum += v[i];
     }
     uint32_t incl = sum;
@@ -128,50 +137,50 @@ __device__ __forceinline__ void scan_keys(SortShared &s, uint32_t K) {
     __syncthreads();
     uint32_t at = incl - sum;
 #pragma unroll
-    for (int w = 0; w < kSortWaves; ++w)
+    for (int w = 0; w < WAVES; ++w)
         if (uint32_t(w) < wave) at += s.sums[w];
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-        if (first + i < K) s.total[first + i] = at;
+        if (first + i < K) g(first + i, at);
         at += v[i];
     }
     __syncthreads();
 }
 
-// A workgroup's share of the pairs to their slots.  Its wavefronts take equal parts of the share
-// in order; a wavefront ranks 64 pairs at a time among those of the same key, which ballots of the
-// key's bits find, and keeps each key's next slot in LDS.
-template <bool WIDE>
-__global__ __launch_bounds__(kSortThreads) void sort_kernel(SortArgs a) {
-    __shared__ SortShared s;
+// place(pair, key, slot) for the pairs lo .. hi of a workgroup, whose `blocks` workgroups' shares
+// follow each other.  Its wavefronts take equal parts of the share in order; a wavefront ranks 64
+// pairs at a time among those of the same key, and keeps each key's next slot in LDS.
+template <bool WIDE, int WAVES, typename F>
+__device__ __forceinline__ void sort_share(const SortArgs &a, SortShared<WAVES> &s, uint32_t lo, uint32_t hi, uint32_t block,
+                                           uint32_t blocks, F &&place) {
+    constexpr int THREADS = 64 * WAVES;
     const uint32_t K = a.E + 1, lane = threadIdx.x & 63u;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    for (uint32_t e = threadIdx.x; e < K; e += kSortThreads) {
+    for (uint32_t e = threadIdx.x; e < K; e += THREADS) {
         s.total[e] = s.before[e] = 0;
 #pragma unroll
-        for (int w = 0; w < kSortWaves; ++w) s.wave[w][e] = 0;
+        for (int w = 0; w < WAVES; ++w) s.wave[w][e] = 0;
     }
     __syncthreads();
-    const uint32_t lo = min(a.P, blockIdx.x * a.share), hi = min(a.P, lo + a.share);
-    const uint32_t part = (a.share / kSortWaves + 63u) & ~63u;
+    const uint32_t part = ((hi - lo + WAVES - 1) / WAVES + 63u) & ~63u;
     const uint32_t from = min(hi, lo + wave * part), to = min(hi, from + part);
     const int bits = key_bits(a);
     if (a.hist) {
-        // four keys a lane, a wavefront every kSortWaves-th share's counts, AHEAD of them at once
+        // four keys a lane, a wavefront every WAVES-th share's counts, AHEAD of them at once
         constexpr uint32_t AHEAD = 8;
         const uint32_t stride = uint32_t(hist_stride(a.E));
         for (uint32_t e = 4 * lane; e < K; e += 256) {
             uint4_t total = {0, 0, 0, 0}, before = {0, 0, 0, 0};
-            for (uint32_t b0 = wave; b0 < gridDim.x; b0 += AHEAD * kSortWaves) {
+            for (uint32_t b0 = wave; b0 < blocks; b0 += AHEAD * WAVES) {
                 uint4_t n[AHEAD];
 #pragma unroll
                 for (uint32_t i = 0; i < AHEAD; ++i)
-                    n[i] = load_u4(a.hist + size_t(min(b0 + i * kSortWaves, gridDim.x - 1u)) * stride + e);
+                    n[i] = load_u4(a.hist + size_t(min(b0 + i * WAVES, blocks - 1u)) * stride + e);
 #pragma unroll
                 for (uint32_t i = 0; i < AHEAD; ++i) {
-                    const uint32_t b = b0 + i * kSortWaves;
-                    if (b < gridDim.x) total += n[i];
-                    if (b < blockIdx.x) before += n[i];
+                    const uint32_t b = b0 + i * WAVES;
+                    if (b < blocks) total += n[i];
+                    if (b < block) before += n[i];
                 }
             }
 #pragma unroll
@@ -183,27 +192,39 @@ __global__ __launch_bounds__(kSortThreads) void sort_kernel(SortArgs a) {
             }
         }
     } else {
-        // 64 pairs lie on one side of the share's start
-        count_keys<WIDE, kSortThreads>(a, 64 * wave, a.P, bits, [&](uint32_t key, uint32_t n, uint32_t p) {
+        count_keys<WIDE, THREADS>(a, 64 * wave, a.P, [&](uint32_t key, uint32_t p, uint32_t n) {
             atomicAdd(&s.total[key], n);
-            if (p < lo) atomicAdd(&s.before[key], n);
+            if (p < lo) atomicAdd(&s.before[key], min(n, lo - p));
         });
     }
-    count_keys<WIDE, 64>(a, from, to, bits, [&](uint32_t key, uint32_t n, uint32_t) { atomicAdd(&s.wave[wave][key], n); });
+    count_keys<WIDE, 64>(a, from, to, [&](uint32_t key, uint32_t, uint32_t n) { atomicAdd(&s.wave[wave][key], n); });
     __syncthreads();
-    scan_keys(s, K);
-    for (uint32_t e = threadIdx.x; e < K; e += kSortThreads) {
-        uint32_t at = s.total[e];
-        if (blockIdx.x == 0) a.offsets[e] = int32_t(at);
+    const bool first = block == 0;
+    const auto own = [&](uint32_t e, uint32_t at) {  // the next slots of a key in this share, at: its first slot
         at += s.before[e];
 #pragma unroll
-        for (int w = 0; w < kSortWaves; ++w) {
+        for (int w = 0; w < WAVES; ++w) {
             const uint32_t n = s.wave[w][e];
             s.wave[w][e] = at;
             at += n;
         }
+    };
+    if (a.tiles) {
+        // a key's pairs begin at a tile: their slots are places in the tiles
+        const auto whole = [](uint32_t n) { return (n + kSortTile - 1) / kSortTile * uint32_t(kSortTile); };
+        scan_keys(s, K, [&](uint32_t e) { return whole(s.total[e]); }, [&](uint32_t e, uint32_t at) {
+            own(e, at);
+            s.before[e] = at + s.total[e];  // where the key's pairs end
+            if (e == K - 1) s.sums[0] = (at + whole(s.total[e])) / kSortTile;  // all tiles with pairs
+        });
+        if (first)
+            for (uint32_t i = s.sums[0] + threadIdx.x; i < a.n_tiles; i += THREADS) a.tiles[i] = uint4_t{0, 0, 0, 0};
+    } else {
+        scan_keys(s, K, [&](uint32_t e) { return s.total[e]; }, [&](uint32_t e, uint32_t at) {
+            if (first) a.offsets[e] = int32_t(at);
+            own(e, at);
+        });
     }
-    __syncthreads();
     volatile uint32_t *const next = s.wave[wave];
     for (uint32_t base = from; base < to; base += 64) {
         const uint32_t p = base + lane;
@@ -215,14 +236,28 @@ __global__ __launch_bounds__(kSortThreads) void sort_kernel(SortArgs a) {
             const uint32_t slot = next[key] + rank;
             __builtin_amdgcn_wave_barrier();  // all lanes have read before the last of each key writes
             if (rank + 1 == uint32_t(__popcll(same))) next[key] = slot + 1;
-            if (slot < a.P) {  // unless another stream changed the ids meanwhile
-                if (a.slots) a.slots[p] = int32_t(slot);
-                if (a.sorted_ids) a.sorted_ids[slot] = int32_t(key);
-                a.tokens[slot] = int32_t(p / a.k);
-            }
+            place(p, key, slot);
         }
         __builtin_amdgcn_wave_barrier();
     }
+}
+
+template <bool WIDE, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void sort_kernel(SortArgs a) {
+    __shared__ SortShared<WAVES> s;
+    const uint32_t lo = min(a.P, blockIdx.x * a.share), hi = min(a.P, lo + a.share);
+    sort_share<WIDE, WAVES>(a, s, lo, hi, blockIdx.x, gridDim.x, [&](uint32_t p, uint32_t key, uint32_t slot) {
+        if (a.tiles) {
+            if (slot >= a.n_tiles * uint32_t(kSortTile)) return;
+            a.tile_pairs[slot] = p;
+            if (slot % kSortTile == 0)
+                a.tiles[slot / kSortTile] = uint4_t{key, 0, uint32_t(min(s.before[key] - slot, uint32_t(kSortTile))), 0};
+        } else if (slot < a.P) {  // unless another stream changed the ids meanwhile
+            a.slots[p] = int32_t(slot);
+            a.sorted_ids[slot] = int32_t(key);
+            a.tokens[slot] = int32_t(p / a.k);
+        }
+    });
 }
 
 // --------------------------------------------------------------------- rows ---
@@ -528,15 +563,20 @@ int sort_launch(const SortCall &c, hipStream_t stream) {
     a.k = uint32_t(c.per_token);
     a.per_id = uint32_t(c.per_id);
     a.share = uint32_t(plan.share);
-    const auto run = [&](auto kernel) {
-        hipLaunchKernelGGL(kernel, dim3{uint32_t(plan.blocks)}, dim3{kSortThreads}, 0, stream, a);
+    a.tiles = static_cast<uint4_t *>(c.tiles);
+    a.tile_pairs = c.tile_pairs;
+    a.n_tiles = uint32_t(c.n_tiles);
+    const auto run = [&](auto kernel, int threads) {
+        hipLaunchKernelGGL(kernel, dim3{uint32_t(plan.blocks)}, dim3{uint32_t(threads)}, 0, stream, a);
         return hipGetLastError();
     };
     if (plan.words) {
-        const hipError_t err = c.wide ? run(sort_count_kernel<true>) : run(sort_count_kernel<false>);
+        const hipError_t err = c.wide ? run(sort_count_kernel<true>, kSortThreads) : run(sort_count_kernel<false>, kSortThreads);
         if (err != hipSuccess) return record_launch(err);
     }
-    return record_launch(c.wide ? run(sort_kernel<true>) : run(sort_kernel<false>));
+    if (c.pairs <= 256)  // one pair a thread
+        return record_launch(c.wide ? run(sort_kernel<true, 4>, 256) : run(sort_kernel<false, 4>, 256));
+    return record_launch(c.wide ? run(sort_kernel<true, kSortWaves>, kSortThreads) : run(sort_kernel<false, kSortWaves>, kSortThreads));
 }
 
 namespace {

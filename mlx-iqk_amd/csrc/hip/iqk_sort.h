@@ -16,17 +16,27 @@ struct SortPlan {
 };
 SortPlan sort_plan(int64_t pairs, int64_t experts);
 
-// Pair p has the key ids[p / per_id], experts where that is outside [0, experts).
+constexpr int64_t kSortTile = 64;
+
+// Pair p has the key ids[p / per_id], experts where that is outside [0, experts).  Its outputs are
+// the lists of iqk_sort, or each key's pairs in tiles of their own.
 struct SortCall {
     const void *ids;
-    bool wide;           // 64-bit ids
+    bool wide;            // 64-bit ids
     int64_t pairs, experts, per_token, per_id;
     uint32_t *work;
-    int32_t *offsets;    // [experts + 1]: the pairs of lower keys
-    int32_t *sorted_ids; // [pairs] each slot's key, or null
-    int32_t *tokens;     // [pairs] each slot's p / per_token
-    int32_t *slots;      // [pairs] each pair's slot, or null
+    int32_t *offsets, *sorted_ids, *tokens, *slots;
+    void *tiles;          // null, or u32 [n_tiles][4]: key, -, pairs (0: none), -
+    uint32_t *tile_pairs; // [n_tiles][kSortTile], those past a tile's pairs unwritten
+    int64_t n_tiles;      // at least sort_tiles(pairs, experts)
 };
+
+// Tiles that any ids fill at most: every key may end in a part of one.
+inline int64_t sort_tiles(int64_t pairs, int64_t experts) {
+    const int64_t most = pairs / kSortTile + experts + 1;
+    return most < pairs ? most : pairs;
+}
+
 int sort_launch(const SortCall &c, hipStream_t stream);
 
 }  // namespace iqk
