@@ -387,15 +387,16 @@ int64_t iqk_sort_work(int64_t n_tokens, int64_t pairs_per_token, int64_t num_exp
 int iqk_sort(const void *ids, int wide_ids, int64_t n_tokens, int64_t pairs_per_token, int64_t num_experts,
              uint32_t *work, int32_t *offsets, int32_t *sorted_ids, int32_t *tokens, int32_t *slots, void *stream);
 
-// rows[slots[t, j]] = x[t], zeros in slots >= *kept (kept: offsets + num_experts; NULL: none).  x:
-// dtype [n_tokens, cols], rows: [n_tokens pairs_per_token, cols], at any element's address.
-// cols < 2^28.  A slot outside the rows is not written.
-int iqk_dispatch(int dtype, const void *x, const int32_t *slots, const int32_t *kept, int64_t n_tokens,
-                 int64_t pairs_per_token, int64_t cols, void *rows, void *stream);
+// iqk_sort's lists, and each token's row to its slots: rows[slots[t, j]] = x[t], zeros in the
+// slots of pairs left out.  x: dtype [n_tokens, cols], rows: [n_tokens pairs_per_token, cols], at
+// any element's address.  cols < 2^28.  One launch for at most 1024 pairs.
+int iqk_dispatch(int dtype, const void *x, const void *ids, int wide_ids, int64_t n_tokens, int64_t pairs_per_token,
+                 int64_t num_experts, int64_t cols, uint32_t *work, int32_t *offsets, int32_t *sorted_ids,
+                 int32_t *tokens, int32_t *slots, void *rows, void *stream);
 
 // out[t] = sum_j weights[t, j] y[slots[t, j]] + add[t], f32 sums in the order of j, one rounding.
-// slots NULL: pair p's row is p; slots >= *kept are skipped; weights NULL: ones (the gradient of
-// iqk_dispatch); add NULL: none.  y: dtype [n_tokens pairs_per_token, cols].
+// slots NULL: pair p's row is p; slots >= *kept (offsets + num_experts; NULL: none) are skipped;
+// weights NULL: ones (the gradient of iqk_dispatch); add NULL: none.  y: dtype [n_tokens pairs_per_token, cols].
 int iqk_combine(int dtype, const void *y, const int32_t *slots, const int32_t *kept, const float *weights,
                 const void *add, int64_t n_tokens, int64_t pairs_per_token, int64_t cols, void *out, void *stream);
 

@@ -389,6 +389,50 @@ __global__ __launch_bounds__(256) void dispatch_kernel(RowArgs a) {
         dispatch_chunk<false>(a, at);
 }
 
+// Few pairs: the rows' workgroups sort for themselves, in one launch.  Each counts all pairs, ranks
+// those of its own tokens, and moves its part of their rows; one of a token's workgroups writes
+// its lists.  (A launch before costs 3 us of the GPU's time and 2 of the host's.)
+constexpr int64_t kDispatchOne = 1024;  // pairs
+
+template <bool WIDE>
+__global__ __launch_bounds__(256) void sort_dispatch_kernel(SortArgs sort, RowArgs a) {
+    __shared__ SortShared<4> s;
+    __shared__ uint32_t slots[kDispatchOne];
+    const uint32_t tokens = 256u >> a.log_width, block = blockIdx.x / a.columns;
+    const uint32_t lo = min(sort.P, block * tokens * a.k), hi = min(sort.P, lo + tokens * a.k);
+    const bool writes = blockIdx.x % a.columns == 0;
+    const uint32_t t = block * tokens + (threadIdx.x >> a.log_width);
+    const uint32_t chunk = (blockIdx.x % a.columns << a.log_width) + (threadIdx.x & ((1u << a.log_width) - 1u));
+    const bool live = t < a.T && chunk < a.chunks;
+    const uint32_t halves = min(8u, (a.row - 16u * chunk) / 2u);
+    const size_t column = size_t(chunk) * 16;
+    uint4_t w = {0, 0, 0, 0};
+    if (live) {  // on its way while the pairs are sorted
+        const uint8_t *const from = a.in + size_t(t) * a.row + column;
+        w = halves == 8 ? load_chunk<true>(from, 8) : load_chunk<false>(from, halves);
+    }
+    sort_share<WIDE, 4>(sort, s, lo, hi, writes ? block : 1u, 1u, [&](uint32_t p, uint32_t key, uint32_t slot) {
+        slots[p - lo] = key < sort.E ? slot : slot | 0x80000000u;  // left out
+        if (writes && slot < sort.P) {
+            sort.slots[p] = int32_t(slot);
+            sort.sorted_ids[slot] = int32_t(key);
+            sort.tokens[slot] = int32_t(p / a.k);
+        }
+    });
+    __syncthreads();
+    if (!live) return;
+    for (uint32_t j = 0; j < a.k; ++j) {
+        const uint32_t slot = slots[t * a.k + j - lo], at = slot & 0x7fffffffu;
+        if (at >= a.P) continue;
+        uint8_t *const to = a.out + size_t(at) * a.row + column;
+        const uint4_t v = slot >> 31 ? uint4_t{0, 0, 0, 0} : w;
+        if (halves == 8)
+            store_chunk<true>(to, v, 8);
+        else
+            store_chunk<false>(to, v, halves);
+    }
+}
+
 template <int DT, bool WHOLE, typename PLACE>
 __device__ __forceinline__ void combine_chunk(const RowArgs &a, const PLACE &at) {
     constexpr int N = kChunk<DT>;
@@ -654,23 +698,50 @@ int iqk_sort(const void *ids, int wide_ids, int64_t n_tokens, int64_t pairs_per_
     return sort_launch(c, as_stream(stream));
 }
 
-int iqk_dispatch(int dtype, const void *x, const int32_t *slots, const int32_t *kept, int64_t n_tokens,
-                 int64_t pairs_per_token, int64_t cols, void *rows, void *stream) {
+int iqk_dispatch(int dtype, const void *x, const void *ids, int wide_ids, int64_t n_tokens, int64_t pairs_per_token,
+                 int64_t num_experts, int64_t cols, uint32_t *work, int32_t *offsets, int32_t *sorted_ids,
+                 int32_t *tokens, int32_t *slots, void *rows, void *stream) {
     using namespace iqk;
-    if (!rows_shape_ok(dtype, n_tokens, pairs_per_token, cols)) return IQK_ERR_GEOMETRY;
-    if (n_tokens == 0) return IQK_OK;
-    if (!x || !slots || !rows) return IQK_ERR_ARGUMENT;
+    if (!rows_shape_ok(dtype, n_tokens, pairs_per_token, cols) || !sort_shape_ok(n_tokens, pairs_per_token, num_experts))
+        return IQK_ERR_GEOMETRY;
+    if (n_tokens && (!x || !rows)) return IQK_ERR_ARGUMENT;
     RowArgs a = row_args(dtype, n_tokens, pairs_per_token, cols);
+    if (n_tokens == 0 || n_tokens * pairs_per_token > kDispatchOne) {
+        if (const int rc = iqk_sort(ids, wide_ids, n_tokens, pairs_per_token, num_experts, work, offsets, sorted_ids,
+                                    tokens, slots, stream);
+            rc != IQK_OK || n_tokens == 0)
+            return rc;
+        a.in = static_cast<const uint8_t *>(x);
+        a.slots = slots;
+        a.kept = offsets + num_experts;
+        a.out = static_cast<uint8_t *>(rows);
+        by_tokens(a, 256 >> a.log_width, a.columns, [&](const RowArgs &part, uint32_t blocks) {
+            if (part.log_width >= 6)
+                hipLaunchKernelGGL(dispatch_kernel<true>, dim3{blocks}, dim3{256}, 0, as_stream(stream), part);
+            else
+                hipLaunchKernelGGL(dispatch_kernel<false>, dim3{blocks}, dim3{256}, 0, as_stream(stream), part);
+        });
+        return record_launch(hipGetLastError());
+    }
+    if (!ids || !offsets || !sorted_ids || !tokens || !slots) return IQK_ERR_ARGUMENT;
+    SortArgs sort{};
+    sort.ids = static_cast<const uint32_t *>(ids);
+    sort.offsets = offsets;
+    sort.sorted_ids = sorted_ids;
+    sort.tokens = tokens;
+    sort.slots = slots;
+    sort.P = a.P;
+    sort.E = uint32_t(num_experts);
+    sort.k = a.k;
+    sort.per_id = 1;
     a.in = static_cast<const uint8_t *>(x);
-    a.slots = slots;
-    a.kept = kept;
     a.out = static_cast<uint8_t *>(rows);
-    by_tokens(a, 256 >> a.log_width, a.columns, [&](const RowArgs &part, uint32_t blocks) {
-        if (part.log_width >= 6)
-            hipLaunchKernelGGL(dispatch_kernel<true>, dim3{blocks}, dim3{256}, 0, as_stream(stream), part);
-        else
-            hipLaunchKernelGGL(dispatch_kernel<false>, dim3{blocks}, dim3{256}, 0, as_stream(stream), part);
-    });
+    const int64_t each = 256 >> a.log_width, blocks = (n_tokens + each - 1) / each * a.columns;
+    if (!grid_ok(blocks, 256)) return IQK_ERR_GEOMETRY;
+    if (wide_ids)
+        hipLaunchKernelGGL(sort_dispatch_kernel<true>, dim3{uint32_t(blocks)}, dim3{256}, 0, as_stream(stream), sort, a);
+    else
+        hipLaunchKernelGGL(sort_dispatch_kernel<false>, dim3{uint32_t(blocks)}, dim3{256}, 0, as_stream(stream), sort, a);
     return record_launch(hipGetLastError());
 }
 

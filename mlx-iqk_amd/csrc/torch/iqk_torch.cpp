@@ -11,6 +11,7 @@
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <ATen/ATen.h>
+#include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPException.h>
 #include <c10/hip/HIPStream.h>
 
@@ -186,17 +187,35 @@ struct Sorted {
     Tensor offsets, ids, tokens, slots;
 };
 
+// A tensor of its own in a part of base's storage.  (An allocation takes 1 us, this a tenth.)
+Tensor part_of(const Tensor &base, int64_t offset, c10::IntArrayRef shape) {
+    Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(base.storage()), base.key_set(), base.dtype());
+    t.unsafeGetTensorImpl()->set_storage_offset(offset);
+    t.unsafeGetTensorImpl()->set_sizes_contiguous(shape);
+    return t;
+}
+
+// The lists of ids [..., k], each at 16 bytes of one allocation.
+Sorted empty_lists(const Tensor &ids, int64_t experts) {
+    const int64_t pairs = ids.numel();
+    const auto whole = [](int64_t n) { return (n + 3) / 4 * 4; };
+    const int64_t ids_at = whole(experts + 1), tokens_at = ids_at + whole(pairs), slots_at = tokens_at + whole(pairs);
+    const Tensor all = empty({slots_at + whole(pairs)}, at::kInt, ids);
+    return {part_of(all, 0, {experts + 1}), part_of(all, ids_at, {pairs}), part_of(all, tokens_at, {pairs}),
+            part_of(all, slots_at, ids.sizes())};
+}
+
+Tensor sort_work(const Tensor &ids, int64_t experts) {
+    const int64_t k = ids.size(-1), words = iqk_sort_work(ids.numel() / k, k, experts);
+    check(words < 0 ? IQK_ERR_GEOMETRY : IQK_OK, "iqk_sort_work");
+    return words > 0 ? empty({words}, at::kInt, ids) : Tensor();
+}
+
 // ids [..., k], contiguous, i32 or i64
 Sorted sort_pairs(const Tensor &ids, int64_t experts) {
-    const int64_t k = ids.size(-1), pairs = ids.numel(), tokens = pairs / k;
-    Sorted s;
-    s.offsets = empty({experts + 1}, at::kInt, ids);
-    s.ids = empty({pairs}, at::kInt, ids);
-    s.tokens = empty({pairs}, at::kInt, ids);
-    s.slots = empty(ids.sizes(), at::kInt, ids);
-    const int64_t words = iqk_sort_work(tokens, k, experts);
-    check(words < 0 ? IQK_ERR_GEOMETRY : IQK_OK, "iqk_sort_work");
-    const Tensor work = words ? empty({words}, at::kInt, ids) : Tensor();
+    const int64_t k = ids.size(-1), tokens = ids.numel() / k;
+    const Sorted s = empty_lists(ids, experts);
+    const Tensor work = sort_work(ids, experts);
     check(iqk_sort(ids.data_ptr(), ids.scalar_type() == at::kLong, tokens, k, experts, ptr<uint32_t>(work),
                    ptr<int32_t>(s.offsets), ptr<int32_t>(s.ids), ptr<int32_t>(s.tokens), ptr<int32_t>(s.slots),
                    stream_of(ids)),
@@ -209,11 +228,14 @@ const int32_t *kept(const Tensor &offsets) {
     return offsets.defined() ? ptr<int32_t>(offsets) + offsets.numel() - 1 : nullptr;
 }
 
-Tensor dispatch_forward(const Tensor &x, const Tensor &slots, const Tensor &offsets) {
-    const int64_t k = slots.size(-1), tokens = slots.numel() / k, cols = x.size(-1);
+// x [tokens, cols] by ids [tokens, k]: the rows, and the lists in `s`.
+Tensor dispatch_forward(const Tensor &x, const Tensor &ids, int64_t experts, const Sorted &s) {
+    const int64_t k = ids.size(-1), tokens = ids.numel() / k, cols = x.size(-1);
     Tensor rows = empty({tokens * k, cols}, x.scalar_type(), x);
-    check(iqk_dispatch(type_code(x), x.data_ptr(), ptr<int32_t>(slots), kept(offsets), tokens, k, cols, rows.data_ptr(),
-                       stream_of(x)),
+    const Tensor work = sort_work(ids, experts);
+    check(iqk_dispatch(type_code(x), x.data_ptr(), ids.data_ptr(), ids.scalar_type() == at::kLong, tokens, k, experts,
+                       cols, ptr<uint32_t>(work), ptr<int32_t>(s.offsets), ptr<int32_t>(s.ids), ptr<int32_t>(s.tokens),
+                       ptr<int32_t>(s.slots), rows.data_ptr(), stream_of(x)),
           "iqk_dispatch");
     return rows;
 }
@@ -233,18 +255,22 @@ Tensor combine_forward(const Tensor &y, const Tensor &weights, const Tensor &slo
 }
 
 struct Dispatch : torch::autograd::Function<Dispatch> {
-    static variable_list forward(AutogradContext *ctx, const Tensor &x, const Tensor &slots, const Tensor &offsets) {
+    // the lists are written here, and the caller's
+    static variable_list forward(AutogradContext *ctx, const Tensor &x, const Tensor &ids, int64_t experts,
+                                 const Tensor &offsets, const Tensor &sorted_ids, const Tensor &tokens,
+                                 const Tensor &slots) {
         ctx->set_materialize_grads(false);
         ctx->save_for_backward({slots, offsets});
-        return {dispatch_forward(x, slots, offsets)};
+        return {dispatch_forward(x, ids, experts, {offsets, sorted_ids, tokens, slots})};
     }
     static variable_list backward(AutogradContext *ctx, variable_list grads) {
         refuse_capture();
-        if (!grads[0].defined()) return {Tensor(), Tensor(), Tensor()};
+        if (!grads[0].defined()) return variable_list(7);
         const auto saved = ctx->get_saved_variables();
+        const c10::DeviceGuard guard(grads[0].device());
         const Tensor dx = combine_forward(grads[0].detach().contiguous(), Tensor(), saved[0], saved[1], Tensor());
         auto out = once(dx, grads, Tensor());
-        out.resize(3);
+        out.resize(7);
         return out;
     }
 };
@@ -270,6 +296,7 @@ struct Combine : torch::autograd::Function<Combine> {
         if (!grads[0].defined()) return out;
         const auto saved = ctx->get_saved_variables();
         const Tensor &y = saved[0], &weights = saved[1], &slots = saved[2], &offsets = saved[3];
+        const c10::DeviceGuard guard(grads[0].device());
         const Tensor dout = grads[0].detach().contiguous();
         Tensor dy, dweights;
         if (ctx->saved_data["dy"].toBool()) dy = empty(ctx->saved_data["shape"].toIntVector(), dout.scalar_type(), dout);
@@ -391,36 +418,91 @@ PyObject *tuple(std::initializer_list<Tensor> tensors) {
     return t;
 }
 
-// sort(ids, experts) -> (offsets, ids, tokens, slots); ids contiguous, i32 or i64
+// Whether the sort and row calls take t as it is: dense, on a GPU (of like's device).
+bool dense(const Tensor &t) { return t.is_cuda() && t.dim() && t.is_contiguous(); }
+bool dense(const Tensor &t, const Tensor &like) { return dense(t) && t.get_device() == like.get_device(); }
+
+bool rows_type(const Tensor &t) {
+    const auto type = t.scalar_type();
+    return type == at::kFloat || type == at::kHalf || type == at::kBFloat16;
+}
+
+constexpr int64_t kPairs = int64_t(1) << 31;  // fewer than these
+constexpr int64_t kMaxK = 64, kMaxExperts = 1024, kMaxCols = int64_t(1) << 28;
+
+bool ids_ready(const Tensor &ids, int64_t experts) {
+    const auto type = ids.scalar_type();
+    return (type == at::kInt || type == at::kLong) && dense(ids) && ids.size(-1) > 0 && ids.size(-1) <= kMaxK &&
+           ids.numel() < kPairs && experts > 0 && experts <= kMaxExperts;
+}
+
+// Whether t is [..., cols] with the leading shape of pairs [..., k].
+bool of_tokens(const Tensor &t, const Tensor &pairs, int64_t cols) {
+    return t.dim() == pairs.dim() && t.size(-1) == cols && t.sizes().slice(0, t.dim() - 1) == pairs.sizes().slice(0, t.dim() - 1);
+}
+
+// The calls below answer None where an operand is not one that the kernels take as it is,
+// with nothing launched: the caller says what is wrong with it, or copies it.
+
+// sort(ids, experts) -> (offsets, ids, tokens, slots)
 PyObject *py_sort(PyObject *, PyObject *const *args, Py_ssize_t n) {
     HANDLE_TH_ERRORS
     arguments(n, 2);
-    const Sorted s = sort_pairs(tensor(args[0]), integer(args[1]));
+    if (!THPVariable_Check(args[0])) Py_RETURN_NONE;
+    const Tensor &ids = tensor(args[0]);
+    const int64_t experts = integer(args[1]);
+    if (!ids_ready(ids, experts)) Py_RETURN_NONE;
+    const c10::DeviceGuard guard(ids.device());
+    const Sorted s = sort_pairs(ids, experts);
     return tuple({s.offsets, s.ids, s.tokens, s.slots});
     END_HANDLE_TH_ERRORS
 }
 
-// dispatch(x, ids, experts) -> (rows, offsets, ids, tokens, slots); x and ids contiguous
+// dispatch(x, ids, experts) -> (rows, offsets, ids, tokens, slots)
 PyObject *py_dispatch(PyObject *, PyObject *const *args, Py_ssize_t n) {
     HANDLE_TH_ERRORS
     arguments(n, 3);
-    const Tensor &x = tensor(args[0]);
+    if (!THPVariable_Check(args[0]) || !THPVariable_Check(args[1])) Py_RETURN_NONE;
+    const Tensor &x = tensor(args[0]), &ids = tensor(args[1]);
+    const int64_t experts = integer(args[2]);
+    if (!ids_ready(ids, experts) || !dense(x, ids) || !rows_type(x) || x.size(-1) <= 0 || x.size(-1) >= kMaxCols ||
+        !of_tokens(x, ids, x.size(-1)))
+        Py_RETURN_NONE;
     refuse_tangent(x, "x");
-    const Sorted s = sort_pairs(tensor(args[1]), integer(args[2]));
-    const Tensor rows = wants_grad(x) ? Dispatch::apply(x, s.slots, s.offsets)[0] : dispatch_forward(x, s.slots, s.offsets);
+    const c10::DeviceGuard guard(x.device());
+    const Sorted s = empty_lists(ids, experts);
+    const Tensor rows = wants_grad(x) ? Dispatch::apply(x, ids, experts, s.offsets, s.ids, s.tokens, s.slots)[0]
+                                      : dispatch_forward(x, ids, experts, s);
     return tuple({rows, s.offsets, s.ids, s.tokens, s.slots});
     END_HANDLE_TH_ERRORS
 }
 
-// combine(y, weights, slots | None, offsets | None, add | None) -> out; all contiguous
+// combine(y, weights, slots | None, offsets | None, add | None) -> out
 PyObject *py_combine(PyObject *, PyObject *const *args, Py_ssize_t n) {
     HANDLE_TH_ERRORS
     arguments(n, 5);
+    for (int i = 0; i < 5; ++i)
+        if (!THPVariable_Check(args[i]) && (i < 2 || args[i] != Py_None)) Py_RETURN_NONE;
     const Tensor &y = tensor(args[0]), &weights = tensor(args[1]);
     const Tensor slots = tensor_or_none(args[2]), offsets = tensor_or_none(args[3]), add = tensor_or_none(args[4]);
+    if (!dense(y) || !rows_type(y) || y.size(-1) <= 0 || y.size(-1) >= kMaxCols || !dense(weights, y) ||
+        weights.scalar_type() != at::kFloat || weights.size(-1) <= 0 || weights.size(-1) > kMaxK ||
+        weights.numel() >= kPairs || slots.defined() != offsets.defined())
+        Py_RETURN_NONE;
+    const int64_t cols = y.size(-1);
+    if (slots.defined()) {
+        if (!dense(slots, y) || slots.scalar_type() != at::kInt || slots.sizes() != weights.sizes() || !dense(offsets, y) ||
+            offsets.scalar_type() != at::kInt || !offsets.numel() || y.dim() != 2 || y.size(0) != weights.numel())
+            Py_RETURN_NONE;
+    } else if (y.dim() != weights.dim() + 1 || y.sizes().slice(0, weights.dim()) != weights.sizes()) {
+        Py_RETURN_NONE;
+    }
+    if (add.defined() && (!dense(add, y) || add.scalar_type() != y.scalar_type() || !of_tokens(add, weights, cols)))
+        Py_RETURN_NONE;
     refuse_tangent(y, "y");
     refuse_tangent(weights, "weights");
     if (add.defined()) refuse_tangent(add, "add");
+    const c10::DeviceGuard guard(y.device());
     if (wants_grad(y) || wants_grad(weights) || (add.defined() && wants_grad(add))) {
         const auto given = [](const Tensor &t) { return t.defined() ? std::optional<Tensor>(t) : std::nullopt; };
         return THPVariable_Wrap(Combine::apply(y, weights, given(slots), given(offsets), given(add))[0]);
@@ -429,27 +511,44 @@ PyObject *py_combine(PyObject *, PyObject *const *args, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
-// adapters(x, ids, rows_per_id, down, up, scales, y, out | None) -> out; all contiguous
+// adapters(x, ids, y, down, up, scales, out | None) -> out; out may be y
 PyObject *py_adapters(PyObject *, PyObject *const *args, Py_ssize_t n) {
     HANDLE_TH_ERRORS
-    arguments(n, 8);
-    const Tensor &x = tensor(args[0]), &ids = tensor(args[1]), &down = tensor(args[3]), &up = tensor(args[4]),
-                 &scales = tensor(args[5]), &y = tensor(args[6]);
-    refuse_tangent(x, "x");
-    refuse_tangent(y, "y");
+    arguments(n, 7);
+    for (int i = 0; i < 6; ++i)
+        if (!THPVariable_Check(args[i])) Py_RETURN_NONE;
+    const Tensor &x = tensor(args[0]), &ids = tensor(args[1]), &y = tensor(args[2]), &down = tensor(args[3]),
+                 &up = tensor(args[4]), &scales = tensor(args[5]);
+    const auto type = down.scalar_type(), id_type = ids.scalar_type();
+    if ((type != at::kHalf && type != at::kBFloat16) || up.scalar_type() != type || scales.scalar_type() != at::kFloat ||
+        x.scalar_type() != type || y.scalar_type() != type || (id_type != at::kInt && id_type != at::kLong) ||
+        !dense(down) || !dense(up, down) || !dense(scales, down) || !dense(x, down) || !dense(y, down) ||
+        !ids.is_cuda() || ids.get_device() != down.get_device() || !ids.is_contiguous())
+        Py_RETURN_NONE;
     TORCH_CHECK(down.dim() == 4 && up.dim() == 4 && up.size(0) == down.size(0) && 8 * up.size(1) == down.size(2) &&
-                    down.size(3) == 8 && up.size(3) == 8 && scales.numel() == down.size(0) &&
-                    x.size(-1) == 8 * down.size(1) && y.size(-1) == up.size(2),
+                    down.size(3) == 8 && up.size(3) == 8 && scales.numel() == down.size(0),
                 "the bank's tensors do not belong together: down ", down.sizes(), ", up ", up.sizes(), ", scales ",
                 scales.sizes());
-    const int64_t adapters = down.size(0), rank = down.size(2), in = 8 * down.size(1), out = up.size(2);
+    const int64_t adapters = down.size(0), rank = down.size(2), in = 8 * down.size(1), out = up.size(2), lead = x.dim() - 1;
+    if (x.size(-1) != in || y.size(-1) != out || y.dim() != x.dim() || ids.dim() != lead || !x.numel() ||
+        x.sizes().slice(0, lead) != y.sizes().slice(0, lead) || wants_grad(x) || wants_grad(y))
+        Py_RETURN_NONE;
+    int64_t same = 0, rows_per_id = 1;  // the rows' shape up to some dimension, 1 from there on
+    while (same < lead && ids.size(same) == x.size(same)) ++same;
+    for (int64_t i = same; i < lead; ++i) {
+        if (ids.size(i) != 1) Py_RETURN_NONE;
+        rows_per_id *= x.size(i);
+    }
+    refuse_tangent(x, "x");
+    refuse_tangent(y, "y");
+    const c10::DeviceGuard guard(x.device());
     const int64_t rows = x.numel() / in, words = iqk_adapters_work(in, out, rank, adapters, rows);
     check(words < 0 ? IQK_ERR_GEOMETRY : IQK_OK, "iqk_adapters_work");
-    const Tensor sum = args[7] == Py_None ? empty(y.sizes(), y.scalar_type(), y) : tensor(args[7]);
+    const Tensor sum = args[6] == Py_None ? empty(y.sizes(), type, y) : tensor(args[6]);
     const Tensor work = words ? empty({words}, at::kInt, x) : Tensor();
-    check(iqk_adapters(type_code(x), in, out, rank, adapters, x.data_ptr(), rows, ids.data_ptr(),
-                       ids.scalar_type() == at::kLong, integer(args[2]), down.data_ptr(), up.data_ptr(),
-                       ptr<float>(scales), ptr<uint32_t>(work), y.data_ptr(), sum.data_ptr(), stream_of(x)),
+    check(iqk_adapters(type_code(x), in, out, rank, adapters, x.data_ptr(), rows, ids.data_ptr(), id_type == at::kLong,
+                       rows_per_id, down.data_ptr(), up.data_ptr(), ptr<float>(scales), ptr<uint32_t>(work),
+                       y.data_ptr(), sum.data_ptr(), stream_of(x)),
           "iqk_adapters");
     return THPVariable_Wrap(sum);
     END_HANDLE_TH_ERRORS

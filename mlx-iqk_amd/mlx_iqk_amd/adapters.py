@@ -91,8 +91,11 @@ class LowRankAdapters(torch.nn.Module):
         return self._add(x, ids, y, None)
 
     def _add(self, x, ids, y, out) -> torch.Tensor:
-        buffers = self._buffers
+        buffers, add = self._buffers, _native.torch_binding().adapters
         down, up, scales = buffers["down"], buffers["up"], buffers["scales"]
+        if (got := add(x, ids, y, down, up, scales, out)) is not None:
+            return got
+        # what the kernels do not take as it is
         dtype = down.dtype
         if not down.is_cuda:
             raise IqkKernelError(f"the bank must live on a GPU, got {down.device}")
@@ -118,16 +121,15 @@ class LowRankAdapters(torch.nn.Module):
             raise IqkKernelError("ids must be an integer tensor")
         if ids.device != down.device:
             raise IqkKernelError(f"ids are on {ids.device}, the bank on {down.device}")
-        per_id = _pairs_per_x_row(ids.shape, lead) if ids.dim() == len(lead) else None
-        if per_id is None:
+        if ids.dim() != len(lead) or _pairs_per_x_row(ids.shape, lead) is None:
             raise IqkRuntimeError(f"ids {tuple(ids.shape)} must have the rows' shape {tuple(lead)}, or 1 from some "
                                   "dimension on")
         if not x.numel():
             return y.clone() if out is None else out
         if ids.dtype not in _KERNEL_IDS:
             ids = torch.clamp(ids.to(torch.int64), -2, self.num_adapters)
-        return _native.torch_binding().adapters(x.contiguous(), ids.contiguous(), per_id, down.contiguous(),
-                                                up.contiguous(), scales.contiguous(), y.contiguous(), out)
+        return add(x.contiguous(), ids.contiguous(), y.contiguous(), down.contiguous(), up.contiguous(),
+                   scales.contiguous(), out)
 
     def extra_repr(self) -> str:
         return f"{self.num_adapters}, {self.out_features}, {self.in_features}, rank={self.rank}"

@@ -153,8 +153,10 @@ def sort(ids: torch.Tensor, num_experts: int) -> Order:
     another rank's experts.  ``ids`` and ``tokens`` of the order are what
     ``gemv_sorted`` and ``gemv_union`` take.
     """
-    ids, experts = _check_ids(ids, num_experts)
-    return Order(*_native.torch_binding().sort(ids, experts))
+    sort_pairs = _native.torch_binding().sort
+    if (lists := sort_pairs(ids, num_experts)) is None:  # ids that the kernels do not take as they are
+        lists = sort_pairs(*_check_ids(ids, num_experts))
+    return Order(*lists)
 
 
 def _check_rows(t: torch.Tensor, name: str, device: torch.device) -> None:
@@ -177,12 +179,15 @@ def dispatch(x: torch.Tensor, ids: torch.Tensor, num_experts: int) -> tuple[torc
     ``proj(rows[:, None], order.ids, sorted_indices=True)``.  Differentiable in ``x``: a token's gradient is the
     sum of its rows' (f32, rounded once), those left out not counted.
     """
-    ids, experts = _check_ids(ids, num_experts)
-    _check_rows(x, "x", ids.device)
-    if x.shape[:-1] != ids.shape[:-1]:
-        raise IqkKernelError(f"x {tuple(x.shape)} and ids {tuple(ids.shape)} are not of the same tokens")
-    rows, *order = _native.torch_binding().dispatch(x.contiguous(), ids, experts)
-    return rows, Order(*order)
+    dispatch_rows = _native.torch_binding().dispatch
+    if (got := dispatch_rows(x, ids, num_experts)) is None:  # what the kernels do not take as it is
+        ids, experts = _check_ids(ids, num_experts)
+        _check_rows(x, "x", ids.device)
+        if x.shape[:-1] != ids.shape[:-1]:
+            raise IqkKernelError(f"x {tuple(x.shape)} and ids {tuple(ids.shape)} are not of the same tokens")
+        got = dispatch_rows(x.contiguous(), ids, experts)
+    rows, offsets, sorted_ids, tokens, slots = got
+    return rows, Order(offsets, sorted_ids, tokens, slots)
 
 
 def combine(y: torch.Tensor, weights: torch.Tensor, order: Order | None = None, *,
@@ -196,6 +201,16 @@ def combine(y: torch.Tensor, weights: torch.Tensor, order: Order | None = None, 
     for nothing, whatever their rows hold; without an order every row counts.  Differentiable in
     ``y``, ``weights`` and ``add``; the gradients of pairs left out are 0.
     """
+    combine_rows = _native.torch_binding().combine
+    if order is None:
+        out = combine_rows(y, weights, None, None, add)
+    elif type(order) is Order:
+        out = combine_rows(y, weights, order.slots, order.offsets, add)
+    else:
+        raise IqkKernelError(f"order must be an Order, got {type(order).__name__}")
+    if out is not None:
+        return out
+    # what the kernels do not take as it is
     if not isinstance(y, torch.Tensor) or not y.is_cuda:
         raise IqkKernelError(f"y must live on a GPU, got {getattr(y, 'device', type(y).__name__)}")
     _check_rows(y, "y", y.device)
@@ -208,8 +223,8 @@ def combine(y: torch.Tensor, weights: torch.Tensor, order: Order | None = None, 
     if order is None:
         want = (*weights.shape, y.shape[-1])
     else:
-        if not isinstance(order, Order) or order.slots.shape != weights.shape:
-            raise IqkKernelError(f"order must be an Order of pairs {tuple(weights.shape)}, got {order!r}")
+        if order.slots.shape != weights.shape:
+            raise IqkKernelError(f"order must be one of pairs {tuple(weights.shape)}, got {order!r}")
         slots, offsets = order.slots, order.offsets
         for t in (slots, offsets):
             if t.device != y.device or t.dtype != torch.int32 or not t.is_contiguous():
@@ -223,7 +238,7 @@ def combine(y: torch.Tensor, weights: torch.Tensor, order: Order | None = None, 
             raise IqkKernelError(f"add must be {y.dtype} {(*weights.shape[:-1], y.shape[-1])}, got {add.dtype} "
                                  f"{tuple(add.shape)}")
         add = add.contiguous()
-    return _native.torch_binding().combine(y.contiguous(), weights.float().contiguous(), slots, offsets, add)
+    return combine_rows(y.contiguous(), weights.float().contiguous(), slots, offsets, add)
 
 
 __all__ = ["MAX_COLS", "MAX_EXPERTS", "MAX_GROUPS", "MAX_K", "Order", "balance_loss", "combine", "dispatch", "sort", "topk"]

@@ -82,19 +82,22 @@ def test_sort_and_rows_refuse_bad_arguments(lib):
     assert lib.iqk_sort(p, 0, 1 << 20, 6, 8, None, p, p, p, p, None) == _native.ERR_ARGUMENT  # no workspace
     for dtype, tokens, k, cols in ((3, 8, 6, 64), (-1, 8, 6, 64), (0, -1, 6, 64), (0, 8, 0, 64), (0, 8, 65, 64),
                                    (0, 8, 6, 0), (0, 8, 6, 1 << 28), (0, 1 << 30, 2, 64), (0, big, 1, 64)):
-        assert lib.iqk_dispatch(dtype, p, p, p, tokens, k, cols, p, None) == _native.ERR_GEOMETRY
+        assert lib.iqk_dispatch(dtype, p, p, 0, tokens, k, 8, cols, p, p, p, p, p, p, None) == _native.ERR_GEOMETRY
         assert lib.iqk_combine(dtype, p, p, p, p, p, tokens, k, cols, p, None) == _native.ERR_GEOMETRY
         assert lib.iqk_combine_grad(dtype, p, p, p, p, p, tokens, k, cols, p, p, None) == _native.ERR_GEOMETRY
-    assert lib.iqk_dispatch(0, None, p, p, 8, 6, 64, p, None) == _native.ERR_ARGUMENT
-    assert lib.iqk_dispatch(0, p, None, p, 8, 6, 64, p, None) == _native.ERR_ARGUMENT
-    assert lib.iqk_dispatch(0, p, p, p, 8, 6, 64, None, None) == _native.ERR_ARGUMENT
+    for experts in (0, 1025):
+        assert lib.iqk_dispatch(0, p, p, 0, 8, 6, experts, 64, p, p, p, p, p, p, None) == _native.ERR_GEOMETRY
+    for tokens in (8, 1 << 18):  # sorting in its own launch, and before
+        good = [0, p, p, 0, tokens, 6, 8, 64, p, p, p, p, p, p, None]
+        for place in (1, 2, 9, 10, 11, 12, 13):
+            assert lib.iqk_dispatch(*[None if i == place else v for i, v in enumerate(good)]) == _native.ERR_ARGUMENT
+    assert lib.iqk_dispatch(*[None if i == 8 else v for i, v in enumerate(good)]) == _native.ERR_ARGUMENT  # no workspace
     assert lib.iqk_combine(0, None, p, p, p, p, 8, 6, 64, p, None) == _native.ERR_ARGUMENT
     assert lib.iqk_combine(0, p, p, p, p, p, 8, 6, 64, None, None) == _native.ERR_ARGUMENT
     assert lib.iqk_combine_grad(0, None, p, p, p, p, 8, 6, 64, p, p, None) == _native.ERR_ARGUMENT
     assert lib.iqk_combine_grad(0, p, None, p, p, p, 8, 6, 64, p, p, None) == _native.ERR_ARGUMENT  # dweights want y
     assert lib.iqk_combine_grad(0, p, p, p, p, None, 8, 6, 64, p, p, None) == _native.ERR_ARGUMENT
     # nothing to do: no launch
-    assert lib.iqk_dispatch(0, None, None, None, 0, 6, 64, None, None) == _native.OK
     assert lib.iqk_combine(0, None, None, None, None, None, 0, 6, 64, None, None) == _native.OK
     assert lib.iqk_combine_grad(0, p, p, p, p, p, 8, 6, 64, None, None, None) == _native.OK
 
