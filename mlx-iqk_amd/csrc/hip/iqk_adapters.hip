@@ -31,8 +31,8 @@ struct AdapterArgs {
     // grouped form
     const uint4_t *tiles;      // adapter (the bank's size: none), -, slots (0: no such tile), -
     const uint32_t *tile_rows; // [tile][slots] their rows
-    uint4_t *pieces;          // A x of a tile's slots, split, as operand B of the second product
-    float *powers;            // [tile][slots] what the pieces are multiplied with
+    float *sums;              // [splits][tile][slots][rank] A x, in parts
+    uint32_t n_tiles, splits;
     uint32_t columns;         // 256s of outputs of a workgroup
 };
 
@@ -171,10 +171,12 @@ __global__ __launch_bounds__(kAloneThreads) void adapter_row_kernel(AdapterArgs 
 //
 // Rows sorted by adapter, in tiles of 64 slots of one adapter; both products on the
 // 16x16x32 MFMAs, operand A the adapter's (16 ranks, 16 outputs), operand B 16 slots'.  The
-// first kernel leaves A x split into 16-bit pieces that give f32 back: a bf16 product takes three
-// pieces of eight bits (truncated, so that their sum is exact), an f16 product two of eleven
-// bits over a power of two of the slot's largest, which is multiplied back in f32.
+// first kernel leaves A x in f32, a sum for each part of the columns; the second adds these
+// and splits them into 16-bit pieces that give f32 back: a bf16 product takes three pieces of eight
+// bits (truncated, so that their sum is exact), an f16 product two of eleven bits over a
+// power of two of the slot's largest, which is multiplied back in f32.
 
+constexpr uint32_t kMaxSplits = 4;  // parts of the columns
 constexpr int kTileSlots = int(kSortTile), kTileGroups = kTileSlots / 16;
 
 template <bool BF>
@@ -196,20 +198,22 @@ __device__ __forceinline__ void wavefront_fence() {
     __builtin_amdgcn_wave_barrier();
 }
 
-// A x of 16 CT slots of a tile.  WAVES wavefronts take 64 columns in turn and their sums meet in
-// LDS.  A wavefront reads 128 bytes of a row together and turns them into operand B in its
-// own part of LDS (rows read as the operand wants them, 16 of them 64 bytes each in an
-// instruction, kept the loads waiting for the cache: 8192 rows of 4096, rank 16, 34 us);
-// XD steps of x and AD of A are on their way at once.
+// A x of 16 CT slots of a tile over one of a.splits parts of the columns.  WAVES wavefronts take 64
+// columns in turn and their sums meet in LDS.  A wavefront reads 128 bytes of a row together and
+// turns them into operand B in its own part of LDS (rows read as the operand wants them, 16 of
+// them 64 bytes each in an instruction, kept the loads waiting for the cache: 8192 rows of 4096,
+// rank 16, 34 us); XD steps of x and AD of A are on their way at once.
 template <bool BF, int RT, int CT, int WAVES, int XD, int AD>
 __global__ __launch_bounds__(64 * WAVES) void adapter_down_tiles_kernel(AdapterArgs a) {
-    constexpr int SLOTS = 16 * CT, RANKS = 16 * RT, THREADS = 64 * WAVES, KC = (RT + 1) / 2, PARTS = kTileGroups / CT;
+    constexpr int SLOTS = 16 * CT, RANKS = 16 * RT, THREADS = 64 * WAVES, PARTS = kTileGroups / CT;
     constexpr int SUMS = SLOTS * (RANKS + 4), STAGE = SLOTS * 32;  // floats of a wavefront's sums, of its turned rows
     __shared__ __attribute__((aligned(16))) float shared[WAVES][SUMS > STAGE ? SUMS : STAGE];
-    const uint32_t t = blockIdx.x / PARTS, group = blockIdx.x % PARTS * CT;  // the first of its groups of 16
+    const uint32_t split = blockIdx.x % a.splits, block = blockIdx.x / a.splits;
+    const uint32_t t = block / PARTS, group = block % PARTS * CT;  // the first of its groups of 16
     const uint4_t tile = a.tiles[t];
-    const uint32_t adapter = tile.x, slots = tile.z;
-    if (slots <= 16 * group || adapter >= a.adapters) return;  // uniform
+    const uint32_t adapter = tile.x;
+    if (tile.z <= 16 * group || adapter >= a.adapters) return;  // uniform
+    const uint32_t slots = min(tile.z - 16 * group, uint32_t(SLOTS));
     const uint32_t lane = threadIdx.x & 63u, g = lane >> 4, m = lane & 15u, c8 = lane & 7u, r8 = lane >> 3;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint16_t *w[RT], *x[2 * CT];
@@ -218,7 +222,7 @@ __global__ __launch_bounds__(64 * WAVES) void adapter_down_tiles_kernel(AdapterA
         w[r] = a.down + size_t(adapter) * a.rank * a.in + 8 * min(16u * r + m, a.rank - 1u);
 #pragma unroll
     for (int c = 0; c < 2 * CT; ++c) {
-        const uint32_t slot = 16 * group + 8 * c + r8, row = a.tile_rows[t * kTileSlots + slot];
+        const uint32_t slot = 8 * c + r8, row = a.tile_rows[t * kTileSlots + 16 * group + slot];
         x[c] = a.x + size_t(slot < slots ? row : 0u) * a.in;  // past the tile's: row 0, its sums not used
     }
     float4_t acc[RT][CT];
@@ -232,7 +236,8 @@ __global__ __launch_bounds__(64 * WAVES) void adapter_down_tiles_kernel(AdapterA
     const auto load_x = [&](int d, uint32_t k0) {
         const uint32_t k = k0 + 8 * c8, at = k < a.in ? k : 0u;
 #pragma unroll
-        for (int c = 0; c < 2 * CT; ++c) xv[d][c] = *reinterpret_cast<const chunk_t *>(x[c] + at);
+        for (int c = 0; c < 2 * CT; ++c)
+            if (8u * c < slots) xv[d][c] = *reinterpret_cast<const chunk_t *>(x[c] + at);  // uniform
     };
     const auto load_w = [&](int d, uint32_t k0) {
 #pragma unroll
@@ -247,6 +252,7 @@ __global__ __launch_bounds__(64 * WAVES) void adapter_down_tiles_kernel(AdapterA
         wavefront_fence();
 #pragma unroll
         for (int c = 0; c < 2 * CT; ++c) {
+            if (8u * c >= slots) continue;
             if (rest && k0 + 8 * c8 >= a.in) xv[xd][c] = uint4_t{0, 0, 0, 0};
             turned[(8 * c + r8) * 8 + (c8 ^ r8)] = xv[xd][c];
         }
@@ -261,20 +267,26 @@ __global__ __launch_bounds__(64 * WAVES) void adapter_down_tiles_kernel(AdapterA
                 for (int r = 0; r < RT; ++r) wv[ad][h][r] = uint4_t{0, 0, 0, 0};
             }
 #pragma unroll
-            for (int r = 0; r < RT; ++r)
+            for (int c = 0; c < CT; ++c) {
+                if (16u * c >= slots) continue;
 #pragma unroll
-                for (int c = 0; c < CT; ++c) acc[r][c] = mfma<BF>(wv[ad][h][r], b[c], acc[r][c]);
+                for (int r = 0; r < RT; ++r) acc[r][c] = mfma<BF>(wv[ad][h][r], b[c], acc[r][c]);
+            }
         }
     };
     constexpr int UNROLL = XD > AD ? XD : AD;
     static_assert(UNROLL % XD == 0 && UNROLL % AD == 0, "a turn of the loop is whole turns of both rings");
     // Each workgroup begins at another step: in step with each other they would all read the same
-    // eighth of rows that lie a power of two apart, from few of the memory's channels.
-    const uint32_t steps = (a.in + STEP - 1) / STEP, turn = blockIdx.x % steps;
-    const auto column = [&](uint32_t i) { return 64 * wave + STEP * (i + turn < steps ? i + turn : i + turn - steps); };
+    // part of rows that lie a power of two apart, from few of the memory's channels.
+    const uint32_t units = (a.in + 63) / 64, each = (units + a.splits - 1) / a.splits;
+    const uint32_t first = min(units, split * each), last = min(units, first + each);
+    const uint32_t steps = (last - first + WAVES - 1) / WAVES, turn = steps ? block % steps : 0u;
+    const auto column = [&](uint32_t i) {
+        return 64 * (first + wave) + STEP * (i + turn < steps ? i + turn : i + turn - steps);
+    };
 #pragma unroll
     for (int d = 0; d < UNROLL - 1; ++d) {  // the oldest step's loads first
-        if (d < XD - 1) load_x(d, column(min(uint32_t(d), steps - 1u)));
+        if (d < XD - 1) load_x(d, column(min(uint32_t(d), steps - 1u)));  // (with no steps: any, not used)
         if (d < AD - 1) load_w(d, column(min(uint32_t(d), steps - 1u)));
         __builtin_amdgcn_sched_barrier(0);
     }
@@ -284,7 +296,7 @@ __global__ __launch_bounds__(64 * WAVES) void adapter_down_tiles_kernel(AdapterA
             load_x((d + XD - 1) % XD, column(min(i0 + d + XD - 1, steps - 1u)));
             load_w((d + AD - 1) % AD, column(min(i0 + d + AD - 1, steps - 1u)));
             __builtin_amdgcn_sched_barrier(0);
-            if (i0 + d < steps && column(i0 + d) < a.in) multiply(d % XD, d % AD, column(i0 + d));  // uniform
+            if (i0 + d < steps && column(i0 + d) < 64 * last) multiply(d % XD, d % AD, column(i0 + d));  // uniform
         }
     }
     wavefront_fence();
@@ -294,73 +306,31 @@ __global__ __launch_bounds__(64 * WAVES) void adapter_down_tiles_kernel(AdapterA
 #pragma unroll
         for (int c = 0; c < CT; ++c) *reinterpret_cast<float4_t *>(&part(wave, 16 * c + m, 16 * r + 4 * g)) = acc[r][c];
     __syncthreads();
-    const float scale = a.scales[adapter];
-    constexpr int UNITS = 4 * KC;  // eights of a slot's ranks, rounded up to whole operands
-    for (uint32_t u = threadIdx.x; u < SLOTS * UNITS; u += THREADS) {
-        const uint32_t slot = u / UNITS, unit = u % UNITS, r0 = 8 * unit;
-        float v[8];
+    for (uint32_t u = threadIdx.x; u < SLOTS * 2 * RT; u += THREADS) {
+        const uint32_t slot = u / (2 * RT), r0 = 8 * (u % (2 * RT));
+        if (r0 >= a.rank || slot >= slots) continue;
+        float4_t lo = {0, 0, 0, 0}, hi = {0, 0, 0, 0};
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = 0.f;
-        if (r0 < a.rank) {  // whole eights
-#pragma unroll
-            for (int k = 0; k < WAVES; ++k)
-#pragma unroll
-                for (int i = 0; i < 8; ++i) v[i] += part(k, slot, r0 + i);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] *= scale;
+        for (int k = 0; k < WAVES; ++k) {
+            lo += *reinterpret_cast<const float4_t *>(&part(k, slot, r0));
+            hi += *reinterpret_cast<const float4_t *>(&part(k, slot, r0 + 4));
         }
-        // operand B of chunk kc: lane 16 g + n has slot n's ranks 32 kc + 8 g ..
-        const size_t at = ((size_t(t) * kTileGroups + group + slot / 16) * KC + unit / 4) * kPieces<BF> * 64 +
-                          16 * (unit & 3u) + (slot & 15u);
-        if constexpr (BF) {
-#pragma unroll
-            for (int p = 0; p < 3; ++p) {
-                uint4_t out;
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const uint32_t bits = __builtin_bit_cast(uint32_t, v[i]);
-                    const bool finite = (bits & 0x7f800000u) != 0x7f800000u;
-                    uint32_t top = bits >> 16;
-                    if (!finite && (bits & 0x7fffffu)) top |= 0x40u;  // a NaN stays one
-                    v[i] = finite ? v[i] - __builtin_bit_cast(float, bits & 0xffff0000u) : 0.f;
-                    out[i / 2] = i & 1 ? out[i / 2] | top << 16 : top;
-                }
-                a.pieces[at + 64 * p] = out;
-            }
-        } else {
-            float most = 0.f;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) most = fmaxf(most, fabsf(v[i]));
-#pragma unroll
-            for (int off = 1; off < UNITS; off <<= 1) most = fmaxf(most, __shfl_xor(most, off, 64));
-            // the largest to 2^14 .. 2^15; with an infinity (or nothing) as it is
-            const int e = most > 0.f && most < __builtin_inff() ? 14 - ilogbf(most) : 0;
-            uint4_t hi, lo;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float scaled = ldexpf(v[i], e);
-                const uint32_t top = float_to_half_bits(scaled);
-                const float rest = fabsf(scaled) < __builtin_inff() ? scaled - half_bits_to_float(top) : 0.f;
-                const uint32_t low = float_to_half_bits(rest);
-                hi[i / 2] = i & 1 ? hi[i / 2] | top << 16 : top;
-                lo[i / 2] = i & 1 ? lo[i / 2] | low << 16 : low;
-            }
-            a.pieces[at] = hi;
-            a.pieces[at + 64] = lo;
-            if (unit == 0) a.powers[size_t(t) * kTileSlots + 16 * group + slot] = ldexpf(1.f, -e);
-        }
+        float4_t *const out = reinterpret_cast<float4_t *>(
+            a.sums + ((size_t(split) * a.n_tiles + t) * kTileSlots + 16 * group + slot) * a.rank + r0);
+        out[0] = lo;
+        out[1] = hi;
     }
 }
 
 // Outputs of a tile: 256 at a time, of which a wavefront takes 64 for all slots, the next 256's
-// y and B on their way meanwhile.  The slots' operands lie in LDS for all of them (KC chunks of
-// 32 ranks), and the sums go through it: the matrix cores leave four outputs of 16 slots to
+// y and B on their way meanwhile.  The slots' operands are made once, in LDS (KC chunks of 32 ranks), and the sums go through it: the matrix cores leave four outputs of 16 slots to
 // 64 lanes, memory wants 64 outputs of a slot together.
 template <bool BF, int KC>
 __global__ __launch_bounds__(256) void adapter_up_tiles_kernel(AdapterArgs a) {
     constexpr int P = kPieces<BF>, CT = kTileGroups, STAGE = KC < 2 ? KC : 2;  // chunks of B in registers at once
     constexpr bool AHEAD = KC <= 2;  // of B; y always is
     __shared__ uint4_t operands[CT][KC][P][64];
+    __shared__ float powers[kTileSlots];  // what an f16 slot's sums are multiplied with
     __shared__ __attribute__((aligned(16))) float turned[4][16][64 + 4];
     const uint32_t groups = (a.N + 256 * a.columns - 1) / (256 * a.columns), t = blockIdx.x / groups;
     const uint32_t lane = threadIdx.x & 63u, g = lane >> 4, m = lane & 15u, s8 = lane >> 3;
@@ -423,15 +393,74 @@ __global__ __launch_bounds__(256) void adapter_up_tiles_kernel(AdapterArgs a) {
     load_y(0, column(0));
     if (AHEAD) load_w(0, column(0), 0);
     __builtin_amdgcn_sched_barrier(0);
+    // A x: the parts' sum, scaled, in pieces; a thread has eight ranks of a slot, 4 KC threads a slot
+    constexpr int EIGHTS = 4 * KC;
+    const float scale = a.scales[adapter];
 #pragma unroll
-    for (int i = 0; i < CT * KC * P * 64 / 256; ++i) {  // a group's operands lie together
-        const uint32_t u = 256 * i + threadIdx.x;
-        if (16 * (u / (KC * P * 64)) < slots) (&operands[0][0][0][0])[u] = a.pieces[size_t(t) * CT * KC * P * 64 + u];
+    for (int i = 0; i < kTileSlots * EIGHTS / 256; ++i) {
+        const uint32_t u = 256 * i + threadIdx.x, slot = u / EIGHTS, eight = u % EIGHTS;
+        float v[8] = {};
+        if (8 * eight < a.rank && slot < slots) {
+            const float *const from = a.sums + (size_t(t) * kTileSlots + slot) * a.rank + 8 * eight;
+            float4_t parts[kMaxSplits][2];  // all on their way at once; past the last: it again
+#pragma unroll
+            for (uint32_t p = 0; p < kMaxSplits; ++p) {
+                const float4_t *const part = reinterpret_cast<const float4_t *>(
+                    from + size_t(min(p, a.splits - 1u)) * a.n_tiles * kTileSlots * a.rank);
+                parts[p][0] = part[0];
+                parts[p][1] = part[1];
+            }
+#pragma unroll
+            for (uint32_t p = 0; p < kMaxSplits; ++p) {
+                if (p >= a.splits) continue;  // uniform
+#pragma unroll
+                for (int k = 0; k < 4; ++k) v[k] += parts[p][0][k], v[4 + k] += parts[p][1][k];
+            }
+#pragma unroll
+            for (int k = 0; k < 8; ++k) v[k] *= scale;
+        }
+        // operand B of a chunk of 32 ranks: lane 16 g + n has slot n's ranks 8 g ..
+        uint4_t(*const to)[64] = operands[slot / 16][eight / 4];
+        const uint32_t at = 16 * (eight & 3u) + (slot & 15u);
+        if constexpr (BF) {
+#pragma unroll
+            for (int p = 0; p < 3; ++p) {
+                uint4_t out;
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    const uint32_t bits = __builtin_bit_cast(uint32_t, v[k]);
+                    const bool finite = (bits & 0x7f800000u) != 0x7f800000u;
+                    uint32_t top = bits >> 16;
+                    if (!finite && (bits & 0x7fffffu)) top |= 0x40u;  // a NaN stays one
+                    v[k] = finite ? v[k] - __builtin_bit_cast(float, bits & 0xffff0000u) : 0.f;
+                    out[k / 2] = k & 1 ? out[k / 2] | top << 16 : top;
+                }
+                to[p][at] = out;
+            }
+        } else {
+            float most = 0.f;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) most = fmaxf(most, fabsf(v[k]));
+#pragma unroll
+            for (int off = 1; off < EIGHTS; off <<= 1) most = fmaxf(most, __shfl_xor(most, off, 64));
+            // the largest to 2^14 .. 2^15; with an infinity (or nothing) as it is
+            const int e = most > 0.f && most < __builtin_inff() ? 14 - ilogbf(most) : 0;
+            uint4_t hi, lo;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const float scaled = ldexpf(v[k], e);
+                const uint32_t top = float_to_half_bits(scaled);
+                const float rest = fabsf(scaled) < __builtin_inff() ? scaled - half_bits_to_float(top) : 0.f;
+                const uint32_t low = float_to_half_bits(rest);
+                hi[k / 2] = k & 1 ? hi[k / 2] | top << 16 : top;
+                lo[k / 2] = k & 1 ? lo[k / 2] | low << 16 : low;
+            }
+            to[0][at] = hi;
+            to[1][at] = lo;
+            if (eight == 0) powers[slot] = ldexpf(1.f, -e);
+        }
     }
     __syncthreads();
-    float power[CT];
-#pragma unroll
-    for (int c = 0; c < CT; ++c) power[c] = BF || 16u * c >= slots ? 1.f : a.powers[size_t(t) * kTileSlots + 16 * c + m];
     const auto compute = [&](int d, uint32_t n0) {
         const uint32_t n = n0 + mine, have = n < a.N ? min(a.N - n, 8u) : 0u;
         if constexpr (AHEAD) {  // past the ranks: zeros, as in the slots' operands
@@ -470,10 +499,11 @@ __global__ __launch_bounds__(256) void adapter_up_tiles_kernel(AdapterArgs a) {
                     }
             }
             wavefront_fence();
+            const float power = BF ? 1.f : powers[16 * c + m];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 float4_t v = acc[j];
-                if constexpr (!BF) v *= power[c];
+                if constexpr (!BF) v *= power;
                 *reinterpret_cast<float4_t *>(&turned[wave][m][16 * j + 4 * g]) = v;
             }
             wavefront_fence();
@@ -523,18 +553,20 @@ bool adapters_shape_ok(int64_t in, int64_t out, int64_t rank, int64_t adapters, 
            adapters > 0 && adapters <= kAdaptersMax && rows >= 0 && rows < kLim;
 }
 
-constexpr int64_t kRowsAlone = 64;  // rows up to which each is computed on its own
+constexpr int64_t kRowsAlone = 0;  // rows up to which each is computed on its own
 
 // The grouped form's workspace, in words: where each part begins.
 struct GroupPlan {
-    int64_t tiles, hist, desc, tile_rows, pieces, powers, words;
+    int64_t tiles, splits, hist, desc, tile_rows, sums, words;
 };
 
-GroupPlan group_plan(int64_t rank, int64_t adapters, int64_t rows) {
+GroupPlan group_plan(int64_t in, int64_t rank, int64_t adapters, int64_t rows) {
     GroupPlan p{};
     p.tiles = sort_tiles(rows, adapters);
-    int64_t chunks = 1;  // operands of 32 ranks: a power of two of them
-    while (32 * chunks < rank) chunks *= 2;
+    // the columns in parts where the tiles leave CUs empty: two workgroups a CU, 512 columns each at least
+    const int64_t want = 512 / p.tiles, most = in / 512;
+    p.splits = want < 1 || most < 1 ? 1 : want < most ? want : most;
+    if (p.splits > kMaxSplits) p.splits = kMaxSplits;
     const auto take = [&](int64_t words) {
         const int64_t at = p.words;
         p.words += (words + 3) / 4 * 4;  // 16-byte steps
@@ -543,8 +575,7 @@ GroupPlan group_plan(int64_t rank, int64_t adapters, int64_t rows) {
     p.hist = take(sort_plan(rows, adapters).words);
     p.desc = take(4 * p.tiles);
     p.tile_rows = take(p.tiles * kTileSlots);
-    p.pieces = take(p.tiles * kTileGroups * chunks * 3 * 64 * 4);
-    p.powers = take(p.tiles * kTileSlots);
+    p.sums = take(p.splits * p.tiles * kTileSlots * rank);
     return p;
 }
 
@@ -553,11 +584,11 @@ template <typename F>
 void by_ranks(int64_t rank, F &&f) {
     using std::integer_sequence;
     if (rank <= 16)
-        f(integer_sequence<int, 1, 2, 8, 4, 4>{});
+        f(integer_sequence<int, 1, 4, 4, 4, 4>{});
     else if (rank <= 32)
-        f(integer_sequence<int, 2, 2, 8, 4, 2>{});
+        f(integer_sequence<int, 2, 4, 4, 4, 2>{});
     else if (rank <= 64)
-        f(integer_sequence<int, 4, 2, 8, 4, 2>{});
+        f(integer_sequence<int, 4, 4, 4, 2, 2>{});
     else if (rank <= 128)
         f(integer_sequence<int, 8, 2, 4, 2, 1>{});
     else
@@ -569,7 +600,7 @@ hipError_t launch_tiles(const AdapterArgs &a, int64_t tiles, hipStream_t stream,
                         std::integer_sequence<int, RT, CT, WAVES, XD, AD>) {
     const int64_t ups = tiles * ((int64_t(a.N) + 256 * a.columns - 1) / (256 * a.columns));
     hipLaunchKernelGGL((adapter_down_tiles_kernel<BF, RT, CT, WAVES, XD, AD>),
-                       dim3{uint32_t(tiles * (kTileGroups / CT))}, dim3{64 * WAVES}, 0, stream, a);
+                       dim3{uint32_t(tiles * a.splits * (kTileGroups / CT))}, dim3{64 * WAVES}, 0, stream, a);
     if (const hipError_t err = hipGetLastError(); err != hipSuccess) return err;
     hipLaunchKernelGGL((adapter_up_tiles_kernel<BF, (RT + 1) / 2>), dim3{uint32_t(ups)}, dim3{256}, 0, stream, a);
     return hipGetLastError();
@@ -591,11 +622,14 @@ int rows_alone(const AdapterArgs &a, bool bf, hipStream_t stream) {
 }
 
 int rows_grouped(AdapterArgs a, bool bf, uint32_t *work, hipStream_t stream) {
-    const GroupPlan p = group_plan(a.rank, a.adapters, a.T);
-    // workgroups of up to 8 x 256 outputs, about two a CU
-    const int64_t wide = (int64_t(a.N) + 255) / 256, each = p.tiles * wide / 512;
-    a.columns = uint32_t(each < 1 ? 1 : each > 8 ? 8 : each);
-    if (!grid_ok(p.tiles * wide, 256) || !grid_ok(p.tiles * kTileGroups, 512)) return IQK_ERR_GEOMETRY;
+    const GroupPlan p = group_plan(a.in, a.rank, a.adapters, a.T);
+    // workgroups of up to 4 x 256 outputs, about eight a CU: with two that stay, a last one makes
+    // a CU take half as long again (8192 rows [8192 x 512] of rank 16: 83 us, 75 so).  Beyond rank 64
+    // the slots' operands, made anew by each, cost more than that.
+    const int64_t wide = (int64_t(a.N) + 255) / 256, all = p.tiles * wide, each = a.rank > 64 ? all / 512 : all / 2048;
+    const int64_t most = a.rank > 64 ? 8 : 4;
+    a.columns = uint32_t(each < 1 ? 1 : each > most ? most : each);
+    if (!grid_ok(all, 256) || !grid_ok(p.tiles * p.splits * kTileGroups, 512)) return IQK_ERR_GEOMETRY;
     SortCall c{};
     c.ids = a.ids;
     c.wide = a.wide;
@@ -610,8 +644,9 @@ int rows_grouped(AdapterArgs a, bool bf, uint32_t *work, hipStream_t stream) {
     if (const int rc = sort_launch(c, stream); rc != IQK_OK) return rc;
     a.tiles = reinterpret_cast<const uint4_t *>(work + p.desc);
     a.tile_rows = work + p.tile_rows;
-    a.pieces = reinterpret_cast<uint4_t *>(work + p.pieces);
-    a.powers = reinterpret_cast<float *>(work + p.powers);
+    a.sums = reinterpret_cast<float *>(work + p.sums);
+    a.n_tiles = uint32_t(p.tiles);
+    a.splits = uint32_t(p.splits);
     hipError_t err = hipSuccess;
     by_ranks(a.rank, [&](auto shape) {
         err = bf ? launch_tiles<true>(a, p.tiles, stream, shape) : launch_tiles<false>(a, p.tiles, stream, shape);
@@ -627,7 +662,7 @@ extern "C" {
 int64_t iqk_adapters_work(int64_t in_features, int64_t out_features, int64_t rank, int64_t num_adapters, int64_t rows) {
     using namespace iqk;
     if (!adapters_shape_ok(in_features, out_features, rank, num_adapters, rows)) return -1;
-    return rows <= kRowsAlone ? 0 : group_plan(rank, num_adapters, rows).words;
+    return rows <= kRowsAlone ? 0 : group_plan(in_features, rank, num_adapters, rows).words;
 }
 
 int iqk_adapters(int dtype, int64_t in_features, int64_t out_features, int64_t rank, int64_t num_adapters,
