@@ -237,7 +237,7 @@ __global__ __launch_bounds__(64 * WAVES) void adapter_down_tiles_kernel(AdapterA
         const uint32_t k = k0 + 8 * c8, at = k < a.in ? k : 0u;
 #pragma unroll
         for (int c = 0; c < 2 * CT; ++c)
-            if (8u * c < slots) xv[d][c] = *reinterpret_cast<const chunk_t *>(x[c] + at);  // uniform
+            if (8u * c < slots) xv[d][c] = __builtin_nontemporal_load(reinterpret_cast<const chunk_t *>(x[c] + at));  // uniform
     };
     const auto load_w = [&](int d, uint32_t k0) {
 #pragma unroll
@@ -324,7 +324,8 @@ __global__ __launch_bounds__(64 * WAVES) void adapter_down_tiles_kernel(AdapterA
 
 // Outputs of a tile: 256 at a time, of which a wavefront takes 64 for all slots, the next 256's
 // y and B on their way meanwhile.  The slots' operands are made once, in LDS (KC chunks of 32 ranks), and the sums go through it: the matrix cores leave four outputs of 16 slots to
-// 64 lanes, memory wants 64 outputs of a slot together.
+// 64 lanes, memory wants 64 outputs of a slot together.  x, y and the outputs pass through once
+// and do not stay in the caches in place of A, B and the sums (8192 rows of rank 64 [8192 x 4096]: 101 us, 96 so).
 template <bool BF, int KC>
 __global__ __launch_bounds__(256) void adapter_up_tiles_kernel(AdapterArgs a) {
     constexpr int P = kPieces<BF>, CT = kTileGroups, STAGE = KC < 2 ? KC : 2;  // chunks of B in registers at once
@@ -376,7 +377,10 @@ __global__ __launch_bounds__(256) void adapter_up_tiles_kernel(AdapterArgs a) {
             if (16u * c >= slots) continue;  // uniform
 #pragma unroll
             for (int h = 0; h < 2; ++h)
-                if (n0 + mine + 8 <= a.N) y[d][c][h] = *reinterpret_cast<const chunk_t *>(a.y + size_t(row[c][h]) * a.N + n0 + mine);
+                if (n0 + mine + 8 <= a.N) {
+                    const uint16_t *const from = a.y + size_t(row[c][h]) * a.N + n0 + mine;
+                    y[d][c][h] = __builtin_nontemporal_load(reinterpret_cast<const chunk_t *>(from));
+                }
         }
     };
     const auto load_w = [&](int d, uint32_t n0, uint32_t k0) {
@@ -521,7 +525,7 @@ __global__ __launch_bounds__(256) void adapter_up_tiles_kernel(AdapterArgs a) {
                         const float v0 = i < 2 ? lo[2 * i] : hi[2 * i - 4], v1 = i < 2 ? lo[2 * i + 1] : hi[2 * i - 3];
                         out[i] = pair_bits<BF>(old.x + v0, old.y + v1);
                     }
-                    *reinterpret_cast<chunk_t *>(a.out + at) = out;
+                    __builtin_nontemporal_store(chunk_t(out), reinterpret_cast<chunk_t *>(a.out + at));
                 } else {
                     for (uint32_t i = 0; i < have; ++i) {
                         const float sum = float_of16<BF>(a.y[at + i]) + v[i];
@@ -553,7 +557,7 @@ bool adapters_shape_ok(int64_t in, int64_t out, int64_t rank, int64_t adapters, 
            adapters > 0 && adapters <= kAdaptersMax && rows >= 0 && rows < kLim;
 }
 
-constexpr int64_t kRowsAlone = 0;  // rows up to which each is computed on its own
+constexpr int64_t kRowsAlone = 64;  // rows up to which each is computed on its own
 
 // The grouped form's workspace, in words: where each part begins.
 struct GroupPlan {

@@ -306,10 +306,15 @@ __device__ __forceinline__ uint4_t pack(const float (&v)[kChunk<DT>]) {
     return w;
 }
 
-// A chunk, or (not WHOLE) its first `halves` (1 .. 7) 16-bit halves and zeros behind them.
-template <bool WHOLE>
+// A chunk, or (not WHOLE) its first `halves` (1 .. 7) 16-bit halves and zeros behind them.  ONCE:
+// of the slots' rows, which are many and pass through once, so that they do not stay in the caches in
+// place of what does not (16384 tokens, 6 rows of 8 KiB each: their sum 185 us, 161 so; rows and
+// gradient of a training step 391, 345).
+template <bool WHOLE, bool ONCE = false>
 __device__ __forceinline__ uint4_t load_chunk(const uint8_t *p, uint32_t halves) {
-    if constexpr (WHOLE) {
+    if constexpr (WHOLE && ONCE) {
+        return __builtin_nontemporal_load(reinterpret_cast<const chunk_t *>(p));
+    } else if constexpr (WHOLE) {
         return *reinterpret_cast<const chunk_t *>(p);
     } else {
         uint4_t w = {0, 0, 0, 0};
@@ -320,9 +325,11 @@ __device__ __forceinline__ uint4_t load_chunk(const uint8_t *p, uint32_t halves)
     }
 }
 
-template <bool WHOLE>
+template <bool WHOLE, bool ONCE = false>
 __device__ __forceinline__ void store_chunk(uint8_t *p, uint4_t w, uint32_t halves) {
-    if constexpr (WHOLE) {
+    if constexpr (WHOLE && ONCE) {
+        __builtin_nontemporal_store(chunk_t(w), reinterpret_cast<chunk_t *>(p));
+    } else if constexpr (WHOLE) {
         *reinterpret_cast<chunk_t *>(p) = w;
     } else {
 #pragma unroll
@@ -374,7 +381,7 @@ __device__ __forceinline__ void dispatch_chunk(const RowArgs &a, const PLACE &at
     for (uint32_t j = 0; j < a.k; ++j) {
         const uint32_t slot = uint32_t(a.slots[size_t(at.t) * a.k + j]);
         if (slot < a.P)
-            store_chunk<WHOLE>(a.out + size_t(slot) * a.row + column, slot < kept ? w : uint4_t{0, 0, 0, 0}, at.halves);
+            store_chunk<WHOLE, true>(a.out + size_t(slot) * a.row + column, slot < kept ? w : uint4_t{0, 0, 0, 0}, at.halves);
     }
 }
 
@@ -452,7 +459,7 @@ __device__ __forceinline__ void combine_chunk(const RowArgs &a, const PLACE &at)
         }
 #pragma unroll
         for (int i = 0; i < kAhead; ++i)
-            if (slot[i] < kept) w[i] = load_chunk<WHOLE>(a.in + size_t(slot[i]) * a.row + column, at.halves);
+            if (slot[i] < kept) w[i] = load_chunk<WHOLE, true>(a.in + size_t(slot[i]) * a.row + column, at.halves);
 #pragma unroll
         for (int i = 0; i < kAhead; ++i) {
             if (slot[i] >= kept) continue;
@@ -494,7 +501,7 @@ __device__ __forceinline__ void grad_chunk(const RowArgs &a, uint32_t t, uint32_
     if (a.dweights) {
 #pragma unroll
         for (int i = 0; i < kAhead; ++i)
-            if (slot[i] < kept) w[i] = load_chunk<WHOLE>(a.y + size_t(slot[i]) * a.row + column, halves);
+            if (slot[i] < kept) w[i] = load_chunk<WHOLE, true>(a.y + size_t(slot[i]) * a.row + column, halves);
     }
     float g[N];
     unpack<DT>(gw, g);
@@ -505,7 +512,7 @@ __device__ __forceinline__ void grad_chunk(const RowArgs &a, uint32_t t, uint32_
             float v[N];
 #pragma unroll
             for (int n = 0; n < N; ++n) v[n] = weight[i] * g[n];
-            store_chunk<WHOLE>(a.out + size_t(slot[i]) * a.row + column,
+            store_chunk<WHOLE, true>(a.out + size_t(slot[i]) * a.row + column,
                                slot[i] < kept ? pack<DT>(v) : uint4_t{0, 0, 0, 0}, halves);
         }
     }
