@@ -78,10 +78,9 @@ constexpr uint16_t kNaN16 = BF ? 0x7fc0 : kHalfNaN;
 // wavefront four units at a time; B's and y's loads, which wait for nothing, are on their way from the start.
 constexpr int kAloneWaves = 16, kAloneThreads = 64 * kAloneWaves;
 
-// UP: eights of ranks whose B is loaded ahead (0: none).
-template <bool BF, int UP>
+// GROUPS of 16 ranks and AHEAD units at once; UP: eights of ranks whose B is loaded ahead (0: none).
+template <bool BF, int GROUPS, int AHEAD, int UP>
 __global__ __launch_bounds__(kAloneThreads) void adapter_row_kernel(AdapterArgs a) {
-    constexpr int GROUPS = 4, AHEAD = 4;  // groups of 16 ranks, and units, at once
     __shared__ float part[kAloneWaves][kRankMax];
     __shared__ __attribute__((aligned(16))) float t[kRankMax];
     const uint32_t columns = (a.N + kAloneThreads - 1) / kAloneThreads, row = blockIdx.x / columns;
@@ -107,6 +106,7 @@ __global__ __launch_bounds__(kAloneThreads) void adapter_row_kernel(AdapterArgs 
             uint4_t xv[AHEAD], wv[AHEAD][GROUPS];
 #pragma unroll
             for (int i = 0; i < AHEAD; ++i) {
+                if (c0 - (lane >> 4) + 4 * kAloneWaves * i >= units) continue;  // uniform
                 const uint32_t c = min(c0 + 4 * kAloneWaves * i, units - 1u);
                 xv[i] = *reinterpret_cast<const chunk_t *>(x + 8 * size_t(c));
 #pragma unroll
@@ -557,7 +557,16 @@ bool adapters_shape_ok(int64_t in, int64_t out, int64_t rank, int64_t adapters, 
            adapters > 0 && adapters <= kAdaptersMax && rows >= 0 && rows < kLim;
 }
 
-constexpr int64_t kRowsAlone = 64;  // rows up to which each is computed on its own
+// Whether rows are computed each on its own, by what its workgroups read of the adapters, each and
+// together.  us alone and grouped, bf16, 64 adapters: [8192 x 4096] of rank 16, 64 rows (80 MiB) 11.6,
+// 19.3, 128 rows (160 MiB) 25.8, 22.6; of rank 32, 32 rows (80 MiB) 12.6, 17.5, 64 rows (160 MiB) 21.7, 20.7; of
+// rank 64, 16 rows (80 MiB) 15.6, 16.3, 32 rows (160 MiB) 20.2, 20.8; [4096 x 4096] of rank 128, one row
+// (1.3 MiB a workgroup) 18.5, 14.5; [1001 x 1440] of rank 20, 512 rows (57 MiB) 11.2, 19.0; [512 x 512] of rank
+// 8, 512 rows 7.1, 13.6, 1024 rows 17.4, 15.7.
+bool rows_stand_alone(int64_t in, int64_t out, int64_t rank, int64_t rows) {
+    const int64_t groups = rows * ((out + kAloneThreads - 1) / kAloneThreads), each = rank * (in + kAloneThreads) * 2;
+    return groups <= 1024 && each <= int64_t(1) << 20 && groups * each <= int64_t(128) << 20;
+}
 
 // The grouped form's workspace, in words: where each part begins.
 struct GroupPlan {
@@ -617,11 +626,11 @@ int rows_alone(const AdapterArgs &a, bool bf, hipStream_t stream) {
         hipLaunchKernelGGL(kernel, dim3{uint32_t(blocks)}, dim3{kAloneThreads}, 0, stream, a);
     };
     if (a.rank <= 16)
-        bf ? run(adapter_row_kernel<true, 2>) : run(adapter_row_kernel<false, 2>);
+        bf ? run(adapter_row_kernel<true, 1, 2, 2>) : run(adapter_row_kernel<false, 1, 2, 2>);
     else if (a.rank <= 32)
-        bf ? run(adapter_row_kernel<true, 4>) : run(adapter_row_kernel<false, 4>);
+        bf ? run(adapter_row_kernel<true, 2, 2, 4>) : run(adapter_row_kernel<false, 2, 2, 4>);
     else
-        bf ? run(adapter_row_kernel<true, 0>) : run(adapter_row_kernel<false, 0>);
+        bf ? run(adapter_row_kernel<true, 4, 4, 0>) : run(adapter_row_kernel<false, 4, 4, 0>);
     return record_launch(hipGetLastError());
 }
 
@@ -666,7 +675,8 @@ extern "C" {
 int64_t iqk_adapters_work(int64_t in_features, int64_t out_features, int64_t rank, int64_t num_adapters, int64_t rows) {
     using namespace iqk;
     if (!adapters_shape_ok(in_features, out_features, rank, num_adapters, rows)) return -1;
-    return rows <= kRowsAlone ? 0 : group_plan(in_features, rank, num_adapters, rows).words;
+    return rows_stand_alone(in_features, out_features, rank, rows)
+               ? 0 : group_plan(in_features, rank, num_adapters, rows).words;
 }
 
 int iqk_adapters(int dtype, int64_t in_features, int64_t out_features, int64_t rank, int64_t num_adapters,
@@ -676,8 +686,9 @@ int iqk_adapters(int dtype, int64_t in_features, int64_t out_features, int64_t r
     if (dtype != MX_F16 && dtype != MX_BF16) return IQK_ERR_ARGUMENT;
     if (!adapters_shape_ok(in_features, out_features, rank, num_adapters, rows)) return IQK_ERR_GEOMETRY;
     if (rows == 0) return IQK_OK;
+    const bool alone = rows_stand_alone(in_features, out_features, rank, rows);
     if (!x || !ids || rows_per_id <= 0 || rows_per_id >= (int64_t(1) << 31) || !down || !up || !scales || !y || !out ||
-        (rows > kRowsAlone && !work))
+        (!alone && !work))
         return IQK_ERR_ARGUMENT;
     if ((reinterpret_cast<uintptr_t>(down) | reinterpret_cast<uintptr_t>(up) | reinterpret_cast<uintptr_t>(work)) & 15u)
         return IQK_ERR_ARGUMENT;
@@ -697,7 +708,7 @@ int iqk_adapters(int dtype, int64_t in_features, int64_t out_features, int64_t r
     a.wide = wide_ids != 0;
     a.per_id = uint32_t(rows_per_id);
     const bool bf = dtype == MX_BF16;
-    return rows <= kRowsAlone ? rows_alone(a, bf, as_stream(stream)) : rows_grouped(a, bf, work, as_stream(stream));
+    return alone ? rows_alone(a, bf, as_stream(stream)) : rows_grouped(a, bf, work, as_stream(stream));
 }
 
 }  // extern "C"

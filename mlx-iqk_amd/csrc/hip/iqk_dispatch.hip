@@ -27,12 +27,12 @@ constexpr int64_t kSortMaxK = 64;
 constexpr int kSortKeys = int(kSortMaxExperts) + 1;
 constexpr int kSortWaves = 16, kSortThreads = 64 * kSortWaves;
 // Pairs up to which every workgroup counts all of them itself, in one launch.
-constexpr int64_t kSortOne = 16384;
+constexpr int64_t kSortOne = 12288;
 constexpr int64_t kSortBlocks = 64;  // workgroups of a sort, at most
 
 struct SortArgs {
     const uint32_t *ids;
-    uint32_t *hist;  // [blocks][hist_stride(E)], 16-byte aligned, or null: every workgroup counts all pairs
+    uint32_t *hist;  // [blocks][E + 1], or null: every workgroup counts all pairs
     int32_t *offsets, *sorted_ids, *tokens, *slots;
     uint32_t P, E, k, share;  // share: pairs of a workgroup, in order
     uint32_t per_id;          // pairs of an id
@@ -69,7 +69,7 @@ __device__ __forceinline__ uint32_t rank_in(uint64_t lanes) {
 // loads of ids are on their way at once.
 template <bool WIDE, uint32_t STRIDE, typename F>
 __device__ __forceinline__ void count_keys(const SortArgs &a, uint32_t base, uint32_t end, F &&add) {
-    constexpr int AHEAD = 4;
+    constexpr int AHEAD = 8;
     const uint32_t lane = threadIdx.x & 63u;
     for (; base < end; base += AHEAD * STRIDE) {
         uint32_t key[AHEAD];
@@ -90,22 +90,19 @@ __device__ __forceinline__ void count_keys(const SortArgs &a, uint32_t base, uin
 
 __device__ __forceinline__ int key_bits(const SortArgs &a) { return 32 - __clz(int(a.E)); }  // of the largest key, E
 
-// Words from one workgroup's counts to the next one's: whole 16 bytes.
-__host__ __device__ constexpr int64_t hist_stride(int64_t experts) { return (experts + 1 + 3) / 4 * 4; }
-
 // A workgroup's counts of its share of the pairs, by key.
 template <bool WIDE>
 __global__ __launch_bounds__(kSortThreads) void sort_count_kernel(SortArgs a) {
-    __shared__ uint32_t count[kSortKeys + 3];
-    const uint32_t stride = uint32_t(hist_stride(a.E));
-    for (uint32_t e = threadIdx.x; e < stride; e += kSortThreads) count[e] = 0;
+    __shared__ uint32_t count[kSortKeys];
+    const uint32_t K = a.E + 1;
+    for (uint32_t e = threadIdx.x; e < K; e += kSortThreads) count[e] = 0;
     __syncthreads();
     const uint32_t lo = min(a.P, blockIdx.x * a.share), hi = min(a.P, lo + a.share);
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     count_keys<WIDE, kSortThreads>(a, lo + 64 * wave, hi,
                                    [&](uint32_t key, uint32_t, uint32_t n) { atomicAdd(&count[key], n); });
     __syncthreads();
-    for (uint32_t e = threadIdx.x; e < stride; e += kSortThreads) a.hist[size_t(blockIdx.x) * stride + e] = count[e];
+    for (uint32_t e = threadIdx.x; e < K; e += kSortThreads) a.hist[size_t(blockIdx.x) * K + e] = count[e];
 }
 
 template <int WAVES>
@@ -149,45 +146,52 @@ __device__ __forceinline__ void scan_keys(SortShared<WAVES> &s, uint32_t K, F &&
 
 // place(pair, key, slot) for the pairs lo .. hi of a workgroup, whose `blocks` workgroups' shares
 // follow each other.  Its wavefronts take equal parts of the share in order; a wavefront ranks 64
-// pairs at a time among those of the same key, and keeps each key's next slot in LDS.
-template <bool WIDE, int WAVES, typename F>
+// pairs at a time among those of the same key, and keeps each key's next slot in LDS.  ROUNDS: the
+// 64s of pairs of a wavefront whose keys stay in registers from the first load on (0: any
+// number, read again where they are placed).
+template <bool WIDE, int WAVES, int ROUNDS, typename F>
 __device__ __forceinline__ void sort_share(const SortArgs &a, SortShared<WAVES> &s, uint32_t lo, uint32_t hi, uint32_t block,
                                            uint32_t blocks, F &&place) {
     constexpr int THREADS = 64 * WAVES;
     const uint32_t K = a.E + 1, lane = threadIdx.x & 63u;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t part = ((hi - lo + WAVES - 1) / WAVES + 63u) & ~63u;
+    const uint32_t from = min(hi, lo + wave * part), to = min(hi, from + part);
+    uint32_t mine[ROUNDS ? ROUNDS : 1];
+#pragma unroll
+    for (int r = 0; r < ROUNDS; ++r) mine[r] = from + 64 * r + lane < to ? key_of<WIDE>(a, from + 64 * r + lane) : 0u;
     for (uint32_t e = threadIdx.x; e < K; e += THREADS) {
         s.total[e] = s.before[e] = 0;
 #pragma unroll
         for (int w = 0; w < WAVES; ++w) s.wave[w][e] = 0;
     }
     __syncthreads();
-    const uint32_t part = ((hi - lo + WAVES - 1) / WAVES + 63u) & ~63u;
-    const uint32_t from = min(hi, lo + wave * part), to = min(hi, from + part);
     const int bits = key_bits(a);
     if (a.hist) {
-        // four keys a lane, a wavefront every WAVES-th share's counts, AHEAD of them at once
-        constexpr uint32_t AHEAD = 8;
-        const uint32_t stride = uint32_t(hist_stride(a.E));
-        for (uint32_t e = 4 * lane; e < K; e += 256) {
-            uint4_t total = {0, 0, 0, 0}, before = {0, 0, 0, 0};
+        // every 64th key a lane, every WAVES-th share's counts a wavefront, AHEAD of them at once
+        constexpr uint32_t AHEAD = 4, KEYS = 5;
+        for (uint32_t e0 = lane; e0 < K + lane; e0 += 64 * KEYS) {
+            uint32_t total[KEYS] = {}, before[KEYS] = {};
             for (uint32_t b0 = wave; b0 < blocks; b0 += AHEAD * WAVES) {
-                uint4_t n[AHEAD];
+                uint32_t n[AHEAD][KEYS];
 #pragma unroll
                 for (uint32_t i = 0; i < AHEAD; ++i)
-                    n[i] = load_u4(a.hist + size_t(min(b0 + i * WAVES, blocks - 1u)) * stride + e);
 #pragma unroll
-                for (uint32_t i = 0; i < AHEAD; ++i) {
-                    const uint32_t b = b0 + i * WAVES;
-                    if (b < blocks) total += n[i];
-                    if (b < block) before += n[i];
-                }
+                    for (uint32_t k = 0; k < KEYS; ++k)
+                        n[i][k] = a.hist[size_t(min(b0 + i * WAVES, blocks - 1u)) * K + min(e0 + 64 * k, K - 1u)];
+#pragma unroll
+                for (uint32_t i = 0; i < AHEAD; ++i)
+#pragma unroll
+                    for (uint32_t k = 0; k < KEYS; ++k) {
+                        if (b0 + i * WAVES < blocks) total[k] += n[i][k];
+                        if (b0 + i * WAVES < block) before[k] += n[i][k];
+                    }
             }
 #pragma unroll
-            for (uint32_t i = 0; i < 4; ++i) {
-                if (e + i < K) {
-                    atomicAdd(&s.total[e + i], total[i]);
-                    atomicAdd(&s.before[e + i], before[i]);
+            for (uint32_t k = 0; k < KEYS; ++k) {
+                if (e0 + 64 * k < K) {
+                    atomicAdd(&s.total[e0 + 64 * k], total[k]);
+                    atomicAdd(&s.before[e0 + 64 * k], before[k]);
                 }
             }
         }
@@ -197,7 +201,17 @@ __device__ __forceinline__ void sort_share(const SortArgs &a, SortShared<WAVES> 
             if (p < lo) atomicAdd(&s.before[key], min(n, lo - p));
         });
     }
-    count_keys<WIDE, 64>(a, from, to, [&](uint32_t key, uint32_t, uint32_t n) { atomicAdd(&s.wave[wave][key], n); });
+    uint64_t same[ROUNDS ? ROUNDS : 1];
+    if constexpr (ROUNDS > 0) {
+#pragma unroll
+        for (int r = 0; r < ROUNDS; ++r) {
+            const bool live = from + 64 * r + lane < to;
+            same[r] = same_key(mine[r], live, bits);
+            if (live && rank_in(same[r]) == 0) atomicAdd(&s.wave[wave][mine[r]], uint32_t(__popcll(same[r])));
+        }
+    } else {
+        count_keys<WIDE, 64>(a, from, to, [&](uint32_t key, uint32_t, uint32_t n) { atomicAdd(&s.wave[wave][key], n); });
+    }
     __syncthreads();
     const bool first = block == 0;
     const auto own = [&](uint32_t e, uint32_t at) {  // the next slots of a key in this share, at: its first slot
@@ -226,27 +240,32 @@ __device__ __forceinline__ void sort_share(const SortArgs &a, SortShared<WAVES> 
         });
     }
     volatile uint32_t *const next = s.wave[wave];
-    for (uint32_t base = from; base < to; base += 64) {
-        const uint32_t p = base + lane;
-        const bool live = p < to;
-        const uint32_t key = live ? key_of<WIDE>(a, p) : 0u;
-        const uint64_t same = same_key(key, live, bits);
-        const uint32_t rank = rank_in(same);
-        if (live) {
-            const uint32_t slot = next[key] + rank;
+    const auto put = [&](uint32_t base, uint32_t key, uint64_t same) {
+        if (base + lane < to) {
+            const uint32_t rank = rank_in(same), slot = next[key] + rank;
             __builtin_amdgcn_wave_barrier();  // all lanes have read before the last of each key writes
             if (rank + 1 == uint32_t(__popcll(same))) next[key] = slot + 1;
-            place(p, key, slot);
+            place(base + lane, key, slot);
         }
         __builtin_amdgcn_wave_barrier();
+    };
+    if constexpr (ROUNDS > 0) {
+#pragma unroll
+        for (int r = 0; r < ROUNDS; ++r) put(from + 64 * r, mine[r], same[r]);
+    } else {
+        for (uint32_t base = from; base < to; base += 64) {
+            const bool live = base + lane < to;
+            const uint32_t key = live ? key_of<WIDE>(a, base + lane) : 0u;
+            put(base, key, same_key(key, live, bits));
+        }
     }
 }
 
-template <bool WIDE, int WAVES>
+template <bool WIDE, int WAVES, int ROUNDS>
 __global__ __launch_bounds__(64 * WAVES) void sort_kernel(SortArgs a) {
     __shared__ SortShared<WAVES> s;
     const uint32_t lo = min(a.P, blockIdx.x * a.share), hi = min(a.P, lo + a.share);
-    sort_share<WIDE, WAVES>(a, s, lo, hi, blockIdx.x, gridDim.x, [&](uint32_t p, uint32_t key, uint32_t slot) {
+    sort_share<WIDE, WAVES, ROUNDS>(a, s, lo, hi, blockIdx.x, gridDim.x, [&](uint32_t p, uint32_t key, uint32_t slot) {
         if (a.tiles) {
             if (slot >= a.n_tiles * uint32_t(kSortTile)) return;
             a.tile_pairs[slot] = p;
@@ -418,7 +437,7 @@ __global__ __launch_bounds__(256) void sort_dispatch_kernel(SortArgs sort, RowAr
         const uint8_t *const from = a.in + size_t(t) * a.row + column;
         w = halves == 8 ? load_chunk<true>(from, 8) : load_chunk<false>(from, halves);
     }
-    sort_share<WIDE, 4>(sort, s, lo, hi, writes ? block : 1u, 1u, [&](uint32_t p, uint32_t key, uint32_t slot) {
+    sort_share<WIDE, 4, 0>(sort, s, lo, hi, writes ? block : 1u, 1u, [&](uint32_t p, uint32_t key, uint32_t slot) {
         slots[p - lo] = key < sort.E ? slot : slot | 0x80000000u;  // left out
         if (writes && slot < sort.P) {
             sort.slots[p] = int32_t(slot);
@@ -588,7 +607,7 @@ SortPlan sort_plan(int64_t pairs, int64_t experts) {
     const int64_t turns = (pairs + kSortThreads - 1) / kSortThreads;
     const int64_t per = turns ? (turns + kSortBlocks - 1) / kSortBlocks : 1;
     const int64_t blocks = turns ? (turns + per - 1) / per : 1;
-    return {blocks, per * kSortThreads, pairs > kSortOne ? blocks * hist_stride(experts) : 0};
+    return {blocks, per * kSortThreads, pairs > kSortOne ? blocks * (experts + 1) : 0};
 }
 
 namespace {
@@ -625,9 +644,14 @@ int sort_launch(const SortCall &c, hipStream_t stream) {
         const hipError_t err = c.wide ? run(sort_count_kernel<true>, kSortThreads) : run(sort_count_kernel<false>, kSortThreads);
         if (err != hipSuccess) return record_launch(err);
     }
-    if (c.pairs <= 256)  // one pair a thread
-        return record_launch(c.wide ? run(sort_kernel<true, 4>, 256) : run(sort_kernel<false, 4>, 256));
-    return record_launch(c.wide ? run(sort_kernel<true, kSortWaves>, kSortThreads) : run(sort_kernel<false, kSortWaves>, kSortThreads));
+    const auto sized = [&](auto wide) {
+        constexpr bool W = decltype(wide)::value;
+        if (c.pairs <= 256) return run(sort_kernel<W, 4, 1>, 256);  // one pair a thread
+        if (plan.share == kSortThreads) return run(sort_kernel<W, kSortWaves, 1>, kSortThreads);
+        if (plan.share <= 4 * kSortThreads) return run(sort_kernel<W, kSortWaves, 4>, kSortThreads);
+        return run(sort_kernel<W, kSortWaves, 0>, kSortThreads);
+    };
+    return record_launch(c.wide ? sized(std::true_type{}) : sized(std::false_type{}));
 }
 
 namespace {
