@@ -233,49 +233,6 @@ __global__ __launch_bounds__(64 * WAVES) void adapter_down_tiles_kernel(AdapterA
     uint4_t xv[XD][2 * CT], wv[AD][2][RT];
     constexpr uint32_t STEP = 64 * WAVES;
     uint4_t *const turned = reinterpret_cast<uint4_t *>(shared[wave]);  // [slot][8 chunks], chunk c at c ^ slot % 8
-    const auto load_x = [&](int d, uint32_t k0) {
-        const uint32_t k = k0 + 8 * c8, at = k < a.in ? k : 0u;
-#pragma unroll
-        for (int c = 0; c < 2 * CT; ++c)
-            if (8u * c < slots) xv[d][c] = __builtin_nontemporal_load(reinterpret_cast<const chunk_t *>(x[c] + at));  // uniform
-    };
-    const auto load_w = [&](int d, uint32_t k0) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const uint32_t k = k0 + 32 * h + 8 * g, at = k < a.in ? k : 0u;
-#pragma unroll
-            for (int r = 0; r < RT; ++r) wv[d][h][r] = load_u4(w[r] + size_t(at) * a.rank);
-        }
-    };
-    const auto multiply = [&](int xd, int ad, uint32_t k0) {
-        const bool rest = k0 + 64 > a.in;  // uniform: columns past the row, zeros on both sides
-        wavefront_fence();
-#pragma unroll
-        for (int c = 0; c < 2 * CT; ++c) {
-            if (8u * c >= slots) continue;
-            if (rest && k0 + 8 * c8 >= a.in) xv[xd][c] = uint4_t{0, 0, 0, 0};
-            turned[(8 * c + r8) * 8 + (c8 ^ r8)] = xv[xd][c];
-        }
-        wavefront_fence();
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            uint4_t b[CT];
-#pragma unroll
-            for (int c = 0; c < CT; ++c) b[c] = turned[(16 * c + m) * 8 + ((4 * h + g) ^ (m & 7u))];
-            if (rest && k0 + 32 * h + 8 * g >= a.in) {
-#pragma unroll
-                for (int r = 0; r < RT; ++r) wv[ad][h][r] = uint4_t{0, 0, 0, 0};
-            }
-#pragma unroll
-            for (int c = 0; c < CT; ++c) {
-                if (16u * c >= slots) continue;
-#pragma unroll
-                for (int r = 0; r < RT; ++r) acc[r][c] = mfma<BF>(wv[ad][h][r], b[c], acc[r][c]);
-            }
-        }
-    };
-    constexpr int UNROLL = XD > AD ? XD : AD;
-    static_assert(UNROLL % XD == 0 && UNROLL % AD == 0, "a turn of the loop is whole turns of both rings");
     // Each workgroup begins at another step: in step with each other they would all read the same
     // part of rows that lie a power of two apart, from few of the memory's channels.
     const uint32_t units = (a.in + 63) / 64, each = (units + a.splits - 1) / a.splits;
@@ -284,21 +241,72 @@ __global__ __launch_bounds__(64 * WAVES) void adapter_down_tiles_kernel(AdapterA
     const auto column = [&](uint32_t i) {
         return 64 * (first + wave) + STEP * (i + turn < steps ? i + turn : i + turn - steps);
     };
+    // The loop for LIVE groups of 16 slots.  Nothing in it is loaded under a condition: the waits count
+    // loads, and one that may not have been issued makes the compiler wait for all of them.
+    const auto run = [&](auto live) {
+        constexpr int LIVE = decltype(live)::value;
+        const auto load_x = [&](int d, uint32_t k0) {
+            const uint32_t k = k0 + 8 * c8, at = k < a.in ? k : 0u;
 #pragma unroll
-    for (int d = 0; d < UNROLL - 1; ++d) {  // the oldest step's loads first
-        if (d < XD - 1) load_x(d, column(min(uint32_t(d), steps - 1u)));  // (with no steps: any, not used)
-        if (d < AD - 1) load_w(d, column(min(uint32_t(d), steps - 1u)));
-        __builtin_amdgcn_sched_barrier(0);
-    }
-    for (uint32_t i0 = 0; i0 < steps; i0 += UNROLL) {
+            for (int c = 0; c < 2 * LIVE; ++c)
+                xv[d][c] = __builtin_nontemporal_load(reinterpret_cast<const chunk_t *>(x[c] + at));
+        };
+        const auto load_w = [&](int d, uint32_t k0) {
 #pragma unroll
-        for (int d = 0; d < UNROLL; ++d) {
-            load_x((d + XD - 1) % XD, column(min(i0 + d + XD - 1, steps - 1u)));
-            load_w((d + AD - 1) % AD, column(min(i0 + d + AD - 1, steps - 1u)));
+            for (int h = 0; h < 2; ++h) {
+                const uint32_t k = k0 + 32 * h + 8 * g, at = k < a.in ? k : 0u;
+#pragma unroll
+                for (int r = 0; r < RT; ++r) wv[d][h][r] = load_u4(w[r] + size_t(at) * a.rank);
+            }
+        };
+        const auto multiply = [&](int xd, int ad, uint32_t k0) {
+            const bool rest = k0 + 64 > a.in;  // uniform: columns past the row, zeros on both sides
+            wavefront_fence();
+#pragma unroll
+            for (int c = 0; c < 2 * LIVE; ++c) {
+                if (rest && k0 + 8 * c8 >= a.in) xv[xd][c] = uint4_t{0, 0, 0, 0};
+                turned[(8 * c + r8) * 8 + (c8 ^ r8)] = xv[xd][c];
+            }
+            wavefront_fence();
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                uint4_t b[LIVE];
+#pragma unroll
+                for (int c = 0; c < LIVE; ++c) b[c] = turned[(16 * c + m) * 8 + ((4 * h + g) ^ (m & 7u))];
+                if (rest && k0 + 32 * h + 8 * g >= a.in) {
+#pragma unroll
+                    for (int r = 0; r < RT; ++r) wv[ad][h][r] = uint4_t{0, 0, 0, 0};
+                }
+#pragma unroll
+                for (int r = 0; r < RT; ++r)
+#pragma unroll
+                    for (int c = 0; c < LIVE; ++c) acc[r][c] = mfma<BF>(wv[ad][h][r], b[c], acc[r][c]);
+            }
+        };
+        constexpr int UNROLL = XD > AD ? XD : AD;
+        static_assert(UNROLL % XD == 0 && UNROLL % AD == 0, "a turn of the loop is whole turns of both rings");
+#pragma unroll
+        for (int d = 0; d < UNROLL - 1; ++d) {  // the oldest step's loads first
+            if (d < XD - 1) load_x(d, column(min(uint32_t(d), steps - 1u)));
+            if (d < AD - 1) load_w(d, column(min(uint32_t(d), steps - 1u)));
             __builtin_amdgcn_sched_barrier(0);
-            if (i0 + d < steps && column(i0 + d) < 64 * last) multiply(d % XD, d % AD, column(i0 + d));  // uniform
         }
-    }
+        for (uint32_t i0 = 0; i0 < steps; i0 += UNROLL) {
+#pragma unroll
+            for (int d = 0; d < UNROLL; ++d) {
+                load_x((d + XD - 1) % XD, column(min(i0 + d + XD - 1, steps - 1u)));
+                load_w((d + AD - 1) % AD, column(min(i0 + d + AD - 1, steps - 1u)));
+                __builtin_amdgcn_sched_barrier(0);
+                if (i0 + d < steps && column(i0 + d) < 64 * last) multiply(d % XD, d % AD, column(i0 + d));  // uniform
+            }
+        }
+    };
+    if (CT == 1 || slots <= 16)
+        run(std::integral_constant<int, 1>{});
+    else if (CT == 2 || slots <= 32)
+        run(std::integral_constant<int, CT < 2 ? CT : 2>{});
+    else
+        run(std::integral_constant<int, CT>{});
     wavefront_fence();
     const auto part = [&](uint32_t w, uint32_t slot, uint32_t rank) -> float & { return shared[w][slot * (RANKS + 4) + rank]; };
 #pragma unroll
@@ -327,9 +335,11 @@ __global__ __launch_bounds__(64 * WAVES) void adapter_down_tiles_kernel(AdapterA
 // 64 lanes, memory wants 64 outputs of a slot together.  x, y and the outputs pass through once
 // and do not stay in the caches in place of A, B and the sums (8192 rows of rank 64 [8192 x 4096]: 101 us, 96 so).
 template <bool BF, int KC>
-__global__ __launch_bounds__(256) void adapter_up_tiles_kernel(AdapterArgs a) {
+__global__ __launch_bounds__(256, KC <= 4 ? 2 : 1) void adapter_up_tiles_kernel(AdapterArgs a) {
     constexpr int P = kPieces<BF>, CT = kTileGroups, STAGE = KC < 2 ? KC : 2;  // chunks of B in registers at once
-    constexpr bool AHEAD = KC <= 2;  // of B; y always is
+    // B is loaded with the column before's, or (more registers than there are) with its own, once for
+    // all slots, or (more than those) for each group of slots again; y always is ahead
+    constexpr bool AHEAD = KC == 1, ONCE = KC <= 2;
     __shared__ uint4_t operands[CT][KC][P][64];
     __shared__ float powers[kTileSlots];  // what an f16 slot's sums are multiplied with
     __shared__ __attribute__((aligned(16))) float turned[4][16][64 + 4];
@@ -346,7 +356,7 @@ __global__ __launch_bounds__(256) void adapter_up_tiles_kernel(AdapterArgs a) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             const uint32_t slot = 16 * c + 8 * h + s8, of = a.tile_rows[t * kTileSlots + slot];
-            row[c][h] = slot < slots ? of : 0u;
+            row[c][h] = slot < slots ? of : 0u;  // past the tile's: read, not written
         }
     const uint32_t mine = 8 * (lane & 7u);
     if (adapter >= a.adapters) {  // rows without an adapter; uniform
@@ -371,19 +381,19 @@ __global__ __launch_bounds__(256) void adapter_up_tiles_kernel(AdapterArgs a) {
     }
     const uint16_t *const up = a.up + size_t(adapter) * a.rank * a.N;
     uint4_t y[2][CT][2], w[AHEAD ? 2 : 1][STAGE][4];
-    const auto load_y = [&](int d, uint32_t n0) {
+    // Nothing is loaded under a condition, as in the first product.  Outputs past the last, and of rows of
+    // fewer than eight, are not used: any others stand in for them.
+    const auto load_y = [&](auto live, int d, uint32_t n0) __attribute__((always_inline)) {
+        const uint32_t n = a.N < 8 ? 0u : min(n0 + mine, a.N - 8u);
 #pragma unroll
-        for (int c = 0; c < CT; ++c) {
-            if (16u * c >= slots) continue;  // uniform
+        for (int c = 0; c < decltype(live)::value; ++c)
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
-                if (n0 + mine + 8 <= a.N) {
-                    const uint16_t *const from = a.y + size_t(row[c][h]) * a.N + n0 + mine;
-                    y[d][c][h] = __builtin_nontemporal_load(reinterpret_cast<const chunk_t *>(from));
-                }
-        }
+            for (int h = 0; h < 2; ++h) {
+                const uint16_t *const from = a.N < 8 ? up : a.y + size_t(row[c][h]) * a.N + n;
+                y[d][c][h] = __builtin_nontemporal_load(reinterpret_cast<const chunk_t *>(from));
+            }
     };
-    const auto load_w = [&](int d, uint32_t n0, uint32_t k0) {
+    const auto load_w = [&](int d, uint32_t n0, uint32_t k0) __attribute__((always_inline)) {
 #pragma unroll
         for (int s = 0; s < STAGE; ++s) {
             const uint32_t k = k0 + 32 * s + 8 * g, eight = min(k / 8, a.rank / 8 - 1u);
@@ -394,8 +404,16 @@ __global__ __launch_bounds__(256) void adapter_up_tiles_kernel(AdapterArgs a) {
     // tiles begin at different columns, as their A x does
     const uint32_t turns = (end - begin + 255) / 256, turn = t % turns;
     const auto column = [&](uint32_t i) { return begin + 64 * wave + 256 * (i + turn < turns ? i + turn : i + turn - turns); };
-    load_y(0, column(0));
-    if (AHEAD) load_w(0, column(0), 0);
+    const auto by_live = [&](auto &&f) {
+        if (slots <= 16)
+            f(std::integral_constant<int, 1>{});
+        else if (slots <= 32)
+            f(std::integral_constant<int, 2>{});
+        else
+            f(std::integral_constant<int, 4>{});
+    };
+    by_live([&](auto live) { load_y(live, 0, column(0)); });
+    if (ONCE) load_w(0, column(0), 0);
     __builtin_amdgcn_sched_barrier(0);
     // A x: the parts' sum, scaled, in pieces; a thread has eight ranks of a slot, 4 KC threads a slot
     constexpr int EIGHTS = 4 * KC;
@@ -465,26 +483,28 @@ __global__ __launch_bounds__(256) void adapter_up_tiles_kernel(AdapterArgs a) {
         }
     }
     __syncthreads();
-    const auto compute = [&](int d, uint32_t n0) {
+    // WHOLE: every slot and output of the columns is there, and stored without a condition
+    const auto compute = [&](auto live, auto whole, uint32_t n0) __attribute__((always_inline)) {
+        constexpr int LIVE = decltype(live)::value;
+        constexpr bool WHOLE = decltype(whole)::value;
         const uint32_t n = n0 + mine, have = n < a.N ? min(a.N - n, 8u) : 0u;
-        if constexpr (AHEAD) {  // past the ranks: zeros, as in the slots' operands
+        if constexpr (ONCE) {  // past the ranks: zeros, as in the slots' operands
 #pragma unroll
             for (int s = 0; s < STAGE; ++s)
                 if (32 * s + 8 * g >= a.rank) {
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) w[d][s][j] = uint4_t{0, 0, 0, 0};
+                    for (int j = 0; j < 4; ++j) w[0][s][j] = uint4_t{0, 0, 0, 0};
                 }
         }
 #pragma unroll
-        for (int c = 0; c < CT; ++c) {
-            if (16u * c >= slots) continue;  // uniform
+        for (int c = 0; c < LIVE; ++c) {
             float4_t acc[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) acc[j] = float4_t{0, 0, 0, 0};
 #pragma unroll
             for (int k0 = 0; k0 < 32 * KC; k0 += 32 * STAGE) {
                 if (k0 && uint32_t(k0) >= a.rank) continue;  // uniform
-                if constexpr (!AHEAD) {
+                if constexpr (!ONCE) {
                     load_w(0, n0, k0);
 #pragma unroll
                     for (int s = 0; s < STAGE; ++s)
@@ -499,7 +519,7 @@ __global__ __launch_bounds__(256) void adapter_up_tiles_kernel(AdapterArgs a) {
                     for (int p = P - 1; p >= 0; --p) {  // the small pieces first
                         const uint4_t b = operands[c][k0 / 32 + s][p][lane];
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) acc[j] = mfma<BF>(w[AHEAD ? d : 0][s][j], b, acc[j]);
+                        for (int j = 0; j < 4; ++j) acc[j] = mfma<BF>(w[0][s][j], b, acc[j]);
                     }
             }
             wavefront_fence();
@@ -513,15 +533,15 @@ __global__ __launch_bounds__(256) void adapter_up_tiles_kernel(AdapterArgs a) {
             wavefront_fence();
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                if (16u * c + 8 * h + s8 >= slots) continue;
+                if (!WHOLE && 16u * c + 8 * h + s8 >= slots) continue;
                 const float *const v = &turned[wave][8 * h + s8][mine];
                 const size_t at = size_t(row[c][h]) * a.N + n;
-                if (have == 8) {
+                if (WHOLE || have == 8) {
                     const float4_t lo = *reinterpret_cast<const float4_t *>(v), hi = *reinterpret_cast<const float4_t *>(v + 4);
                     uint4_t out;
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        const float2v_t old = floats<BF>(y[d][c][h][i]);
+                        const float2v_t old = floats<BF>(y[0][c][h][i]);
                         const float v0 = i < 2 ? lo[2 * i] : hi[2 * i - 4], v1 = i < 2 ? lo[2 * i + 1] : hi[2 * i - 3];
                         out[i] = pair_bits<BF>(old.x + v0, old.y + v1);
                     }
@@ -535,18 +555,32 @@ __global__ __launch_bounds__(256) void adapter_up_tiles_kernel(AdapterArgs a) {
             }
         }
     };
-    for (uint32_t i = 0; i < turns; i += 2) {
-#pragma unroll
-        for (int d = 0; d < 2; ++d) {
-            if (i + d >= turns) break;  // uniform
-            if (i + d + 1 < turns) {
-                load_y(1 - d, column(i + d + 1));
-                if (AHEAD) load_w(1 - d, column(i + d + 1), 0);
-            }
+    const auto all = [&](auto live, auto whole) __attribute__((always_inline)) {
+        for (uint32_t i = 0; i + 1 < turns; ++i) {
+            if (ONCE && !AHEAD && i) load_w(0, column(i), 0);
             __builtin_amdgcn_sched_barrier(0);
-            compute(d, column(i + d));
+            load_y(live, 1, column(i + 1));
+            if (AHEAD) load_w(AHEAD ? 1 : 0, column(i + 1), 0);
+            __builtin_amdgcn_sched_barrier(0);
+            compute(live, whole, column(i));
+#pragma unroll
+            for (int c = 0; c < decltype(live)::value; ++c)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) y[0][c][h] = y[1][c][h];
+            if constexpr (AHEAD) {
+#pragma unroll
+                for (int s = 0; s < STAGE; ++s)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) w[0][s][j] = w[1][s][j];
+            }
         }
-    }
+        if (ONCE && !AHEAD && turns > 1) load_w(0, column(turns - 1), 0);
+        compute(live, whole, column(turns - 1));
+    };
+    if (slots == kTileSlots && (end - begin) % 256 == 0)
+        all(std::integral_constant<int, 4>{}, std::true_type{});
+    else
+        by_live([&](auto live) { all(live, std::false_type{}); });
 }
 
 namespace {
