@@ -202,8 +202,9 @@ __device__ __forceinline__ void wavefront_fence() {
 // columns in turn and their sums meet in LDS.  A wavefront reads 128 bytes of a row together and
 // turns them into operand B in its own part of LDS (rows read as the operand wants them, 16 of
 // them 64 bytes each in an instruction, kept the loads waiting for the cache: 8192 rows of 4096,
-// rank 16, 34 us); XD steps of x and AD of A are on their way at once.
-template <bool BF, int RT, int CT, int WAVES, int XD, int AD>
+// rank 16, 34 us; 17 now).  Nothing is loaded a step ahead: the registers that it takes keep other
+// wavefronts off the CU, whose loads do as well (24 us with four steps on their way).
+template <bool BF, int RT, int CT, int WAVES>
 __global__ __launch_bounds__(64 * WAVES) void adapter_down_tiles_kernel(AdapterArgs a) {
     constexpr int SLOTS = 16 * CT, RANKS = 16 * RT, THREADS = 64 * WAVES, PARTS = kTileGroups / CT;
     constexpr int SUMS = SLOTS * (RANKS + 4), STAGE = SLOTS * 32;  // floats of a wavefront's sums, of its turned rows
@@ -230,7 +231,6 @@ __global__ __launch_bounds__(64 * WAVES) void adapter_down_tiles_kernel(AdapterA
     for (int r = 0; r < RT; ++r)
 #pragma unroll
         for (int c = 0; c < CT; ++c) acc[r][c] = float4_t{0, 0, 0, 0};
-    uint4_t xv[XD][2 * CT], wv[AD][2][RT];
     constexpr uint32_t STEP = 64 * WAVES;
     uint4_t *const turned = reinterpret_cast<uint4_t *>(shared[wave]);  // [slot][8 chunks], chunk c at c ^ slot % 8
     // Each workgroup begins at another step: in step with each other they would all read the same
@@ -241,31 +241,28 @@ __global__ __launch_bounds__(64 * WAVES) void adapter_down_tiles_kernel(AdapterA
     const auto column = [&](uint32_t i) {
         return 64 * (first + wave) + STEP * (i + turn < steps ? i + turn : i + turn - steps);
     };
-    // The loop for LIVE groups of 16 slots.  Nothing in it is loaded under a condition: the waits count
-    // loads, and one that may not have been issued makes the compiler wait for all of them.
-    const auto run = [&](auto live) {
+    const auto run = [&](auto live) {  // LIVE groups of 16 slots
         constexpr int LIVE = decltype(live)::value;
-        const auto load_x = [&](int d, uint32_t k0) {
-            const uint32_t k = k0 + 8 * c8, at = k < a.in ? k : 0u;
+        for (uint32_t i = 0; i < steps; ++i) {
+            const uint32_t k0 = column(i);
+            if (k0 >= 64 * last) continue;  // uniform
+            const bool rest = k0 + 64 > a.in;  // uniform: columns past the row, zeros on both sides
+            uint4_t xv[2 * LIVE], wv[2][RT];
+            const uint32_t kx = k0 + 8 * c8;
 #pragma unroll
             for (int c = 0; c < 2 * LIVE; ++c)
-                xv[d][c] = __builtin_nontemporal_load(reinterpret_cast<const chunk_t *>(x[c] + at));
-        };
-        const auto load_w = [&](int d, uint32_t k0) {
+                xv[c] = __builtin_nontemporal_load(reinterpret_cast<const chunk_t *>(x[c] + (kx < a.in ? kx : 0u)));
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                const uint32_t k = k0 + 32 * h + 8 * g, at = k < a.in ? k : 0u;
+                const uint32_t kw = k0 + 32 * h + 8 * g;
 #pragma unroll
-                for (int r = 0; r < RT; ++r) wv[d][h][r] = load_u4(w[r] + size_t(at) * a.rank);
+                for (int r = 0; r < RT; ++r) wv[h][r] = load_u4(w[r] + size_t(kw < a.in ? kw : 0u) * a.rank);
             }
-        };
-        const auto multiply = [&](int xd, int ad, uint32_t k0) {
-            const bool rest = k0 + 64 > a.in;  // uniform: columns past the row, zeros on both sides
             wavefront_fence();
 #pragma unroll
             for (int c = 0; c < 2 * LIVE; ++c) {
-                if (rest && k0 + 8 * c8 >= a.in) xv[xd][c] = uint4_t{0, 0, 0, 0};
-                turned[(8 * c + r8) * 8 + (c8 ^ r8)] = xv[xd][c];
+                if (rest && kx >= a.in) xv[c] = uint4_t{0, 0, 0, 0};
+                turned[(8 * c + r8) * 8 + (c8 ^ r8)] = xv[c];
             }
             wavefront_fence();
 #pragma unroll
@@ -275,29 +272,12 @@ __global__ __launch_bounds__(64 * WAVES) void adapter_down_tiles_kernel(AdapterA
                 for (int c = 0; c < LIVE; ++c) b[c] = turned[(16 * c + m) * 8 + ((4 * h + g) ^ (m & 7u))];
                 if (rest && k0 + 32 * h + 8 * g >= a.in) {
 #pragma unroll
-                    for (int r = 0; r < RT; ++r) wv[ad][h][r] = uint4_t{0, 0, 0, 0};
+                    for (int r = 0; r < RT; ++r) wv[h][r] = uint4_t{0, 0, 0, 0};
                 }
 #pragma unroll
                 for (int r = 0; r < RT; ++r)
 #pragma unroll
-                    for (int c = 0; c < LIVE; ++c) acc[r][c] = mfma<BF>(wv[ad][h][r], b[c], acc[r][c]);
-            }
-        };
-        constexpr int UNROLL = XD > AD ? XD : AD;
-        static_assert(UNROLL % XD == 0 && UNROLL % AD == 0, "a turn of the loop is whole turns of both rings");
-#pragma unroll
-        for (int d = 0; d < UNROLL - 1; ++d) {  // the oldest step's loads first
-            if (d < XD - 1) load_x(d, column(min(uint32_t(d), steps - 1u)));
-            if (d < AD - 1) load_w(d, column(min(uint32_t(d), steps - 1u)));
-            __builtin_amdgcn_sched_barrier(0);
-        }
-        for (uint32_t i0 = 0; i0 < steps; i0 += UNROLL) {
-#pragma unroll
-            for (int d = 0; d < UNROLL; ++d) {
-                load_x((d + XD - 1) % XD, column(min(i0 + d + XD - 1, steps - 1u)));
-                load_w((d + AD - 1) % AD, column(min(i0 + d + AD - 1, steps - 1u)));
-                __builtin_amdgcn_sched_barrier(0);
-                if (i0 + d < steps && column(i0 + d) < 64 * last) multiply(d % XD, d % AD, column(i0 + d));  // uniform
+                    for (int c = 0; c < LIVE; ++c) acc[r][c] = mfma<BF>(wv[h][r], b[c], acc[r][c]);
             }
         }
     };
@@ -626,27 +606,27 @@ GroupPlan group_plan(int64_t in, int64_t rank, int64_t adapters, int64_t rows) {
     return p;
 }
 
-// f(16s of ranks, groups of slots, wavefronts, steps of x and of A on their way)
+// f(16s of ranks, groups of slots, wavefronts)
 template <typename F>
 void by_ranks(int64_t rank, F &&f) {
     using std::integer_sequence;
     if (rank <= 16)
-        f(integer_sequence<int, 1, 4, 4, 4, 4>{});
+        f(integer_sequence<int, 1, 4, 4>{});
     else if (rank <= 32)
-        f(integer_sequence<int, 2, 4, 4, 4, 2>{});
+        f(integer_sequence<int, 2, 4, 4>{});
     else if (rank <= 64)
-        f(integer_sequence<int, 4, 4, 4, 2, 2>{});
+        f(integer_sequence<int, 4, 4, 4>{});
     else if (rank <= 128)
-        f(integer_sequence<int, 8, 2, 4, 2, 1>{});
+        f(integer_sequence<int, 8, 2, 4>{});
     else
-        f(integer_sequence<int, 16, 1, 4, 2, 1>{});
+        f(integer_sequence<int, 16, 1, 4>{});
 }
 
-template <bool BF, int RT, int CT, int WAVES, int XD, int AD>
+template <bool BF, int RT, int CT, int WAVES>
 hipError_t launch_tiles(const AdapterArgs &a, int64_t tiles, hipStream_t stream,
-                        std::integer_sequence<int, RT, CT, WAVES, XD, AD>) {
+                        std::integer_sequence<int, RT, CT, WAVES>) {
     const int64_t ups = tiles * ((int64_t(a.N) + 256 * a.columns - 1) / (256 * a.columns));
-    hipLaunchKernelGGL((adapter_down_tiles_kernel<BF, RT, CT, WAVES, XD, AD>),
+    hipLaunchKernelGGL((adapter_down_tiles_kernel<BF, RT, CT, WAVES>),
                        dim3{uint32_t(tiles * a.splits * (kTileGroups / CT))}, dim3{64 * WAVES}, 0, stream, a);
     if (const hipError_t err = hipGetLastError(); err != hipSuccess) return err;
     hipLaunchKernelGGL((adapter_up_tiles_kernel<BF, (RT + 1) / 2>), dim3{uint32_t(ups)}, dim3{256}, 0, stream, a);
