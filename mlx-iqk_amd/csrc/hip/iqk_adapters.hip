@@ -656,7 +656,8 @@ int rows_grouped(AdapterArgs a, bool bf, uint32_t *work, hipStream_t stream) {
     const int64_t wide = (int64_t(a.N) + 255) / 256, all = p.tiles * wide, each = a.rank > 64 ? all / 512 : all / 2048;
     const int64_t most = a.rank > 64 ? 8 : 4;
     a.columns = uint32_t(each < 1 ? 1 : each > most ? most : each);
-    if (!grid_ok(all, 256) || !grid_ok(p.tiles * p.splits * kTileGroups, 512)) return IQK_ERR_GEOMETRY;
+    const int64_t ups = p.tiles * ((int64_t(a.N) + 256 * a.columns - 1) / (256 * a.columns));
+    if (!grid_ok(ups, 256) || !grid_ok(p.tiles * p.splits * kTileGroups, 256)) return IQK_ERR_GEOMETRY;
     SortCall c{};
     c.ids = a.ids;
     c.wide = a.wide;

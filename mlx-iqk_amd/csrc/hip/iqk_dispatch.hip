@@ -737,7 +737,8 @@ int iqk_dispatch(int dtype, const void *x, const void *ids, int wide_ids, int64_
         return IQK_ERR_GEOMETRY;
     if (n_tokens && (!x || !rows)) return IQK_ERR_ARGUMENT;
     RowArgs a = row_args(dtype, n_tokens, pairs_per_token, cols);
-    if (n_tokens == 0 || n_tokens * pairs_per_token > kDispatchOne) {
+    const int64_t each = 256 >> a.log_width, blocks = (n_tokens + each - 1) / each * a.columns;
+    if (n_tokens == 0 || n_tokens * pairs_per_token > kDispatchOne || !grid_ok(blocks, 256)) {
         if (const int rc = iqk_sort(ids, wide_ids, n_tokens, pairs_per_token, num_experts, work, offsets, sorted_ids,
                                     tokens, slots, stream);
             rc != IQK_OK || n_tokens == 0)
@@ -767,8 +768,6 @@ int iqk_dispatch(int dtype, const void *x, const void *ids, int wide_ids, int64_
     sort.per_id = 1;
     a.in = static_cast<const uint8_t *>(x);
     a.out = static_cast<uint8_t *>(rows);
-    const int64_t each = 256 >> a.log_width, blocks = (n_tokens + each - 1) / each * a.columns;
-    if (!grid_ok(blocks, 256)) return IQK_ERR_GEOMETRY;
     if (wide_ids)
         hipLaunchKernelGGL(sort_dispatch_kernel<true>, dim3{uint32_t(blocks)}, dim3{256}, 0, as_stream(stream), sort, a);
     else

@@ -65,13 +65,18 @@ class LowRankAdapters(torch.nn.Module):
                 or down.shape[1] != self.in_features or up.shape[0] != self.out_features:
             raise IqkRuntimeError(f"an adapter is [r, {self.in_features}] and [{self.out_features}, r] with r up to "
                                   f"{self.rank}, got {tuple(down.shape)} and {tuple(up.shape)}")
-        r, ranks = down.shape[0], self.down.shape[2]
+        r, a, b = down.shape[0], self.down[index], self.up[index]
+        whole = r // 8 * 8
         with torch.no_grad():
-            a, b = (t.new_zeros(n, ranks, dtype=self.down.dtype) for t, n in ((down, self.in_features), (up, self.out_features)))
-            a[:, :r], b[:, :r] = down.T, up
-            self.down[index].copy_(a.view(-1, 8, ranks).transpose(1, 2))
-            self.up[index].copy_(b.view(-1, ranks // 8, 8).transpose(0, 1))
-            self.scales[index] = float(scale)
+            (a if r == a.shape[1] else a[:, :r]).copy_(down.reshape(r, -1, 8).transpose(0, 1))
+            if whole:
+                b[:whole // 8].copy_(up[:, :whole].reshape(-1, whole // 8, 8).transpose(0, 1))
+            if r < a.shape[1]:
+                a[:, r:].zero_()
+                b[whole // 8:].zero_()
+                if whole < r:
+                    b[whole // 8, :, :r - whole].copy_(up[:, whole:])
+            self.scales[index].fill_(float(scale))
 
     def adapter(self, index: int) -> tuple[torch.Tensor, torch.Tensor, float]:
         """Adapter ``index`` as :meth:`load` takes it, of rank R: ``(down, up, scale)``."""
