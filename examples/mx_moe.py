@@ -1,11 +1,12 @@
 """A mixture-of-experts layer whose experts are frozen 4-bit microscaled weights:
 its router trained with the balance loss, then the layer served.
 
-    python examples/mx_moe.py [--experts 64 --hidden 2048 --inner 1024 --top-k 6]
+    python examples/mx_moe.py [--experts 64 --hidden 2048 --inner 1024 --top-k 6 --requests 8]
 
 Training runs the prompts' tokens, in quantised activations, grouped by expert;
 the gradient reaches the router through the choice's weights and the balance
-loss.  Serving runs one token a step in 16 bits, from a captured graph.
+loss.  Serving runs one token of each request a step in 16 bits, from a captured graph, beside
+a projection that all tokens share, to which each request brings a low-rank adapter.
 """
 
 from __future__ import annotations
@@ -18,15 +19,17 @@ import torch
 
 sys.path.insert(0, os.path.join(os.path.dirname(os.path.abspath(__file__)), "..", "mlx-iqk_amd"))
 
-from mlx_iqk_amd import mx, router  # noqa: E402
+from mlx_iqk_amd import adapters, mx, router  # noqa: E402
 
 
 class MoE(torch.nn.Module):
-    """``y = sum_i w_i down_i(silu(gate_i x) * up_i x)`` over a token's top-k experts."""
+    """``y = sum_i w_i down_i(silu(gate_i x) * up_i x)`` over a token's top-k experts, and with a
+    ``shared`` projection (an ``MxLinear``) its output added."""
 
     def __init__(self, experts: int, hidden: int, inner: int, k: int, device="cuda"):
         super().__init__()
         self.k = k
+        self.shared = None
         self.score = torch.nn.Linear(hidden, experts, bias=False, device=device)
         self.gate = mx.MxSwitchLinear(experts, inner, hidden, device=device)
         self.up = mx.MxSwitchLinear(experts, inner, hidden, device=device)
@@ -37,11 +40,12 @@ class MoE(torch.nn.Module):
         for projection, w in ((self.gate, gate), (self.up, up), (self.down, down)):
             projection.load(mx.quantize(w))
 
-    def forward(self, x: torch.Tensor, quantized: bool = False):
+    def forward(self, x: torch.Tensor, quantized: bool = False, bank=None, requests=None):
         """``x`` 16-bit ``[tokens, hidden]`` -> (y ``[tokens, hidden]``, logits, ids).
 
         ``quantized``: the experts' activations in 4 bits too.  The experts have no
-        gradient in ``x``: one that wants it is refused.
+        gradient in ``x``: one that wants it is refused.  ``bank``: adapters of the shared
+        projection, of which ``requests`` ``[tokens]`` names each token's.
         """
         logits = self.score(x.float())
         weights, ids = router.topk(logits, self.k)
@@ -49,7 +53,8 @@ class MoE(torch.nn.Module):
         rows = cast(x[:, None, None])  # [tokens, 1, 1, hidden]: a row for all its pairs
         hidden = torch.nn.functional.silu(self.gate(rows, ids)) * self.up(rows, ids)
         y = self.down(cast(hidden), ids)[:, :, 0]  # [tokens, k, hidden]: a row a pair
-        return (weights[..., None] * y).sum(1).to(x.dtype), logits, ids
+        shared = None if self.shared is None else self.shared(x, bank, requests)
+        return router.combine(y, weights, add=shared), logits, ids
 
 
 def train_step(moe: MoE, optimizer, x: torch.Tensor, target: torch.Tensor, mask: torch.Tensor, alpha: float):
@@ -68,22 +73,27 @@ def train_step(moe: MoE, optimizer, x: torch.Tensor, target: torch.Tensor, mask:
 
 
 class Server:
-    """One decode step of the layer, captured once and replayed."""
+    """One decode step of the layer, captured once and replayed; with a ``bank``, each
+    token's adapter may be another one in every step."""
 
-    def __init__(self, moe: MoE, tokens: int, dtype=torch.bfloat16):
-        self.x = torch.zeros(tokens, moe.gate.in_features, dtype=dtype, device=moe.score.weight.device)
+    def __init__(self, moe: MoE, tokens: int, dtype=torch.bfloat16, bank=None):
+        device = moe.score.weight.device
+        self.x = torch.zeros(tokens, moe.gate.in_features, dtype=dtype, device=device)
+        self.requests = None if bank is None else torch.full((tokens,), -1, dtype=torch.int32, device=device)
         with torch.no_grad():
             side = torch.cuda.Stream()
             side.wait_stream(torch.cuda.current_stream())
             with torch.cuda.stream(side):
-                moe(self.x)
+                moe(self.x, bank=bank, requests=self.requests)
             torch.cuda.current_stream().wait_stream(side)
             self.graph = torch.cuda.CUDAGraph()
             with torch.cuda.graph(self.graph):
-                self.y = moe(self.x)[0]
+                self.y = moe(self.x, bank=bank, requests=self.requests)[0]
 
-    def __call__(self, x: torch.Tensor) -> torch.Tensor:
+    def __call__(self, x: torch.Tensor, requests: torch.Tensor | None = None) -> torch.Tensor:
         self.x.copy_(x)
+        if requests is not None:
+            self.requests.copy_(requests)
         self.graph.replay()
         return self.y
 
@@ -95,6 +105,18 @@ def random_layer(experts: int, hidden: int, inner: int, k: int) -> MoE:
     return moe
 
 
+def random_bank(moe: MoE, adapters_held: int, rank: int, dtype=torch.bfloat16) -> adapters.LowRankAdapters:
+    """Give the layer a shared projection, and it a bank of adapters."""
+    hidden, device = moe.gate.in_features, moe.score.weight.device
+    moe.shared = mx.MxLinear(hidden, hidden, device=device)
+    moe.shared.load(mx.quantize(0.02 * torch.randn(hidden, hidden, device=device, dtype=torch.bfloat16)))
+    bank = adapters.LowRankAdapters(adapters_held, hidden, hidden, rank, dtype=dtype, device=device)
+    for i in range(adapters_held):
+        bank.load(i, hidden ** -0.5 * torch.randn(rank, hidden, device=device),
+                  0.02 * torch.randn(hidden, rank, device=device), 2.0)
+    return bank
+
+
 def main(argv=None) -> list[float]:
     p = argparse.ArgumentParser(description=__doc__.split("\n\n")[0])
     p.add_argument("--experts", type=int, default=64)
@@ -104,6 +126,7 @@ def main(argv=None) -> list[float]:
     p.add_argument("--sequences", type=int, default=4)
     p.add_argument("--tokens", type=int, default=500)
     p.add_argument("--steps", type=int, default=20)
+    p.add_argument("--requests", type=int, default=8, help="requests served together, each with its adapter")
     a = p.parse_args(argv)
     torch.manual_seed(0)
     moe = random_layer(a.experts, a.hidden, a.inner, a.top_k)
@@ -121,14 +144,19 @@ def main(argv=None) -> list[float]:
         if step % 5 == 0 or step == a.steps - 1:
             print(f"step {step}: fit {float(fit):.4g}, balance {balances[-1]:.3f}, "
                   f"most tokens of one expert {int(counts.sum(0).max())}", flush=True)
-    serve = Server(moe, 1)
+    bank = random_bank(moe, a.requests, 16)
+    serve = Server(moe, a.requests, bank=bank)
+    requests = torch.arange(a.requests, device="cuda")
+    prompts = x.view(-1, a.hidden)
     start, end = (torch.cuda.Event(enable_timing=True) for _ in range(2))
     start.record()
     for t in range(200):
-        y = serve(x[0, t % a.tokens])
+        at = t * a.requests % (prompts.shape[0] - a.requests + 1)
+        y = serve(prompts[at:at + a.requests], requests)
     end.record()
     end.synchronize()
-    print(f"serving: {start.elapsed_time(end) / 200 * 1e3:.1f} us a token, |y| {float(y.float().abs().mean()):.3g}")
+    print(f"serving {a.requests} requests: {start.elapsed_time(end) / 200 * 1e3:.1f} us a step, "
+          f"|y| {float(y.float().abs().mean()):.3g}")
     return balances
 
 
