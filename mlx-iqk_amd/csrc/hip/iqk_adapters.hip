@@ -227,7 +227,7 @@ __global__ __launch_bounds__(64 * WAVES) void adapter_down_tiles_kernel(AdapterA
 #pragma unroll
     for (int c = 0; c < 2 * CT; ++c) {
         const uint32_t slot = 8 * c + r8, row = a.tile_rows[t * kTileSlots + 16 * group + slot];
-        x[c] = a.x + size_t(slot < slots ? row : 0u) * a.in;  // past the tile's: row 0, its sums not used
+        x[c] = a.x + size_t(slot < slots && row < a.T ? row : 0u) * a.in;  // past the tile's: row 0, its sums not used
     }
     float4_t acc[RT][CT];
 #pragma unroll
@@ -332,7 +332,7 @@ __global__ __launch_bounds__(256, KC <= 4 ? 2 : 1) void adapter_up_tiles_kernel(
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t begin = blockIdx.x % groups * 256 * a.columns, end = min(a.N, begin + 256 * a.columns);
     const uint4_t tile = a.tiles[t];
-    const uint32_t adapter = tile.x, slots = tile.z;
+    const uint32_t adapter = tile.x, slots = min(tile.z, uint32_t(kTileSlots));
     if (slots == 0) return;  // uniform
     uint32_t row[CT][2];  // a lane's outputs are of slots s8 and s8 + 8 of each group
 #pragma unroll
@@ -340,7 +340,7 @@ __global__ __launch_bounds__(256, KC <= 4 ? 2 : 1) void adapter_up_tiles_kernel(
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             const uint32_t slot = 16 * c + 8 * h + s8, of = a.tile_rows[t * kTileSlots + slot];
-            row[c][h] = slot < slots ? of : 0u;  // past the tile's: read, not written
+            row[c][h] = slot < slots && of < a.T ? of : 0u;  // past the tile's: read, not written
         }
     const uint32_t mine = 8 * (lane & 7u);
     if (adapter >= a.adapters) {  // rows without an adapter; uniform

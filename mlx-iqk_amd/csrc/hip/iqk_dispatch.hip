@@ -117,6 +117,7 @@ template <int WAVES>
 struct SortShared {
     __attribute__((aligned(16))) uint32_t words[(WAVES + 2) * kSortKeys + 3];
     uint32_t sums[WAVES];
+    uint32_t used;  // tiles with pairs
     __device__ __forceinline__ uint32_t *total() { return words; }  // pairs of each key
     // those of the shares before this one, then (tiles) where the key's pairs end
     __device__ __forceinline__ uint32_t *before(uint32_t K) { return words + K; }
@@ -244,10 +245,10 @@ __device__ __forceinline__ void sort_share(const SortArgs &a, SortShared<WAVES> 
         scan_keys(s, K, [&](uint32_t e) { return whole(totals[e]); }, [&](uint32_t e, uint32_t at) {
             own(e, at);
             befores[e] = at + totals[e];  // where the key's pairs end
-            if (e == K - 1) s.sums[0] = (at + whole(totals[e])) / kSortTile;  // all tiles with pairs
+            if (e == K - 1) s.used = (at + whole(totals[e])) / uint32_t(kSortTile);
         });
         if (first)
-            for (uint32_t i = s.sums[0] + threadIdx.x; i < a.n_tiles; i += THREADS) a.tiles[i] = uint4_t{0, 0, 0, 0};
+            for (uint32_t i = s.used + threadIdx.x; i < a.n_tiles; i += THREADS) a.tiles[i] = uint4_t{0, 0, 0, 0};
     } else {
         scan_keys(s, K, [&](uint32_t e) { return totals[e]; }, [&](uint32_t e, uint32_t at) {
             if (first) a.offsets[e] = int32_t(at);

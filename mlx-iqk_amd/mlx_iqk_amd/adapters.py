@@ -6,7 +6,8 @@ A server holds one set of weights and many small corrections to it: request by r
 output; :class:`~mlx_iqk_amd.mx.MxLinear` takes one in its call.
 
 Products are exact and summed in f32, the sum with the projection's output is rounded
-once.  Adapters are for serving: no gradient flows through, and rows that want one, or have
+once.  A call repeats bit for bit; a row's last bits may differ between calls that hold other
+rows beside it.  Adapters are for serving: no gradient flows through, and rows that want one, or have
 a forward-mode derivative, are refused, as the projections refuse them.
 """
 
