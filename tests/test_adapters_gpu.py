@@ -316,3 +316,29 @@ def test_refusals(device):
         LowRankAdapters(4, 48, 32, 8)(x, ids, y)  # a bank on the host
     with pytest.raises(IqkKernelError):
         LowRankAdapters(4, 48, 32, 8, device=device).half()(x.half(), ids, y.half())  # scales in 16 bits
+
+
+# rows sorted by adapter: banks of many adapters with a row or two each, one for all, none; columns
+# that do not divide among the parts; every count of ranks that has a form of its own, and its neighbours
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("rows,adapters,rank,out,n", (
+    (3000, 1024, 8, 40, 64), (1100, 1000, 16, 24, 72), (2500, 1, 17, 300, 4104), (1600, 2, 33, 1030, 1032), (1100, 5, 65, 264, 520),
+    (1090, 3, 72, 1025, 2056), (1200, 4, 129, 90, 1160), (1050, 2, 200, 513, 4096), (5000, 13, 40, 256, 256), (1030, 64, 64, 2048, 512)))
+def test_sorted_rows(device, dtype, rows, adapters, rank, out, n):
+    print(f"sorted rows {dtype} {rows} {adapters} {rank} {out} {n}", flush=True)
+    rng = np.random.default_rng(rows + rank)
+    bank = _bank(rng, min(adapters, 8), out, n, rank, dtype, device) if adapters <= 8 else None
+    if bank is None:  # a large bank, filled at once
+        bank = LowRankAdapters(adapters, out, n, rank, dtype=dtype, device=device)
+        g = torch.Generator(device=device).manual_seed(rows)
+        bank.down.normal_(0, n ** -0.5, generator=g)
+        bank.up.normal_(0, rank ** -0.5, generator=g)
+        bank.scales.uniform_(0.5, 2.0, generator=g)
+    x, y = _rows(rng, rows, n, dtype, device), _rows(rng, rows, out, dtype, device)
+    kinds = (rng.integers(-1, adapters, rows), np.sort(rng.integers(0, adapters, rows)), np.full(rows, -1),
+             np.where(rng.random(rows) < 0.02, rng.integers(0, adapters, rows), -1))
+    for ids in kinds if adapters <= 64 else kinds[:1] + kinds[2:]:
+        named = torch.from_numpy(ids).to(device)
+        got = bank(x, named, y)
+        _check(got, bank, x, ids, y, dtype)
+        assert torch.equal(bank(x, named, y), got)  # again, bit for bit
