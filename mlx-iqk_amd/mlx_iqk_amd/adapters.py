@@ -59,7 +59,8 @@ class LowRankAdapters(torch.nn.Module):
 
     def load(self, index: int, down: torch.Tensor, up: torch.Tensor, scale: float = 1.0) -> None:
         """Take adapter ``index``: ``down`` ``[r, in]`` and ``up`` ``[out, r]``, r up to the
-        bank's rank, rounded to its type; ``scale`` is alpha / r, say."""
+        bank's rank, rounded to its type; ``scale`` is alpha / r, say.  Ranks past r are zeros,
+        with which an infinity in ``x`` gives NaN."""
         if not 0 <= index < self.num_adapters:
             raise IqkRuntimeError(f"the bank holds adapters 0 .. {self.num_adapters - 1}, got {index}")
         if down.dim() != 2 or up.dim() != 2 or down.shape[0] != up.shape[1] or not 0 < down.shape[0] <= self.rank \

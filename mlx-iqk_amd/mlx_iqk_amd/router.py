@@ -229,6 +229,8 @@ def combine(y: torch.Tensor, weights: torch.Tensor, order: Order | None = None, 
         for t in (slots, offsets):
             if t.device != y.device or t.dtype != torch.int32 or not t.is_contiguous():
                 raise IqkKernelError(f"order must hold contiguous int32 tensors on {y.device}")
+        if not offsets.numel():
+            raise IqkKernelError("order must hold an offset behind its experts")
         want = (weights.numel(), y.shape[-1])
     if tuple(y.shape) != want:
         raise IqkKernelError(f"y must be {want} for weights {tuple(weights.shape)}, got {tuple(y.shape)}")

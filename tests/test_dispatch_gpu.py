@@ -441,6 +441,14 @@ def test_refusals(device):
             router.combine(*args, add=add)
 
 
+def test_an_order_without_offsets_is_refused(device):
+    print("order without offsets", flush=True)
+    order = router.sort(torch.zeros((3, 2), dtype=I32, device=device), 4)
+    bare = router.Order(order.offsets[:0], order.ids, order.tokens, order.slots)
+    with pytest.raises(IqkKernelError, match="offset"):
+        router.combine(torch.zeros((6, 8), device=device), torch.ones((3, 2), device=device), bare)
+
+
 def test_an_order_with_foreign_slots_reads_and_writes_nothing_outside(device):
     """Slots are bounded where they are used: what lies outside is skipped, as if left out."""
     print("foreign slots", flush=True)
