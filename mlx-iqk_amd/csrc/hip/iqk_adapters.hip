@@ -591,7 +591,7 @@ struct GroupPlan {
     int64_t tiles, splits, hist, desc, tile_rows, sums, words;
 };
 
-GroupPlan group_plan(int64_t in, int64_t rank, int64_t adapters, int64_t rows) {
+GroupPlan group_plan(int64_t in, int64_t rank, int64_t adapters, int64_t rows) {  // of a row at least
     GroupPlan p{};
     p.tiles = sort_tiles(rows, adapters);
     // the columns in parts where the tiles leave CUs empty: two workgroups a CU, 512 columns each at least
@@ -694,7 +694,7 @@ extern "C" {
 int64_t iqk_adapters_work(int64_t in_features, int64_t out_features, int64_t rank, int64_t num_adapters, int64_t rows) {
     using namespace iqk;
     if (!adapters_shape_ok(in_features, out_features, rank, num_adapters, rows)) return -1;
-    return rows_stand_alone(in_features, out_features, rank, rows)
+    return rows == 0 || rows_stand_alone(in_features, out_features, rank, rows)
                ? 0 : group_plan(in_features, rank, num_adapters, rows).words;
 }
 

@@ -123,3 +123,13 @@ def test_adapters_refuse_bad_arguments(lib):
     for per_id in (0, -1, 1 << 31):
         assert f(*[per_id if i == 9 else v for i, v in enumerate(good)]) == _native.ERR_ARGUMENT
     assert f(2, 64, 48, 8, 4, None, 0, None, 0, 1, None, None, None, None, None, None, None) == _native.OK
+
+
+def test_no_rows_need_no_workspace(lib):
+    """Also for sizes of which one row is too much for a workgroup of its own, and so is sorted."""
+    p = ctypes.c_void_p(16)  # never dereferenced: no rows, no launch
+    for n, out, rank, adapters in ((4096, 4096, 16, 64), (4096, 4096, 128, 64), (4096, 4096, 256, 1024), (1 << 20, 8, 8, 1)):
+        assert lib.iqk_adapters_work(n, out, rank, adapters, 0) == 0
+        assert lib.iqk_adapters(1, n, out, rank, adapters, p, 0, p, 0, 1, p, p, p, None, p, p, None) == _native.OK
+        assert lib.iqk_adapters_work(n, out, rank, adapters, 1) >= 0
+    assert lib.iqk_adapters_work(4096, 4096, 128, 64, 1) > 0
