@@ -175,15 +175,22 @@ __global__ __launch_bounds__(kAloneThreads) void adapter_row_kernel(AdapterArgs 
 // Rows sorted by adapter, in tiles of 64 slots of one adapter; both products on the
 // 16x16x32 MFMAs, operand A the adapter's (16 ranks, 16 outputs), operand B 16 slots'.  The
 // first kernel leaves A x in f32, a sum for each part of the columns; the second adds these
-// and splits them into 16-bit pieces that give f32 back: a bf16 product takes three pieces of eight
-// bits (truncated, so that their sum is exact), an f16 product two of eleven bits over a
-// power of two of the slot's largest, which is multiplied back in f32.
+// and splits each value into three 16-bit pieces.  bf16 has f32's exponents: pieces of eight bits,
+// truncated, whose sum is the value.  f16 has fewer: a slot's values are multiplied with a power of
+// two that brings the largest to 2^14 .. 2^15 (their sums are divided by it), and two pieces of
+// eleven bits leave a rest of at most 2^-23 of the value or 2^-25, the third piece, times 2^24.  That
+// is off by at most 2^-12 of the rest, so that the sum is off by 2^-24 of a value, an f32
+// rounding, down to 2^-13, 2^27 below the slot's largest.  (Two pieces are off by 2^-23, and lose more from
+// 2^17 below the largest on; rank 64 as below, 88.9 us with two, 90.1 with three.)  Where a rank of
+// 16 slots is smaller still, or finite beside an infinity, their chunk of 32 ranks stays f32 and goes through
+// the 16x16x4 f32 MFMAs (146 us with such a rank in every tile).
 
 constexpr uint32_t kMaxSplits = 4;  // parts of the columns
 constexpr int kTileSlots = int(kSortTile), kTileGroups = kTileSlots / 16;
 
-template <bool BF>
-constexpr int kPieces = BF ? 3 : 2;
+constexpr int kPieces = 3;
+constexpr float kThird = 0x1p24f;  // what f16's third piece is multiplied with
+constexpr uint32_t kLeastBits = 0x39000000u;  // 2^-13, the smallest value that f16 pieces stand for
 
 template <bool BF>
 __device__ __forceinline__ float4_t mfma(uint4_t a, uint4_t b, float4_t c) {
@@ -320,12 +327,13 @@ __global__ __launch_bounds__(64 * WAVES) void adapter_down_tiles_kernel(AdapterA
 // 89 now, of which this kernel 62, 4.3 TB/s of y read and written).
 template <bool BF, int KC>
 __global__ __launch_bounds__(256, KC <= 4 ? 2 : 1) void adapter_up_tiles_kernel(AdapterArgs a) {
-    constexpr int P = kPieces<BF>, CT = kTileGroups, STAGE = KC < 2 ? KC : 2;  // chunks of B in registers at once
+    constexpr int P = kPieces, CT = kTileGroups, STAGE = KC < 2 ? KC : 2;  // chunks of B in registers at once
     // B is loaded with the column before's, or (more registers than there are) with its own, once for
     // all slots, or (more than those) for each group of slots again; y always is ahead
     constexpr bool AHEAD = KC == 1, ONCE = KC <= 2;
     __shared__ uint4_t operands[CT][KC][P][64];
     __shared__ float powers[kTileSlots];  // what an f16 slot's sums are multiplied with
+    __shared__ uint32_t chunks_in_f32[4];
     __shared__ __attribute__((aligned(16))) float turned[4][16][64 + 4];
     const uint32_t groups = (a.N + 256 * a.columns - 1) / (256 * a.columns), t = blockIdx.x / groups;
     const uint32_t lane = threadIdx.x & 63u, g = lane >> 4, m = lane & 15u, s8 = lane >> 3;
@@ -402,35 +410,54 @@ __global__ __launch_bounds__(256, KC <= 4 ? 2 : 1) void adapter_up_tiles_kernel(
     // A x: the parts' sum, scaled, in pieces; a thread has eight ranks of a slot, 4 KC threads a slot
     constexpr int EIGHTS = 4 * KC;
     const float scale = a.scales[adapter];
+    uint32_t in_f32 = 0;  // f16: the chunks of a group of slots (bit KC c + chunk) that stay f32
+    const auto values = [&](uint32_t slot, uint32_t eight, float(&v)[8]) __attribute__((always_inline)) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] = 0.f;
+        if (8 * eight >= a.rank || slot >= slots) return;
+        const float *const from = a.sums + (size_t(t) * kTileSlots + slot) * a.rank + 8 * eight;
+        float4_t parts[kMaxSplits][2];  // all on their way at once; past the last: it again
+#pragma unroll
+        for (uint32_t p = 0; p < kMaxSplits; ++p) {
+            const float4_t *const part = reinterpret_cast<const float4_t *>(
+                from + size_t(min(p, a.splits - 1u)) * a.n_tiles * kTileSlots * a.rank);
+            parts[p][0] = part[0];
+            parts[p][1] = part[1];
+        }
+#pragma unroll
+        for (uint32_t p = 0; p < kMaxSplits; ++p) {
+            if (p >= a.splits) continue;  // uniform
+#pragma unroll
+            for (int k = 0; k < 4; ++k) v[k] += parts[p][0][k], v[4 + k] += parts[p][1][k];
+        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] *= scale;
+    };
+    // f16: the slot's power of two, and the values times it.  The largest comes to 2^14 .. 2^15; with an
+    // infinity (or nothing) all stay as they are.
+    const auto by_power = [&](float(&v)[8], float &most) __attribute__((always_inline)) {
+        most = 0.f;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) most = fmaxf(most, fabsf(v[k]));
+#pragma unroll
+        for (int off = 1; off < EIGHTS; off <<= 1) most = fmaxf(most, __shfl_xor(most, off, 64));
+        const int e = most > 0.f && most < __builtin_inff() ? 14 - ilogbf(most) : 0;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] = ldexpf(v[k], e);
+        return e;
+    };
+    // operand B of a chunk of 32 ranks: lane 16 g + n has slot n's ranks 8 g ..
+    const auto place = [&](uint32_t slot, uint32_t eight, int p) -> uint4_t & {
+        return operands[slot / 16][eight / 4][p][16 * (eight & 3u) + (slot & 15u)];
+    };
 #pragma unroll
     for (int i = 0; i < kTileSlots * EIGHTS / 256; ++i) {
         const uint32_t u = 256 * i + threadIdx.x, slot = u / EIGHTS, eight = u % EIGHTS;
-        float v[8] = {};
-        if (8 * eight < a.rank && slot < slots) {
-            const float *const from = a.sums + (size_t(t) * kTileSlots + slot) * a.rank + 8 * eight;
-            float4_t parts[kMaxSplits][2];  // all on their way at once; past the last: it again
-#pragma unroll
-            for (uint32_t p = 0; p < kMaxSplits; ++p) {
-                const float4_t *const part = reinterpret_cast<const float4_t *>(
-                    from + size_t(min(p, a.splits - 1u)) * a.n_tiles * kTileSlots * a.rank);
-                parts[p][0] = part[0];
-                parts[p][1] = part[1];
-            }
-#pragma unroll
-            for (uint32_t p = 0; p < kMaxSplits; ++p) {
-                if (p >= a.splits) continue;  // uniform
-#pragma unroll
-                for (int k = 0; k < 4; ++k) v[k] += parts[p][0][k], v[4 + k] += parts[p][1][k];
-            }
-#pragma unroll
-            for (int k = 0; k < 8; ++k) v[k] *= scale;
-        }
-        // operand B of a chunk of 32 ranks: lane 16 g + n has slot n's ranks 8 g ..
-        uint4_t(*const to)[64] = operands[slot / 16][eight / 4];
-        const uint32_t at = 16 * (eight & 3u) + (slot & 15u);
+        float v[8];
+        values(slot, eight, v);
         if constexpr (BF) {
 #pragma unroll
-            for (int p = 0; p < 3; ++p) {
+            for (int p = 0; p < P; ++p) {
                 uint4_t out;
 #pragma unroll
                 for (int k = 0; k < 8; ++k) {
@@ -441,36 +468,63 @@ __global__ __launch_bounds__(256, KC <= 4 ? 2 : 1) void adapter_up_tiles_kernel(
                     v[k] = finite ? v[k] - __builtin_bit_cast(float, bits & 0xffff0000u) : 0.f;
                     out[k / 2] = k & 1 ? out[k / 2] | top << 16 : top;
                 }
-                to[p][at] = out;
+                place(slot, eight, p) = out;
             }
         } else {
-            float most = 0.f;
+            float most;
+            const int e = by_power(v, most);
+            uint32_t least = ~0u;  // bits of the smallest value but zeros, less 1
 #pragma unroll
-            for (int k = 0; k < 8; ++k) most = fmaxf(most, fabsf(v[k]));
-#pragma unroll
-            for (int off = 1; off < EIGHTS; off <<= 1) most = fmaxf(most, __shfl_xor(most, off, 64));
-            // the largest to 2^14 .. 2^15; with an infinity (or nothing) as it is
-            const int e = most > 0.f && most < __builtin_inff() ? 14 - ilogbf(most) : 0;
-            uint4_t hi, lo;
-#pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                const float scaled = ldexpf(v[k], e);
-                const uint32_t top = float_to_half_bits(scaled);
-                const float rest = fabsf(scaled) < __builtin_inff() ? scaled - half_bits_to_float(top) : 0.f;
-                const uint32_t low = float_to_half_bits(rest);
-                hi[k / 2] = k & 1 ? hi[k / 2] | top << 16 : top;
-                lo[k / 2] = k & 1 ? lo[k / 2] | low << 16 : low;
-            }
-            to[0][at] = hi;
-            to[1][at] = lo;
+            for (int k = 0; k < 8; ++k) least = min(least, (__builtin_bit_cast(uint32_t, v[k]) & 0x7fffffffu) - 1u);
+            // zeros are all ones here, NaN goes through the pieces
+            if (least < kLeastBits - 1u || most == __builtin_inff()) in_f32 |= 1u << (slot / 16 * KC + eight / 4);
             if (eight == 0) powers[slot] = ldexpf(1.f, -e);
+#pragma unroll
+            for (int p = 0; p < P; ++p) {
+                uint4_t out;
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    const uint32_t top = float_to_half_bits(v[k]);
+                    v[k] = (v[k] - half_bits_to_float(top)) * (p == 1 ? kThird : 1.f);
+                    out[k / 2] = k & 1 ? out[k / 2] | top << 16 : top;
+                }
+                place(slot, eight, p) = out;
+            }
         }
     }
+    if constexpr (!BF) {
+        if (__ballot(in_f32 != 0)) {
+#pragma unroll
+            for (int off = 32; off > 0; off >>= 1) in_f32 |= uint32_t(__shfl_xor(int(in_f32), off, 64));
+        }
+        if (lane == 0) chunks_in_f32[wave] = in_f32;
+    }
     __syncthreads();
-    // WHOLE: every slot and output of the columns is there, and stored without a condition
-    const auto compute = [&](auto live, auto whole, uint32_t n0) __attribute__((always_inline)) {
+    if constexpr (!BF) {
+        in_f32 = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) in_f32 |= chunks_in_f32[i];
+        in_f32 = __builtin_amdgcn_readfirstlane(in_f32);
+        if (in_f32) {
+            for (int i = 0; i < kTileSlots * EIGHTS / 256; ++i) {
+                const uint32_t u = 256 * i + threadIdx.x, slot = u / EIGHTS, eight = u % EIGHTS;
+                float v[8], most;
+                values(slot, eight, v);
+                by_power(v, most);
+                if (in_f32 >> (slot / 16 * KC + eight / 4) & 1u) {
+#pragma unroll
+                    for (int p = 0; p < 2; ++p)
+                        place(slot, eight, p) = __builtin_bit_cast(uint4_t, float4_t{v[4 * p], v[4 * p + 1], v[4 * p + 2], v[4 * p + 3]});
+                }
+            }
+            __syncthreads();
+        }
+    }
+    // WHOLE: every slot and output of the columns is there, and stored without a condition.  ANY_F32: a chunk
+    // may be in f32 (a loop of its own with nothing ahead: the others have no registers left)
+    const auto compute = [&](auto live, auto whole, auto any_f32, uint32_t n0) __attribute__((always_inline)) {
         constexpr int LIVE = decltype(live)::value;
-        constexpr bool WHOLE = decltype(whole)::value;
+        constexpr bool WHOLE = decltype(whole)::value, ANY_F32 = decltype(any_f32)::value;
         const uint32_t n = n0 + mine, have = n < a.N ? min(a.N - n, 8u) : 0u;
         if constexpr (ONCE) {  // past the ranks: zeros, as in the slots' operands
 #pragma unroll
@@ -497,14 +551,43 @@ __global__ __launch_bounds__(256, KC <= 4 ? 2 : 1) void adapter_up_tiles_kernel(
                             for (int j = 0; j < 4; ++j) w[0][s][j] = uint4_t{0, 0, 0, 0};
                         }
                 }
+                if (!BF && k0) {
 #pragma unroll
-                for (int s = 0; s < STAGE; ++s)
+                    for (int j = 0; j < 4; ++j) acc[j] *= kThird;  // a power of two, as the third pieces are
+                }
 #pragma unroll
-                    for (int p = P - 1; p >= 0; --p) {  // the small pieces first
+                for (int p = P - 1; p >= 0; --p) {  // the small pieces first
+#pragma unroll
+                    for (int s = 0; s < STAGE; ++s) {
+                        if (ANY_F32 && (in_f32 >> (KC * c + k0 / 32 + s) & 1u)) continue;  // uniform
                         const uint4_t b = operands[c][k0 / 32 + s][p][lane];
 #pragma unroll
                         for (int j = 0; j < 4; ++j) acc[j] = mfma<BF>(w[0][s][j], b, acc[j]);
                     }
+                    if (!BF && p == 2) {
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) acc[j] *= 1 / kThird;
+                    }
+                }
+                if constexpr (ANY_F32) {
+#pragma unroll
+                    for (int s = 0; s < STAGE; ++s) {
+                        if (!(in_f32 >> (KC * c + k0 / 32 + s) & 1u)) continue;  // uniform
+                        const auto *const operand = operands[c][k0 / 32 + s];
+                        const float4_t b[2] = {__builtin_bit_cast(float4_t, operand[0][lane]),
+                                               __builtin_bit_cast(float4_t, operand[1][lane])};
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) {
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) {
+                                uint32_t pair = w[0][s][j][k / 2];
+                                asm volatile("" : "+v"(pair));  // made f32 here, not once for all groups and kept
+                                acc[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(
+                                    float_of16<BF>(uint16_t(k & 1 ? pair >> 16 : pair)), b[k / 4][k % 4], acc[j], 0, 0, 0);
+                            }
+                        }
+                    }
+                }
             }
             wavefront_fence();
             const float power = BF ? 1.f : powers[16 * c + m];
@@ -546,7 +629,7 @@ __global__ __launch_bounds__(256, KC <= 4 ? 2 : 1) void adapter_up_tiles_kernel(
             load_y(live, 1, column(i + 1));
             if (AHEAD) load_w(AHEAD ? 1 : 0, column(i + 1), 0);
             __builtin_amdgcn_sched_barrier(0);
-            compute(live, whole, column(i));
+            compute(live, whole, std::false_type{}, column(i));
 #pragma unroll
             for (int c = 0; c < decltype(live)::value; ++c)
 #pragma unroll
@@ -559,8 +642,19 @@ __global__ __launch_bounds__(256, KC <= 4 ? 2 : 1) void adapter_up_tiles_kernel(
             }
         }
         if (ONCE && !AHEAD && turns > 1) load_w(0, column(turns - 1), 0);
-        compute(live, whole, column(turns - 1));
+        compute(live, whole, std::false_type{}, column(turns - 1));
     };
+    if constexpr (!BF) {
+        if (in_f32) {
+            const std::integral_constant<int, CT> live{};
+            for (uint32_t i = 0; i < turns; ++i) {
+                load_y(live, 0, column(i));
+                if (ONCE) load_w(0, column(i), 0);
+                compute(live, std::false_type{}, std::true_type{}, column(i));
+            }
+            return;
+        }
+    }
     if (slots == kTileSlots && (end - begin) % 256 == 0)
         all(std::integral_constant<int, 4>{}, std::true_type{});
     else
