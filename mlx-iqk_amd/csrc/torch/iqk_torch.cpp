@@ -278,12 +278,13 @@ struct Dispatch : torch::autograd::Function<Dispatch> {
 struct Combine : torch::autograd::Function<Combine> {
     static variable_list forward(AutogradContext *ctx, const Tensor &y, const Tensor &weights,
                                  const std::optional<Tensor> &slots, const std::optional<Tensor> &offsets,
-                                 const std::optional<Tensor> &add) {
+                                 const std::optional<Tensor> &add, bool permutation) {
         ctx->set_materialize_grads(false);
         const bool dy = y.requires_grad(), dw = weights.requires_grad();
         ctx->saved_data["dy"] = dy;
         ctx->saved_data["dw"] = dw;
         ctx->saved_data["dadd"] = add && add->requires_grad();
+        ctx->saved_data["every_row"] = permutation;  // has a pair that writes its gradient
         ctx->saved_data["shape"] = y.sizes().vec();
         const Tensor s = slots.value_or(Tensor()), o = offsets.value_or(Tensor());
         // y for the weights' gradient only, which is the larger by far
@@ -292,14 +293,17 @@ struct Combine : torch::autograd::Function<Combine> {
     }
     static variable_list backward(AutogradContext *ctx, variable_list grads) {
         refuse_capture();
-        variable_list out(5);
+        variable_list out(6);
         if (!grads[0].defined()) return out;
         const auto saved = ctx->get_saved_variables();
         const Tensor &y = saved[0], &weights = saved[1], &slots = saved[2], &offsets = saved[3];
         const c10::DeviceGuard guard(grads[0].device());
         const Tensor dout = grads[0].detach().contiguous();
         Tensor dy, dweights;
-        if (ctx->saved_data["dy"].toBool()) dy = empty(ctx->saved_data["shape"].toIntVector(), dout.scalar_type(), dout);
+        if (ctx->saved_data["dy"].toBool()) {
+            dy = empty(ctx->saved_data["shape"].toIntVector(), dout.scalar_type(), dout);
+            if (!ctx->saved_data["every_row"].toBool()) dy.zero_();
+        }
         if (ctx->saved_data["dw"].toBool()) dweights = empty(weights.sizes(), at::kFloat, dout);
         if (dy.defined() || dweights.defined()) {
             const int64_t k = weights.size(-1);
@@ -477,10 +481,10 @@ PyObject *py_dispatch(PyObject *, PyObject *const *args, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
-// combine(y, weights, slots | None, offsets | None, add | None) -> out
+// combine(y, weights, slots | None, offsets | None, add | None, whether sort gave the slots) -> out
 PyObject *py_combine(PyObject *, PyObject *const *args, Py_ssize_t n) {
     HANDLE_TH_ERRORS
-    arguments(n, 5);
+    arguments(n, 6);
     for (int i = 0; i < 5; ++i)
         if (!THPVariable_Check(args[i]) && (i < 2 || args[i] != Py_None)) Py_RETURN_NONE;
     const Tensor &y = tensor(args[0]), &weights = tensor(args[1]);
@@ -505,7 +509,9 @@ PyObject *py_combine(PyObject *, PyObject *const *args, Py_ssize_t n) {
     const c10::DeviceGuard guard(y.device());
     if (wants_grad(y) || wants_grad(weights) || (add.defined() && wants_grad(add))) {
         const auto given = [](const Tensor &t) { return t.defined() ? std::optional<Tensor>(t) : std::nullopt; };
-        return THPVariable_Wrap(Combine::apply(y, weights, given(slots), given(offsets), given(add))[0]);
+        // what sort gave is a permutation until it is written to
+        const bool permutation = !slots.defined() || (args[5] == Py_True && !slots.is_inference() && slots._version() == 0);
+        return THPVariable_Wrap(Combine::apply(y, weights, given(slots), given(offsets), given(add), permutation)[0]);
     }
     return THPVariable_Wrap(combine_forward(y, weights, slots, offsets, add));
     END_HANDLE_TH_ERRORS

@@ -100,7 +100,11 @@ def balance_loss(logits: torch.Tensor, ids: torch.Tensor, *,
     return _native.torch_binding().balance(logits.contiguous(), ids.contiguous(), mask)
 
 
-class Order:
+class _Slots:
+    __slots__ = ("_permutation",)  # an order's slots, where they are known to be one
+
+
+class Order(_Slots):
     """Token-expert pairs in the order of their experts (:func:`sort`): int32 tensors on
     the ids' device,
 
@@ -110,13 +114,19 @@ class Order:
     * ``tokens`` ``[pairs]``: each slot's token;
     * ``slots`` ``[..., k]``: each pair's slot, a permutation.
 
-    Within an expert the pairs keep their order.
+    Within an expert the pairs keep their order.  :func:`combine` also takes an order with other
+    slots: one outside ``0 .. pairs - 1`` (-1, say) leaves its pair out.  A slot of
+    several pairs counts for each of them, but has no gradient that is defined.
     """
 
     __slots__ = ("offsets", "ids", "tokens", "slots")
 
     def __init__(self, offsets: torch.Tensor, ids: torch.Tensor, tokens: torch.Tensor, slots: torch.Tensor):
         self.offsets, self.ids, self.tokens, self.slots = offsets, ids, tokens, slots
+        self._permutation = None
+
+    def __reduce__(self):  # a copy's slots may have been changed before
+        return Order, (self.offsets, self.ids, self.tokens, self.slots)
 
     @property
     def num_experts(self) -> int:
@@ -156,7 +166,14 @@ def sort(ids: torch.Tensor, num_experts: int) -> Order:
     sort_pairs = _native.torch_binding().sort
     if (lists := sort_pairs(ids, num_experts)) is None:  # ids that the kernels do not take as they are
         lists = sort_pairs(*_check_ids(ids, num_experts))
-    return Order(*lists)
+    return _sorted(*lists)
+
+
+def _sorted(offsets, ids, tokens, slots) -> Order:
+    """The order of the binding's lists."""
+    order = Order(offsets, ids, tokens, slots)
+    order._permutation = slots
+    return order
 
 
 def _check_rows(t: torch.Tensor, name: str, device: torch.device) -> None:
@@ -187,7 +204,7 @@ def dispatch(x: torch.Tensor, ids: torch.Tensor, num_experts: int) -> tuple[torc
             raise IqkKernelError(f"x {tuple(x.shape)} and ids {tuple(ids.shape)} are not of the same tokens")
         got = dispatch_rows(x.contiguous(), ids, experts)
     rows, offsets, sorted_ids, tokens, slots = got
-    return rows, Order(offsets, sorted_ids, tokens, slots)
+    return rows, _sorted(offsets, sorted_ids, tokens, slots)
 
 
 def combine(y: torch.Tensor, weights: torch.Tensor, order: Order | None = None, *,
@@ -199,13 +216,13 @@ def combine(y: torch.Tensor, weights: torch.Tensor, order: Order | None = None, 
     ``[..., k]``; ``add`` ``[..., n]``, y's type, is added (a shared
     expert's output, the residual).  Sums are f32, rounded once.  Pairs that the order leaves out count
     for nothing, whatever their rows hold; without an order every row counts.  Differentiable in
-    ``y``, ``weights`` and ``add``; the gradients of pairs left out are 0.
+    ``y``, ``weights`` and ``add``; the gradients of pairs left out are 0, as are those of rows that no pair has.
     """
     combine_rows = _native.torch_binding().combine
     if order is None:
-        out = combine_rows(y, weights, None, None, add)
+        out = combine_rows(y, weights, None, None, add, False)
     elif type(order) is Order:
-        out = combine_rows(y, weights, order.slots, order.offsets, add)
+        out = combine_rows(y, weights, order.slots, order.offsets, add, order._permutation is order.slots)
     else:
         raise IqkKernelError(f"order must be an Order, got {type(order).__name__}")
     if out is not None:
@@ -220,12 +237,13 @@ def combine(y: torch.Tensor, weights: torch.Tensor, order: Order | None = None, 
         raise IqkKernelError(f"weights must be [..., k] with k 1 .. {MAX_K} and fewer than 2**31 pairs, got "
                              f"{tuple(weights.shape)}")
     slots = offsets = None
+    permutation = False
     if order is None:
         want = (*weights.shape, y.shape[-1])
     else:
         if order.slots.shape != weights.shape:
             raise IqkKernelError(f"order must be one of pairs {tuple(weights.shape)}, got {order!r}")
-        slots, offsets = order.slots, order.offsets
+        slots, offsets, permutation = order.slots, order.offsets, order._permutation is order.slots
         for t in (slots, offsets):
             if t.device != y.device or t.dtype != torch.int32 or not t.is_contiguous():
                 raise IqkKernelError(f"order must hold contiguous int32 tensors on {y.device}")
@@ -240,7 +258,7 @@ def combine(y: torch.Tensor, weights: torch.Tensor, order: Order | None = None, 
             raise IqkKernelError(f"add must be {y.dtype} {(*weights.shape[:-1], y.shape[-1])}, got {add.dtype} "
                                  f"{tuple(add.shape)}")
         add = add.contiguous()
-    return combine_rows(y.contiguous(), weights.float().contiguous(), slots, offsets, add)
+    return combine_rows(y.contiguous(), weights.float().contiguous(), slots, offsets, add, permutation)
 
 
 __all__ = ["MAX_COLS", "MAX_EXPERTS", "MAX_GROUPS", "MAX_K", "Order", "balance_loss", "combine", "dispatch", "sort", "topk"]

@@ -3,6 +3,8 @@ plain 64-bit forms on the CPU."""
 
 from __future__ import annotations
 
+import copy
+
 import numpy as np
 import pytest
 import torch
@@ -572,3 +574,48 @@ def test_trained_experts(device):
     for got, want in zip(grads, torch.autograd.grad(out, (x64, w64, l64), dout.cpu().double())):
         # f32 throughout: sums of at most 24 to 80 terms of the size of the largest results
         assert float((got.cpu().double() - want).abs().max()) <= 100 * U * 8 * float(want.abs().max())
+
+
+def test_rows_that_no_pair_has_get_zero_gradients(device):
+    """Orders whose slots are no permutation: made by a caller, assigned, or changed in place (pairs dropped)."""
+    print("rows without a pair", flush=True)
+    experts, tokens, k = 7, 300, 3
+    rng = np.random.default_rng(21)
+    ids = torch.from_numpy(rng.integers(0, experts, (tokens, k))).to(device)
+    for cols, dtype in ((8, F32), (2048, F16)):
+        y = torch.from_numpy(rng.standard_normal((tokens * k, cols))).to(dtype).to(device).requires_grad_()
+        w = torch.from_numpy(rng.random((tokens, k)).astype(np.float32)).to(device).requires_grad_()
+        dout = torch.from_numpy(rng.standard_normal((tokens, cols))).to(dtype).to(device)
+        whole = router.sort(ids, experts)
+        want_dy, want_dw = torch.autograd.grad(router.combine(y, w, whole), (y, w), dout)
+        drop = torch.from_numpy(rng.random((tokens, k)) < 0.4).to(device)
+        kept = torch.ones(tokens * k, dtype=torch.bool, device=device)
+        kept[whole.slots[drop].long()] = False
+        lists = whole.offsets, whole.ids, whole.tokens
+        made = router.Order(*lists, whole.slots.masked_fill(drop, -1))
+        assigned = router.sort(ids, experts)
+        assigned.slots = made.slots
+        changed = router.sort(ids, experts)
+        changed.slots.masked_fill_(drop, tokens * k)
+        _, moved = router.dispatch(torch.zeros((tokens, 4), device=device), ids, experts)
+        moved.slots[drop] = -1
+        for order in (made, assigned, changed, moved, copy.copy(changed), copy.deepcopy(changed)):
+            for _ in range(2):
+                torch.full_like(y, float("nan"))  # what memory that is taken up again holds
+                dy, dw = torch.autograd.grad(router.combine(y, w, order), (y, w), dout)
+                assert torch.equal(dy[kept], want_dy[kept]) and not dy[~kept].any() and not dy.isnan().any()
+                assert torch.equal(dw, want_dw.masked_fill(drop, 0.0))
+        for order in (whole, copy.copy(whole), copy.deepcopy(whole)):
+            got = torch.autograd.grad(router.combine(y, w, order), (y, w), dout)
+            assert torch.equal(got[0], want_dy) and torch.equal(got[1], want_dw)
+
+
+def test_an_orders_foreign_slots_leave_zero_gradients(device):
+    print("foreign slots' gradients", flush=True)
+    order = router.sort(torch.tensor([[0, 1], [2, 0]], device=device), 3)
+    y = torch.ones((4, 8), device=device, requires_grad=True)
+    bad = router.Order(order.offsets, order.ids, order.tokens,
+                       torch.tensor([[-1, 2 ** 30], [4, 1]], dtype=I32, device=device))
+    torch.full((4, 8), float("nan"), device=device)
+    (dy,) = torch.autograd.grad(router.combine(y, torch.ones((2, 2), device=device), bad), y, torch.ones((2, 8), device=device))
+    assert dy.tolist() == [[0.0] * 8, [1.0] * 8, [0.0] * 8, [0.0] * 8]
