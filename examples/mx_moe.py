@@ -128,6 +128,9 @@ def main(argv=None) -> list[float]:
     p.add_argument("--steps", type=int, default=20)
     p.add_argument("--requests", type=int, default=8, help="requests served together, each with its adapter")
     a = p.parse_args(argv)
+    if not 0 < a.requests <= min(a.sequences * a.tokens, adapters.MAX_ADAPTERS):
+        p.error(f"--requests must be 1 .. {min(a.sequences * a.tokens, adapters.MAX_ADAPTERS)}, the prompts' tokens or the "
+                f"adapters of a bank, got {a.requests}")
     torch.manual_seed(0)
     moe = random_layer(a.experts, a.hidden, a.inner, a.top_k)
     with torch.no_grad():  # a router that favours a few experts

@@ -3,6 +3,8 @@
 from __future__ import annotations
 
 import ctypes
+import importlib.util
+from pathlib import Path
 
 import pytest
 import torch
@@ -133,3 +135,14 @@ def test_no_rows_need_no_workspace(lib):
         assert lib.iqk_adapters(1, n, out, rank, adapters, p, 0, p, 0, 1, p, p, p, None, p, p, None) == _native.OK
         assert lib.iqk_adapters_work(n, out, rank, adapters, 1) >= 0
     assert lib.iqk_adapters_work(4096, 4096, 128, 64, 1) > 0
+
+
+@pytest.mark.parametrize("requests", ("0", "-3", "41", "1025"))
+def test_the_example_refuses_requests_that_its_prompts_do_not_hold(requests, capsys):
+    spec = importlib.util.spec_from_file_location("mx_moe", Path(__file__).parents[1] / "examples" / "mx_moe.py")
+    mx_moe = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(mx_moe)
+    tokens = "10" if requests != "1025" else "2000"
+    with pytest.raises(SystemExit):
+        mx_moe.main(["--sequences", "4", "--tokens", tokens, "--requests", requests])
+    assert "--requests must be" in capsys.readouterr().err
