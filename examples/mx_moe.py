@@ -53,6 +53,8 @@ class MoE(torch.nn.Module):
         rows = cast(x[:, None, None])  # [tokens, 1, 1, hidden]: a row for all its pairs
         hidden = torch.nn.functional.silu(self.gate(rows, ids)) * self.up(rows, ids)
         y = self.down(cast(hidden), ids)[:, :, 0]  # [tokens, k, hidden]: a row a pair
+        if self.shared is None and (bank is not None or requests is not None):
+            raise ValueError("adapters add to the shared projection, which this layer has not")
         shared = None if self.shared is None else self.shared(x, bank, requests)
         return router.combine(y, weights, add=shared), logits, ids
 
@@ -91,6 +93,10 @@ class Server:
                 self.y = moe(self.x, bank=bank, requests=self.requests)[0]
 
     def __call__(self, x: torch.Tensor, requests: torch.Tensor | None = None) -> torch.Tensor:
+        """``requests``: each token's adapter (-1: none), with a bank and only with one."""
+        if (requests is None) != (self.requests is None):
+            raise ValueError("requests name adapters of the bank, for which the server was made without" if requests is not None
+                             else "the server was made with a bank: name each token's adapter, -1 for none")
         self.x.copy_(x)
         if requests is not None:
             self.requests.copy_(requests)

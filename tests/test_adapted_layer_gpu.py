@@ -169,3 +169,33 @@ def test_narrow_outputs(device, out, rows):
         error = 60 * U * size
         want = old + t @ up.T
         assert (np.abs(got[at] - want) <= error + mxref.HALF_ULP[F16] * (np.abs(want) + error) + mxref.TINY[F16]).all()
+
+
+def test_the_example_server_wants_requests_with_a_bank_only(mx_moe):
+    """A step without requests would take those of the step before."""
+    print("example server's requests", flush=True)
+    torch.manual_seed(3)
+    moe = mx_moe.random_layer(6, 64, 32, 2)
+    x = torch.randn(2, 64, device="cuda", dtype=BF16)
+    requests = torch.tensor([0, 1], device="cuda")
+    bare = mx_moe.Server(moe, 2)
+    with torch.no_grad():
+        assert torch.equal(bare(x), moe(x)[0])
+    with pytest.raises(ValueError, match="without"):
+        bare(x, requests)
+    bank = LowRankAdapters(2, 64, 64, 4, device="cuda")
+    for given in ((bank, requests), (bank, None), (None, requests)):
+        with pytest.raises(ValueError, match="shared"):
+            moe(x, bank=given[0], requests=given[1])
+    bank = mx_moe.random_bank(moe, 2, 4)
+    serve = mx_moe.Server(moe, 2, bank=bank)
+    with torch.no_grad():
+        assert torch.equal(serve(x, requests), moe(x, bank=bank, requests=requests)[0])
+    with pytest.raises(ValueError, match="-1 for none"):
+        serve(x)
+
+
+def test_the_example_serves_as_many_requests_as_its_prompts_hold(mx_moe):
+    print("example of few prompts", flush=True)
+    assert len(mx_moe.main(["--experts", "8", "--hidden", "256", "--inner", "128", "--top-k", "2", "--sequences", "2",
+                            "--tokens", "6", "--steps", "2", "--requests", "12"])) == 2
