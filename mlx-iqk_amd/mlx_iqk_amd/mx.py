@@ -398,6 +398,8 @@ class MxLinear(_MxStack):
         """Project ``x``; with ``adapters`` (a :class:`~mlx_iqk_amd.adapters.LowRankAdapters` of
         this matrix's size, ``x`` in its 16-bit type) each row's own, which ``adapter_ids``
         names, is added to the rounded product."""
+        if adapters is None and adapter_ids is not None:
+            raise IqkRuntimeError("adapter_ids name rows of adapters, and none were given")
         tiles = self._buffers["tiles"]
         rows = self._activations(x, tiles)
         lead = rows[1].shape[:-1]

@@ -10,7 +10,7 @@ import pytest
 import torch
 
 import mlx_iqk_amd
-from mlx_iqk_amd import _native, build, router
+from mlx_iqk_amd import _native, build, mx, router
 from mlx_iqk_amd.adapters import MAX_ADAPTERS, MAX_RANK, LowRankAdapters
 from mlx_iqk_amd.kernels import IqkKernelError
 from mlx_iqk_amd.nn import IqkRuntimeError
@@ -146,3 +146,11 @@ def test_the_example_refuses_requests_that_its_prompts_do_not_hold(requests, cap
     with pytest.raises(SystemExit):
         mx_moe.main(["--sequences", "4", "--tokens", tokens, "--requests", requests])
     assert "--requests must be" in capsys.readouterr().err
+
+
+def test_ids_without_adapters_are_refused():
+    proj = mx.MxLinear(64, 32)
+    with pytest.raises(IqkRuntimeError, match="adapter_ids"):
+        proj(torch.zeros(3, 32, dtype=torch.bfloat16), adapter_ids=torch.zeros(3, dtype=torch.int32))
+    with pytest.raises(IqkRuntimeError, match="adapter_ids"):
+        proj(torch.zeros(3, 32, dtype=torch.bfloat16), None, torch.zeros(3, dtype=torch.int32))
