@@ -416,7 +416,9 @@ class MxLinear(_MxStack):
             raise IqkRuntimeError(f"the adapters are for [{adapters.out_features}, {adapters.in_features}], the weights "
                                   f"are [{self.out_features}, {self.in_features}]")
         y = self._project(rows, None, shape, n, 1, 1, grouped)
-        return adapters._add(x, adapter_ids, y, y)
+        if adapters._called_as_it_is():
+            return adapters._add(x, adapter_ids, y, y)
+        return adapters(x, adapter_ids, y)
 
     def extra_repr(self) -> str:
         return f"{self.out_features}, {self.in_features}"

@@ -342,3 +342,46 @@ def test_sorted_rows(device, dtype, rows, adapters, rank, out, n):
         got = bank(x, named, y)
         _check(got, bank, x, ids, y, dtype)
         assert torch.equal(bank(x, named, y), got)  # again, bit for bit
+
+
+def test_hooks_and_other_forwards_run_beside_a_projection(device):
+    print("adapters' hooks", flush=True)
+    rng = np.random.default_rng(8)
+    proj = mx.MxLinear(64, 96, device=device)
+    proj.load(mx.quantize(torch.from_numpy(0.05 * rng.standard_normal((64, 96))).to(BF16).to(device)))
+    bank = _bank(rng, 3, 64, 96, 8, BF16, device)
+    x, ids = _rows(rng, 5, 96, BF16, device), torch.tensor([0, 1, -1, 2, 1], device=device)
+    plain = proj(x)
+    want = bank(x, ids, plain)
+    seen = []
+
+    def before(module, args):
+        seen.append([t.clone() for t in args])
+
+    def after(module, args, out):
+        seen.append(out)
+        return out * 2
+
+    handles = [bank.register_forward_pre_hook(before), bank.register_forward_hook(after)]
+    assert torch.equal(proj(x, bank, ids), want * 2)
+    assert len(seen) == 2 and all(torch.equal(a, b) for a, b in zip(seen[0], (x, ids, plain))) and torch.equal(seen[1], want)
+    for handle in handles:
+        handle.remove()
+    assert torch.equal(proj(x, bank, ids), want) and len(seen) == 2
+    calls = []
+    handle = torch.nn.modules.module.register_module_forward_hook(lambda module, args, out: calls.append(module))
+    try:
+        assert torch.equal(proj(x, bank, ids), want)
+    finally:
+        handle.remove()
+    assert any(m is bank for m in calls)
+
+    class Doubled(LowRankAdapters):
+        def forward(self, x, ids, y):
+            return super().forward(x, ids, y) * 2
+
+    other = Doubled(3, 64, 96, 8, device=device)
+    other.load_state_dict(bank.state_dict())
+    assert torch.equal(proj(x, other, ids), want * 2)
+    bank.forward = lambda x, ids, y: y * 3
+    assert torch.equal(proj(x, bank, ids), plain * 3)
