@@ -140,7 +140,10 @@ class LowRankAdapters(torch.nn.Module):
         if not x.numel():
             return y.clone() if out is None else out
         if ids.dtype not in _KERNEL_IDS:
+            wraps = ids.dtype == torch.uint64  # 2**63 and more: not -1, but outside
             ids = torch.clamp(ids.to(torch.int64), -2, self.num_adapters)
+            if wraps:
+                ids = ids.masked_fill(ids < 0, self.num_adapters)
         return add(x.contiguous(), ids.contiguous(), y.contiguous(), down.contiguous(), up.contiguous(),
                    scales.contiguous(), out)
 

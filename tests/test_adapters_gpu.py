@@ -385,3 +385,18 @@ def test_hooks_and_other_forwards_run_beside_a_projection(device):
     assert torch.equal(proj(x, other, ids), want * 2)
     bank.forward = lambda x, ids, y: y * 3
     assert torch.equal(proj(x, bank, ids), plain * 3)
+
+
+@pytest.mark.parametrize("dtype", (torch.uint8, torch.int8, torch.int16, torch.uint16, torch.uint32, torch.uint64))
+def test_ids_of_any_integer_type(device, dtype):
+    """-1 where the type has it; its largest value lies outside the bank."""
+    print(f"ids of {dtype}", flush=True)
+    rng = np.random.default_rng(9)
+    bank = _bank(rng, 3, 40, 32, 8, F16, device)
+    x, y = _rows(rng, 4, 32, F16, device), _rows(rng, 4, 40, F16, device)
+    info = torch.iinfo(dtype)
+    ids = np.array([2, 0, info.max, -1 if info.min < 0 else info.max - 1], dtype=str(dtype).split(".")[1])
+    got = bank(x, torch.from_numpy(ids).to(device), y)
+    _check(got[:2], bank, x[:2], np.array([2, 0]), y[:2], F16)
+    assert bool(got[2].isnan().all())
+    assert torch.equal(got[3], y[3]) if info.min < 0 else bool(got[3].isnan().all())
