@@ -670,11 +670,12 @@ bool adapters_shape_ok(int64_t in, int64_t out, int64_t rank, int64_t adapters, 
 }
 
 // Whether rows are computed each on its own, by what its workgroups read of the adapters, each and
-// together.  us alone and grouped, bf16, 64 adapters: [8192 x 4096] of rank 16, 64 rows (80 MiB) 11.6,
-// 19.3, 128 rows (160 MiB) 25.8, 22.6; of rank 32, 32 rows (80 MiB) 12.6, 17.5, 64 rows (160 MiB) 21.7, 20.7; of
-// rank 64, 16 rows (80 MiB) 15.6, 16.3, 32 rows (160 MiB) 20.2, 20.8; [4096 x 4096] of rank 128, one row
-// (1.3 MiB a workgroup) 18.5, 14.5; [1001 x 1440] of rank 20, 512 rows (57 MiB) 11.2, 19.0; [512 x 512] of rank
-// 8, 512 rows 7.1, 13.6, 1024 rows 17.4, 15.7.
+// together.  us alone and grouped, bf16, 64 adapters, from a graph: [8192 x 4096] of rank 16, 64 rows (80 MiB) 13.0,
+// 20.4, 128 rows (160 MiB) 21.6, 23.4; of rank 32, 32 rows (80 MiB) 13.1, 17.8, 64 rows (160 MiB) 23.1, 21.8; of
+// rank 64, 16 rows (80 MiB) 15.2, 15.8, 32 rows (160 MiB) 21.6, 21.2; [4096 x 4096] of rank 128, one row
+// (1.3 MiB a workgroup) 16.5, 15.3.  Adapters that are small beside the launches: [512 x 512] of rank 8, 1024 rows
+// 6.5, 13.8, 1536 rows 8.7, 16.4, 4096 rows 20.5, 19.3; [1024 x 512] of rank 32, 1024 rows 14.0, 15.3, 1280 rows
+// 17.0, 16.6: beyond 1024 workgroups it depends on their size, and is left to the tiles.
 bool rows_stand_alone(int64_t in, int64_t out, int64_t rank, int64_t rows) {
     const int64_t groups = rows * ((out + kAloneThreads - 1) / kAloneThreads), each = rank * (in + kAloneThreads) * 2;
     return groups <= 1024 && each <= int64_t(1) << 20 && groups * each <= int64_t(128) << 20;
