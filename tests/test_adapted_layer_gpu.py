@@ -13,7 +13,7 @@ import torch
 import mxref
 import wirepack
 from mlx_iqk_amd import format as fmt
-from mlx_iqk_amd import mx, router
+from mlx_iqk_amd import _native, mx, router
 from mlx_iqk_amd.adapters import LowRankAdapters
 from mlx_iqk_amd.nn import IqkSwitchLinear
 
@@ -199,3 +199,31 @@ def test_the_example_serves_as_many_requests_as_its_prompts_hold(mx_moe):
     print("example of few prompts", flush=True)
     assert len(mx_moe.main(["--experts", "8", "--hidden", "256", "--inner", "128", "--top-k", "2", "--sequences", "2",
                             "--tokens", "6", "--steps", "2", "--requests", "12"])) == 2
+
+
+def test_the_examples_layer_of_many_rows(mx_moe):
+    """As many rows as go through the adapters' tiles, served from a graph as called."""
+    print("example with tiles", flush=True)
+    torch.manual_seed(9)
+    tokens = 1100
+    moe = mx_moe.random_layer(12, 160, 96, 3)
+    x = torch.randn(tokens, 160, device="cuda", dtype=BF16)
+    requests = torch.arange(tokens, device="cuda") % 6 - 1
+    with torch.no_grad():
+        alone = moe(x)[0]
+        bank = mx_moe.random_bank(moe, 5, 8)
+        assert _native.load().iqk_adapters_work(160, 160, 8, 5, tokens) > 0
+        y = moe(x, bank=bank, requests=requests)[0]
+        shared = bank(x, requests, moe.shared(x))
+    # `alone` is rounded once, y once: the sum of both lies within those roundings
+    want, bound = alone.double() + shared.double(), mxref.HALF_ULP[BF16] * alone.double().abs()
+    assert bool(((y.double() - want).abs() <= bound + mxref.HALF_ULP[BF16] * (want.abs() + bound) + 2.0 ** -100).all())
+    serve = mx_moe.Server(moe, tokens, bank=bank)
+    for turn in range(3):
+        x = torch.randn(tokens, 160, device="cuda", dtype=BF16)
+        requests = (requests + 2 + turn) % 6 - 1
+        with torch.no_grad():
+            want = moe(x, bank=bank, requests=requests)[0]
+        torch.cuda.synchronize()
+        assert torch.equal(serve(x, requests), want)
+        torch.cuda.synchronize()
