@@ -29,7 +29,9 @@ constexpr int kSortWaves = 16, kSortThreads = 64 * kSortWaves;
 // Pairs up to which every workgroup counts all of them itself, in one launch: 7108 pairs of 60 experts
 // 6.6 us, in two launches 8.4; 12288 of 256 8.5 and 8.6; 16200 (64-bit ids) 11.3 and 10.1.
 constexpr int64_t kSortOne = 12288;
-constexpr int64_t kSortBlocks = 64;  // workgroups of a sort, at most: each reads the counts of all
+// Workgroups of a sort, at most: each reads the counts of all.  us with 32, 64 and 128: 98304 pairs of 256 experts 13.5, 12.4,
+// 10.8, 786432 pairs 42.0, 26.9, 21.4; 196608 pairs of 1000 experts 21.5, 19.5, 21.9.
+constexpr int64_t kSortBlocks = 64;
 
 struct SortArgs {
     const uint32_t *ids;
@@ -344,7 +346,9 @@ __device__ __forceinline__ uint4_t pack(const float (&v)[kChunk<DT>]) {
 // A chunk, or (not WHOLE) its first `halves` (1 .. 7) 16-bit halves and zeros behind them.  ONCE:
 // of the slots' rows, which are many and pass through once, so that they do not stay in the caches in
 // place of what does not (16384 tokens, 6 rows of 8 KiB each: their sum 185 us, 161 so; rows and
-// gradient of a training step 391, 345).
+// gradient of a training step 391, 345).  What reads the rows at once loses by it while the caches hold them: dispatched
+// and scaled by a kernel of torch's, 2048 tokens 61.6 us, 69.1 so, 8192 tokens 221, 242; dispatched and combined
+// 46.8, 50.3 and 216, 177.
 template <bool WHOLE, bool ONCE = false>
 __device__ __forceinline__ uint4_t load_chunk(const uint8_t *p, uint32_t halves) {
     if constexpr (WHOLE && ONCE) {
@@ -434,7 +438,8 @@ __global__ __launch_bounds__(256) void dispatch_kernel(RowArgs a) {
 
 // Few pairs: the rows' workgroups sort for themselves, in one launch.  Each counts all pairs, ranks
 // those of its own tokens, and moves its part of their rows; one of a token's workgroups writes
-// its lists.  (A launch before costs 3 us of the GPU's time and 2 of the host's.)
+// its lists.  (A launch before costs 3 us of the GPU's time and 2 of the host's.)  us in one launch and in two, 256
+// experts: 1020 pairs' rows of 1 KiB 6.1, 8.5, of 8 KiB 7.2, 8.9; 4092 pairs' 7.7, 9.5, of 8 KiB 17.0, 13.7.
 constexpr int64_t kDispatchOne = 1024;  // pairs
 
 template <bool WIDE>
@@ -667,7 +672,8 @@ int sort_launch(const SortCall &c, hipStream_t stream) {
     }
     const auto sized = [&](auto wide) {
         constexpr bool W = decltype(wide)::value;
-        if (c.pairs <= 256) return run(sort_kernel<W, 4, 1>, 256);  // one pair a thread
+        // one pair a thread; in 16 wavefronts 48 pairs take 4.5 us, 4.1 so, 252 pairs 4.5, 4.2
+        if (c.pairs <= 256) return run(sort_kernel<W, 4, 1>, 256);
         if (plan.share == kSortThreads) return run(sort_kernel<W, kSortWaves, 1>, kSortThreads);
         if (plan.share <= 4 * kSortThreads) return run(sort_kernel<W, kSortWaves, 4>, kSortThreads);
         return run(sort_kernel<W, kSortWaves, 0>, kSortThreads);

@@ -32,7 +32,10 @@ class LowRankAdapters(torch.nn.Module):
     * ``down`` 16-bit ``[num_adapters, in/8, R, 8]`` and ``up`` ``[num_adapters, R/8, out, 8]``;
     * ``scales`` f32 ``[num_adapters]``.
 
-    All zeros, which add nothing, until :meth:`load`; :meth:`adapter` gives one back.
+    All zeros, which add nothing, until :meth:`load`; :meth:`adapter` gives one back.  Of the ranks up to R those
+    past an adapter's own are zeros, with which an infinity in a row of ``x`` gives NaN.  An
+    infinity in an adapter makes sums of its rows infinite or NaN.  ``scales`` stay f32: a bank that a model's ``half()`` or
+    ``to(dtype)`` has cast is refused, so cast first and make the bank after.
     """
 
     def __init__(self, num_adapters: int, out_features: int, in_features: int, rank: int,
@@ -59,8 +62,7 @@ class LowRankAdapters(torch.nn.Module):
 
     def load(self, index: int, down: torch.Tensor, up: torch.Tensor, scale: float = 1.0) -> None:
         """Take adapter ``index``: ``down`` ``[r, in]`` and ``up`` ``[out, r]``, r up to the
-        bank's rank, rounded to its type; ``scale`` is alpha / r, say.  Ranks past r are zeros,
-        with which an infinity in ``x`` gives NaN."""
+        bank's rank, rounded to its type; ``scale`` is alpha / r, say.  Ranks past r become zeros."""
         if not 0 <= index < self.num_adapters:
             raise IqkRuntimeError(f"the bank holds adapters 0 .. {self.num_adapters - 1}, got {index}")
         if down.dim() != 2 or up.dim() != 2 or down.shape[0] != up.shape[1] or not 0 < down.shape[0] <= self.rank \

@@ -166,13 +166,8 @@ def sort(ids: torch.Tensor, num_experts: int) -> Order:
     sort_pairs = _native.torch_binding().sort
     if (lists := sort_pairs(ids, num_experts)) is None:  # ids that the kernels do not take as they are
         lists = sort_pairs(*_check_ids(ids, num_experts))
-    return _sorted(*lists)
-
-
-def _sorted(offsets, ids, tokens, slots) -> Order:
-    """The order of the binding's lists."""
-    order = Order(offsets, ids, tokens, slots)
-    order._permutation = slots
+    order = Order(*lists)
+    order._permutation = order.slots
     return order
 
 
@@ -203,8 +198,9 @@ def dispatch(x: torch.Tensor, ids: torch.Tensor, num_experts: int) -> tuple[torc
         if x.shape[:-1] != ids.shape[:-1]:
             raise IqkKernelError(f"x {tuple(x.shape)} and ids {tuple(ids.shape)} are not of the same tokens")
         got = dispatch_rows(x.contiguous(), ids, experts)
-    rows, offsets, sorted_ids, tokens, slots = got
-    return rows, _sorted(offsets, sorted_ids, tokens, slots)
+    order = Order(*got[1:])
+    order._permutation = order.slots
+    return got[0], order
 
 
 def combine(y: torch.Tensor, weights: torch.Tensor, order: Order | None = None, *,
