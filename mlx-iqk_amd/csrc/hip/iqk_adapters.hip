@@ -554,9 +554,13 @@ __global__ __launch_bounds__(256, KC <= 4 ? 2 : 1) void adapter_up_tiles_kernel(
                             for (int j = 0; j < 4; ++j) w[0][s][j] = uint4_t{0, 0, 0, 0};
                         }
                 }
-                if (!BF && k0) {
+                // Sums as large as the third pieces, by a power of two: of slots without an infinity, whose chunks all
+                // are f32, they are far from f32's end.
+                constexpr uint32_t CHUNKS = (1u << STAGE) - 1u;
+                const bool third = !BF && (!ANY_F32 || (in_f32 >> (KC * c + k0 / 32) & CHUNKS) != CHUNKS);
+                if (third && k0) {
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) acc[j] *= kThird;  // a power of two, as the third pieces are
+                    for (int j = 0; j < 4; ++j) acc[j] *= kThird;
                 }
 #pragma unroll
                 for (int p = P - 1; p >= 0; --p) {  // the small pieces first
@@ -567,7 +571,7 @@ __global__ __launch_bounds__(256, KC <= 4 ? 2 : 1) void adapter_up_tiles_kernel(
 #pragma unroll
                         for (int j = 0; j < 4; ++j) acc[j] = mfma<BF>(w[0][s][j], b, acc[j]);
                     }
-                    if (!BF && p == 2) {
+                    if (third && p == 2) {
 #pragma unroll
                         for (int j = 0; j < 4; ++j) acc[j] *= 1 / kThird;
                     }

@@ -105,6 +105,25 @@ def test_an_infinity_beside_large_ranks(device, dtype, rank, rows):
         np.testing.assert_array_equal(got[r], rest if r % 3 == 2 else want)
 
 
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("rank,at", ((2, 1), (40, 33), (72, 70), (128, 127), (200, 150), (256, 64)))
+@pytest.mark.parametrize("rows", (3, 4300))
+def test_an_infinity_behind_large_ranks(device, dtype, rank, at, rows):
+    """Finite sums near f32's end in the ranks before an infinity do not become infinities of their own."""
+    print(f"infinity behind large ranks {dtype} {rank} {at} {rows}", flush=True)
+    bank = LowRankAdapters(1, 24, 16, rank, dtype=dtype, device=device)
+    down, up = torch.zeros((rank, 16)), torch.zeros((24, rank))
+    down[0, 0], down[at, 1] = 2.0 ** -6, 1.0
+    up[:, 0] = 1.0
+    up[:, at] = torch.arange(24) % 2 * 2.0 - 1
+    bank.load(0, down, up, 2.0 ** 126)
+    x = torch.zeros((rows, 16), dtype=dtype, device=device)
+    x[:, 0], x[:, 1] = 2.0 ** -4, 8.0  # 2^116 and 2^129 when scaled
+    assert (_words(bank, rows) > 0) == (rows > 64)
+    got = _f64(bank(x, torch.zeros(rows, dtype=torch.int32, device=device), torch.ones((rows, 24), dtype=dtype, device=device)))
+    np.testing.assert_array_equal(got, np.broadcast_to(np.sign(_f64(up[:, at])) * np.inf, got.shape))
+
+
 def _normal(rng, *shape):
     return torch.from_numpy(rng.standard_normal(shape))
 
