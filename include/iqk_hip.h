@@ -36,7 +36,7 @@
 extern "C" {
 #endif
 
-#define IQK_HIP_ABI_VERSION 8
+#define IQK_HIP_ABI_VERSION 9
 
 #define IQK_MEMBER_IQ2_KS 0
 #define IQK_MEMBER_IQ2_K 1
@@ -402,10 +402,15 @@ int iqk_combine(int dtype, const void *y, const int32_t *slots, const int32_t *k
 
 // Its gradients from dout, dtype [n_tokens, cols]: dy[slots[t, j]] = weights[t, j] dout[t] (zeros
 // in slots >= *kept) and dweights[t, j] = dout[t] . y[slots[t, j]] (0 there); either may be NULL,
-// and y where dweights is.
+// and y where dweights is.  dy takes slots that are a permutation, as iqk_sort's are.
 int iqk_combine_grad(int dtype, const void *dout, const void *y, const int32_t *slots, const int32_t *kept,
                      const float *weights, int64_t n_tokens, int64_t pairs_per_token, int64_t cols, void *dy,
                      float *dweights, void *stream);
+
+// dy for any slots: dy[s] = the sum of weights[t, j] dout[t] over the pairs whose slot is s < *kept, f32 sums in the
+// pairs' order, one rounding; zeros where there is none.  work: 2 n_tokens pairs_per_token words.
+int iqk_combine_grad_rows(int dtype, const void *dout, const int32_t *slots, const int32_t *kept, const float *weights,
+                          int64_t n_tokens, int64_t pairs_per_token, int64_t cols, uint32_t *work, void *dy, void *stream);
 
 // -- low-rank adapters ---------------------------------------------------------
 //

@@ -627,6 +627,76 @@ __global__ __launch_bounds__(256) void combine_grad_kernel(RowArgs a) {
     }
 }
 
+// dy where the slots are no permutation (a caller's order): a slot's first and last pair, then a wavefront for
+// each slot, which looks between them for others and adds them in the pairs' order.  16384 tokens of 6 rows of
+// 8 KiB: a fifth of the pairs dropped 257 us (a permutation, by its tokens, 156); six pairs of each row far
+// apart 2.2 ms, which the looking takes.
+__global__ __launch_bounds__(256) void slot_span_clear_kernel(int32_t *first, int32_t *last, uint32_t n) {
+    const uint32_t s = blockIdx.x * 256 + threadIdx.x;
+    if (s < n) first[s] = 0x7fffffff, last[s] = -1;
+}
+
+__global__ __launch_bounds__(256) void slot_span_kernel(RowArgs a, int32_t *first, int32_t *last) {
+    const uint32_t p = blockIdx.x * 256 + threadIdx.x;
+    if (p >= a.P) return;
+    const uint32_t slot = uint32_t(a.slots[p]);
+    if (slot >= slots_kept(a)) return;
+    atomicMin(&first[slot], int32_t(p));
+    atomicMax(&last[slot], int32_t(p));
+}
+
+template <int DT>
+__global__ __launch_bounds__(256) void combine_grad_rows_kernel(RowArgs a, const int32_t *first, const int32_t *last) {
+    constexpr int N = kChunk<DT>;
+    const uint32_t lane = threadIdx.x & 63u;
+    const uint32_t slot = a.first + blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    if (slot >= a.T) return;  // whole wavefronts
+    const uint32_t lo = __builtin_amdgcn_readfirstlane(first[slot]);
+    const int32_t hi = __builtin_amdgcn_readfirstlane(last[slot]);  // -1: no pair
+    for (uint32_t c0 = 0; c0 < a.chunks; c0 += 64) {
+        const uint32_t c = c0 + lane, halves = c < a.chunks ? min(8u, (a.row - 16u * c) / 2u) : 0u;
+        const size_t column = size_t(c) * 16;
+        uint8_t *const to = a.out + size_t(slot) * a.row + column;
+        float sum[N] = {}, g[N];
+        const auto load = [&](uint32_t p) __attribute__((always_inline)) {  // p: uniform
+            const uint8_t *const from = a.in + size_t(p / a.k) * a.row + column;
+            unpack<DT>(halves == 8 ? load_chunk<true>(from, 8) : load_chunk<false>(from, halves), g);
+        };
+        const auto add = [&](uint32_t p) __attribute__((always_inline)) {
+            if (halves == 0) return;
+            load(p);
+#pragma unroll
+            for (int n = 0; n < N; ++n) sum[n] = fmaf(a.weights[p], g[n], sum[n]);
+        };
+        if (hi >= 0 && uint32_t(hi) == lo) {  // one pair: as combine_grad_kernel has it, bit for bit
+            const uint8_t *const from = a.in + size_t(lo / a.k) * a.row + column;
+            const auto move = [&](auto whole) __attribute__((always_inline)) {
+                constexpr bool WHOLE = decltype(whole)::value;
+                unpack<DT>(load_chunk<WHOLE>(from, halves), g);
+                float v[N];
+#pragma unroll
+                for (int n = 0; n < N; ++n) v[n] = a.weights[lo] * g[n];
+                store_chunk<WHOLE>(to, pack<DT>(v), halves);
+            };
+            if (halves == 8)
+                move(std::true_type{});
+            else if (halves)
+                move(std::false_type{});
+            continue;
+        }
+        if (hi >= 0) add(lo);
+        for (uint32_t base = lo + 1; hi >= 0 && base <= uint32_t(hi); base += 64) {
+            const uint32_t p = base + lane;
+            for (uint64_t own = __ballot(p <= uint32_t(hi) && uint32_t(a.slots[min(p, uint32_t(hi))]) == slot); own; own &= own - 1)
+                add(base + uint32_t(__builtin_ctzll(own)));
+        }
+        if (halves == 8)
+            store_chunk<true>(to, pack<DT>(sum), 8);
+        else if (halves)
+            store_chunk<false>(to, pack<DT>(sum), halves);
+    }
+}
+
 // --------------------------------------------------------------------- host ---
 
 SortPlan sort_plan(int64_t pairs, int64_t experts) {
@@ -852,6 +922,32 @@ int iqk_combine_grad(int dtype, const void *dout, const void *y, const int32_t *
             by_tokens(a, 1, 1, [&](const RowArgs &part, uint32_t blocks) {
                 hipLaunchKernelGGL((combine_grad_kernel<DT, 4>), dim3{blocks}, dim3{256}, 0, as_stream(stream), part);
             });
+    });
+    return record_launch(hipGetLastError());
+}
+
+int iqk_combine_grad_rows(int dtype, const void *dout, const int32_t *slots, const int32_t *kept, const float *weights,
+                          int64_t n_tokens, int64_t pairs_per_token, int64_t cols, uint32_t *work, void *dy, void *stream) {
+    using namespace iqk;
+    if (!rows_shape_ok(dtype, n_tokens, pairs_per_token, cols)) return IQK_ERR_GEOMETRY;
+    if (n_tokens == 0) return IQK_OK;
+    if (!dout || !slots || !weights || !work || !dy) return IQK_ERR_ARGUMENT;
+    RowArgs a = row_args(dtype, n_tokens, pairs_per_token, cols);
+    a.in = static_cast<const uint8_t *>(dout);
+    a.slots = slots;
+    a.kept = kept;
+    a.weights = weights;
+    a.out = static_cast<uint8_t *>(dy);
+    int32_t *const first = reinterpret_cast<int32_t *>(work), *const last = first + a.P;
+    const uint32_t blocks = (a.P + 255u) / 256u;  // fewer than 2^31 threads
+    hipLaunchKernelGGL(slot_span_clear_kernel, dim3{blocks}, dim3{256}, 0, as_stream(stream), first, last, a.P);
+    hipLaunchKernelGGL(slot_span_kernel, dim3{blocks}, dim3{256}, 0, as_stream(stream), a, first, last);
+    a.T = a.P;  // a wavefront for each slot
+    by_dtype(dtype, [&](auto dt) {
+        by_tokens(a, 4, 1, [&](const RowArgs &part, uint32_t groups) {
+            hipLaunchKernelGGL((combine_grad_rows_kernel<decltype(dt)::value>), dim3{groups}, dim3{256}, 0, as_stream(stream),
+                               part, first, last);
+        });
     });
     return record_launch(hipGetLastError());
 }

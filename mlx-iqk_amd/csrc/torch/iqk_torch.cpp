@@ -284,7 +284,7 @@ struct Combine : torch::autograd::Function<Combine> {
         ctx->saved_data["dy"] = dy;
         ctx->saved_data["dw"] = dw;
         ctx->saved_data["dadd"] = add && add->requires_grad();
-        ctx->saved_data["every_row"] = permutation;  // has a pair that writes its gradient
+        ctx->saved_data["permutation"] = permutation;  // of the slots: each row has one pair, which writes its gradient
         ctx->saved_data["shape"] = y.sizes().vec();
         const Tensor s = slots.value_or(Tensor()), o = offsets.value_or(Tensor());
         // y for the weights' gradient only, which is the larger by far
@@ -300,15 +300,20 @@ struct Combine : torch::autograd::Function<Combine> {
         const c10::DeviceGuard guard(grads[0].device());
         const Tensor dout = grads[0].detach().contiguous();
         Tensor dy, dweights;
-        if (ctx->saved_data["dy"].toBool()) {
-            dy = empty(ctx->saved_data["shape"].toIntVector(), dout.scalar_type(), dout);
-            if (!ctx->saved_data["every_row"].toBool()) dy.zero_();
-        }
+        if (ctx->saved_data["dy"].toBool()) dy = empty(ctx->saved_data["shape"].toIntVector(), dout.scalar_type(), dout);
         if (ctx->saved_data["dw"].toBool()) dweights = empty(weights.sizes(), at::kFloat, dout);
         if (dy.defined() || dweights.defined()) {
-            const int64_t k = weights.size(-1);
+            const int64_t k = weights.size(-1), tokens = weights.numel() / k;
+            const bool rows_apart = dy.defined() && !ctx->saved_data["permutation"].toBool();
+            if (rows_apart) {
+                const Tensor work = empty({2 * weights.numel()}, at::kInt, dout);
+                check(iqk_combine_grad_rows(type_code(dout), dout.data_ptr(), ptr<int32_t>(slots), kept(offsets),
+                                            ptr<float>(weights), tokens, k, dout.size(-1), ptr<uint32_t>(work),
+                                            dy.data_ptr(), stream_of(dout)),
+                      "iqk_combine_grad_rows");
+            }
             check(iqk_combine_grad(type_code(dout), dout.data_ptr(), ptr<void>(y), ptr<int32_t>(slots), kept(offsets),
-                                   ptr<float>(weights), weights.numel() / k, k, dout.size(-1), ptr<void>(dy),
+                                   ptr<float>(weights), tokens, k, dout.size(-1), rows_apart ? nullptr : ptr<void>(dy),
                                    ptr<float>(dweights), stream_of(dout)),
                   "iqk_combine_grad");
             if (dy.defined()) out[0] = once(dy, grads, weights)[0];

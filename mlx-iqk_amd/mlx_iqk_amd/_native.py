@@ -13,7 +13,7 @@ from pathlib import Path
 from . import build
 from .build import HIP_LIB, LAUNCH_EXT, TORCH_EXT
 
-ABI_VERSION = 8
+ABI_VERSION = 9
 
 OK, ERR_MEMBER, ERR_GEOMETRY, ERR_ARGUMENT, ERR_LAUNCH = 0, 1, 2, 3, 4
 _CODES = {ERR_MEMBER: "unknown member", ERR_GEOMETRY: "unsized geometry",
@@ -92,6 +92,8 @@ SIGNATURES = {
                             c_void_p]),
     "iqk_combine_grad": (c_int, [c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64,
                                  c_void_p, c_void_p, c_void_p]),
+    "iqk_combine_grad_rows": (c_int, [c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_void_p,
+                                      c_void_p, c_void_p]),
     "iqk_adapters_work": (c_int64, [c_int64, c_int64, c_int64, c_int64, c_int64]),
     "iqk_adapters": (c_int, [c_int, c_int64, c_int64, c_int64, c_int64, c_void_p, c_int64, c_void_p, c_int, c_int64,
                              c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),

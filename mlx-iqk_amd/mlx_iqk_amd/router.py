@@ -115,8 +115,8 @@ class Order(_Slots):
     * ``slots`` ``[..., k]``: each pair's slot, a permutation.
 
     Within an expert the pairs keep their order.  :func:`combine` also takes an order with other
-    slots: one outside ``0 .. pairs - 1`` (-1, say) leaves its pair out.  A slot of
-    several pairs counts for each of them, but has no gradient that is defined.
+    slots: one outside ``0 .. pairs - 1`` (-1, say) leaves its pair out, and one of several pairs
+    counts for each of them.
     """
 
     __slots__ = ("offsets", "ids", "tokens", "slots")

@@ -154,3 +154,15 @@ def test_ids_without_adapters_are_refused():
         proj(torch.zeros(3, 32, dtype=torch.bfloat16), adapter_ids=torch.zeros(3, dtype=torch.int32))
     with pytest.raises(IqkRuntimeError, match="adapter_ids"):
         proj(torch.zeros(3, 32, dtype=torch.bfloat16), None, torch.zeros(3, dtype=torch.int32))
+
+
+def test_gradients_of_any_slots_refuse_bad_arguments(lib):
+    p = ctypes.c_void_p(16)  # never dereferenced: every call below is refused first
+    f = lib.iqk_combine_grad_rows
+    for dtype, tokens, k, cols in ((3, 8, 6, 64), (0, -1, 6, 64), (0, 8, 0, 64), (0, 8, 65, 64), (0, 8, 6, 0), (0, 8, 6, 1 << 28),
+                                   (0, 1 << 30, 2, 64)):
+        assert f(dtype, p, p, p, p, tokens, k, cols, p, p, None) == _native.ERR_GEOMETRY
+    good = [0, p, p, p, p, 8, 6, 64, p, p, None]
+    for place in (1, 2, 4, 8, 9):
+        assert f(*[None if i == place else v for i, v in enumerate(good)]) == _native.ERR_ARGUMENT
+    assert f(0, None, None, None, None, 0, 6, 64, None, None, None) == _native.OK

@@ -619,3 +619,40 @@ def test_an_orders_foreign_slots_leave_zero_gradients(device):
     torch.full((4, 8), float("nan"), device=device)
     (dy,) = torch.autograd.grad(router.combine(y, torch.ones((2, 2), device=device), bad), y, torch.ones((2, 8), device=device))
     assert dy.tolist() == [[0.0] * 8, [1.0] * 8, [0.0] * 8, [0.0] * 8]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("tokens,k,cols,spread", ((1, 1, 8, 1), (3, 2, 7, 2), (40, 5, 64, 9), (300, 3, 1030, 200), (700, 6, 33, 4), (64, 64, 8, 1),
+                                                  (500, 4, 4100, 1500)))
+def test_a_row_of_several_pairs_gets_the_sum_of_their_gradients(device, dtype, tokens, k, cols, spread):
+    """A caller's order in which pairs share rows (tokens alike, say), some rows without a pair, some pairs left out."""
+    print(f"shared rows {dtype} {tokens} {k} {cols} {spread}", flush=True)
+    rng = np.random.default_rng(tokens + cols)
+    pairs = tokens * k
+    slots = rng.integers(0, min(spread, pairs), (tokens, k))
+    slots[rng.random((tokens, k)) < 0.1] = -1
+    kept = max(1, min(spread, pairs) - 1)  # the last of these are left out
+    order = router.Order(torch.tensor([0, kept], dtype=I32, device=device), *(torch.zeros(pairs, dtype=I32, device=device),) * 2,
+                         torch.from_numpy(slots).to(device, I32))
+    y = torch.from_numpy(rng.standard_normal((pairs, cols))).to(dtype).to(device).requires_grad_()
+    w = torch.from_numpy(rng.standard_normal((tokens, k)).astype(np.float32)).to(device).requires_grad_()
+    dout = torch.from_numpy(rng.standard_normal((tokens, cols))).to(dtype).to(device)
+    out = router.combine(y, w, order)
+    dy, dw = torch.autograd.grad(out, (y, w), dout)
+    w64, d64, y64 = _f64(w), _f64(dout), _f64(y)
+    live = (slots >= 0) & (slots < kept)
+    want, size = np.zeros((pairs, cols)), np.zeros((pairs, cols))
+    for t, j in zip(*np.nonzero(live)):
+        want[slots[t, j]] += w64[t, j] * d64[t]
+        size[slots[t, j]] += np.abs(w64[t, j] * d64[t])
+    most = int(np.bincount(slots[live], minlength=1).max()) if live.any() else 1
+    # so many fused additions in f32, half a step of the sum each; one rounding
+    error = most * U * size
+    assert (np.abs(_f64(dy) - want) <= error + _rounded(dtype) * (np.abs(want) + error) + mxref.TINY[dtype]).all()
+    sums = np.where(live[..., None], w64[..., None] * y64[np.where(live, slots, 0)], 0.0)
+    error = k * U * np.abs(sums).sum(1)
+    assert (np.abs(_f64(out) - sums.sum(1)) <= error + _rounded(dtype) * (np.abs(sums.sum(1)) + error) + mxref.TINY[dtype]).all()
+    dots = np.where(live[..., None], d64[:, None] * y64[np.where(live, slots, 0)], 0.0)
+    assert (np.abs(_f64(dw) - dots.sum(-1)) <= cols * U * np.abs(dots).sum(-1) + 2.0 ** -140).all()
+    again = torch.autograd.grad(router.combine(y, w, order), (y,), dout)[0]
+    assert torch.equal(again, dy)
